@@ -1,0 +1,340 @@
+// delta_chunk.hpp — what the chunked kernels of the gated delta rule share: a chunk's gates,
+// its rows in LDS and its two triangles.
+//
+// Mathematics. Inside a chunk of 64 tokens with the state S before it, G_i the sum of g up to
+// token i (from the chunk's first on), D_ij = exp(G_i - G_j) for i >= j of one episode and 0
+// for two, E_i = exp(G_i) as long as no episode has started, F_i = exp(G_last - G_i) where
+// none starts after i, the updates u of all tokens solve one unit lower triangular system:
+//
+//     (I + A) u = r,  A_ij = D_ij (k_i . k_j) beta_j  (i > j),   r_i = v_i - E_i S^T k_i
+//     o_i = scale E_i S^T q_i + sum_j P_ij u_j,  P_ij = scale D_ij (q_i . k_j) beta_j  (i >= j)
+//     S  <- E_last S + sum_i k_i (F_i beta_i u_i)^T
+//
+// and with X = (I + A)^-1, u = X r. X and P are the chunk's two triangles; they do not depend
+// on S or v. (k_i . k_j is close to 1 between frames that look alike, so X comes from
+// substitution in 16 x 16 blocks, whose entries stay bounded, not from powers of A.)
+//
+// G is summed in float64 and kept as a float and its rest: D needs differences of sums that
+// may be large, to float32's precision.
+#pragma once
+
+#include "policy_common.hpp"
+
+namespace navi_policy {
+
+constexpr int kChunk = NAVI_POLICY_CHUNK;
+constexpr int kTiles = 10;         // 16 x 16 tiles of a lower triangle of 64
+constexpr float kStart = -1e5f;    // a decay below exp(kStart) is the start of an episode
+constexpr float kLog2E = 1.44269504088896340736f;
+
+struct RuleParams {
+    navi_delta_rule r;
+    navi_delta_gradients d;
+    int32_t group;        // value heads of a key head
+    int32_t n_chunks;
+    int32_t wide_qk, wide_v, wide_do;  // rows that 16-byte loads can read
+    int32_t wide_state;   // rows of states and updates that 16-byte accesses can
+    float* dstates;       // [env, head][chunks - 1][K][V] gradient of the state after each chunk but the last
+    float* rgrads;        // [env, head][steps][V] gradient of r
+    float* dq_heads;      // [env][step][value head][K] where heads are shared
+    float* dk_heads;
+};
+
+// Tile (i, j), j <= i, of a triangle; a tile is 64 lanes of four numbers as products leave
+// them: slot l has column l % 16, rows 4 (l / 16) to 4 (l / 16) + 3.
+__device__ constexpr int tile_of(int i, int j) { return i * (i + 1) / 2 + j; }
+
+using Triangle = uint16_t[kTiles][3][64][4];  // its three planes
+
+struct ChunkGates {
+    float hi[kChunk], lo[kChunk];  // G
+    float e[kChunk], f[kChunk], beta[kChunk];
+    int32_t episode[kChunk];       // episodes started in the chunk so far
+};
+
+template <class E, int KP>
+struct ChunkRows {
+    static constexpr int kPitch = KP + 8;
+    uint16_t q[kPlanes<E>][kChunk][kPitch];
+    uint16_t k[kPlanes<E>][kChunk][kPitch];
+};
+
+struct ChunkTriangles {
+    Triangle x, p;
+    float work[kChunk][kChunk + 4];  // A, then X
+};
+
+template <class E>
+__device__ inline const E* at(const void* base, const int64_t (&stride)[3], int64_t env, int64_t step, int64_t head) {
+    return static_cast<const E*>(base) + env * stride[0] + step * stride[1] + head * stride[2];
+}
+
+// Eight elements of a row as floats, those from `valid` on as zeros.
+template <class E>
+__device__ inline void load8(const E* row, int valid, bool wide, float (&x)[8]) {
+    if (wide && valid >= 8) {
+        union {
+            u4 words[sizeof(E) == 4 ? 2 : 1];
+            E elements[8];
+        } got;
+        got.words[0] = *reinterpret_cast<const u4*>(row);
+        if constexpr (sizeof(E) == 4) got.words[1] = *reinterpret_cast<const u4*>(row + 4);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = to_float(got.elements[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = i < valid ? to_float(row[i]) : 0.0f;
+    }
+}
+
+// The chunk's queries and keys into LDS, zeros past the last token and the key dimension.
+template <class E, int KP>
+__device__ inline void load_rows(const RuleParams& P, ChunkRows<E, KP>& rows, int64_t env, int head, int64_t t0,
+                                 int tokens) {
+    constexpr int kPieces = KP / 8;
+    const int key_head = head / P.group;
+    for (int piece = threadIdx.x; piece < kChunk * kPieces; piece += blockDim.x) {
+        const int t = piece / kPieces, c = piece % kPieces * 8;
+        const int valid = t < tokens ? P.r.key_dim - c : 0;
+        float x[8];
+        u4 plane[kPlanes<E>];
+        load8(at<E>(P.r.q, P.r.q_stride, env, t0 + (t < tokens ? t : 0), key_head) + c, valid, P.wide_qk, x);
+        split8(x, plane);
+#pragma unroll
+        for (int n = 0; n < kPlanes<E>; ++n) *reinterpret_cast<u4*>(&rows.q[n][t][c]) = plane[n];
+        load8(at<E>(P.r.k, P.r.k_stride, env, t0 + (t < tokens ? t : 0), key_head) + c, valid, P.wide_qk, x);
+        split8(x, plane);
+#pragma unroll
+        for (int n = 0; n < kPlanes<E>; ++n) *reinterpret_cast<u4*>(&rows.k[n][t][c]) = plane[n];
+    }
+}
+
+// One wave's scan of the chunk's gates, a token a lane.
+__device__ inline void load_gates(const RuleParams& P, ChunkGates& gates, int64_t env, int head, int64_t t0,
+                                  int tokens) {
+    const int lane = threadIdx.x & 63;
+    float g = 0.0f, beta = 0.0f;
+    int start = 0;
+    if (lane < tokens) {
+        g = *at<float>(P.r.g, P.r.g_stride, env, t0 + lane, head);
+        beta = *at<float>(P.r.beta, P.r.beta_stride, env, t0 + lane, head);
+        start = g < kStart ||
+                (P.r.starts && P.r.starts[env * P.r.starts_stride[0] + (t0 + lane) * P.r.starts_stride[1]]);
+    }
+    double sum = start ? 0.0 : static_cast<double>(g);
+    int episode = start;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const double s = __shfl_up(sum, d);
+        const int e = __shfl_up(episode, d);
+        sum += lane >= d ? s : 0.0;
+        episode += lane >= d ? e : 0;
+    }
+    const float hi = static_cast<float>(sum), lo = static_cast<float>(sum - hi);
+    const double last = __shfl(sum, 63);
+    const int last_episode = __shfl(episode, 63);
+    gates.hi[lane] = hi;
+    gates.lo[lane] = lo;
+    gates.e[lane] = episode == 0 ? expf(hi) * (1.0f + lo) : 0.0f;
+    gates.f[lane] = episode == last_episode ? expf(static_cast<float>(last - sum)) : 0.0f;
+    gates.beta[lane] = beta;
+    gates.episode[lane] = episode;
+}
+
+__device__ inline float decay(const ChunkGates& gates, int i, float hi_j, float lo_j, int episode_j) {
+    const float d = (gates.hi[i] - hi_j) + (gates.lo[i] - lo_j);
+    return gates.episode[i] == episode_j ? __builtin_amdgcn_exp2f(d * kLog2E) : 0.0f;
+}
+
+// Operands of products from rows in LDS: rows row0 to row0 + 15, eight columns of 32 m to
+// 32 m + 31 a lane, in their order;
+template <int N, int kPitch>
+__device__ inline void operand_rows(const uint16_t (&rows)[N][kChunk][kPitch], int row0, int m, u4 (&x)[N]) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+        x[n] = *reinterpret_cast<const u4*>(&rows[n][row0 + (lane & 15)][32 * m + 8 * (lane >> 4)]);
+}
+
+// the same in the order in which two tiles of a product's result hold a column (rows 4 g to
+// 4 g + 3 of each, g = l / 16), so that such a result is the other operand without a move;
+template <int N, int kPitch>
+__device__ inline void operand_rows_as_results(const uint16_t (&rows)[N][kChunk][kPitch], int row0, int m,
+                                               u4 (&x)[N]) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        const uint16_t* row = &rows[n][row0 + (lane & 15)][32 * m + 4 * (lane >> 4)];
+        const u2 a = *reinterpret_cast<const u2*>(row), b = *reinterpret_cast<const u2*>(row + 16);
+        x[n] = u4{a.x, a.y, b.x, b.y};
+    }
+}
+
+// and columns 16 c to 16 c + 15 as the operand's rows, tokens 32 m to 32 m + 31 contracted in
+// that same order.
+template <int N, int kPitch>
+__device__ inline void operand_columns(const uint16_t (&rows)[N][kChunk][kPitch], int c, int m, u4 (&x)[N]) {
+    const int lane = threadIdx.x & 63, i = lane & 15;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        const uint16_t* from = &rows[n][32 * m + 4 * (lane >> 4) + (i >> 2)][16 * c + 4 * (i & 3)];
+        const u2 a = read_transposed(from), b = read_transposed(from + 16 * kPitch);
+        x[n] = u4{a.x, a.y, b.x, b.y};
+    }
+}
+
+// A triangle's rows 16 i to 16 i + 15, columns 32 m to 32 m + 31 (32 m <= 16 i) as an operand
+// whose contracted axis is in the order of results;
+__device__ inline void operand_triangle(const Triangle& t, int i, int m, u4 (&x)[3]) {
+    const int lane = threadIdx.x & 63, l = lane & 15;
+    const int slot = (l & 3) * 16 + 4 * (lane >> 4) + (l >> 2);
+#pragma unroll
+    for (int n = 0; n < 3; ++n) {
+        const u2 a = read_transposed(t[tile_of(i, 2 * m)][n][slot]);
+        const u2 b = 2 * m + 1 <= i ? read_transposed(t[tile_of(i, 2 * m + 1)][n][slot]) : u2{0, 0};
+        x[n] = u4{a.x, a.y, b.x, b.y};
+    }
+}
+
+// and of its transpose, rows 16 j on, columns 32 m on (16 j < 32 m + 32).
+__device__ inline void operand_transpose(const Triangle& t, int j, int m, u4 (&x)[3]) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int n = 0; n < 3; ++n) {
+        const u2 a = 2 * m >= j ? *reinterpret_cast<const u2*>(t[tile_of(2 * m, j)][n][lane]) : u2{0, 0};
+        const u2 b = *reinterpret_cast<const u2*>(t[tile_of(2 * m + 1, j)][n][lane]);
+        x[n] = u4{a.x, a.y, b.x, b.y};
+    }
+}
+
+__device__ inline void store_tile(Triangle& t, int tile, f4 x) {
+    const int lane = threadIdx.x & 63;
+    uint32_t a[3], b[3];
+    split_pair<3>(x[0], x[1], a);
+    split_pair<3>(x[2], x[3], b);
+#pragma unroll
+    for (int n = 0; n < 3; ++n) *reinterpret_cast<u2*>(t[tile][n][lane]) = u2{a[n], b[n]};
+}
+
+__device__ constexpr int tile_row(int tile) { return tile < 1 ? 0 : tile < 3 ? 1 : tile < 6 ? 2 : 3; }
+
+// The inverse of I + the strictly lower triangle in `a`, in its place (unit diagonal and zeros
+// above it within diagonal tiles; tiles above are not touched). All threads of the workgroup.
+__device__ inline void invert_triangle(float (&a)[kChunk][kChunk + 4], int wave, int waves) {
+    const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+    // Diagonal tiles by forward substitution, a column a lane, four tiles in a wave.
+    if (wave == 0) {
+        const int at = 16 * g;
+        float x[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            float s = i == col ? 1.0f : 0.0f;
+#pragma unroll
+            for (int m = 0; m < i; m += 4) {
+                const f4 row = *reinterpret_cast<const f4*>(&a[at + i][at + m]);
+#pragma unroll
+                for (int n = 0; n < 4; ++n)
+                    if (m + n < i) s -= row[n] * x[m + n];
+            }
+            x[i] = s;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) a[at + i][at + col] = x[i];
+    }
+    __syncthreads();
+    // The tile below two diagonal ones: -X22 A21 X11.
+    for (int pair = wave; pair < 2; pair += waves) {
+        const int lo = 32 * pair, hi = lo + 16;
+        const f4 below = *reinterpret_cast<const f4*>(&a[hi + col][lo + 4 * g]);
+        const f4 left = *reinterpret_cast<const f4*>(&a[hi + col][hi + 4 * g]);
+        f4 t = {0, 0, 0, 0}, x = {0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < 4; ++s) t = mfma_f32(below[s], a[lo + 4 * g + s][lo + col], t);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) x = mfma_f32(left[s], t[s], x);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) a[hi + 4 * g + s][lo + col] = -x[s];
+    }
+    __syncthreads();
+    // The four tiles below those pairs, by columns of tiles.
+    f4 x[2][2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        if (j % waves != wave) continue;
+        f4 t[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            t[i] = f4{0, 0, 0, 0};
+#pragma unroll
+            for (int m = j; m < 2; ++m) {
+                const f4 below = *reinterpret_cast<const f4*>(&a[32 + 16 * i + col][16 * m + 4 * g]);
+#pragma unroll
+                for (int s = 0; s < 4; ++s) t[i] = mfma_f32(below[s], a[16 * m + 4 * g + s][16 * j + col], t[i]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            x[j][i] = f4{0, 0, 0, 0};
+#pragma unroll
+            for (int m = 0; m <= i; ++m) {
+                const f4 left = *reinterpret_cast<const f4*>(&a[32 + 16 * i + col][32 + 16 * m + 4 * g]);
+#pragma unroll
+                for (int s = 0; s < 4; ++s) x[j][i] = mfma_f32(left[s], t[m][s], x[j][i]);
+            }
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+        if (j % waves == wave)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int s = 0; s < 4; ++s) a[32 + 16 * i + 4 * g + s][16 * j + col] = -x[j][i][s];
+    __syncthreads();
+}
+
+// X and P of the chunk whose rows and gates are in LDS. All threads; ends with a barrier.
+template <class E, int KP>
+__device__ inline void make_triangles(const ChunkRows<E, KP>& rows, const ChunkGates& gates, ChunkTriangles& tri,
+                                      float scale, int wave, int waves) {
+    constexpr int N = kPlanes<E>;
+    const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+    for (int tile = wave; tile < kTiles; tile += waves) {
+        const int i = tile_row(tile), j = tile - tile_of(i, 0);
+        f4 kk = {0, 0, 0, 0}, qk = {0, 0, 0, 0};
+#pragma unroll
+        for (int m = 0; m < KP / 32; ++m) {
+            u4 ki[N], qi[N], kj[N];
+            operand_rows(rows.k, 16 * j, m, kj);
+            operand_rows(rows.k, 16 * i, m, ki);
+            kk = mma(ki, kj, kk);
+            operand_rows(rows.q, 16 * i, m, qi);
+            qk = mma(qi, kj, qk);
+        }
+        const int column = 16 * j + col;
+        const float hi = gates.hi[column], lo = gates.lo[column], beta = gates.beta[column];
+        const int episode = gates.episode[column];
+        f4 p;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            const int row = 16 * i + 4 * g + s;
+            const float d = row >= column ? decay(gates, row, hi, lo, episode) * beta : 0.0f;
+            tri.work[row][column] = row > column ? d * kk[s] : 0.0f;
+            p[s] = scale * d * qk[s];
+        }
+        store_tile(tri.p, tile, p);
+    }
+    __syncthreads();
+    invert_triangle(tri.work, wave, waves);
+    for (int tile = wave; tile < kTiles; tile += waves) {
+        const int i = tile_row(tile), j = tile - tile_of(i, 0);
+        f4 x;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) x[s] = tri.work[16 * i + 4 * g + s][16 * j + col];
+        store_tile(tri.x, tile, x);
+    }
+    __syncthreads();
+}
+
+}  // namespace navi_policy

@@ -1,0 +1,775 @@
+// delta_rule.hip — the gated delta rule over chunks of 64 tokens: forward, and the two
+// kernels of its backward pass (mathematics in delta_chunk.hpp).
+#include <algorithm>
+#include <climits>
+
+#include "delta_chunk.hpp"
+
+namespace navi_policy {
+namespace {
+
+constexpr int kMaxWaves = 8;  // of 16 value columns each in a workgroup
+
+// One column of 16 tokens' tiles in the layout of products: row 4 (l / 16) + s of tile i.
+template <class E>
+__device__ inline f4 load_results(const E* base, int64_t step_stride, int row, int tokens, bool inside) {
+    f4 x;
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+        x[s] = inside && row + s < tokens ? to_float(base[(row + s) * step_stride]) : 0.0f;
+    return x;
+}
+
+__device__ inline f4 four(const float (&x)[kChunk], int row) { return *reinterpret_cast<const f4*>(&x[row]); }
+
+// x * factor, 0 where the factor is 0 whatever x is: a state that an episode's start clears.
+__device__ inline f4 gated(f4 x, f4 factor) {
+    f4 y;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) y[s] = factor[s] == 0.0f ? 0.0f : x[s] * factor[s];
+    return y;
+}
+
+template <class E, int KP>
+struct ScanLds {
+    ChunkRows<E, KP> rows;
+    ChunkTriangles tri;
+    ChunkGates gates;
+};
+
+// A wave holds 16 columns of the state as results of products (KP / 16 tiles), a workgroup
+// blockDim / 64 such columns of one head; it walks the chunks with the state in registers.
+// The state is the second operand of S^T k without a move: its tiles hold the contracted axis
+// in the order of results, which the other operand is read in as well.
+template <class E, int KP>
+__global__ __launch_bounds__(64 * kMaxWaves) void delta_forward_kernel(RuleParams P) {
+    constexpr int N = kPlanes<E>;
+    extern __shared__ char lds_bytes[];
+    auto& lds = *reinterpret_cast<ScanLds<E, KP>*>(lds_bytes);
+    const int lane = threadIdx.x & 63, wave = wave_of_workgroup(), waves = blockDim.x >> 6;
+    const int col = lane & 15, g = lane >> 4;
+    const int64_t sequence = blockIdx.x;
+    const int64_t env = sequence / P.r.value_heads;
+    const int head = static_cast<int>(sequence % P.r.value_heads);
+    const int column = (blockIdx.y * waves + wave) * 16 + col;
+    const bool inside = column < P.r.value_dim;
+    const int K = P.r.key_dim, V = P.r.value_dim;
+
+    f4 state[KP / 16];
+    const float* from = P.r.initial_state ? P.r.initial_state + sequence * K * V + column : nullptr;
+#pragma unroll
+    for (int c = 0; c < KP / 16; ++c)
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            const int row = 16 * c + 4 * g + s;
+            state[c][s] = from && inside && row < K ? from[static_cast<int64_t>(row) * V] : 0.0f;
+        }
+
+    for (int chunk = 0; chunk < P.n_chunks; ++chunk) {
+        const int64_t t0 = static_cast<int64_t>(chunk) * kChunk;
+        const int tokens = static_cast<int>(P.r.steps - t0 < kChunk ? P.r.steps - t0 : kChunk);
+        __syncthreads();
+        load_rows<E, KP>(P, lds.rows, env, head, t0, tokens);
+        if (wave == 0) load_gates(P, lds.gates, env, head, t0, tokens);
+        __syncthreads();
+        make_triangles<E, KP>(lds.rows, lds.gates, lds.tri, P.r.scale, wave, waves);
+
+        if (P.r.states && chunk > 0) {
+            float* to = P.r.states + (sequence * (P.n_chunks - 1) + chunk - 1) * K * V + column;
+#pragma unroll
+            for (int c = 0; c < KP / 16; ++c)
+#pragma unroll
+                for (int s = 0; s < 4; ++s)
+                    if (inside && 16 * c + 4 * g + s < K) to[static_cast<int64_t>(16 * c + 4 * g + s) * V] = state[c][s];
+        }
+
+        f4 u[4], o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) u[i] = o[i] = f4{0, 0, 0, 0};
+        if (chunk > 0 || from) {
+#pragma unroll
+            for (int m = 0; m < KP / 32; ++m) {
+                u4 b[3], a[N];
+                split8(state[2 * m], state[2 * m + 1], b);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    operand_rows_as_results(lds.rows.k, 16 * i, m, a);
+                    u[i] = mma(a, b, u[i]);
+                    operand_rows_as_results(lds.rows.q, 16 * i, m, a);
+                    o[i] = mma(a, b, o[i]);
+                }
+            }
+        }
+        const E* v = at<E>(P.r.v, P.r.v_stride, env, t0, head) + column;
+        u4 r[2][3];
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            f4 x[2];
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                const int i = 2 * m + n, row = 16 * i + 4 * g;
+                const f4 e = four(lds.gates.e, row);
+                x[n] = load_results(v, P.r.v_stride[1], row, tokens, inside) - gated(u[i], e);
+                o[i] = P.r.scale * gated(o[i], e);
+                u[i] = f4{0, 0, 0, 0};
+            }
+            split8(x[0], x[1], r[m]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int m = 0; m <= i / 2; ++m) {
+                u4 a[3];
+                operand_triangle(lds.tri.x, i, m, a);
+                u[i] = mma(a, r[m], u[i]);
+            }
+        if (P.r.updates) {
+            float* to = P.r.updates + (sequence * P.r.steps + t0) * V + column;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int s = 0; s < 4; ++s)
+                    if (inside && 16 * i + 4 * g + s < tokens)
+                        to[static_cast<int64_t>(16 * i + 4 * g + s) * V] = u[i][s];
+        }
+#pragma unroll
+        for (int m = 0; m < 2; ++m) split8(u[2 * m], u[2 * m + 1], r[m]);
+        E* out = static_cast<E*>(P.r.out) + ((env * P.r.steps + t0) * P.r.value_heads + head) * V + column;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+            for (int m = 0; m <= i / 2; ++m) {
+                u4 a[3];
+                operand_triangle(lds.tri.p, i, m, a);
+                o[i] = mma(a, r[m], o[i]);
+            }
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                const int t = 16 * i + 4 * g + s;
+                if (inside && t < tokens) out[static_cast<int64_t>(t) * P.r.value_heads * V] = from_float<E>(o[i][s]);
+            }
+        }
+        const float keep = lds.gates.e[kChunk - 1];
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            f4 x[2];
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                const int row = 16 * (2 * m + n) + 4 * g;
+                x[n] = u[2 * m + n] * four(lds.gates.f, row) * four(lds.gates.beta, row);
+            }
+            split8(x[0], x[1], r[m]);
+        }
+#pragma unroll
+        for (int c = 0; c < KP / 16; ++c) {
+            state[c] = gated(state[c], f4{keep, keep, keep, keep});
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                u4 a[N];
+                operand_columns(lds.rows.k, c, m, a);
+                state[c] = mma(a, r[m], state[c]);
+            }
+        }
+    }
+    if (P.r.final_state && inside) {
+        float* to = P.r.final_state + sequence * K * V + column;
+#pragma unroll
+        for (int c = 0; c < KP / 16; ++c)
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+                if (16 * c + 4 * g + s < K) to[static_cast<int64_t>(16 * c + 4 * g + s) * V] = state[c][s];
+    }
+}
+
+// Backward through the chunks from the last to the first, the gradient dS of the state after
+// a chunk in registers as the state is in the forward pass:
+//
+//     du = P^T do + beta F (k dS),   dr = X^T du  (= dv),
+//     dS <- E_last dS + q^T (scale E do) - k^T (E dr)
+//
+// dS and dr go to memory for delta_gradients_kernel.
+template <class E, int KP>
+__global__ __launch_bounds__(64 * kMaxWaves) void delta_reverse_kernel(RuleParams P) {
+    constexpr int N = kPlanes<E>;
+    extern __shared__ char lds_bytes[];
+    auto& lds = *reinterpret_cast<ScanLds<E, KP>*>(lds_bytes);
+    const int lane = threadIdx.x & 63, wave = wave_of_workgroup(), waves = blockDim.x >> 6;
+    const int col = lane & 15, g = lane >> 4;
+    const int64_t sequence = blockIdx.x;
+    const int64_t env = sequence / P.r.value_heads;
+    const int head = static_cast<int>(sequence % P.r.value_heads);
+    const int column = (blockIdx.y * waves + wave) * 16 + col;
+    const bool inside = column < P.r.value_dim;
+    const int K = P.r.key_dim, V = P.r.value_dim;
+
+    f4 dstate[KP / 16];
+    const float* from = P.d.grad_final_state ? P.d.grad_final_state + sequence * K * V + column : nullptr;
+#pragma unroll
+    for (int c = 0; c < KP / 16; ++c)
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            const int row = 16 * c + 4 * g + s;
+            dstate[c][s] = from && inside && row < K ? from[static_cast<int64_t>(row) * V] : 0.0f;
+        }
+
+    for (int chunk = P.n_chunks - 1; chunk >= 0; --chunk) {
+        const int64_t t0 = static_cast<int64_t>(chunk) * kChunk;
+        const int tokens = static_cast<int>(P.r.steps - t0 < kChunk ? P.r.steps - t0 : kChunk);
+        __syncthreads();
+        load_rows<E, KP>(P, lds.rows, env, head, t0, tokens);
+        if (wave == 0) load_gates(P, lds.gates, env, head, t0, tokens);
+        __syncthreads();
+        make_triangles<E, KP>(lds.rows, lds.gates, lds.tri, P.r.scale, wave, waves);
+
+        const bool last = chunk + 1 == P.n_chunks;
+        if (!last) {
+            float* to = P.dstates + (sequence * (P.n_chunks - 1) + chunk) * K * V + column;
+#pragma unroll
+            for (int c = 0; c < KP / 16; ++c)
+#pragma unroll
+                for (int s = 0; s < 4; ++s)
+                    if (inside && 16 * c + 4 * g + s < K) to[static_cast<int64_t>(16 * c + 4 * g + s) * V] = dstate[c][s];
+        }
+
+        f4 du[4], dO[4];
+        const E* grad = at<E>(P.d.grad_out, P.d.grad_out_stride, env, t0, head) + column;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            du[i] = f4{0, 0, 0, 0};
+            dO[i] = load_results(grad, P.d.grad_out_stride[1], 16 * i + 4 * g, tokens, inside);
+        }
+        if (!last || from) {
+#pragma unroll
+            for (int m = 0; m < KP / 32; ++m) {
+                u4 b[3], a[N];
+                split8(dstate[2 * m], dstate[2 * m + 1], b);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    operand_rows_as_results(lds.rows.k, 16 * i, m, a);
+                    du[i] = mma(a, b, du[i]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                du[i] = du[i] * four(lds.gates.f, 16 * i + 4 * g) * four(lds.gates.beta, 16 * i + 4 * g);
+        }
+        u4 b[2][3];
+        {
+            u4 raw[2][N];
+#pragma unroll
+            for (int m = 0; m < 2; ++m) split8(dO[2 * m], dO[2 * m + 1], raw[m]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int m = j / 2; m < 2; ++m) {
+                    u4 a[3];
+                    operand_transpose(lds.tri.p, j, m, a);
+                    du[j] = mma(a, raw[m], du[j]);
+                }
+        }
+#pragma unroll
+        for (int m = 0; m < 2; ++m) split8(du[2 * m], du[2 * m + 1], b[m]);
+        E* dv = static_cast<E*>(P.d.d_v) + ((env * P.r.steps + t0) * P.r.value_heads + head) * V + column;
+        float* to = P.rgrads + (sequence * P.r.steps + t0) * V + column;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            f4 dr = {0, 0, 0, 0};
+#pragma unroll
+            for (int m = j / 2; m < 2; ++m) {
+                u4 a[3];
+                operand_transpose(lds.tri.x, j, m, a);
+                dr = mma(a, b[m], dr);
+            }
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                const int t = 16 * j + 4 * g + s;
+                if (inside && t < tokens) {
+                    dv[static_cast<int64_t>(t) * P.r.value_heads * V] = from_float<E>(dr[s]);
+                    to[static_cast<int64_t>(t) * V] = dr[s];
+                }
+            }
+            const f4 e = four(lds.gates.e, 16 * j + 4 * g);
+            du[j] = -e * dr;
+            dO[j] = P.r.scale * e * dO[j];
+        }
+        if (chunk > 0 || P.d.d_initial_state) {
+            const float keep = lds.gates.e[kChunk - 1];
+            u4 c3[2][3];
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                split8(du[2 * m], du[2 * m + 1], b[m]);
+                split8(dO[2 * m], dO[2 * m + 1], c3[m]);
+            }
+#pragma unroll
+            for (int c = 0; c < KP / 16; ++c) {
+                dstate[c] = gated(dstate[c], f4{keep, keep, keep, keep});
+#pragma unroll
+                for (int m = 0; m < 2; ++m) {
+                    u4 a[N];
+                    operand_columns(lds.rows.k, c, m, a);
+                    dstate[c] = mma(a, b[m], dstate[c]);
+                    operand_columns(lds.rows.q, c, m, a);
+                    dstate[c] = mma(a, c3[m], dstate[c]);
+                }
+            }
+        }
+    }
+    if (P.d.d_initial_state && inside) {
+        float* to = P.d.d_initial_state + sequence * K * V + column;
+#pragma unroll
+        for (int c = 0; c < KP / 16; ++c)
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+                if (16 * c + 4 * g + s < K) to[static_cast<int64_t>(16 * c + 4 * g + s) * V] = dstate[c][s];
+    }
+}
+
+// The gradients of one chunk of one head, all chunks at once, from the states S before and
+// the state gradients dS after each, u and dr. With H = do u^T, R = dr u^T (lower triangles),
+// Y = do S^T, Z = dr S^T, W = u dS^T:
+//
+//     N_ij = scale D_ij H_ij beta_j (i >= j),  M_ij = -R_ij D_ij beta_j (i > j)
+//     dq_i = scale E_i Y_i + sum_j N_ij k_j
+//     dk_i = beta_i F_i W_i - E_i Z_i + sum_j M_ij k_j + sum_j (N_ji q_j + M_ji k_j)
+//     dbeta_j = F_j k_j . W_j + sum_i (scale D_ij H_ij q_i . k_j - R_ij D_ij k_i . k_j)
+//     dG_i = sum_j B_ij - sum_j B_ji + scale E_i q_i . Y_i - E_i k_i . Z_i - beta_i F_i k_i . W_i,
+//     B_ij = N_ij q_i . k_j + M_ij k_i . k_j (i > j),
+//     dG_last += sum_j beta_j F_j k_j . W_j + E_last <S, dS>,  dg_t = sum_{i >= t} dG_i
+//
+// The same number stands at +i and -j of dG, so what cancels in dg cancels to its rounding.
+template <class E, int KP>
+struct GradientLds {
+    union {
+        struct {
+            uint16_t s[KP / 16][3][64][8], ds[KP / 16][3][64][8];  // 32 columns of S and dS as operands
+            uint16_t u[4][3][64][8];                                // and of u
+        } stage;
+        ChunkRows<E, KP> rows;
+    };
+    Triangle n, m;
+    ChunkGates gates;
+    float beta_part[4][kChunk], g_part[4][kChunk], beta_row[kChunk], g_row[kChunk], f_row[kChunk];
+    float dot_part[4];
+};
+
+// Eight floats of a row of `valid` columns.
+__device__ inline void load_state8(const float* row, int valid, bool wide, float (&x)[8]) { load8(row, valid, wide, x); }
+
+__device__ inline float sum16(float x) {  // over 16 lanes in a row
+#pragma unroll
+    for (int d = 1; d < 16; d *= 2) x += __shfl_xor(x, d);
+    return x;
+}
+
+template <class E, int KP>
+__global__ __launch_bounds__(256) void delta_gradients_kernel(RuleParams P) {
+    constexpr int N = kPlanes<E>;
+    extern __shared__ char lds_bytes[];
+    auto& lds = *reinterpret_cast<GradientLds<E, KP>*>(lds_bytes);
+    const int lane = threadIdx.x & 63, wave = wave_of_workgroup();
+    const int col = lane & 15, g = lane >> 4;
+    const int64_t sequence = blockIdx.x / static_cast<uint32_t>(P.n_chunks);
+    const int chunk = static_cast<int>(blockIdx.x % static_cast<uint32_t>(P.n_chunks));
+    const int64_t env = sequence / P.r.value_heads;
+    const int head = static_cast<int>(sequence % P.r.value_heads);
+    const int K = P.r.key_dim, V = P.r.value_dim;
+    const int64_t t0 = static_cast<int64_t>(chunk) * kChunk;
+    const int tokens = static_cast<int>(P.r.steps - t0 < kChunk ? P.r.steps - t0 : kChunk);
+
+    const int64_t kv = static_cast<int64_t>(K) * V, inner = sequence * (P.n_chunks - 1);
+    const float* S = chunk > 0 ? P.r.states + (inner + chunk - 1) * kv
+                               : P.r.initial_state ? P.r.initial_state + sequence * kv : nullptr;
+    const float* dS = chunk + 1 < P.n_chunks ? P.dstates + (inner + chunk) * kv
+                                              : P.d.grad_final_state ? P.d.grad_final_state + sequence * kv : nullptr;
+    const float* u = P.r.updates + (sequence * P.r.steps + t0) * V;
+    const float* dr = P.rgrads + (sequence * P.r.steps + t0) * V;
+    const int my_token = 16 * wave + col;  // of the wave's tile of tokens, as an operand's row
+    const E* my_do = at<E>(P.d.grad_out, P.d.grad_out_stride, env, t0 + (my_token < tokens ? my_token : 0), head);
+    const float* my_dr = dr + static_cast<int64_t>(my_token < tokens ? my_token : 0) * V;
+
+    if (wave == 0) load_gates(P, lds.gates, env, head, t0, tokens);
+    f4 y[KP / 16], z[KP / 16], w[KP / 16], h[4], rr[4];
+#pragma unroll
+    for (int c = 0; c < KP / 16; ++c) y[c] = z[c] = w[c] = f4{0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) h[j] = rr[j] = f4{0, 0, 0, 0};
+    float dot = 0.0f;
+    for (int v0 = 0; v0 < V; v0 += 32) {
+        __syncthreads();
+        for (int piece = threadIdx.x; piece < 4 * KP; piece += 256) {
+            const int row = piece >> 2, c = (piece & 3) * 8;
+            const int valid = row < K ? V - v0 - c : 0;
+            const int64_t offset = static_cast<int64_t>(row < K ? row : 0) * V + v0 + c;
+            float a[8] = {}, b[8] = {};
+            if (S) load_state8(S + offset, valid, P.wide_state, a);
+            if (dS) load_state8(dS + offset, valid, P.wide_state, b);
+            u4 plane[3];
+            const int slot = (row & 15) + 16 * (piece & 3);
+            if (S) {
+                split8(a, plane);
+#pragma unroll
+                for (int n = 0; n < 3; ++n) *reinterpret_cast<u4*>(lds.stage.s[row >> 4][n][slot]) = plane[n];
+            }
+            if (dS) {
+                split8(b, plane);
+#pragma unroll
+                for (int n = 0; n < 3; ++n) *reinterpret_cast<u4*>(lds.stage.ds[row >> 4][n][slot]) = plane[n];
+            }
+#pragma unroll
+            for (int n = 0; n < 8; ++n) dot += a[n] * b[n];
+        }
+        {
+            const int row = threadIdx.x >> 2, c = (threadIdx.x & 3) * 8;
+            float a[8];
+            u4 plane[3];
+            load_state8(u + static_cast<int64_t>(row < tokens ? row : 0) * V + v0 + c, row < tokens ? V - v0 - c : 0,
+                        P.wide_state, a);
+            split8(a, plane);
+#pragma unroll
+            for (int n = 0; n < 3; ++n)
+                *reinterpret_cast<u4*>(lds.stage.u[row >> 4][n][(row & 15) + 16 * (threadIdx.x & 3)]) = plane[n];
+        }
+        u4 a_do[N], a_dr[3], a_u[3];
+        {
+            float x[8];
+            const int valid = my_token < tokens ? V - v0 - 8 * g : 0;
+            load8(my_do + v0 + 8 * g, valid, P.wide_do, x);
+            split8(x, a_do);
+            load_state8(my_dr + v0 + 8 * g, valid, P.wide_state, x);
+            split8(x, a_dr);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < 3; ++n) a_u[n] = *reinterpret_cast<const u4*>(lds.stage.u[wave][n][lane]);
+#pragma unroll
+        for (int c = 0; c < KP / 16; ++c) {
+            u4 b[3];
+            if (S) {
+#pragma unroll
+                for (int n = 0; n < 3; ++n) b[n] = *reinterpret_cast<const u4*>(lds.stage.s[c][n][lane]);
+                y[c] = mma(a_do, b, y[c]);
+                z[c] = mma(a_dr, b, z[c]);
+            }
+            if (dS) {
+#pragma unroll
+                for (int n = 0; n < 3; ++n) b[n] = *reinterpret_cast<const u4*>(lds.stage.ds[c][n][lane]);
+                w[c] = mma(a_u, b, w[c]);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (j > wave) continue;
+            u4 b[3];
+#pragma unroll
+            for (int n = 0; n < 3; ++n) b[n] = *reinterpret_cast<const u4*>(lds.stage.u[j][n][lane]);
+            h[j] = mma(a_do, b, h[j]);
+            rr[j] = mma(a_dr, b, rr[j]);
+        }
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) dot += __shfl_xor(dot, d);
+    if (lane == 0) lds.dot_part[wave] = dot;
+    __syncthreads();
+    load_rows<E, KP>(P, lds.rows, env, head, t0, tokens);
+    __syncthreads();
+
+    // The triangles N and M; the sums over their rows and columns.
+    const int row = 16 * wave + 4 * g;
+    f4 row_sum = {0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        float beta_sum = 0.0f, g_sum = 0.0f;
+        if (j <= wave) {
+            f4 kk = {0, 0, 0, 0}, qk = {0, 0, 0, 0};
+#pragma unroll
+            for (int m = 0; m < KP / 32; ++m) {
+                u4 a[N], b[N];
+                operand_rows(lds.rows.k, 16 * j, m, b);
+                operand_rows(lds.rows.k, 16 * wave, m, a);
+                kk = mma(a, b, kk);
+                operand_rows(lds.rows.q, 16 * wave, m, a);
+                qk = mma(a, b, qk);
+            }
+            const int column = 16 * j + col;
+            const float hi = lds.gates.hi[column], lo = lds.gates.lo[column], beta = lds.gates.beta[column];
+            const int episode = lds.gates.episode[column];
+            f4 n, mm;
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                const bool below = row + s > column, on = row + s >= column;
+                const float d = on ? decay(lds.gates, row + s, hi, lo, episode) : 0.0f;
+                const float ph = P.r.scale * d * h[j][s];
+                const float rd = below ? rr[j][s] * d : 0.0f;
+                n[s] = on ? ph * beta : 0.0f;
+                mm[s] = -rd * beta;
+                const float pair = below ? n[s] * qk[s] + mm[s] * kk[s] : 0.0f;
+                beta_sum += on ? ph * qk[s] - rd * kk[s] : 0.0f;
+                g_sum += pair;
+                row_sum[s] += pair;
+            }
+            store_tile(lds.n, tile_of(wave, j), n);
+            store_tile(lds.m, tile_of(wave, j), mm);
+        }
+#pragma unroll
+        for (int d = 16; d < 64; d *= 2) {
+            beta_sum += __shfl_xor(beta_sum, d);
+            g_sum += __shfl_xor(g_sum, d);
+        }
+        if (g == 0) {
+            lds.beta_part[wave][16 * j + col] = beta_sum;
+            lds.g_part[wave][16 * j + col] = g_sum;
+        }
+    }
+    const f4 e = four(lds.gates.e, row), f = four(lds.gates.f, row), beta = four(lds.gates.beta, row);
+    f4 qy = {0, 0, 0, 0}, kz = {0, 0, 0, 0}, kw = {0, 0, 0, 0};
+#pragma unroll
+    for (int c = 0; c < KP / 16; ++c) {
+        y[c] = P.r.scale * gated(y[c], e);
+        z[c] = gated(z[c], e);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            float qx = 0.0f, kx = 0.0f;
+#pragma unroll
+            for (int n = N - 1; n >= 0; --n) {
+                qx += to_float(bf16{lds.rows.q[n][row + s][16 * c + col]});
+                kx += to_float(bf16{lds.rows.k[n][row + s][16 * c + col]});
+            }
+            qy[s] += qx * y[c][s];
+            kz[s] += kx * z[c][s];
+            kw[s] += kx * w[c][s];
+        }
+    }
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+        const float own = sum16(row_sum[s] + qy[s] - kz[s]), left = f[s] * sum16(kw[s]);
+        if (col == 0) {
+            lds.beta_row[row + s] = left;
+            lds.f_row[row + s] = beta[s] * left;
+            lds.g_row[row + s] = own - beta[s] * left;
+        }
+    }
+    __syncthreads();
+    if (wave == 0) {
+        float dbeta = lds.beta_row[lane], dG = lds.g_row[lane], f_all = lds.f_row[lane];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            dbeta += lds.beta_part[n][lane];
+            dG -= lds.g_part[n][lane];
+        }
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) f_all += __shfl_xor(f_all, d);
+        if (lane == 63) {
+            const float keep = lds.gates.e[63];
+            dG += f_all;
+            if (keep != 0.0f)
+                dG += keep * ((lds.dot_part[0] + lds.dot_part[1]) + (lds.dot_part[2] + lds.dot_part[3]));
+        }
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const float later = __shfl_down(dG, d);
+            dG += lane + d < 64 ? later : 0.0f;
+        }
+        if (lane < tokens) {
+            const int before = lane > 0 ? lds.gates.episode[lane - 1] : 0;
+            const int64_t to = (env * P.r.steps + t0 + lane) * P.r.value_heads + head;
+            P.d.d_g[to] = lds.gates.episode[lane] != before ? 0.0f : dG;
+            P.d.d_beta[to] = dbeta;
+        }
+    }
+
+    // dq and dk, 16 columns of the key dimension at a time.
+#pragma unroll
+    for (int c = 0; c < KP / 16; ++c) {
+        f4 dq = y[c], dk = beta * f * w[c] - z[c];
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            u4 a[3], b[N];
+            operand_columns(lds.rows.k, c, m, b);
+            if (2 * m <= wave) {
+                operand_triangle(lds.n, wave, m, a);
+                dq = mma(a, b, dq);
+                operand_triangle(lds.m, wave, m, a);
+                dk = mma(a, b, dk);
+            }
+            if (2 * m + 1 >= wave) {
+                operand_transpose(lds.m, wave, m, a);
+                dk = mma(a, b, dk);
+                operand_columns(lds.rows.q, c, m, b);
+                operand_transpose(lds.n, wave, m, a);
+                dk = mma(a, b, dk);
+            }
+        }
+        const int column = 16 * c + col;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            if (row + s >= tokens || column >= K) continue;
+            if (P.group == 1) {
+                const int64_t to = ((env * P.r.steps + t0 + row + s) * P.r.key_heads + head) * K + column;
+                static_cast<E*>(P.d.d_q)[to] = from_float<E>(dq[s]);
+                static_cast<E*>(P.d.d_k)[to] = from_float<E>(dk[s]);
+            } else {
+                const int64_t to = ((env * P.r.steps + t0 + row + s) * P.r.value_heads + head) * K + column;
+                P.dq_heads[to] = dq[s];
+                P.dk_heads[to] = dk[s];
+            }
+        }
+    }
+}
+
+// A key head's gradients are the sum of its value heads', in their order.
+template <class E>
+__global__ __launch_bounds__(256) void delta_join_heads_kernel(RuleParams P, int64_t count) {
+    const int K = P.r.key_dim;
+    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < count; i += gridDim.x * 256ll) {
+        const int64_t row = i / K;
+        const int64_t from = row * P.group * K + i % K;
+        float q = 0.0f, k = 0.0f;
+        for (int n = 0; n < P.group; ++n) {
+            q += P.dq_heads[from + static_cast<int64_t>(n) * K];
+            k += P.dk_heads[from + static_cast<int64_t>(n) * K];
+        }
+        static_cast<E*>(P.d.d_q)[i] = from_float<E>(q);
+        static_cast<E*>(P.d.d_k)[i] = from_float<E>(k);
+    }
+}
+
+int launched(const char* what) {
+    const hipError_t err = hipGetLastError();
+    if (err != hipSuccess) return set_error(NAVI_POLICY_E_LAUNCH, "%s: kernel launch failed: %s", what, hipGetErrorString(err));
+    return NAVI_POLICY_OK;
+}
+
+// Waves of a workgroup: all of a head's columns up to 128, so that the triangles are made once.
+int waves_of(int value_dim) { return std::min(kMaxWaves, (value_dim + 15) / 16); }
+
+template <class E, int KP>
+int forward(const RuleParams& P, hipStream_t stream) {
+    const int waves = waves_of(P.r.value_dim);
+    const dim3 grid(static_cast<unsigned>(P.r.envs * P.r.value_heads), (P.r.value_dim + 16 * waves - 1) / (16 * waves));
+    hipLaunchKernelGGL((delta_forward_kernel<E, KP>), grid, dim3(64 * waves), sizeof(ScanLds<E, KP>), stream, P);
+    return launched("navi_delta_forward");
+}
+
+template <class E, int KP>
+int backward(const RuleParams& P, hipStream_t stream) {
+    const int waves = waves_of(P.r.value_dim);
+    const dim3 grid(static_cast<unsigned>(P.r.envs * P.r.value_heads), (P.r.value_dim + 16 * waves - 1) / (16 * waves));
+    hipLaunchKernelGGL((delta_reverse_kernel<E, KP>), grid, dim3(64 * waves), sizeof(ScanLds<E, KP>), stream, P);
+    int code = launched("navi_delta_backward");
+    if (code != NAVI_POLICY_OK) return code;
+    hipLaunchKernelGGL((delta_gradients_kernel<E, KP>), dim3(grid.x * static_cast<unsigned>(P.n_chunks)), dim3(256),
+                       sizeof(GradientLds<E, KP>), stream, P);
+    code = launched("navi_delta_backward");
+    if (code != NAVI_POLICY_OK || P.group == 1) return code;
+    const int64_t count = P.r.envs * P.r.steps * P.r.key_heads * P.r.key_dim;
+    hipLaunchKernelGGL(delta_join_heads_kernel<E>, dim3(static_cast<unsigned>(std::min<int64_t>((count + 255) / 256, 8192))),
+                       dim3(256), 0, stream, P, count);
+    return launched("navi_delta_backward");
+}
+
+template <class E>
+int run(const RuleParams& P, bool back, hipStream_t stream) {
+    if (P.r.key_dim <= 64) return back ? backward<E, 64>(P, stream) : forward<E, 64>(P, stream);
+    return back ? backward<E, 128>(P, stream) : forward<E, 128>(P, stream);
+}
+
+int run_typed(const RuleParams& P, bool back, hipStream_t stream) {
+    if (P.r.dtype == NAVI_POLICY_F32) return run<float>(P, back, stream);
+    if (P.r.dtype == NAVI_POLICY_BF16) return run<bf16>(P, back, stream);
+    return run<f16>(P, back, stream);
+}
+
+int64_t chunks_of(int64_t steps) { return (steps + kChunk - 1) / kChunk; }
+
+bool wide_rows(const void* p, const int64_t (&stride)[3], int64_t bytes, int64_t dim) {
+    return aligned16(p) && dim % 8 == 0 && stride[0] * bytes % 16 == 0 && stride[1] * bytes % 16 == 0 &&
+           stride[2] * bytes % 16 == 0;
+}
+
+}  // namespace
+
+// Sizes that every form needs; 1 where there is nothing to do.
+int check_rule(const navi_delta_rule* r) {
+    if (!r) return set_error(NAVI_POLICY_E_ARG, "rule must be non-null");
+    if (r->dtype < NAVI_POLICY_F32 || r->dtype > NAVI_POLICY_F16)
+        return set_error(NAVI_POLICY_E_ARG, "dtype must be float32, bfloat16 or float16");
+    if (r->key_heads <= 0 || r->value_heads <= 0 || r->value_heads % r->key_heads != 0)
+        return set_error(NAVI_POLICY_E_ARG, "value_heads must be a positive multiple of key_heads");
+    if (r->key_dim <= 0 || r->key_dim > NAVI_POLICY_MAX_KEY_DIM)
+        return set_error(NAVI_POLICY_E_ARG, "key_dim must be in [1, %d]", NAVI_POLICY_MAX_KEY_DIM);
+    if (r->value_dim <= 0 || r->value_dim > 65536) return set_error(NAVI_POLICY_E_ARG, "value_dim must be in [1, 65536]");
+    if (r->envs < 0 || r->steps < 0) return set_error(NAVI_POLICY_E_ARG, "envs and steps must not be negative");
+    if (r->envs > INT32_MAX / r->value_heads || r->steps > INT32_MAX)
+        return set_error(NAVI_POLICY_E_ARG, "envs * value_heads and steps must be below 2^31");
+    if (r->envs == 0) return 1;
+    if (r->steps > 0 && (!r->q || !r->k || !r->v || !r->g || !r->beta || !r->out))
+        return set_error(NAVI_POLICY_E_ARG, "q, k, v, g, beta and out must be non-null");
+    return NAVI_POLICY_OK;
+}
+
+namespace {
+
+int setup(const navi_delta_rule* r, RuleParams& P) {
+    const int code = check_rule(r);
+    if (code != NAVI_POLICY_OK) return code;
+    P.r = *r;
+    P.group = r->value_heads / r->key_heads;
+    P.n_chunks = static_cast<int32_t>(chunks_of(r->steps));
+    const int64_t bytes = r->dtype == NAVI_POLICY_F32 ? 4 : 2;
+    P.wide_qk = wide_rows(r->q, r->q_stride, bytes, r->key_dim) && wide_rows(r->k, r->k_stride, bytes, r->key_dim);
+    return NAVI_POLICY_OK;
+}
+
+}  // namespace
+}  // namespace navi_policy
+
+using namespace navi_policy;
+
+extern "C" int navi_delta_forward(const navi_delta_rule* rule, void* stream) {
+    RuleParams P{};
+    const int code = setup(rule, P);
+    if (code != NAVI_POLICY_OK) return code < 0 ? code : NAVI_POLICY_OK;
+    if (!rule->states != !rule->updates && P.n_chunks > 1)
+        return set_error(NAVI_POLICY_E_ARG, "states and updates are saved together or not at all");
+    if (P.n_chunks == 0 && !rule->final_state) return NAVI_POLICY_OK;
+    return run_typed(P, false, as_stream(stream));
+}
+
+extern "C" int64_t navi_delta_workspace(const navi_delta_rule* rule) {
+    const int code = check_rule(rule);
+    if (code < 0) return code;
+    const int64_t sequences = rule->envs * rule->value_heads, steps = rule->steps;
+    const int64_t inner = std::max<int64_t>(0, chunks_of(steps) - 1);
+    const int64_t states = sequences * inner * rule->key_dim * rule->value_dim;
+    const int64_t rows = sequences * steps * rule->value_dim;
+    const int64_t heads = rule->value_heads > rule->key_heads ? sequences * steps * rule->key_dim : 0;
+    const auto rounded = [](int64_t n) { return (n + 3) / 4 * 4; };
+    return 4 * (rounded(states) + rounded(rows) + 2 * rounded(heads));
+}
+
+extern "C" int navi_delta_backward(const navi_delta_rule* rule, const navi_delta_gradients* gradients, void* stream) {
+    RuleParams P{};
+    const int code = setup(rule, P);
+    if (code != NAVI_POLICY_OK) return code < 0 ? code : NAVI_POLICY_OK;
+    if (!gradients) return set_error(NAVI_POLICY_E_ARG, "gradients must be non-null");
+    P.d = *gradients;
+    if (rule->steps == 0) return set_error(NAVI_POLICY_E_ARG, "the backward pass needs at least one step");
+    if (!P.d.grad_out || !P.d.d_q || !P.d.d_k || !P.d.d_v || !P.d.d_g || !P.d.d_beta || !P.d.workspace)
+        return set_error(NAVI_POLICY_E_ARG, "grad_out, the gradients and workspace must be non-null");
+    if (!rule->updates || (P.n_chunks > 1 && !rule->states))
+        return set_error(NAVI_POLICY_E_ARG, "the backward pass needs the forward pass's states and updates");
+    const int64_t sequences = rule->envs * rule->value_heads;
+    if (sequences * P.n_chunks > INT32_MAX)
+        return set_error(NAVI_POLICY_E_ARG, "envs * value_heads * chunks must be below 2^31");
+    if (!aligned16(P.d.workspace)) return set_error(NAVI_POLICY_E_ARG, "workspace must be 16-byte aligned");
+    const auto rounded = [](int64_t n) { return (n + 3) / 4 * 4; };
+    P.dstates = static_cast<float*>(P.d.workspace);
+    P.rgrads = P.dstates + rounded(sequences * (P.n_chunks - 1) * rule->key_dim * rule->value_dim);
+    P.dq_heads = P.rgrads + rounded(sequences * rule->steps * rule->value_dim);
+    P.dk_heads = P.dq_heads + rounded(P.group > 1 ? sequences * rule->steps * rule->key_dim : 0);
+    const int64_t bytes = rule->dtype == NAVI_POLICY_F32 ? 4 : 2;
+    P.wide_do = wide_rows(P.d.grad_out, P.d.grad_out_stride, bytes, 8) && rule->value_dim % 8 == 0;
+    P.wide_state = rule->value_dim % 4 == 0 && aligned16(rule->states) && aligned16(rule->updates) &&
+                   aligned16(rule->initial_state) && aligned16(P.d.grad_final_state);
+    return run_typed(P, true, as_stream(stream));
+}

@@ -1,0 +1,216 @@
+// grad_norm.hip — the norm of all gradients of a model, and their clipping by it.
+//
+// Two passes: sums of squares, a number a workgroup; then every workgroup adds those numbers
+// (in the same order, in float64) and scales its share. Bound by memory: the gradients are
+// read twice and written once. The second pass walks them from the last to the first, so that
+// what the first left in the caches is read there. Tensors are named in the kernels'
+// arguments, kTensors a launch: nothing is copied to the device or kept.
+#include <algorithm>
+#include <climits>
+
+#include "policy_common.hpp"
+
+namespace navi_policy {
+namespace {
+
+constexpr int kTensors = 112;       // 32 bytes each: a launch's arguments stay under 4 KiB
+constexpr int64_t kPiece = 8192;    // elements that a workgroup takes at once
+
+struct Tensor {
+    const void* from;
+    void* to;
+    int64_t count;
+    int32_t first_piece;
+    int32_t dtype;
+};
+
+struct ClipParams {
+    Tensor tensor[kTensors];
+    float* norm;
+    float* partial;
+    int32_t n_tensors, pieces, n_partials;
+    float max_norm, eps;
+};
+
+// The last tensor whose first piece is not after `piece` (empty tensors own none).
+__device__ inline int tensor_of(const ClipParams& P, int piece) {
+    int lo = 0, hi = P.n_tensors - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (P.tensor[mid].first_piece <= piece)
+            lo = mid;
+        else
+            hi = mid - 1;
+    }
+    return lo;
+}
+
+// Sixteen bytes at any element's address (vector accesses of global memory need no more).
+template <class E>
+struct __attribute__((packed, aligned(sizeof(E)))) Vector {
+    u4 words;
+};
+
+template <class E>
+__device__ inline float square_sum(const E* from, int64_t count) {
+    constexpr int kEach = 16 / sizeof(E);
+    float sum[kEach] = {};
+    const int64_t whole = count / kEach;
+    for (int64_t i = threadIdx.x; i < whole; i += 256) {
+        union {
+            u4 words;
+            E elements[kEach];
+        } got;
+        got.words = reinterpret_cast<const Vector<E>*>(from)[i].words;
+#pragma unroll
+        for (int n = 0; n < kEach; ++n) {
+            const float x = to_float(got.elements[n]);
+            sum[n] += x * x;
+        }
+    }
+    const int64_t left = whole * kEach + threadIdx.x;
+    if (left < count) {
+        const float x = to_float(from[left]);
+        sum[0] += x * x;
+    }
+    float all = 0.0f;
+#pragma unroll
+    for (int n = 0; n < kEach; ++n) all += sum[n];
+    return all;
+}
+
+__device__ inline double sum_block(double x) {
+    __shared__ double part[4];
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) x += __shfl_xor(x, d);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = x;
+    __syncthreads();
+    return (part[0] + part[1]) + (part[2] + part[3]);
+}
+
+__global__ __launch_bounds__(256) void square_sums_kernel(ClipParams P) {
+    double sum = 0.0;
+    for (int piece = blockIdx.x; piece < P.pieces; piece += gridDim.x) {
+        const Tensor& t = P.tensor[tensor_of(P, piece)];
+        const int64_t first = (piece - t.first_piece) * kPiece;
+        const int64_t count = t.count - first < kPiece ? t.count - first : kPiece;
+        if (t.dtype == NAVI_POLICY_F32)
+            sum += square_sum(static_cast<const float*>(t.from) + first, count);
+        else if (t.dtype == NAVI_POLICY_BF16)
+            sum += square_sum(static_cast<const bf16*>(t.from) + first, count);
+        else
+            sum += square_sum(static_cast<const f16*>(t.from) + first, count);
+    }
+    sum = sum_block(sum);
+    if (threadIdx.x == 0) P.partial[blockIdx.x] = static_cast<float>(sum);
+}
+
+template <class E>
+__device__ inline void scale(const E* from, E* to, int64_t count, float factor) {
+    constexpr int kEach = 16 / sizeof(E);
+    const int64_t whole = count / kEach;
+    for (int64_t i = threadIdx.x; i < whole; i += 256) {
+        union {
+            u4 words;
+            E elements[kEach];
+        } got;
+        got.words = reinterpret_cast<const Vector<E>*>(from)[i].words;
+#pragma unroll
+        for (int n = 0; n < kEach; ++n) got.elements[n] = from_float<E>(to_float(got.elements[n]) * factor);
+        reinterpret_cast<Vector<E>*>(to)[i].words = got.words;
+    }
+    const int64_t left = whole * kEach + threadIdx.x;
+    if (left < count) to[left] = from_float<E>(to_float(from[left]) * factor);
+}
+
+__global__ __launch_bounds__(256) void clip_kernel(ClipParams P) {
+    double sum = 0.0;
+    for (int i = threadIdx.x; i < P.n_partials; i += 256) sum += P.partial[i];
+    const float norm = static_cast<float>(sqrt(sum_block(sum)));
+    if (P.norm && blockIdx.x == 0 && threadIdx.x == 0) *P.norm = norm;
+    float factor = P.max_norm / (norm + P.eps);
+    factor = factor > 1.0f ? 1.0f : factor;  // (NaN stays)
+    for (int piece = P.pieces - 1 - static_cast<int>(blockIdx.x); piece >= 0; piece -= gridDim.x) {
+        const Tensor& t = P.tensor[tensor_of(P, piece)];
+        if (factor == 1.0f && t.from == t.to) continue;
+        const int64_t first = (piece - t.first_piece) * kPiece;
+        const int64_t count = t.count - first < kPiece ? t.count - first : kPiece;
+        if (t.dtype == NAVI_POLICY_F32)
+            scale(static_cast<const float*>(t.from) + first, static_cast<float*>(t.to) + first, count, factor);
+        else if (t.dtype == NAVI_POLICY_BF16)
+            scale(static_cast<const bf16*>(t.from) + first, static_cast<bf16*>(t.to) + first, count, factor);
+        else
+            scale(static_cast<const f16*>(t.from) + first, static_cast<f16*>(t.to) + first, count, factor);
+    }
+}
+
+int launched() {
+    const hipError_t err = hipGetLastError();
+    if (err != hipSuccess)
+        return set_error(NAVI_POLICY_E_LAUNCH, "navi_clip_grad_norm: kernel launch failed: %s", hipGetErrorString(err));
+    return NAVI_POLICY_OK;
+}
+
+// Fills in tensors from `at` on; returns where the next launch goes on.
+int fill(ClipParams& P, int at, int n, const void* const* from, void* const* to, const int64_t* counts, const int32_t* dtypes) {
+    P.n_tensors = P.pieces = 0;
+    for (; at < n && P.n_tensors < kTensors; ++at) {
+        if (counts[at] == 0) continue;
+        const int64_t pieces = (counts[at] + kPiece - 1) / kPiece;
+        if (P.n_tensors > 0 && P.pieces + pieces > INT32_MAX / 2) break;
+        P.tensor[P.n_tensors++] = Tensor{from[at], to[at], counts[at], P.pieces, dtypes[at]};
+        P.pieces += static_cast<int32_t>(pieces);
+    }
+    return at;
+}
+
+}  // namespace
+}  // namespace navi_policy
+
+extern "C" int navi_clip_grad_norm(int32_t n_tensors, const void* const* from, void* const* to, const int64_t* counts,
+                                   const int32_t* dtypes, float max_norm, float eps, float* norm, float* partial,
+                                   void* stream) {
+    using namespace navi_policy;
+    if (n_tensors < 0 || (n_tensors > 0 && (!from || !to || !counts || !dtypes)))
+        return set_error(NAVI_POLICY_E_ARG, "from, to, counts and dtypes must be non-null");
+    if (!norm || !partial) return set_error(NAVI_POLICY_E_ARG, "norm and partial must be non-null");
+    if (!(max_norm >= 0.0f) || !(eps >= 0.0f)) return set_error(NAVI_POLICY_E_ARG, "max_norm and eps must not be negative");
+    for (int i = 0; i < n_tensors; ++i) {
+        if (counts[i] < 0 || counts[i] > (INT32_MAX / 2) * kPiece)
+            return set_error(NAVI_POLICY_E_ARG, "tensor %d has an invalid count", i);
+        if (counts[i] > 0 && (!from[i] || !to[i])) return set_error(NAVI_POLICY_E_ARG, "tensor %d is null", i);
+        if (dtypes[i] < NAVI_POLICY_F32 || dtypes[i] > NAVI_POLICY_F16)
+            return set_error(NAVI_POLICY_E_ARG, "tensor %d must be float32, bfloat16 or float16", i);
+    }
+    ClipParams P{};
+    int launches = 0;
+    for (int at = 0; at < n_tensors; ++launches) at = fill(P, at, n_tensors, from, to, counts, dtypes);
+    if (launches > NAVI_POLICY_NORM_PARTIALS) return set_error(NAVI_POLICY_E_ARG, "too many tensors");
+    const int most = NAVI_POLICY_NORM_PARTIALS / std::max(1, launches);
+    int partials = 0;
+    for (int at = 0; at < n_tensors;) {
+        at = fill(P, at, n_tensors, from, to, counts, dtypes);
+        if (P.pieces == 0) continue;
+        const int blocks = std::min(P.pieces, most);
+        P.partial = partial + partials;
+        hipLaunchKernelGGL(square_sums_kernel, dim3(blocks), dim3(256), 0, as_stream(stream), P);
+        partials += blocks;
+    }
+    P.partial = partial;
+    P.n_partials = partials;
+    P.max_norm = max_norm;
+    P.eps = eps;
+    P.norm = norm;
+    if (launches <= 1) {  // what the first pass was given serves the second
+        hipLaunchKernelGGL(clip_kernel, dim3(std::max(1, std::min(P.pieces, 2048))), dim3(256), 0, as_stream(stream), P);
+        return launched();
+    }
+    for (int at = 0; at < n_tensors;) {
+        at = fill(P, at, n_tensors, from, to, counts, dtypes);
+        if (P.pieces == 0 && !P.norm) continue;
+        hipLaunchKernelGGL(clip_kernel, dim3(std::max(1, std::min(P.pieces, 2048))), dim3(256), 0, as_stream(stream), P);
+        P.norm = nullptr;
+    }
+    return launched();
+}

@@ -1,0 +1,133 @@
+// policy_common.hpp — element types, exact splits into bfloat16 planes and matrix-core
+// products shared by the policy's operators (libnavi_policy.so).
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "navi_policy.h"
+
+namespace navi_policy {
+
+int set_error(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
+
+using f4 = float __attribute__((ext_vector_type(4)));
+using u2 = uint32_t __attribute__((ext_vector_type(2)));
+using u4 = uint32_t __attribute__((ext_vector_type(4)));
+using bf16x8 = __bf16 __attribute__((ext_vector_type(8)));
+using s4 = short __attribute__((ext_vector_type(4)));
+
+struct bf16 {
+    uint16_t bits;
+};
+struct f16 {
+    _Float16 value;
+};
+
+__device__ inline uint32_t bits_of(float x) { return __builtin_bit_cast(uint32_t, x); }
+__device__ inline float float_of(uint32_t x) { return __builtin_bit_cast(float, x); }
+
+__device__ inline float to_float(float x) { return x; }
+__device__ inline float to_float(bf16 x) { return float_of(static_cast<uint32_t>(x.bits) << 16); }
+__device__ inline float to_float(f16 x) { return static_cast<float>(x.value); }
+
+template <class E>
+__device__ inline E from_float(float x);
+template <>
+__device__ inline float from_float<float>(float x) {
+    return x;
+}
+template <>
+__device__ inline bf16 from_float<bf16>(float x) {  // to nearest even, NaN kept (v_cvt_pk_bf16_f32)
+    return bf16{__builtin_bit_cast(uint16_t, static_cast<__bf16>(x))};
+}
+template <>
+__device__ inline f16 from_float<f16>(float x) {
+    return f16{static_cast<_Float16>(x)};
+}
+
+// A float32 is the sum of three bfloat16 whose bits are its mantissa's in turn (8 each), a
+// float16's 11 bits fit two, so products of such planes on the matrix cores keep float32's
+// precision at a third to a sixth of the bfloat16 rate: five to two times float32's own.
+template <class E>
+inline constexpr int kPlanes = 3;
+template <>
+inline constexpr int kPlanes<bf16> = 1;
+template <>
+inline constexpr int kPlanes<f16> = 2;
+
+// Two floats' upper halves as two bfloat16 (a in the low half).
+__device__ inline uint32_t upper_halves(float a, float b) {
+    return __builtin_amdgcn_perm(bits_of(b), bits_of(a), 0x07060302u);
+}
+
+// The planes of two floats; with N = 3 their sum is exact (a normal float's).
+template <int N>
+__device__ inline void split_pair(float a, float b, uint32_t (&plane)[N]) {
+#pragma unroll
+    for (int p = 0; p < N; ++p) {
+        plane[p] = upper_halves(a, b);
+        if (p + 1 < N) {
+            a -= float_of(bits_of(a) & 0xffff0000u);
+            b -= float_of(bits_of(b) & 0xffff0000u);
+        }
+    }
+}
+
+// The wave's place in its workgroup, in a scalar register: matrix products run whatever the
+// execution mask says, so a branch around them has to be one that the wave takes or not.
+__device__ inline int wave_of_workgroup() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+
+// Eight floats of a lane as an operand of 16x16x32 products.
+template <int N>
+__device__ inline void split8(const float (&x)[8], u4 (&plane)[N]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        uint32_t p[N];
+        split_pair<N>(x[2 * j], x[2 * j + 1], p);
+#pragma unroll
+        for (int n = 0; n < N; ++n) plane[n][j] = p[n];
+    }
+}
+
+template <int N>
+__device__ inline void split8(f4 a, f4 b, u4 (&plane)[N]) {
+    const float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    split8<N>(x, plane);
+}
+
+// D += A B on the matrix cores, 16 x 32 by 32 x 16: lane l holds row (of A) or column (of B,
+// C and D) l % 16; of A and B the eight numbers at 8 (l / 16) of the contracted axis (in any
+// order that A and B share), of C and D rows 4 (l / 16) to 4 (l / 16) + 3.
+__device__ inline f4 mfma(u4 a, u4 b, f4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
+                                                   0, 0);
+}
+
+// The product of two sums of planes, smallest terms first; terms below 2^-24 are left out.
+template <int NA, int NB>
+__device__ inline f4 mma(const u4 (&a)[NA], const u4 (&b)[NB], f4 c) {
+#pragma unroll
+    for (int s = (NA + NB - 2 < 2 ? NA + NB - 2 : 2); s >= 0; --s)
+#pragma unroll
+        for (int i = 0; i < NA; ++i)
+            if (s - i >= 0 && s - i < NB) c = mfma(a[i], b[s - i], c);
+    return c;
+}
+
+// 16x16x4 in float32: A's lane holds row l % 16, B's column l % 16, at l / 16 of the four.
+__device__ inline f4 mfma_f32(float a, float b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+
+// Four 16-bit numbers of a 4 x 16 block's column for each of 16 lanes; lane i of the 16 gives
+// the address of row i / 4, columns 4 (i % 4) to 4 (i % 4) + 3.
+__device__ inline u2 read_transposed(const uint16_t* lds) {
+    using pointer = __attribute__((address_space(3))) s4*;
+    return __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((pointer)(lds)));
+}
+
+inline hipStream_t as_stream(void* stream) { return static_cast<hipStream_t>(stream); }
+
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+}  // namespace navi_policy
