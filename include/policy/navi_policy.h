@@ -31,6 +31,8 @@ extern "C" {
 #define NAVI_POLICY_MAX_NORM_DIM 1024
 /* Tokens that the chunked form takes at once: saved states lie this far apart. */
 #define NAVI_POLICY_CHUNK 64
+/* Floats that a chunk's matrices take in navi_delta_rule.matrices. */
+#define NAVI_POLICY_CHUNK_MATRICES 5248
 
 /*
  * The gated delta rule. Per env b and value head h (key head h / (value_heads / key_heads)),
@@ -66,9 +68,12 @@ typedef struct navi_delta_rule {
     void* out;
     float* final_state;         /* as initial_state, or NULL; may be initial_state itself in
                                    navi_delta_step */
-    /* what the backward pass reads again, or NULL both: */
+    float* matrices; /* [envs * value_heads][chunks][NAVI_POLICY_CHUNK_MATRICES], 16-byte aligned:
+                        written by navi_delta_forward, read again by the backward pass (not used by
+                        navi_delta_step); chunks = ceil(steps / NAVI_POLICY_CHUNK) */
+    /* what the backward pass reads as well, or NULL both: */
     float* states;  /* [envs * value_heads][chunks - 1][key_dim][value_dim] the state before each
-                       chunk but the first; chunks = ceil(steps / NAVI_POLICY_CHUNK) */
+                       chunk but the first */
     float* updates; /* [envs * value_heads][steps][value_dim]: u */
 } navi_delta_rule;
 

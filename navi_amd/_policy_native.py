@@ -17,7 +17,7 @@ NAVI_POLICY_OK = 0
 NAVI_POLICY_E_ARG = -1
 NAVI_POLICY_E_LAUNCH = -2
 F32, BF16, F16 = 0, 1, 2
-MAX_KEY_DIM, MAX_NORM_DIM, CHUNK = 128, 1024, 64
+MAX_KEY_DIM, MAX_NORM_DIM, CHUNK, CHUNK_MATRICES = 128, 1024, 64, 5248
 NORM_RMS, NORM_L2 = 0, 1
 NORM_PARTIALS = 2048
 
@@ -39,7 +39,7 @@ class DeltaRule(ctypes.Structure):
                 ("envs", _i64), ("steps", _i64), ("scale", _f32), ("q", _vp), ("k", _vp), ("v", _vp),
                 ("q_stride", _three), ("k_stride", _three), ("v_stride", _three), ("g", _vp), ("beta", _vp),
                 ("g_stride", _three), ("beta_stride", _three), ("starts", _vp), ("starts_stride", _two),
-                ("initial_state", _vp), ("out", _vp), ("final_state", _vp), ("states", _vp), ("updates", _vp)]
+                ("initial_state", _vp), ("out", _vp), ("final_state", _vp), ("matrices", _vp), ("states", _vp), ("updates", _vp)]
 
 
 class DeltaGradients(ctypes.Structure):

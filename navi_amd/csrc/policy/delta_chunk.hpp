@@ -18,6 +18,8 @@
 // may be large, to float32's precision.
 #pragma once
 
+#include <cstddef>
+
 #include "policy_common.hpp"
 
 namespace navi_policy {
@@ -44,7 +46,15 @@ struct RuleParams {
 // them: slot l has column l % 16, rows 4 (l / 16) to 4 (l / 16) + 3.
 __device__ constexpr int tile_of(int i, int j) { return i * (i + 1) / 2 + j; }
 
-using Triangle = uint16_t[kTiles][3][64][4];  // its three planes
+template <int N>
+using Triangle = uint16_t[kTiles][N][64][4];  // its planes
+
+// What delta_triangles_kernel leaves of a chunk for the kernels that walk the chunks.
+struct ChunkMatrices {
+    f4 x[kTiles][64], p[kTiles][64];
+    float e[kChunk], fb[kChunk];  // E, and F beta
+};
+static_assert(sizeof(ChunkMatrices) == 4 * NAVI_POLICY_CHUNK_MATRICES, "the header's size");
 
 struct ChunkGates {
     float hi[kChunk], lo[kChunk];  // G
@@ -57,11 +67,6 @@ struct ChunkRows {
     static constexpr int kPitch = KP + 8;
     uint16_t q[kPlanes<E>][kChunk][kPitch];
     uint16_t k[kPlanes<E>][kChunk][kPitch];
-};
-
-struct ChunkTriangles {
-    Triangle x, p;
-    float work[kChunk][kChunk + 4];  // A, then X
 };
 
 template <class E>
@@ -93,6 +98,7 @@ __device__ inline void load_rows(const RuleParams& P, ChunkRows<E, KP>& rows, in
                                  int tokens) {
     constexpr int kPieces = KP / 8;
     const int key_head = head / P.group;
+#pragma unroll 1
     for (int piece = threadIdx.x; piece < kChunk * kPieces; piece += blockDim.x) {
         const int t = piece / kPieces, c = piece % kPieces * 8;
         const int valid = t < tokens ? P.r.key_dim - c : 0;
@@ -185,11 +191,12 @@ __device__ inline void operand_columns(const uint16_t (&rows)[N][kChunk][kPitch]
 
 // A triangle's rows 16 i to 16 i + 15, columns 32 m to 32 m + 31 (32 m <= 16 i) as an operand
 // whose contracted axis is in the order of results;
-__device__ inline void operand_triangle(const Triangle& t, int i, int m, u4 (&x)[3]) {
+template <int N>
+__device__ inline void operand_triangle(const Triangle<N>& t, int i, int m, u4 (&x)[N]) {
     const int lane = threadIdx.x & 63, l = lane & 15;
     const int slot = (l & 3) * 16 + 4 * (lane >> 4) + (l >> 2);
 #pragma unroll
-    for (int n = 0; n < 3; ++n) {
+    for (int n = 0; n < N; ++n) {
         const u2 a = read_transposed(t[tile_of(i, 2 * m)][n][slot]);
         const u2 b = 2 * m + 1 <= i ? read_transposed(t[tile_of(i, 2 * m + 1)][n][slot]) : u2{0, 0};
         x[n] = u4{a.x, a.y, b.x, b.y};
@@ -197,23 +204,24 @@ __device__ inline void operand_triangle(const Triangle& t, int i, int m, u4 (&x)
 }
 
 // and of its transpose, rows 16 j on, columns 32 m on (16 j < 32 m + 32).
-__device__ inline void operand_transpose(const Triangle& t, int j, int m, u4 (&x)[3]) {
+template <int N>
+__device__ inline void operand_transpose(const Triangle<N>& t, int j, int m, u4 (&x)[N]) {
     const int lane = threadIdx.x & 63;
 #pragma unroll
-    for (int n = 0; n < 3; ++n) {
+    for (int n = 0; n < N; ++n) {
         const u2 a = 2 * m >= j ? *reinterpret_cast<const u2*>(t[tile_of(2 * m, j)][n][lane]) : u2{0, 0};
         const u2 b = *reinterpret_cast<const u2*>(t[tile_of(2 * m + 1, j)][n][lane]);
         x[n] = u4{a.x, a.y, b.x, b.y};
     }
 }
 
-__device__ inline void store_tile(Triangle& t, int tile, f4 x) {
-    const int lane = threadIdx.x & 63;
-    uint32_t a[3], b[3];
-    split_pair<3>(x[0], x[1], a);
-    split_pair<3>(x[2], x[3], b);
+template <int N>
+__device__ inline void store_slot(Triangle<N>& t, int tile, int slot, f4 x) {
+    uint32_t a[N], b[N];
+    split_pair<N>(x[0], x[1], a);
+    split_pair<N>(x[2], x[3], b);
 #pragma unroll
-    for (int n = 0; n < 3; ++n) *reinterpret_cast<u2*>(t[tile][n][lane]) = u2{a[n], b[n]};
+    for (int n = 0; n < N; ++n) *reinterpret_cast<u2*>(t[tile][n][slot]) = u2{a[n], b[n]};
 }
 
 __device__ constexpr int tile_row(int tile) { return tile < 1 ? 0 : tile < 3 ? 1 : tile < 6 ? 2 : 3; }
@@ -294,10 +302,11 @@ __device__ inline void invert_triangle(float (&a)[kChunk][kChunk + 4], int wave,
     __syncthreads();
 }
 
-// X and P of the chunk whose rows and gates are in LDS. All threads; ends with a barrier.
+// X and P of the chunk whose rows and gates are in LDS, by all threads of the workgroup.
 template <class E, int KP>
-__device__ inline void make_triangles(const ChunkRows<E, KP>& rows, const ChunkGates& gates, ChunkTriangles& tri,
-                                      float scale, int wave, int waves) {
+__device__ inline void make_triangles(const ChunkRows<E, KP>& rows, const ChunkGates& gates,
+                                      float (&work)[kChunk][kChunk + 4], ChunkMatrices& to, float scale, int wave,
+                                      int waves) {
     constexpr int N = kPlanes<E>;
     const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
     for (int tile = wave; tile < kTiles; tile += waves) {
@@ -320,21 +329,102 @@ __device__ inline void make_triangles(const ChunkRows<E, KP>& rows, const ChunkG
         for (int s = 0; s < 4; ++s) {
             const int row = 16 * i + 4 * g + s;
             const float d = row >= column ? decay(gates, row, hi, lo, episode) * beta : 0.0f;
-            tri.work[row][column] = row > column ? d * kk[s] : 0.0f;
+            work[row][column] = row > column ? d * kk[s] : 0.0f;
             p[s] = scale * d * qk[s];
         }
-        store_tile(tri.p, tile, p);
+        to.p[tile][lane] = p;
     }
     __syncthreads();
-    invert_triangle(tri.work, wave, waves);
+    invert_triangle(work, wave, waves);
     for (int tile = wave; tile < kTiles; tile += waves) {
         const int i = tile_row(tile), j = tile - tile_of(i, 0);
         f4 x;
 #pragma unroll
-        for (int s = 0; s < 4; ++s) x[s] = tri.work[16 * i + 4 * g + s][16 * j + col];
-        store_tile(tri.x, tile, x);
+        for (int s = 0; s < 4; ++s) x[s] = work[16 * i + 4 * g + s][16 * j + col];
+        to.x[tile][lane] = x;
     }
-    __syncthreads();
 }
+
+// A chunk's inputs on their way: read into registers while the chunk before it is computed,
+// put into LDS once that is done with it. (Rows that 16-byte loads cannot read come then.)
+template <class E, int KP, int kThreads>
+struct ChunkFetch {
+    static constexpr int kPieces = kChunk * KP / 8 / kThreads;                  // of rows of q, and of k
+    static constexpr int kSlots = (2 * kTiles * 64 + kThreads - 1) / kThreads;  // of X and P
+    static constexpr int kWords = sizeof(E) == 4 ? 2 : 1;
+    u4 q[kPieces][kWords], k[kPieces][kWords];
+    f4 slot[kSlots];
+    float gate;
+
+    __device__ void fetch(const RuleParams& P, const ChunkMatrices& from, int64_t env, int head, int64_t t0, int tokens) {
+        if (P.wide_qk) {
+            const int key_head = head / P.group;
+            fetch_rows(at<E>(P.r.q, P.r.q_stride, env, t0, key_head), static_cast<uint32_t>(P.r.q_stride[1]) * sizeof(E),
+                       P.r.key_dim, tokens, q);
+            fetch_rows(at<E>(P.r.k, P.r.k_stride, env, t0, key_head), static_cast<uint32_t>(P.r.k_stride[1]) * sizeof(E),
+                       P.r.key_dim, tokens, k);
+        }
+        const Buffer matrices = buffer_of(&from, sizeof from);
+#pragma unroll
+        for (int i = 0; i < kSlots; ++i)  // (P follows X, the gates P)
+            slot[i] = __builtin_bit_cast(f4, buffer_load16(matrices, 16 * (threadIdx.x + i * kThreads)));
+        gate = buffer_load<float>(matrices, threadIdx.x < 2 * kChunk ? offsetof(ChunkMatrices, e) + 4 * threadIdx.x : kOutside);
+    }
+
+    __device__ static void fetch_rows(const E* base, uint32_t row_bytes, int dim, int tokens, u4 (&to)[kPieces][kWords]) {
+        const Buffer rows = buffer_of(base, tokens > 0 ? (tokens - 1) * row_bytes + dim * sizeof(E) : 0);
+        constexpr int kAcross = KP / 8, kDown = kThreads / kAcross;  // pieces of a row; rows at once
+        const int t = threadIdx.x / kAcross, c = threadIdx.x % kAcross * 8;
+        const uint32_t lane = c < dim ? t * row_bytes + c * sizeof(E) : kOutside;
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i)
+#pragma unroll
+            for (int w = 0; w < kWords; ++w) to[i][w] = buffer_load16(rows, lane + i * kDown * row_bytes + 16 * w);
+    }
+
+    __device__ static void put_piece(uint16_t (&rows)[kPlanes<E>][kChunk][KP + 8], int t, int c, const u4 (&from)[kWords]) {
+        if constexpr (kPlanes<E> == 1) {
+            *reinterpret_cast<u4*>(&rows[0][t][c]) = from[0];
+        } else {
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if constexpr (kWords == 2)
+                    x[i] = float_of(from[i / 4][i % 4]);
+                else
+                    x[i] = to_float(__builtin_bit_cast(f16, static_cast<uint16_t>(from[0][i / 2] >> (16 * (i % 2)))));
+            }
+            u4 plane[kPlanes<E>];
+            split8(x, plane);
+#pragma unroll
+            for (int n = 0; n < kPlanes<E>; ++n) *reinterpret_cast<u4*>(&rows[n][t][c]) = plane[n];
+        }
+    }
+
+    template <int NP>
+    __device__ void put(const RuleParams& P, ChunkRows<E, KP>& rows, Triangle<3>& x, Triangle<NP>& p, float (&gates)[2][kChunk],
+                        int64_t env, int head, int64_t t0, int tokens) const {
+        if (P.wide_qk) {
+            constexpr int kAcross = KP / 8, kDown = kThreads / kAcross;
+            const int t = threadIdx.x / kAcross, c = threadIdx.x % kAcross * 8;
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) {
+                put_piece(rows.q, t + i * kDown, c, q[i]);
+                put_piece(rows.k, t + i * kDown, c, k[i]);
+            }
+        } else {
+            load_rows<E, KP>(P, rows, env, head, t0, tokens);
+        }
+#pragma unroll
+        for (int i = 0; i < kSlots; ++i) {
+            const int n = threadIdx.x + i * kThreads;
+            if (n < kTiles * 64)
+                store_slot<3>(x, n >> 6, n & 63, slot[i]);
+            else if (n < 2 * kTiles * 64)
+                store_slot<NP>(p, (n >> 6) - kTiles, n & 63, slot[i]);
+        }
+        if (threadIdx.x < 2 * kChunk) (&gates[0][0])[threadIdx.x] = gate;
+    }
+};
 
 }  // namespace navi_policy

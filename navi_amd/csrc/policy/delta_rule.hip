@@ -8,16 +8,55 @@
 namespace navi_policy {
 namespace {
 
-constexpr int kMaxWaves = 8;  // of 16 value columns each in a workgroup
+// A wave's 16 columns of an array of T in the layout of products: lane l has column l % 16 and
+// rows 4 (l / 16) + s of each tile of 16. A row's address is a scalar, the lane's part of it
+// one register for all rows and chunks.
+template <class T>
+struct Columns {
+    uint32_t row_bytes, lane, width;
 
-// One column of 16 tokens' tiles in the layout of products: row 4 (l / 16) + s of tile i.
-template <class E>
-__device__ inline f4 load_results(const E* base, int64_t step_stride, int row, int tokens, bool inside) {
-    f4 x;
+    // `stride` elements from row to row; `columns` from the wave's first to the array's last
+    __device__ Columns(int64_t stride, int columns) {
+        const int l = threadIdx.x & 63;
+        row_bytes = static_cast<uint32_t>(stride) * sizeof(T);
+        width = (columns < 0 ? 0 : columns < 16 ? columns : 16) * static_cast<uint32_t>(sizeof(T));
+        lane = (l & 15) < columns ? 4 * (l >> 4) * row_bytes + (l & 15) * sizeof(T) : kOutside;
+    }
+
+    __device__ Buffer rows(const T* base, int rows) const {
+        return buffer_of(base, rows > 0 ? (rows - 1) * row_bytes + width : 0);
+    }
+
+    // The lane's part, where the compiler does not see that it is the same for every chunk: it
+    // would keep the offset of every row in a register.
+    __device__ uint32_t fresh() const {
+        uint32_t x = lane;
+        asm volatile("" : "+v"(x));
+        return x;
+    }
+
+    template <int kTilesOfRows, class F>
+    __device__ void load(Buffer from, F to) const {
+        const uint32_t own = fresh();
 #pragma unroll
-    for (int s = 0; s < 4; ++s)
-        x[s] = inside && row + s < tokens ? to_float(base[(row + s) * step_stride]) : 0.0f;
-    return x;
+        for (int i = 0; i < kTilesOfRows; ++i)
+#pragma unroll
+            for (int s = 0; s < 4; ++s) to(i, s, buffer_load<T>(from, own + (16 * i + s) * row_bytes));
+    }
+
+    template <int kTilesOfRows, class F>
+    __device__ void store(Buffer to, F from) const {
+        const uint32_t own = fresh();
+#pragma unroll
+        for (int i = 0; i < kTilesOfRows; ++i)
+#pragma unroll
+            for (int s = 0; s < 4; ++s) buffer_store<T>(to, own + (16 * i + s) * row_bytes, from(i, s));
+    }
+};
+
+template <class E>
+__device__ inline f4 to_floats(const E (&x)[4]) {
+    return f4{to_float(x[0]), to_float(x[1]), to_float(x[2]), to_float(x[3])};
 }
 
 __device__ inline f4 four(const float (&x)[kChunk], int row) { return *reinterpret_cast<const f4*>(&x[row]); }
@@ -30,136 +69,173 @@ __device__ inline f4 gated(f4 x, f4 factor) {
     return y;
 }
 
+// Keeps the compiler from reading the operands of later products early: it would hold them
+// in more registers than there are.
+__device__ inline void stage() { __builtin_amdgcn_sched_barrier(0); }
+
+__device__ inline int tokens_of(const RuleParams& P, int chunk) {
+    const int64_t left = P.r.steps - static_cast<int64_t>(chunk) * kChunk;
+    return static_cast<int>(left < kChunk ? left : kChunk);
+}
+
+// The triangles and gates of every chunk, which need no state: a workgroup each.
 template <class E, int KP>
-struct ScanLds {
+struct TriangleLds {
     ChunkRows<E, KP> rows;
-    ChunkTriangles tri;
     ChunkGates gates;
+    float work[kChunk][kChunk + 4];
 };
 
+template <class E, int KP>
+__global__ __launch_bounds__(256) void delta_triangles_kernel(RuleParams P) {
+    extern __shared__ char lds_bytes[];
+    auto& lds = *reinterpret_cast<TriangleLds<E, KP>*>(lds_bytes);
+    const int wave = wave_of_workgroup();
+    const int64_t sequence = blockIdx.x / static_cast<uint32_t>(P.n_chunks);
+    const int chunk = static_cast<int>(blockIdx.x % static_cast<uint32_t>(P.n_chunks));
+    const int64_t env = sequence / P.r.value_heads, t0 = static_cast<int64_t>(chunk) * kChunk;
+    const int head = static_cast<int>(sequence % P.r.value_heads), tokens = tokens_of(P, chunk);
+    ChunkMatrices& to = reinterpret_cast<ChunkMatrices*>(P.r.matrices)[blockIdx.x];
+    load_rows<E, KP>(P, lds.rows, env, head, t0, tokens);
+    if (wave == 0) load_gates(P, lds.gates, env, head, t0, tokens);
+    __syncthreads();
+    if (threadIdx.x < kChunk) {
+        to.e[threadIdx.x] = lds.gates.e[threadIdx.x];
+        to.fb[threadIdx.x] = lds.gates.f[threadIdx.x] * lds.gates.beta[threadIdx.x];
+    }
+    make_triangles<E, KP>(lds.rows, lds.gates, lds.work, to, P.r.scale, wave, 4);
+}
+
+// What reaches the output alone is rounded with it: for 16-bit outputs, two planes (2^-16)
+// of S, P and u there are far below that rounding (2^-9 and 2^-12).
+template <class E>
+inline constexpr int kOutPlanes = sizeof(E) == 4 ? 3 : 2;
+
+template <class E, int KP, int NP>
+struct ScanLds {
+    ChunkRows<E, KP> rows;
+    Triangle<3> x;
+    Triangle<NP> p;
+    float gates[2][kChunk];  // E, F beta
+};
+
+template <int N>
+__device__ inline void first_planes(const u4 (&from)[3], u4 (&to)[N]) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) to[n] = from[n];
+}
+
+template <int KP>
+__device__ inline void load_state(const Columns<float>& at, const float* from, int K, f4 (&state)[KP / 16]) {
+    at.load<KP / 16>(at.rows(from, from ? K : 0), [&](int c, int s, float x) { state[c][s] = x; });
+}
+
+template <int KP>
+__device__ inline void store_state(const Columns<float>& at, float* to, int K, const f4 (&state)[KP / 16]) {
+    at.store<KP / 16>(at.rows(to, K), [&](int c, int s) { return state[c][s]; });
+}
+
 // A wave holds 16 columns of the state as results of products (KP / 16 tiles), a workgroup
-// blockDim / 64 such columns of one head; it walks the chunks with the state in registers.
+// kThreads / 64 such columns of one head; it walks the chunks with the state in registers.
 // The state is the second operand of S^T k without a move: its tiles hold the contracted axis
 // in the order of results, which the other operand is read in as well.
-template <class E, int KP>
-__global__ __launch_bounds__(64 * kMaxWaves) void delta_forward_kernel(RuleParams P) {
-    constexpr int N = kPlanes<E>;
+template <class E, int KP, int kThreads>
+__global__ __launch_bounds__(kThreads) void delta_forward_kernel(RuleParams P) {
+    constexpr int N = kPlanes<E>, NP = kOutPlanes<E>;
     extern __shared__ char lds_bytes[];
-    auto& lds = *reinterpret_cast<ScanLds<E, KP>*>(lds_bytes);
-    const int lane = threadIdx.x & 63, wave = wave_of_workgroup(), waves = blockDim.x >> 6;
-    const int col = lane & 15, g = lane >> 4;
+    auto& lds = *reinterpret_cast<ScanLds<E, KP, NP>*>(lds_bytes);
+    const int wave = wave_of_workgroup(), g = (threadIdx.x & 63) >> 4;
     const int64_t sequence = blockIdx.x;
     const int64_t env = sequence / P.r.value_heads;
     const int head = static_cast<int>(sequence % P.r.value_heads);
-    const int column = (blockIdx.y * waves + wave) * 16 + col;
-    const bool inside = column < P.r.value_dim;
+    const int first = (blockIdx.y * (kThreads / 64) + wave) * 16;
     const int K = P.r.key_dim, V = P.r.value_dim;
+    const bool working = first < V;
+    const ChunkMatrices* matrices = reinterpret_cast<const ChunkMatrices*>(P.r.matrices) + sequence * P.n_chunks;
+    const E* v = at<E>(P.r.v, P.r.v_stride, env, 0, head) + first;
+    const Columns<E> rows_v(P.r.v_stride[1], V - first), rows_out(static_cast<int64_t>(P.r.value_heads) * V, V - first);
+    const Columns<float> rows_state(V, V - first);
 
     f4 state[KP / 16];
-    const float* from = P.r.initial_state ? P.r.initial_state + sequence * K * V + column : nullptr;
-#pragma unroll
-    for (int c = 0; c < KP / 16; ++c)
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            const int row = 16 * c + 4 * g + s;
-            state[c][s] = from && inside && row < K ? from[static_cast<int64_t>(row) * V] : 0.0f;
-        }
+    const float* from = P.r.initial_state ? P.r.initial_state + sequence * K * V + first : nullptr;
+    load_state<KP>(rows_state, from, K, state);
 
+    ChunkFetch<E, KP, kThreads> next;
+    E v_next[4][4];
+    if (P.n_chunks > 0) {
+        next.fetch(P, matrices[0], env, head, 0, tokens_of(P, 0));
+        rows_v.template load<4>(rows_v.rows(v, tokens_of(P, 0)), [&](int i, int s, E x) { v_next[i][s] = x; });
+    }
     for (int chunk = 0; chunk < P.n_chunks; ++chunk) {
         const int64_t t0 = static_cast<int64_t>(chunk) * kChunk;
-        const int tokens = static_cast<int>(P.r.steps - t0 < kChunk ? P.r.steps - t0 : kChunk);
-        __syncthreads();
-        load_rows<E, KP>(P, lds.rows, env, head, t0, tokens);
-        if (wave == 0) load_gates(P, lds.gates, env, head, t0, tokens);
-        __syncthreads();
-        make_triangles<E, KP>(lds.rows, lds.gates, lds.tri, P.r.scale, wave, waves);
-
-        if (P.r.states && chunk > 0) {
-            float* to = P.r.states + (sequence * (P.n_chunks - 1) + chunk - 1) * K * V + column;
+        const int tokens = tokens_of(P, chunk);
+        if (chunk > 0) __syncthreads();
+        next.template put<NP>(P, lds.rows, lds.x, lds.p, lds.gates, env, head, t0, tokens);
+        f4 values[4];
 #pragma unroll
-            for (int c = 0; c < KP / 16; ++c)
-#pragma unroll
-                for (int s = 0; s < 4; ++s)
-                    if (inside && 16 * c + 4 * g + s < K) to[static_cast<int64_t>(16 * c + 4 * g + s) * V] = state[c][s];
+        for (int i = 0; i < 4; ++i) values[i] = to_floats(v_next[i]);
+        __syncthreads();
+        if (chunk + 1 < P.n_chunks) {
+            next.fetch(P, matrices[chunk + 1], env, head, t0 + kChunk, tokens_of(P, chunk + 1));
+            rows_v.template load<4>(rows_v.rows(v + (t0 + kChunk) * P.r.v_stride[1], tokens_of(P, chunk + 1)),
+                                    [&](int i, int s, E x) { v_next[i][s] = x; });
         }
+        if (!working) continue;
+        stage();
 
+        if (P.r.states && chunk > 0)
+            store_state<KP>(rows_state, P.r.states + (sequence * (P.n_chunks - 1) + chunk - 1) * K * V + first, K, state);
         f4 u[4], o[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) u[i] = o[i] = f4{0, 0, 0, 0};
         if (chunk > 0 || from) {
 #pragma unroll
             for (int m = 0; m < KP / 32; ++m) {
-                u4 b[3], a[N];
+                u4 b[3], b_out[NP], a[N];
                 split8(state[2 * m], state[2 * m + 1], b);
+                first_planes(b, b_out);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     operand_rows_as_results(lds.rows.k, 16 * i, m, a);
                     u[i] = mma(a, b, u[i]);
                     operand_rows_as_results(lds.rows.q, 16 * i, m, a);
-                    o[i] = mma(a, b, o[i]);
+                    o[i] = mma(a, b_out, o[i]);
                 }
+                stage();
             }
         }
-        const E* v = at<E>(P.r.v, P.r.v_stride, env, t0, head) + column;
         u4 r[2][3];
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
             f4 x[2];
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
-                const int i = 2 * m + n, row = 16 * i + 4 * g;
-                const f4 e = four(lds.gates.e, row);
-                x[n] = load_results(v, P.r.v_stride[1], row, tokens, inside) - gated(u[i], e);
+                const int i = 2 * m + n;
+                const f4 e = four(lds.gates[0], 16 * i + 4 * g);
+                x[n] = values[i] - gated(u[i], e);
                 o[i] = P.r.scale * gated(o[i], e);
                 u[i] = f4{0, 0, 0, 0};
             }
             split8(x[0], x[1], r[m]);
         }
+        stage();
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int m = 0; m <= i / 2; ++m) {
                 u4 a[3];
-                operand_triangle(lds.tri.x, i, m, a);
+                operand_triangle<3>(lds.x, i, m, a);
                 u[i] = mma(a, r[m], u[i]);
+                stage();
             }
-        if (P.r.updates) {
-            float* to = P.r.updates + (sequence * P.r.steps + t0) * V + column;
+        if (P.r.updates)
+            rows_state.store<4>(rows_state.rows(P.r.updates + (sequence * P.r.steps + t0) * V + first, tokens),
+                                [&](int i, int s) { return u[i][s]; });
+        // The state first: the next chunk waits for it.
+        const float keep = lds.gates[0][kChunk - 1];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int s = 0; s < 4; ++s)
-                    if (inside && 16 * i + 4 * g + s < tokens)
-                        to[static_cast<int64_t>(16 * i + 4 * g + s) * V] = u[i][s];
-        }
-#pragma unroll
-        for (int m = 0; m < 2; ++m) split8(u[2 * m], u[2 * m + 1], r[m]);
-        E* out = static_cast<E*>(P.r.out) + ((env * P.r.steps + t0) * P.r.value_heads + head) * V + column;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-#pragma unroll
-            for (int m = 0; m <= i / 2; ++m) {
-                u4 a[3];
-                operand_triangle(lds.tri.p, i, m, a);
-                o[i] = mma(a, r[m], o[i]);
-            }
-#pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                const int t = 16 * i + 4 * g + s;
-                if (inside && t < tokens) out[static_cast<int64_t>(t) * P.r.value_heads * V] = from_float<E>(o[i][s]);
-            }
-        }
-        const float keep = lds.gates.e[kChunk - 1];
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-            f4 x[2];
-#pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                const int row = 16 * (2 * m + n) + 4 * g;
-                x[n] = u[2 * m + n] * four(lds.gates.f, row) * four(lds.gates.beta, row);
-            }
-            split8(x[0], x[1], r[m]);
-        }
+        for (int m = 0; m < 2; ++m)
+            split8(u[2 * m] * four(lds.gates[1], 32 * m + 4 * g), u[2 * m + 1] * four(lds.gates[1], 32 * m + 16 + 4 * g), r[m]);
 #pragma unroll
         for (int c = 0; c < KP / 16; ++c) {
             state[c] = gated(state[c], f4{keep, keep, keep, keep});
@@ -169,16 +245,26 @@ __global__ __launch_bounds__(64 * kMaxWaves) void delta_forward_kernel(RuleParam
                 operand_columns(lds.rows.k, c, m, a);
                 state[c] = mma(a, r[m], state[c]);
             }
+            if (c % 2) stage();
         }
-    }
-    if (P.r.final_state && inside) {
-        float* to = P.r.final_state + sequence * K * V + column;
+        u4 w[2][NP];
 #pragma unroll
-        for (int c = 0; c < KP / 16; ++c)
+        for (int m = 0; m < 2; ++m) split8(u[2 * m], u[2 * m + 1], w[m]);
 #pragma unroll
-            for (int s = 0; s < 4; ++s)
-                if (16 * c + 4 * g + s < K) to[static_cast<int64_t>(16 * c + 4 * g + s) * V] = state[c][s];
+        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+            for (int m = 0; m <= i / 2; ++m) {
+                u4 a[NP];
+                operand_triangle<NP>(lds.p, i, m, a);
+                o[i] = mma(a, w[m], o[i]);
+                stage();
+            }
+        }
+        rows_out.template store<4>(
+            rows_out.rows(static_cast<E*>(P.r.out) + ((env * P.r.steps + t0) * P.r.value_heads + head) * V + first, tokens),
+            [&](int i, int s) { return from_float<E>(o[i][s]); });
     }
+    if (P.r.final_state && working) store_state<KP>(rows_state, P.r.final_state + sequence * K * V + first, K, state);
 }
 
 // Backward through the chunks from the last to the first, the gradient dS of the state after
@@ -188,56 +274,58 @@ __global__ __launch_bounds__(64 * kMaxWaves) void delta_forward_kernel(RuleParam
 //     dS <- E_last dS + q^T (scale E do) - k^T (E dr)
 //
 // dS and dr go to memory for delta_gradients_kernel.
-template <class E, int KP>
-__global__ __launch_bounds__(64 * kMaxWaves) void delta_reverse_kernel(RuleParams P) {
+template <class E, int KP, int kThreads>
+__global__ __launch_bounds__(kThreads) void delta_reverse_kernel(RuleParams P) {
     constexpr int N = kPlanes<E>;
     extern __shared__ char lds_bytes[];
-    auto& lds = *reinterpret_cast<ScanLds<E, KP>*>(lds_bytes);
-    const int lane = threadIdx.x & 63, wave = wave_of_workgroup(), waves = blockDim.x >> 6;
-    const int col = lane & 15, g = lane >> 4;
+    auto& lds = *reinterpret_cast<ScanLds<E, KP, 3>*>(lds_bytes);
+    const int wave = wave_of_workgroup(), g = (threadIdx.x & 63) >> 4;
     const int64_t sequence = blockIdx.x;
     const int64_t env = sequence / P.r.value_heads;
     const int head = static_cast<int>(sequence % P.r.value_heads);
-    const int column = (blockIdx.y * waves + wave) * 16 + col;
-    const bool inside = column < P.r.value_dim;
+    const int first = (blockIdx.y * (kThreads / 64) + wave) * 16;
     const int K = P.r.key_dim, V = P.r.value_dim;
+    const bool working = first < V;
+    const ChunkMatrices* matrices = reinterpret_cast<const ChunkMatrices*>(P.r.matrices) + sequence * P.n_chunks;
+    const E* grad = at<E>(P.d.grad_out, P.d.grad_out_stride, env, 0, head) + first;
+    const Columns<E> rows_grad(P.d.grad_out_stride[1], V - first), rows_v(static_cast<int64_t>(P.r.value_heads) * V, V - first);
+    const Columns<float> rows_state(V, V - first);
 
     f4 dstate[KP / 16];
-    const float* from = P.d.grad_final_state ? P.d.grad_final_state + sequence * K * V + column : nullptr;
-#pragma unroll
-    for (int c = 0; c < KP / 16; ++c)
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            const int row = 16 * c + 4 * g + s;
-            dstate[c][s] = from && inside && row < K ? from[static_cast<int64_t>(row) * V] : 0.0f;
-        }
+    const float* from = P.d.grad_final_state ? P.d.grad_final_state + sequence * K * V + first : nullptr;
+    load_state<KP>(rows_state, from, K, dstate);
 
+    ChunkFetch<E, KP, kThreads> next;
+    E grad_next[4][4];
+    {
+        const int64_t t0 = (P.n_chunks - 1) * static_cast<int64_t>(kChunk);
+        next.fetch(P, matrices[P.n_chunks - 1], env, head, t0, tokens_of(P, P.n_chunks - 1));
+        rows_grad.template load<4>(rows_grad.rows(grad + t0 * P.d.grad_out_stride[1], tokens_of(P, P.n_chunks - 1)),
+                                   [&](int i, int s, E x) { grad_next[i][s] = x; });
+    }
     for (int chunk = P.n_chunks - 1; chunk >= 0; --chunk) {
         const int64_t t0 = static_cast<int64_t>(chunk) * kChunk;
-        const int tokens = static_cast<int>(P.r.steps - t0 < kChunk ? P.r.steps - t0 : kChunk);
-        __syncthreads();
-        load_rows<E, KP>(P, lds.rows, env, head, t0, tokens);
-        if (wave == 0) load_gates(P, lds.gates, env, head, t0, tokens);
-        __syncthreads();
-        make_triangles<E, KP>(lds.rows, lds.gates, lds.tri, P.r.scale, wave, waves);
-
+        const int tokens = tokens_of(P, chunk);
         const bool last = chunk + 1 == P.n_chunks;
-        if (!last) {
-            float* to = P.dstates + (sequence * (P.n_chunks - 1) + chunk) * K * V + column;
+        if (!last) __syncthreads();
+        next.template put<3>(P, lds.rows, lds.x, lds.p, lds.gates, env, head, t0, tokens);
+        f4 dO[4];
 #pragma unroll
-            for (int c = 0; c < KP / 16; ++c)
-#pragma unroll
-                for (int s = 0; s < 4; ++s)
-                    if (inside && 16 * c + 4 * g + s < K) to[static_cast<int64_t>(16 * c + 4 * g + s) * V] = dstate[c][s];
+        for (int i = 0; i < 4; ++i) dO[i] = to_floats(grad_next[i]);
+        __syncthreads();
+        if (chunk > 0) {
+            next.fetch(P, matrices[chunk - 1], env, head, t0 - kChunk, kChunk);
+            rows_grad.template load<4>(rows_grad.rows(grad + (t0 - kChunk) * P.d.grad_out_stride[1], kChunk),
+                                       [&](int i, int s, E x) { grad_next[i][s] = x; });
         }
+        if (!working) continue;
+        stage();
 
-        f4 du[4], dO[4];
-        const E* grad = at<E>(P.d.grad_out, P.d.grad_out_stride, env, t0, head) + column;
+        if (!last)
+            store_state<KP>(rows_state, P.dstates + (sequence * (P.n_chunks - 1) + chunk) * K * V + first, K, dstate);
+        f4 du[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            du[i] = f4{0, 0, 0, 0};
-            dO[i] = load_results(grad, P.d.grad_out_stride[1], 16 * i + 4 * g, tokens, inside);
-        }
+        for (int i = 0; i < 4; ++i) du[i] = f4{0, 0, 0, 0};
         if (!last || from) {
 #pragma unroll
             for (int m = 0; m < KP / 32; ++m) {
@@ -248,12 +336,11 @@ __global__ __launch_bounds__(64 * kMaxWaves) void delta_reverse_kernel(RuleParam
                     operand_rows_as_results(lds.rows.k, 16 * i, m, a);
                     du[i] = mma(a, b, du[i]);
                 }
+                stage();
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                du[i] = du[i] * four(lds.gates.f, 16 * i + 4 * g) * four(lds.gates.beta, 16 * i + 4 * g);
+            for (int i = 0; i < 4; ++i) du[i] = du[i] * four(lds.gates[1], 16 * i + 4 * g);
         }
-        u4 b[2][3];
         {
             u4 raw[2][N];
 #pragma unroll
@@ -263,37 +350,38 @@ __global__ __launch_bounds__(64 * kMaxWaves) void delta_reverse_kernel(RuleParam
 #pragma unroll
                 for (int m = j / 2; m < 2; ++m) {
                     u4 a[3];
-                    operand_transpose(lds.tri.p, j, m, a);
+                    operand_transpose<3>(lds.p, j, m, a);
                     du[j] = mma(a, raw[m], du[j]);
+                    stage();
                 }
         }
+        u4 b[2][3];
 #pragma unroll
         for (int m = 0; m < 2; ++m) split8(du[2 * m], du[2 * m + 1], b[m]);
-        E* dv = static_cast<E*>(P.d.d_v) + ((env * P.r.steps + t0) * P.r.value_heads + head) * V + column;
-        float* to = P.rgrads + (sequence * P.r.steps + t0) * V + column;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            f4 dr = {0, 0, 0, 0};
+            du[j] = f4{0, 0, 0, 0};
 #pragma unroll
             for (int m = j / 2; m < 2; ++m) {
                 u4 a[3];
-                operand_transpose(lds.tri.x, j, m, a);
-                dr = mma(a, b[m], dr);
+                operand_transpose<3>(lds.x, j, m, a);
+                du[j] = mma(a, b[m], du[j]);  // dr
+                stage();
             }
+        }
+        rows_v.template store<4>(
+            rows_v.rows(static_cast<E*>(P.d.d_v) + ((env * P.r.steps + t0) * P.r.value_heads + head) * V + first, tokens),
+            [&](int j, int s) { return from_float<E>(du[j][s]); });
+        rows_state.store<4>(rows_state.rows(P.rgrads + (sequence * P.r.steps + t0) * V + first, tokens),
+                            [&](int j, int s) { return du[j][s]; });
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                const int t = 16 * j + 4 * g + s;
-                if (inside && t < tokens) {
-                    dv[static_cast<int64_t>(t) * P.r.value_heads * V] = from_float<E>(dr[s]);
-                    to[static_cast<int64_t>(t) * V] = dr[s];
-                }
-            }
-            const f4 e = four(lds.gates.e, 16 * j + 4 * g);
-            du[j] = -e * dr;
+        for (int j = 0; j < 4; ++j) {
+            const f4 e = four(lds.gates[0], 16 * j + 4 * g);
+            du[j] = -e * du[j];
             dO[j] = P.r.scale * e * dO[j];
         }
         if (chunk > 0 || P.d.d_initial_state) {
-            const float keep = lds.gates.e[kChunk - 1];
+            const float keep = lds.gates[0][kChunk - 1];
             u4 c3[2][3];
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
@@ -311,17 +399,12 @@ __global__ __launch_bounds__(64 * kMaxWaves) void delta_reverse_kernel(RuleParam
                     operand_columns(lds.rows.q, c, m, a);
                     dstate[c] = mma(a, c3[m], dstate[c]);
                 }
+                stage();
             }
         }
     }
-    if (P.d.d_initial_state && inside) {
-        float* to = P.d.d_initial_state + sequence * K * V + column;
-#pragma unroll
-        for (int c = 0; c < KP / 16; ++c)
-#pragma unroll
-            for (int s = 0; s < 4; ++s)
-                if (16 * c + 4 * g + s < K) to[static_cast<int64_t>(16 * c + 4 * g + s) * V] = dstate[c][s];
-    }
+    if (P.d.d_initial_state && working)
+        store_state<KP>(rows_state, P.d.d_initial_state + sequence * K * V + first, K, dstate);
 }
 
 // The gradients of one chunk of one head, all chunks at once, from the states S before and
@@ -346,7 +429,7 @@ struct GradientLds {
         } stage;
         ChunkRows<E, KP> rows;
     };
-    Triangle n, m;
+    Triangle<3> n, m;
     ChunkGates gates;
     float beta_part[4][kChunk], g_part[4][kChunk], beta_row[kChunk], g_row[kChunk], f_row[kChunk];
     float dot_part[4];
@@ -507,8 +590,8 @@ __global__ __launch_bounds__(256) void delta_gradients_kernel(RuleParams P) {
                 g_sum += pair;
                 row_sum[s] += pair;
             }
-            store_tile(lds.n, tile_of(wave, j), n);
-            store_tile(lds.m, tile_of(wave, j), mm);
+            store_slot<3>(lds.n, tile_of(wave, j), lane, n);
+            store_slot<3>(lds.m, tile_of(wave, j), lane, mm);
         }
 #pragma unroll
         for (int d = 16; d < 64; d *= 2) {
@@ -586,16 +669,16 @@ __global__ __launch_bounds__(256) void delta_gradients_kernel(RuleParams P) {
             u4 a[3], b[N];
             operand_columns(lds.rows.k, c, m, b);
             if (2 * m <= wave) {
-                operand_triangle(lds.n, wave, m, a);
+                operand_triangle<3>(lds.n, wave, m, a);
                 dq = mma(a, b, dq);
-                operand_triangle(lds.m, wave, m, a);
+                operand_triangle<3>(lds.m, wave, m, a);
                 dk = mma(a, b, dk);
             }
             if (2 * m + 1 >= wave) {
-                operand_transpose(lds.m, wave, m, a);
+                operand_transpose<3>(lds.m, wave, m, a);
                 dk = mma(a, b, dk);
                 operand_columns(lds.rows.q, c, m, b);
-                operand_transpose(lds.n, wave, m, a);
+                operand_transpose<3>(lds.n, wave, m, a);
                 dk = mma(a, b, dk);
             }
         }
@@ -639,22 +722,39 @@ int launched(const char* what) {
     return NAVI_POLICY_OK;
 }
 
-// Waves of a workgroup: all of a head's columns up to 128, so that the triangles are made once.
-int waves_of(int value_dim) { return std::min(kMaxWaves, (value_dim + 15) / 16); }
+// Columns of a head that a workgroup takes: up to 64, or up to 128 where the head has more.
+int columns_of(int value_dim) { return value_dim <= 64 ? 64 : 128; }
+
+dim3 scan_grid(const RuleParams& P) {
+    const int columns = columns_of(P.r.value_dim);
+    return dim3(static_cast<unsigned>(P.r.envs * P.r.value_heads), (P.r.value_dim + columns - 1) / columns);
+}
 
 template <class E, int KP>
 int forward(const RuleParams& P, hipStream_t stream) {
-    const int waves = waves_of(P.r.value_dim);
-    const dim3 grid(static_cast<unsigned>(P.r.envs * P.r.value_heads), (P.r.value_dim + 16 * waves - 1) / (16 * waves));
-    hipLaunchKernelGGL((delta_forward_kernel<E, KP>), grid, dim3(64 * waves), sizeof(ScanLds<E, KP>), stream, P);
+    const dim3 grid = scan_grid(P);
+    if (P.n_chunks > 0) {
+        hipLaunchKernelGGL((delta_triangles_kernel<E, KP>), dim3(grid.x * static_cast<unsigned>(P.n_chunks)), dim3(256),
+                           sizeof(TriangleLds<E, KP>), stream, P);
+        const int code = launched("navi_delta_forward");
+        if (code != NAVI_POLICY_OK) return code;
+    }
+    constexpr size_t lds = sizeof(ScanLds<E, KP, kOutPlanes<E>>);
+    if (columns_of(P.r.value_dim) == 64)
+        hipLaunchKernelGGL((delta_forward_kernel<E, KP, 256>), grid, dim3(256), lds, stream, P);
+    else
+        hipLaunchKernelGGL((delta_forward_kernel<E, KP, 512>), grid, dim3(512), lds, stream, P);
     return launched("navi_delta_forward");
 }
 
 template <class E, int KP>
 int backward(const RuleParams& P, hipStream_t stream) {
-    const int waves = waves_of(P.r.value_dim);
-    const dim3 grid(static_cast<unsigned>(P.r.envs * P.r.value_heads), (P.r.value_dim + 16 * waves - 1) / (16 * waves));
-    hipLaunchKernelGGL((delta_reverse_kernel<E, KP>), grid, dim3(64 * waves), sizeof(ScanLds<E, KP>), stream, P);
+    const dim3 grid = scan_grid(P);
+    constexpr size_t lds = sizeof(ScanLds<E, KP, 3>);
+    if (columns_of(P.r.value_dim) == 64)
+        hipLaunchKernelGGL((delta_reverse_kernel<E, KP, 256>), grid, dim3(256), lds, stream, P);
+    else
+        hipLaunchKernelGGL((delta_reverse_kernel<E, KP, 512>), grid, dim3(512), lds, stream, P);
     int code = launched("navi_delta_backward");
     if (code != NAVI_POLICY_OK) return code;
     hipLaunchKernelGGL((delta_gradients_kernel<E, KP>), dim3(grid.x * static_cast<unsigned>(P.n_chunks)), dim3(256),
@@ -680,6 +780,13 @@ int run_typed(const RuleParams& P, bool back, hipStream_t stream) {
 }
 
 int64_t chunks_of(int64_t steps) { return (steps + kChunk - 1) / kChunk; }
+
+// Whether the rows of steps lie one after another, 64 of them within reach of a buffer access
+// (the bytes from one to the next times 64, and a row, stay below 2^31).
+constexpr int64_t kFarthest = INT32_MAX / kChunk - 65536 * 4;
+bool rows_apart(const int64_t (&stride)[3], int64_t bytes, int64_t dim) {
+    return stride[1] >= dim && stride[1] <= kFarthest / bytes;
+}
 
 bool wide_rows(const void* p, const int64_t (&stride)[3], int64_t bytes, int64_t dim) {
     return aligned16(p) && dim % 8 == 0 && stride[0] * bytes % 16 == 0 && stride[1] * bytes % 16 == 0 &&
@@ -716,7 +823,20 @@ int setup(const navi_delta_rule* r, RuleParams& P) {
     P.group = r->value_heads / r->key_heads;
     P.n_chunks = static_cast<int32_t>(chunks_of(r->steps));
     const int64_t bytes = r->dtype == NAVI_POLICY_F32 ? 4 : 2;
-    P.wide_qk = wide_rows(r->q, r->q_stride, bytes, r->key_dim) && wide_rows(r->k, r->k_stride, bytes, r->key_dim);
+    if (r->envs * r->value_heads * chunks_of(r->steps) > INT32_MAX)
+        return set_error(NAVI_POLICY_E_ARG, "envs * value_heads * chunks must be below 2^31");
+    if (P.n_chunks > 0 && (!r->matrices || !aligned16(r->matrices)))
+        return set_error(NAVI_POLICY_E_ARG, "matrices must be non-null and 16-byte aligned");
+    if (r->value_heads > kFarthest / 4 / r->value_dim)
+        return set_error(NAVI_POLICY_E_ARG, "value_heads * value_dim is too large");
+    if (r->steps == 1) {  // (the stride of an axis of one may be anything)
+        P.r.q_stride[1] = P.r.k_stride[1] = r->key_dim;
+        P.r.v_stride[1] = r->value_dim;
+    }
+    if (!(rows_apart(P.r.q_stride, bytes, r->key_dim) && rows_apart(P.r.k_stride, bytes, r->key_dim) &&
+          rows_apart(P.r.v_stride, bytes, r->value_dim)) && r->steps > 0)
+        return set_error(NAVI_POLICY_E_ARG, "the steps of q, k and v overlap or lie too far apart");
+    P.wide_qk = wide_rows(r->q, P.r.q_stride, bytes, r->key_dim) && wide_rows(r->k, P.r.k_stride, bytes, r->key_dim);
     return NAVI_POLICY_OK;
 }
 
@@ -759,8 +879,6 @@ extern "C" int navi_delta_backward(const navi_delta_rule* rule, const navi_delta
     if (!rule->updates || (P.n_chunks > 1 && !rule->states))
         return set_error(NAVI_POLICY_E_ARG, "the backward pass needs the forward pass's states and updates");
     const int64_t sequences = rule->envs * rule->value_heads;
-    if (sequences * P.n_chunks > INT32_MAX)
-        return set_error(NAVI_POLICY_E_ARG, "envs * value_heads * chunks must be below 2^31");
     if (!aligned16(P.d.workspace)) return set_error(NAVI_POLICY_E_ARG, "workspace must be 16-byte aligned");
     const auto rounded = [](int64_t n) { return (n + 3) / 4 * 4; };
     P.dstates = static_cast<float*>(P.d.workspace);
@@ -768,6 +886,9 @@ extern "C" int navi_delta_backward(const navi_delta_rule* rule, const navi_delta
     P.dq_heads = P.rgrads + rounded(sequences * rule->steps * rule->value_dim);
     P.dk_heads = P.dq_heads + rounded(P.group > 1 ? sequences * rule->steps * rule->key_dim : 0);
     const int64_t bytes = rule->dtype == NAVI_POLICY_F32 ? 4 : 2;
+    if (rule->steps == 1) P.d.grad_out_stride[1] = rule->value_dim;
+    if (!rows_apart(P.d.grad_out_stride, bytes, rule->value_dim))
+        return set_error(NAVI_POLICY_E_ARG, "the steps of grad_out overlap or lie too far apart");
     P.wide_do = wide_rows(P.d.grad_out, P.d.grad_out_stride, bytes, 8) && rule->value_dim % 8 == 0;
     P.wide_state = rule->value_dim % 4 == 0 && aligned16(rule->states) && aligned16(rule->updates) &&
                    aligned16(rule->initial_state) && aligned16(P.d.grad_final_state);

@@ -126,6 +126,37 @@ __device__ inline u2 read_transposed(const uint16_t* lds) {
     return __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((pointer)(lds)));
 }
 
+// Buffer accesses: a scalar base and size and a lane's 32-bit offset; loads from kOutside or
+// past the size give 0, stores there are dropped, so tails need no branches. The whole offset
+// is the lane's: a scalar part beyond the size would turn the range check around (it compares
+// the lane's part with the size less the scalar part, unsigned).
+using Buffer = __amdgpu_buffer_rsrc_t;
+constexpr uint32_t kOutside = 0x80000000u;  // (sizes and what is added to an offset are below 2^31)
+
+__device__ inline Buffer buffer_of(const void* base, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, static_cast<int>(bytes), 0x00020000);
+}
+
+template <class E>
+__device__ inline E buffer_load(Buffer from, uint32_t offset) {
+    if constexpr (sizeof(E) == 4)
+        return __builtin_bit_cast(E, __builtin_amdgcn_raw_buffer_load_b32(from, offset, 0, 0));
+    else
+        return __builtin_bit_cast(E, __builtin_amdgcn_raw_buffer_load_b16(from, offset, 0, 0));
+}
+
+template <class E>
+__device__ inline void buffer_store(Buffer to, uint32_t offset, E x) {
+    if constexpr (sizeof(E) == 4)
+        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, x), to, offset, 0, 0);
+    else
+        __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, x), to, offset, 0, 0);
+}
+
+__device__ inline u4 buffer_load16(Buffer from, uint32_t offset) {
+    return __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(from, offset, 0, 0));
+}
+
 inline hipStream_t as_stream(void* stream) { return static_cast<hipStream_t>(stream); }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }

@@ -97,6 +97,17 @@ def _check_state(name: str, state, q, v, envs: int) -> None:
     _check(state.is_contiguous(), f"{name} must be contiguous")
 
 
+_FARTHEST = ((1 << 31) - 1) // _native.CHUNK - (1 << 18)  # bytes between steps that the chunked kernels reach
+
+
+def _rows_apart(t: torch.Tensor) -> torch.Tensor:
+    """``t`` as the chunked kernels read it: steps that do not overlap (an expanded axis) and lie
+    within reach; else a copy."""
+    if t.size(1) <= 1 or t.size(3) <= t.stride(1) <= _FARTHEST // t.element_size():
+        return t
+    return t.contiguous()
+
+
 def _strides(t: torch.Tensor, step: bool) -> ctypes.Array:
     s = t.stride()
     return (ctypes.c_int64 * 3)(s[0], s[1], s[2]) if step else (ctypes.c_int64 * 3)(s[0], 0, s[1])
@@ -117,28 +128,29 @@ def _rule_args(q, k, v, g, beta, starts, scale, initial_state, out, final_state,
 
 
 def _forward(q, k, v, g, beta, starts, scale, initial_state, return_state, save):
-    """(out, final state or None, states, updates): the last two for a backward pass."""
+    """(out, final state or None, matrices, states, updates): the last three for a backward pass."""
     envs, steps, heads, dim = v.shape
     out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
     state = states = updates = None
     if return_state:
         state = torch.empty((envs, heads, q.size(-1), dim), dtype=torch.float32, device=v.device)
+    chunks = -(-steps // _native.CHUNK)
+    matrices = torch.empty((envs * heads, chunks, _native.CHUNK_MATRICES), dtype=torch.float32, device=v.device)
     if save:
-        chunks = -(-steps // _native.CHUNK)
         states = torch.empty((envs * heads, max(0, chunks - 1), q.size(-1), dim), dtype=torch.float32, device=v.device)
         updates = torch.empty((envs * heads, steps, dim), dtype=torch.float32, device=v.device)
     a = _rule_args(q, k, v, g, beta, starts, scale, initial_state, out, state)
-    a.states, a.updates = _ptr(states), _ptr(updates)
+    a.matrices, a.states, a.updates = matrices.data_ptr(), _ptr(states), _ptr(updates)
     with torch.cuda.device(q.device):
         _native.check(_native.lib().navi_delta_forward(ctypes.byref(a), _stream(q.device)))
-    return out, state, states, updates
+    return out, state, matrices, states, updates
 
 
 class _DeltaRule(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, g, beta, initial_state, starts, scale, return_state):
-        out, state, states, updates = _forward(q, k, v, g, beta, starts, scale, initial_state, return_state, True)
-        ctx.save_for_backward(q, k, v, g, beta, initial_state, starts, states, updates)
+        out, state, *saved = _forward(q, k, v, g, beta, starts, scale, initial_state, return_state, True)
+        ctx.save_for_backward(q, k, v, g, beta, initial_state, starts, *saved)
         ctx.scale = scale
         ctx.set_materialize_grads(False)
         return (out, state) if return_state else out
@@ -146,13 +158,14 @@ class _DeltaRule(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_out, grad_state=None):
-        q, k, v, g, beta, initial_state, starts, states, updates = ctx.saved_tensors
+        q, k, v, g, beta, initial_state, starts, matrices, states, updates = ctx.saved_tensors
         if grad_out is None and grad_state is None:
             return (None,) * 9
         if grad_out is None:
             grad_out = torch.zeros((), dtype=v.dtype, device=v.device).expand(v.shape)
         if not _dense_last(grad_out):  # (of a broadcast, for one)
             grad_out = grad_out.contiguous()
+        grad_out = _rows_apart(grad_out)
         if grad_state is not None:
             grad_state = grad_state.contiguous()
         d_q, d_k, d_v, d_g, d_beta = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v, g, beta))
@@ -162,7 +175,7 @@ class _DeltaRule(torch.autograd.Function):
                 d_state = torch.zeros_like(d_state) if grad_state is None else grad_state.clone()
             return d_q, d_k, d_v, d_g, d_beta, d_state, None, None, None
         a = _rule_args(q, k, v, g, beta, starts, ctx.scale, initial_state, grad_out, None)
-        a.states, a.updates = states.data_ptr(), updates.data_ptr()
+        a.matrices, a.states, a.updates = matrices.data_ptr(), states.data_ptr(), updates.data_ptr()
         lib = _native.lib()
         size = _native.check(lib.navi_delta_workspace(ctypes.byref(a)))
         workspace = torch.empty(size // 4, dtype=torch.float32, device=q.device)
@@ -200,9 +213,10 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     if initial_state is not None:
         _check_state("initial_state", initial_state, q, v, q.size(0))
     scale = q.size(-1) ** -0.5 if scale is None else float(scale)
+    q, k, v = (_rows_apart(t) for t in (q, k, v))
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, g, beta, initial_state)):
         return _DeltaRule.apply(q, k, v, g, beta, initial_state, starts, scale, bool(return_state))
-    out, state, _, _ = _forward(q, k, v, g, beta, starts, scale, initial_state, return_state, False)
+    out, state, *_ = _forward(q, k, v, g, beta, starts, scale, initial_state, return_state, False)
     return (out, state) if return_state else out
 
 

@@ -198,6 +198,22 @@ def test_one_gate_for_all_heads(policy):
     assert gate.grad.shape == gate.shape and torch.isfinite(gate.grad).all()
 
 
+def test_one_query_and_one_value_for_all_steps(policy):
+    """Expanded axes of steps, in a rollout that does not fill its last chunk."""
+    x, state, _ = make(2, 70, 1, 1, 64, 64, torch.bfloat16)
+    x = {n: t[:, :1].expand(t.shape) if n in "qv" else t for n, t in x.items()}
+    leaves = [t.detach().requires_grad_() for t in x.values()]
+    s0 = state.clone().requires_grad_()
+    o = policy.gated_delta_rule(*leaves, initial_state=s0)
+    whole = [t.contiguous().requires_grad_() for t in x.values()]
+    s1 = state.clone().requires_grad_()
+    want = policy.gated_delta_rule(*whole, initial_state=s1)
+    assert torch.equal(o, want)
+    for a, b in zip(torch.autograd.grad(o.float().sum(), leaves + [s0]),
+                    torch.autograd.grad(want, whole + [s1], torch.ones_like(want))):
+        assert torch.equal(a, b)
+
+
 def test_far_offsets(policy):
     """Environments that lie more than 2^32 bytes apart."""
     x, _, starts = make(2, 66, 1, 1, 64, 64, torch.bfloat16)

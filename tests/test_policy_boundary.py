@@ -40,8 +40,10 @@ def test_structures_match_the_header(tmp_path):
 
 def rule(**over):
     a = native.DeltaRule(dtype=native.F32, key_heads=2, value_heads=4, key_dim=16, value_dim=16, envs=2, steps=100, scale=1.0)
-    for name in ("q", "k", "v", "g", "beta", "out"):
+    for name in ("q", "k", "v", "g", "beta", "out", "matrices"):
         setattr(a, name, 4096)  # never read: every call here is refused before a launch
+    for name, dim in (("q", 16), ("k", 16), ("v", 16)):
+        setattr(a, name + "_stride", (ctypes.c_int64 * 3)(1 << 20, 4 * dim, dim))
     for name, value in over.items():
         setattr(a, name, value)
     return a
@@ -81,6 +83,17 @@ def test_rule_refusals_of_saved_arrays():
     d.workspace = 4100
     assert lib.navi_delta_backward(ctypes.byref(rule(states=4096, updates=4096)), ctypes.byref(d), None) < 0
     assert "16-byte aligned" in native.last_error()
+
+
+@pytest.mark.parametrize("name", ["q_stride", "v_stride"])
+@pytest.mark.parametrize("step", [0, 15, 1 << 23, -64])
+def test_steps_that_overlap_or_lie_far_apart_are_refused(name, step):
+    a = rule(**{name: (ctypes.c_int64 * 3)(1 << 30, step, 16)})
+    assert native.lib().navi_delta_forward(ctypes.byref(a), None) == native.NAVI_POLICY_E_ARG
+    assert "overlap or lie too far apart" in native.last_error()
+    wide = rule(value_heads=1 << 18, key_heads=1 << 18, value_dim=64, envs=1)
+    assert native.lib().navi_delta_forward(ctypes.byref(wide), None) == native.NAVI_POLICY_E_ARG
+    assert "value_heads * value_dim" in native.last_error()
 
 
 def test_workspace_sizes():
