@@ -302,45 +302,70 @@ __device__ inline void invert_triangle(float (&a)[kChunk][kChunk + 4], int wave,
     __syncthreads();
 }
 
-// X and P of the chunk whose rows and gates are in LDS, by all threads of the workgroup.
+// A chunk's rows, then (when no wave needs them) its triangle, in the same memory: more
+// workgroups of a CU hide each other's waits.
 template <class E, int KP>
-__device__ inline void make_triangles(const ChunkRows<E, KP>& rows, const ChunkGates& gates,
-                                      float (&work)[kChunk][kChunk + 4], ChunkMatrices& to, float scale, int wave,
-                                      int waves) {
-    constexpr int N = kPlanes<E>;
+struct TriangleLds {
+    union {
+        ChunkRows<E, KP> rows;
+        float work[kChunk][kChunk + 4];  // A, then X
+    };
+    ChunkGates gates;
+};
+
+// X and P of the chunk whose rows and gates are in LDS, by the four waves of a workgroup.
+template <class E, int KP>
+__device__ inline void make_triangles(TriangleLds<E, KP>& lds, ChunkMatrices& to, float scale, int wave) {
+    constexpr int N = kPlanes<E>, kEach = (kTiles + 3) / 4;
     const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
-    for (int tile = wave; tile < kTiles; tile += waves) {
+    f4 a[kEach];
+#pragma unroll
+    for (int n = 0; n < kEach; ++n) {
+        const int tile = wave + 4 * n;
+        if (tile >= kTiles) continue;
         const int i = tile_row(tile), j = tile - tile_of(i, 0);
         f4 kk = {0, 0, 0, 0}, qk = {0, 0, 0, 0};
 #pragma unroll
         for (int m = 0; m < KP / 32; ++m) {
             u4 ki[N], qi[N], kj[N];
-            operand_rows(rows.k, 16 * j, m, kj);
-            operand_rows(rows.k, 16 * i, m, ki);
+            operand_rows(lds.rows.k, 16 * j, m, kj);
+            operand_rows(lds.rows.k, 16 * i, m, ki);
             kk = mma(ki, kj, kk);
-            operand_rows(rows.q, 16 * i, m, qi);
+            operand_rows(lds.rows.q, 16 * i, m, qi);
             qk = mma(qi, kj, qk);
         }
         const int column = 16 * j + col;
-        const float hi = gates.hi[column], lo = gates.lo[column], beta = gates.beta[column];
-        const int episode = gates.episode[column];
+        const float hi = lds.gates.hi[column], lo = lds.gates.lo[column], beta = lds.gates.beta[column];
+        const int episode = lds.gates.episode[column];
         f4 p;
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
             const int row = 16 * i + 4 * g + s;
-            const float d = row >= column ? decay(gates, row, hi, lo, episode) * beta : 0.0f;
-            work[row][column] = row > column ? d * kk[s] : 0.0f;
+            const float d = row >= column ? decay(lds.gates, row, hi, lo, episode) * beta : 0.0f;
+            a[n][s] = row > column ? d * kk[s] : 0.0f;
             p[s] = scale * d * qk[s];
         }
         to.p[tile][lane] = p;
     }
     __syncthreads();
-    invert_triangle(work, wave, waves);
-    for (int tile = wave; tile < kTiles; tile += waves) {
+#pragma unroll
+    for (int n = 0; n < kEach; ++n) {
+        const int tile = wave + 4 * n;
+        if (tile >= kTiles) continue;
+        const int i = tile_row(tile), j = tile - tile_of(i, 0);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) lds.work[16 * i + 4 * g + s][16 * j + col] = a[n][s];
+    }
+    __syncthreads();
+    invert_triangle(lds.work, wave, 4);
+#pragma unroll
+    for (int n = 0; n < kEach; ++n) {
+        const int tile = wave + 4 * n;
+        if (tile >= kTiles) continue;
         const int i = tile_row(tile), j = tile - tile_of(i, 0);
         f4 x;
 #pragma unroll
-        for (int s = 0; s < 4; ++s) x[s] = work[16 * i + 4 * g + s][16 * j + col];
+        for (int s = 0; s < 4; ++s) x[s] = lds.work[16 * i + 4 * g + s][16 * j + col];
         to.x[tile][lane] = x;
     }
 }

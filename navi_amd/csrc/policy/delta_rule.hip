@@ -2,6 +2,7 @@
 // kernels of its backward pass (mathematics in delta_chunk.hpp).
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 #include "delta_chunk.hpp"
 
@@ -80,13 +81,6 @@ __device__ inline int tokens_of(const RuleParams& P, int chunk) {
 
 // The triangles and gates of every chunk, which need no state: a workgroup each.
 template <class E, int KP>
-struct TriangleLds {
-    ChunkRows<E, KP> rows;
-    ChunkGates gates;
-    float work[kChunk][kChunk + 4];
-};
-
-template <class E, int KP>
 __global__ __launch_bounds__(256) void delta_triangles_kernel(RuleParams P) {
     extern __shared__ char lds_bytes[];
     auto& lds = *reinterpret_cast<TriangleLds<E, KP>*>(lds_bytes);
@@ -103,7 +97,7 @@ __global__ __launch_bounds__(256) void delta_triangles_kernel(RuleParams P) {
         to.e[threadIdx.x] = lds.gates.e[threadIdx.x];
         to.fb[threadIdx.x] = lds.gates.f[threadIdx.x] * lds.gates.beta[threadIdx.x];
     }
-    make_triangles<E, KP>(lds.rows, lds.gates, lds.work, to, P.r.scale, wave, 4);
+    make_triangles<E, KP>(lds, to, P.r.scale, wave);
 }
 
 // What reaches the output alone is rounded with it: for 16-bit outputs, two planes (2^-16)
@@ -407,6 +401,16 @@ __global__ __launch_bounds__(kThreads) void delta_reverse_kernel(RuleParams P) {
         store_state<KP>(rows_state, P.d.d_initial_state + sequence * K * V + first, K, dstate);
 }
 
+// Sixteen rows of results, KP / 16 tiles across, into `rows` rows of `columns` numbers.
+template <class T, int KP>
+__device__ inline void store_tiles(T* base, int64_t stride, int rows, int columns, const f4 (&x)[KP / 16]) {
+#pragma unroll
+    for (int c = 0; c < KP / 16; ++c) {
+        const Columns<T> at(stride, columns - 16 * c);
+        at.template store<1>(at.rows(base + 16 * c, rows < 16 ? rows : 16), [&](int, int s) { return from_float<T>(x[c][s]); });
+    }
+}
+
 // The gradients of one chunk of one head, all chunks at once, from the states S before and
 // the state gradients dS after each, u and dr. With H = do u^T, R = dr u^T (lower triangles),
 // Y = do S^T, Z = dr S^T, W = u dS^T:
@@ -427,26 +431,77 @@ struct GradientLds {
             uint16_t s[KP / 16][3][64][8], ds[KP / 16][3][64][8];  // 32 columns of S and dS as operands
             uint16_t u[4][3][64][8];                                // and of u
         } stage;
-        ChunkRows<E, KP> rows;
+        struct {
+            ChunkRows<E, KP> rows;
+            Triangle<kOutPlanes<E>> n, m;  // (they reach dq and dk alone)
+        };
     };
-    Triangle<3> n, m;
     ChunkGates gates;
-    float beta_part[4][kChunk], g_part[4][kChunk], beta_row[kChunk], g_row[kChunk], f_row[kChunk];
+    float beta_part[16][kChunk], g_part[16][kChunk], beta_row[kChunk], g_row[kChunk], f_row[kChunk];
     float dot_part[4];
 };
 
-// Eight floats of a row of `valid` columns.
-__device__ inline void load_state8(const float* row, int valid, bool wide, float (&x)[8]) { load8(row, valid, wide, x); }
-
 __device__ inline float sum16(float x) {  // over 16 lanes in a row
-#pragma unroll
-    for (int d = 1; d < 16; d *= 2) x += __shfl_xor(x, d);
+    const auto moved = [](float y, auto control) {
+        return float_of(__builtin_amdgcn_mov_dpp(bits_of(y), decltype(control)::value, 0xf, 0xf, true));
+    };
+    x += moved(x, std::integral_constant<int, 0xb1>{});   // lanes 1, 0, 3, 2 of four
+    x += moved(x, std::integral_constant<int, 0x4e>{});   // 2, 3, 0, 1
+    x += moved(x, std::integral_constant<int, 0x141>{});  // the other four of eight
+    x += moved(x, std::integral_constant<int, 0x140>{});  // the other eight
     return x;
 }
 
+// Eight numbers of a row from `offset` bytes on: in 16-byte loads where rows are multiples of
+// eight, else one by one, those from `valid` on as zeros.
+template <class T>
+struct Eight {
+    static constexpr int kWords = sizeof(T) == 4 ? 2 : 1;
+    u4 words[kWords];
+
+    __device__ void load(Buffer from, uint32_t offset, int valid, bool wide) {
+        if (wide) {
+            const uint32_t lane = valid > 0 ? offset : kOutside;
+#pragma unroll
+            for (int w = 0; w < kWords; ++w) words[w] = buffer_load16(from, lane + 16 * w);
+            return;
+        }
+        uint32_t x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const T y = buffer_load<T>(from, i < valid ? offset + i * sizeof(T) : kOutside);
+            if constexpr (sizeof(T) == 4)
+                x[i] = bits_of(y);
+            else
+                x[i] = __builtin_bit_cast(uint16_t, y);
+        }
+#pragma unroll
+        for (int i = 0; i < 4 * kWords; ++i)
+            words[i / 4][i % 4] = kWords == 2 ? x[i] : x[2 * i % 8] | x[(2 * i + 1) % 8] << 16;
+    }
+
+    __device__ void floats(float (&x)[8]) const {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if constexpr (kWords == 2)
+                x[i] = float_of(words[i / 4][i % 4]);
+            else
+                x[i] = to_float(__builtin_bit_cast(T, static_cast<uint16_t>(words[0][i / 2] >> (16 * (i % 2)))));
+        }
+    }
+};
+
+// The inputs of 32 columns of V: of S, dS and u for the workgroup, of do and dr for the wave.
 template <class E, int KP>
-__global__ __launch_bounds__(256) void delta_gradients_kernel(RuleParams P) {
-    constexpr int N = kPlanes<E>;
+struct GradientFetch {
+    static constexpr int kPieces = KP / 64;
+    Eight<float> s[kPieces], ds[kPieces], u, dr;
+    Eight<E> grad;
+};
+
+template <class E, int KP>
+__global__ __launch_bounds__(256, KP == 64 ? 3 : 1) void delta_gradients_kernel(RuleParams P) {
+    constexpr int N = kPlanes<E>, NP = kOutPlanes<E>;
     extern __shared__ char lds_bytes[];
     auto& lds = *reinterpret_cast<GradientLds<E, KP>*>(lds_bytes);
     const int lane = threadIdx.x & 63, wave = wave_of_workgroup();
@@ -457,19 +512,39 @@ __global__ __launch_bounds__(256) void delta_gradients_kernel(RuleParams P) {
     const int head = static_cast<int>(sequence % P.r.value_heads);
     const int K = P.r.key_dim, V = P.r.value_dim;
     const int64_t t0 = static_cast<int64_t>(chunk) * kChunk;
-    const int tokens = static_cast<int>(P.r.steps - t0 < kChunk ? P.r.steps - t0 : kChunk);
+    const int tokens = tokens_of(P, chunk);
 
     const int64_t kv = static_cast<int64_t>(K) * V, inner = sequence * (P.n_chunks - 1);
     const float* S = chunk > 0 ? P.r.states + (inner + chunk - 1) * kv
                                : P.r.initial_state ? P.r.initial_state + sequence * kv : nullptr;
     const float* dS = chunk + 1 < P.n_chunks ? P.dstates + (inner + chunk) * kv
                                               : P.d.grad_final_state ? P.d.grad_final_state + sequence * kv : nullptr;
-    const float* u = P.r.updates + (sequence * P.r.steps + t0) * V;
-    const float* dr = P.rgrads + (sequence * P.r.steps + t0) * V;
+    const int64_t rows_at = (sequence * P.r.steps + t0) * V;
+    const uint32_t row_bytes = 4 * V, grad_row_bytes = static_cast<uint32_t>(P.d.grad_out_stride[1]) * sizeof(E);
+    const Buffer from_s = buffer_of(S, S ? K * row_bytes : 0), from_ds = buffer_of(dS, dS ? K * row_bytes : 0);
+    const Buffer from_u = buffer_of(P.r.updates + rows_at, tokens * row_bytes);
+    const Buffer from_dr = buffer_of(P.rgrads + rows_at, tokens * row_bytes);
+    const Buffer from_grad = buffer_of(at<E>(P.d.grad_out, P.d.grad_out_stride, env, t0, head),
+                                       (tokens - 1) * grad_row_bytes + V * sizeof(E));
+    const int piece_row = threadIdx.x >> 2, piece_column = (threadIdx.x & 3) * 8;
     const int my_token = 16 * wave + col;  // of the wave's tile of tokens, as an operand's row
-    const E* my_do = at<E>(P.d.grad_out, P.d.grad_out_stride, env, t0 + (my_token < tokens ? my_token : 0), head);
-    const float* my_dr = dr + static_cast<int64_t>(my_token < tokens ? my_token : 0) * V;
 
+    GradientFetch<E, KP> next;
+    const auto fetch = [&](int v0) {
+        const int c = v0 + piece_column;
+#pragma unroll
+        for (int i = 0; i < KP / 64; ++i) {
+            const uint32_t offset = (piece_row + 64 * i) * row_bytes + 4 * c;
+            const int valid = piece_row + 64 * i < K ? V - c : 0;
+            if (S) next.s[i].load(from_s, offset, valid, P.wide_state);
+            if (dS) next.ds[i].load(from_ds, offset, valid, P.wide_state);
+        }
+        next.u.load(from_u, piece_row * row_bytes + 4 * c, piece_row < tokens ? V - c : 0, P.wide_state);
+        const int valid = my_token < tokens ? V - v0 - 8 * g : 0;
+        next.dr.load(from_dr, my_token * row_bytes + 4 * (v0 + 8 * g), valid, P.wide_state);
+        next.grad.load(from_grad, my_token * grad_row_bytes + (v0 + 8 * g) * sizeof(E), valid, P.wide_do);
+    };
+    fetch(0);
     if (wave == 0) load_gates(P, lds.gates, env, head, t0, tokens);
     f4 y[KP / 16], z[KP / 16], w[KP / 16], h[4], rr[4];
 #pragma unroll
@@ -478,79 +553,75 @@ __global__ __launch_bounds__(256) void delta_gradients_kernel(RuleParams P) {
     for (int j = 0; j < 4; ++j) h[j] = rr[j] = f4{0, 0, 0, 0};
     float dot = 0.0f;
     for (int v0 = 0; v0 < V; v0 += 32) {
-        __syncthreads();
-        for (int piece = threadIdx.x; piece < 4 * KP; piece += 256) {
-            const int row = piece >> 2, c = (piece & 3) * 8;
-            const int valid = row < K ? V - v0 - c : 0;
-            const int64_t offset = static_cast<int64_t>(row < K ? row : 0) * V + v0 + c;
-            float a[8] = {}, b[8] = {};
-            if (S) load_state8(S + offset, valid, P.wide_state, a);
-            if (dS) load_state8(dS + offset, valid, P.wide_state, b);
-            u4 plane[3];
-            const int slot = (row & 15) + 16 * (piece & 3);
+        if (v0 > 0) __syncthreads();
+        float a[8], b[8];
+        u4 plane[3];
+#pragma unroll
+        for (int i = 0; i < KP / 64; ++i) {
+            const int tile = (piece_row >> 4) + 4 * i, slot = (piece_row & 15) + 16 * (threadIdx.x & 3);
             if (S) {
+                next.s[i].floats(a);
                 split8(a, plane);
 #pragma unroll
-                for (int n = 0; n < 3; ++n) *reinterpret_cast<u4*>(lds.stage.s[row >> 4][n][slot]) = plane[n];
+                for (int n = 0; n < 3; ++n) *reinterpret_cast<u4*>(lds.stage.s[tile][n][slot]) = plane[n];
             }
             if (dS) {
+                next.ds[i].floats(b);
                 split8(b, plane);
 #pragma unroll
-                for (int n = 0; n < 3; ++n) *reinterpret_cast<u4*>(lds.stage.ds[row >> 4][n][slot]) = plane[n];
+                for (int n = 0; n < 3; ++n) *reinterpret_cast<u4*>(lds.stage.ds[tile][n][slot]) = plane[n];
             }
+            if (S && dS)
 #pragma unroll
-            for (int n = 0; n < 8; ++n) dot += a[n] * b[n];
+                for (int n = 0; n < 8; ++n) dot += a[n] * b[n];
         }
-        {
-            const int row = threadIdx.x >> 2, c = (threadIdx.x & 3) * 8;
-            float a[8];
-            u4 plane[3];
-            load_state8(u + static_cast<int64_t>(row < tokens ? row : 0) * V + v0 + c, row < tokens ? V - v0 - c : 0,
-                        P.wide_state, a);
-            split8(a, plane);
+        next.u.floats(a);
+        split8(a, plane);
 #pragma unroll
-            for (int n = 0; n < 3; ++n)
-                *reinterpret_cast<u4*>(lds.stage.u[row >> 4][n][(row & 15) + 16 * (threadIdx.x & 3)]) = plane[n];
-        }
+        for (int n = 0; n < 3; ++n)
+            *reinterpret_cast<u4*>(lds.stage.u[piece_row >> 4][n][(piece_row & 15) + 16 * (threadIdx.x & 3)]) = plane[n];
         u4 a_do[N], a_dr[3], a_u[3];
-        {
-            float x[8];
-            const int valid = my_token < tokens ? V - v0 - 8 * g : 0;
-            load8(my_do + v0 + 8 * g, valid, P.wide_do, x);
-            split8(x, a_do);
-            load_state8(my_dr + v0 + 8 * g, valid, P.wide_state, x);
-            split8(x, a_dr);
-        }
+        next.grad.floats(a);
+        split8(a, a_do);
+        next.dr.floats(a);
+        split8(a, a_dr);
         __syncthreads();
+        if (v0 + 32 < V) fetch(v0 + 32);
+        stage();
+        if (dS) {
 #pragma unroll
-        for (int n = 0; n < 3; ++n) a_u[n] = *reinterpret_cast<const u4*>(lds.stage.u[wave][n][lane]);
+            for (int n = 0; n < 3; ++n) a_u[n] = *reinterpret_cast<const u4*>(lds.stage.u[wave][n][lane]);
+        }
 #pragma unroll
         for (int c = 0; c < KP / 16; ++c) {
-            u4 b[3];
+            u4 x[3];
             if (S) {
 #pragma unroll
-                for (int n = 0; n < 3; ++n) b[n] = *reinterpret_cast<const u4*>(lds.stage.s[c][n][lane]);
-                y[c] = mma(a_do, b, y[c]);
-                z[c] = mma(a_dr, b, z[c]);
+                for (int n = 0; n < 3; ++n) x[n] = *reinterpret_cast<const u4*>(lds.stage.s[c][n][lane]);
+                y[c] = mma(a_do, x, y[c]);
+                z[c] = mma(a_dr, x, z[c]);
             }
             if (dS) {
 #pragma unroll
-                for (int n = 0; n < 3; ++n) b[n] = *reinterpret_cast<const u4*>(lds.stage.ds[c][n][lane]);
-                w[c] = mma(a_u, b, w[c]);
+                for (int n = 0; n < 3; ++n) x[n] = *reinterpret_cast<const u4*>(lds.stage.ds[c][n][lane]);
+                w[c] = mma(a_u, x, w[c]);
             }
+            stage();
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             if (j > wave) continue;
-            u4 b[3];
+            u4 x[3];
 #pragma unroll
-            for (int n = 0; n < 3; ++n) b[n] = *reinterpret_cast<const u4*>(lds.stage.u[j][n][lane]);
-            h[j] = mma(a_do, b, h[j]);
-            rr[j] = mma(a_dr, b, rr[j]);
+            for (int n = 0; n < 3; ++n) x[n] = *reinterpret_cast<const u4*>(lds.stage.u[j][n][lane]);
+            h[j] = mma(a_do, x, h[j]);
+            rr[j] = mma(a_dr, x, rr[j]);
+            stage();
         }
     }
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) dot += __shfl_xor(dot, d);
+    dot = sum16(dot);
+    dot += __shfl_xor(dot, 16);
+    dot += __shfl_xor(dot, 32);
     if (lane == 0) lds.dot_part[wave] = dot;
     __syncthreads();
     load_rows<E, KP>(P, lds.rows, env, head, t0, tokens);
@@ -590,18 +661,11 @@ __global__ __launch_bounds__(256) void delta_gradients_kernel(RuleParams P) {
                 g_sum += pair;
                 row_sum[s] += pair;
             }
-            store_slot<3>(lds.n, tile_of(wave, j), lane, n);
-            store_slot<3>(lds.m, tile_of(wave, j), lane, mm);
+            store_slot<NP>(lds.n, tile_of(wave, j), lane, n);
+            store_slot<NP>(lds.m, tile_of(wave, j), lane, mm);
         }
-#pragma unroll
-        for (int d = 16; d < 64; d *= 2) {
-            beta_sum += __shfl_xor(beta_sum, d);
-            g_sum += __shfl_xor(g_sum, d);
-        }
-        if (g == 0) {
-            lds.beta_part[wave][16 * j + col] = beta_sum;
-            lds.g_part[wave][16 * j + col] = g_sum;
-        }
+        lds.beta_part[4 * wave + g][16 * j + col] = beta_sum;
+        lds.g_part[4 * wave + g][16 * j + col] = g_sum;
     }
     const f4 e = four(lds.gates.e, row), f = four(lds.gates.f, row), beta = four(lds.gates.beta, row);
     f4 qy = {0, 0, 0, 0}, kz = {0, 0, 0, 0}, kw = {0, 0, 0, 0};
@@ -621,6 +685,7 @@ __global__ __launch_bounds__(256) void delta_gradients_kernel(RuleParams P) {
             kz[s] += kx * z[c][s];
             kw[s] += kx * w[c][s];
         }
+        z[c] = beta * f * w[c] - z[c];  // dk's part
     }
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
@@ -635,12 +700,13 @@ __global__ __launch_bounds__(256) void delta_gradients_kernel(RuleParams P) {
     if (wave == 0) {
         float dbeta = lds.beta_row[lane], dG = lds.g_row[lane], f_all = lds.f_row[lane];
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
+        for (int n = 0; n < 16; ++n) {
             dbeta += lds.beta_part[n][lane];
             dG -= lds.g_part[n][lane];
         }
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) f_all += __shfl_xor(f_all, d);
+        f_all = sum16(f_all);
+        f_all += __shfl_xor(f_all, 16);
+        f_all += __shfl_xor(f_all, 32);
         if (lane == 63) {
             const float keep = lds.gates.e[63];
             dG += f_all;
@@ -660,42 +726,47 @@ __global__ __launch_bounds__(256) void delta_gradients_kernel(RuleParams P) {
         }
     }
 
-    // dq and dk, 16 columns of the key dimension at a time.
+    // dq (in y) and dk (in z).
 #pragma unroll
-    for (int c = 0; c < KP / 16; ++c) {
-        f4 dq = y[c], dk = beta * f * w[c] - z[c];
+    for (int m = 0; m < 2; ++m) {
+        const bool left = 2 * m <= wave, below = 2 * m + 1 >= wave;
+        u4 n_left[NP], m_left[NP], n_below[NP], m_below[NP];
+        if (left) {
+            operand_triangle<NP>(lds.n, wave, m, n_left);
+            operand_triangle<NP>(lds.m, wave, m, m_left);
+        }
+        if (below) {
+            operand_transpose<NP>(lds.n, wave, m, n_below);
+            operand_transpose<NP>(lds.m, wave, m, m_below);
+        }
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
-            u4 a[3], b[N];
+        for (int c = 0; c < KP / 16; ++c) {
+            u4 b[N];
             operand_columns(lds.rows.k, c, m, b);
-            if (2 * m <= wave) {
-                operand_triangle<3>(lds.n, wave, m, a);
-                dq = mma(a, b, dq);
-                operand_triangle<3>(lds.m, wave, m, a);
-                dk = mma(a, b, dk);
+            if (left) {
+                y[c] = mma(n_left, b, y[c]);
+                z[c] = mma(m_left, b, z[c]);
             }
-            if (2 * m + 1 >= wave) {
-                operand_transpose<3>(lds.m, wave, m, a);
-                dk = mma(a, b, dk);
+            if (below) {
+                z[c] = mma(m_below, b, z[c]);
                 operand_columns(lds.rows.q, c, m, b);
-                operand_transpose<3>(lds.n, wave, m, a);
-                dk = mma(a, b, dk);
+                z[c] = mma(n_below, b, z[c]);
             }
+            if (c % 2) stage();
         }
-        const int column = 16 * c + col;
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            if (row + s >= tokens || column >= K) continue;
-            if (P.group == 1) {
-                const int64_t to = ((env * P.r.steps + t0 + row + s) * P.r.key_heads + head) * K + column;
-                static_cast<E*>(P.d.d_q)[to] = from_float<E>(dq[s]);
-                static_cast<E*>(P.d.d_k)[to] = from_float<E>(dk[s]);
-            } else {
-                const int64_t to = ((env * P.r.steps + t0 + row + s) * P.r.value_heads + head) * K + column;
-                P.dq_heads[to] = dq[s];
-                P.dk_heads[to] = dk[s];
-            }
-        }
+    }
+    const int left = tokens - 16 * wave;  // rows of the wave's tile
+    if (left <= 0) return;
+    if (P.group == 1) {
+        const int64_t to = ((env * P.r.steps + t0 + 16 * wave) * P.r.key_heads + head) * K;
+        const int64_t stride = static_cast<int64_t>(P.r.key_heads) * K;
+        store_tiles<E, KP>(static_cast<E*>(P.d.d_q) + to, stride, left, K, y);
+        store_tiles<E, KP>(static_cast<E*>(P.d.d_k) + to, stride, left, K, z);
+    } else {
+        const int64_t to = ((env * P.r.steps + t0 + 16 * wave) * P.r.value_heads + head) * K;
+        const int64_t stride = static_cast<int64_t>(P.r.value_heads) * K;
+        store_tiles<float, KP>(P.dq_heads + to, stride, left, K, y);
+        store_tiles<float, KP>(P.dk_heads + to, stride, left, K, z);
     }
 }
 
@@ -827,8 +898,8 @@ int setup(const navi_delta_rule* r, RuleParams& P) {
         return set_error(NAVI_POLICY_E_ARG, "envs * value_heads * chunks must be below 2^31");
     if (P.n_chunks > 0 && (!r->matrices || !aligned16(r->matrices)))
         return set_error(NAVI_POLICY_E_ARG, "matrices must be non-null and 16-byte aligned");
-    if (r->value_heads > kFarthest / 4 / r->value_dim)
-        return set_error(NAVI_POLICY_E_ARG, "value_heads * value_dim is too large");
+    if (r->value_heads > kFarthest / 4 / std::max(r->value_dim, r->key_dim))
+        return set_error(NAVI_POLICY_E_ARG, "value_heads * value_dim or value_heads * key_dim is too large");
     if (r->steps == 1) {  // (the stride of an axis of one may be anything)
         P.r.q_stride[1] = P.r.k_stride[1] = r->key_dim;
         P.r.v_stride[1] = r->value_dim;
@@ -889,8 +960,10 @@ extern "C" int navi_delta_backward(const navi_delta_rule* rule, const navi_delta
     if (rule->steps == 1) P.d.grad_out_stride[1] = rule->value_dim;
     if (!rows_apart(P.d.grad_out_stride, bytes, rule->value_dim))
         return set_error(NAVI_POLICY_E_ARG, "the steps of grad_out overlap or lie too far apart");
-    P.wide_do = wide_rows(P.d.grad_out, P.d.grad_out_stride, bytes, 8) && rule->value_dim % 8 == 0;
-    P.wide_state = rule->value_dim % 4 == 0 && aligned16(rule->states) && aligned16(rule->updates) &&
-                   aligned16(rule->initial_state) && aligned16(P.d.grad_final_state);
+    // (16-byte buffer loads need addresses of whole 4-byte words)
+    P.wide_state = rule->value_dim % 8 == 0;
+    P.wide_do = P.wide_state && reinterpret_cast<uintptr_t>(P.d.grad_out) % 4 == 0 &&
+                P.d.grad_out_stride[0] * bytes % 4 == 0 && P.d.grad_out_stride[1] * bytes % 4 == 0 &&
+                P.d.grad_out_stride[2] * bytes % 4 == 0;
     return run_typed(P, true, as_stream(stream));
 }

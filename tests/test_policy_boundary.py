@@ -93,7 +93,7 @@ def test_steps_that_overlap_or_lie_far_apart_are_refused(name, step):
     assert "overlap or lie too far apart" in native.last_error()
     wide = rule(value_heads=1 << 18, key_heads=1 << 18, value_dim=64, envs=1)
     assert native.lib().navi_delta_forward(ctypes.byref(wide), None) == native.NAVI_POLICY_E_ARG
-    assert "value_heads * value_dim" in native.last_error()
+    assert "value_heads * value_dim or" in native.last_error()
 
 
 def test_workspace_sizes():
