@@ -45,9 +45,9 @@ extern "C" {
  * [value_dim] of it, g and beta: [envs][steps][value_heads] of float32, starts: [envs][steps]
  * of bytes (0 or not) or NULL. Strides are in elements, of the env, step and head axes; the
  * last axis is contiguous, and so are out and the states. g is meant to be <= 0; one of
- * -infinity (below -1e5) starts an episode as `starts` does. A state that an episode's
- * start clears may hold anything; other inputs are finite: a NaN or infinity among q, k, v
- * may reach every token of its chunk of 64 and head.
+ * -infinity (below -1e5) starts an episode as `starts` does. An initial state that a start at
+ * the first step clears may hold anything. Other inputs are finite: in the chunked form a NaN
+ * or infinity may reach every token of its chunk of 64 and what follows them.
  */
 typedef struct navi_delta_rule {
     int32_t dtype;              /* NAVI_POLICY_* of q, k, v, out and their gradients */
@@ -71,6 +71,8 @@ typedef struct navi_delta_rule {
     float* matrices; /* [envs * value_heads][chunks][NAVI_POLICY_CHUNK_MATRICES], 16-byte aligned:
                         written by navi_delta_forward, read again by the backward pass (not used by
                         navi_delta_step); chunks = ceil(steps / NAVI_POLICY_CHUNK) */
+    void* scratch;   /* navi_delta_scratch bytes for navi_delta_forward alone, 16-byte aligned (NULL where
+                        that is 0) */
     /* what the backward pass reads as well, or NULL both: */
     float* states;  /* [envs * value_heads][chunks - 1][key_dim][value_dim] the state before each
                        chunk but the first */
@@ -80,6 +82,10 @@ typedef struct navi_delta_rule {
 /* Chunked form: matrix products over chunks of 64 tokens, the states passed from one to the
  * next. For rollouts, and the forward pass of training. */
 int navi_delta_forward(const navi_delta_rule* rule, void* stream);
+
+/* Bytes of scratch that navi_delta_forward needs (0 but for long sequences of few heads);
+ * negative for invalid sizes. */
+int64_t navi_delta_scratch(const navi_delta_rule* rule);
 
 /* Recurrent form: one token after another with the state in registers; for single tokens
  * and short runs. final_state may be initial_state (updated in place). Saves nothing for a

@@ -39,7 +39,8 @@ class DeltaRule(ctypes.Structure):
                 ("envs", _i64), ("steps", _i64), ("scale", _f32), ("q", _vp), ("k", _vp), ("v", _vp),
                 ("q_stride", _three), ("k_stride", _three), ("v_stride", _three), ("g", _vp), ("beta", _vp),
                 ("g_stride", _three), ("beta_stride", _three), ("starts", _vp), ("starts_stride", _two),
-                ("initial_state", _vp), ("out", _vp), ("final_state", _vp), ("matrices", _vp), ("states", _vp), ("updates", _vp)]
+                ("initial_state", _vp), ("out", _vp), ("final_state", _vp), ("matrices", _vp), ("scratch", _vp),
+                ("states", _vp), ("updates", _vp)]
 
 
 class DeltaGradients(ctypes.Structure):
@@ -67,8 +68,9 @@ _lib.navi_policy_last_error.argtypes = []
 for _name in ("navi_delta_forward", "navi_delta_step"):
     getattr(_lib, _name).restype = ctypes.c_int
     getattr(_lib, _name).argtypes = [ctypes.POINTER(DeltaRule), _vp]
-_lib.navi_delta_workspace.restype = _i64
-_lib.navi_delta_workspace.argtypes = [ctypes.POINTER(DeltaRule)]
+for _name in ("navi_delta_scratch", "navi_delta_workspace"):
+    getattr(_lib, _name).restype = _i64
+    getattr(_lib, _name).argtypes = [ctypes.POINTER(DeltaRule)]
 _lib.navi_delta_backward.restype = ctypes.c_int
 _lib.navi_delta_backward.argtypes = [ctypes.POINTER(DeltaRule), ctypes.POINTER(DeltaGradients), _vp]
 for _name in ("navi_qk_norm", "navi_qk_norm_backward"):

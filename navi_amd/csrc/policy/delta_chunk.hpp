@@ -38,6 +38,10 @@ struct RuleParams {
     int32_t wide_state;   // rows of states and updates that 16-byte accesses can
     float* dstates;       // [env, head][chunks - 1][K][V] gradient of the state after each chunk but the last
     float* rgrads;        // [env, head][steps][V] gradient of r
+    // Long sequences of few heads are walked in segments of chunks (delta_join_kernel)
+    int32_t n_segments;
+    float* segment_states;    // [env, head][n_segments - 1][K][V]
+    float* segment_matrices;  // [env, head][n_segments - 1][K][K]
     float* dq_heads;      // [env][step][value head][K] where heads are shared
     float* dk_heads;
 };
@@ -372,20 +376,22 @@ __device__ inline void make_triangles(TriangleLds<E, KP>& lds, ChunkMatrices& to
 
 // A chunk's inputs on their way: read into registers while the chunk before it is computed,
 // put into LDS once that is done with it. (Rows that 16-byte loads cannot read come then.)
-template <class E, int KP, int kThreads>
+// Without kAll, keys and X alone: what the state needs of a chunk whose outputs nobody asks for.
+template <class E, int KP, int kThreads, bool kAll>
 struct ChunkFetch {
     static constexpr int kPieces = kChunk * KP / 8 / kThreads;                  // of rows of q, and of k
-    static constexpr int kSlots = (2 * kTiles * 64 + kThreads - 1) / kThreads;  // of X and P
+    static constexpr int kSlots = ((kAll ? 2 : 1) * kTiles * 64 + kThreads - 1) / kThreads;  // of X and P
     static constexpr int kWords = sizeof(E) == 4 ? 2 : 1;
-    u4 q[kPieces][kWords], k[kPieces][kWords];
+    u4 q[kAll ? kPieces : 1][kWords], k[kPieces][kWords];
     f4 slot[kSlots];
     float gate;
 
     __device__ void fetch(const RuleParams& P, const ChunkMatrices& from, int64_t env, int head, int64_t t0, int tokens) {
         if (P.wide_qk) {
             const int key_head = head / P.group;
-            fetch_rows(at<E>(P.r.q, P.r.q_stride, env, t0, key_head), static_cast<uint32_t>(P.r.q_stride[1]) * sizeof(E),
-                       P.r.key_dim, tokens, q);
+            if constexpr (kAll)
+                fetch_rows(at<E>(P.r.q, P.r.q_stride, env, t0, key_head), static_cast<uint32_t>(P.r.q_stride[1]) * sizeof(E),
+                           P.r.key_dim, tokens, q);
             fetch_rows(at<E>(P.r.k, P.r.k_stride, env, t0, key_head), static_cast<uint32_t>(P.r.k_stride[1]) * sizeof(E),
                        P.r.key_dim, tokens, k);
         }
@@ -434,7 +440,7 @@ struct ChunkFetch {
             const int t = threadIdx.x / kAcross, c = threadIdx.x % kAcross * 8;
 #pragma unroll
             for (int i = 0; i < kPieces; ++i) {
-                put_piece(rows.q, t + i * kDown, c, q[i]);
+                if constexpr (kAll) put_piece(rows.q, t + i * kDown, c, q[i]);
                 put_piece(rows.k, t + i * kDown, c, k[i]);
             }
         } else {
@@ -445,7 +451,7 @@ struct ChunkFetch {
             const int n = threadIdx.x + i * kThreads;
             if (n < kTiles * 64)
                 store_slot<3>(x, n >> 6, n & 63, slot[i]);
-            else if (n < 2 * kTiles * 64)
+            else if (kAll && n < 2 * kTiles * 64)
                 store_slot<NP>(p, (n >> 6) - kTiles, n & 63, slot[i]);
         }
         if (threadIdx.x < 2 * kChunk) (&gates[0][0])[threadIdx.x] = gate;

@@ -129,11 +129,117 @@ __device__ inline void store_state(const Columns<float>& at, float* to, int K, c
     at.store<KP / 16>(at.rows(to, K), [&](int c, int s) { return state[c][s]; });
 }
 
+// The chunks of a segment in the order that a kernel walks them, and the state before the
+// first: segment 0 begins with `given` (or zeros), the others with what delta_join_kernel
+// found. In summary, the columns past V (rounded up to 16) are those of the unit matrix, and
+// there are no inputs for them: the state after the segment is then the matrix that it
+// multiplies the state before it with.
+struct Walk {
+    int32_t begin, end;  // chunks, counted in the walk's order
+    const float* from;   // state before, or NULL for zeros
+    float* to;           // state after, or NULL
+    int32_t first;       // column of the wave's first
+    int32_t columns;     // that the array behind `from` and `to` has
+    bool working, unit;
+
+    template <bool kSummary>
+    __device__ static Walk of(const RuleParams& P, int64_t sequence, int first, const float* given, float* result) {
+        const int segment = blockIdx.z, V = P.r.value_dim, K = P.r.key_dim;
+        const int64_t slots = sequence * (P.n_segments - 1);
+        Walk w;
+        w.begin = static_cast<int>(static_cast<int64_t>(segment) * P.n_chunks / P.n_segments);
+        w.end = static_cast<int>((segment + 1ll) * P.n_chunks / P.n_segments);
+        w.first = first;
+        w.columns = V;
+        w.working = first < V;
+        w.unit = false;
+        const int64_t kv = static_cast<int64_t>(K) * V;
+        w.from = segment == 0 ? (given ? given + sequence * kv : nullptr)
+                              : kSummary ? nullptr : P.segment_states + (slots + segment - 1) * kv;
+        w.to = kSummary ? P.segment_states + (slots + segment) * kv
+                        : result && segment + 1 == P.n_segments ? result + sequence * kv : nullptr;
+        const int rounded = (V + 15) / 16 * 16;
+        if (kSummary && first >= rounded) {
+            w.unit = true;
+            w.first = first - rounded;
+            w.columns = K;
+            w.working = segment > 0 && w.first < K;
+            w.from = nullptr;
+            w.to = P.segment_matrices + (slots + segment) * K * K;
+        }
+        return w;
+    }
+
+    template <int KP>
+    __device__ void begin_state(const Columns<float>& at, int K, f4 (&state)[KP / 16]) const {
+        load_state<KP>(at, from ? from + first : nullptr, K, state);
+        if (unit) {
+            const int l = threadIdx.x & 63;
+#pragma unroll
+            for (int c = 0; c < KP / 16; ++c)
+#pragma unroll
+                for (int s = 0; s < 4; ++s)
+                    state[c][s] = 16 * c + 4 * (l >> 4) + s == first + (l & 15) ? 1.0f : 0.0f;
+        }
+    }
+};
+
+// u or its gradient from the rows of X, all tiles of a stage side by side.
+template <int N, int NB>
+__device__ inline void times_triangle(const Triangle<N>& t, const u4 (&b)[2][NB], f4 (&x)[4]) {
+    u4 a[4][N];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) operand_triangle<N>(t, i, 0, a[i]);
+    mma_each<4>(a, b[0], x);
+    stage();
+    u4 below[2][N];
+    f4 y[2] = {x[2], x[3]};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) operand_triangle<N>(t, 2 + i, 1, below[i]);
+    mma_each<2>(below, b[1], y);
+    x[2] = y[0];
+    x[3] = y[1];
+    stage();
+}
+
+template <int N, int NB>
+__device__ inline void times_transpose(const Triangle<N>& t, const u4 (&b)[2][NB], f4 (&x)[4]) {
+    u4 a[4][N];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) operand_transpose<N>(t, j, 1, a[j]);
+    mma_each<4>(a, b[1], x);
+    stage();
+    u4 left[2][N];
+    f4 y[2] = {x[0], x[1]};
+#pragma unroll
+    for (int j = 0; j < 2; ++j) operand_transpose<N>(t, j, 0, left[j]);
+    mma_each<2>(left, b[0], y);
+    x[0] = y[0];
+    x[1] = y[1];
+    stage();
+}
+
+// Columns of rows in LDS times b, added to four tiles of a state from tile c on.
+template <int N, int kPitch, int NB, int kCount>
+__device__ inline void add_columns(const uint16_t (&rows)[N][kChunk][kPitch], int c, const u4 (&b)[2][NB], f4 (&state)[kCount]) {
+    f4 x[4] = {state[c], state[c + 1], state[c + 2], state[c + 3]};
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+        u4 a[4][N];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) operand_columns(rows, c + n, m, a[n]);
+        mma_each<4>(a, b[m], x);
+        stage();
+    }
+#pragma unroll
+    for (int n = 0; n < 4; ++n) state[c + n] = x[n];
+}
+
 // A wave holds 16 columns of the state as results of products (KP / 16 tiles), a workgroup
 // kThreads / 64 such columns of one head; it walks the chunks with the state in registers.
 // The state is the second operand of S^T k without a move: its tiles hold the contracted axis
 // in the order of results, which the other operand is read in as well.
-template <class E, int KP, int kThreads>
+template <class E, int KP, int kThreads, bool kSummary>
 __global__ __launch_bounds__(kThreads) void delta_forward_kernel(RuleParams P) {
     constexpr int N = kPlanes<E>, NP = kOutPlanes<E>;
     extern __shared__ char lds_bytes[];
@@ -142,58 +248,60 @@ __global__ __launch_bounds__(kThreads) void delta_forward_kernel(RuleParams P) {
     const int64_t sequence = blockIdx.x;
     const int64_t env = sequence / P.r.value_heads;
     const int head = static_cast<int>(sequence % P.r.value_heads);
-    const int first = (blockIdx.y * (kThreads / 64) + wave) * 16;
     const int K = P.r.key_dim, V = P.r.value_dim;
-    const bool working = first < V;
+    const Walk walk = Walk::of<kSummary>(P, sequence, (blockIdx.y * (kThreads / 64) + wave) * 16, P.r.initial_state,
+                                         P.r.final_state);
+    const int first = walk.first;
     const ChunkMatrices* matrices = reinterpret_cast<const ChunkMatrices*>(P.r.matrices) + sequence * P.n_chunks;
     const E* v = at<E>(P.r.v, P.r.v_stride, env, 0, head) + first;
-    const Columns<E> rows_v(P.r.v_stride[1], V - first), rows_out(static_cast<int64_t>(P.r.value_heads) * V, V - first);
-    const Columns<float> rows_state(V, V - first);
+    const Columns<E> rows_v(P.r.v_stride[1], walk.unit ? 0 : V - first),
+        rows_out(static_cast<int64_t>(P.r.value_heads) * V, V - first);
+    const Columns<float> rows_state(walk.columns, walk.columns - first);
 
     f4 state[KP / 16];
-    const float* from = P.r.initial_state ? P.r.initial_state + sequence * K * V + first : nullptr;
-    load_state<KP>(rows_state, from, K, state);
+    walk.begin_state<KP>(rows_state, K, state);
 
-    ChunkFetch<E, KP, kThreads> next;
+    ChunkFetch<E, KP, kThreads, !kSummary> next;
     E v_next[4][4];
-    if (P.n_chunks > 0) {
-        next.fetch(P, matrices[0], env, head, 0, tokens_of(P, 0));
-        rows_v.template load<4>(rows_v.rows(v, tokens_of(P, 0)), [&](int i, int s, E x) { v_next[i][s] = x; });
-    }
-    for (int chunk = 0; chunk < P.n_chunks; ++chunk) {
+    const auto fetch = [&](int chunk) {
+        const int64_t t0 = static_cast<int64_t>(chunk) * kChunk;
+        next.fetch(P, matrices[chunk], env, head, t0, tokens_of(P, chunk));
+        rows_v.template load<4>(rows_v.rows(v + t0 * P.r.v_stride[1], tokens_of(P, chunk)),
+                                [&](int i, int s, E x) { v_next[i][s] = x; });
+    };
+    if (walk.begin < walk.end) fetch(walk.begin);
+    for (int chunk = walk.begin; chunk < walk.end; ++chunk) {
         const int64_t t0 = static_cast<int64_t>(chunk) * kChunk;
         const int tokens = tokens_of(P, chunk);
-        if (chunk > 0) __syncthreads();
+        if (chunk > walk.begin) __syncthreads();
         next.template put<NP>(P, lds.rows, lds.x, lds.p, lds.gates, env, head, t0, tokens);
         f4 values[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) values[i] = to_floats(v_next[i]);
         __syncthreads();
-        if (chunk + 1 < P.n_chunks) {
-            next.fetch(P, matrices[chunk + 1], env, head, t0 + kChunk, tokens_of(P, chunk + 1));
-            rows_v.template load<4>(rows_v.rows(v + (t0 + kChunk) * P.r.v_stride[1], tokens_of(P, chunk + 1)),
-                                    [&](int i, int s, E x) { v_next[i][s] = x; });
-        }
-        if (!working) continue;
+        if (chunk + 1 < walk.end) fetch(chunk + 1);
+        if (!walk.working) continue;
         stage();
 
-        if (P.r.states && chunk > 0)
+        if (!kSummary && P.r.states && chunk > 0)
             store_state<KP>(rows_state, P.r.states + (sequence * (P.n_chunks - 1) + chunk - 1) * K * V + first, K, state);
         f4 u[4], o[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) u[i] = o[i] = f4{0, 0, 0, 0};
-        if (chunk > 0 || from) {
+        if (chunk > walk.begin || walk.from || walk.unit) {
 #pragma unroll
             for (int m = 0; m < KP / 32; ++m) {
-                u4 b[3], b_out[NP], a[N];
+                u4 b[3], a[4][N];
                 split8(state[2 * m], state[2 * m + 1], b);
-                first_planes(b, b_out);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    operand_rows_as_results(lds.rows.k, 16 * i, m, a);
-                    u[i] = mma(a, b, u[i]);
-                    operand_rows_as_results(lds.rows.q, 16 * i, m, a);
-                    o[i] = mma(a, b_out, o[i]);
+                for (int i = 0; i < 4; ++i) operand_rows_as_results(lds.rows.k, 16 * i, m, a[i]);
+                mma_each<4>(a, b, u);
+                if constexpr (!kSummary) {
+                    u4 b_out[NP];
+                    first_planes(b, b_out);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) operand_rows_as_results(lds.rows.q, 16 * i, m, a[i]);
+                    mma_each<4>(a, b_out, o);
                 }
                 stage();
             }
@@ -213,16 +321,8 @@ __global__ __launch_bounds__(kThreads) void delta_forward_kernel(RuleParams P) {
             split8(x[0], x[1], r[m]);
         }
         stage();
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int m = 0; m <= i / 2; ++m) {
-                u4 a[3];
-                operand_triangle<3>(lds.x, i, m, a);
-                u[i] = mma(a, r[m], u[i]);
-                stage();
-            }
-        if (P.r.updates)
+        times_triangle<3>(lds.x, r, u);
+        if (!kSummary && P.r.updates)
             rows_state.store<4>(rows_state.rows(P.r.updates + (sequence * P.r.steps + t0) * V + first, tokens),
                                 [&](int i, int s) { return u[i][s]; });
         // The state first: the next chunk waits for it.
@@ -231,34 +331,20 @@ __global__ __launch_bounds__(kThreads) void delta_forward_kernel(RuleParams P) {
         for (int m = 0; m < 2; ++m)
             split8(u[2 * m] * four(lds.gates[1], 32 * m + 4 * g), u[2 * m + 1] * four(lds.gates[1], 32 * m + 16 + 4 * g), r[m]);
 #pragma unroll
-        for (int c = 0; c < KP / 16; ++c) {
-            state[c] = gated(state[c], f4{keep, keep, keep, keep});
+        for (int c = 0; c < KP / 16; ++c) state[c] = gated(state[c], f4{keep, keep, keep, keep});
 #pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                u4 a[N];
-                operand_columns(lds.rows.k, c, m, a);
-                state[c] = mma(a, r[m], state[c]);
-            }
-            if (c % 2) stage();
+        for (int c = 0; c < KP / 16; c += 4) add_columns(lds.rows.k, c, r, state);
+        if constexpr (!kSummary) {
+            u4 w[2][NP];
+#pragma unroll
+            for (int m = 0; m < 2; ++m) split8(u[2 * m], u[2 * m + 1], w[m]);
+            times_triangle<NP>(lds.p, w, o);
+            rows_out.template store<4>(
+                rows_out.rows(static_cast<E*>(P.r.out) + ((env * P.r.steps + t0) * P.r.value_heads + head) * V + first, tokens),
+                [&](int i, int s) { return from_float<E>(o[i][s]); });
         }
-        u4 w[2][NP];
-#pragma unroll
-        for (int m = 0; m < 2; ++m) split8(u[2 * m], u[2 * m + 1], w[m]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-#pragma unroll
-            for (int m = 0; m <= i / 2; ++m) {
-                u4 a[NP];
-                operand_triangle<NP>(lds.p, i, m, a);
-                o[i] = mma(a, w[m], o[i]);
-                stage();
-            }
-        }
-        rows_out.template store<4>(
-            rows_out.rows(static_cast<E*>(P.r.out) + ((env * P.r.steps + t0) * P.r.value_heads + head) * V + first, tokens),
-            [&](int i, int s) { return from_float<E>(o[i][s]); });
     }
-    if (P.r.final_state && working) store_state<KP>(rows_state, P.r.final_state + sequence * K * V + first, K, state);
+    if (walk.to && walk.working) store_state<KP>(rows_state, walk.to + first, K, state);
 }
 
 // Backward through the chunks from the last to the first, the gradient dS of the state after
@@ -268,7 +354,7 @@ __global__ __launch_bounds__(kThreads) void delta_forward_kernel(RuleParams P) {
 //     dS <- E_last dS + q^T (scale E do) - k^T (E dr)
 //
 // dS and dr go to memory for delta_gradients_kernel.
-template <class E, int KP, int kThreads>
+template <class E, int KP, int kThreads, bool kSummary>
 __global__ __launch_bounds__(kThreads) void delta_reverse_kernel(RuleParams P) {
     constexpr int N = kPlanes<E>;
     extern __shared__ char lds_bytes[];
@@ -277,59 +363,56 @@ __global__ __launch_bounds__(kThreads) void delta_reverse_kernel(RuleParams P) {
     const int64_t sequence = blockIdx.x;
     const int64_t env = sequence / P.r.value_heads;
     const int head = static_cast<int>(sequence % P.r.value_heads);
-    const int first = (blockIdx.y * (kThreads / 64) + wave) * 16;
     const int K = P.r.key_dim, V = P.r.value_dim;
-    const bool working = first < V;
+    const Walk walk = Walk::of<kSummary>(P, sequence, (blockIdx.y * (kThreads / 64) + wave) * 16, P.d.grad_final_state,
+                                         P.d.d_initial_state);
+    const int first = walk.first;
     const ChunkMatrices* matrices = reinterpret_cast<const ChunkMatrices*>(P.r.matrices) + sequence * P.n_chunks;
     const E* grad = at<E>(P.d.grad_out, P.d.grad_out_stride, env, 0, head) + first;
-    const Columns<E> rows_grad(P.d.grad_out_stride[1], V - first), rows_v(static_cast<int64_t>(P.r.value_heads) * V, V - first);
-    const Columns<float> rows_state(V, V - first);
+    const Columns<E> rows_grad(P.d.grad_out_stride[1], walk.unit ? 0 : V - first),
+        rows_v(static_cast<int64_t>(P.r.value_heads) * V, V - first);
+    const Columns<float> rows_state(walk.columns, walk.columns - first);
 
     f4 dstate[KP / 16];
-    const float* from = P.d.grad_final_state ? P.d.grad_final_state + sequence * K * V + first : nullptr;
-    load_state<KP>(rows_state, from, K, dstate);
+    walk.begin_state<KP>(rows_state, K, dstate);
 
-    ChunkFetch<E, KP, kThreads> next;
+    ChunkFetch<E, KP, kThreads, true> next;
     E grad_next[4][4];
-    {
-        const int64_t t0 = (P.n_chunks - 1) * static_cast<int64_t>(kChunk);
-        next.fetch(P, matrices[P.n_chunks - 1], env, head, t0, tokens_of(P, P.n_chunks - 1));
-        rows_grad.template load<4>(rows_grad.rows(grad + t0 * P.d.grad_out_stride[1], tokens_of(P, P.n_chunks - 1)),
+    const auto fetch = [&](int chunk) {
+        const int64_t t0 = static_cast<int64_t>(chunk) * kChunk;
+        next.fetch(P, matrices[chunk], env, head, t0, tokens_of(P, chunk));
+        rows_grad.template load<4>(rows_grad.rows(grad + t0 * P.d.grad_out_stride[1], tokens_of(P, chunk)),
                                    [&](int i, int s, E x) { grad_next[i][s] = x; });
-    }
-    for (int chunk = P.n_chunks - 1; chunk >= 0; --chunk) {
+    };
+    const int last = P.n_chunks - 1;
+    if (walk.begin < walk.end) fetch(last - walk.begin);
+    for (int step = walk.begin; step < walk.end; ++step) {
+        const int chunk = last - step;
         const int64_t t0 = static_cast<int64_t>(chunk) * kChunk;
         const int tokens = tokens_of(P, chunk);
-        const bool last = chunk + 1 == P.n_chunks;
-        if (!last) __syncthreads();
+        if (step > walk.begin) __syncthreads();
         next.template put<3>(P, lds.rows, lds.x, lds.p, lds.gates, env, head, t0, tokens);
         f4 dO[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) dO[i] = to_floats(grad_next[i]);
         __syncthreads();
-        if (chunk > 0) {
-            next.fetch(P, matrices[chunk - 1], env, head, t0 - kChunk, kChunk);
-            rows_grad.template load<4>(rows_grad.rows(grad + (t0 - kChunk) * P.d.grad_out_stride[1], kChunk),
-                                       [&](int i, int s, E x) { grad_next[i][s] = x; });
-        }
-        if (!working) continue;
+        if (step + 1 < walk.end) fetch(chunk - 1);
+        if (!walk.working) continue;
         stage();
 
-        if (!last)
+        if (!kSummary && step > 0)
             store_state<KP>(rows_state, P.dstates + (sequence * (P.n_chunks - 1) + chunk) * K * V + first, K, dstate);
         f4 du[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) du[i] = f4{0, 0, 0, 0};
-        if (!last || from) {
+        if (step > walk.begin || walk.from || walk.unit) {
 #pragma unroll
             for (int m = 0; m < KP / 32; ++m) {
-                u4 b[3], a[N];
+                u4 b[3], a[4][N];
                 split8(dstate[2 * m], dstate[2 * m + 1], b);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    operand_rows_as_results(lds.rows.k, 16 * i, m, a);
-                    du[i] = mma(a, b, du[i]);
-                }
+                for (int i = 0; i < 4; ++i) operand_rows_as_results(lds.rows.k, 16 * i, m, a[i]);
+                mma_each<4>(a, b, du);
                 stage();
             }
 #pragma unroll
@@ -339,66 +422,104 @@ __global__ __launch_bounds__(kThreads) void delta_reverse_kernel(RuleParams P) {
             u4 raw[2][N];
 #pragma unroll
             for (int m = 0; m < 2; ++m) split8(dO[2 * m], dO[2 * m + 1], raw[m]);
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int m = j / 2; m < 2; ++m) {
-                    u4 a[3];
-                    operand_transpose<3>(lds.p, j, m, a);
-                    du[j] = mma(a, raw[m], du[j]);
-                    stage();
-                }
+            times_transpose<3>(lds.p, raw, du);
         }
         u4 b[2][3];
 #pragma unroll
         for (int m = 0; m < 2; ++m) split8(du[2 * m], du[2 * m + 1], b[m]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            du[j] = f4{0, 0, 0, 0};
-#pragma unroll
-            for (int m = j / 2; m < 2; ++m) {
-                u4 a[3];
-                operand_transpose<3>(lds.x, j, m, a);
-                du[j] = mma(a, b[m], du[j]);  // dr
-                stage();
-            }
+        for (int j = 0; j < 4; ++j) du[j] = f4{0, 0, 0, 0};
+        times_transpose<3>(lds.x, b, du);  // dr
+        if constexpr (!kSummary) {
+            rows_v.template store<4>(
+                rows_v.rows(static_cast<E*>(P.d.d_v) + ((env * P.r.steps + t0) * P.r.value_heads + head) * V + first, tokens),
+                [&](int j, int s) { return from_float<E>(du[j][s]); });
+            rows_state.store<4>(rows_state.rows(P.rgrads + (sequence * P.r.steps + t0) * V + first, tokens),
+                                [&](int j, int s) { return du[j][s]; });
         }
-        rows_v.template store<4>(
-            rows_v.rows(static_cast<E*>(P.d.d_v) + ((env * P.r.steps + t0) * P.r.value_heads + head) * V + first, tokens),
-            [&](int j, int s) { return from_float<E>(du[j][s]); });
-        rows_state.store<4>(rows_state.rows(P.rgrads + (sequence * P.r.steps + t0) * V + first, tokens),
-                            [&](int j, int s) { return du[j][s]; });
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const f4 e = four(lds.gates[0], 16 * j + 4 * g);
-            du[j] = -e * du[j];
-            dO[j] = P.r.scale * e * dO[j];
-        }
-        if (chunk > 0 || P.d.d_initial_state) {
+        if (chunk > 0 || kSummary || P.d.d_initial_state) {
             const float keep = lds.gates[0][kChunk - 1];
-            u4 c3[2][3];
 #pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                split8(du[2 * m], du[2 * m + 1], b[m]);
-                split8(dO[2 * m], dO[2 * m + 1], c3[m]);
+            for (int j = 0; j < 4; ++j) {
+                const f4 e = four(lds.gates[0], 16 * j + 4 * g);
+                du[j] = -e * du[j];
+                dO[j] = P.r.scale * e * dO[j];
             }
 #pragma unroll
-            for (int c = 0; c < KP / 16; ++c) {
-                dstate[c] = gated(dstate[c], f4{keep, keep, keep, keep});
+            for (int c = 0; c < KP / 16; ++c) dstate[c] = gated(dstate[c], f4{keep, keep, keep, keep});
 #pragma unroll
-                for (int m = 0; m < 2; ++m) {
-                    u4 a[N];
-                    operand_columns(lds.rows.k, c, m, a);
-                    dstate[c] = mma(a, b[m], dstate[c]);
-                    operand_columns(lds.rows.q, c, m, a);
-                    dstate[c] = mma(a, c3[m], dstate[c]);
-                }
-                stage();
-            }
+            for (int m = 0; m < 2; ++m) split8(du[2 * m], du[2 * m + 1], b[m]);
+#pragma unroll
+            for (int c = 0; c < KP / 16; c += 4) add_columns(lds.rows.k, c, b, dstate);
+#pragma unroll
+            for (int m = 0; m < 2; ++m) split8(dO[2 * m], dO[2 * m + 1], b[m]);
+#pragma unroll
+            for (int c = 0; c < KP / 16; c += 4) add_columns(lds.rows.q, c, b, dstate);
         }
     }
-    if (P.d.d_initial_state && working)
-        store_state<KP>(rows_state, P.d.d_initial_state + sequence * K * V + first, K, dstate);
+    if (walk.to && walk.working) store_state<KP>(rows_state, walk.to + first, K, dstate);
+}
+
+// The states before the segments but the first, one after another, from what the summary left
+// of each: S <- M S + N with N the state that it makes of zeros (of the given state, for
+// segment 0) and M its matrix. Takes N's place. A workgroup holds 64 columns; M's planes go
+// through LDS.
+template <int KP>
+__global__ __launch_bounds__(256) void delta_join_kernel(RuleParams P) {
+    extern __shared__ char lds_bytes[];
+    auto& m_planes = *reinterpret_cast<uint16_t(*)[KP / 16][KP / 32][3][64][8]>(lds_bytes);
+    const int wave = wave_of_workgroup();
+    const int64_t sequence = blockIdx.x;
+    const int first = (blockIdx.y * 4 + wave) * 16;
+    const int K = P.r.key_dim, V = P.r.value_dim;
+    const int64_t kv = static_cast<int64_t>(K) * V, slots = sequence * (P.n_segments - 1);
+    const Columns<float> rows_state(V, V - first);
+    f4 state[KP / 16], next[KP / 16];
+    load_state<KP>(rows_state, P.segment_states + slots * kv + first, K, state);
+    for (int segment = 1; segment + 1 < P.n_segments; ++segment) {
+        const Buffer matrix = buffer_of(P.segment_matrices + (slots + segment) * K * K, 4 * K * K);
+        load_state<KP>(rows_state, P.segment_states + (slots + segment) * kv + first, K, next);
+        if (segment > 1) __syncthreads();
+        // an operand's lane holds columns 4 g and 16 + 4 g on of 32, in the order of results
+#pragma unroll 4
+        for (int n = threadIdx.x; n < KP * KP / 8; n += 256) {
+            const int lane = n & 63, m = (n >> 6) % (KP / 32), c = (n >> 6) / (KP / 32);
+            const int row = 16 * c + (lane & 15), column = 32 * m + 4 * (lane >> 4);
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int at = column + i % 4 + i / 4 * 16;
+                x[i] = buffer_load<float>(matrix, row < K && at < K ? 4 * (row * K + at) : kOutside);
+            }
+            u4 plane[3];
+            split8(x, plane);
+#pragma unroll
+            for (int i = 0; i < 3; ++i) *reinterpret_cast<u4*>(m_planes[c][m][i][lane]) = plane[i];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int m = 0; m < KP / 32; ++m) {
+            u4 b[3];
+            split8(state[2 * m], state[2 * m + 1], b);
+#pragma unroll
+            for (int c = 0; c < KP / 16; c += 2) {
+                u4 a[2][3];
+                f4 x[2] = {next[c], next[c + 1]};
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int i = 0; i < 3; ++i)
+                        a[n][i] = *reinterpret_cast<const u4*>(m_planes[c + n][m][i][threadIdx.x & 63]);
+                mma_each<2>(a, b, x);
+                next[c] = x[0];
+                next[c + 1] = x[1];
+            }
+            stage();
+        }
+#pragma unroll
+        for (int c = 0; c < KP / 16; ++c) state[c] = next[c];
+        store_state<KP>(rows_state, P.segment_states + (slots + segment) * kv + first, K, state);
+    }
 }
 
 // Sixteen rows of results, KP / 16 tiles across, into `rows` rows of `columns` numbers.
@@ -796,40 +917,66 @@ int launched(const char* what) {
 // Columns of a head that a workgroup takes: up to 64, or up to 128 where the head has more.
 int columns_of(int value_dim) { return value_dim <= 64 ? 64 : 128; }
 
-dim3 scan_grid(const RuleParams& P) {
-    const int columns = columns_of(P.r.value_dim);
-    return dim3(static_cast<unsigned>(P.r.envs * P.r.value_heads), (P.r.value_dim + columns - 1) / columns);
+int blocks_of(int value_dim) { return (value_dim + columns_of(value_dim) - 1) / columns_of(value_dim); }
+
+// Walks in segments: 0 workgroups of a whole walk are too few to fill the card's 256 CUs, and
+// the chunks enough that the summary pass and the join (about as long as four chunks) pay.
+int segments_of(int64_t sequences, int value_dim, int64_t chunks) {
+    const int64_t blocks = sequences * blocks_of(value_dim);
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({256 / std::max<int64_t>(1, blocks), chunks / 4, 16})));
+}
+
+int64_t segment_floats(int64_t sequences, int key_dim, int value_dim, int segments) {
+    return sequences * (segments - 1) * (static_cast<int64_t>(key_dim) * value_dim + key_dim * key_dim);
+}
+
+template <class E, int KP, int kThreads, bool kBack, bool kSummary>
+int walk(const RuleParams& P, dim3 grid, hipStream_t stream) {
+    constexpr size_t lds = sizeof(ScanLds<E, KP, kBack ? 3 : kOutPlanes<E>>);
+    if constexpr (kBack)
+        hipLaunchKernelGGL((delta_reverse_kernel<E, KP, kThreads, kSummary>), grid, dim3(kThreads), lds, stream, P);
+    else
+        hipLaunchKernelGGL((delta_forward_kernel<E, KP, kThreads, kSummary>), grid, dim3(kThreads), lds, stream, P);
+    return launched("the gated delta rule");
+}
+
+template <class E, int KP, bool kBack>
+int walk_all(const RuleParams& P, hipStream_t stream) {
+    const unsigned sequences = static_cast<unsigned>(P.r.envs * P.r.value_heads);
+    const unsigned segments = static_cast<unsigned>(P.n_segments);
+    if (segments > 1) {
+        const int columns = (P.r.value_dim + 15) / 16 * 16 + P.r.key_dim;
+        int code = walk<E, KP, 256, kBack, true>(P, dim3(sequences, (columns + 63) / 64, segments - 1), stream);
+        if (code != NAVI_POLICY_OK) return code;
+        if (segments > 2) {
+            hipLaunchKernelGGL(delta_join_kernel<KP>, dim3(sequences, (P.r.value_dim + 63) / 64), dim3(256),
+                               KP * KP * 6, stream, P);
+            code = launched("the gated delta rule");
+            if (code != NAVI_POLICY_OK) return code;
+        }
+    }
+    const dim3 grid(sequences, blocks_of(P.r.value_dim), segments);
+    return columns_of(P.r.value_dim) == 64 ? walk<E, KP, 256, kBack, false>(P, grid, stream)
+                                           : walk<E, KP, 512, kBack, false>(P, grid, stream);
 }
 
 template <class E, int KP>
 int forward(const RuleParams& P, hipStream_t stream) {
-    const dim3 grid = scan_grid(P);
     if (P.n_chunks > 0) {
-        hipLaunchKernelGGL((delta_triangles_kernel<E, KP>), dim3(grid.x * static_cast<unsigned>(P.n_chunks)), dim3(256),
-                           sizeof(TriangleLds<E, KP>), stream, P);
+        hipLaunchKernelGGL((delta_triangles_kernel<E, KP>), dim3(static_cast<unsigned>(P.r.envs * P.r.value_heads * P.n_chunks)),
+                           dim3(256), sizeof(TriangleLds<E, KP>), stream, P);
         const int code = launched("navi_delta_forward");
         if (code != NAVI_POLICY_OK) return code;
     }
-    constexpr size_t lds = sizeof(ScanLds<E, KP, kOutPlanes<E>>);
-    if (columns_of(P.r.value_dim) == 64)
-        hipLaunchKernelGGL((delta_forward_kernel<E, KP, 256>), grid, dim3(256), lds, stream, P);
-    else
-        hipLaunchKernelGGL((delta_forward_kernel<E, KP, 512>), grid, dim3(512), lds, stream, P);
-    return launched("navi_delta_forward");
+    return walk_all<E, KP, false>(P, stream);
 }
 
 template <class E, int KP>
 int backward(const RuleParams& P, hipStream_t stream) {
-    const dim3 grid = scan_grid(P);
-    constexpr size_t lds = sizeof(ScanLds<E, KP, 3>);
-    if (columns_of(P.r.value_dim) == 64)
-        hipLaunchKernelGGL((delta_reverse_kernel<E, KP, 256>), grid, dim3(256), lds, stream, P);
-    else
-        hipLaunchKernelGGL((delta_reverse_kernel<E, KP, 512>), grid, dim3(512), lds, stream, P);
-    int code = launched("navi_delta_backward");
+    int code = walk_all<E, KP, true>(P, stream);
     if (code != NAVI_POLICY_OK) return code;
-    hipLaunchKernelGGL((delta_gradients_kernel<E, KP>), dim3(grid.x * static_cast<unsigned>(P.n_chunks)), dim3(256),
-                       sizeof(GradientLds<E, KP>), stream, P);
+    hipLaunchKernelGGL((delta_gradients_kernel<E, KP>), dim3(static_cast<unsigned>(P.r.envs * P.r.value_heads * P.n_chunks)),
+                       dim3(256), sizeof(GradientLds<E, KP>), stream, P);
     code = launched("navi_delta_backward");
     if (code != NAVI_POLICY_OK || P.group == 1) return code;
     const int64_t count = P.r.envs * P.r.steps * P.r.key_heads * P.r.key_dim;
@@ -893,6 +1040,7 @@ int setup(const navi_delta_rule* r, RuleParams& P) {
     P.r = *r;
     P.group = r->value_heads / r->key_heads;
     P.n_chunks = static_cast<int32_t>(chunks_of(r->steps));
+    P.n_segments = segments_of(r->envs * r->value_heads, r->value_dim, P.n_chunks);
     const int64_t bytes = r->dtype == NAVI_POLICY_F32 ? 4 : 2;
     if (r->envs * r->value_heads * chunks_of(r->steps) > INT32_MAX)
         return set_error(NAVI_POLICY_E_ARG, "envs * value_heads * chunks must be below 2^31");
@@ -911,6 +1059,13 @@ int setup(const navi_delta_rule* r, RuleParams& P) {
     return NAVI_POLICY_OK;
 }
 
+float* place_segments(RuleParams& P, float* at) {
+    const int64_t slots = P.r.envs * P.r.value_heads * (P.n_segments - 1);
+    P.segment_states = at;
+    P.segment_matrices = at + slots * P.r.key_dim * P.r.value_dim;
+    return P.segment_matrices + slots * P.r.key_dim * P.r.key_dim;
+}
+
 }  // namespace
 }  // namespace navi_policy
 
@@ -923,7 +1078,18 @@ extern "C" int navi_delta_forward(const navi_delta_rule* rule, void* stream) {
     if (!rule->states != !rule->updates && P.n_chunks > 1)
         return set_error(NAVI_POLICY_E_ARG, "states and updates are saved together or not at all");
     if (P.n_chunks == 0 && !rule->final_state) return NAVI_POLICY_OK;
+    if (P.n_segments > 1 && (!rule->scratch || !aligned16(rule->scratch)))
+        return set_error(NAVI_POLICY_E_ARG, "scratch must be non-null and 16-byte aligned");
+    place_segments(P, static_cast<float*>(rule->scratch));
     return run_typed(P, false, as_stream(stream));
+}
+
+extern "C" int64_t navi_delta_scratch(const navi_delta_rule* rule) {
+    const int code = check_rule(rule);
+    if (code < 0) return code;
+    const int64_t sequences = rule->envs * rule->value_heads;
+    return 4 * segment_floats(sequences, rule->key_dim, rule->value_dim,
+                              segments_of(sequences, rule->value_dim, chunks_of(rule->steps)));
 }
 
 extern "C" int64_t navi_delta_workspace(const navi_delta_rule* rule) {
@@ -935,7 +1101,9 @@ extern "C" int64_t navi_delta_workspace(const navi_delta_rule* rule) {
     const int64_t rows = sequences * steps * rule->value_dim;
     const int64_t heads = rule->value_heads > rule->key_heads ? sequences * steps * rule->key_dim : 0;
     const auto rounded = [](int64_t n) { return (n + 3) / 4 * 4; };
-    return 4 * (rounded(states) + rounded(rows) + 2 * rounded(heads));
+    const int64_t segments = segment_floats(sequences, rule->key_dim, rule->value_dim,
+                                            segments_of(sequences, rule->value_dim, chunks_of(steps)));
+    return 4 * (rounded(states) + rounded(rows) + 2 * rounded(heads) + segments);
 }
 
 extern "C" int navi_delta_backward(const navi_delta_rule* rule, const navi_delta_gradients* gradients, void* stream) {
@@ -956,6 +1124,7 @@ extern "C" int navi_delta_backward(const navi_delta_rule* rule, const navi_delta
     P.rgrads = P.dstates + rounded(sequences * (P.n_chunks - 1) * rule->key_dim * rule->value_dim);
     P.dq_heads = P.rgrads + rounded(sequences * rule->steps * rule->value_dim);
     P.dk_heads = P.dq_heads + rounded(P.group > 1 ? sequences * rule->steps * rule->key_dim : 0);
+    place_segments(P, P.dk_heads + rounded(P.group > 1 ? sequences * rule->steps * rule->key_dim : 0));
     const int64_t bytes = rule->dtype == NAVI_POLICY_F32 ? 4 : 2;
     if (rule->steps == 1) P.d.grad_out_stride[1] = rule->value_dim;
     if (!rows_apart(P.d.grad_out_stride, bytes, rule->value_dim))

@@ -116,6 +116,19 @@ __device__ inline f4 mma(const u4 (&a)[NA], const u4 (&b)[NB], f4 c) {
     return c;
 }
 
+// The products of several left operands with one right operand, term by term over all of them:
+// a product waits for the one before it in the same sum, so neighbours are of different sums.
+template <int kCount, int NA, int NB>
+__device__ inline void mma_each(const u4 (&a)[kCount][NA], const u4 (&b)[NB], f4 (&c)[kCount]) {
+#pragma unroll
+    for (int s = (NA + NB - 2 < 2 ? NA + NB - 2 : 2); s >= 0; --s)
+#pragma unroll
+        for (int i = 0; i < NA; ++i)
+            if (s - i >= 0 && s - i < NB)
+#pragma unroll
+                for (int n = 0; n < kCount; ++n) c[n] = mfma(a[n][i], b[s - i], c[n]);
+}
+
 // 16x16x4 in float32: A's lane holds row l % 16, B's column l % 16, at l / 16 of the four.
 __device__ inline f4 mfma_f32(float a, float b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 

@@ -141,6 +141,10 @@ def _forward(q, k, v, g, beta, starts, scale, initial_state, return_state, save)
         updates = torch.empty((envs * heads, steps, dim), dtype=torch.float32, device=v.device)
     a = _rule_args(q, k, v, g, beta, starts, scale, initial_state, out, state)
     a.matrices, a.states, a.updates = matrices.data_ptr(), _ptr(states), _ptr(updates)
+    scratch = _native.check(_native.lib().navi_delta_scratch(ctypes.byref(a)))
+    if scratch:
+        scratch = torch.empty(scratch // 4, dtype=torch.float32, device=v.device)
+        a.scratch = scratch.data_ptr()
     with torch.cuda.device(q.device):
         _native.check(_native.lib().navi_delta_forward(ctypes.byref(a), _stream(q.device)))
     return out, state, matrices, states, updates
@@ -199,15 +203,15 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     ``ValueHeads`` a multiple of ``KeyHeads`` (value head h reads key head
     ``h // (ValueHeads // KeyHeads)``). ``g`` (the logarithm of the decay, at most 0; -inf
     forgets everything) and ``beta``: ``[Envs, Steps, ValueHeads]`` float32. ``starts``:
-    ``[Envs, Steps]`` bool or uint8, tokens that begin an episode (the state before one is
-    forgotten, whatever it holds). ``initial_state``: ``[Envs, ValueHeads, KeyDim, ValueDim]``
+    ``[Envs, Steps]`` bool or uint8, tokens that begin an episode: the state before one is
+    forgotten (at the first step, whatever it holds). ``initial_state``: ``[Envs, ValueHeads, KeyDim, ValueDim]``
     float32, zeros by default. ``scale`` defaults to ``KeyDim ** -0.5``.
 
     Returns ``o`` like ``v``, with ``return_state`` also the state after the last token. Keys
     are meant to have norm 1 (``qk_norm`` with ``norm="l2"``) and beta to lie in [0, 1]: the
     memory contracts then. Arithmetic is of float32's precision for every type, rounded
-    once at the end. A NaN or infinity among q, k, v may reach every token of its chunk of 64
-    tokens and head.
+    once at the end. A NaN or infinity in the inputs may reach every token of its chunk of 64
+    tokens and what follows them, beyond the start of an episode too.
     """
     _check_rule(q, k, v, g, beta, starts, ("Envs", "Steps"))
     if initial_state is not None:

@@ -101,6 +101,42 @@ def test_rule_and_gradients(policy, size, with_state):
         assert torch.equal(back["g"].cpu()[starts.cpu()], torch.zeros_like(back["g"].cpu()[starts.cpu()]))
 
 
+LONG = [  # few heads and many chunks: walked in segments that are joined
+    (1, 64 * 8, 1, 1, 64, 64, torch.float32),
+    (1, 64 * 9 + 5, 1, 2, 33, 70, torch.bfloat16),
+    (2, 64 * 12 + 1, 1, 2, 128, 128, torch.float16),
+    (1, 64 * 21 + 63, 1, 1, 100, 150, torch.float32),
+]
+
+
+@pytest.mark.parametrize("ends", [True, False], ids=["episodes", "one episode"])
+@pytest.mark.parametrize("size", LONG, ids=str)
+def test_long_walks(policy, size, ends):
+    dtype = size[-1]
+    x, state, starts = make(*size, seed=21)
+    starts = (torch.rand(starts.shape, device="cuda") < 0.003) if ends else None
+    x["g"] *= 0.05  # (a state that lasts through segments)
+    leaves = [t.clone().requires_grad_() for t in x.values()]
+    s0 = state.clone().requires_grad_()
+    o, final = policy.gated_delta_rule(*leaves, starts=starts, initial_state=s0, return_state=True)
+    exact = [t.detach().cpu().double().requires_grad_() for t in leaves]
+    e0 = state.cpu().double().requires_grad_()
+    want_o, want_final = ref.rule(*exact, starts, e0, size[4] ** -0.5)
+    assert ref.off(o, want_o) <= tolerance(dtype)
+    assert ref.off(final, want_final) <= TOL
+    gen = torch.Generator().manual_seed(5)
+    go, gs = torch.randn(o.shape, generator=gen).to(dtype), torch.randn(final.shape, generator=gen)
+    back = torch.autograd.grad([o, final], leaves + [s0], [go.cuda(), gs.cuda()])
+    want = torch.autograd.grad([want_o, want_final], exact + [e0], [go.double(), gs.double()])
+    for a, b in zip(back[:3], want[:3]):
+        assert ref.off(a, b) <= tolerance(dtype)
+    assert ref.off(back[4], want[4]) <= 2 * TOL
+    room = 2 * TOL * float(want[3].norm() + (want[4] * exact[4].detach()).norm())
+    assert float((back[3].cpu().double() - want[3]).norm()) <= room
+    if float(want[5].norm()):
+        assert ref.off(back[5], want[5]) <= TOL
+
+
 @pytest.mark.parametrize("size", [SIZES[4], SIZES[7], SIZES[9]], ids=str)
 def test_steps_give_what_the_rollout_gives(policy, size):
     x, state, starts = make(*size, seed=3)
