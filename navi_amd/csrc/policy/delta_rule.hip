@@ -70,10 +70,6 @@ __device__ inline f4 gated(f4 x, f4 factor) {
     return y;
 }
 
-// Keeps the compiler from reading the operands of later products early: it would hold them
-// in more registers than there are.
-__device__ inline void stage() { __builtin_amdgcn_sched_barrier(0); }
-
 __device__ inline int tokens_of(const RuleParams& P, int chunk) {
     const int64_t left = P.r.steps - static_cast<int64_t>(chunk) * kChunk;
     return static_cast<int>(left < kChunk ? left : kChunk);
@@ -191,7 +187,6 @@ __device__ inline void times_triangle(const Triangle<N>& t, const u4 (&b)[2][NB]
 #pragma unroll
     for (int i = 0; i < 4; ++i) operand_triangle<N>(t, i, 0, a[i]);
     mma_each<4>(a, b[0], x);
-    stage();
     u4 below[2][N];
     f4 y[2] = {x[2], x[3]};
 #pragma unroll
@@ -199,7 +194,6 @@ __device__ inline void times_triangle(const Triangle<N>& t, const u4 (&b)[2][NB]
     mma_each<2>(below, b[1], y);
     x[2] = y[0];
     x[3] = y[1];
-    stage();
 }
 
 template <int N, int NB>
@@ -208,7 +202,6 @@ __device__ inline void times_transpose(const Triangle<N>& t, const u4 (&b)[2][NB
 #pragma unroll
     for (int j = 0; j < 4; ++j) operand_transpose<N>(t, j, 1, a[j]);
     mma_each<4>(a, b[1], x);
-    stage();
     u4 left[2][N];
     f4 y[2] = {x[0], x[1]};
 #pragma unroll
@@ -216,7 +209,6 @@ __device__ inline void times_transpose(const Triangle<N>& t, const u4 (&b)[2][NB
     mma_each<2>(left, b[0], y);
     x[0] = y[0];
     x[1] = y[1];
-    stage();
 }
 
 // Columns of rows in LDS times b, added to four tiles of a state from tile c on.
@@ -229,7 +221,6 @@ __device__ inline void add_columns(const uint16_t (&rows)[N][kChunk][kPitch], in
 #pragma unroll
         for (int n = 0; n < 4; ++n) operand_columns(rows, c + n, m, a[n]);
         mma_each<4>(a, b[m], x);
-        stage();
     }
 #pragma unroll
     for (int n = 0; n < 4; ++n) state[c + n] = x[n];
@@ -281,7 +272,6 @@ __global__ __launch_bounds__(kThreads) void delta_forward_kernel(RuleParams P) {
         __syncthreads();
         if (chunk + 1 < walk.end) fetch(chunk + 1);
         if (!walk.working) continue;
-        stage();
 
         if (!kSummary && P.r.states && chunk > 0)
             store_state<KP>(rows_state, P.r.states + (sequence * (P.n_chunks - 1) + chunk - 1) * K * V + first, K, state);
@@ -303,7 +293,6 @@ __global__ __launch_bounds__(kThreads) void delta_forward_kernel(RuleParams P) {
                     for (int i = 0; i < 4; ++i) operand_rows_as_results(lds.rows.q, 16 * i, m, a[i]);
                     mma_each<4>(a, b_out, o);
                 }
-                stage();
             }
         }
         u4 r[2][3];
@@ -320,7 +309,6 @@ __global__ __launch_bounds__(kThreads) void delta_forward_kernel(RuleParams P) {
             }
             split8(x[0], x[1], r[m]);
         }
-        stage();
         times_triangle<3>(lds.x, r, u);
         if (!kSummary && P.r.updates)
             rows_state.store<4>(rows_state.rows(P.r.updates + (sequence * P.r.steps + t0) * V + first, tokens),
@@ -398,7 +386,6 @@ __global__ __launch_bounds__(kThreads) void delta_reverse_kernel(RuleParams P) {
         __syncthreads();
         if (step + 1 < walk.end) fetch(chunk - 1);
         if (!walk.working) continue;
-        stage();
 
         if (!kSummary && step > 0)
             store_state<KP>(rows_state, P.dstates + (sequence * (P.n_chunks - 1) + chunk) * K * V + first, K, dstate);
@@ -413,7 +400,6 @@ __global__ __launch_bounds__(kThreads) void delta_reverse_kernel(RuleParams P) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) operand_rows_as_results(lds.rows.k, 16 * i, m, a[i]);
                 mma_each<4>(a, b, du);
-                stage();
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) du[i] = du[i] * four(lds.gates[1], 16 * i + 4 * g);
@@ -476,48 +462,68 @@ __global__ __launch_bounds__(256) void delta_join_kernel(RuleParams P) {
     const Columns<float> rows_state(V, V - first);
     f4 state[KP / 16], next[KP / 16];
     load_state<KP>(rows_state, P.segment_states + slots * kv + first, K, state);
-    for (int segment = 1; segment + 1 < P.n_segments; ++segment) {
+    // of a segment while the one before it is computed: its N, and an operand's parts of its M (a
+    // lane holds columns 4 g and 16 + 4 g on of 32, in the order of results)
+    constexpr int kParts = KP * KP / 8 / 256;
+    f4 part[kParts][2];
+    const bool wide = K % 4 == 0;
+    const auto fetch = [&](int segment) {
         const Buffer matrix = buffer_of(P.segment_matrices + (slots + segment) * K * K, 4 * K * K);
         load_state<KP>(rows_state, P.segment_states + (slots + segment) * kv + first, K, next);
-        if (segment > 1) __syncthreads();
-        // an operand's lane holds columns 4 g and 16 + 4 g on of 32, in the order of results
-#pragma unroll 4
-        for (int n = threadIdx.x; n < KP * KP / 8; n += 256) {
-            const int lane = n & 63, m = (n >> 6) % (KP / 32), c = (n >> 6) / (KP / 32);
-            const int row = 16 * c + (lane & 15), column = 32 * m + 4 * (lane >> 4);
-            float x[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int at = column + i % 4 + i / 4 * 16;
-                x[i] = buffer_load<float>(matrix, row < K && at < K ? 4 * (row * K + at) : kOutside);
+        for (int n = 0; n < kParts; ++n) {
+            const int at = threadIdx.x + 256 * n, lane = at & 63, m = (at >> 6) % (KP / 32), c = (at >> 6) / (KP / 32);
+            const int row = 16 * c + (lane & 15);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int column = 32 * m + 4 * (lane >> 4) + 16 * h;
+                const uint32_t offset = 4 * (row * K + column);
+                if (wide) {
+                    part[n][h] = __builtin_bit_cast(f4, buffer_load16(matrix, row < K && column < K ? offset : kOutside));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        part[n][h][i] = buffer_load<float>(matrix, row < K && column + i < K ? offset + 4 * i : kOutside);
+                }
             }
-            u4 plane[3];
-            split8(x, plane);
-#pragma unroll
-            for (int i = 0; i < 3; ++i) *reinterpret_cast<u4*>(m_planes[c][m][i][lane]) = plane[i];
         }
+    };
+    if (P.n_segments > 2) fetch(1);
+    for (int segment = 1; segment + 1 < P.n_segments; ++segment) {
+        if (segment > 1) __syncthreads();
+#pragma unroll
+        for (int n = 0; n < kParts; ++n) {
+            const int at = threadIdx.x + 256 * n;
+            u4 plane[3];
+            split8(part[n][0], part[n][1], plane);
+#pragma unroll
+            for (int i = 0; i < 3; ++i) *reinterpret_cast<u4*>(m_planes[(at >> 6) / (KP / 32)][(at >> 6) % (KP / 32)][i][at & 63]) = plane[i];
+        }
+        f4 x[KP / 16];
+#pragma unroll
+        for (int c = 0; c < KP / 16; ++c) x[c] = next[c];
         __syncthreads();
+        if (segment + 2 < P.n_segments) fetch(segment + 1);
 #pragma unroll
         for (int m = 0; m < KP / 32; ++m) {
             u4 b[3];
             split8(state[2 * m], state[2 * m + 1], b);
 #pragma unroll
-            for (int c = 0; c < KP / 16; c += 2) {
-                u4 a[2][3];
-                f4 x[2] = {next[c], next[c + 1]};
+            for (int c = 0; c < KP / 16; c += 4) {
+                u4 a[4][3];
+                f4 y[4] = {x[c], x[c + 1], x[c + 2], x[c + 3]};
 #pragma unroll
-                for (int n = 0; n < 2; ++n)
+                for (int n = 0; n < 4; ++n)
 #pragma unroll
                     for (int i = 0; i < 3; ++i)
                         a[n][i] = *reinterpret_cast<const u4*>(m_planes[c + n][m][i][threadIdx.x & 63]);
-                mma_each<2>(a, b, x);
-                next[c] = x[0];
-                next[c + 1] = x[1];
+                mma_each<4>(a, b, y);
+#pragma unroll
+                for (int n = 0; n < 4; ++n) x[c + n] = y[n];
             }
-            stage();
         }
 #pragma unroll
-        for (int c = 0; c < KP / 16; ++c) state[c] = next[c];
+        for (int c = 0; c < KP / 16; ++c) state[c] = x[c];
         store_state<KP>(rows_state, P.segment_states + (slots + segment) * kv + first, K, state);
     }
 }
@@ -708,7 +714,6 @@ __global__ __launch_bounds__(256, KP == 64 ? 3 : 1) void delta_gradients_kernel(
         split8(a, a_dr);
         __syncthreads();
         if (v0 + 32 < V) fetch(v0 + 32);
-        stage();
         if (dS) {
 #pragma unroll
             for (int n = 0; n < 3; ++n) a_u[n] = *reinterpret_cast<const u4*>(lds.stage.u[wave][n][lane]);
@@ -727,7 +732,6 @@ __global__ __launch_bounds__(256, KP == 64 ? 3 : 1) void delta_gradients_kernel(
                 for (int n = 0; n < 3; ++n) x[n] = *reinterpret_cast<const u4*>(lds.stage.ds[c][n][lane]);
                 w[c] = mma(a_u, x, w[c]);
             }
-            stage();
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -737,7 +741,6 @@ __global__ __launch_bounds__(256, KP == 64 ? 3 : 1) void delta_gradients_kernel(
             for (int n = 0; n < 3; ++n) x[n] = *reinterpret_cast<const u4*>(lds.stage.u[j][n][lane]);
             h[j] = mma(a_do, x, h[j]);
             rr[j] = mma(a_dr, x, rr[j]);
-            stage();
         }
     }
     dot = sum16(dot);
@@ -873,7 +876,6 @@ __global__ __launch_bounds__(256, KP == 64 ? 3 : 1) void delta_gradients_kernel(
                 operand_columns(lds.rows.q, c, m, b);
                 z[c] = mma(n_below, b, z[c]);
             }
-            if (c % 2) stage();
         }
     }
     const int left = tokens - 16 * wave;  // rows of the wave's tile
