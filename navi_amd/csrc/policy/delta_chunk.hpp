@@ -159,8 +159,7 @@ __device__ inline float decay(const ChunkGates& gates, int i, float hi_j, float 
 // Operands of products from rows in LDS: rows row0 to row0 + 15, eight columns of 32 m to
 // 32 m + 31 a lane, in their order;
 template <int N, int kPitch>
-__device__ inline void operand_rows(const uint16_t (&rows)[N][kChunk][kPitch], int row0, int m, u4 (&x)[N]) {
-    const int lane = threadIdx.x & 63;
+__device__ inline void operand_rows(int lane, const uint16_t (&rows)[N][kChunk][kPitch], int row0, int m, u4 (&x)[N]) {
 #pragma unroll
     for (int n = 0; n < N; ++n)
         x[n] = *reinterpret_cast<const u4*>(&rows[n][row0 + (lane & 15)][32 * m + 8 * (lane >> 4)]);
@@ -169,9 +168,8 @@ __device__ inline void operand_rows(const uint16_t (&rows)[N][kChunk][kPitch], i
 // the same in the order in which two tiles of a product's result hold a column (rows 4 g to
 // 4 g + 3 of each, g = l / 16), so that such a result is the other operand without a move;
 template <int N, int kPitch>
-__device__ inline void operand_rows_as_results(const uint16_t (&rows)[N][kChunk][kPitch], int row0, int m,
+__device__ inline void operand_rows_as_results(int lane, const uint16_t (&rows)[N][kChunk][kPitch], int row0, int m,
                                                u4 (&x)[N]) {
-    const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
         const uint16_t* row = &rows[n][row0 + (lane & 15)][32 * m + 4 * (lane >> 4)];
@@ -183,8 +181,8 @@ __device__ inline void operand_rows_as_results(const uint16_t (&rows)[N][kChunk]
 // and columns 16 c to 16 c + 15 as the operand's rows, tokens 32 m to 32 m + 31 contracted in
 // that same order.
 template <int N, int kPitch>
-__device__ inline void operand_columns(const uint16_t (&rows)[N][kChunk][kPitch], int c, int m, u4 (&x)[N]) {
-    const int lane = threadIdx.x & 63, i = lane & 15;
+__device__ inline void operand_columns(int lane, const uint16_t (&rows)[N][kChunk][kPitch], int c, int m, u4 (&x)[N]) {
+    const int i = lane & 15;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
         const uint16_t* from = &rows[n][32 * m + 4 * (lane >> 4) + (i >> 2)][16 * c + 4 * (i & 3)];
@@ -196,8 +194,8 @@ __device__ inline void operand_columns(const uint16_t (&rows)[N][kChunk][kPitch]
 // A triangle's rows 16 i to 16 i + 15, columns 32 m to 32 m + 31 (32 m <= 16 i) as an operand
 // whose contracted axis is in the order of results;
 template <int N>
-__device__ inline void operand_triangle(const Triangle<N>& t, int i, int m, u4 (&x)[N]) {
-    const int lane = threadIdx.x & 63, l = lane & 15;
+__device__ inline void operand_triangle(int lane, const Triangle<N>& t, int i, int m, u4 (&x)[N]) {
+    const int l = lane & 15;
     const int slot = (l & 3) * 16 + 4 * (lane >> 4) + (l >> 2);
 #pragma unroll
     for (int n = 0; n < N; ++n) {
@@ -209,8 +207,7 @@ __device__ inline void operand_triangle(const Triangle<N>& t, int i, int m, u4 (
 
 // and of its transpose, rows 16 j on, columns 32 m on (16 j < 32 m + 32).
 template <int N>
-__device__ inline void operand_transpose(const Triangle<N>& t, int j, int m, u4 (&x)[N]) {
-    const int lane = threadIdx.x & 63;
+__device__ inline void operand_transpose(int lane, const Triangle<N>& t, int j, int m, u4 (&x)[N]) {
 #pragma unroll
     for (int n = 0; n < N; ++n) {
         const u2 a = 2 * m >= j ? *reinterpret_cast<const u2*>(t[tile_of(2 * m, j)][n][lane]) : u2{0, 0};
@@ -332,10 +329,10 @@ __device__ inline void make_triangles(TriangleLds<E, KP>& lds, ChunkMatrices& to
 #pragma unroll
         for (int m = 0; m < KP / 32; ++m) {
             u4 ki[N], qi[N], kj[N];
-            operand_rows(lds.rows.k, 16 * j, m, kj);
-            operand_rows(lds.rows.k, 16 * i, m, ki);
+            operand_rows(lane, lds.rows.k, 16 * j, m, kj);
+            operand_rows(lane, lds.rows.k, 16 * i, m, ki);
             kk = mma(ki, kj, kk);
-            operand_rows(lds.rows.q, 16 * i, m, qi);
+            operand_rows(lane, lds.rows.q, 16 * i, m, qi);
             qk = mma(qi, kj, qk);
         }
         const int column = 16 * j + col;

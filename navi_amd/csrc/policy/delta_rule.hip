@@ -70,6 +70,18 @@ __device__ inline f4 gated(f4 x, f4 factor) {
     return y;
 }
 
+// The lane, where the compiler does not see that it has been asked for before: it would hold
+// every address that comes from it in a register of its own from the first step on.
+__device__ inline int fresh_lane() {
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));
+    return lane;
+}
+
+// Keeps the compiler from reading what later steps need from LDS early, into more registers
+// than there are.
+__device__ inline void settle() { __builtin_amdgcn_sched_barrier(0); }
+
 __device__ inline int tokens_of(const RuleParams& P, int chunk) {
     const int64_t left = P.r.steps - static_cast<int64_t>(chunk) * kChunk;
     return static_cast<int>(left < kChunk ? left : kChunk);
@@ -182,30 +194,30 @@ struct Walk {
 
 // u or its gradient from the rows of X, all tiles of a stage side by side.
 template <int N, int NB>
-__device__ inline void times_triangle(const Triangle<N>& t, const u4 (&b)[2][NB], f4 (&x)[4]) {
+__device__ inline void times_triangle(int lane, const Triangle<N>& t, const u4 (&b)[2][NB], f4 (&x)[4]) {
     u4 a[4][N];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) operand_triangle<N>(t, i, 0, a[i]);
+    for (int i = 0; i < 4; ++i) operand_triangle<N>(lane, t, i, 0, a[i]);
     mma_each<4>(a, b[0], x);
     u4 below[2][N];
     f4 y[2] = {x[2], x[3]};
 #pragma unroll
-    for (int i = 0; i < 2; ++i) operand_triangle<N>(t, 2 + i, 1, below[i]);
+    for (int i = 0; i < 2; ++i) operand_triangle<N>(lane, t, 2 + i, 1, below[i]);
     mma_each<2>(below, b[1], y);
     x[2] = y[0];
     x[3] = y[1];
 }
 
 template <int N, int NB>
-__device__ inline void times_transpose(const Triangle<N>& t, const u4 (&b)[2][NB], f4 (&x)[4]) {
+__device__ inline void times_transpose(int lane, const Triangle<N>& t, const u4 (&b)[2][NB], f4 (&x)[4]) {
     u4 a[4][N];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) operand_transpose<N>(t, j, 1, a[j]);
+    for (int j = 0; j < 4; ++j) operand_transpose<N>(lane, t, j, 1, a[j]);
     mma_each<4>(a, b[1], x);
     u4 left[2][N];
     f4 y[2] = {x[0], x[1]};
 #pragma unroll
-    for (int j = 0; j < 2; ++j) operand_transpose<N>(t, j, 0, left[j]);
+    for (int j = 0; j < 2; ++j) operand_transpose<N>(lane, t, j, 0, left[j]);
     mma_each<2>(left, b[0], y);
     x[0] = y[0];
     x[1] = y[1];
@@ -213,13 +225,13 @@ __device__ inline void times_transpose(const Triangle<N>& t, const u4 (&b)[2][NB
 
 // Columns of rows in LDS times b, added to four tiles of a state from tile c on.
 template <int N, int kPitch, int NB, int kCount>
-__device__ inline void add_columns(const uint16_t (&rows)[N][kChunk][kPitch], int c, const u4 (&b)[2][NB], f4 (&state)[kCount]) {
+__device__ inline void add_columns(int lane, const uint16_t (&rows)[N][kChunk][kPitch], int c, const u4 (&b)[2][NB], f4 (&state)[kCount]) {
     f4 x[4] = {state[c], state[c + 1], state[c + 2], state[c + 3]};
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
         u4 a[4][N];
 #pragma unroll
-        for (int n = 0; n < 4; ++n) operand_columns(rows, c + n, m, a[n]);
+        for (int n = 0; n < 4; ++n) operand_columns(lane, rows, c + n, m, a[n]);
         mma_each<4>(a, b[m], x);
     }
 #pragma unroll
@@ -235,7 +247,7 @@ __global__ __launch_bounds__(kThreads) void delta_forward_kernel(RuleParams P) {
     constexpr int N = kPlanes<E>, NP = kOutPlanes<E>;
     extern __shared__ char lds_bytes[];
     auto& lds = *reinterpret_cast<ScanLds<E, KP, NP>*>(lds_bytes);
-    const int wave = wave_of_workgroup(), g = (threadIdx.x & 63) >> 4;
+    const int wave = wave_of_workgroup(), lane = threadIdx.x & 63, g = lane >> 4;
     const int64_t sequence = blockIdx.x;
     const int64_t env = sequence / P.r.value_heads;
     const int head = static_cast<int>(sequence % P.r.value_heads);
@@ -284,13 +296,13 @@ __global__ __launch_bounds__(kThreads) void delta_forward_kernel(RuleParams P) {
                 u4 b[3], a[4][N];
                 split8(state[2 * m], state[2 * m + 1], b);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) operand_rows_as_results(lds.rows.k, 16 * i, m, a[i]);
+                for (int i = 0; i < 4; ++i) operand_rows_as_results(lane, lds.rows.k, 16 * i, m, a[i]);
                 mma_each<4>(a, b, u);
                 if constexpr (!kSummary) {
                     u4 b_out[NP];
                     first_planes(b, b_out);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) operand_rows_as_results(lds.rows.q, 16 * i, m, a[i]);
+                    for (int i = 0; i < 4; ++i) operand_rows_as_results(lane, lds.rows.q, 16 * i, m, a[i]);
                     mma_each<4>(a, b_out, o);
                 }
             }
@@ -309,7 +321,7 @@ __global__ __launch_bounds__(kThreads) void delta_forward_kernel(RuleParams P) {
             }
             split8(x[0], x[1], r[m]);
         }
-        times_triangle<3>(lds.x, r, u);
+        times_triangle<3>(lane, lds.x, r, u);
         if (!kSummary && P.r.updates)
             rows_state.store<4>(rows_state.rows(P.r.updates + (sequence * P.r.steps + t0) * V + first, tokens),
                                 [&](int i, int s) { return u[i][s]; });
@@ -321,12 +333,12 @@ __global__ __launch_bounds__(kThreads) void delta_forward_kernel(RuleParams P) {
 #pragma unroll
         for (int c = 0; c < KP / 16; ++c) state[c] = gated(state[c], f4{keep, keep, keep, keep});
 #pragma unroll
-        for (int c = 0; c < KP / 16; c += 4) add_columns(lds.rows.k, c, r, state);
+        for (int c = 0; c < KP / 16; c += 4) add_columns(lane, lds.rows.k, c, r, state);
         if constexpr (!kSummary) {
             u4 w[2][NP];
 #pragma unroll
             for (int m = 0; m < 2; ++m) split8(u[2 * m], u[2 * m + 1], w[m]);
-            times_triangle<NP>(lds.p, w, o);
+            times_triangle<NP>(lane, lds.p, w, o);
             rows_out.template store<4>(
                 rows_out.rows(static_cast<E*>(P.r.out) + ((env * P.r.steps + t0) * P.r.value_heads + head) * V + first, tokens),
                 [&](int i, int s) { return from_float<E>(o[i][s]); });
@@ -347,7 +359,7 @@ __global__ __launch_bounds__(kThreads) void delta_reverse_kernel(RuleParams P) {
     constexpr int N = kPlanes<E>;
     extern __shared__ char lds_bytes[];
     auto& lds = *reinterpret_cast<ScanLds<E, KP, 3>*>(lds_bytes);
-    const int wave = wave_of_workgroup(), g = (threadIdx.x & 63) >> 4;
+    const int wave = wave_of_workgroup(), lane = threadIdx.x & 63, g = lane >> 4;
     const int64_t sequence = blockIdx.x;
     const int64_t env = sequence / P.r.value_heads;
     const int head = static_cast<int>(sequence % P.r.value_heads);
@@ -398,7 +410,7 @@ __global__ __launch_bounds__(kThreads) void delta_reverse_kernel(RuleParams P) {
                 u4 b[3], a[4][N];
                 split8(dstate[2 * m], dstate[2 * m + 1], b);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) operand_rows_as_results(lds.rows.k, 16 * i, m, a[i]);
+                for (int i = 0; i < 4; ++i) operand_rows_as_results(lane, lds.rows.k, 16 * i, m, a[i]);
                 mma_each<4>(a, b, du);
             }
 #pragma unroll
@@ -408,14 +420,14 @@ __global__ __launch_bounds__(kThreads) void delta_reverse_kernel(RuleParams P) {
             u4 raw[2][N];
 #pragma unroll
             for (int m = 0; m < 2; ++m) split8(dO[2 * m], dO[2 * m + 1], raw[m]);
-            times_transpose<3>(lds.p, raw, du);
+            times_transpose<3>(lane, lds.p, raw, du);
         }
         u4 b[2][3];
 #pragma unroll
         for (int m = 0; m < 2; ++m) split8(du[2 * m], du[2 * m + 1], b[m]);
 #pragma unroll
         for (int j = 0; j < 4; ++j) du[j] = f4{0, 0, 0, 0};
-        times_transpose<3>(lds.x, b, du);  // dr
+        times_transpose<3>(lane, lds.x, b, du);  // dr
         if constexpr (!kSummary) {
             rows_v.template store<4>(
                 rows_v.rows(static_cast<E*>(P.d.d_v) + ((env * P.r.steps + t0) * P.r.value_heads + head) * V + first, tokens),
@@ -436,11 +448,11 @@ __global__ __launch_bounds__(kThreads) void delta_reverse_kernel(RuleParams P) {
 #pragma unroll
             for (int m = 0; m < 2; ++m) split8(du[2 * m], du[2 * m + 1], b[m]);
 #pragma unroll
-            for (int c = 0; c < KP / 16; c += 4) add_columns(lds.rows.k, c, b, dstate);
+            for (int c = 0; c < KP / 16; c += 4) add_columns(lane, lds.rows.k, c, b, dstate);
 #pragma unroll
             for (int m = 0; m < 2; ++m) split8(dO[2 * m], dO[2 * m + 1], b[m]);
 #pragma unroll
-            for (int c = 0; c < KP / 16; c += 4) add_columns(lds.rows.q, c, b, dstate);
+            for (int c = 0; c < KP / 16; c += 4) add_columns(lane, lds.rows.q, c, b, dstate);
         }
     }
     if (walk.to && walk.working) store_state<KP>(rows_state, walk.to + first, K, dstate);
@@ -551,21 +563,62 @@ __device__ inline void store_tiles(T* base, int64_t stride, int rows, int column
 //     dG_last += sum_j beta_j F_j k_j . W_j + E_last <S, dS>,  dg_t = sum_{i >= t} dG_i
 //
 // The same number stands at +i and -j of dG, so what cancels in dg cancels to its rounding.
+//
+// Four waves of 16 tokens each take the terms of do (Y, H, W, N, dq, their part of dk) and those
+// of dr (Z, R, M, the rest of dk), or eight waves one of the two. V is taken 32 columns at a
+// time. With 64 keys of 16 bits three workgroups of four waves fit a CU and hide each other's
+// waits; with more, one or two of eight do (1024 x 128 steps, 4 heads of 64: 299 us with four
+// waves, 430 with eight; 2 x 4001 steps, 8 heads of 128: 165 and 120).
 template <class E, int KP>
+inline constexpr int kGradientWaves = KP == 64 && sizeof(E) == 2 ? 4 : 8;
+
+template <int KP>
+struct GradientStage {
+    uint16_t s[KP / 16][3][64][8], ds[KP / 16][3][64][8];  // 32 columns of S and dS as operands
+    uint16_t u[4][3][64][8];                                // and of u
+};
+
+template <class E, int KP>
+struct GradientTriangles {
+    Triangle<kOutPlanes<E>> n, m;  // (they reach dq and dk alone)
+    float beta_part[4 * kGradientWaves<E, KP>][kChunk], g_part[4 * kGradientWaves<E, KP>][kChunk];
+};
+
+struct GradientRest {
+    ChunkGates gates;
+    float beta_row[kChunk], g_row[2][kChunk], f_row[kChunk], dot_part[8];
+};
+
+template <class E, int KP>
+union GradientRows {
+    ChunkRows<E, KP> rows;
+    f4 exchange[4][KP / 16][64];
+};
+
+// The rows of q and k stay in LDS where a workgroup has the room; else they come after V.
+template <class E, int KP>
+inline constexpr bool kRowsStay = kGradientWaves<E, KP> == 8 && (sizeof(E) == 2 || KP == 64);
+
+template <class E, int KP, bool kStay = kRowsStay<E, KP>>
 struct GradientLds {
     union {
+        GradientStage<KP> stage;
+        GradientTriangles<E, KP> tri;
+    };
+    GradientRows<E, KP> of;
+    GradientRest rest;
+};
+
+template <class E, int KP>
+struct GradientLds<E, KP, false> {
+    union {
+        GradientStage<KP> stage;
         struct {
-            uint16_t s[KP / 16][3][64][8], ds[KP / 16][3][64][8];  // 32 columns of S and dS as operands
-            uint16_t u[4][3][64][8];                                // and of u
-        } stage;
-        struct {
-            ChunkRows<E, KP> rows;
-            Triangle<kOutPlanes<E>> n, m;  // (they reach dq and dk alone)
+            GradientTriangles<E, KP> tri;
+            GradientRows<E, KP> of;
         };
     };
-    ChunkGates gates;
-    float beta_part[16][kChunk], g_part[16][kChunk], beta_row[kChunk], g_row[kChunk], f_row[kChunk];
-    float dot_part[4];
+    GradientRest rest;
 };
 
 __device__ inline float sum16(float x) {  // over 16 lanes in a row
@@ -579,11 +632,11 @@ __device__ inline float sum16(float x) {  // over 16 lanes in a row
     return x;
 }
 
-// Eight numbers of a row from `offset` bytes on: in 16-byte loads where rows are multiples of
-// eight, else one by one, those from `valid` on as zeros.
-template <class T>
-struct Eight {
-    static constexpr int kWords = sizeof(T) == 4 ? 2 : 1;
+// Numbers of a row from `offset` bytes on: in 16-byte loads where rows are multiples of eight,
+// else one by one, those from `valid` on as zeros.
+template <class T, int kCount>
+struct Part {
+    static constexpr int kWords = kCount * sizeof(T) / 16;
     u4 words[kWords];
 
     __device__ void load(Buffer from, uint32_t offset, int valid, bool wide) {
@@ -593,9 +646,9 @@ struct Eight {
             for (int w = 0; w < kWords; ++w) words[w] = buffer_load16(from, lane + 16 * w);
             return;
         }
-        uint32_t x[8];
+        uint32_t x[kCount];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < kCount; ++i) {
             const T y = buffer_load<T>(from, i < valid ? offset + i * sizeof(T) : kOutside);
             if constexpr (sizeof(T) == 4)
                 x[i] = bits_of(y);
@@ -604,13 +657,13 @@ struct Eight {
         }
 #pragma unroll
         for (int i = 0; i < 4 * kWords; ++i)
-            words[i / 4][i % 4] = kWords == 2 ? x[i] : x[2 * i % 8] | x[(2 * i + 1) % 8] << 16;
+            words[i / 4][i % 4] = sizeof(T) == 4 ? x[i] : x[2 * i % kCount] | x[(2 * i + 1) % kCount] << 16;
     }
 
-    __device__ void floats(float (&x)[8]) const {
+    __device__ void floats(float (&x)[kCount]) const {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if constexpr (kWords == 2)
+        for (int i = 0; i < kCount; ++i) {
+            if constexpr (sizeof(T) == 4)
                 x[i] = float_of(words[i / 4][i % 4]);
             else
                 x[i] = to_float(__builtin_bit_cast(T, static_cast<uint16_t>(words[0][i / 2] >> (16 * (i % 2)))));
@@ -618,21 +671,178 @@ struct Eight {
     }
 };
 
-// The inputs of 32 columns of V: of S, dS and u for the workgroup, of do and dr for the wave.
-template <class E, int KP>
-struct GradientFetch {
-    static constexpr int kPieces = KP / 64;
-    Eight<float> s[kPieces], ds[kPieces], u, dr;
-    Eight<E> grad;
+// Four floats into the planes of an operand's lane, its first or second half.
+__device__ inline void stage_part(uint16_t (&tile)[3][64][8], int slot, int half, const float (&x)[4]) {
+    uint32_t a[3], b[3];
+    split_pair<3>(x[0], x[1], a);
+    split_pair<3>(x[2], x[3], b);
+#pragma unroll
+    for (int n = 0; n < 3; ++n) *reinterpret_cast<u2*>(&tile[n][slot][4 * half]) = u2{a[n], b[n]};
+}
+
+__device__ inline void staged_operand(int lane, const uint16_t (&tile)[3][64][8], u4 (&x)[3]) {
+#pragma unroll
+    for (int n = 0; n < 3; ++n) x[n] = *reinterpret_cast<const u4*>(tile[n][lane]);
+}
+
+// A triangle's rows times 32 rows in LDS.
+template <int NP, int N, int kPitch, int kCount>
+__device__ inline void add_products(int lane, const u4 (&a)[NP], const uint16_t (&rows)[N][kChunk][kPitch], int m, f4 (&x)[kCount]) {
+#pragma unroll
+    for (int c = 0; c < kCount; ++c) {
+        u4 b[N];
+        operand_columns(lane, rows, c, m, b);
+        x[c] = mma(a, b, x[c]);
+        if (c % 2) settle();
+    }
+}
+
+// What a wave computes of do's terms (kDo: x is do, y is Y, h is H) or of dr's (dr, Z, R), for
+// the tokens 16 wave on.
+template <class E, int KP, bool kDo>
+struct GradientTerms {
+    static constexpr int N = kPlanes<E>, NP = kOutPlanes<E>, kOwn = kDo ? N : 3;
+    f4 y[KP / 16], h[4], row_sum;
+
+    __device__ void clear() {
+#pragma unroll
+        for (int c = 0; c < KP / 16; ++c) y[c] = f4{0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) h[j] = f4{0, 0, 0, 0};
+    }
+
+    __device__ void products(int lane, int wave, const GradientStage<KP>& stage, bool with_state, const u4 (&x)[kOwn]) {
+        u4 b[3];
+        if (with_state)
+#pragma unroll
+            for (int c = 0; c < KP / 16; ++c) {
+                staged_operand(lane, stage.s[c], b);
+                y[c] = mma(x, b, y[c]);
+                settle();
+            }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (j > wave) continue;
+            staged_operand(lane, stage.u[j], b);
+            h[j] = mma(x, b, h[j]);
+            settle();
+        }
+    }
+
+    __device__ static const auto& left_rows(const ChunkRows<E, KP>& rows) {
+        if constexpr (kDo)
+            return rows.q;
+        else
+            return rows.k;
+    }
+
+    __device__ static auto& triangle(GradientTriangles<E, KP>& tri) {
+        if constexpr (kDo)
+            return tri.n;
+        else
+            return tri.m;
+    }
+
+    // N or M, and the sums over its rows (kept) and columns (parts of the workgroup's sums: with
+    // eight waves M's own, with four N's, which it adds to).
+    __device__ void make_triangle(int lane, int wave, const ChunkRows<E, KP>& rows, const ChunkGates& gates,
+                                  GradientTriangles<E, KP>& tri, float scale) {
+        constexpr bool kAdd = !kDo && kGradientWaves<E, KP> == 4;
+        const int col = lane & 15, g = lane >> 4, row = 16 * wave + 4 * g;
+        const int part = 4 * wave + g + (kDo || kAdd ? 0 : 16);
+        row_sum = f4{0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float beta_sum = 0.0f, g_sum = 0.0f;
+            if (j <= wave) {
+                f4 xk = {0, 0, 0, 0};  // q . k or k . k
+#pragma unroll
+                for (int m = 0; m < KP / 32; ++m) {
+                    u4 a[N], b[N];
+                    operand_rows(lane, rows.k, 16 * j, m, b);
+                    operand_rows(lane, left_rows(rows), 16 * wave, m, a);
+                    xk = mma(a, b, xk);
+                }
+                const int column = 16 * j + col;
+                const float hi = gates.hi[column], lo = gates.lo[column], beta = gates.beta[column];
+                const int episode = gates.episode[column];
+                const float factor = kDo ? scale : -1.0f;
+                f4 n;
+#pragma unroll
+                for (int s = 0; s < 4; ++s) {
+                    const bool below = row + s > column, on = kDo ? row + s >= column : below;
+                    const float d = on ? decay(gates, row + s, hi, lo, episode) : 0.0f;
+                    const float x = on ? factor * d * h[j][s] : 0.0f, xb = x * beta;
+                    n[s] = xb;
+                    const float pair = below ? xb * xk[s] : 0.0f;
+                    beta_sum += on ? x * xk[s] : 0.0f;
+                    g_sum += pair;
+                    row_sum[s] += pair;
+                }
+                store_slot<NP>(triangle(tri), tile_of(wave, j), lane, n);
+                settle();
+            }
+            tri.beta_part[part][16 * j + col] = (kAdd ? tri.beta_part[part][16 * j + col] : 0.0f) + beta_sum;
+            tri.g_part[part][16 * j + col] = (kAdd ? tri.g_part[part][16 * j + col] : 0.0f) + g_sum;
+        }
+    }
+
+    // y becomes scale E Y or -E Z; its product with q or k is added to the sums of rows.
+    __device__ void close_rows(int lane, int wave, const ChunkRows<E, KP>& rows, const ChunkGates& gates, float scale) {
+        const int row = 16 * wave + 4 * (lane >> 4);
+        const f4 e = four(gates.e, row);
+        const float factor = kDo ? scale : -1.0f;
+#pragma unroll
+        for (int c = 0; c < KP / 16; ++c) {
+            y[c] = factor * gated(y[c], e);
+            row_sum = row_sum + row_products(lane, row, left_rows(rows), c, y[c]);
+            settle();
+        }
+    }
+
+    __device__ static f4 row_products(int lane, int row, const uint16_t (&rows)[N][kChunk][KP + 8], int c, f4 x) {
+        f4 product;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            float y = 0.0f;
+#pragma unroll
+            for (int n = N - 1; n >= 0; --n) y += to_float(bf16{rows[n][row + s][16 * c + (lane & 15)]});
+            product[s] = y * x[s];
+        }
+        return product;
+    }
+
+    // dq = y + N k and N^T q into dk; or M k + M^T k into dk = y.
+    __device__ void last_products(int lane, int wave, const ChunkRows<E, KP>& rows, GradientTriangles<E, KP>& tri,
+                                  f4 (&dk)[KP / 16]) {
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            u4 a[NP];
+            if (2 * m <= wave) {
+                operand_triangle<NP>(lane, triangle(tri), wave, m, a);
+                add_products<NP>(lane, a, rows.k, m, y);
+            }
+            if (2 * m + 1 >= wave) {
+                operand_transpose<NP>(lane, triangle(tri), wave, m, a);
+                add_products<NP>(lane, a, left_rows(rows), m, dk);
+            }
+        }
+    }
 };
 
 template <class E, int KP>
-__global__ __launch_bounds__(256, KP == 64 ? 3 : 1) void delta_gradients_kernel(RuleParams P) {
-    constexpr int N = kPlanes<E>, NP = kOutPlanes<E>;
+__global__ __launch_bounds__((64 * kGradientWaves<E, KP>), (kGradientWaves<E, KP> == 4 ? 3 : 2)) void delta_gradients_kernel(RuleParams P) {
+    constexpr int N = kPlanes<E>, kWaves = kGradientWaves<E, KP>;
+    constexpr bool kBoth = kWaves == 4;                      // a wave has both kinds of terms
+    constexpr int kPieces = 8 * KP / (64 * kWaves), kRowsOfU = 8 / kWaves;
+    constexpr int kDown = 8 * kWaves;                        // rows that the workgroup's pieces are of
     extern __shared__ char lds_bytes[];
     auto& lds = *reinterpret_cast<GradientLds<E, KP>*>(lds_bytes);
-    const int lane = threadIdx.x & 63, wave = wave_of_workgroup();
-    const int col = lane & 15, g = lane >> 4;
+    auto& rows = lds.of.rows;
+    const ChunkGates& gates = lds.rest.gates;
+    const int wave = wave_of_workgroup() & 3;
+    const bool of_do = kBoth || wave_of_workgroup() < 4, of_dr = kBoth || !of_do;
+    int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
     const int64_t sequence = blockIdx.x / static_cast<uint32_t>(P.n_chunks);
     const int chunk = static_cast<int>(blockIdx.x % static_cast<uint32_t>(P.n_chunks));
     const int64_t env = sequence / P.r.value_heads;
@@ -653,189 +863,161 @@ __global__ __launch_bounds__(256, KP == 64 ? 3 : 1) void delta_gradients_kernel(
     const Buffer from_dr = buffer_of(P.rgrads + rows_at, tokens * row_bytes);
     const Buffer from_grad = buffer_of(at<E>(P.d.grad_out, P.d.grad_out_stride, env, t0, head),
                                        (tokens - 1) * grad_row_bytes + V * sizeof(E));
-    const int piece_row = threadIdx.x >> 2, piece_column = (threadIdx.x & 3) * 8;
+    const int piece_row = threadIdx.x >> 3, piece_column = (threadIdx.x & 7) * 4;
+    const int slot = (piece_row & 15) + 16 * ((threadIdx.x & 7) >> 1), half = threadIdx.x & 1;
     const int my_token = 16 * wave + col;  // of the wave's tile of tokens, as an operand's row
 
-    GradientFetch<E, KP> next;
+    Part<float, 4> next_s[kPieces], next_ds[kPieces], next_u[kRowsOfU];
+    Part<float, 8> next_dr;
+    Part<E, 8> next_do;
     const auto fetch = [&](int v0) {
         const int c = v0 + piece_column;
 #pragma unroll
-        for (int i = 0; i < KP / 64; ++i) {
-            const uint32_t offset = (piece_row + 64 * i) * row_bytes + 4 * c;
-            const int valid = piece_row + 64 * i < K ? V - c : 0;
-            if (S) next.s[i].load(from_s, offset, valid, P.wide_state);
-            if (dS) next.ds[i].load(from_ds, offset, valid, P.wide_state);
+        for (int i = 0; i < kPieces; ++i) {
+            const int row = piece_row + kDown * i, valid = row < K ? V - c : 0;
+            if (S) next_s[i].load(from_s, row * row_bytes + 4 * c, valid, P.wide_state);
+            if (dS) next_ds[i].load(from_ds, row * row_bytes + 4 * c, valid, P.wide_state);
         }
-        next.u.load(from_u, piece_row * row_bytes + 4 * c, piece_row < tokens ? V - c : 0, P.wide_state);
+#pragma unroll
+        for (int i = 0; i < kRowsOfU; ++i) {
+            const int row = piece_row + kDown * i;
+            next_u[i].load(from_u, row * row_bytes + 4 * c, row < tokens ? V - c : 0, P.wide_state);
+        }
         const int valid = my_token < tokens ? V - v0 - 8 * g : 0;
-        next.dr.load(from_dr, my_token * row_bytes + 4 * (v0 + 8 * g), valid, P.wide_state);
-        next.grad.load(from_grad, my_token * grad_row_bytes + (v0 + 8 * g) * sizeof(E), valid, P.wide_do);
+        if (of_do) next_do.load(from_grad, my_token * grad_row_bytes + (v0 + 8 * g) * sizeof(E), valid, P.wide_do);
+        if (of_dr) next_dr.load(from_dr, my_token * row_bytes + 4 * (v0 + 8 * g), valid, P.wide_state);
     };
     fetch(0);
-    if (wave == 0) load_gates(P, lds.gates, env, head, t0, tokens);
-    f4 y[KP / 16], z[KP / 16], w[KP / 16], h[4], rr[4];
+    if (wave_of_workgroup() == kWaves - 1) load_gates(P, lds.rest.gates, env, head, t0, tokens);
+    if constexpr (kRowsStay<E, KP>) load_rows<E, KP>(P, rows, env, head, t0, tokens);
+    // With eight waves, those of dr use the registers of do's terms
+    GradientTerms<E, KP, true> terms;
+    GradientTerms<E, KP, false> others;
+    const auto as_dr = [&]() -> GradientTerms<E, KP, false>& {
+        if constexpr (kBoth)
+            return others;
+        else
+            return reinterpret_cast<GradientTerms<E, KP, false>&>(terms);
+    };
+    f4 w[KP / 16];
+    terms.clear();
+    if constexpr (kBoth) others.clear();
 #pragma unroll
-    for (int c = 0; c < KP / 16; ++c) y[c] = z[c] = w[c] = f4{0, 0, 0, 0};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) h[j] = rr[j] = f4{0, 0, 0, 0};
+    for (int c = 0; c < KP / 16; ++c) w[c] = f4{0, 0, 0, 0};
     float dot = 0.0f;
     for (int v0 = 0; v0 < V; v0 += 32) {
         if (v0 > 0) __syncthreads();
-        float a[8], b[8];
-        u4 plane[3];
+        float a[4], x[8];
 #pragma unroll
-        for (int i = 0; i < KP / 64; ++i) {
-            const int tile = (piece_row >> 4) + 4 * i, slot = (piece_row & 15) + 16 * (threadIdx.x & 3);
+        for (int i = 0; i < kPieces; ++i) {
+            const int tile = (piece_row + kDown * i) >> 4;
             if (S) {
-                next.s[i].floats(a);
-                split8(a, plane);
-#pragma unroll
-                for (int n = 0; n < 3; ++n) *reinterpret_cast<u4*>(lds.stage.s[tile][n][slot]) = plane[n];
+                next_s[i].floats(a);
+                stage_part(lds.stage.s[tile], slot, half, a);
             }
             if (dS) {
-                next.ds[i].floats(b);
-                split8(b, plane);
+                next_ds[i].floats(a);
+                stage_part(lds.stage.ds[tile], slot, half, a);
+                if (S)
 #pragma unroll
-                for (int n = 0; n < 3; ++n) *reinterpret_cast<u4*>(lds.stage.ds[tile][n][slot]) = plane[n];
+                    for (int n = 0; n < 4; ++n) dot += float_of(next_s[i].words[0][n]) * a[n];
             }
-            if (S && dS)
-#pragma unroll
-                for (int n = 0; n < 8; ++n) dot += a[n] * b[n];
         }
-        next.u.floats(a);
-        split8(a, plane);
 #pragma unroll
-        for (int n = 0; n < 3; ++n)
-            *reinterpret_cast<u4*>(lds.stage.u[piece_row >> 4][n][(piece_row & 15) + 16 * (threadIdx.x & 3)]) = plane[n];
-        u4 a_do[N], a_dr[3], a_u[3];
-        next.grad.floats(a);
-        split8(a, a_do);
-        next.dr.floats(a);
-        split8(a, a_dr);
+        for (int i = 0; i < kRowsOfU; ++i) {
+            next_u[i].floats(a);
+            stage_part(lds.stage.u[(piece_row + kDown * i) >> 4], slot, half, a);
+        }
+        u4 a_do[N], a_dr[3];
+        if (of_do) {
+            next_do.floats(x);
+            split8(x, a_do);
+        }
+        if (of_dr) {
+            next_dr.floats(x);
+            split8(x, a_dr);
+        }
         __syncthreads();
         if (v0 + 32 < V) fetch(v0 + 32);
-        if (dS) {
-#pragma unroll
-            for (int n = 0; n < 3; ++n) a_u[n] = *reinterpret_cast<const u4*>(lds.stage.u[wave][n][lane]);
-        }
-#pragma unroll
-        for (int c = 0; c < KP / 16; ++c) {
-            u4 x[3];
-            if (S) {
-#pragma unroll
-                for (int n = 0; n < 3; ++n) x[n] = *reinterpret_cast<const u4*>(lds.stage.s[c][n][lane]);
-                y[c] = mma(a_do, x, y[c]);
-                z[c] = mma(a_dr, x, z[c]);
-            }
+        settle();
+        if (of_dr) as_dr().products(lane, wave, lds.stage, S, a_dr);
+        if (of_do) {
+            terms.products(lane, wave, lds.stage, S, a_do);
             if (dS) {
+                u4 a_u[3], b[3];
+                staged_operand(lane, lds.stage.u[wave], a_u);
 #pragma unroll
-                for (int n = 0; n < 3; ++n) x[n] = *reinterpret_cast<const u4*>(lds.stage.ds[c][n][lane]);
-                w[c] = mma(a_u, x, w[c]);
+                for (int c = 0; c < KP / 16; ++c) {
+                    staged_operand(lane, lds.stage.ds[c], b);
+                    w[c] = mma(a_u, b, w[c]);
+                    settle();
+                }
             }
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (j > wave) continue;
-            u4 x[3];
-#pragma unroll
-            for (int n = 0; n < 3; ++n) x[n] = *reinterpret_cast<const u4*>(lds.stage.u[j][n][lane]);
-            h[j] = mma(a_do, x, h[j]);
-            rr[j] = mma(a_dr, x, rr[j]);
         }
     }
     dot = sum16(dot);
     dot += __shfl_xor(dot, 16);
     dot += __shfl_xor(dot, 32);
-    if (lane == 0) lds.dot_part[wave] = dot;
+    if (lane == 0) lds.rest.dot_part[threadIdx.x >> 6] = dot;
     __syncthreads();
-    load_rows<E, KP>(P, lds.rows, env, head, t0, tokens);
-    __syncthreads();
+    if constexpr (!kRowsStay<E, KP>) {
+        load_rows<E, KP>(P, rows, env, head, t0, tokens);
+        __syncthreads();
+    }
 
     // The triangles N and M; the sums over their rows and columns.
+    lane = fresh_lane(), col = lane & 15, g = lane >> 4;
     const int row = 16 * wave + 4 * g;
-    f4 row_sum = {0, 0, 0, 0};
+    if (of_do) {
+        terms.make_triangle(lane, wave, rows, gates, lds.tri, P.r.scale);
+        terms.close_rows(lane, wave, rows, gates, P.r.scale);
+        const f4 f = four(gates.f, row), beta = four(gates.beta, row);
+        f4 kw = {0, 0, 0, 0};
+        if (dS)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        float beta_sum = 0.0f, g_sum = 0.0f;
-        if (j <= wave) {
-            f4 kk = {0, 0, 0, 0}, qk = {0, 0, 0, 0};
-#pragma unroll
-            for (int m = 0; m < KP / 32; ++m) {
-                u4 a[N], b[N];
-                operand_rows(lds.rows.k, 16 * j, m, b);
-                operand_rows(lds.rows.k, 16 * wave, m, a);
-                kk = mma(a, b, kk);
-                operand_rows(lds.rows.q, 16 * wave, m, a);
-                qk = mma(a, b, qk);
+            for (int c = 0; c < KP / 16; ++c) {
+                kw = kw + terms.row_products(lane, row, rows.k, c, w[c]);
+                w[c] = beta * f * w[c];
+                settle();
             }
-            const int column = 16 * j + col;
-            const float hi = lds.gates.hi[column], lo = lds.gates.lo[column], beta = lds.gates.beta[column];
-            const int episode = lds.gates.episode[column];
-            f4 n, mm;
-#pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                const bool below = row + s > column, on = row + s >= column;
-                const float d = on ? decay(lds.gates, row + s, hi, lo, episode) : 0.0f;
-                const float ph = P.r.scale * d * h[j][s];
-                const float rd = below ? rr[j][s] * d : 0.0f;
-                n[s] = on ? ph * beta : 0.0f;
-                mm[s] = -rd * beta;
-                const float pair = below ? n[s] * qk[s] + mm[s] * kk[s] : 0.0f;
-                beta_sum += on ? ph * qk[s] - rd * kk[s] : 0.0f;
-                g_sum += pair;
-                row_sum[s] += pair;
-            }
-            store_slot<NP>(lds.n, tile_of(wave, j), lane, n);
-            store_slot<NP>(lds.m, tile_of(wave, j), lane, mm);
-        }
-        lds.beta_part[4 * wave + g][16 * j + col] = beta_sum;
-        lds.g_part[4 * wave + g][16 * j + col] = g_sum;
-    }
-    const f4 e = four(lds.gates.e, row), f = four(lds.gates.f, row), beta = four(lds.gates.beta, row);
-    f4 qy = {0, 0, 0, 0}, kz = {0, 0, 0, 0}, kw = {0, 0, 0, 0};
-#pragma unroll
-    for (int c = 0; c < KP / 16; ++c) {
-        y[c] = P.r.scale * gated(y[c], e);
-        z[c] = gated(z[c], e);
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-            float qx = 0.0f, kx = 0.0f;
-#pragma unroll
-            for (int n = N - 1; n >= 0; --n) {
-                qx += to_float(bf16{lds.rows.q[n][row + s][16 * c + col]});
-                kx += to_float(bf16{lds.rows.k[n][row + s][16 * c + col]});
+            const float own = sum16(terms.row_sum[s]), left = f[s] * sum16(kw[s]);
+            if (col == 0) {
+                lds.rest.g_row[0][row + s] = own - beta[s] * left;
+                lds.rest.beta_row[row + s] = left;
+                lds.rest.f_row[row + s] = beta[s] * left;
             }
-            qy[s] += qx * y[c][s];
-            kz[s] += kx * z[c][s];
-            kw[s] += kx * w[c][s];
         }
-        z[c] = beta * f * w[c] - z[c];  // dk's part
     }
+    if (of_dr) {
+        as_dr().make_triangle(lane, wave, rows, gates, lds.tri, P.r.scale);
+        as_dr().close_rows(lane, wave, rows, gates, P.r.scale);
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-        const float own = sum16(row_sum[s] + qy[s] - kz[s]), left = f[s] * sum16(kw[s]);
-        if (col == 0) {
-            lds.beta_row[row + s] = left;
-            lds.f_row[row + s] = beta[s] * left;
-            lds.g_row[row + s] = own - beta[s] * left;
+        for (int s = 0; s < 4; ++s) {
+            const float own = sum16(as_dr().row_sum[s]);
+            if (col == 0) lds.rest.g_row[1][row + s] = own;
         }
     }
     __syncthreads();
-    if (wave == 0) {
-        float dbeta = lds.beta_row[lane], dG = lds.g_row[lane], f_all = lds.f_row[lane];
+    if (wave_of_workgroup() == 0) {
+        float dbeta = lds.rest.beta_row[lane], dG = lds.rest.g_row[0][lane] + lds.rest.g_row[1][lane];
+        float f_all = lds.rest.f_row[lane];
 #pragma unroll
-        for (int n = 0; n < 16; ++n) {
-            dbeta += lds.beta_part[n][lane];
-            dG -= lds.g_part[n][lane];
+        for (int n = 0; n < 4 * kWaves; ++n) {
+            dbeta += lds.tri.beta_part[n][lane];
+            dG -= lds.tri.g_part[n][lane];
         }
         f_all = sum16(f_all);
         f_all += __shfl_xor(f_all, 16);
         f_all += __shfl_xor(f_all, 32);
         if (lane == 63) {
-            const float keep = lds.gates.e[63];
+            const float keep = gates.e[63];
             dG += f_all;
-            if (keep != 0.0f)
-                dG += keep * ((lds.dot_part[0] + lds.dot_part[1]) + (lds.dot_part[2] + lds.dot_part[3]));
+            float all = 0.0f;
+#pragma unroll
+            for (int n = 0; n < kWaves; ++n) all += lds.rest.dot_part[n];
+            if (keep != 0.0f) dG += keep * all;
         }
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) {
@@ -843,53 +1025,40 @@ __global__ __launch_bounds__(256, KP == 64 ? 3 : 1) void delta_gradients_kernel(
             dG += lane + d < 64 ? later : 0.0f;
         }
         if (lane < tokens) {
-            const int before = lane > 0 ? lds.gates.episode[lane - 1] : 0;
+            const int before = lane > 0 ? gates.episode[lane - 1] : 0;
             const int64_t to = (env * P.r.steps + t0 + lane) * P.r.value_heads + head;
-            P.d.d_g[to] = lds.gates.episode[lane] != before ? 0.0f : dG;
+            P.d.d_g[to] = gates.episode[lane] != before ? 0.0f : dG;
             P.d.d_beta[to] = dbeta;
         }
     }
 
-    // dq (in y) and dk (in z).
+    lane = fresh_lane();
+    if (of_do) terms.last_products(lane, wave, rows, lds.tri, w);
+    if (of_dr) as_dr().last_products(lane, wave, rows, lds.tri, as_dr().y);
+    if constexpr (kBoth) {
 #pragma unroll
-    for (int m = 0; m < 2; ++m) {
-        const bool left = 2 * m <= wave, below = 2 * m + 1 >= wave;
-        u4 n_left[NP], m_left[NP], n_below[NP], m_below[NP];
-        if (left) {
-            operand_triangle<NP>(lds.n, wave, m, n_left);
-            operand_triangle<NP>(lds.m, wave, m, m_left);
-        }
-        if (below) {
-            operand_transpose<NP>(lds.n, wave, m, n_below);
-            operand_transpose<NP>(lds.m, wave, m, m_below);
-        }
+        for (int c = 0; c < KP / 16; ++c) w[c] = w[c] + others.y[c];
+    } else {
+        __syncthreads();  // the rows are done with: do's part of dk goes to the waves that have dr's
+        if (of_do)
 #pragma unroll
-        for (int c = 0; c < KP / 16; ++c) {
-            u4 b[N];
-            operand_columns(lds.rows.k, c, m, b);
-            if (left) {
-                y[c] = mma(n_left, b, y[c]);
-                z[c] = mma(m_left, b, z[c]);
-            }
-            if (below) {
-                z[c] = mma(m_below, b, z[c]);
-                operand_columns(lds.rows.q, c, m, b);
-                z[c] = mma(n_below, b, z[c]);
-            }
-        }
+            for (int c = 0; c < KP / 16; ++c) lds.of.exchange[wave][c][lane] = w[c];
+        __syncthreads();
+        if (of_dr)
+#pragma unroll
+            for (int c = 0; c < KP / 16; ++c) w[c] = terms.y[c] + lds.of.exchange[wave][c][lane];
     }
     const int left = tokens - 16 * wave;  // rows of the wave's tile
     if (left <= 0) return;
+    const int64_t token = env * P.r.steps + t0 + 16 * wave;
     if (P.group == 1) {
-        const int64_t to = ((env * P.r.steps + t0 + 16 * wave) * P.r.key_heads + head) * K;
-        const int64_t stride = static_cast<int64_t>(P.r.key_heads) * K;
-        store_tiles<E, KP>(static_cast<E*>(P.d.d_q) + to, stride, left, K, y);
-        store_tiles<E, KP>(static_cast<E*>(P.d.d_k) + to, stride, left, K, z);
+        const int64_t to = (token * P.r.key_heads + head) * K, stride = static_cast<int64_t>(P.r.key_heads) * K;
+        if (of_do) store_tiles<E, KP>(static_cast<E*>(P.d.d_q) + to, stride, left, K, terms.y);
+        if (of_dr) store_tiles<E, KP>(static_cast<E*>(P.d.d_k) + to, stride, left, K, w);
     } else {
-        const int64_t to = ((env * P.r.steps + t0 + 16 * wave) * P.r.value_heads + head) * K;
-        const int64_t stride = static_cast<int64_t>(P.r.value_heads) * K;
-        store_tiles<float, KP>(P.dq_heads + to, stride, left, K, y);
-        store_tiles<float, KP>(P.dk_heads + to, stride, left, K, z);
+        const int64_t to = (token * P.r.value_heads + head) * K, stride = static_cast<int64_t>(P.r.value_heads) * K;
+        if (of_do) store_tiles<float, KP>(P.dq_heads + to, stride, left, K, terms.y);
+        if (of_dr) store_tiles<float, KP>(P.dk_heads + to, stride, left, K, w);
     }
 }
 
@@ -978,7 +1147,7 @@ int backward(const RuleParams& P, hipStream_t stream) {
     int code = walk_all<E, KP, true>(P, stream);
     if (code != NAVI_POLICY_OK) return code;
     hipLaunchKernelGGL((delta_gradients_kernel<E, KP>), dim3(static_cast<unsigned>(P.r.envs * P.r.value_heads * P.n_chunks)),
-                       dim3(256), sizeof(GradientLds<E, KP>), stream, P);
+                       dim3(64 * kGradientWaves<E, KP>), sizeof(GradientLds<E, KP>), stream, P);
     code = launched("navi_delta_backward");
     if (code != NAVI_POLICY_OK || P.group == 1) return code;
     const int64_t count = P.r.envs * P.r.steps * P.r.key_heads * P.r.key_dim;
