@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from pathlib import Path
 
 LIB_DIR = Path(__file__).resolve().parent / "_lib"
@@ -63,24 +64,30 @@ class QkNorm(ctypes.Structure):
                 ("d_q_weight", _vp), ("d_k_weight", _vp), ("partial", _vp)]
 
 
+def _packer(structure) -> struct.Struct:
+    """The structure's fields in order as a packer of plain numbers (an array's one by one): a
+    call's arguments in one step, a fifth of the time that setting the fields takes."""
+    codes = {_i32: "i", _i64: "q", _f32: "f", _vp: "P", _three: "3q", _two: "2q"}
+    packer = struct.Struct("@" + "".join(codes[kind] for _, kind in structure._fields_) + "0q")
+    assert packer.size == ctypes.sizeof(structure)
+    return packer
+
+
+PACK_RULE, PACK_GRADIENTS, PACK_NORM = (_packer(s).pack for s in (DeltaRule, DeltaGradients, QkNorm))
+
 _lib.navi_policy_last_error.restype = ctypes.c_char_p
 _lib.navi_policy_last_error.argtypes = []
-for _name in ("navi_delta_forward", "navi_delta_step"):
+# (structures as bytes or by reference)
+for _name in ("navi_delta_forward", "navi_delta_step", "navi_qk_norm", "navi_qk_norm_backward"):
     getattr(_lib, _name).restype = ctypes.c_int
-    getattr(_lib, _name).argtypes = [ctypes.POINTER(DeltaRule), _vp]
-for _name in ("navi_delta_scratch", "navi_delta_workspace"):
+    getattr(_lib, _name).argtypes = [_vp, _vp]
+for _name in ("navi_delta_scratch", "navi_delta_workspace", "navi_qk_norm_workspace"):
     getattr(_lib, _name).restype = _i64
-    getattr(_lib, _name).argtypes = [ctypes.POINTER(DeltaRule)]
+    getattr(_lib, _name).argtypes = [_vp]
 _lib.navi_delta_backward.restype = ctypes.c_int
-_lib.navi_delta_backward.argtypes = [ctypes.POINTER(DeltaRule), ctypes.POINTER(DeltaGradients), _vp]
-for _name in ("navi_qk_norm", "navi_qk_norm_backward"):
-    getattr(_lib, _name).restype = ctypes.c_int
-    getattr(_lib, _name).argtypes = [ctypes.POINTER(QkNorm), _vp]
-_lib.navi_qk_norm_workspace.restype = _i64
-_lib.navi_qk_norm_workspace.argtypes = [ctypes.POINTER(QkNorm)]
+_lib.navi_delta_backward.argtypes = [_vp, _vp, _vp]
 _lib.navi_clip_grad_norm.restype = ctypes.c_int
-_lib.navi_clip_grad_norm.argtypes = [_i32, ctypes.POINTER(_vp), ctypes.POINTER(_vp), ctypes.POINTER(_i64),
-                                     ctypes.POINTER(_i32), _f32, _f32, _vp, _vp, _vp]
+_lib.navi_clip_grad_norm.argtypes = [_i32, _vp, _vp, _vp, _vp, _f32, _f32, _vp, _vp, _vp]
 
 
 def lib() -> ctypes.CDLL:

@@ -19,8 +19,8 @@ axis's). Misuse raises ``RuntimeError``; there is no CPU fallback.
 
 from __future__ import annotations
 
-import ctypes
 import math
+import struct
 from typing import Iterable
 
 import torch
@@ -32,6 +32,9 @@ __all__ = ["gated_delta_rule", "gated_delta_step", "qk_norm", "clip_grad_norm"]
 
 _DTYPES = {torch.float32: _native.F32, torch.bfloat16: _native.BF16, torch.float16: _native.F16}
 _MASKS = (torch.bool, torch.uint8)
+
+# Arguments are looked over twice: `_fine` in one expression on every call (a call of one frame
+# is bound by the host), and by name, for the message, where that found something.
 
 
 def _check(cond: bool, msg: str) -> None:
@@ -50,25 +53,52 @@ def _dense_last(t: torch.Tensor) -> bool:
     return t.stride(-1) == 1 or t.size(-1) <= 1
 
 
-def _stream(device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+def _call(function, device: torch.device, *args) -> None:
+    """An entry point on the device's current stream."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        code = function(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            code = function(*args, torch._C._cuda_getCurrentRawStream(index))
+    if code:
+        _native.check(code)
 
 
-def _ptr(t) -> int | None:
-    return None if t is None else t.data_ptr()
+def _ptr(t) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
-def _written(t: torch.Tensor) -> None:
-    """Tells autograd of a write by a kernel."""
-    if not t.is_inference():
-        torch.autograd.graph.increment_version(t)
+def _written(tensors: list[torch.Tensor]) -> None:
+    """Tells autograd of writes by a kernel."""
+    tensors = [t for t in tensors if not t.is_inference()]
+    if tensors:
+        torch.autograd.graph.increment_version(tensors)
 
 
 # ---- the gated delta rule ----
 
 
+def _fine_rule(q, k, v, g, beta, starts) -> bool:
+    """Whether the inputs are in order ([Envs, Steps, ...] and [Envs, ...] alike)."""
+    try:
+        lead, device, dtype = q.shape[:-2], q.device, q.dtype
+        (hk, kd), (hv, vd) = q.shape[-2:], v.shape[-2:]
+        return (dtype in _DTYPES and k.dtype is dtype and v.dtype is dtype and device.type == "cuda"
+                and k.device == device and v.device == device and g.device == device and beta.device == device
+                and g.dtype is torch.float32 and beta.dtype is torch.float32 and k.shape == q.shape
+                and v.shape[:-2] == lead and g.shape == v.shape[:-1] and beta.shape == g.shape
+                and 0 < hk <= hv and hv % hk == 0 and 0 < kd <= _native.MAX_KEY_DIM and vd > 0
+                and (q.stride(-1) == 1 or kd == 1) and (k.stride(-1) == 1 or kd == 1) and (v.stride(-1) == 1 or vd == 1)
+                and (starts is None or (starts.dtype in _MASKS and starts.device == device and starts.shape == lead)))
+    except (AttributeError, TypeError, ValueError, IndexError):
+        return False
+
+
 def _check_rule(q, k, v, g, beta, starts, lead: tuple[str, ...]) -> None:
     n = len(lead)
+    if _fine_rule(q, k, v, g, beta, starts) and q.dim() == n + 2:
+        return
     shape = ", ".join(lead)
     _check_tensor("q", q, tuple(_DTYPES), n + 2)
     for name, t in (("k", k), ("v", v)):
@@ -88,13 +118,17 @@ def _check_rule(q, k, v, g, beta, starts, lead: tuple[str, ...]) -> None:
     if starts is not None:
         _check_tensor("starts", starts, _MASKS, n, q.device)
         _check(starts.shape == q.shape[:n], f"starts must be [{shape}]")
+    raise RuntimeError("q, k, v, g, beta and starts do not go together")
 
 
-def _check_state(name: str, state, q, v, envs: int) -> None:
+def _check_state(name: str, state, q, v) -> None:
+    want = (q.size(0), v.size(-2), q.size(-1), v.size(-1))
+    if (isinstance(state, torch.Tensor) and state.dtype is torch.float32 and state.device == q.device
+            and state.shape == want and state.is_contiguous()):
+        return
     _check_tensor(name, state, (torch.float32,), 4, q.device)
-    want = (envs, v.size(-2), q.size(-1), v.size(-1))
     _check(tuple(state.shape) == want, f"{name} must be [Envs, ValueHeads, KeyDim, ValueDim] = {list(want)}")
-    _check(state.is_contiguous(), f"{name} must be contiguous")
+    raise RuntimeError(f"{name} must be contiguous")
 
 
 _FARTHEST = ((1 << 31) - 1) // _native.CHUNK - (1 << 18)  # bytes between steps that the chunked kernels reach
@@ -108,45 +142,38 @@ def _rows_apart(t: torch.Tensor) -> torch.Tensor:
     return t.contiguous()
 
 
-def _strides(t: torch.Tensor, step: bool) -> ctypes.Array:
-    s = t.stride()
-    return (ctypes.c_int64 * 3)(s[0], s[1], s[2]) if step else (ctypes.c_int64 * 3)(s[0], 0, s[1])
-
-
-def _rule_args(q, k, v, g, beta, starts, scale, initial_state, out, final_state, step=True) -> _native.DeltaRule:
-    a = _native.DeltaRule(
-        dtype=_DTYPES[q.dtype], key_heads=q.size(-2), value_heads=v.size(-2), key_dim=q.size(-1),
-        value_dim=v.size(-1), envs=q.size(0), steps=q.size(1) if step else 1, scale=scale, q=q.data_ptr(),
-        k=k.data_ptr(), v=v.data_ptr(), q_stride=_strides(q, step), k_stride=_strides(k, step),
-        v_stride=_strides(v, step), g=g.data_ptr(), beta=beta.data_ptr(), g_stride=_strides(g, step),
-        beta_stride=_strides(beta, step), initial_state=_ptr(initial_state), out=_ptr(out),
-        final_state=_ptr(final_state))
-    if starts is not None:
-        a.starts = starts.data_ptr()
-        a.starts_stride = (ctypes.c_int64 * 2)(starts.stride(0), starts.stride(1) if step else 0)
-    return a
+def _pack_rule(q, k, v, g, beta, starts, scale, initial_state, out, final_state, matrices=None, scratch=None, states=None,
+               updates=None) -> bytes:
+    envs, steps, key_heads, key_dim = q.shape
+    value_heads, value_dim = v.shape[2:]
+    return _native.PACK_RULE(
+        _DTYPES[q.dtype], key_heads, value_heads, key_dim, value_dim, envs, steps, scale,
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
+        g.data_ptr(), beta.data_ptr(), *g.stride(), *beta.stride(),
+        *((0, 0, 0) if starts is None else (starts.data_ptr(), *starts.stride())),
+        _ptr(initial_state), out.data_ptr(), _ptr(final_state), _ptr(matrices), _ptr(scratch), _ptr(states), _ptr(updates))
 
 
 def _forward(q, k, v, g, beta, starts, scale, initial_state, return_state, save):
     """(out, final state or None, matrices, states, updates): the last three for a backward pass."""
     envs, steps, heads, dim = v.shape
-    out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
-    state = states = updates = None
+    device, key_dim, chunks = v.device, q.size(3), -(-steps // _native.CHUNK)
+    floats = dict(dtype=torch.float32, device=device)
+    out = torch.empty(v.shape, dtype=v.dtype, device=device)
+    state = states = updates = scratch = None
     if return_state:
-        state = torch.empty((envs, heads, q.size(-1), dim), dtype=torch.float32, device=v.device)
-    chunks = -(-steps // _native.CHUNK)
-    matrices = torch.empty((envs * heads, chunks, _native.CHUNK_MATRICES), dtype=torch.float32, device=v.device)
+        state = torch.empty((envs, heads, key_dim, dim), **floats)
+    matrices = torch.empty((envs * heads, chunks, _native.CHUNK_MATRICES), **floats)
     if save:
-        states = torch.empty((envs * heads, max(0, chunks - 1), q.size(-1), dim), dtype=torch.float32, device=v.device)
-        updates = torch.empty((envs * heads, steps, dim), dtype=torch.float32, device=v.device)
-    a = _rule_args(q, k, v, g, beta, starts, scale, initial_state, out, state)
-    a.matrices, a.states, a.updates = matrices.data_ptr(), _ptr(states), _ptr(updates)
-    scratch = _native.check(_native.lib().navi_delta_scratch(ctypes.byref(a)))
-    if scratch:
-        scratch = torch.empty(scratch // 4, dtype=torch.float32, device=v.device)
-        a.scratch = scratch.data_ptr()
-    with torch.cuda.device(q.device):
-        _native.check(_native.lib().navi_delta_forward(ctypes.byref(a), _stream(q.device)))
+        states = torch.empty((envs * heads, max(0, chunks - 1), key_dim, dim), **floats)
+        updates = torch.empty((envs * heads, steps, dim), **floats)
+    args = (q, k, v, g, beta, starts, scale, initial_state, out, state, matrices)
+    rule = _pack_rule(*args, None, states, updates)
+    size = _native.check(_native.lib().navi_delta_scratch(rule))
+    if size:
+        scratch = torch.empty(size // 4, **floats)
+        rule = _pack_rule(*args, scratch, states, updates)
+    _call(_native.lib().navi_delta_forward, device, rule)
     return out, state, matrices, states, updates
 
 
@@ -172,23 +199,21 @@ class _DeltaRule(torch.autograd.Function):
         grad_out = _rows_apart(grad_out)
         if grad_state is not None:
             grad_state = grad_state.contiguous()
-        d_q, d_k, d_v, d_g, d_beta = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v, g, beta))
+        device = q.device
+        d_q, d_k, d_v, d_g, d_beta = (torch.empty(t.shape, dtype=t.dtype, device=device) for t in (q, k, v, g, beta))
         d_state = torch.empty_like(initial_state) if initial_state is not None and ctx.needs_input_grad[5] else None
         if v.numel() == 0:
             if d_state is not None:
                 d_state = torch.zeros_like(d_state) if grad_state is None else grad_state.clone()
             return d_q, d_k, d_v, d_g, d_beta, d_state, None, None, None
-        a = _rule_args(q, k, v, g, beta, starts, ctx.scale, initial_state, grad_out, None)
-        a.matrices, a.states, a.updates = matrices.data_ptr(), states.data_ptr(), updates.data_ptr()
+        rule = _pack_rule(q, k, v, g, beta, starts, ctx.scale, initial_state, grad_out, None, matrices, None, states, updates)
         lib = _native.lib()
-        size = _native.check(lib.navi_delta_workspace(ctypes.byref(a)))
-        workspace = torch.empty(size // 4, dtype=torch.float32, device=q.device)
-        d = _native.DeltaGradients(
-            grad_out=grad_out.data_ptr(), grad_out_stride=_strides(grad_out, True), grad_final_state=_ptr(grad_state),
-            d_q=d_q.data_ptr(), d_k=d_k.data_ptr(), d_v=d_v.data_ptr(), d_g=d_g.data_ptr(), d_beta=d_beta.data_ptr(),
-            d_initial_state=_ptr(d_state), workspace=workspace.data_ptr())
-        with torch.cuda.device(q.device):
-            _native.check(lib.navi_delta_backward(ctypes.byref(a), ctypes.byref(d), _stream(q.device)))
+        size = _native.check(lib.navi_delta_workspace(rule))
+        workspace = torch.empty(size // 4, dtype=torch.float32, device=device)
+        gradients = _native.PACK_GRADIENTS(
+            grad_out.data_ptr(), *grad_out.stride()[:3], _ptr(grad_state), d_q.data_ptr(), d_k.data_ptr(), d_v.data_ptr(),
+            d_g.data_ptr(), d_beta.data_ptr(), _ptr(d_state), workspace.data_ptr())
+        _call(lib.navi_delta_backward, device, rule, gradients)
         return d_q, d_k, d_v, d_g, d_beta, d_state, None, None, None
 
 
@@ -215,10 +240,11 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     """
     _check_rule(q, k, v, g, beta, starts, ("Envs", "Steps"))
     if initial_state is not None:
-        _check_state("initial_state", initial_state, q, v, q.size(0))
+        _check_state("initial_state", initial_state, q, v)
     scale = q.size(-1) ** -0.5 if scale is None else float(scale)
-    q, k, v = (_rows_apart(t) for t in (q, k, v))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, g, beta, initial_state)):
+    q, k, v = _rows_apart(q), _rows_apart(k), _rows_apart(v)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad
+                                    or beta.requires_grad or (initial_state is not None and initial_state.requires_grad)):
         return _DeltaRule.apply(q, k, v, g, beta, initial_state, starts, scale, bool(return_state))
     out, state, *_ = _forward(q, k, v, g, beta, starts, scale, initial_state, return_state, False)
     return (out, state) if return_state else out
@@ -234,40 +260,45 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     for acting.
     """
     _check_rule(q, k, v, g, beta, starts, ("Envs",))
-    _check_state("state", state, q, v, q.size(0))
-    _check(not (torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, g, beta, state))),
-           "gated_delta_step has no gradients; use gated_delta_rule, or torch.no_grad()")
+    _check_state("state", state, q, v)
+    if torch.is_grad_enabled():
+        _check(not (q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad or beta.requires_grad
+                    or state.requires_grad), "gated_delta_step has no gradients; use gated_delta_rule, or torch.no_grad()")
+    device = q.device
     if out is None:
-        out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+        out = torch.empty(v.shape, dtype=v.dtype, device=device)
     else:
-        _check_tensor("out", out, (v.dtype,), 3, q.device)
+        _check_tensor("out", out, (v.dtype,), 3, device)
         _check(out.shape == v.shape and out.is_contiguous(), "out must be like v, contiguous")
-    a = _rule_args(q, k, v, g, beta, starts, q.size(-1) ** -0.5 if scale is None else float(scale), state, out, state,
-                   step=False)
-    with torch.cuda.device(q.device):
-        _native.check(_native.lib().navi_delta_step(ctypes.byref(a), _stream(q.device)))
-    _written(state)
+    envs, key_heads, key_dim = q.shape
+    (q0, q1, _), (k0, k1, _), (v0, v1, _) = q.stride(), k.stride(), v.stride()
+    (g0, g1), (b0, b1), at = g.stride(), beta.stride(), state.data_ptr()
+    rule = _native.PACK_RULE(
+        _DTYPES[q.dtype], key_heads, v.size(1), key_dim, v.size(2), envs, 1,
+        key_dim ** -0.5 if scale is None else float(scale), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+        q0, 0, q1, k0, 0, k1, v0, 0, v1, g.data_ptr(), beta.data_ptr(), g0, 0, g1, b0, 0, b1,
+        *((0, 0, 0) if starts is None else (starts.data_ptr(), starts.stride(0), 0)),
+        at, out.data_ptr(), at, 0, 0, 0, 0)
+    _call(_native.lib().navi_delta_step, device, rule)
+    _written([state] if out.grad_fn is None else [state, out])
     return out
 
 
 # ---- norms of queries and keys, rotation by position ----
 
 
-def _norm_args(q, k, q_weight, k_weight, cos, sin, positions, norm, eps, interleaved) -> _native.QkNorm:
-    a = _native.QkNorm(
-        dtype=_DTYPES[q.dtype], norm=_NORMS[norm], query_heads=q.size(2), key_heads=k.size(2), head_dim=q.size(3),
-        pairs=0 if cos is None else cos.size(1), interleaved=int(interleaved), envs=q.size(0), steps=q.size(1),
-        eps=eps, q=q.data_ptr(), k=k.data_ptr(), q_stride=_strides(q, True), k_stride=_strides(k, True),
-        q_weight=_ptr(q_weight), k_weight=_ptr(k_weight), cos=_ptr(cos), sin=_ptr(sin),
-        positions_end=0 if cos is None else cos.size(0))
-    if positions is not None:
-        a.positions = positions.data_ptr()
-        a.positions_stride = (ctypes.c_int64 * 2)(*positions.stride())
-        a.positions_wide = int(positions.dtype == torch.int64)
-    return a
-
-
 _NORMS = {"rms": _native.NORM_RMS, "l2": _native.NORM_L2}
+
+
+def _pack_norm(q, k, q_weight, k_weight, cos, sin, positions, norm, eps, interleaved, outputs, backward=(0,) * 13) -> bytes:
+    envs, steps, query_heads, dim = q.shape
+    end, pairs = (0, 0) if cos is None else cos.shape
+    return _native.PACK_NORM(
+        _DTYPES[q.dtype], _NORMS[norm], query_heads, k.size(2), dim, pairs, interleaved,
+        positions is not None and positions.dtype is torch.int64, envs, steps, eps, q.data_ptr(), k.data_ptr(),
+        *q.stride()[:3], *k.stride()[:3], _ptr(q_weight), _ptr(k_weight),
+        *((0, 0, 0) if positions is None else (positions.data_ptr(), *positions.stride())), _ptr(cos), _ptr(sin), end,
+        *outputs, *backward)
 
 
 class _QkNorm(torch.autograd.Function):
@@ -290,30 +321,70 @@ class _QkNorm(torch.autograd.Function):
                 grad = torch.zeros((), dtype=t.dtype, device=t.device).expand(t.shape)
             grads.append(grad if _dense_last(grad) else grad.contiguous())
         grad_q, grad_k = grads
-        a = _norm_args(q, k, q_weight, k_weight, cos, sin, positions, *ctx.rest)
-        d_q, d_k = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k))
-        weights = [torch.empty_like(w) if w is not None and ctx.needs_input_grad[2 + i] else None
-                   for i, w in enumerate((q_weight, k_weight))]
-        a.grad_q, a.grad_k, a.d_q, a.d_k = grad_q.data_ptr(), grad_k.data_ptr(), d_q.data_ptr(), d_k.data_ptr()
-        a.grad_q_stride, a.grad_k_stride = _strides(grad_q, True), _strides(grad_k, True)
-        a.d_q_weight, a.d_k_weight = _ptr(weights[0]), _ptr(weights[1])
-        lib = _native.lib()
-        if any(w is not None for w in weights):
-            size = _native.check(lib.navi_qk_norm_workspace(ctypes.byref(a)))
-            partial = torch.empty(size // 4, dtype=torch.float32, device=q.device)
-            a.partial = partial.data_ptr()
-        with torch.cuda.device(q.device):
-            _native.check(lib.navi_qk_norm_backward(ctypes.byref(a), _stream(q.device)))
-        return d_q, d_k, weights[0], weights[1], None, None, None, None, None, None
+        device = q.device
+        d_q, d_k = (torch.empty(t.shape, dtype=t.dtype, device=device) for t in (q, k))
+        d_weights = [torch.empty_like(w) if w is not None and ctx.needs_input_grad[2 + i] else None
+                     for i, w in enumerate((q_weight, k_weight))]
+        args = (q, k, q_weight, k_weight, cos, sin, positions, *ctx.rest)
+        lib, partial = _native.lib(), None
+        if any([w is not None for w in d_weights]):
+            size = _native.check(lib.navi_qk_norm_workspace(_pack_norm(*args, (0, 0))))
+            partial = torch.empty(size // 4, dtype=torch.float32, device=device)
+        packed = _pack_norm(*args, (0, 0), (grad_q.data_ptr(), grad_k.data_ptr(), *grad_q.stride()[:3], *grad_k.stride()[:3],
+                                            d_q.data_ptr(), d_k.data_ptr(), _ptr(d_weights[0]), _ptr(d_weights[1]),
+                                            _ptr(partial)))
+        _call(lib.navi_qk_norm_backward, device, packed)
+        return d_q, d_k, d_weights[0], d_weights[1], None, None, None, None, None, None
 
 
-def _norm_forward(q, k, q_weight, k_weight, cos, sin, positions, norm, eps, interleaved):
-    a = _norm_args(q, k, q_weight, k_weight, cos, sin, positions, norm, eps, interleaved)
-    q_out, k_out = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k))
-    a.q_out, a.k_out = q_out.data_ptr(), k_out.data_ptr()
-    with torch.cuda.device(q.device):
-        _native.check(_native.lib().navi_qk_norm(ctypes.byref(a), _stream(q.device)))
+def _norm_forward(q, k, *rest):
+    q_out, k_out = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    _call(_native.lib().navi_qk_norm, q.device, _pack_norm(q, k, *rest, (q_out.data_ptr(), k_out.data_ptr())))
     return q_out, k_out
+
+
+def _fine_norm(q, k, q_weight, k_weight, cos, sin, positions, norm) -> bool:
+    try:
+        device, dtype, (envs, steps, _, dim) = q.device, q.dtype, q.shape
+        return (dtype in _DTYPES and k.dtype is dtype and device.type == "cuda" and k.device == device and norm in _NORMS
+                and k.dim() == 4 and k.shape[:2] == (envs, steps) and k.size(3) == dim and 0 < dim <= _native.MAX_NORM_DIM
+                and (q.stride(3) == 1 or dim == 1) and (k.stride(3) == 1 or dim == 1)
+                and all(w is None or (w.dtype is torch.float32 and w.device == device and w.shape == (dim,)
+                                      and w.is_contiguous()) for w in (q_weight, k_weight))
+                and ((cos is None and sin is None and positions is None)
+                     or (cos.dtype is torch.float32 and sin.dtype is torch.float32 and cos.device == device
+                         and sin.device == device and cos.dim() == 2 and cos.shape == sin.shape and cos.is_contiguous()
+                         and sin.is_contiguous() and cos.size(0) > 0 and 0 < 2 * cos.size(1) <= dim
+                         and (positions is None or (positions.dtype in (torch.int32, torch.int64)
+                                                    and positions.device == device and positions.shape == (envs, steps))))))
+    except (AttributeError, TypeError, ValueError, IndexError):
+        return False
+
+
+def _check_norm(q, k, q_weight, k_weight, cos, sin, positions, norm) -> None:
+    if _fine_norm(q, k, q_weight, k_weight, cos, sin, positions, norm):
+        return
+    _check_tensor("q", q, tuple(_DTYPES), 4)
+    _check_tensor("k", k, (q.dtype,), 4, q.device)
+    _check(q.shape[:2] == k.shape[:2] and q.size(3) == k.size(3), "q and k must be [Envs, Steps, Heads, HeadDim], alike but for Heads")
+    _check(0 < q.size(3) <= _native.MAX_NORM_DIM, f"the head dimension must be in [1, {_native.MAX_NORM_DIM}]")
+    _check(_dense_last(q) and _dense_last(k), "q and k must be contiguous in their last dimension")
+    _check(norm in _NORMS, "norm must be 'rms' or 'l2'")
+    for name, t in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if t is not None:
+            _check_tensor(name, t, (torch.float32,), 1, q.device)
+            _check(t.size(0) == q.size(3) and t.is_contiguous(), f"{name} must be [HeadDim], contiguous")
+    _check((cos is None) == (sin is None), "cos and sin go together")
+    if cos is not None:
+        for name, t in (("cos", cos), ("sin", sin)):
+            _check_tensor(name, t, (torch.float32,), 2, q.device)
+            _check(t.shape == cos.shape and t.is_contiguous(), "cos and sin must be alike and contiguous")
+        _check(cos.size(0) > 0 and 0 < 2 * cos.size(1) <= q.size(3), "cos and sin must be [Positions, Pairs], 2 * Pairs <= HeadDim")
+    if positions is not None:
+        _check(cos is not None, "positions need cos and sin")
+        _check_tensor("positions", positions, (torch.int32, torch.int64), 2, q.device)
+        _check(positions.shape == q.shape[:2], "positions must be [Envs, Steps]")
+    raise RuntimeError("q, k, the weights, cos, sin and positions do not go together")
 
 
 def qk_norm(q: torch.Tensor, k: torch.Tensor, *, q_weight: torch.Tensor | None = None,
@@ -332,30 +403,12 @@ def qk_norm(q: torch.Tensor, k: torch.Tensor, *, q_weight: torch.Tensor | None =
     ``positions``: ``[Envs, Steps]`` int32 or int64 rows of the tables (a token's step by
     default); one outside the tables gives NaN in the numbers that it would rotate.
     """
-    _check_tensor("q", q, tuple(_DTYPES), 4)
-    _check_tensor("k", k, (q.dtype,), 4, q.device)
-    _check(q.shape[:2] == k.shape[:2] and q.size(3) == k.size(3), "q and k must be [Envs, Steps, Heads, HeadDim], alike but for Heads")
-    _check(0 < q.size(3) <= _native.MAX_NORM_DIM, f"the head dimension must be in [1, {_native.MAX_NORM_DIM}]")
-    _check(_dense_last(q) and _dense_last(k), "q and k must be contiguous in their last dimension")
-    _check(norm in _NORMS, "norm must be 'rms' or 'l2'")
+    _check_norm(q, k, q_weight, k_weight, cos, sin, positions, norm)
     eps = float(eps)
     _check(math.isfinite(eps) and eps >= 0.0, "eps must be finite and not negative")
-    for name, t in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if t is not None:
-            _check_tensor(name, t, (torch.float32,), 1, q.device)
-            _check(t.size(0) == q.size(3) and t.is_contiguous(), f"{name} must be [HeadDim], contiguous")
-    _check((cos is None) == (sin is None), "cos and sin go together")
-    if cos is not None:
-        for name, t in (("cos", cos), ("sin", sin)):
-            _check_tensor(name, t, (torch.float32,), 2, q.device)
-            _check(t.shape == cos.shape and t.is_contiguous(), "cos and sin must be alike and contiguous")
-        _check(cos.size(0) > 0 and 0 < 2 * cos.size(1) <= q.size(3), "cos and sin must be [Positions, Pairs], 2 * Pairs <= HeadDim")
-    if positions is not None:
-        _check(cos is not None, "positions need cos and sin")
-        _check_tensor("positions", positions, (torch.int32, torch.int64), 2, q.device)
-        _check(positions.shape == q.shape[:2], "positions must be [Envs, Steps]")
     args = (q, k, q_weight, k_weight, cos, sin, positions, norm, eps, bool(interleaved))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:4]):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or (q_weight is not None and q_weight.requires_grad)
+                                    or (k_weight is not None and k_weight.requires_grad)):
         return _QkNorm.apply(*args)
     return _norm_forward(*args)
 
@@ -379,28 +432,42 @@ def clip_grad_norm(grads: Iterable[torch.Tensor | None], max_norm: float, *, eps
     grads = list(grads)
     to = grads if out is None else list(out)
     _check(len(to) == len(grads), "out must be as long as grads")
-    pairs = [(x, y) for x, y in zip(grads, to) if x is not None]
-    _check(len(pairs) > 0, "grads must hold at least one tensor")
-    device = pairs[0][0].device
-    for x, y in pairs:
-        _check(isinstance(x, torch.Tensor) and x.is_cuda and x.layout == torch.strided, "grads must be dense CUDA tensors")
-        _check(x.dtype in _DTYPES, "grads must be float32, bfloat16 or float16")
-        _check(x.device == device, "grads must be on one device")
-        _check(x.is_contiguous() or torch.ops.aten.is_non_overlapping_and_dense(x), "grads must fill their memory without gaps")
-        if y is not x:
-            _check(isinstance(y, torch.Tensor) and y.dtype == x.dtype and y.shape == x.shape and y.device == device
-                   and (y.is_contiguous() if x.is_contiguous() else y.stride() == x.stride()),
-                   "out must be like grads in shapes, types, strides and device")
-    n = len(pairs)
+    if any([x is None for x in grads]):
+        to = [y for x, y in zip(grads, to) if x is not None]
+        grads = [x for x in grads if x is not None]
+    _check(len(grads) > 0, "grads must hold at least one tensor")
+    if not _fine_grads(grads, to):
+        _check_grads(grads, to)
+    n, device = len(grads), grads[0].device
     norm = torch.empty((), dtype=torch.float32, device=device)
     partial = torch.empty(_native.NORM_PARTIALS, dtype=torch.float32, device=device)
-    with torch.cuda.device(device):
-        _native.check(_native.lib().navi_clip_grad_norm(
-            n, (ctypes.c_void_p * n)(*[x.data_ptr() for x, _ in pairs]),
-            (ctypes.c_void_p * n)(*[y.data_ptr() for _, y in pairs]),
-            (ctypes.c_int64 * n)(*[x.numel() for x, _ in pairs]),
-            (ctypes.c_int32 * n)(*[_DTYPES[x.dtype] for x, _ in pairs]),
-            max_norm, eps, norm.data_ptr(), partial.data_ptr(), _stream(device)))
-    for _, y in pairs:
-        _written(y)
+    at = struct.pack(f"{n}P", *[x.data_ptr() for x in grads])
+    _call(_native.lib().navi_clip_grad_norm, device,
+          n, at, at if to is grads else struct.pack(f"{n}P", *[y.data_ptr() for y in to]),
+          struct.pack(f"{n}q", *[x.numel() for x in grads]), struct.pack(f"{n}i", *[_DTYPES[x.dtype] for x in grads]),
+          max_norm, eps, norm.data_ptr(), partial.data_ptr())
+    _written(to)
     return norm
+
+
+def _fine_grads(grads: list, to: list) -> bool:
+    """Whether all are contiguous and alike: what nearly every call brings."""
+    try:
+        device = grads[0].get_device()
+        return (device >= 0 and all([x.is_contiguous() and x.get_device() == device and x.dtype in _DTYPES for x in grads])
+                and (to is grads or all([y.is_contiguous() and y.get_device() == device and y.dtype is x.dtype
+                                         and y.shape == x.shape for x, y in zip(grads, to)])))
+    except (AttributeError, TypeError, RuntimeError):
+        return False
+
+
+def _check_grads(grads: list, to: list) -> None:
+    for x, y in zip(grads, to):
+        _check(isinstance(x, torch.Tensor) and x.is_cuda and x.layout == torch.strided, "grads must be dense CUDA tensors")
+        _check(x.dtype in _DTYPES, "grads must be float32, bfloat16 or float16")
+        _check(x.device == grads[0].device, "grads must be on one device")
+        _check(x.is_contiguous() or torch.ops.aten.is_non_overlapping_and_dense(x), "grads must fill their memory without gaps")
+        if y is not x:
+            _check(isinstance(y, torch.Tensor) and y.dtype == x.dtype and y.shape == x.shape and y.device == x.device
+                   and (y.is_contiguous() if x.is_contiguous() else y.stride() == x.stride()),
+                   "out must be like grads in shapes, types, strides and device")
