@@ -119,37 +119,43 @@ __device__ inline void load_rows(const RuleParams& P, ChunkRows<E, KP>& rows, in
     }
 }
 
-// One wave's scan of the chunk's gates, a token a lane.
-__device__ inline void load_gates(const RuleParams& P, ChunkGates& gates, int64_t env, int head, int64_t t0,
-                                  int tokens) {
-    const int lane = threadIdx.x & 63;
-    float g = 0.0f, beta = 0.0f;
-    int start = 0;
-    if (lane < tokens) {
-        g = *at<float>(P.r.g, P.r.g_stride, env, t0 + lane, head);
-        beta = *at<float>(P.r.beta, P.r.beta_stride, env, t0 + lane, head);
-        start = g < kStart ||
-                (P.r.starts && P.r.starts[env * P.r.starts_stride[0] + (t0 + lane) * P.r.starts_stride[1]]);
+// A chunk's gates, a token a lane of one wave: read, and summed into LDS.
+struct GatesFetch {
+    float g, beta;
+    int start;
+
+    __device__ void fetch(const RuleParams& P, int64_t env, int head, int64_t t0, int tokens) {
+        const int lane = threadIdx.x & 63;
+        g = beta = 0.0f;
+        start = 0;
+        if (lane < tokens) {
+            g = *at<float>(P.r.g, P.r.g_stride, env, t0 + lane, head);
+            beta = *at<float>(P.r.beta, P.r.beta_stride, env, t0 + lane, head);
+            if (P.r.starts) start = P.r.starts[env * P.r.starts_stride[0] + (t0 + lane) * P.r.starts_stride[1]];
+        }
     }
-    double sum = start ? 0.0 : static_cast<double>(g);
-    int episode = start;
+
+    __device__ void put(ChunkGates& gates) const {
+        const int lane = threadIdx.x & 63;
+        const bool starts = start != 0 || g < kStart;
+        double sum = starts ? 0.0 : static_cast<double>(g);
+        const uint64_t all = __ballot(starts);
+        const int episode = __popcll(all << (63 - lane)), last_episode = __popcll(all);
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const double s = __shfl_up(sum, d);
-        const int e = __shfl_up(episode, d);
-        sum += lane >= d ? s : 0.0;
-        episode += lane >= d ? e : 0;
+        for (int d = 1; d < 64; d *= 2) {
+            const double s = __shfl_up(sum, d);
+            sum += lane >= d ? s : 0.0;
+        }
+        const float hi = static_cast<float>(sum), lo = static_cast<float>(sum - hi);
+        const double last = __shfl(sum, 63);
+        gates.hi[lane] = hi;
+        gates.lo[lane] = lo;
+        gates.e[lane] = episode == 0 ? expf(hi) * (1.0f + lo) : 0.0f;
+        gates.f[lane] = episode == last_episode ? expf(static_cast<float>(last - sum)) : 0.0f;
+        gates.beta[lane] = beta;
+        gates.episode[lane] = episode;
     }
-    const float hi = static_cast<float>(sum), lo = static_cast<float>(sum - hi);
-    const double last = __shfl(sum, 63);
-    const int last_episode = __shfl(episode, 63);
-    gates.hi[lane] = hi;
-    gates.lo[lane] = lo;
-    gates.e[lane] = episode == 0 ? expf(hi) * (1.0f + lo) : 0.0f;
-    gates.f[lane] = episode == last_episode ? expf(static_cast<float>(last - sum)) : 0.0f;
-    gates.beta[lane] = beta;
-    gates.episode[lane] = episode;
-}
+};
 
 __device__ inline float decay(const ChunkGates& gates, int i, float hi_j, float lo_j, int episode_j) {
     const float d = (gates.hi[i] - hi_j) + (gates.lo[i] - lo_j);
@@ -314,7 +320,8 @@ struct TriangleLds {
     ChunkGates gates;
 };
 
-// X and P of the chunk whose rows and gates are in LDS, by the four waves of a workgroup.
+// X and P of the chunk whose rows and gates are in LDS, by the four waves of a workgroup, three
+// tiles each (the last of the ten thrice, with the same numbers: no branch stands between tiles).
 template <class E, int KP>
 __device__ inline void make_triangles(TriangleLds<E, KP>& lds, ChunkMatrices& to, float scale, int wave) {
     constexpr int N = kPlanes<E>, kEach = (kTiles + 3) / 4;
@@ -322,8 +329,7 @@ __device__ inline void make_triangles(TriangleLds<E, KP>& lds, ChunkMatrices& to
     f4 a[kEach];
 #pragma unroll
     for (int n = 0; n < kEach; ++n) {
-        const int tile = wave + 4 * n;
-        if (tile >= kTiles) continue;
+        const int tile = wave + 4 * n < kTiles ? wave + 4 * n : kTiles - 1;
         const int i = tile_row(tile), j = tile - tile_of(i, 0);
         f4 kk = {0, 0, 0, 0}, qk = {0, 0, 0, 0};
 #pragma unroll
@@ -351,8 +357,7 @@ __device__ inline void make_triangles(TriangleLds<E, KP>& lds, ChunkMatrices& to
     __syncthreads();
 #pragma unroll
     for (int n = 0; n < kEach; ++n) {
-        const int tile = wave + 4 * n;
-        if (tile >= kTiles) continue;
+        const int tile = wave + 4 * n < kTiles ? wave + 4 * n : kTiles - 1;
         const int i = tile_row(tile), j = tile - tile_of(i, 0);
 #pragma unroll
         for (int s = 0; s < 4; ++s) lds.work[16 * i + 4 * g + s][16 * j + col] = a[n][s];
@@ -361,8 +366,7 @@ __device__ inline void make_triangles(TriangleLds<E, KP>& lds, ChunkMatrices& to
     invert_triangle(lds.work, wave, 4);
 #pragma unroll
     for (int n = 0; n < kEach; ++n) {
-        const int tile = wave + 4 * n;
-        if (tile >= kTiles) continue;
+        const int tile = wave + 4 * n < kTiles ? wave + 4 * n : kTiles - 1;
         const int i = tile_row(tile), j = tile - tile_of(i, 0);
         f4 x;
 #pragma unroll
@@ -429,17 +433,36 @@ struct ChunkFetch {
         }
     }
 
+    // The rows alone, at once.
+    __device__ static void load(const RuleParams& P, ChunkRows<E, KP>& rows, int64_t env, int head, int64_t t0, int tokens) {
+        if (!P.wide_qk) {
+            load_rows<E, KP>(P, rows, env, head, t0, tokens);
+            return;
+        }
+        u4 q[kPieces][kWords], k[kPieces][kWords];
+        const int key_head = head / P.group;
+        fetch_rows(at<E>(P.r.q, P.r.q_stride, env, t0, key_head), static_cast<uint32_t>(P.r.q_stride[1]) * sizeof(E),
+                   P.r.key_dim, tokens, q);
+        fetch_rows(at<E>(P.r.k, P.r.k_stride, env, t0, key_head), static_cast<uint32_t>(P.r.k_stride[1]) * sizeof(E),
+                   P.r.key_dim, tokens, k);
+        put_rows(rows, q, k);
+    }
+
+    __device__ static void put_rows(ChunkRows<E, KP>& rows, const u4 (&q)[kAll ? kPieces : 1][kWords], const u4 (&k)[kPieces][kWords]) {
+        constexpr int kAcross = KP / 8, kDown = kThreads / kAcross;
+        const int t = threadIdx.x / kAcross, c = threadIdx.x % kAcross * 8;
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            if constexpr (kAll) put_piece(rows.q, t + i * kDown, c, q[i]);
+            put_piece(rows.k, t + i * kDown, c, k[i]);
+        }
+    }
+
     template <int NP>
     __device__ void put(const RuleParams& P, ChunkRows<E, KP>& rows, Triangle<3>& x, Triangle<NP>& p, float (&gates)[2][kChunk],
                         int64_t env, int head, int64_t t0, int tokens) const {
         if (P.wide_qk) {
-            constexpr int kAcross = KP / 8, kDown = kThreads / kAcross;
-            const int t = threadIdx.x / kAcross, c = threadIdx.x % kAcross * 8;
-#pragma unroll
-            for (int i = 0; i < kPieces; ++i) {
-                if constexpr (kAll) put_piece(rows.q, t + i * kDown, c, q[i]);
-                put_piece(rows.k, t + i * kDown, c, k[i]);
-            }
+            put_rows(rows, q, k);
         } else {
             load_rows<E, KP>(P, rows, env, head, t0, tokens);
         }

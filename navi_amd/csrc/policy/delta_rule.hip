@@ -98,8 +98,10 @@ __global__ __launch_bounds__(256) void delta_triangles_kernel(RuleParams P) {
     const int64_t env = sequence / P.r.value_heads, t0 = static_cast<int64_t>(chunk) * kChunk;
     const int head = static_cast<int>(sequence % P.r.value_heads), tokens = tokens_of(P, chunk);
     ChunkMatrices& to = reinterpret_cast<ChunkMatrices*>(P.r.matrices)[blockIdx.x];
-    load_rows<E, KP>(P, lds.rows, env, head, t0, tokens);
-    if (wave == 0) load_gates(P, lds.gates, env, head, t0, tokens);
+    GatesFetch gates;
+    if (wave == 0) gates.fetch(P, env, head, t0, tokens);
+    ChunkFetch<E, KP, 256, true>::load(P, lds.rows, env, head, t0, tokens);
+    if (wave == 0) gates.put(lds.gates);
     __syncthreads();
     if (threadIdx.x < kChunk) {
         to.e[threadIdx.x] = lds.gates.e[threadIdx.x];
@@ -888,8 +890,10 @@ __global__ __launch_bounds__((64 * kGradientWaves<E, KP>), (kGradientWaves<E, KP
         if (of_dr) next_dr.load(from_dr, my_token * row_bytes + 4 * (v0 + 8 * g), valid, P.wide_state);
     };
     fetch(0);
-    if (wave_of_workgroup() == kWaves - 1) load_gates(P, lds.rest.gates, env, head, t0, tokens);
-    if constexpr (kRowsStay<E, KP>) load_rows<E, KP>(P, rows, env, head, t0, tokens);
+    GatesFetch of_gates;
+    if (wave_of_workgroup() == kWaves - 1) of_gates.fetch(P, env, head, t0, tokens);
+    if constexpr (kRowsStay<E, KP>) ChunkFetch<E, KP, 64 * kWaves, true>::load(P, rows, env, head, t0, tokens);
+    if (wave_of_workgroup() == kWaves - 1) of_gates.put(lds.rest.gates);
     // With eight waves, those of dr use the registers of do's terms
     GradientTerms<E, KP, true> terms;
     GradientTerms<E, KP, false> others;
@@ -961,7 +965,7 @@ __global__ __launch_bounds__((64 * kGradientWaves<E, KP>), (kGradientWaves<E, KP
     if (lane == 0) lds.rest.dot_part[threadIdx.x >> 6] = dot;
     __syncthreads();
     if constexpr (!kRowsStay<E, KP>) {
-        load_rows<E, KP>(P, rows, env, head, t0, tokens);
+        ChunkFetch<E, KP, 64 * kWaves, true>::load(P, rows, env, head, t0, tokens);
         __syncthreads();
     }
 
