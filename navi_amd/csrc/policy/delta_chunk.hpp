@@ -66,6 +66,22 @@ struct ChunkGates {
     int32_t episode[kChunk];       // episodes started in the chunk so far
 };
 
+// Rows in LDS hold every 32 columns in the order in which two tiles of a product's result hold a
+// column: 4 g to 4 g + 3 of the first tile, then of the second, for g = 0 to 3. A lane's part
+// (g) of an operand is then 16 adjacent bytes, whether the other operand is such a result or
+// rows like these.
+__device__ inline int place_of(int column) {
+    return (column & ~31) + ((column & 12) << 1) + ((column & 16) >> 2) + (column & 3);
+}
+
+// Eight columns from a multiple of eight on, to their places.
+template <int kPitch>
+__device__ inline void put_columns(uint16_t (&row)[kPitch], int column, u4 x) {
+    uint16_t* to = &row[place_of(column)];
+    *reinterpret_cast<u2*>(to) = u2{x[0], x[1]};
+    *reinterpret_cast<u2*>(to + 8) = u2{x[2], x[3]};
+}
+
 template <class E, int KP>
 struct ChunkRows {
     static constexpr int kPitch = KP + 8;
@@ -111,11 +127,11 @@ __device__ inline void load_rows(const RuleParams& P, ChunkRows<E, KP>& rows, in
         load8(at<E>(P.r.q, P.r.q_stride, env, t0 + (t < tokens ? t : 0), key_head) + c, valid, P.wide_qk, x);
         split8(x, plane);
 #pragma unroll
-        for (int n = 0; n < kPlanes<E>; ++n) *reinterpret_cast<u4*>(&rows.q[n][t][c]) = plane[n];
+        for (int n = 0; n < kPlanes<E>; ++n) put_columns(rows.q[n][t], c, plane[n]);
         load8(at<E>(P.r.k, P.r.k_stride, env, t0 + (t < tokens ? t : 0), key_head) + c, valid, P.wide_qk, x);
         split8(x, plane);
 #pragma unroll
-        for (int n = 0; n < kPlanes<E>; ++n) *reinterpret_cast<u4*>(&rows.k[n][t][c]) = plane[n];
+        for (int n = 0; n < kPlanes<E>; ++n) put_columns(rows.k[n][t], c, plane[n]);
     }
 }
 
@@ -162,8 +178,8 @@ __device__ inline float decay(const ChunkGates& gates, int i, float hi_j, float 
     return gates.episode[i] == episode_j ? __builtin_amdgcn_exp2f(d * kLog2E) : 0.0f;
 }
 
-// Operands of products from rows in LDS: rows row0 to row0 + 15, eight columns of 32 m to
-// 32 m + 31 a lane, in their order;
+// Operands of products from rows in LDS: rows row0 to row0 + 15, the lane's part of columns 32 m
+// to 32 m + 31 (the other operand: a result's two tiles 2 m, or rows read in the same way);
 template <int N, int kPitch>
 __device__ inline void operand_rows(int lane, const uint16_t (&rows)[N][kChunk][kPitch], int row0, int m, u4 (&x)[N]) {
 #pragma unroll
@@ -171,27 +187,14 @@ __device__ inline void operand_rows(int lane, const uint16_t (&rows)[N][kChunk][
         x[n] = *reinterpret_cast<const u4*>(&rows[n][row0 + (lane & 15)][32 * m + 8 * (lane >> 4)]);
 }
 
-// the same in the order in which two tiles of a product's result hold a column (rows 4 g to
-// 4 g + 3 of each, g = l / 16), so that such a result is the other operand without a move;
-template <int N, int kPitch>
-__device__ inline void operand_rows_as_results(int lane, const uint16_t (&rows)[N][kChunk][kPitch], int row0, int m,
-                                               u4 (&x)[N]) {
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-        const uint16_t* row = &rows[n][row0 + (lane & 15)][32 * m + 4 * (lane >> 4)];
-        const u2 a = *reinterpret_cast<const u2*>(row), b = *reinterpret_cast<const u2*>(row + 16);
-        x[n] = u4{a.x, a.y, b.x, b.y};
-    }
-}
-
 // and columns 16 c to 16 c + 15 as the operand's rows, tokens 32 m to 32 m + 31 contracted in
-// that same order.
+// the order of results.
 template <int N, int kPitch>
 __device__ inline void operand_columns(int lane, const uint16_t (&rows)[N][kChunk][kPitch], int c, int m, u4 (&x)[N]) {
     const int i = lane & 15;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-        const uint16_t* from = &rows[n][32 * m + 4 * (lane >> 4) + (i >> 2)][16 * c + 4 * (i & 3)];
+        const uint16_t* from = &rows[n][32 * m + 4 * (lane >> 4) + (i >> 2)][32 * (c >> 1) + 4 * (c & 1) + 8 * (i & 3)];
         const u2 a = read_transposed(from), b = read_transposed(from + 16 * kPitch);
         x[n] = u4{a.x, a.y, b.x, b.y};
     }
@@ -416,7 +419,7 @@ struct ChunkFetch {
 
     __device__ static void put_piece(uint16_t (&rows)[kPlanes<E>][kChunk][KP + 8], int t, int c, const u4 (&from)[kWords]) {
         if constexpr (kPlanes<E> == 1) {
-            *reinterpret_cast<u4*>(&rows[0][t][c]) = from[0];
+            put_columns(rows[0][t], c, from[0]);
         } else {
             float x[8];
 #pragma unroll
@@ -429,7 +432,7 @@ struct ChunkFetch {
             u4 plane[kPlanes<E>];
             split8(x, plane);
 #pragma unroll
-            for (int n = 0; n < kPlanes<E>; ++n) *reinterpret_cast<u4*>(&rows[n][t][c]) = plane[n];
+            for (int n = 0; n < kPlanes<E>; ++n) put_columns(rows[n][t], c, plane[n]);
         }
     }
 

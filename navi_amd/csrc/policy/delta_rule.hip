@@ -243,7 +243,7 @@ __device__ inline void add_columns(int lane, const uint16_t (&rows)[N][kChunk][k
 // A wave holds 16 columns of the state as results of products (KP / 16 tiles), a workgroup
 // kThreads / 64 such columns of one head; it walks the chunks with the state in registers.
 // The state is the second operand of S^T k without a move: its tiles hold the contracted axis
-// in the order of results, which the other operand is read in as well.
+// in the order of results, which the rows in LDS are kept in as well.
 template <class E, int KP, int kThreads, bool kSummary>
 __global__ __launch_bounds__(kThreads) void delta_forward_kernel(RuleParams P) {
     constexpr int N = kPlanes<E>, NP = kOutPlanes<E>;
@@ -298,13 +298,13 @@ __global__ __launch_bounds__(kThreads) void delta_forward_kernel(RuleParams P) {
                 u4 b[3], a[4][N];
                 split8(state[2 * m], state[2 * m + 1], b);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) operand_rows_as_results(lane, lds.rows.k, 16 * i, m, a[i]);
+                for (int i = 0; i < 4; ++i) operand_rows(lane, lds.rows.k, 16 * i, m, a[i]);
                 mma_each<4>(a, b, u);
                 if constexpr (!kSummary) {
                     u4 b_out[NP];
                     first_planes(b, b_out);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) operand_rows_as_results(lane, lds.rows.q, 16 * i, m, a[i]);
+                    for (int i = 0; i < 4; ++i) operand_rows(lane, lds.rows.q, 16 * i, m, a[i]);
                     mma_each<4>(a, b_out, o);
                 }
             }
@@ -412,7 +412,7 @@ __global__ __launch_bounds__(kThreads) void delta_reverse_kernel(RuleParams P) {
                 u4 b[3], a[4][N];
                 split8(dstate[2 * m], dstate[2 * m + 1], b);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) operand_rows_as_results(lane, lds.rows.k, 16 * i, m, a[i]);
+                for (int i = 0; i < 4; ++i) operand_rows(lane, lds.rows.k, 16 * i, m, a[i]);
                 mma_each<4>(a, b, du);
             }
 #pragma unroll
@@ -808,7 +808,7 @@ struct GradientTerms {
         for (int s = 0; s < 4; ++s) {
             float y = 0.0f;
 #pragma unroll
-            for (int n = N - 1; n >= 0; --n) y += to_float(bf16{rows[n][row + s][16 * c + (lane & 15)]});
+            for (int n = N - 1; n >= 0; --n) y += to_float(bf16{rows[n][row + s][place_of(16 * c + (lane & 15))]});
             product[s] = y * x[s];
         }
         return product;
