@@ -101,6 +101,21 @@ def test_rule_and_gradients(policy, size, with_state):
         assert torch.equal(back["g"].cpu()[starts.cpu()], torch.zeros_like(back["g"].cpu()[starts.cpu()]))
 
 
+@pytest.mark.parametrize("steps", [1, 2, 4, 5])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_short_rollouts_without_gradients(policy, steps, dtype):
+    x, state, starts = make(3, 6, 2, 4, 50, 36, dtype, seed=steps)
+    starts = torch.rand(starts.shape, device="cuda") < 0.3
+    x = {n: t[:, 1:1 + steps] for n, t in x.items()}  # (views)
+    x["q"] = x["q"][:, :1].expand(x["q"].shape)
+    o, final = policy.gated_delta_rule(*x.values(), starts=starts[:, 1:1 + steps], initial_state=state, return_state=True)
+    want_o, want_final = ref.rule(*x.values(), starts[:, 1:1 + steps], state, 50 ** -0.5)
+    assert ref.off(o, want_o) <= tolerance(dtype)
+    assert ref.off(final, want_final) <= TOL
+    o = policy.gated_delta_rule(*x.values())
+    assert ref.off(o, ref.rule(*x.values(), None, None, 50 ** -0.5)[0]) <= tolerance(dtype)
+
+
 LONG = [  # few heads and many chunks: walked in segments that are joined
     (1, 64 * 8, 1, 1, 64, 64, torch.float32),
     (1, 64 * 9 + 5, 1, 2, 33, 70, torch.bfloat16),
