@@ -40,6 +40,7 @@ struct RuleParams {
     float* rgrads;        // [env, head][steps][V] gradient of r
     // Long sequences of few heads are walked in segments of chunks (delta_join_kernel)
     int32_t n_segments;
+    int32_t blocks, summary_blocks;  // of 64 columns: of V, and of V and the unit matrix
     float* segment_states;    // [env, head][n_segments - 1][K][V]
     float* segment_matrices;  // [env, head][n_segments - 1][K][K]
     float* dq_heads;      // [env][step][value head][K] where heads are shared

@@ -55,12 +55,77 @@ struct Columns {
     }
 };
 
-template <class E>
-__device__ inline f4 to_floats(const E (&x)[4]) {
-    return f4{to_float(x[0]), to_float(x[1]), to_float(x[2]), to_float(x[3])};
-}
-
 __device__ inline f4 four(const float (&x)[kChunk], int row) { return *reinterpret_cast<const f4*>(&x[row]); }
+
+// A wave's 16 columns of 64 rows on their way to the layout of products: two loads of a lane hold
+// 8 columns of a row each, of tile 2 m (lanes 0 to 31) and 2 m + 1; a product with the unit matrix
+// (exact: each sum has one term) puts them where results stand.
+template <class E>
+struct ColumnFetch {
+    Part<E, 8> part[2];
+
+    __device__ void fetch(const E* base, int64_t stride, int columns, int tokens, bool wide) {
+        const int l = threadIdx.x & 63, g = l >> 4;
+        const uint32_t row_bytes = static_cast<uint32_t>(stride) * sizeof(E);
+        const int width = columns < 0 ? 0 : columns < 16 ? columns : 16;
+        const Buffer from = buffer_of(base, (tokens - 1) * row_bytes + width * sizeof(E));
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            const int token = 32 * m + 16 * (g >> 1) + (l & 15), column = 8 * (g & 1);
+            part[m].load(from, token * row_bytes + column * sizeof(E), token < tokens ? width - column : 0, wide);
+        }
+    }
+
+    // x of the 64 rows added to `to`.
+    __device__ void add(f4 (&to)[4]) const {
+        const int l = threadIdx.x & 63, at = (l & 15) - 8 * ((l >> 4) & 1);  // the one of the lane's eight, if any
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            u4 x[kPlanes<E>];
+            if constexpr (kPlanes<E> == 1) {
+                x[0] = part[m].words[0];
+            } else {
+                float y[8];
+                part[m].floats(y);
+                split8(y, x);
+            }
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                u4 unit;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    unit[i] = l >> 5 == n && at >> 1 == i ? (at & 1 ? 0x3f800000u : 0x3f80u) : 0u;
+#pragma unroll
+                for (int p = kPlanes<E> - 1; p >= 0; --p) to[2 * m + n] = mfma(x[p], unit, to[2 * m + n]);
+            }
+        }
+    }
+};
+
+// Sixteen columns of 64 rows from transposed results: a lane has row l % 16 of each tile, four
+// columns of it.
+template <class E>
+__device__ inline void store_transposed(E* base, int64_t stride, int columns, int tokens, const f4 (&x)[4]) {
+    const int l = threadIdx.x & 63, column = 4 * (l >> 4);
+    const uint32_t row_bytes = static_cast<uint32_t>(stride) * sizeof(E);
+    const int width = columns < 16 ? columns : 16;
+    const Buffer to = buffer_of(base, (tokens - 1) * row_bytes + width * sizeof(E));
+    const uint32_t lane = (l & 15) * row_bytes + column * sizeof(E);
+    if (stride % 4 == 0 && columns % 4 == 0) {
+        const uint32_t own = column < width ? lane : kOutside;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const E y[4] = {from_float<E>(x[i][0]), from_float<E>(x[i][1]), from_float<E>(x[i][2]), from_float<E>(x[i][3])};
+            buffer_store_four(to, own + 16 * i * row_bytes, y);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+                buffer_store<E>(to, column + s < width ? lane + 16 * i * row_bytes + s * sizeof(E) : kOutside, from_float<E>(x[i][s]));
+    }
+}
 
 // x * factor, 0 where the factor is 0 whatever x is: a state that an episode's start clears.
 __device__ inline f4 gated(f4 x, f4 factor) {
@@ -139,6 +204,15 @@ __device__ inline void store_state(const Columns<float>& at, float* to, int K, c
     at.store<KP / 16>(at.rows(to, K), [&](int c, int s) { return state[c][s]; });
 }
 
+// Columns of the state that a workgroup holds, 16 a wave. Two workgroups of 64 fit a CU and wait
+// apart: 2 x 4001 steps, 8 heads of 128, 445 us forward and back against 502 with one of 128; 256 x
+// 128 steps, 4 heads of 128, forward, 100 and 102. Rows of 128 float32 leave a CU's LDS to one
+// workgroup, which then has eight waves: the same, 195 us against 304.
+template <class E, int KP>
+inline constexpr int kWalkColumns = sizeof(E) == 4 && KP == 128 ? 128 : 64;
+template <class E, int KP>
+inline constexpr int kWalkThreads = 4 * kWalkColumns<E, KP>;
+
 // The chunks of a segment in the order that a kernel walks them, and the state before the
 // first: segment 0 begins with `given` (or zeros), the others with what delta_join_kernel
 // found. In summary, the columns past V (rounded up to 16) are those of the unit matrix, and
@@ -151,6 +225,16 @@ struct Walk {
     int32_t first;       // column of the wave's first
     int32_t columns;     // that the array behind `from` and `to` has
     bool working, unit;
+
+    // The sequence and columns of a workgroup. Workgroups go round the 8 XCDs in turn: those of
+    // one sequence are 8 apart, so that what they all read is in one XCD's L2.
+    template <int kColumns>
+    __device__ static bool place(const RuleParams& P, int blocks, int64_t& sequence, int& first) {
+        const uint32_t id = blockIdx.x, round = id / 8;
+        sequence = static_cast<int64_t>(round / blocks) * 8 + id % 8;
+        first = static_cast<int>(round % blocks) * kColumns;
+        return sequence < P.r.envs * P.r.value_heads;
+    }
 
     template <bool kSummary>
     __device__ static Walk of(const RuleParams& P, int64_t sequence, int first, const float* given, float* result) {
@@ -210,6 +294,22 @@ __device__ inline void times_triangle(int lane, const Triangle<N>& t, const u4 (
     x[3] = y[1];
 }
 
+// The same with the result transposed.
+template <int N, int NB>
+__device__ inline void times_triangle_transposed(int lane, const Triangle<N>& t, const u4 (&b)[2][NB], f4 (&x)[4]) {
+    u4 a[4][N];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) operand_triangle<N>(lane, t, i, 0, a[i]);
+    mma_each_transposed<4>(a, b[0], x);
+    u4 below[2][N];
+    f4 y[2] = {x[2], x[3]};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) operand_triangle<N>(lane, t, 2 + i, 1, below[i]);
+    mma_each_transposed<2>(below, b[1], y);
+    x[2] = y[0];
+    x[3] = y[1];
+}
+
 template <int N, int NB>
 __device__ inline void times_transpose(int lane, const Triangle<N>& t, const u4 (&b)[2][NB], f4 (&x)[4]) {
     u4 a[4][N];
@@ -240,39 +340,38 @@ __device__ inline void add_columns(int lane, const uint16_t (&rows)[N][kChunk][k
     for (int n = 0; n < 4; ++n) state[c + n] = x[n];
 }
 
-// A wave holds 16 columns of the state as results of products (KP / 16 tiles), a workgroup
-// kThreads / 64 such columns of one head; it walks the chunks with the state in registers.
+// A wave holds 16 columns of the state as results of products (KP / 16 tiles), a workgroup of
+// four waves 64 of one head; it walks the chunks with the state in registers.
 // The state is the second operand of S^T k without a move: its tiles hold the contracted axis
 // in the order of results, which the rows in LDS are kept in as well.
-template <class E, int KP, int kThreads, bool kSummary>
-__global__ __launch_bounds__(kThreads) void delta_forward_kernel(RuleParams P) {
+template <class E, int KP, bool kSummary>
+__global__ __launch_bounds__((kWalkThreads<E, KP>), 2) void delta_forward_kernel(RuleParams P) {
     constexpr int N = kPlanes<E>, NP = kOutPlanes<E>;
     extern __shared__ char lds_bytes[];
     auto& lds = *reinterpret_cast<ScanLds<E, KP, NP>*>(lds_bytes);
     const int wave = wave_of_workgroup(), lane = threadIdx.x & 63, g = lane >> 4;
-    const int64_t sequence = blockIdx.x;
+    int64_t sequence;
+    int block;
+    if (!Walk::place<kWalkColumns<E, KP>>(P, kSummary ? P.summary_blocks : P.blocks, sequence, block)) return;
     const int64_t env = sequence / P.r.value_heads;
     const int head = static_cast<int>(sequence % P.r.value_heads);
     const int K = P.r.key_dim, V = P.r.value_dim;
-    const Walk walk = Walk::of<kSummary>(P, sequence, (blockIdx.y * (kThreads / 64) + wave) * 16, P.r.initial_state,
+    const Walk walk = Walk::of<kSummary>(P, sequence, block + 16 * wave, P.r.initial_state,
                                          P.r.final_state);
     const int first = walk.first;
     const ChunkMatrices* matrices = reinterpret_cast<const ChunkMatrices*>(P.r.matrices) + sequence * P.n_chunks;
     const E* v = at<E>(P.r.v, P.r.v_stride, env, 0, head) + first;
-    const Columns<E> rows_v(P.r.v_stride[1], walk.unit ? 0 : V - first),
-        rows_out(static_cast<int64_t>(P.r.value_heads) * V, V - first);
     const Columns<float> rows_state(walk.columns, walk.columns - first);
 
     f4 state[KP / 16];
     walk.begin_state<KP>(rows_state, K, state);
 
-    ChunkFetch<E, KP, kThreads, !kSummary> next;
-    E v_next[4][4];
+    ChunkFetch<E, KP, kWalkThreads<E, KP>, !kSummary> next;
+    ColumnFetch<E> v_next;
     const auto fetch = [&](int chunk) {
         const int64_t t0 = static_cast<int64_t>(chunk) * kChunk;
         next.fetch(P, matrices[chunk], env, head, t0, tokens_of(P, chunk));
-        rows_v.template load<4>(rows_v.rows(v + t0 * P.r.v_stride[1], tokens_of(P, chunk)),
-                                [&](int i, int s, E x) { v_next[i][s] = x; });
+        v_next.fetch(v + t0 * P.r.v_stride[1], P.r.v_stride[1], walk.unit ? 0 : V - first, tokens_of(P, chunk), P.wide_v);
     };
     if (walk.begin < walk.end) fetch(walk.begin);
     for (int chunk = walk.begin; chunk < walk.end; ++chunk) {
@@ -280,9 +379,7 @@ __global__ __launch_bounds__(kThreads) void delta_forward_kernel(RuleParams P) {
         const int tokens = tokens_of(P, chunk);
         if (chunk > walk.begin) __syncthreads();
         next.template put<NP>(P, lds.rows, lds.x, lds.p, lds.gates, env, head, t0, tokens);
-        f4 values[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) values[i] = to_floats(v_next[i]);
+        const ColumnFetch<E> values = v_next;
         __syncthreads();
         if (chunk + 1 < walk.end) fetch(chunk + 1);
         if (!walk.working) continue;
@@ -292,7 +389,12 @@ __global__ __launch_bounds__(kThreads) void delta_forward_kernel(RuleParams P) {
         f4 u[4], o[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) u[i] = o[i] = f4{0, 0, 0, 0};
-        if (chunk > walk.begin || walk.from || walk.unit) {
+        // (a state that the chunk's first token forgets may hold anything)
+        const bool forgotten = lds.gates[0][0] == 0.0f;
+        if (forgotten)
+#pragma unroll
+            for (int c = 0; c < KP / 16; ++c) state[c] = f4{0, 0, 0, 0};
+        if (!forgotten && (chunk > walk.begin || walk.from || walk.unit)) {
 #pragma unroll
             for (int m = 0; m < KP / 32; ++m) {
                 u4 b[3], a[4][N];
@@ -305,24 +407,21 @@ __global__ __launch_bounds__(kThreads) void delta_forward_kernel(RuleParams P) {
                     first_planes(b, b_out);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) operand_rows(lane, lds.rows.q, 16 * i, m, a[i]);
-                    mma_each<4>(a, b_out, o);
+                    mma_each_transposed<4>(a, b_out, o);
                 }
             }
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            u[i] = -four(lds.gates[0], 16 * i + 4 * g) * u[i];
+            o[i] = P.r.scale * lds.gates[0][16 * i + (lane & 15)] * o[i];
+        }
+        values.add(u);
         u4 r[2][3];
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
-            f4 x[2];
+        for (int m = 0; m < 2; ++m) split8(u[2 * m], u[2 * m + 1], r[m]);
 #pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                const int i = 2 * m + n;
-                const f4 e = four(lds.gates[0], 16 * i + 4 * g);
-                x[n] = values[i] - gated(u[i], e);
-                o[i] = P.r.scale * gated(o[i], e);
-                u[i] = f4{0, 0, 0, 0};
-            }
-            split8(x[0], x[1], r[m]);
-        }
+        for (int i = 0; i < 4; ++i) u[i] = f4{0, 0, 0, 0};
         times_triangle<3>(lane, lds.x, r, u);
         if (!kSummary && P.r.updates)
             rows_state.store<4>(rows_state.rows(P.r.updates + (sequence * P.r.steps + t0) * V + first, tokens),
@@ -333,17 +432,16 @@ __global__ __launch_bounds__(kThreads) void delta_forward_kernel(RuleParams P) {
         for (int m = 0; m < 2; ++m)
             split8(u[2 * m] * four(lds.gates[1], 32 * m + 4 * g), u[2 * m + 1] * four(lds.gates[1], 32 * m + 16 + 4 * g), r[m]);
 #pragma unroll
-        for (int c = 0; c < KP / 16; ++c) state[c] = gated(state[c], f4{keep, keep, keep, keep});
+        for (int c = 0; c < KP / 16; ++c) state[c] = keep * state[c];
 #pragma unroll
         for (int c = 0; c < KP / 16; c += 4) add_columns(lane, lds.rows.k, c, r, state);
         if constexpr (!kSummary) {
             u4 w[2][NP];
 #pragma unroll
             for (int m = 0; m < 2; ++m) split8(u[2 * m], u[2 * m + 1], w[m]);
-            times_triangle<NP>(lane, lds.p, w, o);
-            rows_out.template store<4>(
-                rows_out.rows(static_cast<E*>(P.r.out) + ((env * P.r.steps + t0) * P.r.value_heads + head) * V + first, tokens),
-                [&](int i, int s) { return from_float<E>(o[i][s]); });
+            times_triangle_transposed<NP>(lane, lds.p, w, o);
+            store_transposed(static_cast<E*>(P.r.out) + ((env * P.r.steps + t0) * P.r.value_heads + head) * V + first,
+                             static_cast<int64_t>(P.r.value_heads) * V, V - first, tokens, o);
         }
     }
     if (walk.to && walk.working) store_state<KP>(rows_state, walk.to + first, K, state);
@@ -356,35 +454,36 @@ __global__ __launch_bounds__(kThreads) void delta_forward_kernel(RuleParams P) {
 //     dS <- E_last dS + q^T (scale E do) - k^T (E dr)
 //
 // dS and dr go to memory for delta_gradients_kernel.
-template <class E, int KP, int kThreads, bool kSummary>
-__global__ __launch_bounds__(kThreads) void delta_reverse_kernel(RuleParams P) {
+template <class E, int KP, bool kSummary>
+__global__ __launch_bounds__((kWalkThreads<E, KP>), 2) void delta_reverse_kernel(RuleParams P) {
     constexpr int N = kPlanes<E>;
     extern __shared__ char lds_bytes[];
     auto& lds = *reinterpret_cast<ScanLds<E, KP, 3>*>(lds_bytes);
     const int wave = wave_of_workgroup(), lane = threadIdx.x & 63, g = lane >> 4;
-    const int64_t sequence = blockIdx.x;
+    int64_t sequence;
+    int block;
+    if (!Walk::place<kWalkColumns<E, KP>>(P, kSummary ? P.summary_blocks : P.blocks, sequence, block)) return;
     const int64_t env = sequence / P.r.value_heads;
     const int head = static_cast<int>(sequence % P.r.value_heads);
     const int K = P.r.key_dim, V = P.r.value_dim;
-    const Walk walk = Walk::of<kSummary>(P, sequence, (blockIdx.y * (kThreads / 64) + wave) * 16, P.d.grad_final_state,
+    const Walk walk = Walk::of<kSummary>(P, sequence, block + 16 * wave, P.d.grad_final_state,
                                          P.d.d_initial_state);
     const int first = walk.first;
     const ChunkMatrices* matrices = reinterpret_cast<const ChunkMatrices*>(P.r.matrices) + sequence * P.n_chunks;
     const E* grad = at<E>(P.d.grad_out, P.d.grad_out_stride, env, 0, head) + first;
-    const Columns<E> rows_grad(P.d.grad_out_stride[1], walk.unit ? 0 : V - first),
-        rows_v(static_cast<int64_t>(P.r.value_heads) * V, V - first);
+    const Columns<E> rows_v(static_cast<int64_t>(P.r.value_heads) * V, V - first);
     const Columns<float> rows_state(walk.columns, walk.columns - first);
 
     f4 dstate[KP / 16];
     walk.begin_state<KP>(rows_state, K, dstate);
 
-    ChunkFetch<E, KP, kThreads, true> next;
-    E grad_next[4][4];
+    ChunkFetch<E, KP, kWalkThreads<E, KP>, true> next;
+    ColumnFetch<E> grad_next;
     const auto fetch = [&](int chunk) {
         const int64_t t0 = static_cast<int64_t>(chunk) * kChunk;
         next.fetch(P, matrices[chunk], env, head, t0, tokens_of(P, chunk));
-        rows_grad.template load<4>(rows_grad.rows(grad + t0 * P.d.grad_out_stride[1], tokens_of(P, chunk)),
-                                   [&](int i, int s, E x) { grad_next[i][s] = x; });
+        grad_next.fetch(grad + t0 * P.d.grad_out_stride[1], P.d.grad_out_stride[1], walk.unit ? 0 : V - first,
+                        tokens_of(P, chunk), P.wide_do);
     };
     const int last = P.n_chunks - 1;
     if (walk.begin < walk.end) fetch(last - walk.begin);
@@ -394,18 +493,17 @@ __global__ __launch_bounds__(kThreads) void delta_reverse_kernel(RuleParams P) {
         const int tokens = tokens_of(P, chunk);
         if (step > walk.begin) __syncthreads();
         next.template put<3>(P, lds.rows, lds.x, lds.p, lds.gates, env, head, t0, tokens);
-        f4 dO[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) dO[i] = to_floats(grad_next[i]);
+        const ColumnFetch<E> grads = grad_next;
         __syncthreads();
         if (step + 1 < walk.end) fetch(chunk - 1);
         if (!walk.working) continue;
 
         if (!kSummary && step > 0)
             store_state<KP>(rows_state, P.dstates + (sequence * (P.n_chunks - 1) + chunk) * K * V + first, K, dstate);
-        f4 du[4];
+        f4 du[4], dO[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) du[i] = f4{0, 0, 0, 0};
+        for (int i = 0; i < 4; ++i) du[i] = dO[i] = f4{0, 0, 0, 0};
+        grads.add(dO);
         if (step > walk.begin || walk.from || walk.unit) {
 #pragma unroll
             for (int m = 0; m < KP / 32; ++m) {
@@ -446,7 +544,7 @@ __global__ __launch_bounds__(kThreads) void delta_reverse_kernel(RuleParams P) {
                 dO[j] = P.r.scale * e * dO[j];
             }
 #pragma unroll
-            for (int c = 0; c < KP / 16; ++c) dstate[c] = gated(dstate[c], f4{keep, keep, keep, keep});
+            for (int c = 0; c < KP / 16; ++c) dstate[c] = keep * dstate[c];
 #pragma unroll
             for (int m = 0; m < 2; ++m) split8(du[2 * m], du[2 * m + 1], b[m]);
 #pragma unroll
@@ -633,45 +731,6 @@ __device__ inline float sum16(float x) {  // over 16 lanes in a row
     x += moved(x, std::integral_constant<int, 0x140>{});  // the other eight
     return x;
 }
-
-// Numbers of a row from `offset` bytes on: in 16-byte loads where rows are multiples of eight,
-// else one by one, those from `valid` on as zeros.
-template <class T, int kCount>
-struct Part {
-    static constexpr int kWords = kCount * sizeof(T) / 16;
-    u4 words[kWords];
-
-    __device__ void load(Buffer from, uint32_t offset, int valid, bool wide) {
-        if (wide) {
-            const uint32_t lane = valid > 0 ? offset : kOutside;
-#pragma unroll
-            for (int w = 0; w < kWords; ++w) words[w] = buffer_load16(from, lane + 16 * w);
-            return;
-        }
-        uint32_t x[kCount];
-#pragma unroll
-        for (int i = 0; i < kCount; ++i) {
-            const T y = buffer_load<T>(from, i < valid ? offset + i * sizeof(T) : kOutside);
-            if constexpr (sizeof(T) == 4)
-                x[i] = bits_of(y);
-            else
-                x[i] = __builtin_bit_cast(uint16_t, y);
-        }
-#pragma unroll
-        for (int i = 0; i < 4 * kWords; ++i)
-            words[i / 4][i % 4] = sizeof(T) == 4 ? x[i] : x[2 * i % kCount] | x[(2 * i + 1) % kCount] << 16;
-    }
-
-    __device__ void floats(float (&x)[kCount]) const {
-#pragma unroll
-        for (int i = 0; i < kCount; ++i) {
-            if constexpr (sizeof(T) == 4)
-                x[i] = float_of(words[i / 4][i % 4]);
-            else
-                x[i] = to_float(__builtin_bit_cast(T, static_cast<uint16_t>(words[0][i / 2] >> (16 * (i % 2)))));
-        }
-    }
-};
 
 // Four floats into the planes of an operand's lane, its first or second half.
 __device__ inline void stage_part(uint16_t (&tile)[3][64][8], int slot, int half, const float (&x)[4]) {
@@ -1089,50 +1148,53 @@ int launched(const char* what) {
     return NAVI_POLICY_OK;
 }
 
-// Columns of a head that a workgroup takes: up to 64, or up to 128 where the head has more.
-int columns_of(int value_dim) { return value_dim <= 64 ? 64 : 128; }
-
-int blocks_of(int value_dim) { return (value_dim + columns_of(value_dim) - 1) / columns_of(value_dim); }
-
-// Walks in segments: 0 workgroups of a whole walk are too few to fill the card's 256 CUs, and
-// the chunks enough that the summary pass and the join (about as long as four chunks) pay.
-int segments_of(int64_t sequences, int value_dim, int64_t chunks) {
-    const int64_t blocks = sequences * blocks_of(value_dim);
-    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({256 / std::max<int64_t>(1, blocks), chunks / 4, 16})));
+int blocks_of(const navi_delta_rule& r, int columns) {
+    const int each = r.dtype == NAVI_POLICY_F32 && r.key_dim > 64 ? kWalkColumns<float, 128> : kWalkColumns<bf16, 64>;
+    return (columns + each - 1) / each;
 }
 
-int64_t segment_floats(int64_t sequences, int key_dim, int value_dim, int segments) {
-    return sequences * (segments - 1) * (static_cast<int64_t>(key_dim) * value_dim + key_dim * key_dim);
+int64_t chunks_of(int64_t steps) { return (steps + kChunk - 1) / kChunk; }
+
+// Segments of a walk: one where workgroups of 64 columns for whole walks fill the card's 256 CUs; else
+// as many as do, as long as each has enough chunks that the summary pass and the join pay (the join
+// takes about as long as a chunk for each segment). 2 x 4001 steps, 8 heads of 128: 434 us forward
+// and back in 8 segments, 498 in 16, 515 in 4; 8 x 2048 steps, 8 heads of 64: 299 in 4, 375 in 2.
+int segments_of(const navi_delta_rule& r) {
+    const int64_t blocks = r.envs * r.value_heads * ((r.value_dim + 63) / 64);
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({256 / std::max<int64_t>(1, blocks), chunks_of(r.steps) / 4, 16})));
 }
 
-template <class E, int KP, int kThreads, bool kBack, bool kSummary>
-int walk(const RuleParams& P, dim3 grid, hipStream_t stream) {
+int64_t segment_floats(const navi_delta_rule& r) {
+    return r.envs * r.value_heads * (segments_of(r) - 1) * (static_cast<int64_t>(r.key_dim) * r.value_dim + r.key_dim * r.key_dim);
+}
+
+template <class E, int KP, bool kBack, bool kSummary>
+int walk(const RuleParams& P, unsigned segments, hipStream_t stream) {
     constexpr size_t lds = sizeof(ScanLds<E, KP, kBack ? 3 : kOutPlanes<E>>);
+    const int64_t blocks = (P.r.envs * P.r.value_heads + 7) / 8 * 8 * (kSummary ? P.summary_blocks : P.blocks);
+    if (blocks > INT32_MAX) return set_error(NAVI_POLICY_E_ARG, "envs * value_heads * value_dim is too large");
+    const dim3 grid(static_cast<unsigned>(blocks), 1, segments), threads(kWalkThreads<E, KP>);
     if constexpr (kBack)
-        hipLaunchKernelGGL((delta_reverse_kernel<E, KP, kThreads, kSummary>), grid, dim3(kThreads), lds, stream, P);
+        hipLaunchKernelGGL((delta_reverse_kernel<E, KP, kSummary>), grid, threads, lds, stream, P);
     else
-        hipLaunchKernelGGL((delta_forward_kernel<E, KP, kThreads, kSummary>), grid, dim3(kThreads), lds, stream, P);
+        hipLaunchKernelGGL((delta_forward_kernel<E, KP, kSummary>), grid, threads, lds, stream, P);
     return launched("the gated delta rule");
 }
 
 template <class E, int KP, bool kBack>
 int walk_all(const RuleParams& P, hipStream_t stream) {
-    const unsigned sequences = static_cast<unsigned>(P.r.envs * P.r.value_heads);
     const unsigned segments = static_cast<unsigned>(P.n_segments);
     if (segments > 1) {
-        const int columns = (P.r.value_dim + 15) / 16 * 16 + P.r.key_dim;
-        int code = walk<E, KP, 256, kBack, true>(P, dim3(sequences, (columns + 63) / 64, segments - 1), stream);
+        int code = walk<E, KP, kBack, true>(P, segments - 1, stream);
         if (code != NAVI_POLICY_OK) return code;
         if (segments > 2) {
-            hipLaunchKernelGGL(delta_join_kernel<KP>, dim3(sequences, (P.r.value_dim + 63) / 64), dim3(256),
-                               KP * KP * 6, stream, P);
+            const dim3 grid(static_cast<unsigned>(P.r.envs * P.r.value_heads), (P.r.value_dim + 63) / 64);
+            hipLaunchKernelGGL(delta_join_kernel<KP>, grid, dim3(256), KP * KP * 6, stream, P);
             code = launched("the gated delta rule");
             if (code != NAVI_POLICY_OK) return code;
         }
     }
-    const dim3 grid(sequences, blocks_of(P.r.value_dim), segments);
-    return columns_of(P.r.value_dim) == 64 ? walk<E, KP, 256, kBack, false>(P, grid, stream)
-                                           : walk<E, KP, 512, kBack, false>(P, grid, stream);
+    return walk<E, KP, kBack, false>(P, segments, stream);
 }
 
 template <class E, int KP>
@@ -1172,13 +1234,17 @@ int run_typed(const RuleParams& P, bool back, hipStream_t stream) {
     return run<f16>(P, back, stream);
 }
 
-int64_t chunks_of(int64_t steps) { return (steps + kChunk - 1) / kChunk; }
-
 // Whether the rows of steps lie one after another, 64 of them within reach of a buffer access
 // (the bytes from one to the next times 64, and a row, stay below 2^31).
 constexpr int64_t kFarthest = INT32_MAX / kChunk - 65536 * 4;
 bool rows_apart(const int64_t (&stride)[3], int64_t bytes, int64_t dim) {
     return stride[1] >= dim && stride[1] <= kFarthest / bytes;
+}
+
+// 16-byte buffer loads need addresses of whole 4-byte words, and rows that end between them.
+bool wide_columns(const void* p, const int64_t (&stride)[3], int64_t bytes, int64_t dim) {
+    return reinterpret_cast<uintptr_t>(p) % 4 == 0 && dim % 8 == 0 && stride[0] * bytes % 4 == 0 && stride[1] * bytes % 4 == 0 &&
+           stride[2] * bytes % 4 == 0;
 }
 
 bool wide_rows(const void* p, const int64_t (&stride)[3], int64_t bytes, int64_t dim) {
@@ -1215,7 +1281,9 @@ int setup(const navi_delta_rule* r, RuleParams& P) {
     P.r = *r;
     P.group = r->value_heads / r->key_heads;
     P.n_chunks = static_cast<int32_t>(chunks_of(r->steps));
-    P.n_segments = segments_of(r->envs * r->value_heads, r->value_dim, P.n_chunks);
+    P.blocks = blocks_of(*r, r->value_dim);
+    P.summary_blocks = blocks_of(*r, (r->value_dim + 15) / 16 * 16 + r->key_dim);
+    P.n_segments = segments_of(*r);
     const int64_t bytes = r->dtype == NAVI_POLICY_F32 ? 4 : 2;
     if (r->envs * r->value_heads * chunks_of(r->steps) > INT32_MAX)
         return set_error(NAVI_POLICY_E_ARG, "envs * value_heads * chunks must be below 2^31");
@@ -1231,6 +1299,7 @@ int setup(const navi_delta_rule* r, RuleParams& P) {
           rows_apart(P.r.v_stride, bytes, r->value_dim)) && r->steps > 0)
         return set_error(NAVI_POLICY_E_ARG, "the steps of q, k and v overlap or lie too far apart");
     P.wide_qk = wide_rows(r->q, P.r.q_stride, bytes, r->key_dim) && wide_rows(r->k, P.r.k_stride, bytes, r->key_dim);
+    P.wide_v = wide_columns(r->v, P.r.v_stride, bytes, r->value_dim);
     return NAVI_POLICY_OK;
 }
 
@@ -1262,9 +1331,7 @@ extern "C" int navi_delta_forward(const navi_delta_rule* rule, void* stream) {
 extern "C" int64_t navi_delta_scratch(const navi_delta_rule* rule) {
     const int code = check_rule(rule);
     if (code < 0) return code;
-    const int64_t sequences = rule->envs * rule->value_heads;
-    return 4 * segment_floats(sequences, rule->key_dim, rule->value_dim,
-                              segments_of(sequences, rule->value_dim, chunks_of(rule->steps)));
+    return 4 * segment_floats(*rule);
 }
 
 extern "C" int64_t navi_delta_workspace(const navi_delta_rule* rule) {
@@ -1276,9 +1343,7 @@ extern "C" int64_t navi_delta_workspace(const navi_delta_rule* rule) {
     const int64_t rows = sequences * steps * rule->value_dim;
     const int64_t heads = rule->value_heads > rule->key_heads ? sequences * steps * rule->key_dim : 0;
     const auto rounded = [](int64_t n) { return (n + 3) / 4 * 4; };
-    const int64_t segments = segment_floats(sequences, rule->key_dim, rule->value_dim,
-                                            segments_of(sequences, rule->value_dim, chunks_of(steps)));
-    return 4 * (rounded(states) + rounded(rows) + 2 * rounded(heads) + segments);
+    return 4 * (rounded(states) + rounded(rows) + 2 * rounded(heads) + segment_floats(*rule));
 }
 
 extern "C" int navi_delta_backward(const navi_delta_rule* rule, const navi_delta_gradients* gradients, void* stream) {
@@ -1304,10 +1369,7 @@ extern "C" int navi_delta_backward(const navi_delta_rule* rule, const navi_delta
     if (rule->steps == 1) P.d.grad_out_stride[1] = rule->value_dim;
     if (!rows_apart(P.d.grad_out_stride, bytes, rule->value_dim))
         return set_error(NAVI_POLICY_E_ARG, "the steps of grad_out overlap or lie too far apart");
-    // (16-byte buffer loads need addresses of whole 4-byte words)
     P.wide_state = rule->value_dim % 8 == 0;
-    P.wide_do = P.wide_state && reinterpret_cast<uintptr_t>(P.d.grad_out) % 4 == 0 &&
-                P.d.grad_out_stride[0] * bytes % 4 == 0 && P.d.grad_out_stride[1] * bytes % 4 == 0 &&
-                P.d.grad_out_stride[2] * bytes % 4 == 0;
+    P.wide_do = wide_columns(P.d.grad_out, P.d.grad_out_stride, bytes, rule->value_dim);
     return run_typed(P, true, as_stream(stream));
 }

@@ -129,6 +129,19 @@ __device__ inline void mma_each(const u4 (&a)[kCount][NA], const u4 (&b)[NB], f4
                 for (int n = 0; n < kCount; ++n) c[n] = mfma(a[n][i], b[s - i], c[n]);
 }
 
+// The same, each result transposed: the operands hold rows and columns alike, so exchanging them
+// does. A lane then has row l % 16 of the result, columns 4 (l / 16) to 4 (l / 16) + 3.
+template <int kCount, int NA, int NB>
+__device__ inline void mma_each_transposed(const u4 (&a)[kCount][NA], const u4 (&b)[NB], f4 (&c)[kCount]) {
+#pragma unroll
+    for (int s = (NA + NB - 2 < 2 ? NA + NB - 2 : 2); s >= 0; --s)
+#pragma unroll
+        for (int i = 0; i < NA; ++i)
+            if (s - i >= 0 && s - i < NB)
+#pragma unroll
+                for (int n = 0; n < kCount; ++n) c[n] = mfma(b[s - i], a[n][i], c[n]);
+}
+
 // 16x16x4 in float32: A's lane holds row l % 16, B's column l % 16, at l / 16 of the four.
 __device__ inline f4 mfma_f32(float a, float b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 
@@ -169,6 +182,60 @@ __device__ inline void buffer_store(Buffer to, uint32_t offset, E x) {
 __device__ inline u4 buffer_load16(Buffer from, uint32_t offset) {
     return __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(from, offset, 0, 0));
 }
+
+// Four numbers of a row in one store (the address a multiple of their bytes).
+__device__ inline void buffer_store_four(Buffer to, uint32_t offset, const bf16 (&x)[4]) {
+    __builtin_amdgcn_raw_buffer_store_b64(u2{x[0].bits | static_cast<uint32_t>(x[1].bits) << 16,
+                                             x[2].bits | static_cast<uint32_t>(x[3].bits) << 16}, to, offset, 0, 0);
+}
+__device__ inline void buffer_store_four(Buffer to, uint32_t offset, const f16 (&x)[4]) {
+    bf16 y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i].bits = __builtin_bit_cast(uint16_t, x[i].value);
+    buffer_store_four(to, offset, y);
+}
+__device__ inline void buffer_store_four(Buffer to, uint32_t offset, const float (&x)[4]) {
+    __builtin_amdgcn_raw_buffer_store_b128(u4{bits_of(x[0]), bits_of(x[1]), bits_of(x[2]), bits_of(x[3])}, to, offset, 0, 0);
+}
+
+// Numbers of a row from `offset` bytes on: in 16-byte loads where rows are multiples of eight,
+// else one by one, those from `valid` on as zeros.
+template <class T, int kCount>
+struct Part {
+    static constexpr int kWords = kCount * sizeof(T) / 16;
+    u4 words[kWords];
+
+    __device__ void load(Buffer from, uint32_t offset, int valid, bool wide) {
+        if (wide) {
+            const uint32_t lane = valid > 0 ? offset : kOutside;
+#pragma unroll
+            for (int w = 0; w < kWords; ++w) words[w] = buffer_load16(from, lane + 16 * w);
+            return;
+        }
+        uint32_t x[kCount];
+#pragma unroll
+        for (int i = 0; i < kCount; ++i) {
+            const T y = buffer_load<T>(from, i < valid ? offset + i * sizeof(T) : kOutside);
+            if constexpr (sizeof(T) == 4)
+                x[i] = bits_of(y);
+            else
+                x[i] = __builtin_bit_cast(uint16_t, y);
+        }
+#pragma unroll
+        for (int i = 0; i < 4 * kWords; ++i)
+            words[i / 4][i % 4] = sizeof(T) == 4 ? x[i] : x[2 * i % kCount] | x[(2 * i + 1) % kCount] << 16;
+    }
+
+    __device__ void floats(float (&x)[kCount]) const {
+#pragma unroll
+        for (int i = 0; i < kCount; ++i) {
+            if constexpr (sizeof(T) == 4)
+                x[i] = float_of(words[i / 4][i % 4]);
+            else
+                x[i] = to_float(__builtin_bit_cast(T, static_cast<uint16_t>(words[0][i / 2] >> (16 * (i % 2)))));
+        }
+    }
+};
 
 inline hipStream_t as_stream(void* stream) { return static_cast<hipStream_t>(stream); }
 
