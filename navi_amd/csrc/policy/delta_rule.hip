@@ -558,88 +558,6 @@ __global__ __launch_bounds__((kWalkThreads<E, KP>), 2) void delta_reverse_kernel
     if (walk.to && walk.working) store_state<KP>(rows_state, walk.to + first, K, dstate);
 }
 
-// The states before the segments but the first, one after another, from what the summary left
-// of each: S <- M S + N with N the state that it makes of zeros (of the given state, for
-// segment 0) and M its matrix. Takes N's place. A workgroup holds 64 columns; M's planes go
-// through LDS.
-template <int KP>
-__global__ __launch_bounds__(256) void delta_join_kernel(RuleParams P) {
-    extern __shared__ char lds_bytes[];
-    auto& m_planes = *reinterpret_cast<uint16_t(*)[KP / 16][KP / 32][3][64][8]>(lds_bytes);
-    const int wave = wave_of_workgroup();
-    const int64_t sequence = blockIdx.x;
-    const int first = (blockIdx.y * 4 + wave) * 16;
-    const int K = P.r.key_dim, V = P.r.value_dim;
-    const int64_t kv = static_cast<int64_t>(K) * V, slots = sequence * (P.n_segments - 1);
-    const Columns<float> rows_state(V, V - first);
-    f4 state[KP / 16], next[KP / 16];
-    load_state<KP>(rows_state, P.segment_states + slots * kv + first, K, state);
-    // of a segment while the one before it is computed: its N, and an operand's parts of its M (a
-    // lane holds columns 4 g and 16 + 4 g on of 32, in the order of results)
-    constexpr int kParts = KP * KP / 8 / 256;
-    f4 part[kParts][2];
-    const bool wide = K % 4 == 0;
-    const auto fetch = [&](int segment) {
-        const Buffer matrix = buffer_of(P.segment_matrices + (slots + segment) * K * K, 4 * K * K);
-        load_state<KP>(rows_state, P.segment_states + (slots + segment) * kv + first, K, next);
-#pragma unroll
-        for (int n = 0; n < kParts; ++n) {
-            const int at = threadIdx.x + 256 * n, lane = at & 63, m = (at >> 6) % (KP / 32), c = (at >> 6) / (KP / 32);
-            const int row = 16 * c + (lane & 15);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int column = 32 * m + 4 * (lane >> 4) + 16 * h;
-                const uint32_t offset = 4 * (row * K + column);
-                if (wide) {
-                    part[n][h] = __builtin_bit_cast(f4, buffer_load16(matrix, row < K && column < K ? offset : kOutside));
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        part[n][h][i] = buffer_load<float>(matrix, row < K && column + i < K ? offset + 4 * i : kOutside);
-                }
-            }
-        }
-    };
-    if (P.n_segments > 2) fetch(1);
-    for (int segment = 1; segment + 1 < P.n_segments; ++segment) {
-        if (segment > 1) __syncthreads();
-#pragma unroll
-        for (int n = 0; n < kParts; ++n) {
-            const int at = threadIdx.x + 256 * n;
-            u4 plane[3];
-            split8(part[n][0], part[n][1], plane);
-#pragma unroll
-            for (int i = 0; i < 3; ++i) *reinterpret_cast<u4*>(m_planes[(at >> 6) / (KP / 32)][(at >> 6) % (KP / 32)][i][at & 63]) = plane[i];
-        }
-        f4 x[KP / 16];
-#pragma unroll
-        for (int c = 0; c < KP / 16; ++c) x[c] = next[c];
-        __syncthreads();
-        if (segment + 2 < P.n_segments) fetch(segment + 1);
-#pragma unroll
-        for (int m = 0; m < KP / 32; ++m) {
-            u4 b[3];
-            split8(state[2 * m], state[2 * m + 1], b);
-#pragma unroll
-            for (int c = 0; c < KP / 16; c += 4) {
-                u4 a[4][3];
-                f4 y[4] = {x[c], x[c + 1], x[c + 2], x[c + 3]};
-#pragma unroll
-                for (int n = 0; n < 4; ++n)
-#pragma unroll
-                    for (int i = 0; i < 3; ++i)
-                        a[n][i] = *reinterpret_cast<const u4*>(m_planes[c + n][m][i][threadIdx.x & 63]);
-                mma_each<4>(a, b, y);
-#pragma unroll
-                for (int n = 0; n < 4; ++n) x[c + n] = y[n];
-            }
-        }
-#pragma unroll
-        for (int c = 0; c < KP / 16; ++c) state[c] = x[c];
-        store_state<KP>(rows_state, P.segment_states + (slots + segment) * kv + first, K, state);
-    }
-}
-
 // Sixteen rows of results, KP / 16 tiles across, into `rows` rows of `columns` numbers.
 template <class T, int KP>
 __device__ inline void store_tiles(T* base, int64_t stride, int rows, int columns, const f4 (&x)[KP / 16]) {
@@ -744,6 +662,77 @@ __device__ inline void stage_part(uint16_t (&tile)[3][64][8], int slot, int half
 __device__ inline void staged_operand(int lane, const uint16_t (&tile)[3][64][8], u4 (&x)[3]) {
 #pragma unroll
     for (int n = 0; n < 3; ++n) x[n] = *reinterpret_cast<const u4*>(tile[n][lane]);
+}
+
+// The states before the segments but the first, one after another, from what the summary left
+// of each: S <- M S + N with N the state that it makes of zeros (of the given state, for
+// segment 0) and M its matrix. Takes N's place. A workgroup holds 16 columns, its four waves a
+// quarter of the rows each: M's rows come straight into the wave that multiplies with them, S's
+// planes go through LDS. A chain of products that only waiting bounds.
+template <int KP>
+__global__ __launch_bounds__(256) void delta_join_kernel(RuleParams P) {
+    constexpr int kOwn = KP / 64;  // tiles of a wave's rows
+    __shared__ alignas(16) uint16_t planes[2][KP / 32][3][64][8];
+    const int wave = wave_of_workgroup(), lane = threadIdx.x & 63;
+    const int64_t sequence = blockIdx.x;
+    const int first = blockIdx.y * 16, top = 16 * kOwn * wave;
+    const int K = P.r.key_dim, V = P.r.value_dim;
+    const int64_t kv = static_cast<int64_t>(K) * V, slots = sequence * (P.n_segments - 1);
+    const Columns<float> columns(V, V - first);
+    const auto rows_of = [&](int segment) {
+        return columns.rows(P.segment_states + (slots + segment) * kv + static_cast<int64_t>(top) * V + first, K - top);
+    };
+    f4 state[kOwn], next[kOwn], part[kOwn][KP / 32][2];
+    const bool wide = K % 4 == 0;
+    // Of a segment while the one before it is computed: its N, and the wave's rows of its M as
+    // operands (a lane holds columns 4 g and 16 + 4 g on of 32, in the order of results)
+    const auto fetch = [&](int segment) {
+        const Buffer matrix = buffer_of(P.segment_matrices + (slots + segment) * K * K, 4 * K * K);
+#pragma unroll
+        for (int c = 0; c < kOwn; ++c)
+#pragma unroll
+            for (int m = 0; m < KP / 32; ++m)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int row = top + 16 * c + (lane & 15), column = 32 * m + 4 * (lane >> 4) + 16 * h;
+                    const uint32_t offset = 4 * (row * K + column);
+                    if (wide) {
+                        part[c][m][h] = __builtin_bit_cast(f4, buffer_load16(matrix, row < K && column < K ? offset : kOutside));
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            part[c][m][h][i] = buffer_load<float>(matrix, row < K && column + i < K ? offset + 4 * i : kOutside);
+                    }
+                }
+        columns.load<kOwn>(rows_of(segment), [&](int c, int s, float x) { next[c][s] = x; });
+    };
+    columns.load<kOwn>(rows_of(0), [&](int c, int s, float x) { state[c][s] = x; });
+    fetch(1);
+    for (int segment = 1; segment + 1 < P.n_segments; ++segment) {
+        auto& shared = planes[segment & 1];  // (who still reads the other has passed the last barrier but one)
+#pragma unroll
+        for (int c = 0; c < kOwn; ++c) {
+            const int tile = kOwn * wave + c;
+            const float x[4] = {state[c][0], state[c][1], state[c][2], state[c][3]};
+            stage_part(shared[tile / 2], lane, tile % 2, x);
+        }
+        u4 a[KP / 32][kOwn][3];
+#pragma unroll
+        for (int c = 0; c < kOwn; ++c) {
+            state[c] = next[c];
+#pragma unroll
+            for (int m = 0; m < KP / 32; ++m) split8(part[c][m][0], part[c][m][1], a[m][c]);
+        }
+        __syncthreads();
+        if (segment + 2 < P.n_segments) fetch(segment + 1);
+#pragma unroll
+        for (int m = 0; m < KP / 32; ++m) {
+            u4 b[3];
+            staged_operand(lane, shared[m], b);
+            mma_each<kOwn>(a[m], b, state);
+        }
+        columns.store<kOwn>(rows_of(segment), [&](int c, int s) { return state[c][s]; });
+    }
 }
 
 // A triangle's rows times 32 rows in LDS.
@@ -1155,13 +1144,17 @@ int blocks_of(const navi_delta_rule& r, int columns) {
 
 int64_t chunks_of(int64_t steps) { return (steps + kChunk - 1) / kChunk; }
 
-// Segments of a walk: one where workgroups of 64 columns for whole walks fill the card's 256 CUs; else
-// as many as do, as long as each has enough chunks that the summary pass and the join pay (the join
-// takes about as long as a chunk for each segment). 2 x 4001 steps, 8 heads of 128: 434 us forward
-// and back in 8 segments, 498 in 16, 515 in 4; 8 x 2048 steps, 8 heads of 64: 299 in 4, 375 in 2.
+// Segments of a walk, at most 16: one where workgroups of 64 columns for whole walks fill half of the
+// card's 256 CUs (192 sequences of 4096 steps, one head of 64, forward: 336 us in 1, 367 in 2; 128:
+// 266 in 4, 274 in 2); else as many as give each CU a workgroup, of four chunks or more, for the join
+// takes about half as long as a chunk for each. A second workgroup to a CU gives less and needs
+// segments of eight chunks. 2 x 4001 steps, 8 heads of 128: 408 us forward and back in 8 segments, 443
+// in 15; 16384 steps, 16 heads of 128, forward: 347 us in 16, 363 in 8.
 int segments_of(const navi_delta_rule& r) {
-    const int64_t blocks = r.envs * r.value_heads * ((r.value_dim + 63) / 64);
-    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({256 / std::max<int64_t>(1, blocks), chunks_of(r.steps) / 4, 16})));
+    const int64_t blocks = std::max<int64_t>(1, r.envs * r.value_heads * ((r.value_dim + 63) / 64)), chunks = chunks_of(r.steps);
+    if (blocks > 128) return 1;
+    const int64_t most = std::max(std::min(256 / blocks, chunks / 4), chunks / 8);
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({512 / blocks, most, 16})));
 }
 
 int64_t segment_floats(const navi_delta_rule& r) {
@@ -1188,8 +1181,8 @@ int walk_all(const RuleParams& P, hipStream_t stream) {
         int code = walk<E, KP, kBack, true>(P, segments - 1, stream);
         if (code != NAVI_POLICY_OK) return code;
         if (segments > 2) {
-            const dim3 grid(static_cast<unsigned>(P.r.envs * P.r.value_heads), (P.r.value_dim + 63) / 64);
-            hipLaunchKernelGGL(delta_join_kernel<KP>, grid, dim3(256), KP * KP * 6, stream, P);
+            const dim3 grid(static_cast<unsigned>(P.r.envs * P.r.value_heads), (P.r.value_dim + 15) / 16);
+            hipLaunchKernelGGL(delta_join_kernel<KP>, grid, dim3(256), 0, stream, P);
             code = launched("the gated delta rule");
             if (code != NAVI_POLICY_OK) return code;
         }
