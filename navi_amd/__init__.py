@@ -8,6 +8,9 @@ Layers (top to bottom):
   under the reference's module names.
 * :mod:`navi_amd._native` — ctypes binding of ``libnavi_trace.so`` (C ABI in
   ``include/navi_trace.h``), the hand-written HIP/gfx950 kernels in ``navi_amd/csrc``.
+* :mod:`navi_amd.policy` — operators of a policy with a memory over the observations, in
+  ``libnavi_policy.so`` (C ABI in ``include/policy/navi_policy.h``);
+  :mod:`navi_amd.memory_policy` runs them together.
 
 Importing this package does not load the HIP library; the submodules above do.
 """

@@ -152,7 +152,10 @@ __device__ inline int tokens_of(const RuleParams& P, int chunk) {
     return static_cast<int>(left < kChunk ? left : kChunk);
 }
 
-// The triangles and gates of every chunk, which need no state: a workgroup each.
+// The triangles and gates of every chunk, which need no state: a workgroup each, so that the
+// walks, which go from chunk to chunk, do not wait for a substitution. Bound by memory where there are
+// many chunks: 1024 x 128 steps, 4 heads of 64, bfloat16, 70 us for 134 MB of rows and 172 MB of
+// triangles (4.4 TB/s, a large copy reaches 4.8).
 template <class E, int KP>
 __global__ __launch_bounds__(256) void delta_triangles_kernel(RuleParams P) {
     extern __shared__ char lds_bytes[];
@@ -176,7 +179,8 @@ __global__ __launch_bounds__(256) void delta_triangles_kernel(RuleParams P) {
 }
 
 // What reaches the output alone is rounded with it: for 16-bit outputs, two planes (2^-16)
-// of S, P and u there are far below that rounding (2^-9 and 2^-12).
+// of S, P and u there are far below that rounding (2^-9 and 2^-12). What reaches the state keeps
+// float32's three.
 template <class E>
 inline constexpr int kOutPlanes = sizeof(E) == 4 ? 3 : 2;
 
@@ -344,6 +348,12 @@ __device__ inline void add_columns(int lane, const uint16_t (&rows)[N][kChunk][k
 // four waves 64 of one head; it walks the chunks with the state in registers.
 // The state is the second operand of S^T k without a move: its tiles hold the contracted axis
 // in the order of results, which the rows in LDS are kept in as well.
+//
+// With many sequences memory bounds it: 1024 x 128 steps, 4 heads of 64, bfloat16, with what the
+// gradients need, 150 us for 374 MB read and 269 MB written (4.3 TB/s). With few, the chain from
+// chunk to chunk does: 16384 steps, 16 heads of 128 in 16 segments, 132 us, 8.2 us a chunk of which
+// the products' own time is 2.8 (what lies between: reads of LDS for the operands, splits of
+// the state into planes, two barriers).
 template <class E, int KP, bool kSummary>
 __global__ __launch_bounds__((kWalkThreads<E, KP>), 2) void delta_forward_kernel(RuleParams P) {
     constexpr int N = kPlanes<E>, NP = kOutPlanes<E>;
@@ -453,7 +463,8 @@ __global__ __launch_bounds__((kWalkThreads<E, KP>), 2) void delta_forward_kernel
 //     du = P^T do + beta F (k dS),   dr = X^T du  (= dv),
 //     dS <- E_last dS + q^T (scale E do) - k^T (E dr)
 //
-// dS and dr go to memory for delta_gradients_kernel.
+// dS and dr go to memory for delta_gradients_kernel. Bound as the forward pass is: 148 us for the
+// same traffic at 1024 x 128 steps, 4 heads of 64 (4.3 TB/s).
 template <class E, int KP, bool kSummary>
 __global__ __launch_bounds__((kWalkThreads<E, KP>), 2) void delta_reverse_kernel(RuleParams P) {
     constexpr int N = kPlanes<E>;
@@ -586,7 +597,10 @@ __device__ inline void store_tiles(T* base, int64_t stride, int rows, int column
 // of dr (Z, R, M, the rest of dk), or eight waves one of the two. V is taken 32 columns at a
 // time. With 64 keys of 16 bits three workgroups of four waves fit a CU and hide each other's
 // waits; with more, one or two of eight do (1024 x 128 steps, 4 heads of 64: 299 us with four
-// waves, 430 with eight; 2 x 4001 steps, 8 heads of 128: 165 and 120).
+// waves, 430 with eight; 2 x 4001 steps, 8 heads of 128: 165 and 120). 1024 x 128 steps, 4 heads of 64
+// now take 265 to 297 us for 692 MB read and 243 MB written (3.1 to 3.5 TB/s): what a chunk waits for its
+// rows, and its five products' reads of LDS (a third of the time), bound it. Workgroups that take
+// chunk after chunk, the next one's rows asked for early, spill: 395 us.
 template <class E, int KP>
 inline constexpr int kGradientWaves = KP == 64 && sizeof(E) == 2 ? 4 : 8;
 
@@ -668,7 +682,9 @@ __device__ inline void staged_operand(int lane, const uint16_t (&tile)[3][64][8]
 // of each: S <- M S + N with N the state that it makes of zeros (of the given state, for
 // segment 0) and M its matrix. Takes N's place. A workgroup holds 16 columns, its four waves a
 // quarter of the rows each: M's rows come straight into the wave that multiplies with them, S's
-// planes go through LDS. A chain of products that only waiting bounds.
+// planes go through LDS. A chain of products, each after the one before it: 3 us for one of
+// 128 x 128 (64 columns a workgroup, M's planes in LDS: 4.7 us; products of float32 in place of
+// planes: 3 us as well).
 template <int KP>
 __global__ __launch_bounds__(256) void delta_join_kernel(RuleParams P) {
     constexpr int kOwn = KP / 64;  // tiles of a wave's rows
@@ -1114,7 +1130,8 @@ __global__ __launch_bounds__((64 * kGradientWaves<E, KP>), (kGradientWaves<E, KP
     }
 }
 
-// A key head's gradients are the sum of its value heads', in their order.
+// A key head's gradients are the sum of its value heads', in their order (no atomics: the same
+// result every time). Bound by memory: 16 us for 74 MB at 2 x 4001 steps, 8 heads of 128 (4.6 TB/s).
 template <class E>
 __global__ __launch_bounds__(256) void delta_join_heads_kernel(RuleParams P, int64_t count) {
     const int K = P.r.key_dim;

