@@ -132,9 +132,9 @@ def _check_state(name: str, state, q, v) -> None:
 
 
 # Rollouts of so few steps go token by token: a chunk takes as long for one token as for 64. Four
-# steps and a chunk, us, with the state returned: 1 x 8 heads of 128, 18.2 and 18.0; 64 x 4 of 64,
-# float32, 9.0 and 18.7; 1024 x 4 of 64, 51 and 84; 1024 x 4 of 128, 211 and 215. Eight: 31 and 17.9;
-# 13.5 and 19.0; 81 and 85; 327 and 217.
+# steps and a chunk, us, with the state returned: 1 x 8 heads of 128, 9.4 and 16.4; 64 x 4 of 64,
+# float32, 7.4 and 18.2; 1024 x 4 of 64, 39 and 80; 1024 x 4 of 128, 159 and 176. Eight: 15.5 and 16.7;
+# 11.2 and 18.2; 58 and 80; 232 and 178.
 _STEPWISE = 4
 
 _FARTHEST = ((1 << 31) - 1) // _native.CHUNK - (1 << 18)  # bytes between steps that the chunked kernels reach
