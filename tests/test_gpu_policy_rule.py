@@ -121,6 +121,7 @@ LONG = [  # few heads and many chunks: walked in segments that are joined
     (1, 64 * 9 + 5, 1, 2, 33, 70, torch.bfloat16),
     (2, 64 * 12 + 1, 1, 2, 128, 128, torch.float16),
     (1, 64 * 21 + 63, 1, 1, 100, 150, torch.float32),
+    (8, 64 * 39 + 1, 4, 8, 10, 12, torch.bfloat16),  # (workgroups of five segments: more than one to a CU)
 ]
 
 
@@ -160,6 +161,26 @@ def test_steps_give_what_the_rollout_gives(policy, size):
         o = policy.gated_delta_step(*[a[:, t] for a in x.values()], state, starts=starts[:, t])
         assert ref.off(o, want_o[:, t]) <= tolerance(size[-1], 8 * TOL), t  # (a token's own norm is smaller)
     assert ref.off(state, want_state) <= TOL
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dims", [(64, 64), (128, 36), (100, 33), (31, 5)], ids=str)
+def test_steps_of_views_at_any_address(policy, dims, dtype):
+    """The same numbers in rows that 16-byte loads can read and in rows that they cannot."""
+    x, state, starts = make(5, 2, 2, 4, *dims, dtype, seed=13)
+    x = {n: t[:, 0].contiguous() for n, t in x.items()}
+    whole = state.clone()
+    want = policy.gated_delta_step(*x.values(), whole, starts=starts[:, 0])
+    want_o, want_state = ref.rule(*[t[:, None] for t in x.values()], starts[:, :1], state, dims[0] ** -0.5)
+    assert ref.off(want, want_o[:, 0]) <= tolerance(dtype)
+    assert ref.off(whole, want_state) <= TOL
+    for before, after in ((1, 0), (0, 3), (8, 8)):
+        padded = {n: torch.nn.functional.pad(t, (before, after), value=math.nan) for n, t in x.items() if n in "qkv"}
+        views = {n: padded[n][..., before:before + t.shape[-1]] if n in padded else t for n, t in x.items()}
+        views["g"], views["beta"] = (x[n].t().contiguous().t() for n in ("g", "beta"))
+        own = state.clone()
+        assert torch.equal(policy.gated_delta_step(*views.values(), own, starts=starts[:, 0]), want)
+        assert torch.equal(own, whole)
 
 
 @pytest.mark.parametrize("kind", ["every token", "minus infinity", "decays of 1e4", "no writes", "all writes", "no decay",
@@ -359,6 +380,22 @@ def test_captured_steps_replay(policy):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want[i])
+
+
+def test_captured_rollouts_replay(policy):
+    x, state, starts = make(1, 64 * 17, 1, 2, 64, 64, torch.bfloat16)
+    policy.gated_delta_rule(*x.values(), starts=starts, initial_state=state, return_state=True)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o, final = policy.gated_delta_rule(*x.values(), starts=starts, initial_state=state, return_state=True)
+    for n in range(4):
+        x["v"].copy_(torch.randn(x["v"].shape, device="cuda"))
+        state.normal_()
+        want, want_final = policy.gated_delta_rule(*x.values(), starts=starts, initial_state=state, return_state=True)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(o, want) and torch.equal(final, want_final), n
 
 
 def test_refusals(policy):
