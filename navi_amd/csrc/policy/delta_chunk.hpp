@@ -462,8 +462,7 @@ struct ChunkFetch {
         }
     }
 
-    template <int NP>
-    __device__ void put(const RuleParams& P, ChunkRows<E, KP>& rows, Triangle<3>& x, Triangle<NP>& p, float (&gates)[2][kChunk],
+    __device__ void put(const RuleParams& P, ChunkRows<E, KP>& rows, Triangle<3>& x, Triangle<3>& p, float (&gates)[2][kChunk],
                         int64_t env, int head, int64_t t0, int tokens) const {
         if (P.wide_qk) {
             put_rows(rows, q, k);
@@ -476,7 +475,7 @@ struct ChunkFetch {
             if (n < kTiles * 64)
                 store_slot<3>(x, n >> 6, n & 63, slot[i]);
             else if (kAll && n < 2 * kTiles * 64)
-                store_slot<NP>(p, (n >> 6) - kTiles, n & 63, slot[i]);
+                store_slot<3>(p, (n >> 6) - kTiles, n & 63, slot[i]);
         }
         if (threadIdx.x < 2 * kChunk) (&gates[0][0])[threadIdx.x] = gate;
     }

@@ -178,25 +178,12 @@ __global__ __launch_bounds__(256) void delta_triangles_kernel(RuleParams P) {
     make_triangles<E, KP>(lds, to, P.r.scale, wave);
 }
 
-// What reaches the output alone is rounded with it: for 16-bit outputs, two planes (2^-16)
-// of S, P and u there are far below that rounding (2^-9 and 2^-12). What reaches the state keeps
-// float32's three.
-template <class E>
-inline constexpr int kOutPlanes = sizeof(E) == 4 ? 3 : 2;
-
-template <class E, int KP, int NP>
+template <class E, int KP>
 struct ScanLds {
     ChunkRows<E, KP> rows;
-    Triangle<3> x;
-    Triangle<NP> p;
+    Triangle<3> x, p;
     float gates[2][kChunk];  // E, F beta
 };
-
-template <int N>
-__device__ inline void first_planes(const u4 (&from)[3], u4 (&to)[N]) {
-#pragma unroll
-    for (int n = 0; n < N; ++n) to[n] = from[n];
-}
 
 template <int KP>
 __device__ inline void load_state(const Columns<float>& at, const float* from, int K, f4 (&state)[KP / 16]) {
@@ -356,9 +343,9 @@ __device__ inline void add_columns(int lane, const uint16_t (&rows)[N][kChunk][k
 // the state into planes, two barriers).
 template <class E, int KP, bool kSummary>
 __global__ __launch_bounds__((kWalkThreads<E, KP>), 2) void delta_forward_kernel(RuleParams P) {
-    constexpr int N = kPlanes<E>, NP = kOutPlanes<E>;
+    constexpr int N = kPlanes<E>;
     extern __shared__ char lds_bytes[];
-    auto& lds = *reinterpret_cast<ScanLds<E, KP, NP>*>(lds_bytes);
+    auto& lds = *reinterpret_cast<ScanLds<E, KP>*>(lds_bytes);
     const int wave = wave_of_workgroup(), lane = threadIdx.x & 63, g = lane >> 4;
     int64_t sequence;
     int block;
@@ -388,7 +375,7 @@ __global__ __launch_bounds__((kWalkThreads<E, KP>), 2) void delta_forward_kernel
         const int64_t t0 = static_cast<int64_t>(chunk) * kChunk;
         const int tokens = tokens_of(P, chunk);
         if (chunk > walk.begin) __syncthreads();
-        next.template put<NP>(P, lds.rows, lds.x, lds.p, lds.gates, env, head, t0, tokens);
+        next.put(P, lds.rows, lds.x, lds.p, lds.gates, env, head, t0, tokens);
         const ColumnFetch<E> values = v_next;
         __syncthreads();
         if (chunk + 1 < walk.end) fetch(chunk + 1);
@@ -413,11 +400,9 @@ __global__ __launch_bounds__((kWalkThreads<E, KP>), 2) void delta_forward_kernel
                 for (int i = 0; i < 4; ++i) operand_rows(lane, lds.rows.k, 16 * i, m, a[i]);
                 mma_each<4>(a, b, u);
                 if constexpr (!kSummary) {
-                    u4 b_out[NP];
-                    first_planes(b, b_out);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) operand_rows(lane, lds.rows.q, 16 * i, m, a[i]);
-                    mma_each_transposed<4>(a, b_out, o);
+                    mma_each_transposed<4>(a, b, o);
                 }
             }
         }
@@ -446,10 +431,9 @@ __global__ __launch_bounds__((kWalkThreads<E, KP>), 2) void delta_forward_kernel
 #pragma unroll
         for (int c = 0; c < KP / 16; c += 4) add_columns(lane, lds.rows.k, c, r, state);
         if constexpr (!kSummary) {
-            u4 w[2][NP];
 #pragma unroll
-            for (int m = 0; m < 2; ++m) split8(u[2 * m], u[2 * m + 1], w[m]);
-            times_triangle_transposed<NP>(lane, lds.p, w, o);
+            for (int m = 0; m < 2; ++m) split8(u[2 * m], u[2 * m + 1], r[m]);
+            times_triangle_transposed<3>(lane, lds.p, r, o);
             store_transposed(static_cast<E*>(P.r.out) + ((env * P.r.steps + t0) * P.r.value_heads + head) * V + first,
                              static_cast<int64_t>(P.r.value_heads) * V, V - first, tokens, o);
         }
@@ -469,7 +453,7 @@ template <class E, int KP, bool kSummary>
 __global__ __launch_bounds__((kWalkThreads<E, KP>), 2) void delta_reverse_kernel(RuleParams P) {
     constexpr int N = kPlanes<E>;
     extern __shared__ char lds_bytes[];
-    auto& lds = *reinterpret_cast<ScanLds<E, KP, 3>*>(lds_bytes);
+    auto& lds = *reinterpret_cast<ScanLds<E, KP>*>(lds_bytes);
     const int wave = wave_of_workgroup(), lane = threadIdx.x & 63, g = lane >> 4;
     int64_t sequence;
     int block;
@@ -503,7 +487,7 @@ __global__ __launch_bounds__((kWalkThreads<E, KP>), 2) void delta_reverse_kernel
         const int64_t t0 = static_cast<int64_t>(chunk) * kChunk;
         const int tokens = tokens_of(P, chunk);
         if (step > walk.begin) __syncthreads();
-        next.template put<3>(P, lds.rows, lds.x, lds.p, lds.gates, env, head, t0, tokens);
+        next.put(P, lds.rows, lds.x, lds.p, lds.gates, env, head, t0, tokens);
         const ColumnFetch<E> grads = grad_next;
         __syncthreads();
         if (step + 1 < walk.end) fetch(chunk - 1);
@@ -612,13 +596,13 @@ struct GradientStage {
 
 template <class E, int KP>
 struct GradientTriangles {
-    Triangle<kOutPlanes<E>> n, m;  // (they reach dq and dk alone)
-    float beta_part[4 * kGradientWaves<E, KP>][kChunk], g_part[4 * kGradientWaves<E, KP>][kChunk];
+    Triangle<3> n, m;
+    float beta_part[kGradientWaves<E, KP>][kChunk], g_part[kGradientWaves<E, KP>][kChunk];
 };
 
 struct GradientRest {
     ChunkGates gates;
-    float beta_row[kChunk], g_row[2][kChunk], f_row[kChunk], dot_part[8];
+    float beta_row[kChunk], g_row[2][kChunk], dot_part[8];
 };
 
 template <class E, int KP>
@@ -662,6 +646,12 @@ __device__ inline float sum16(float x) {  // over 16 lanes in a row
     x += moved(x, std::integral_constant<int, 0x141>{});  // the other four of eight
     x += moved(x, std::integral_constant<int, 0x140>{});  // the other eight
     return x;
+}
+
+// Over the four lanes that have a column's tokens in a tile of results
+__device__ inline float sum_tokens(float x) {
+    x += __shfl_xor(x, 16);
+    return x + __shfl_xor(x, 32);
 }
 
 // Four floats into the planes of an operand's lane, its first or second half.
@@ -752,8 +742,8 @@ __global__ __launch_bounds__(256) void delta_join_kernel(RuleParams P) {
 }
 
 // A triangle's rows times 32 rows in LDS.
-template <int NP, int N, int kPitch, int kCount>
-__device__ inline void add_products(int lane, const u4 (&a)[NP], const uint16_t (&rows)[N][kChunk][kPitch], int m, f4 (&x)[kCount]) {
+template <int N, int kPitch, int kCount>
+__device__ inline void add_products(int lane, const u4 (&a)[3], const uint16_t (&rows)[N][kChunk][kPitch], int m, f4 (&x)[kCount]) {
 #pragma unroll
     for (int c = 0; c < kCount; ++c) {
         u4 b[N];
@@ -767,7 +757,7 @@ __device__ inline void add_products(int lane, const u4 (&a)[NP], const uint16_t 
 // the tokens 16 wave on.
 template <class E, int KP, bool kDo>
 struct GradientTerms {
-    static constexpr int N = kPlanes<E>, NP = kOutPlanes<E>, kOwn = kDo ? N : 3;
+    static constexpr int N = kPlanes<E>, kOwn = kDo ? N : 3;
     f4 y[KP / 16], h[4], row_sum;
 
     __device__ void clear() {
@@ -815,7 +805,7 @@ struct GradientTerms {
                                   GradientTriangles<E, KP>& tri, float scale) {
         constexpr bool kAdd = !kDo && kGradientWaves<E, KP> == 4;
         const int col = lane & 15, g = lane >> 4, row = 16 * wave + 4 * g;
-        const int part = 4 * wave + g + (kDo || kAdd ? 0 : 16);
+        const int part = wave + (kDo || kAdd ? 0 : 4);
         row_sum = f4{0, 0, 0, 0};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -845,11 +835,15 @@ struct GradientTerms {
                     g_sum += pair;
                     row_sum[s] += pair;
                 }
-                store_slot<NP>(triangle(tri), tile_of(wave, j), lane, n);
+                store_slot<3>(triangle(tri), tile_of(wave, j), lane, n);
                 settle();
             }
-            tri.beta_part[part][16 * j + col] = (kAdd ? tri.beta_part[part][16 * j + col] : 0.0f) + beta_sum;
-            tri.g_part[part][16 * j + col] = (kAdd ? tri.g_part[part][16 * j + col] : 0.0f) + g_sum;
+            beta_sum = sum_tokens(beta_sum);
+            g_sum = sum_tokens(g_sum);
+            if (g == 0) {
+                tri.beta_part[part][16 * j + col] = (kAdd ? tri.beta_part[part][16 * j + col] : 0.0f) + beta_sum;
+                tri.g_part[part][16 * j + col] = (kAdd ? tri.g_part[part][16 * j + col] : 0.0f) + g_sum;
+            }
         }
     }
 
@@ -883,14 +877,14 @@ struct GradientTerms {
                                   f4 (&dk)[KP / 16]) {
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
-            u4 a[NP];
+            u4 a[3];
             if (2 * m <= wave) {
-                operand_triangle<NP>(lane, triangle(tri), wave, m, a);
-                add_products<NP>(lane, a, rows.k, m, y);
+                operand_triangle<3>(lane, triangle(tri), wave, m, a);
+                add_products(lane, a, rows.k, m, y);
             }
             if (2 * m + 1 >= wave) {
-                operand_transpose<NP>(lane, triangle(tri), wave, m, a);
-                add_products<NP>(lane, a, left_rows(rows), m, dk);
+                operand_transpose<3>(lane, triangle(tri), wave, m, a);
+                add_products(lane, a, left_rows(rows), m, dk);
             }
         }
     }
@@ -1023,9 +1017,7 @@ __global__ __launch_bounds__((64 * kGradientWaves<E, KP>), (kGradientWaves<E, KP
             }
         }
     }
-    dot = sum16(dot);
-    dot += __shfl_xor(dot, 16);
-    dot += __shfl_xor(dot, 32);
+    dot = sum_tokens(sum16(dot));
     if (lane == 0) lds.rest.dot_part[threadIdx.x >> 6] = dot;
     __syncthreads();
     if constexpr (!kRowsStay<E, KP>) {
@@ -1054,7 +1046,6 @@ __global__ __launch_bounds__((64 * kGradientWaves<E, KP>), (kGradientWaves<E, KP
             if (col == 0) {
                 lds.rest.g_row[0][row + s] = own - beta[s] * left;
                 lds.rest.beta_row[row + s] = left;
-                lds.rest.f_row[row + s] = beta[s] * left;
             }
         }
     }
@@ -1070,15 +1061,12 @@ __global__ __launch_bounds__((64 * kGradientWaves<E, KP>), (kGradientWaves<E, KP
     __syncthreads();
     if (wave_of_workgroup() == 0) {
         float dbeta = lds.rest.beta_row[lane], dG = lds.rest.g_row[0][lane] + lds.rest.g_row[1][lane];
-        float f_all = lds.rest.f_row[lane];
+        const float f_all = sum_tokens(sum16(gates.beta[lane] * dbeta));  // (before the triangles' parts)
 #pragma unroll
-        for (int n = 0; n < 4 * kWaves; ++n) {
+        for (int n = 0; n < kWaves; ++n) {
             dbeta += lds.tri.beta_part[n][lane];
             dG -= lds.tri.g_part[n][lane];
         }
-        f_all = sum16(f_all);
-        f_all += __shfl_xor(f_all, 16);
-        f_all += __shfl_xor(f_all, 32);
         if (lane == 63) {
             const float keep = gates.e[63];
             dG += f_all;
@@ -1180,7 +1168,7 @@ int64_t segment_floats(const navi_delta_rule& r) {
 
 template <class E, int KP, bool kBack, bool kSummary>
 int walk(const RuleParams& P, unsigned segments, hipStream_t stream) {
-    constexpr size_t lds = sizeof(ScanLds<E, KP, kBack ? 3 : kOutPlanes<E>>);
+    constexpr size_t lds = sizeof(ScanLds<E, KP>);
     const int64_t blocks = (P.r.envs * P.r.value_heads + 7) / 8 * 8 * (kSummary ? P.summary_blocks : P.blocks);
     if (blocks > INT32_MAX) return set_error(NAVI_POLICY_E_ARG, "envs * value_heads * value_dim is too large");
     const dim3 grid(static_cast<unsigned>(blocks), 1, segments), threads(kWalkThreads<E, KP>);
