@@ -12,9 +12,11 @@ namespace navi_policy {
 
 int set_error(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
 
+using f2 = float __attribute__((ext_vector_type(2)));
 using f4 = float __attribute__((ext_vector_type(4)));
 using u2 = uint32_t __attribute__((ext_vector_type(2)));
 using u4 = uint32_t __attribute__((ext_vector_type(4)));
+using bf16x2 = __bf16 __attribute__((ext_vector_type(2)));
 using bf16x8 = __bf16 __attribute__((ext_vector_type(8)));
 using s4 = short __attribute__((ext_vector_type(4)));
 
@@ -47,9 +49,10 @@ __device__ inline f16 from_float<f16>(float x) {
     return f16{static_cast<_Float16>(x)};
 }
 
-// A float32 is the sum of three bfloat16 whose bits are its mantissa's in turn (8 each), a
-// float16's 11 bits fit two, so products of such planes on the matrix cores keep float32's
-// precision at a third to a sixth of the bfloat16 rate: five to two times float32's own.
+// A float32 is the sum of three bfloat16, each the rounding of what those before it leave (8 bits
+// of its 24 and a sign), a float16's 11 bits fit two, so products of such planes on the matrix
+// cores keep float32's precision at a third to a sixth of the bfloat16 rate: five to two times
+// float32's own. (Numbers above 3.39e38, bfloat16's largest, count as infinite.)
 template <class E>
 inline constexpr int kPlanes = 3;
 template <>
@@ -57,20 +60,22 @@ inline constexpr int kPlanes<bf16> = 1;
 template <>
 inline constexpr int kPlanes<f16> = 2;
 
-// Two floats' upper halves as two bfloat16 (a in the low half).
-__device__ inline uint32_t upper_halves(float a, float b) {
-    return __builtin_amdgcn_perm(bits_of(b), bits_of(a), 0x07060302u);
+// Two floats rounded to nearest as two bfloat16 (a in the low half; v_cvt_pk_bf16_f32).
+__device__ inline uint32_t rounded_pair(float a, float b) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{a, b}, bf16x2));
 }
 
-// The planes of two floats; with N = 3 their sum is exact (a normal float's).
+// The planes of two floats; with N = 3 their sum is exact (a normal float's). Plane p's remainder
+// is at most 2^-9 of the one before it, of either sign: cut off instead of rounded, it would be
+// 2^-7 and always of the number's sign, and what products of planes leave out would add up.
 template <int N>
 __device__ inline void split_pair(float a, float b, uint32_t (&plane)[N]) {
 #pragma unroll
     for (int p = 0; p < N; ++p) {
-        plane[p] = upper_halves(a, b);
+        plane[p] = rounded_pair(a, b);
         if (p + 1 < N) {
-            a -= float_of(bits_of(a) & 0xffff0000u);
-            b -= float_of(bits_of(b) & 0xffff0000u);
+            a -= float_of(plane[p] << 16);
+            b -= float_of(plane[p] & 0xffff0000u);
         }
     }
 }
@@ -105,7 +110,8 @@ __device__ inline f4 mfma(u4 a, u4 b, f4 c) {
                                                    0, 0);
 }
 
-// The product of two sums of planes, smallest terms first; terms below 2^-24 are left out.
+// The product of two sums of planes, smallest terms first. Left out is the second plane of one
+// times the third of the other, 2^-27 of the product each, and less.
 template <int NA, int NB>
 __device__ inline f4 mma(const u4 (&a)[NA], const u4 (&b)[NB], f4 c) {
 #pragma unroll

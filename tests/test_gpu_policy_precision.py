@@ -65,3 +65,18 @@ def test_outputs_of_16_bits_are_rounded_once(policy, size, dtype):
     for name, a, b in zip(["o", *names], [o, *back], [want, *back_want]):
         share, expected = shares(a, b)
         assert share <= expected, name
+
+
+def test_float32_numbers_whose_low_bits_are_ones(policy):
+    """One key and a start at every token: o = q k v and the state is k v of the last. A product is
+    summed in float32 with its large term last, so a sum's rounding counts once (2^-23, however the
+    sum rounds), and terms left out are held to 2^-26: 2.5 x 2^-24 a product, of which o has two
+    and the state one."""
+    steps, size = 70, 1 + 2.0 ** -7 - 2.0 ** -23
+    one = torch.full((1, steps, 1, 1), size, device="cuda")
+    v = one.expand(1, steps, 1, 32).contiguous()
+    gate = torch.zeros(1, steps, 1, device="cuda")
+    starts = torch.ones(1, steps, dtype=torch.bool, device="cuda")
+    o, state = policy.gated_delta_rule(one, one, v, gate, torch.ones_like(gate), scale=1.0, starts=starts, return_state=True)
+    assert float((o.double() / size ** 3 - 1).abs().max()) <= 6 * ref.EPS
+    assert float((state.double() / size ** 2 - 1).abs().max()) <= 3 * ref.EPS
