@@ -271,20 +271,22 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     """One token of every environment: ``gated_delta_rule`` without the ``Steps`` axis.
 
     ``state`` (float32, ``[Envs, ValueHeads, KeyDim, ValueDim]``) is updated in place; the
-    output goes to ``out`` (like ``v``, contiguous) if given. No gradients: this is the form
-    for acting.
+    output goes to ``out`` (like ``v``, contiguous) if given. Autograd is told of both writes: what
+    has saved either raises backward. No gradients: this is the form for acting.
     """
     _check_rule(q, k, v, g, beta, starts, ("Envs",))
     _check_state("state", state, q, v)
-    if torch.is_grad_enabled():
-        _check(not (q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad or beta.requires_grad
-                    or state.requires_grad), "gated_delta_step has no gradients; use gated_delta_rule, or torch.no_grad()")
-    device = q.device
-    if out is None:
-        out = torch.empty(v.shape, dtype=v.dtype, device=device)
-    else:
+    device, written = q.device, [state]
+    if out is not None:
+        written.append(out)
         _check_tensor("out", out, (v.dtype,), 3, device)
         _check(out.shape == v.shape and out.is_contiguous(), "out must be like v, contiguous")
+    if torch.is_grad_enabled():
+        _check(not (q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad or beta.requires_grad
+                    or state.requires_grad or (out is not None and out.requires_grad)),
+               "gated_delta_step has no gradients; use gated_delta_rule, or torch.no_grad()")
+    if out is None:
+        out = torch.empty(v.shape, dtype=v.dtype, device=device)
     envs, key_heads, key_dim = q.shape
     (q0, q1, _), (k0, k1, _), (v0, v1, _) = q.stride(), k.stride(), v.stride()
     (g0, g1), (b0, b1), at = g.stride(), beta.stride(), state.data_ptr()
@@ -295,7 +297,7 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
         *((0, 0, 0) if starts is None else (starts.data_ptr(), starts.stride(0), 0)),
         at, out.data_ptr(), at, 0, 0, 0, 0)
     _call(_native.lib().navi_delta_step, device, rule)
-    _written([state] if out.grad_fn is None else [state, out])
+    _written(written)
     return out
 
 
