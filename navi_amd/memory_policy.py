@@ -84,7 +84,7 @@ class MemoryPolicy(torch.nn.Module):
 
 
 class Rollout:
-    """One rollout's frames, episode starts and places, and the state before it."""
+    """One rollout's frames, episode starts and places, and the state before it (None before the first)."""
 
     def __init__(self, actors: int, steps: int, inputs: int, device) -> None:
         self.frames = torch.empty(actors, steps + 1, inputs, device=device)
@@ -96,18 +96,24 @@ class Rollout:
 
 def collect(harness, model: MemoryPolicy, rollout: Rollout, state: torch.Tensor, starts: torch.Tensor,
             positions: torch.Tensor) -> None:
-    """Steps every actor through a rollout; ``state``, ``starts`` and ``positions`` (of the next
-    frame) are carried on in place."""
-    rollout.state = state.clone()
+    """Steps every actor through a rollout; ``state`` (before the rollout's last frame), ``starts`` and
+    ``positions`` (of that frame) are carried on in place. The last frame is only predicted: the next
+    rollout begins with it."""
     steps = rollout.acted.shape[1]
-    for t in range(steps + 1):
+    if rollout.state is None:
         harness.step()
-        rollout.frames[:, t] = features(harness.obs[:, 0])
-        rollout.starts[:, t], rollout.positions[:, t] = starts, positions
-        if t < steps:  # (the last frame is the next rollout's to act on: it is only predicted)
-            rollout.acted[:, t] = model.act(rollout.frames[:, t], starts, positions, state)
-            starts.copy_(harness.collision != 0)
-            positions.add_(1).masked_fill_(starts, 0)
+        rollout.frames[:, 0] = features(harness.obs[:, 0])
+    else:
+        rollout.frames[:, 0] = rollout.frames[:, steps]
+    rollout.state = state.clone()
+    rollout.starts[:, 0], rollout.positions[:, 0] = starts, positions
+    for t in range(steps):
+        rollout.acted[:, t] = model.act(rollout.frames[:, t], starts, positions, state)
+        starts.copy_(harness.collision != 0)  # in frame t: the next one begins an episode
+        positions.add_(1).masked_fill_(starts, 0)
+        harness.step()
+        rollout.frames[:, t + 1] = features(harness.obs[:, 0])
+        rollout.starts[:, t + 1], rollout.positions[:, t + 1] = starts, positions
 
 
 def learn(model: MemoryPolicy, optimizer, rollout: Rollout, max_norm: float) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
@@ -143,7 +149,7 @@ def run(scenes, *, actors: int, steps: int, updates: int, azimuth_bins: int, ele
         collected = time.perf_counter()
         loss, norm, said = learn(model, optimizer, rollout, max_norm)
         torch.cuda.synchronize()
-        act_ms.append((collected - began) * 1e3 / (steps + 1))
+        act_ms.append((collected - began) * 1e3 / steps)
         learn_ms.append((time.perf_counter() - collected) * 1e3)
         losses.append(float(loss))
         norms.append(float(norm))
