@@ -14,7 +14,7 @@ These are the operators of such a core as HIP kernels:
 
 The kernels run on PyTorch's current stream, never wait for the device and keep nothing of a
 call; queries, keys and values may be views of one projection (any strides but the last
-axis's). Misuse raises ``RuntimeError``; there is no CPU fallback.
+axis's). Misuse raises ``RuntimeError``, forward-mode derivatives do too; there is no CPU fallback.
 """
 
 from __future__ import annotations
@@ -24,6 +24,7 @@ import struct
 from typing import Iterable
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _policy_native as _native
@@ -51,6 +52,13 @@ def _check_tensor(name: str, t, dtypes, dims: int, device=None) -> None:
 
 def _dense_last(t: torch.Tensor) -> bool:
     return t.stride(-1) == 1 or t.size(-1) <= 1
+
+
+def _check_tangents(*tensors) -> None:
+    """The kernels would drop the tangents of forward-mode derivatives without a word."""
+    if forward_ad._current_level >= 0:  # (within a dual_level only)
+        _check(all(t is None or forward_ad.unpack_dual(t).tangent is None for t in tensors),
+               "the policy's operators have no forward-mode derivatives")
 
 
 def _call(function, device: torch.device, *args) -> None:
@@ -247,6 +255,7 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     _check_rule(q, k, v, g, beta, starts, ("Envs", "Steps"))
     if initial_state is not None:
         _check_state("initial_state", initial_state, q, v)
+    _check_tangents(q, k, v, g, beta, initial_state)
     scale = q.size(-1) ** -0.5 if scale is None else float(scale)
     grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad
                                       or beta.requires_grad or (initial_state is not None and initial_state.requires_grad))
@@ -281,6 +290,7 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
         written.append(out)
         _check_tensor("out", out, (v.dtype,), 3, device)
         _check(out.shape == v.shape and out.is_contiguous(), "out must be like v, contiguous")
+    _check_tangents(q, k, v, g, beta, state, out)
     if torch.is_grad_enabled():
         _check(not (q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad or beta.requires_grad
                     or state.requires_grad or (out is not None and out.requires_grad)),
@@ -421,6 +431,7 @@ def qk_norm(q: torch.Tensor, k: torch.Tensor, *, q_weight: torch.Tensor | None =
     default); one outside the tables gives NaN in the numbers that it would rotate.
     """
     _check_norm(q, k, q_weight, k_weight, cos, sin, positions, norm)
+    _check_tangents(q, k, q_weight, k_weight, cos, sin)
     eps = float(eps)
     _check(math.isfinite(eps) and eps >= 0.0, "eps must be finite and not negative")
     args = (q, k, q_weight, k_weight, cos, sin, positions, norm, eps, bool(interleaved))
@@ -455,6 +466,7 @@ def clip_grad_norm(grads: Iterable[torch.Tensor | None], max_norm: float, *, eps
     _check(len(grads) > 0, "grads must hold at least one tensor")
     if not _fine_grads(grads, to):
         _check_grads(grads, to)
+    _check_tangents(*grads, *to)
     n, device = len(grads), grads[0].device
     norm = torch.empty((), dtype=torch.float32, device=device)
     partial = torch.empty(_native.NORM_PARTIALS, dtype=torch.float32, device=device)

@@ -1,9 +1,11 @@
-"""The policy's operators (``navi_amd.policy``) and autograd: writes that it is told of."""
+"""The policy's operators (``navi_amd.policy``) and autograd: writes that it is told of, derivatives
+that they do not have."""
 
 from __future__ import annotations
 
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 pytestmark = pytest.mark.gpu
 
@@ -21,6 +23,11 @@ def frame(envs=3, heads=2, dim=32, dtype=torch.float32, seed=0):
     x = [torch.nn.functional.normalize(rand(envs, heads, dim), dim=-1).to(dtype) for _ in range(2)]
     x += [rand(envs, heads, dim).to(dtype), -rand(envs, heads).abs(), torch.sigmoid(rand(envs, heads))]
     return x, rand(envs, heads, dim, dim)
+
+
+def rollout(envs=2, steps=130, heads=2, dim=32, dtype=torch.float32, seed=0):
+    x, state = frame(envs * steps, heads, dim, dtype, seed)
+    return [t.unflatten(0, (envs, steps)) for t in x], state[:envs].clone()
 
 
 # ---- writes ----
@@ -66,3 +73,48 @@ def test_inference_tensors(policy):
         policy.gated_delta_step(*x, state, out=out)
         policy.clip_grad_norm([out], 1.0)
     assert torch.isfinite(out).all()
+
+
+# ---- derivatives that the operators do not have ----
+
+
+@pytest.mark.parametrize("dual", range(6))
+def test_forward_mode_is_refused(policy, dual):
+    x, state = frame()
+    short, long = rollout(steps=3), rollout()
+    with forward_ad.dual_level():
+        with_tangent = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for given, carried in ((x, state), short, long):
+            args = list(given)
+            if dual < 5:
+                args[dual] = with_tangent(args[dual])
+            else:
+                carried = with_tangent(carried)
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                if given is x:
+                    policy.gated_delta_step(*args, carried)
+                else:
+                    policy.gated_delta_rule(*args, initial_state=carried)
+        policy.gated_delta_step(*x, state)  # (none of its own inputs is one)
+        policy.gated_delta_rule(*long[0], initial_state=long[1])
+
+
+@pytest.mark.parametrize("dual", ["q", "k", "q_weight", "k_weight", "cos", "sin"])
+def test_forward_mode_of_norms_is_refused(policy, dual):
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    args = {n: torch.randn(2, 3, 1, 32, generator=gen, device="cuda") for n in ("q", "k")}
+    args |= {n: torch.ones(32, device="cuda") for n in ("q_weight", "k_weight")}
+    args |= {n: torch.ones(3, 8, device="cuda") for n in ("cos", "sin")}
+    with forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            policy.qk_norm(**{**args, dual: forward_ad.make_dual(args[dual], torch.ones_like(args[dual]))})
+        policy.qk_norm(**args)
+
+
+def test_forward_mode_of_clipping_is_refused(policy):
+    g = torch.ones(5, device="cuda")
+    with forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            policy.clip_grad_norm([forward_ad.make_dual(g, torch.ones_like(g))], 1.0)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            policy.clip_grad_norm([g], 1.0, out=[forward_ad.make_dual(g.clone(), torch.ones_like(g))])
