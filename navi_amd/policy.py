@@ -425,7 +425,7 @@ def qk_norm(q: torch.Tensor, k: torch.Tensor, *, q_weight: torch.Tensor | None =
     in float32, bfloat16 or float16 (head dimension up to 1024). ``norm="rms"`` divides by the
     root of the mean square plus eps, ``"l2"`` by that of the sum (rows of norm 1, what the
     gated delta rule takes). ``q_weight``, ``k_weight``: float32 ``[HeadDim]`` factors.
-    ``cos``, ``sin``: float32 ``[Positions, Pairs]`` tables that rotate the first ``2 * Pairs``
+    ``cos``, ``sin``: float32 ``[Positions, Pairs]`` tables (without gradients) that rotate the first ``2 * Pairs``
     numbers of a row, pair i being (i, i + Pairs), or (2 i, 2 i + 1) with ``interleaved``.
     ``positions``: ``[Envs, Steps]`` int32 or int64 rows of the tables (a token's step by
     default); one outside the tables gives NaN in the numbers that it would rotate.
@@ -435,6 +435,8 @@ def qk_norm(q: torch.Tensor, k: torch.Tensor, *, q_weight: torch.Tensor | None =
     eps = float(eps)
     _check(math.isfinite(eps) and eps >= 0.0, "eps must be finite and not negative")
     args = (q, k, q_weight, k_weight, cos, sin, positions, norm, eps, bool(interleaved))
+    if cos is not None and torch.is_grad_enabled():
+        _check(not (cos.requires_grad or sin.requires_grad), "cos and sin have no gradients; detach them")
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or (q_weight is not None and q_weight.requires_grad)
                                     or (k_weight is not None and k_weight.requires_grad)):
         return _QkNorm.apply(*args)

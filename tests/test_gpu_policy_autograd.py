@@ -118,3 +118,13 @@ def test_forward_mode_of_clipping_is_refused(policy):
             policy.clip_grad_norm([forward_ad.make_dual(g, torch.ones_like(g))], 1.0)
         with pytest.raises(RuntimeError, match="forward-mode"):
             policy.clip_grad_norm([g], 1.0, out=[forward_ad.make_dual(g.clone(), torch.ones_like(g))])
+
+
+@pytest.mark.parametrize("name", ["cos", "sin"])
+def test_tables_that_require_grad_are_refused(policy, name):
+    q = torch.randn(2, 3, 1, 32, device="cuda")
+    args = {n: torch.ones(3, 8, device="cuda").requires_grad_(n == name) for n in ("cos", "sin")}
+    with pytest.raises(RuntimeError, match="cos and sin have no gradients"):
+        policy.qk_norm(q, q, **args)
+    with torch.no_grad():
+        policy.qk_norm(q, q, **args)
