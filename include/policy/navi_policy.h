@@ -166,7 +166,8 @@ int64_t navi_qk_norm_workspace(const navi_qk_norm_args* args);
 
 /*
  * The norm of all numbers of n_tensors tensors, sqrt(sum x^2), into norm[0], and the tensors
- * times min(1, max_norm / (norm + eps)) into `to` (which may be the tensors themselves).
+ * times min(1, max_norm / (norm + eps)) into `to`. A tensor may be scaled in place; otherwise what
+ * is written shares no memory with what else is written or read.
  * from, to, counts and dtypes (NAVI_POLICY_*) are host arrays, read during the call; tensors
  * are contiguous and aligned to their elements. `partial`: NAVI_POLICY_NORM_PARTIALS floats.
  * Sums are taken in a fixed order: the same numbers give the same norm.

@@ -8,6 +8,8 @@
 // for 3.07 GB (5.6 TB/s), scaling 1270 us for 6.14 GB (4.8 TB/s).
 #include <algorithm>
 #include <climits>
+#include <memory>
+#include <new>
 
 #include "policy_common.hpp"
 
@@ -166,6 +168,40 @@ int fill(ClipParams& P, int at, int n, const void* const* from, void* const* to,
     return at;
 }
 
+struct Span {  // a tensor's bytes
+    uintptr_t first, end;
+    int32_t tensor;
+};
+
+Span span_of(const void* p, int64_t count, int32_t dtype, int32_t tensor) {
+    const uintptr_t first = reinterpret_cast<uintptr_t>(p);
+    return Span{first, first + static_cast<uintptr_t>(count) * (dtype == NAVI_POLICY_F32 ? 4 : 2), tensor};
+}
+
+// Workgroups scale in any order, so what one writes no other may write or read: tensors of `to`
+// lie apart from each other and from those of `from`, but for a tensor that is scaled in place.
+int check_apart(int n, const void* const* from, void* const* to, const int64_t* counts, const int32_t* dtypes) {
+    const std::unique_ptr<Span[]> spans(new (std::nothrow) Span[n]);
+    if (!spans) return set_error(NAVI_POLICY_E_ARG, "out of host memory for %d tensors", n);
+    int written = 0;
+    for (int i = 0; i < n; ++i)
+        if (counts[i] > 0) spans[written++] = span_of(to[i], counts[i], dtypes[i], i);
+    const auto earlier = [](const Span& a, const Span& b) { return a.first < b.first; };
+    if (!std::is_sorted(&spans[0], &spans[0] + written, earlier)) std::sort(&spans[0], &spans[0] + written, earlier);
+    for (int i = 1; i < written; ++i)
+        if (spans[i - 1].end > spans[i].first)
+            return set_error(NAVI_POLICY_E_ARG, "tensors %d and %d that are written share memory",
+                             std::min(spans[i - 1].tensor, spans[i].tensor), std::max(spans[i - 1].tensor, spans[i].tensor));
+    for (int i = 0; i < n; ++i) {
+        if (counts[i] == 0 || from[i] == to[i]) continue;
+        const Span read = span_of(from[i], counts[i], dtypes[i], i);
+        const Span* next = std::partition_point(&spans[0], &spans[0] + written, [&](const Span& s) { return s.end <= read.first; });
+        if (next != &spans[0] + written && next->first < read.end)
+            return set_error(NAVI_POLICY_E_ARG, "tensor %d that is read and tensor %d that is written share memory", i, next->tensor);
+    }
+    return NAVI_POLICY_OK;
+}
+
 }  // namespace
 }  // namespace navi_policy
 
@@ -183,6 +219,10 @@ extern "C" int navi_clip_grad_norm(int32_t n_tensors, const void* const* from, v
         if (counts[i] > 0 && (!from[i] || !to[i])) return set_error(NAVI_POLICY_E_ARG, "tensor %d is null", i);
         if (dtypes[i] < NAVI_POLICY_F32 || dtypes[i] > NAVI_POLICY_F16)
             return set_error(NAVI_POLICY_E_ARG, "tensor %d must be float32, bfloat16 or float16", i);
+    }
+    if (n_tensors > 0) {
+        const int code = check_apart(n_tensors, from, to, counts, dtypes);
+        if (code != NAVI_POLICY_OK) return code;
     }
     ClipParams P{};
     int launches = 0;

@@ -454,7 +454,8 @@ def clip_grad_norm(grads: Iterable[torch.Tensor | None], max_norm: float, *, eps
     ``grads``: float32, bfloat16 and float16 tensors of one device in any mix (None is
     skipped); each must fill its memory without gaps, in any order of its axes. They are
     scaled in place, or into ``out``, tensors of the same shapes, types and strides (views of
-    an optimizer's flat buffer, for one). A norm that is not finite spoils the gradients as
+    an optimizer's flat buffer, for one). Tensors that are written share no memory with others (a
+    parameter that is used twice is named once). A norm that is not finite spoils the gradients as
     the formula says: NaN gives NaN, infinity gives 0 (NaN where the gradient is infinite).
     """
     max_norm, eps = float(max_norm), float(eps)
