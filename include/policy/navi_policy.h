@@ -3,10 +3,11 @@
  * a policy with a memory runs over the tracer's observations, and of its training step.
  *
  * The reference's policy cores (projects/actor) are PyTorch modules; these entry points
- * have no kernel counterpart there. Every pointer is device memory unless noted. Launches
- * are asynchronous on `stream`; no entry point allocates, waits for the device or keeps
- * anything of a call. Each returns NAVI_POLICY_OK or a negative code and leaves a message
- * in navi_policy_last_error() (thread-local).
+ * have no kernel counterpart there. Every pointer is device memory unless noted, aligned to
+ * its elements, or to more where that is noted. Launches are asynchronous on `stream`; no entry
+ * point allocates device memory, waits for the device or keeps anything of a call. Each
+ * returns NAVI_POLICY_OK or a negative code and leaves a message in navi_policy_last_error()
+ * (thread-local).
  */
 #ifndef NAVI_POLICY_H
 #define NAVI_POLICY_H

@@ -35,6 +35,7 @@ struct RuleParams {
     int32_t group;        // value heads of a key head
     int32_t n_chunks;
     int32_t wide_qk, wide_v, wide_do;  // rows that 16-byte loads can read
+    int32_t wide_out;     // rows of four-number stores
     int32_t wide_state;   // rows of states and updates that 16-byte accesses can
     float* dstates;       // [env, head][chunks - 1][K][V] gradient of the state after each chunk but the last
     float* rgrads;        // [env, head][steps][V] gradient of r

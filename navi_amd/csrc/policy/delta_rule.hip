@@ -105,13 +105,13 @@ struct ColumnFetch {
 // Sixteen columns of 64 rows from transposed results: a lane has row l % 16 of each tile, four
 // columns of it.
 template <class E>
-__device__ inline void store_transposed(E* base, int64_t stride, int columns, int tokens, const f4 (&x)[4]) {
+__device__ inline void store_transposed(E* base, int64_t stride, int columns, int tokens, bool wide, const f4 (&x)[4]) {
     const int l = threadIdx.x & 63, column = 4 * (l >> 4);
     const uint32_t row_bytes = static_cast<uint32_t>(stride) * sizeof(E);
     const int width = columns < 16 ? columns : 16;
     const Buffer to = buffer_of(base, (tokens - 1) * row_bytes + width * sizeof(E));
     const uint32_t lane = (l & 15) * row_bytes + column * sizeof(E);
-    if (stride % 4 == 0 && columns % 4 == 0) {
+    if (wide) {
         const uint32_t own = column < width ? lane : kOutside;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -435,7 +435,7 @@ __global__ __launch_bounds__((kWalkThreads<E, KP>), 2) void delta_forward_kernel
             for (int m = 0; m < 2; ++m) split8(u[2 * m], u[2 * m + 1], r[m]);
             times_triangle_transposed<3>(lane, lds.p, r, o);
             store_transposed(static_cast<E*>(P.r.out) + ((env * P.r.steps + t0) * P.r.value_heads + head) * V + first,
-                             static_cast<int64_t>(P.r.value_heads) * V, V - first, tokens, o);
+                             static_cast<int64_t>(P.r.value_heads) * V, V - first, tokens, P.wide_out, o);
         }
     }
     if (walk.to && walk.working) store_state<KP>(rows_state, walk.to + first, K, state);
@@ -1239,7 +1239,7 @@ bool rows_apart(const int64_t (&stride)[3], int64_t bytes, int64_t dim) {
     return stride[1] >= dim && stride[1] <= kFarthest / bytes;
 }
 
-// 16-byte buffer loads need addresses of whole 4-byte words, and rows that end between them.
+// Wide buffer accesses need addresses of whole 4-byte words, and rows that end between them.
 bool wide_columns(const void* p, const int64_t (&stride)[3], int64_t bytes, int64_t dim) {
     return reinterpret_cast<uintptr_t>(p) % 4 == 0 && dim % 8 == 0 && stride[0] * bytes % 4 == 0 && stride[1] * bytes % 4 == 0 &&
            stride[2] * bytes % 4 == 0;
@@ -1268,6 +1268,10 @@ int check_rule(const navi_delta_rule* r) {
     if (r->envs == 0) return 1;
     if (r->steps > 0 && (!r->q || !r->k || !r->v || !r->g || !r->beta || !r->out))
         return set_error(NAVI_POLICY_E_ARG, "q, k, v, g, beta and out must be non-null");
+    const int64_t bytes = r->dtype == NAVI_POLICY_F32 ? 4 : 2;
+    if (!aligned(bytes, r->q, r->k, r->v, r->out) ||
+        !aligned(4, r->g, r->beta, r->initial_state, r->final_state, r->states, r->updates))
+        return set_error(NAVI_POLICY_E_ARG, "arrays must be aligned to their elements");
     return NAVI_POLICY_OK;
 }
 
@@ -1298,6 +1302,7 @@ int setup(const navi_delta_rule* r, RuleParams& P) {
         return set_error(NAVI_POLICY_E_ARG, "the steps of q, k and v overlap or lie too far apart");
     P.wide_qk = wide_rows(r->q, P.r.q_stride, bytes, r->key_dim) && wide_rows(r->k, P.r.k_stride, bytes, r->key_dim);
     P.wide_v = wide_columns(r->v, P.r.v_stride, bytes, r->value_dim);
+    P.wide_out = reinterpret_cast<uintptr_t>(r->out) % 4 == 0 && r->value_dim % 4 == 0;
     return NAVI_POLICY_OK;
 }
 
@@ -1364,6 +1369,9 @@ extern "C" int navi_delta_backward(const navi_delta_rule* rule, const navi_delta
     P.dk_heads = P.dq_heads + rounded(P.group > 1 ? sequences * rule->steps * rule->key_dim : 0);
     place_segments(P, P.dk_heads + rounded(P.group > 1 ? sequences * rule->steps * rule->key_dim : 0));
     const int64_t bytes = rule->dtype == NAVI_POLICY_F32 ? 4 : 2;
+    if (!aligned(bytes, P.d.grad_out, P.d.d_q, P.d.d_k, P.d.d_v) ||
+        !aligned(4, P.d.grad_final_state, P.d.d_g, P.d.d_beta, P.d.d_initial_state))
+        return set_error(NAVI_POLICY_E_ARG, "arrays must be aligned to their elements");
     if (rule->steps == 1) P.d.grad_out_stride[1] = rule->value_dim;
     if (!rows_apart(P.d.grad_out_stride, bytes, rule->value_dim))
         return set_error(NAVI_POLICY_E_ARG, "the steps of grad_out overlap or lie too far apart");

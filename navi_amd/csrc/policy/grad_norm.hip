@@ -219,6 +219,8 @@ extern "C" int navi_clip_grad_norm(int32_t n_tensors, const void* const* from, v
         if (counts[i] > 0 && (!from[i] || !to[i])) return set_error(NAVI_POLICY_E_ARG, "tensor %d is null", i);
         if (dtypes[i] < NAVI_POLICY_F32 || dtypes[i] > NAVI_POLICY_F16)
             return set_error(NAVI_POLICY_E_ARG, "tensor %d must be float32, bfloat16 or float16", i);
+        if (counts[i] > 0 && !aligned(dtypes[i] == NAVI_POLICY_F32 ? 4 : 2, from[i], to[i]))
+            return set_error(NAVI_POLICY_E_ARG, "tensor %d must be aligned to its elements", i);
     }
     if (n_tensors > 0) {
         const int code = check_apart(n_tensors, from, to, counts, dtypes);

@@ -245,6 +245,11 @@ struct Part {
 
 inline hipStream_t as_stream(void* stream) { return static_cast<hipStream_t>(stream); }
 
+template <class... P>
+bool aligned(int64_t bytes, const P*... p) {
+    return ((reinterpret_cast<uintptr_t>(p) % bytes == 0) && ...);
+}
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 }  // namespace navi_policy

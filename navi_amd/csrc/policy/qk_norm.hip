@@ -389,6 +389,8 @@ int check(const navi_qk_norm_args* a) {
     if (a->pairs < 0 || 2 * a->pairs > a->head_dim) return set_error(NAVI_POLICY_E_ARG, "2 * pairs must be in [0, head_dim]");
     if (a->pairs > 0 && (!a->cos || !a->sin || a->positions_end <= 0))
         return set_error(NAVI_POLICY_E_ARG, "a rotation needs cos and sin");
+    if (!aligned(4, a->cos, a->sin, a->partial) || !aligned(a->positions_wide ? 8 : 4, a->positions))
+        return set_error(NAVI_POLICY_E_ARG, "arrays must be aligned to their elements");
     if (!(a->eps >= 0.0f)) return set_error(NAVI_POLICY_E_ARG, "eps must not be negative");
     return NAVI_POLICY_OK;
 }
@@ -413,6 +415,8 @@ int run(const navi_qk_norm_args* a, bool back, hipStream_t stream) {
         s.grad_dense = dense(s.grad_stride, a, s.heads);
         if (s.rows == 0) continue;
         if (!s.x || !s.out || (back && !s.grad)) return set_error(NAVI_POLICY_E_ARG, "q, k, their gradients and outputs must be non-null");
+        if (!aligned(bytes, s.x, s.out) || (back && !aligned(bytes, s.grad)) || !aligned(4, s.weight, s.d_weight))
+            return set_error(NAVI_POLICY_E_ARG, "arrays must be aligned to their elements");
         wide = wide && wide_rows(s.x, s.x_stride, bytes) && aligned16(s.out) && (!back || wide_rows(s.grad, s.grad_stride, bytes));
     }
     P.steps = a->steps;
