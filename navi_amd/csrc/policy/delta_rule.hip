@@ -755,9 +755,9 @@ __device__ inline void add_products(int lane, const u4 (&a)[3], const uint16_t (
 
 // What a wave computes of do's terms (kDo: x is do, y is Y, h is H) or of dr's (dr, Z, R), for
 // the tokens 16 wave on.
-template <class E, int KP, bool kDo>
+template <class E, int KP>
 struct GradientTerms {
-    static constexpr int N = kPlanes<E>, kOwn = kDo ? N : 3;
+    static constexpr int N = kPlanes<E>;
     f4 y[KP / 16], h[4], row_sum;
 
     __device__ void clear() {
@@ -767,6 +767,7 @@ struct GradientTerms {
         for (int j = 0; j < 4; ++j) h[j] = f4{0, 0, 0, 0};
     }
 
+    template <int kOwn>
     __device__ void products(int lane, int wave, const GradientStage<KP>& stage, bool with_state, const u4 (&x)[kOwn]) {
         u4 b[3];
         if (with_state)
@@ -785,6 +786,7 @@ struct GradientTerms {
         }
     }
 
+    template <bool kDo>
     __device__ static const auto& left_rows(const ChunkRows<E, KP>& rows) {
         if constexpr (kDo)
             return rows.q;
@@ -792,6 +794,7 @@ struct GradientTerms {
             return rows.k;
     }
 
+    template <bool kDo>
     __device__ static auto& triangle(GradientTriangles<E, KP>& tri) {
         if constexpr (kDo)
             return tri.n;
@@ -801,6 +804,7 @@ struct GradientTerms {
 
     // N or M, and the sums over its rows (kept) and columns (parts of the workgroup's sums: with
     // eight waves M's own, with four N's, which it adds to).
+    template <bool kDo>
     __device__ void make_triangle(int lane, int wave, const ChunkRows<E, KP>& rows, const ChunkGates& gates,
                                   GradientTriangles<E, KP>& tri, float scale) {
         constexpr bool kAdd = !kDo && kGradientWaves<E, KP> == 4;
@@ -816,7 +820,7 @@ struct GradientTerms {
                 for (int m = 0; m < KP / 32; ++m) {
                     u4 a[N], b[N];
                     operand_rows(lane, rows.k, 16 * j, m, b);
-                    operand_rows(lane, left_rows(rows), 16 * wave, m, a);
+                    operand_rows(lane, left_rows<kDo>(rows), 16 * wave, m, a);
                     xk = mma(a, b, xk);
                 }
                 const int column = 16 * j + col;
@@ -835,7 +839,7 @@ struct GradientTerms {
                     g_sum += pair;
                     row_sum[s] += pair;
                 }
-                store_slot<3>(triangle(tri), tile_of(wave, j), lane, n);
+                store_slot<3>(triangle<kDo>(tri), tile_of(wave, j), lane, n);
                 settle();
             }
             beta_sum = sum_tokens(beta_sum);
@@ -848,6 +852,7 @@ struct GradientTerms {
     }
 
     // y becomes scale E Y or -E Z; its product with q or k is added to the sums of rows.
+    template <bool kDo>
     __device__ void close_rows(int lane, int wave, const ChunkRows<E, KP>& rows, const ChunkGates& gates, float scale) {
         const int row = 16 * wave + 4 * (lane >> 4);
         const f4 e = four(gates.e, row);
@@ -855,7 +860,7 @@ struct GradientTerms {
 #pragma unroll
         for (int c = 0; c < KP / 16; ++c) {
             y[c] = factor * gated(y[c], e);
-            row_sum = row_sum + row_products(lane, row, left_rows(rows), c, y[c]);
+            row_sum = row_sum + row_products(lane, row, left_rows<kDo>(rows), c, y[c]);
             settle();
         }
     }
@@ -873,18 +878,19 @@ struct GradientTerms {
     }
 
     // dq = y + N k and N^T q into dk; or M k + M^T k into dk = y.
+    template <bool kDo>
     __device__ void last_products(int lane, int wave, const ChunkRows<E, KP>& rows, GradientTriangles<E, KP>& tri,
                                   f4 (&dk)[KP / 16]) {
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
             u4 a[3];
             if (2 * m <= wave) {
-                operand_triangle<3>(lane, triangle(tri), wave, m, a);
+                operand_triangle<3>(lane, triangle<kDo>(tri), wave, m, a);
                 add_products(lane, a, rows.k, m, y);
             }
             if (2 * m + 1 >= wave) {
-                operand_transpose<3>(lane, triangle(tri), wave, m, a);
-                add_products(lane, a, left_rows(rows), m, dk);
+                operand_transpose<3>(lane, triangle<kDo>(tri), wave, m, a);
+                add_products(lane, a, left_rows<kDo>(rows), m, dk);
             }
         }
     }
@@ -952,15 +958,8 @@ __global__ __launch_bounds__((64 * kGradientWaves<E, KP>), (kGradientWaves<E, KP
     if (wave_of_workgroup() == kWaves - 1) of_gates.fetch(P, env, head, t0, tokens);
     if constexpr (kRowsStay<E, KP>) ChunkFetch<E, KP, 64 * kWaves, true>::load(P, rows, env, head, t0, tokens);
     if (wave_of_workgroup() == kWaves - 1) of_gates.put(lds.rest.gates);
-    // With eight waves, those of dr use the registers of do's terms
-    GradientTerms<E, KP, true> terms;
-    GradientTerms<E, KP, false> others;
-    const auto as_dr = [&]() -> GradientTerms<E, KP, false>& {
-        if constexpr (kBoth)
-            return others;
-        else
-            return reinterpret_cast<GradientTerms<E, KP, false>&>(terms);
-    };
+    GradientTerms<E, KP> terms, others;
+    GradientTerms<E, KP>& terms_dr = kBoth ? others : terms;  // with eight waves a wave has one kind
     f4 w[KP / 16];
     terms.clear();
     if constexpr (kBoth) others.clear();
@@ -1002,7 +1001,7 @@ __global__ __launch_bounds__((64 * kGradientWaves<E, KP>), (kGradientWaves<E, KP
         __syncthreads();
         if (v0 + 32 < V) fetch(v0 + 32);
         settle();
-        if (of_dr) as_dr().products(lane, wave, lds.stage, S, a_dr);
+        if (of_dr) terms_dr.products(lane, wave, lds.stage, S, a_dr);
         if (of_do) {
             terms.products(lane, wave, lds.stage, S, a_do);
             if (dS) {
@@ -1029,8 +1028,8 @@ __global__ __launch_bounds__((64 * kGradientWaves<E, KP>), (kGradientWaves<E, KP
     lane = fresh_lane(), col = lane & 15, g = lane >> 4;
     const int row = 16 * wave + 4 * g;
     if (of_do) {
-        terms.make_triangle(lane, wave, rows, gates, lds.tri, P.r.scale);
-        terms.close_rows(lane, wave, rows, gates, P.r.scale);
+        terms.template make_triangle<true>(lane, wave, rows, gates, lds.tri, P.r.scale);
+        terms.template close_rows<true>(lane, wave, rows, gates, P.r.scale);
         const f4 f = four(gates.f, row), beta = four(gates.beta, row);
         f4 kw = {0, 0, 0, 0};
         if (dS)
@@ -1050,11 +1049,11 @@ __global__ __launch_bounds__((64 * kGradientWaves<E, KP>), (kGradientWaves<E, KP
         }
     }
     if (of_dr) {
-        as_dr().make_triangle(lane, wave, rows, gates, lds.tri, P.r.scale);
-        as_dr().close_rows(lane, wave, rows, gates, P.r.scale);
+        terms_dr.template make_triangle<false>(lane, wave, rows, gates, lds.tri, P.r.scale);
+        terms_dr.template close_rows<false>(lane, wave, rows, gates, P.r.scale);
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-            const float own = sum16(as_dr().row_sum[s]);
+            const float own = sum16(terms_dr.row_sum[s]);
             if (col == 0) lds.rest.g_row[1][row + s] = own;
         }
     }
@@ -1089,8 +1088,8 @@ __global__ __launch_bounds__((64 * kGradientWaves<E, KP>), (kGradientWaves<E, KP
     }
 
     lane = fresh_lane();
-    if (of_do) terms.last_products(lane, wave, rows, lds.tri, w);
-    if (of_dr) as_dr().last_products(lane, wave, rows, lds.tri, as_dr().y);
+    if (of_do) terms.template last_products<true>(lane, wave, rows, lds.tri, w);
+    if (of_dr) terms_dr.template last_products<false>(lane, wave, rows, lds.tri, terms_dr.y);
     if constexpr (kBoth) {
 #pragma unroll
         for (int c = 0; c < KP / 16; ++c) w[c] = w[c] + others.y[c];
@@ -1102,7 +1101,7 @@ __global__ __launch_bounds__((64 * kGradientWaves<E, KP>), (kGradientWaves<E, KP
         __syncthreads();
         if (of_dr)
 #pragma unroll
-            for (int c = 0; c < KP / 16; ++c) w[c] = terms.y[c] + lds.of.exchange[wave][c][lane];
+            for (int c = 0; c < KP / 16; ++c) w[c] = terms_dr.y[c] + lds.of.exchange[wave][c][lane];
     }
     const int left = tokens - 16 * wave;  // rows of the wave's tile
     if (left <= 0) return;
