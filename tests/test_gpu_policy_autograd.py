@@ -1,7 +1,9 @@
 """The policy's operators (``navi_amd.policy``) and autograd: writes that it is told of, derivatives
-that they do not have."""
+that they do not have, gradients of some of the inputs, streams and threads."""
 
 from __future__ import annotations
+
+import threading
 
 import pytest
 import torch
@@ -128,3 +130,89 @@ def test_tables_that_require_grad_are_refused(policy, name):
         policy.qk_norm(q, q, **args)
     with torch.no_grad():
         policy.qk_norm(q, q, **args)
+
+
+# ---- gradients ----
+
+
+@pytest.mark.parametrize("wanted", [[0], [1], [2], [3], [4], [5], [0, 3], [2, 5]], ids=str)
+@pytest.mark.parametrize("steps", [3, 130])
+def test_gradients_of_some_inputs(policy, steps, wanted):
+    """The same numbers, whichever inputs they are asked for."""
+    x, state = rollout(steps=steps)
+    inputs = [*x, state]
+    run = lambda args: policy.gated_delta_rule(*args[:5], initial_state=args[5], return_state=True)  # noqa: E731
+    all_of = [t.clone().requires_grad_() for t in inputs]
+    o, final = run(all_of)
+    grads = [torch.randn_like(o), torch.randn_like(final)]
+    want = torch.autograd.grad([o, final], all_of, grads)
+    some = [t.clone().requires_grad_(i in wanted) for i, t in enumerate(inputs)]
+    o, final = run(some)
+    got = torch.autograd.grad([o, final], [some[i] for i in wanted], grads)
+    for i, g in zip(wanted, got):
+        assert torch.equal(g, want[i])
+
+
+def test_a_shared_gates_gradient_is_the_sum_over_heads(policy):
+    x, _ = rollout(heads=4)
+    gate, beta = (t[:, :, :1].clone().requires_grad_() for t in x[3:])
+    o = policy.gated_delta_rule(*x[:3], gate.expand(2, 130, 4), beta.expand(2, 130, 4))
+    whole = [t.detach().expand(2, 130, 4).contiguous().requires_grad_() for t in (gate, beta)]
+    want = policy.gated_delta_rule(*x[:3], *whole)
+    assert torch.equal(o, want)
+    grad = torch.randn_like(o)
+    got = torch.autograd.grad(o, [gate, beta], grad)
+    for a, b in zip(got, torch.autograd.grad(want, whole, grad)):
+        # (four numbers summed in float32: three roundings of partial sums)
+        assert ((a.double() - b.double().sum(-1, keepdim=True)).abs() <= 3 * 2.0 ** -24 * b.abs().sum(-1, keepdim=True)).all()
+        assert float(b.abs().max()) > 0
+
+
+# ---- streams and threads ----
+
+
+def test_two_streams_on_inputs_of_their_own(policy):
+    given = [rollout(envs=6, steps=700, dim=64, dtype=torch.bfloat16, seed=s) for s in (1, 2)]
+    want = [policy.gated_delta_rule(*x, initial_state=s) for x, s in given]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in given], [[], []]
+    for _ in range(4):
+        for i, (x, s) in enumerate(given):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(policy.gated_delta_rule(*x, initial_state=s))
+    for i, stream in enumerate(streams):
+        stream.synchronize()
+        assert all(torch.equal(o, want[i]) for o in got[i])
+
+
+def test_two_threads(policy):
+    given = [rollout(envs=4, steps=200, seed=s) for s in (3, 4)]
+
+    def once(i):
+        x, state = given[i]
+        leaves = [t.clone().requires_grad_() for t in x]
+        o = policy.gated_delta_rule(*leaves, initial_state=state)
+        q, k = policy.qk_norm(x[0], x[1])
+        return [o, q, k, *torch.autograd.grad(o, leaves, torch.ones_like(o))]
+
+    want = [once(i) for i in range(2)]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(5):
+                    got = once(i)
+                    torch.cuda.current_stream().synchronize()
+                    if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                        wrong.append(i)
+        except Exception as error:  # noqa: BLE001 (told to the test's own thread)
+            wrong.append(error)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
