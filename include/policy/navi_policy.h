@@ -68,7 +68,8 @@ typedef struct navi_delta_rule {
     const float* initial_state; /* [envs][value_heads][key_dim][value_dim], or NULL for zeros */
     void* out;
     float* final_state;         /* as initial_state, or NULL; may be initial_state itself in
-                                   navi_delta_step */
+                                   navi_delta_step. Else it shares no memory with what is read, nor
+                                   does out, which may be v itself (contiguous) */
     float* matrices; /* [envs * value_heads][chunks][NAVI_POLICY_CHUNK_MATRICES], 16-byte aligned:
                         written by navi_delta_forward, read again by the backward pass (not used by
                         navi_delta_step); chunks = ceil(steps / NAVI_POLICY_CHUNK) */

@@ -1276,6 +1276,50 @@ int check_rule(const navi_delta_rule* r) {
 
 namespace {
 
+struct Extent {  // the bytes from an array's first number to its last
+    uintptr_t first, end;
+};
+
+Extent extent_of(const void* base, const int64_t (&counts)[4], const int64_t (&strides)[4], int64_t bytes) {
+    uintptr_t first = reinterpret_cast<uintptr_t>(base), last = first;
+    for (int i = 0; i < 4; ++i) {
+        const int64_t reach = (counts[i] - 1) * strides[i] * bytes;
+        (reach < 0 ? first : last) += static_cast<uintptr_t>(reach);
+    }
+    return Extent{first, last + static_cast<uintptr_t>(bytes)};
+}
+
+}  // namespace
+
+// Workgroups read the inputs in any order, so what is written shares no memory with them: out
+// but with v number for number (whose reader writes them), final_state in the recurrent form but
+// with initial_state (the same).
+int check_apart(const navi_delta_rule* r, bool in_place) {
+    if (r->envs == 0) return NAVI_POLICY_OK;
+    const int64_t bytes = r->dtype == NAVI_POLICY_F32 ? 4 : 2, V = r->value_dim, K = r->key_dim;
+    const int64_t row = r->value_heads * V, state = r->value_heads * K * V;
+    const auto of = [&](const void* p, int64_t heads, int64_t dim, const int64_t(&s)[3], int64_t each) {
+        return r->steps > 0 && p ? extent_of(p, {r->envs, r->steps, heads, dim}, {s[0], s[1], s[2], 1}, each) : Extent{0, 0};
+    };
+    const auto of_state = [&](const float* p) { return p ? extent_of(p, {r->envs, 1, 1, state}, {state, 0, 0, 1}, 4) : Extent{0, 0}; };
+    const auto apart = [](const Extent& a, const Extent& b) { return a.first >= a.end || b.first >= b.end || a.end <= b.first || b.end <= a.first; };
+    const Extent out = of(r->out, r->value_heads, V, {r->steps * row, row, V}, bytes), final_state = of_state(r->final_state);
+    const bool own = r->out == r->v && (r->value_heads == 1 || r->v_stride[2] == V) && (r->steps == 1 || r->v_stride[1] == row) &&
+                     (r->envs == 1 || r->v_stride[0] == r->steps * row);
+    const Extent inputs[] = {
+        of(r->q, r->key_heads, K, r->q_stride, bytes), of(r->k, r->key_heads, K, r->k_stride, bytes),
+        of(r->g, r->value_heads, 1, r->g_stride, 4), of(r->beta, r->value_heads, 1, r->beta_stride, 4),
+        of(r->starts, 1, 1, {r->starts_stride[0], r->starts_stride[1], 0}, 1)};
+    bool fine = apart(out, final_state);
+    for (const Extent& x : inputs) fine = fine && apart(out, x) && apart(final_state, x);
+    const Extent v = of(r->v, r->value_heads, V, r->v_stride, bytes), initial = of_state(r->initial_state);
+    fine = fine && (own || apart(out, v)) && apart(out, initial) && apart(final_state, v);
+    fine = fine && ((in_place && r->final_state == r->initial_state) || apart(final_state, initial));
+    return fine ? NAVI_POLICY_OK : set_error(NAVI_POLICY_E_ARG, "out or the state after shares memory with what is read");
+}
+
+namespace {
+
 int setup(const navi_delta_rule* r, RuleParams& P) {
     const int code = check_rule(r);
     if (code != NAVI_POLICY_OK) return code;
@@ -1326,6 +1370,8 @@ extern "C" int navi_delta_forward(const navi_delta_rule* rule, void* stream) {
     if (P.n_chunks == 0 && !rule->final_state) return NAVI_POLICY_OK;
     if (P.n_segments > 1 && (!rule->scratch || !aligned16(rule->scratch)))
         return set_error(NAVI_POLICY_E_ARG, "scratch must be non-null and 16-byte aligned");
+    const int shared = check_apart(rule, false);
+    if (shared != NAVI_POLICY_OK) return shared;
     place_segments(P, static_cast<float*>(rule->scratch));
     return run_typed(P, false, as_stream(stream));
 }

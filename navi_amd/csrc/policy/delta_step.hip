@@ -15,6 +15,7 @@
 namespace navi_policy {
 
 int check_rule(const navi_delta_rule* r);
+int check_apart(const navi_delta_rule* r, bool in_place);
 
 namespace {
 
@@ -178,6 +179,8 @@ extern "C" int navi_delta_step(const navi_delta_rule* rule, void* stream) {
     const int code = check_rule(rule);
     if (code != NAVI_POLICY_OK) return code < 0 ? code : NAVI_POLICY_OK;
     if (rule->states || rule->updates) return set_error(NAVI_POLICY_E_ARG, "the recurrent form saves no states or updates");
+    const int shared = check_apart(rule, true);
+    if (shared != NAVI_POLICY_OK) return shared;
     StepParams P{};
     P.r = *rule;
     P.group = rule->value_heads / rule->key_heads;

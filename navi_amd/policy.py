@@ -280,8 +280,9 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     """One token of every environment: ``gated_delta_rule`` without the ``Steps`` axis.
 
     ``state`` (float32, ``[Envs, ValueHeads, KeyDim, ValueDim]``) is updated in place; the
-    output goes to ``out`` (like ``v``, contiguous) if given. Autograd is told of both writes: what
-    has saved either raises backward. No gradients: this is the form for acting.
+    output goes to ``out`` (like ``v``, contiguous) if given, which shares no memory with the
+    inputs but may be ``v`` itself. Autograd is told of both writes: what has saved either raises
+    backward. No gradients: this is the form for acting.
     """
     _check_rule(q, k, v, g, beta, starts, ("Envs",))
     _check_state("state", state, q, v)
