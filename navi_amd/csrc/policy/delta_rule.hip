@@ -577,16 +577,14 @@ __device__ inline void store_tiles(T* base, int64_t stride, int rows, int column
 //
 // The same number stands at +i and -j of dG, so what cancels in dg cancels to its rounding.
 //
-// Four waves of 16 tokens each take the terms of do (Y, H, W, N, dq, their part of dk) and those
-// of dr (Z, R, M, the rest of dk), or eight waves one of the two. V is taken 32 columns at a
-// time. With 64 keys of 16 bits three workgroups of four waves fit a CU and hide each other's
-// waits; with more, one or two of eight do (1024 x 128 steps, 4 heads of 64: 299 us with four
-// waves, 430 with eight; 2 x 4001 steps, 8 heads of 128: 165 and 120). 1024 x 128 steps, 4 heads of 64
-// now take 265 to 297 us for 692 MB read and 243 MB written (3.1 to 3.5 TB/s): what a chunk waits for its
-// rows, and its five products' reads of LDS (a third of the time), bound it. Workgroups that take
-// chunk after chunk, the next one's rows asked for early, spill: 395 us.
+// Eight waves: four of 16 tokens each take the terms of do (Y, H, W, N, dq, their part of dk), four
+// those of dr (Z, R, M, the rest of dk). V is taken 32 columns at a time. Two workgroups fit a CU
+// with 64 keys of bfloat16, one with more. Rows of 64 float16 (two planes) leave room for one, but
+// for two of four waves with both kinds of terms, whose rows come after V into the stage's place:
+// 1024 x 128 steps, 4 heads of 64, forward and back, float16 733 us with four waves, 835 with
+// eight; bfloat16 626 and 609; 2 x 4001 steps, 8 heads of 128, bfloat16 531 and 413.
 template <class E, int KP>
-inline constexpr int kGradientWaves = KP == 64 && sizeof(E) == 2 ? 4 : 8;
+inline constexpr int kGradientWaves = KP == 64 && kPlanes<E> == 2 ? 4 : 8;
 
 template <int KP>
 struct GradientStage {
@@ -897,7 +895,7 @@ struct GradientTerms {
 };
 
 template <class E, int KP>
-__global__ __launch_bounds__((64 * kGradientWaves<E, KP>), (kGradientWaves<E, KP> == 4 ? 3 : 2)) void delta_gradients_kernel(RuleParams P) {
+__global__ __launch_bounds__((64 * kGradientWaves<E, KP>), 2) void delta_gradients_kernel(RuleParams P) {
     constexpr int N = kPlanes<E>, kWaves = kGradientWaves<E, KP>;
     constexpr bool kBoth = kWaves == 4;                      // a wave has both kinds of terms
     constexpr int kPieces = 8 * KP / (64 * kWaves), kRowsOfU = 8 / kWaves;
