@@ -196,9 +196,9 @@ __device__ inline void store_state(const Columns<float>& at, float* to, int K, c
 }
 
 // Columns of the state that a workgroup holds, 16 a wave. Two workgroups of 64 fit a CU and wait
-// apart: 2 x 4001 steps, 8 heads of 128, 445 us forward and back against 502 with one of 128; 256 x
-// 128 steps, 4 heads of 128, forward, 100 and 102. Rows of 128 float32 leave a CU's LDS to one
-// workgroup, which then has eight waves: the same, 195 us against 304.
+// apart: 2 x 4001 steps, 8 heads of 128, 413 us forward and back against 435 with one of 128; 256 x
+// 128 steps, 4 heads of 128, forward, 93 and 99. Rows of 128 float32 leave a CU's LDS to one
+// workgroup, which then has eight waves: the same, 208 us against 313.
 template <class E, int KP>
 inline constexpr int kWalkColumns = sizeof(E) == 4 && KP == 128 ? 128 : 64;
 template <class E, int KP>
@@ -337,10 +337,10 @@ __device__ inline void add_columns(int lane, const uint16_t (&rows)[N][kChunk][k
 // in the order of results, which the rows in LDS are kept in as well.
 //
 // With many sequences memory bounds it: 1024 x 128 steps, 4 heads of 64, bfloat16, with what the
-// gradients need, 150 us for 374 MB read and 269 MB written (4.3 TB/s). With few, the chain from
-// chunk to chunk does: 16384 steps, 16 heads of 128 in 16 segments, 132 us, 8.2 us a chunk of which
-// the products' own time is 2.8 (what lies between: reads of LDS for the operands, splits of
-// the state into planes, two barriers).
+// gradients need, 152 us for 374 MB read and 269 MB written (4.2 TB/s). With few, the chain from
+// chunk to chunk does: 16384 steps, 16 heads of 128 in 16 segments, 145 us, 9.1 us a chunk of which
+// the products' own time is 3.3 (what lies between: reads of LDS for the operands, with bank
+// conflicts in a fifth of the cycles, splits of the state into planes, two barriers).
 template <class E, int KP, bool kSummary>
 __global__ __launch_bounds__((kWalkThreads<E, KP>), 2) void delta_forward_kernel(RuleParams P) {
     constexpr int N = kPlanes<E>;
@@ -447,8 +447,8 @@ __global__ __launch_bounds__((kWalkThreads<E, KP>), 2) void delta_forward_kernel
 //     du = P^T do + beta F (k dS),   dr = X^T du  (= dv),
 //     dS <- E_last dS + q^T (scale E do) - k^T (E dr)
 //
-// dS and dr go to memory for delta_gradients_kernel. Bound as the forward pass is: 148 us for the
-// same traffic at 1024 x 128 steps, 4 heads of 64 (4.3 TB/s).
+// dS and dr go to memory for delta_gradients_kernel. Bound as the forward pass is: 146 us for the
+// same traffic at 1024 x 128 steps, 4 heads of 64 (4.4 TB/s).
 template <class E, int KP, bool kSummary>
 __global__ __launch_bounds__((kWalkThreads<E, KP>), 2) void delta_reverse_kernel(RuleParams P) {
     constexpr int N = kPlanes<E>;
@@ -582,7 +582,9 @@ __device__ inline void store_tiles(T* base, int64_t stride, int rows, int column
 // with 64 keys of bfloat16, one with more. Rows of 64 float16 (two planes) leave room for one, but
 // for two of four waves with both kinds of terms, whose rows come after V into the stage's place:
 // 1024 x 128 steps, 4 heads of 64, forward and back, float16 733 us with four waves, 835 with
-// eight; bfloat16 626 and 609; 2 x 4001 steps, 8 heads of 128, bfloat16 531 and 413.
+// eight; bfloat16 626 and 609; 2 x 4001 steps, 8 heads of 128, bfloat16 531 and 413. The
+// kernel alone takes 271 to 289 us of the 609, for 622 MB read and 151 MB written (2.7 to 2.8 TB/s):
+// VALU and LDS are each busy half of that time, and waves wait for their chunk's rows.
 template <class E, int KP>
 inline constexpr int kGradientWaves = KP == 64 && kPlanes<E> == 2 ? 4 : 8;
 
@@ -1147,11 +1149,11 @@ int blocks_of(const navi_delta_rule& r, int columns) {
 int64_t chunks_of(int64_t steps) { return (steps + kChunk - 1) / kChunk; }
 
 // Segments of a walk, at most 16: one where workgroups of 64 columns for whole walks fill half of the
-// card's 256 CUs (192 sequences of 4096 steps, one head of 64, forward: 336 us in 1, 367 in 2; 128:
-// 266 in 4, 274 in 2); else as many as give each CU a workgroup, of four chunks or more, for the join
-// takes about half as long as a chunk for each. A second workgroup to a CU gives less and needs
-// segments of eight chunks. 2 x 4001 steps, 8 heads of 128: 408 us forward and back in 8 segments, 443
-// in 15; 16384 steps, 16 heads of 128, forward: 347 us in 16, 363 in 8.
+// card's 256 CUs (192 sequences of 4096 steps, one head of 64, forward: 349 us in 1, 385 in 2; 128:
+// 274 in 4, 286 in 2); else as many as give each CU a workgroup, of four chunks or more, for the join
+// takes about a third of a chunk for each. A second workgroup to a CU gives less and needs
+// segments of eight chunks. 2 x 4001 steps, 8 heads of 128: 410 us forward and back in 8 segments, 437
+// in 15; 16384 steps, 16 heads of 128, forward: 371 us in 16, 387 in 8.
 int segments_of(const navi_delta_rule& r) {
     const int64_t blocks = std::max<int64_t>(1, r.envs * r.value_heads * ((r.value_dim + 63) / 64)), chunks = chunks_of(r.steps);
     if (blocks > 128) return 1;

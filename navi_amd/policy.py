@@ -139,10 +139,11 @@ def _check_state(name: str, state, q, v) -> None:
     raise RuntimeError(f"{name} must be contiguous")
 
 
-# Rollouts of so few steps go token by token: a chunk takes as long for one token as for 64. Four
-# steps and a chunk, us, with the state returned: 1 x 8 heads of 128, 9.4 and 16.4; 64 x 4 of 64,
-# float32, 7.4 and 18.2; 1024 x 4 of 64, 39 and 80; 1024 x 4 of 128, 159 and 176. Eight: 15.5 and 16.7;
-# 11.2 and 18.2; 58 and 80; 232 and 178.
+# Rollouts of so few steps go token by token: a chunk takes as long for one token as for 64, a step
+# as long as its state. Four steps and a chunk on the device, us, with the state returned: 1 x 8 heads
+# of 128, 8.6 and 14.4; 64 x 4 of 64, float32, 6.8 and 17.3; 1024 x 4 of 64, 38 and 81; 1024 x 4 of 128,
+# 157 and 180. Eight: 14.7 and 14.6; 10.6 and 17.6; 53 and 82; 227 and 182: four is safe for states of
+# any size, small ones would gain up to eight.
 _STEPWISE = 4
 
 _FARTHEST = ((1 << 31) - 1) // _native.CHUNK - (1 << 18)  # bytes between steps that the chunked kernels reach
