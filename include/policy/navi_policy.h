@@ -179,6 +179,162 @@ int64_t navi_qk_norm_workspace(const navi_qk_norm_args* args);
 int navi_clip_grad_norm(int32_t n_tensors, const void* const* from, void* const* to, const int64_t* counts,
                         const int32_t* dtypes, float max_norm, float eps, float* norm, float* partial, void* stream);
 
+/*
+ * A short convolution over the last frames, channel by channel:
+ *
+ *     z[t][c] = bias[c] + sum over k < taps of weight[c][taps - 1 - k] x[t - k][c],  out = act(z)
+ *
+ * where inputs before the first step come from `window` (zeros without one) and inputs of another
+ * episode than t's (before the last of `starts` up to t) count as zeros, whatever they hold.
+ * x: [envs][steps][channels] of `dtype` with strides of the env and step axes, the last one
+ * contiguous; out, windows and d_x contiguous. window_out receives the last taps - 1 inputs (with
+ * those of `window` where there are fewer steps), zeros in place of those of an earlier episode
+ * than the last token's. Written arrays share no memory with read ones, but with a single step out
+ * may be x and window_out window.
+ */
+#define NAVI_POLICY_MAX_TAPS 4
+#define NAVI_POLICY_NONE 0
+#define NAVI_POLICY_SILU 1 /* z / (1 + exp(-z)) */
+#define NAVI_POLICY_CONV_PARTIALS 2048
+
+typedef struct navi_causal_conv_args {
+    int32_t dtype, channels;
+    int32_t taps;       /* 2 to NAVI_POLICY_MAX_TAPS */
+    int32_t activation; /* NAVI_POLICY_NONE or NAVI_POLICY_SILU */
+    int64_t envs, steps;
+    const void* x;
+    int64_t x_stride[2];
+    const float* weight; /* [channels][taps] */
+    const float* bias;   /* [channels] or NULL */
+    const uint8_t* starts; /* [envs][steps] or NULL */
+    int64_t starts_stride[2];
+    const void* window; /* [envs][taps - 1][channels] or NULL */
+    void* out;
+    void* window_out;   /* like window, or NULL */
+    /* the backward pass (out and window_out are not read): */
+    const void* grad_out;
+    int64_t grad_out_stride[2];
+    const void* grad_window; /* of window_out, contiguous, or NULL */
+    void* d_x;
+    float* d_weight;    /* or NULL, */
+    float* d_bias;      /* or NULL, through */
+    void* d_window;     /* or NULL */
+    float* partial;     /* navi_causal_conv_workspace bytes (NULL without d_weight and d_bias) */
+} navi_causal_conv_args;
+
+int navi_causal_conv(const navi_causal_conv_args* args, void* stream);
+int navi_causal_conv_backward(const navi_causal_conv_args* args, void* stream);
+int64_t navi_causal_conv_workspace(const navi_causal_conv_args* args);
+
+/*
+ * What stands between two blocks of a residual stream. Per row of `width` numbers:
+ *
+ *     m = y / sqrt(mean y^2 + eps) post_weight silu(gate),   stream = residual + scale m,
+ *     normed = stream / sqrt(mean stream^2 + eps) pre_weight     (of the sum before it is rounded)
+ *
+ * y, gate, normed: `dtype`, residual and stream: `stream_dtype` (dtype or float32); y, residual and
+ * gate [envs][steps][width] with strides of the env and step axes, the last one contiguous; outputs
+ * contiguous. gate, scale and the weights may be NULL (factors of 1). The outputs share no memory with each other or
+ * the inputs, but stream may be residual and normed y, where those are contiguous.
+ */
+#define NAVI_POLICY_MAX_BLOCK_WIDTH 8192
+#define NAVI_POLICY_BLOCK_PARTIALS 1024
+
+typedef struct navi_block_norm_args {
+    int32_t dtype, stream_dtype;
+    int32_t width;
+    float eps;
+    int64_t envs, steps;
+    const void* y;
+    const void* residual;
+    const void* gate; /* or NULL */
+    int64_t y_stride[2], residual_stride[2], gate_stride[2];
+    const float* scale;       /* [width] or NULL, */
+    const float* post_weight; /* likewise, */
+    const float* pre_weight;  /* likewise */
+    void* stream;
+    void* normed;
+    /* the backward pass (stream and normed are not read): */
+    const void* grad_stream; /* or NULL for zeros */
+    const void* grad_normed; /* or NULL for zeros */
+    int64_t grad_stream_stride[2], grad_normed_stride[2];
+    void* d_y;
+    void* d_residual;
+    void* d_gate;         /* or NULL */
+    float* d_scale;       /* or NULL, through */
+    float* d_post_weight; /* or NULL, */
+    float* d_pre_weight;  /* or NULL, */
+    float* partial;       /* navi_block_norm_workspace bytes (NULL without those three) */
+} navi_block_norm_args;
+
+int navi_block_norm(const navi_block_norm_args* args, void* stream);
+int navi_block_norm_backward(const navi_block_norm_args* args, void* stream);
+int64_t navi_block_norm_workspace(const navi_block_norm_args* args);
+
+/*
+ * A selective state space scan. Per env and head h (of group h / (heads / groups)), with beta =
+ * softplus(dt + dt_bias[h]), the state S a state_dim x head_dim matrix of float32, cleared (whatever it
+ * holds) at a token that starts an episode:
+ *
+ *     S <- exp(beta a[h]) S + beta b x^T,   out = S^T c + d[h] x
+ *
+ * x and out: [envs][steps][heads][head_dim] of `dtype`, b and c: [envs][steps][groups][state_dim] of
+ * it, dt: [envs][steps][heads] of float32, a, d and dt_bias: [heads]. Strides are in elements, of the
+ * env, step and head (or group) axes; the last axis is contiguous, and so are out, the states and the
+ * gradients. beta a is meant to be <= 0; below -1e5 it starts an episode as `starts` does. Other
+ * inputs are finite: in the chunked form a NaN or infinity may reach every token of its chunk of
+ * NAVI_POLICY_CHUNK and what follows them.
+ */
+#define NAVI_POLICY_MAX_STATE_DIM 128 /* and head_dim */
+
+typedef struct navi_selective_scan_args {
+    int32_t dtype;
+    int32_t heads, groups;
+    int32_t state_dim, head_dim;
+    int64_t envs, steps;
+    const void* x;
+    const void* b;
+    const void* c;
+    int64_t x_stride[3], b_stride[3], c_stride[3];
+    const float* dt;
+    int64_t dt_stride[3];
+    const float* a;
+    const float* d;       /* or NULL */
+    const float* dt_bias; /* or NULL */
+    const uint8_t* starts; /* [envs][steps] or NULL */
+    int64_t starts_stride[2];
+    const float* initial_state; /* [envs][heads][state_dim][head_dim], or NULL for zeros */
+    void* out;
+    float* final_state;   /* as initial_state, or NULL; may be initial_state itself in
+                             navi_selective_step. Else it shares no memory with what is read, nor does
+                             out, which there may be x itself (contiguous) */
+    void* scratch;        /* navi_selective_scan_scratch bytes for navi_selective_scan, 16-byte aligned (NULL
+                             where that is 0) */
+    /* the backward pass (out, final_state and scratch are not read): */
+    const void* grad_out;
+    int64_t grad_out_stride[3];
+    const float* grad_final_state; /* contiguous, or NULL for zeros */
+    void* d_x;
+    void* d_b;
+    void* d_c;
+    float* d_dt;
+    float* d_a;           /* or NULL, */
+    float* d_d;           /* or NULL, */
+    float* d_dt_bias;     /* or NULL */
+    float* d_initial_state; /* or NULL */
+    void* workspace;      /* navi_selective_scan_workspace bytes, 16-byte aligned */
+} navi_selective_scan_args;
+
+/* Chunked form, for rollouts and training. */
+int navi_selective_scan(const navi_selective_scan_args* args, void* stream);
+int navi_selective_scan_backward(const navi_selective_scan_args* args, void* stream);
+int64_t navi_selective_scan_scratch(const navi_selective_scan_args* args);
+int64_t navi_selective_scan_workspace(const navi_selective_scan_args* args);
+
+/* Recurrent form: one token after another with the state in registers; for single tokens and short
+ * runs. Needs no scratch. */
+int navi_selective_step(const navi_selective_scan_args* args, void* stream);
+
 /* Message of the last failure on the calling thread ("" if none). */
 const char* navi_policy_last_error(void);
 

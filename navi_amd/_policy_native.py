@@ -21,6 +21,8 @@ F32, BF16, F16 = 0, 1, 2
 MAX_KEY_DIM, MAX_NORM_DIM, CHUNK, CHUNK_MATRICES = 128, 1024, 64, 5248
 NORM_RMS, NORM_L2 = 0, 1
 NORM_PARTIALS = 2048
+MAX_TAPS, MAX_BLOCK_WIDTH, MAX_STATE_DIM = 4, 8192, 128
+ACT_NONE, ACT_SILU = 0, 1
 
 if not LIB_PATH.exists():
     raise ImportError(
@@ -64,6 +66,38 @@ class QkNorm(ctypes.Structure):
                 ("d_q_weight", _vp), ("d_k_weight", _vp), ("partial", _vp)]
 
 
+class CausalConv(ctypes.Structure):
+    """navi_causal_conv_args (include/policy/navi_policy.h)."""
+
+    _fields_ = [("dtype", _i32), ("channels", _i32), ("taps", _i32), ("activation", _i32), ("envs", _i64), ("steps", _i64),
+                ("x", _vp), ("x_stride", _two), ("weight", _vp), ("bias", _vp), ("starts", _vp), ("starts_stride", _two),
+                ("window", _vp), ("out", _vp), ("window_out", _vp), ("grad_out", _vp), ("grad_out_stride", _two),
+                ("grad_window", _vp), ("d_x", _vp), ("d_weight", _vp), ("d_bias", _vp), ("d_window", _vp), ("partial", _vp)]
+
+
+class BlockNorm(ctypes.Structure):
+    """navi_block_norm_args (include/policy/navi_policy.h)."""
+
+    _fields_ = [("dtype", _i32), ("stream_dtype", _i32), ("width", _i32), ("eps", _f32), ("envs", _i64), ("steps", _i64),
+                ("y", _vp), ("residual", _vp), ("gate", _vp), ("y_stride", _two), ("residual_stride", _two),
+                ("gate_stride", _two), ("scale", _vp), ("post_weight", _vp), ("pre_weight", _vp), ("stream", _vp),
+                ("normed", _vp), ("grad_stream", _vp), ("grad_normed", _vp), ("grad_stream_stride", _two),
+                ("grad_normed_stride", _two), ("d_y", _vp), ("d_residual", _vp), ("d_gate", _vp), ("d_scale", _vp),
+                ("d_post_weight", _vp), ("d_pre_weight", _vp), ("partial", _vp)]
+
+
+class SelectiveScan(ctypes.Structure):
+    """navi_selective_scan_args (include/policy/navi_policy.h)."""
+
+    _fields_ = [("dtype", _i32), ("heads", _i32), ("groups", _i32), ("state_dim", _i32), ("head_dim", _i32), ("envs", _i64),
+                ("steps", _i64), ("x", _vp), ("b", _vp), ("c", _vp), ("x_stride", _three), ("b_stride", _three),
+                ("c_stride", _three), ("dt", _vp), ("dt_stride", _three), ("a", _vp), ("d", _vp), ("dt_bias", _vp),
+                ("starts", _vp), ("starts_stride", _two), ("initial_state", _vp), ("out", _vp), ("final_state", _vp),
+                ("scratch", _vp), ("grad_out", _vp), ("grad_out_stride", _three), ("grad_final_state", _vp), ("d_x", _vp),
+                ("d_b", _vp), ("d_c", _vp), ("d_dt", _vp), ("d_a", _vp), ("d_d", _vp), ("d_dt_bias", _vp),
+                ("d_initial_state", _vp), ("workspace", _vp)]
+
+
 def _packer(structure) -> struct.Struct:
     """The structure's fields in order as a packer of plain numbers (an array's one by one): a
     call's arguments in one step, a fifth of the time that setting the fields takes."""
@@ -74,14 +108,18 @@ def _packer(structure) -> struct.Struct:
 
 
 PACK_RULE, PACK_GRADIENTS, PACK_NORM = (_packer(s).pack for s in (DeltaRule, DeltaGradients, QkNorm))
+PACK_CONV, PACK_BLOCK, PACK_SCAN = (_packer(s).pack for s in (CausalConv, BlockNorm, SelectiveScan))
 
 _lib.navi_policy_last_error.restype = ctypes.c_char_p
 _lib.navi_policy_last_error.argtypes = []
 # (structures as bytes or by reference)
-for _name in ("navi_delta_forward", "navi_delta_step", "navi_qk_norm", "navi_qk_norm_backward"):
+for _name in ("navi_delta_forward", "navi_delta_step", "navi_qk_norm", "navi_qk_norm_backward",
+              "navi_causal_conv", "navi_causal_conv_backward", "navi_block_norm", "navi_block_norm_backward",
+              "navi_selective_scan", "navi_selective_scan_backward", "navi_selective_step"):
     getattr(_lib, _name).restype = ctypes.c_int
     getattr(_lib, _name).argtypes = [_vp, _vp]
-for _name in ("navi_delta_scratch", "navi_delta_workspace", "navi_qk_norm_workspace"):
+for _name in ("navi_delta_scratch", "navi_delta_workspace", "navi_qk_norm_workspace", "navi_causal_conv_workspace",
+              "navi_block_norm_workspace", "navi_selective_scan_scratch", "navi_selective_scan_workspace"):
     getattr(_lib, _name).restype = _i64
     getattr(_lib, _name).argtypes = [_vp]
 _lib.navi_delta_backward.restype = ctypes.c_int

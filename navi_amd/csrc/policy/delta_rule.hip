@@ -1274,23 +1274,6 @@ int check_rule(const navi_delta_rule* r) {
     return NAVI_POLICY_OK;
 }
 
-namespace {
-
-struct Extent {  // the bytes from an array's first number to its last
-    uintptr_t first, end;
-};
-
-Extent extent_of(const void* base, const int64_t (&counts)[4], const int64_t (&strides)[4], int64_t bytes) {
-    uintptr_t first = reinterpret_cast<uintptr_t>(base), last = first;
-    for (int i = 0; i < 4; ++i) {
-        const int64_t reach = (counts[i] - 1) * strides[i] * bytes;
-        (reach < 0 ? first : last) += static_cast<uintptr_t>(reach);
-    }
-    return Extent{first, last + static_cast<uintptr_t>(bytes)};
-}
-
-}  // namespace
-
 // Workgroups read the inputs in any order, so what is written shares no memory with them: out
 // but with v number for number (whose reader writes them), final_state in the recurrent form but
 // with initial_state (the same).
@@ -1302,7 +1285,6 @@ int check_apart(const navi_delta_rule* r, bool in_place) {
         return r->steps > 0 && p ? extent_of(p, {r->envs, r->steps, heads, dim}, {s[0], s[1], s[2], 1}, each) : Extent{0, 0};
     };
     const auto of_state = [&](const float* p) { return p ? extent_of(p, {r->envs, 1, 1, state}, {state, 0, 0, 1}, 4) : Extent{0, 0}; };
-    const auto apart = [](const Extent& a, const Extent& b) { return a.first >= a.end || b.first >= b.end || a.end <= b.first || b.end <= a.first; };
     const Extent out = of(r->out, r->value_heads, V, {r->steps * row, row, V}, bytes), final_state = of_state(r->final_state);
     const bool own = r->out == r->v && (r->value_heads == 1 || r->v_stride[2] == V) && (r->steps == 1 || r->v_stride[1] == row) &&
                      (r->envs == 1 || r->v_stride[0] == r->steps * row);

@@ -243,6 +243,46 @@ struct Part {
     }
 };
 
+template <class E>
+__device__ inline void load_eight(const E* from, float (&x)[8]) {
+    union {
+        u4 words[sizeof(E) == 4 ? 2 : 1];
+        E elements[8];
+    } got;
+    got.words[0] = *reinterpret_cast<const u4*>(from);
+    if constexpr (sizeof(E) == 4) got.words[1] = *reinterpret_cast<const u4*>(from + 4);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = to_float(got.elements[i]);
+}
+
+template <class E>
+__device__ inline void store_eight(E* to, const float (&x)[8]) {
+    union {
+        u4 words[sizeof(E) == 4 ? 2 : 1];
+        E elements[8];
+    } put;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) put.elements[i] = from_float<E>(x[i]);
+    *reinterpret_cast<u4*>(to) = put.words[0];
+    if constexpr (sizeof(E) == 4) *reinterpret_cast<u4*>(to + 4) = put.words[1];
+}
+
+// n / d for n < 2^31 by one multiplication: with 2^(l-1) < d <= 2^l, m = floor(2^(31+l) / d) + 1
+// exceeds 2^(31+l) / d by at most 1 = 2^l / 2^l, so the product's error stays under n / 2^31 < 1
+// part in d.
+struct Divisor {
+    uint32_t d, m, shift;
+};
+
+inline Divisor divisor_of(int64_t d) {
+    if (d <= 1) return Divisor{1, 0, 0};
+    int l = 0;
+    while ((int64_t{1} << l) < d) ++l;
+    return Divisor{static_cast<uint32_t>(d), static_cast<uint32_t>((uint64_t{1} << (31 + l)) / d + 1), static_cast<uint32_t>(l - 1)};
+}
+
+__device__ inline uint32_t divide(uint32_t n, Divisor by) { return by.m == 0 ? n : __umulhi(n, by.m) >> by.shift; }
+
 inline hipStream_t as_stream(void* stream) { return static_cast<hipStream_t>(stream); }
 
 template <class... P>
@@ -251,5 +291,22 @@ bool aligned(int64_t bytes, const P*... p) {
 }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+struct Extent {  // the bytes from an array's first number to its last
+    uintptr_t first, end;
+};
+
+inline Extent extent_of(const void* base, const int64_t (&counts)[4], const int64_t (&strides)[4], int64_t bytes) {
+    uintptr_t first = reinterpret_cast<uintptr_t>(base), last = first;
+    for (int i = 0; i < 4; ++i) {
+        const int64_t reach = (counts[i] - 1) * strides[i] * bytes;
+        (reach < 0 ? first : last) += static_cast<uintptr_t>(reach);
+    }
+    return Extent{first, last + static_cast<uintptr_t>(bytes)};
+}
+
+inline bool apart(const Extent& a, const Extent& b) {
+    return a.first >= a.end || b.first >= b.end || a.end <= b.first || b.end <= a.first;
+}
 
 }  // namespace navi_policy

@@ -16,22 +16,6 @@ namespace {
 constexpr int kMaxBlocks = 2048;    // workgroups of a launch for each of q and k; they stride over the rows
 constexpr int kWeightBlocks = 512;  // where a pass sums weight gradients: rows of partial sums
 
-// n / d for n < 2^31 by one multiplication: with 2^(l-1) < d <= 2^l, m = floor(2^(31+l) / d) + 1
-// exceeds 2^(31+l) / d by at most 1 = 2^l / 2^l, so the product's error stays under n / 2^31 < 1
-// part in d.
-struct Divisor {
-    uint32_t d, m, shift;
-};
-
-Divisor divisor_of(int64_t d) {
-    if (d <= 1) return Divisor{1, 0, 0};
-    int l = 0;
-    while ((int64_t{1} << l) < d) ++l;
-    return Divisor{static_cast<uint32_t>(d), static_cast<uint32_t>((uint64_t{1} << (31 + l)) / d + 1), static_cast<uint32_t>(l - 1)};
-}
-
-__device__ inline uint32_t divide(uint32_t n, Divisor by) { return by.m == 0 ? n : __umulhi(n, by.m) >> by.shift; }
-
 struct Side {  // of the queries or of the keys
     const void* x;
     const void* grad;
@@ -95,30 +79,6 @@ __device__ inline Row row_of(const NormParams& P, const Side& s, int64_t r) {
                                        : static_cast<const int32_t*>(P.positions)[offset];
     }
     return at;
-}
-
-template <class E>
-__device__ inline void load_eight(const E* from, float (&x)[8]) {
-    union {
-        u4 words[sizeof(E) == 4 ? 2 : 1];
-        E elements[8];
-    } got;
-    got.words[0] = *reinterpret_cast<const u4*>(from);
-    if constexpr (sizeof(E) == 4) got.words[1] = *reinterpret_cast<const u4*>(from + 4);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = to_float(got.elements[i]);
-}
-
-template <class E>
-__device__ inline void store_eight(E* to, const float (&x)[8]) {
-    union {
-        u4 words[sizeof(E) == 4 ? 2 : 1];
-        E elements[8];
-    } put;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) put.elements[i] = from_float<E>(x[i]);
-    *reinterpret_cast<u4*>(to) = put.words[0];
-    if constexpr (sizeof(E) == 4) *reinterpret_cast<u4*>(to + 4) = put.words[1];
 }
 
 // The rotation of eight numbers of a row at element e by its position: its angles, asked for

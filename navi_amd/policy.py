@@ -29,7 +29,8 @@ from torch.autograd.function import once_differentiable
 
 from . import _policy_native as _native
 
-__all__ = ["gated_delta_rule", "gated_delta_step", "qk_norm", "clip_grad_norm"]
+__all__ = ["gated_delta_rule", "gated_delta_step", "qk_norm", "clip_grad_norm", "causal_conv", "causal_conv_step",
+           "selective_scan", "selective_scan_step", "block_norm"]
 
 _DTYPES = {torch.float32: _native.F32, torch.bfloat16: _native.BF16, torch.float16: _native.F16}
 _MASKS = (torch.bool, torch.uint8)
@@ -443,6 +444,505 @@ def qk_norm(q: torch.Tensor, k: torch.Tensor, *, q_weight: torch.Tensor | None =
                                     or (k_weight is not None and k_weight.requires_grad)):
         return _QkNorm.apply(*args)
     return _norm_forward(*args)
+
+
+# ---- a selective state space scan ----
+
+
+def _fine_vectors(device, *wanted) -> bool:
+    """Whether each (vector or None, length) is a dense float32 vector of the device."""
+    for t, n in wanted:
+        if t is not None and not (t.dtype is torch.float32 and t.device == device and t.shape == (n,) and t.is_contiguous()):
+            return False
+    return True
+
+
+def _check_vector(name: str, t, length: int, what: str, device) -> None:
+    if t is None:
+        return
+    _check_tensor(name, t, (torch.float32,), 1, device)
+    _check(t.size(0) == length and t.is_contiguous(), f"{name} must be [{what}], contiguous")
+
+
+def _fine_scan(x, dt, a, b, c, d, dt_bias, starts) -> bool:
+    """Whether the inputs are in order ([Envs, Steps, ...] and [Envs, ...] alike)."""
+    try:
+        lead, device, dtype = x.shape[:-2], x.device, x.dtype
+        (heads, head_dim), (groups, state_dim) = x.shape[-2:], b.shape[-2:]
+        return (dtype in _DTYPES and b.dtype is dtype and c.dtype is dtype and device.type == "cuda" and b.device == device
+                and c.device == device and dt.device == device and dt.dtype is torch.float32 and dt.shape == x.shape[:-1]
+                and b.shape[:-2] == lead and c.shape == b.shape and 0 < groups <= heads and heads % groups == 0
+                and 0 < head_dim <= _native.MAX_STATE_DIM and 0 < state_dim <= _native.MAX_STATE_DIM
+                and (x.stride(-1) == 1 or head_dim == 1) and (b.stride(-1) == 1 or state_dim == 1)
+                and (c.stride(-1) == 1 or state_dim == 1) and a is not None
+                and _fine_vectors(device, (a, heads), (d, heads), (dt_bias, heads))
+                and (starts is None or (starts.dtype in _MASKS and starts.device == device and starts.shape == lead)))
+    except (AttributeError, TypeError, ValueError, IndexError):
+        return False
+
+
+def _check_scan(x, dt, a, b, c, d, dt_bias, starts, lead: tuple[str, ...]) -> None:
+    n = len(lead)
+    if _fine_scan(x, dt, a, b, c, d, dt_bias, starts) and x.dim() == n + 2:
+        return
+    shape = ", ".join(lead)
+    _check(isinstance(x, torch.Tensor) and x.is_cuda, "x must be a CUDA tensor")
+    _check_tensor("x", x, tuple(_DTYPES), n + 2)
+    for name, t in (("b", b), ("c", c)):
+        _check_like("x", name, t, (x.dtype,), n + 2, x.device)
+    _check_like("x", "dt", dt, (torch.float32,), n + 1, x.device)
+    for name, t in (("x", x), ("b", b), ("c", c)):
+        _check(_dense_last(t), f"{name} must be contiguous in its last dimension")
+    _check(b.shape == c.shape and b.shape[:n] == x.shape[:n], f"b and c must both be [{shape}, Groups, StateDim]")
+    heads, groups = x.size(n), b.size(n)
+    _check(heads > 0 and groups > 0 and heads % groups == 0, "the heads must be a multiple of the groups")
+    _check(0 < x.size(-1) <= _native.MAX_STATE_DIM and 0 < b.size(-1) <= _native.MAX_STATE_DIM,
+           f"the head and state dimensions must be in [1, {_native.MAX_STATE_DIM}]")
+    _check(dt.shape == x.shape[:-1], f"dt must be [{shape}, Heads]")
+    _check(isinstance(a, torch.Tensor), "a must be a CUDA tensor")
+    for name, t in (("a", a), ("d", d), ("dt_bias", dt_bias)):
+        _check_vector(name, t, heads, "Heads", x.device)
+    if starts is not None:
+        _check_like("x", "starts", starts, _MASKS, n, x.device)
+        _check(starts.shape == x.shape[:n], f"starts must be [{shape}]")
+    raise RuntimeError("x, dt, a, b, c, d, dt_bias and starts do not go together")
+
+
+def _check_like(of: str, name: str, t, dtypes, dims: int, device) -> None:
+    _check(isinstance(t, torch.Tensor) and t.is_cuda, f"{name} must be a CUDA tensor")
+    _check(t.device == device, f"{name} must be on the same device as {of} ({device})")
+    _check_tensor(name, t, dtypes, dims)
+
+
+def _check_scan_state(name: str, state, x, b) -> None:
+    want = (x.size(0), x.size(-2), b.size(-1), x.size(-1))
+    if (isinstance(state, torch.Tensor) and state.dtype is torch.float32 and state.device == x.device
+            and state.shape == want and state.is_contiguous()):
+        return
+    _check_like("x", name, state, (torch.float32,), 4, x.device)
+    _check(tuple(state.shape) == want, f"{name} must be [Envs, Heads, StateDim, HeadDim] = {list(want)}")
+    raise RuntimeError(f"{name} must be contiguous")
+
+
+def _pack_scan(x, dt, a, b, c, d, dt_bias, starts, initial_state, out, final_state, scratch=None, backward=(0,) * 14) -> bytes:
+    envs, steps, heads, head_dim = x.shape
+    groups, state_dim = b.shape[2:]
+    return _native.PACK_SCAN(
+        _DTYPES[x.dtype], heads, groups, state_dim, head_dim, envs, steps, x.data_ptr(), b.data_ptr(), c.data_ptr(),
+        *x.stride()[:3], *b.stride()[:3], *c.stride()[:3], dt.data_ptr(), *dt.stride(), a.data_ptr(), _ptr(d), _ptr(dt_bias),
+        *((0, 0, 0) if starts is None else (starts.data_ptr(), *starts.stride())), _ptr(initial_state), _ptr(out),
+        _ptr(final_state), _ptr(scratch), *backward)
+
+
+def _scan_forward(x, dt, a, b, c, d, dt_bias, starts, initial_state, return_state):
+    device = x.device
+    out = torch.empty(x.shape, dtype=x.dtype, device=device)
+    state = scratch = None
+    if return_state:
+        state = torch.empty((x.size(0), x.size(2), b.size(3), x.size(3)), dtype=torch.float32, device=device)
+    args = (x, dt, a, b, c, d, dt_bias, starts, initial_state, out, state)
+    packed, lib = _pack_scan(*args), _native.lib()
+    size = _native.check(lib.navi_selective_scan_scratch(packed))
+    if size:
+        scratch = torch.empty(size // 4, dtype=torch.float32, device=device)
+        packed = _pack_scan(*args, scratch)
+    _call(lib.navi_selective_scan, device, packed)
+    return out, state
+
+
+class _SelectiveScan(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, dt, a, b, c, d, dt_bias, initial_state, starts, return_state):
+        out, state = _scan_forward(x, dt, a, b, c, d, dt_bias, starts, initial_state, return_state)
+        ctx.save_for_backward(x, dt, a, b, c, d, dt_bias, initial_state, starts)
+        ctx.set_materialize_grads(False)
+        return (out, state) if return_state else out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out, grad_state=None):
+        x, dt, a, b, c, d, dt_bias, initial_state, starts = ctx.saved_tensors
+        if grad_out is None and grad_state is None:
+            return (None,) * 10
+        if grad_out is None:
+            grad_out = torch.zeros(x.shape, dtype=x.dtype, device=x.device)
+        if not _dense_last(grad_out):  # (of a broadcast, for one)
+            grad_out = grad_out.contiguous()
+        grad_out = _rows_apart(grad_out)
+        if grad_state is not None:
+            grad_state = grad_state.contiguous()
+        need = ctx.needs_input_grad
+        d_state = torch.empty_like(initial_state) if initial_state is not None and need[7] else None
+        d_vectors = [torch.empty_like(t) if t is not None and need[i] else None for i, t in ((2, a), (5, d), (6, dt_bias))]
+        d_x, d_dt, d_b, d_c = (torch.empty(t.shape, dtype=t.dtype, device=x.device) for t in (x, dt, b, c))
+        if x.numel() == 0:
+            if d_state is not None:
+                d_state = torch.zeros_like(d_state) if grad_state is None else grad_state.clone()
+            for t in d_vectors:
+                if t is not None:
+                    t.zero_()
+        else:
+            lib = _native.lib()
+            args = (x, dt, a, b, c, d, dt_bias, starts, initial_state, None, None, None)
+            back = (grad_out.data_ptr(), *grad_out.stride()[:3], _ptr(grad_state), d_x.data_ptr(), d_b.data_ptr(), d_c.data_ptr(),
+                    d_dt.data_ptr(), *[_ptr(t) for t in d_vectors], _ptr(d_state))
+            size = _native.check(lib.navi_selective_scan_workspace(_pack_scan(*args, (*back, 0))))
+            workspace = torch.empty(size // 4, dtype=torch.float32, device=x.device)
+            _call(lib.navi_selective_scan_backward, x.device, _pack_scan(*args, (*back, workspace.data_ptr())))
+        return d_x, d_dt, d_vectors[0], d_b, d_c, d_vectors[1], d_vectors[2], d_state, None, None
+
+
+def selective_scan(x: torch.Tensor, dt: torch.Tensor, a: torch.Tensor, b: torch.Tensor, c: torch.Tensor, *,
+                   d: torch.Tensor | None = None, dt_bias: torch.Tensor | None = None, starts: torch.Tensor | None = None,
+                   initial_state: torch.Tensor | None = None, return_state: bool = False):
+    """A selective state space scan over whole rollouts, differentiable in everything but ``starts``.
+
+    Per head, with ``beta = softplus(dt + dt_bias)`` and a state ``S`` of ``StateDim x HeadDim``
+    numbers: ``S <- exp(beta a) S + beta b x^T``, ``y = S^T c + d x``.
+    ``x``: ``[Envs, Steps, Heads, HeadDim]`` in float32, bfloat16 or float16, ``b``, ``c``:
+    ``[Envs, Steps, Groups, StateDim]`` of the same type, with ``Heads`` a multiple of ``Groups``
+    (head h reads group ``h // (Heads // Groups)``); both dimensions up to 128. ``dt``:
+    ``[Envs, Steps, Heads]`` float32; ``a`` (rates, at most 0), ``d`` and ``dt_bias`` (zeros by
+    default): ``[Heads]`` float32. ``starts``: ``[Envs, Steps]`` bool or uint8, tokens that begin an
+    episode: the state before one is forgotten (at the first step, whatever it holds).
+    ``initial_state``: ``[Envs, Heads, StateDim, HeadDim]`` float32, zeros by default.
+
+    Returns ``y`` like ``x``, with ``return_state`` also the state after the last token.
+    Arithmetic is of float32's precision for every type, rounded once at the end. A NaN or
+    infinity in the inputs may reach every token of its chunk of 64 tokens and what follows
+    them, beyond the start of an episode too.
+    """
+    _check_scan(x, dt, a, b, c, d, dt_bias, starts, ("Envs", "Steps"))
+    if initial_state is not None:
+        _check_scan_state("initial_state", initial_state, x, b)
+    inputs = (x, dt, a, b, c, d, dt_bias, initial_state)
+    _check_tangents(*inputs)
+    grad = torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in inputs])
+    if not grad and x.size(1) <= _STEPWISE:  # (as for the gated delta rule)
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        state = None
+        if return_state:
+            state = torch.empty((x.size(0), x.size(2), b.size(3), x.size(3)), dtype=torch.float32, device=x.device)
+        _call(_native.lib().navi_selective_step, x.device,
+              _pack_scan(x, dt, a, b, c, d, dt_bias, starts, initial_state, out, state))
+        return (out, state) if return_state else out
+    x, b, c = _rows_apart(x), _rows_apart(b), _rows_apart(c)
+    if grad:
+        return _SelectiveScan.apply(x, dt, a, b, c, d, dt_bias, initial_state, starts, bool(return_state))
+    out, state = _scan_forward(x, dt, a, b, c, d, dt_bias, starts, initial_state, return_state)
+    return (out, state) if return_state else out
+
+
+def selective_scan_step(x: torch.Tensor, dt: torch.Tensor, a: torch.Tensor, b: torch.Tensor, c: torch.Tensor,
+                        state: torch.Tensor, *, d: torch.Tensor | None = None, dt_bias: torch.Tensor | None = None,
+                        starts: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """One token of every environment: ``selective_scan`` without the ``Steps`` axis.
+
+    ``state`` (float32, ``[Envs, Heads, StateDim, HeadDim]``) is updated in place; the output
+    goes to ``out`` (like ``x``, contiguous) if given, which shares no memory with the inputs but
+    may be ``x`` itself. Autograd is told of both writes: what has saved either raises backward.
+    No gradients: this is the form for acting.
+    """
+    _check_scan(x, dt, a, b, c, d, dt_bias, starts, ("Envs",))
+    _check_scan_state("state", state, x, b)
+    written = [state]
+    if out is not None:
+        written.append(out)
+        _check_like("x", "out", out, (x.dtype,), 3, x.device)
+        _check(out.shape == x.shape and out.is_contiguous(), "out must be like x, contiguous")
+    inputs = (x, dt, a, b, c, d, dt_bias, state, out)
+    _check_tangents(*inputs)
+    if torch.is_grad_enabled():
+        _check(not any([t is not None and t.requires_grad for t in inputs]),
+               "selective_scan_step has no gradients; use selective_scan, or torch.no_grad()")
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    envs, heads, head_dim = x.shape
+    (x0, x1, _), (b0, b1, _), (c0, c1, _), at = x.stride(), b.stride(), c.stride(), state.data_ptr()
+    packed = _native.PACK_SCAN(
+        _DTYPES[x.dtype], heads, b.size(1), b.size(2), head_dim, envs, 1, x.data_ptr(), b.data_ptr(), c.data_ptr(),
+        x0, 0, x1, b0, 0, b1, c0, 0, c1, dt.data_ptr(), dt.stride(0), 0, dt.stride(1), a.data_ptr(), _ptr(d), _ptr(dt_bias),
+        *((0, 0, 0) if starts is None else (starts.data_ptr(), starts.stride(0), 0)), at, out.data_ptr(), at, 0,
+        0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
+    _call(_native.lib().navi_selective_step, x.device, packed)
+    _written(written)
+    return out
+
+
+# ---- a short convolution over the last frames ----
+
+
+_ACTIVATIONS = {"silu": _native.ACT_SILU, None: _native.ACT_NONE}
+
+
+def _fine_conv(x, weight, bias, starts, activation) -> bool:
+    try:
+        channels, device = x.size(-1), x.device
+        return (x.dtype in _DTYPES and device.type == "cuda" and (x.stride(-1) == 1 or channels == 1) and 0 < channels <= 65536
+                and weight.dtype is torch.float32 and weight.device == device and weight.dim() == 2
+                and weight.size(0) == channels and 2 <= weight.size(1) <= _native.MAX_TAPS and weight.is_contiguous()
+                and _fine_vectors(device, (bias, channels)) and activation in _ACTIVATIONS
+                and (starts is None or (starts.dtype in _MASKS and starts.device == device and starts.shape == x.shape[:-1])))
+    except (AttributeError, TypeError, ValueError, IndexError, RuntimeError):
+        return False
+
+
+def _check_conv(x, weight, bias, starts, activation, lead: tuple[str, ...]) -> None:
+    n = len(lead)
+    if _fine_conv(x, weight, bias, starts, activation) and x.dim() == n + 1:
+        return
+    shape = ", ".join(lead)
+    _check(isinstance(x, torch.Tensor) and x.is_cuda, "x must be a CUDA tensor")
+    _check_tensor("x", x, tuple(_DTYPES), n + 1)
+    _check(_dense_last(x), "x must be contiguous in its last dimension")
+    _check(0 < x.size(-1) <= 65536, "the channels must be in [1, 65536]")
+    _check_like("x", "weight", weight, (torch.float32,), 2, x.device)
+    _check(weight.size(0) == x.size(-1) and 2 <= weight.size(1) <= _native.MAX_TAPS and weight.is_contiguous(),
+           f"weight must be [Channels, Taps], contiguous, with 2 to {_native.MAX_TAPS} taps")
+    _check_vector("bias", bias, x.size(-1), "Channels", x.device)
+    if starts is not None:
+        _check_like("x", "starts", starts, _MASKS, n, x.device)
+        _check(starts.shape == x.shape[:-1], f"starts must be [{shape}]")
+    _check(activation in _ACTIVATIONS, "activation must be 'silu' or None")
+    raise RuntimeError("x, weight, bias and starts do not go together")
+
+
+def _check_window(name: str, window, x, weight) -> None:
+    want = (x.size(0), weight.size(1) - 1, x.size(-1))
+    if (isinstance(window, torch.Tensor) and window.dtype is x.dtype and window.device == x.device
+            and window.shape == want and window.is_contiguous()):
+        return
+    _check_like("x", name, window, (x.dtype,), 3, x.device)
+    _check(tuple(window.shape) == want, f"{name} must be [Envs, Taps - 1, Channels] = {list(want)}")
+    raise RuntimeError(f"{name} must be contiguous")
+
+
+def _pack_conv(x, weight, bias, starts, activation, window, out, window_out, backward=(0,) * 9) -> bytes:
+    envs, steps, channels = x.shape
+    return _native.PACK_CONV(
+        _DTYPES[x.dtype], channels, weight.size(1), _ACTIVATIONS[activation], envs, steps, x.data_ptr(), *x.stride()[:2],
+        weight.data_ptr(), _ptr(bias), *((0, 0, 0) if starts is None else (starts.data_ptr(), *starts.stride())),
+        _ptr(window), _ptr(out), _ptr(window_out), *backward)
+
+
+def _conv_forward(x, weight, bias, starts, activation, window, return_window):
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    after = torch.empty((x.size(0), weight.size(1) - 1, x.size(2)), dtype=x.dtype, device=x.device) if return_window else None
+    _call(_native.lib().navi_causal_conv, x.device, _pack_conv(x, weight, bias, starts, activation, window, out, after))
+    return out, after
+
+
+class _CausalConv(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, window, starts, activation, return_window):
+        ctx.save_for_backward(x, weight, bias, window, starts)
+        ctx.activation = activation
+        ctx.set_materialize_grads(False)
+        out, after = _conv_forward(x, weight, bias, starts, activation, window, return_window)
+        return (out, after) if return_window else out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out, grad_window=None):
+        x, weight, bias, window, starts = ctx.saved_tensors
+        if grad_out is None and grad_window is None:
+            return (None,) * 7
+        if grad_out is None:
+            grad_out = torch.zeros((), dtype=x.dtype, device=x.device).expand(x.shape)
+        if not _dense_last(grad_out):
+            grad_out = grad_out.contiguous()
+        if grad_window is not None:
+            grad_window = grad_window.contiguous()
+        need = ctx.needs_input_grad
+        d_x = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        d_weight = torch.empty_like(weight) if need[1] else None
+        d_bias = torch.empty_like(bias) if bias is not None and need[2] else None
+        d_window = torch.empty_like(window) if window is not None and need[3] else None
+        if x.numel() == 0:
+            for t in (d_weight, d_bias):
+                if t is not None:
+                    t.zero_()
+            if d_window is not None:
+                d_window = torch.zeros_like(d_window) if grad_window is None else grad_window.clone()
+            return d_x, d_weight, d_bias, d_window, None, None, None
+        lib, partial = _native.lib(), None
+        args = (x, weight, bias, starts, ctx.activation, window, None, None)
+        if d_weight is not None or d_bias is not None:
+            size = _native.check(lib.navi_causal_conv_workspace(_pack_conv(*args)))
+            partial = torch.empty(size // 4, dtype=torch.float32, device=x.device)
+        _call(lib.navi_causal_conv_backward, x.device, _pack_conv(*args, (
+            grad_out.data_ptr(), *grad_out.stride()[:2], _ptr(grad_window), d_x.data_ptr(), _ptr(d_weight), _ptr(d_bias),
+            _ptr(d_window), _ptr(partial))))
+        return d_x, d_weight, d_bias, d_window, None, None, None
+
+
+def causal_conv(x: torch.Tensor, weight: torch.Tensor, *, bias: torch.Tensor | None = None,
+                starts: torch.Tensor | None = None, initial_window: torch.Tensor | None = None,
+                return_window: bool = False, activation: str | None = "silu"):
+    """A short convolution over the last frames of a rollout, channel by channel; differentiable in
+    x, weight, bias and initial_window.
+
+    ``y[t] = act(bias + sum_j weight[:, j] x[t - (Taps - 1) + j])``. ``x``: ``[Envs, Steps, Channels]``
+    in float32, bfloat16 or float16; ``weight``: ``[Channels, Taps]`` float32 with 2 to 4 taps;
+    ``bias``: ``[Channels]`` float32. ``activation``: ``"silu"`` or None. ``starts``: ``[Envs, Steps]``
+    bool or uint8, tokens that begin an episode: inputs before one count as zeros for it and what
+    follows, whatever they hold. ``initial_window``: ``[Envs, Taps - 1, Channels]`` like ``x``, the
+    inputs before the first step (zeros by default).
+
+    Returns ``y`` like ``x``, with ``return_window`` also the window after the last step: its last
+    ``Taps - 1`` inputs, zeros in place of those of an earlier episode. Sums are float32's, rounded
+    once at the end.
+    """
+    _check_conv(x, weight, bias, starts, activation, ("Envs", "Steps"))
+    if initial_window is not None:
+        _check_window("initial_window", initial_window, x, weight)
+    inputs = (x, weight, bias, initial_window)
+    _check_tangents(*inputs)
+    if torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in inputs]):
+        return _CausalConv.apply(*inputs, starts, activation, bool(return_window))
+    out, after = _conv_forward(x, weight, bias, starts, activation, initial_window, return_window)
+    return (out, after) if return_window else out
+
+
+def causal_conv_step(x: torch.Tensor, weight: torch.Tensor, window: torch.Tensor, *, bias: torch.Tensor | None = None,
+                     starts: torch.Tensor | None = None, activation: str | None = "silu",
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+    """One frame of every environment: ``causal_conv`` without the ``Steps`` axis.
+
+    ``window`` (``[Envs, Taps - 1, Channels]`` like ``x``) is updated in place; the output goes to
+    ``out`` (like ``x``, contiguous) if given, which shares no memory with the inputs but may be
+    ``x`` itself. Autograd is told of both writes. No gradients: this is the form for acting.
+    """
+    _check_conv(x, weight, bias, starts, activation, ("Envs",))
+    _check_window("window", window, x, weight)
+    written = [window]
+    if out is not None:
+        written.append(out)
+        _check_like("x", "out", out, (x.dtype,), 2, x.device)
+        _check(out.shape == x.shape and out.is_contiguous(), "out must be like x, contiguous")
+    inputs = (x, weight, bias, window, out)
+    _check_tangents(*inputs)
+    if torch.is_grad_enabled():
+        _check(not any([t is not None and t.requires_grad for t in inputs]),
+               "causal_conv_step has no gradients; use causal_conv, or torch.no_grad()")
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    at = window.data_ptr()
+    packed = _native.PACK_CONV(
+        _DTYPES[x.dtype], x.size(1), weight.size(1), _ACTIVATIONS[activation], x.size(0), 1, x.data_ptr(), x.stride(0), 0,
+        weight.data_ptr(), _ptr(bias), *((0, 0, 0) if starts is None else (starts.data_ptr(), starts.stride(0), 0)),
+        at, out.data_ptr(), at, 0, 0, 0, 0, 0, 0, 0, 0, 0)
+    _call(_native.lib().navi_causal_conv, x.device, packed)
+    _written(written)
+    return out
+
+
+# ---- between two blocks of a residual stream ----
+
+
+def _fine_block(y, residual, gate, scale, post_weight, pre_weight) -> bool:
+    try:
+        device, dtype, width = y.device, y.dtype, y.size(-1)
+        return (dtype in _DTYPES and device.type == "cuda" and y.dim() == 3 and residual.device == device
+                and (residual.dtype is dtype or residual.dtype is torch.float32) and residual.shape == y.shape
+                and 0 < width <= _native.MAX_BLOCK_WIDTH and (width == 1 or (y.stride(2) == 1 and residual.stride(2) == 1))
+                and (gate is None or (gate.dtype is dtype and gate.device == device and gate.shape == y.shape
+                                      and (gate.stride(2) == 1 or width == 1)))
+                and _fine_vectors(device, (scale, width), (post_weight, width), (pre_weight, width)))
+    except (AttributeError, TypeError, ValueError, IndexError, RuntimeError):
+        return False
+
+
+def _check_block(y, residual, gate, scale, post_weight, pre_weight) -> None:
+    if _fine_block(y, residual, gate, scale, post_weight, pre_weight):
+        return
+    _check(isinstance(y, torch.Tensor) and y.is_cuda, "y must be a CUDA tensor")
+    _check_tensor("y", y, tuple(_DTYPES), 3)
+    _check_like("y", "residual", residual, tuple({y.dtype, torch.float32}), 3, y.device)
+    _check(residual.shape == y.shape, "residual must be [Envs, Steps, Width] like y")
+    if gate is not None:
+        _check_like("y", "gate", gate, (y.dtype,), 3, y.device)
+        _check(gate.shape == y.shape, "gate must be [Envs, Steps, Width] like y")
+    for name, t in (("y", y), ("residual", residual), ("gate", gate)):
+        _check(t is None or _dense_last(t), f"{name} must be contiguous in its last dimension")
+    _check(0 < y.size(2) <= _native.MAX_BLOCK_WIDTH, f"the width must be in [1, {_native.MAX_BLOCK_WIDTH}]")
+    for name, t in (("scale", scale), ("post_weight", post_weight), ("pre_weight", pre_weight)):
+        _check_vector(name, t, y.size(2), "Width", y.device)
+    raise RuntimeError("y, residual, gate, scale and the weights do not go together")
+
+
+def _pack_block(y, residual, gate, scale, post_weight, pre_weight, eps, outputs, backward=(0,) * 13) -> bytes:
+    envs, steps, width = y.shape
+    return _native.PACK_BLOCK(
+        _DTYPES[y.dtype], _DTYPES[residual.dtype], width, eps, envs, steps, y.data_ptr(), residual.data_ptr(), _ptr(gate),
+        *y.stride()[:2], *residual.stride()[:2], *((0, 0) if gate is None else gate.stride()[:2]), _ptr(scale),
+        _ptr(post_weight), _ptr(pre_weight), *outputs, *backward)
+
+
+def _block_forward(y, residual, *rest):
+    stream = torch.empty(y.shape, dtype=residual.dtype, device=y.device)
+    normed = torch.empty(y.shape, dtype=y.dtype, device=y.device)
+    _call(_native.lib().navi_block_norm, y.device, _pack_block(y, residual, *rest, (stream.data_ptr(), normed.data_ptr())))
+    return stream, normed
+
+
+class _BlockNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, residual, gate, scale, post_weight, pre_weight, eps):
+        ctx.save_for_backward(y, residual, gate, scale, post_weight, pre_weight)
+        ctx.eps = eps
+        ctx.set_materialize_grads(False)
+        return _block_forward(y, residual, gate, scale, post_weight, pre_weight, eps)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_stream, grad_normed):
+        y, residual, gate, *vectors = ctx.saved_tensors
+        if grad_stream is None and grad_normed is None:
+            return (None,) * 7
+        grads = [t if t is None or _dense_last(t) else t.contiguous() for t in (grad_stream, grad_normed)]
+        need = ctx.needs_input_grad
+        d_y, d_residual = (torch.empty(t.shape, dtype=t.dtype, device=y.device) for t in (y, residual))
+        d_gate = torch.empty(y.shape, dtype=y.dtype, device=y.device) if gate is not None and need[2] else None
+        d_vectors = [torch.empty_like(t) if t is not None and need[3 + i] else None for i, t in enumerate(vectors)]
+        if y.numel() == 0:
+            for t in d_vectors:
+                if t is not None:
+                    t.zero_()
+            return d_y, d_residual, d_gate, *d_vectors, None
+        args, lib, partial = (y, residual, gate, *vectors, ctx.eps, (0, 0)), _native.lib(), None
+        if any([t is not None for t in d_vectors]):
+            size = _native.check(lib.navi_block_norm_workspace(_pack_block(*args)))
+            partial = torch.empty(size // 4, dtype=torch.float32, device=y.device)
+        strides = [s for t in grads for s in ((0, 0) if t is None else t.stride()[:2])]
+        _call(lib.navi_block_norm_backward, y.device, _pack_block(*args, (
+            *[_ptr(t) for t in grads], *strides, d_y.data_ptr(), d_residual.data_ptr(), _ptr(d_gate),
+            *[_ptr(t) for t in d_vectors], _ptr(partial))))
+        return d_y, d_residual, d_gate, *d_vectors, None
+
+
+def block_norm(y: torch.Tensor, residual: torch.Tensor, *, gate: torch.Tensor | None = None,
+               scale: torch.Tensor | None = None, post_weight: torch.Tensor | None = None,
+               pre_weight: torch.Tensor | None = None, eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor]:
+    """What stands between two blocks of a residual stream, in one pass: the norm after a block, its
+    gate and scale, the sum with the stream, and the norm before the next block; differentiable in
+    everything.
+
+    ``stream = residual + scale * norm(y) * post_weight * silu(gate)`` and ``normed = norm(stream) *
+    pre_weight``, with ``norm(x) = x / sqrt(mean(x^2) + eps)`` over the last axis; what is not given
+    is left out. ``y`` (the block's output) and ``gate``: ``[Envs, Steps, Width]`` in float32, bfloat16 or
+    float16, width up to 8192; ``residual``: the stream before, of the same type or float32;
+    ``scale``, ``post_weight``, ``pre_weight``: ``[Width]`` float32. Returns ``stream`` like
+    ``residual`` and ``normed`` like ``y``; ``normed`` is that of the sum before it is rounded.
+    """
+    _check_block(y, residual, gate, scale, post_weight, pre_weight)
+    eps = float(eps)
+    _check(math.isfinite(eps) and eps >= 0.0, "eps must be finite and not negative")
+    inputs = (y, residual, gate, scale, post_weight, pre_weight)
+    _check_tangents(*inputs)
+    if torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in inputs]):
+        return _BlockNorm.apply(*inputs, eps)
+    return _block_forward(*inputs, eps)
 
 
 # ---- the norm of all gradients ----
