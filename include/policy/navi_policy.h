@@ -335,6 +335,28 @@ int64_t navi_selective_scan_workspace(const navi_selective_scan_args* args);
  * runs. Needs no scratch. */
 int navi_selective_step(const navi_selective_scan_args* args, void* stream);
 
+/*
+ * Matrices made nearly orthogonal: X = G / (|G| + eps) with |G| the root of the sum of squares, then
+ * `steps` times X <- a X + (b A + c A A) X with A = X X^T (X is G or its transpose, the one with no
+ * more rows than columns), into `to` in G's orientation.
+ * from: rows x cols numbers with the strides (in elements) of rows and columns, one of them 1; to:
+ * any strides. Results in bfloat16 take products of float16, float32 and float16 ones products of
+ * two float16 each (22 bits). A matrix may be written in its place; otherwise what is written shares
+ * no memory with what else is written or read. `matrices` is a host array, read during the call.
+ */
+typedef struct navi_orthogonalize_matrix {
+    const void* from;
+    void* to;
+    int64_t rows, cols; /* at most 2^20 each, 2^31 numbers */
+    int64_t from_stride[2], to_stride[2];
+    int32_t from_dtype, to_dtype; /* NAVI_POLICY_* */
+} navi_orthogonalize_matrix;
+
+/* `workspace`: navi_orthogonalize_workspace bytes, 256-byte aligned. */
+int navi_orthogonalize(int32_t count, const navi_orthogonalize_matrix* matrices, int32_t steps, float a, float b, float c,
+                       float eps, void* workspace, void* stream);
+int64_t navi_orthogonalize_workspace(int32_t count, const navi_orthogonalize_matrix* matrices);
+
 /* Message of the last failure on the calling thread ("" if none). */
 const char* navi_policy_last_error(void);
 

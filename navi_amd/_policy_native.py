@@ -98,6 +98,13 @@ class SelectiveScan(ctypes.Structure):
                 ("d_initial_state", _vp), ("workspace", _vp)]
 
 
+class OrthogonalizeMatrix(ctypes.Structure):
+    """navi_orthogonalize_matrix (include/policy/navi_policy.h)."""
+
+    _fields_ = [("from_", _vp), ("to", _vp), ("rows", _i64), ("cols", _i64), ("from_stride", _two), ("to_stride", _two),
+                ("from_dtype", _i32), ("to_dtype", _i32)]
+
+
 def _packer(structure) -> struct.Struct:
     """The structure's fields in order as a packer of plain numbers (an array's one by one): a
     call's arguments in one step, a fifth of the time that setting the fields takes."""
@@ -109,6 +116,7 @@ def _packer(structure) -> struct.Struct:
 
 PACK_RULE, PACK_GRADIENTS, PACK_NORM = (_packer(s).pack for s in (DeltaRule, DeltaGradients, QkNorm))
 PACK_CONV, PACK_BLOCK, PACK_SCAN = (_packer(s).pack for s in (CausalConv, BlockNorm, SelectiveScan))
+PACK_MATRIX = _packer(OrthogonalizeMatrix).pack
 
 _lib.navi_policy_last_error.restype = ctypes.c_char_p
 _lib.navi_policy_last_error.argtypes = []
@@ -124,6 +132,10 @@ for _name in ("navi_delta_scratch", "navi_delta_workspace", "navi_qk_norm_worksp
     getattr(_lib, _name).argtypes = [_vp]
 _lib.navi_delta_backward.restype = ctypes.c_int
 _lib.navi_delta_backward.argtypes = [_vp, _vp, _vp]
+_lib.navi_orthogonalize.restype = ctypes.c_int
+_lib.navi_orthogonalize.argtypes = [_i32, _vp, _i32, _f32, _f32, _f32, _f32, _vp, _vp]
+_lib.navi_orthogonalize_workspace.restype = _i64
+_lib.navi_orthogonalize_workspace.argtypes = [_i32, _vp]
 _lib.navi_clip_grad_norm.restype = ctypes.c_int
 _lib.navi_clip_grad_norm.argtypes = [_i32, _vp, _vp, _vp, _vp, _f32, _f32, _vp, _vp, _vp]
 

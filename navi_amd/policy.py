@@ -30,7 +30,7 @@ from torch.autograd.function import once_differentiable
 from . import _policy_native as _native
 
 __all__ = ["gated_delta_rule", "gated_delta_step", "qk_norm", "clip_grad_norm", "causal_conv", "causal_conv_step",
-           "selective_scan", "selective_scan_step", "block_norm"]
+           "selective_scan", "selective_scan_step", "block_norm", "orthogonalize"]
 
 _DTYPES = {torch.float32: _native.F32, torch.bfloat16: _native.BF16, torch.float16: _native.F16}
 _MASKS = (torch.bool, torch.uint8)
@@ -1005,3 +1005,82 @@ def _check_grads(grads: list, to: list) -> None:
             _check(isinstance(y, torch.Tensor) and y.dtype == x.dtype and y.shape == x.shape and y.device == x.device
                    and (y.is_contiguous() if x.is_contiguous() else y.stride() == x.stride()),
                    "out must be like grads in shapes, types, strides and device")
+
+
+# ---- orthogonal updates ----
+
+
+_NEWTON = (3.4445, -4.775, 2.0315)
+
+
+def orthogonalize(updates: Iterable[torch.Tensor | None], *, steps: int = 5,
+                  factors: tuple[float, float, float] = _NEWTON, eps: float = 1e-6,
+                  out: Iterable[torch.Tensor | None] | None = None) -> None:
+    """Makes matrices nearly orthogonal by Newton-Schulz products, as an optimizer's update of weight
+    matrices: ``X = G / (|G| + eps)`` (``|G|`` the root of the sum of squares), then ``steps``
+    times ``X <- a X + (b A + c A A) X`` with ``A = X X^T`` and ``(a, b, c) = factors``, where ``X`` is
+    ``G`` or its transpose, the one with no more rows than columns. With the default factors the
+    singular values come out between 0.7 and 1.2.
+
+    ``updates``: float32, bfloat16 and float16 matrices of one device in any mix of sizes and types
+    (None is skipped), each contiguous along its rows or its columns; they are replaced, or the
+    results go to ``out``, tensors of the same shapes (of any of these types and any strides that do
+    not overlap). Tensors that are written share no memory with others. Results in bfloat16 take
+    products of float16 (2 to 5 parts in 10^4 before their rounding), others products of two float16
+    each, of float32's precision. A matrix that holds an infinity or NaN comes out without meaning.
+    """
+    steps, eps = int(steps), float(eps)
+    a, b, c = (float(x) for x in factors)
+    _check(1 <= steps <= 100, "steps must be in [1, 100]")
+    _check(math.isfinite(eps) and eps >= 0.0, "eps must be finite and not negative")
+    _check(math.isfinite(a) and math.isfinite(b) and math.isfinite(c), "factors must be finite")
+    updates = list(updates)
+    to = updates if out is None else list(out)
+    _check(len(to) == len(updates), "out must be as long as updates")
+    if any([x is None for x in updates]):
+        to = [y for x, y in zip(updates, to) if x is not None]
+        updates = [x for x in updates if x is not None]
+    _check(len(updates) > 0, "updates must hold at least one matrix")
+    _check_matrices(updates, to)
+    _check_tangents(*updates, *to)
+    n, device = len(updates), updates[0].device
+    packed = b"".join([_native.PACK_MATRIX(x.data_ptr(), y.data_ptr(), *x.shape, *_strides_of(x), *_strides_of(y),
+                                           _DTYPES[x.dtype], _DTYPES[y.dtype]) for x, y in zip(updates, to)])
+    lib = _native.lib()
+    size = _native.check(lib.navi_orthogonalize_workspace(n, packed))
+    workspace = torch.empty(size, dtype=torch.uint8, device=device)
+    _call(lib.navi_orthogonalize, device, n, packed, steps, a, b, c, eps, workspace.data_ptr())
+    _written(to)
+
+
+def _strides_of(x: torch.Tensor) -> tuple[int, int]:
+    """A matrix's strides, those of axes of one as in a contiguous one."""
+    r, c = x.stride()
+    return (r if x.size(0) > 1 else (x.size(1) if c == 1 else 1), c if x.size(1) > 1 else (1 if r != 1 or x.size(0) <= 1 else x.size(0)))
+
+
+def _check_matrices(updates: list, to: list) -> None:
+    try:
+        device = updates[0].get_device()
+        if device >= 0 and all([x.dim() == 2 and x.get_device() == device and x.dtype in _DTYPES and x.is_contiguous() for x in updates]) and (
+                to is updates or all([y.get_device() == device and y.dtype in _DTYPES and y.shape == x.shape and y.is_contiguous()
+                                      for x, y in zip(updates, to)])):
+            return
+    except (AttributeError, TypeError, RuntimeError):
+        pass
+    for x, y in zip(updates, to):
+        _check(isinstance(x, torch.Tensor) and x.is_cuda and x.layout == torch.strided, "updates must be dense CUDA tensors")
+        _check(x.dim() == 2, "updates must be matrices")
+        _check(x.dtype in _DTYPES, "updates must be float32, bfloat16 or float16")
+        _check(x.device == updates[0].device, "updates must be on one device")
+        _check(1 in _strides_of(x) or x.numel() == 0, "updates must be contiguous along their rows or columns")
+        if y is not x:
+            _check(isinstance(y, torch.Tensor) and y.is_cuda and y.layout == torch.strided and y.dtype in _DTYPES
+                   and y.shape == x.shape and y.device == x.device,
+                   "out must be like updates in shapes and device, float32, bfloat16 or float16")
+        _check(y.numel() == 0 or _apart_elements(y), "what is written must not overlap itself")
+
+
+def _apart_elements(x: torch.Tensor) -> bool:
+    (m, n), (r, c) = x.shape, _strides_of(x)
+    return (c >= 1 and r >= (n - 1) * c + 1) or (r >= 1 and c >= (m - 1) * r + 1)
