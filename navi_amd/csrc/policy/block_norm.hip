@@ -239,20 +239,13 @@ __global__ __launch_bounds__(256) void block_norm_backward_kernel(BlockParams P)
     }
 }
 
-// The partial sums of 64 columns by four waves.
-__global__ __launch_bounds__(256) void block_norm_sums_kernel(BlockParams P) {
-    __shared__ double part[4][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int column = blockIdx.x * 64 + lane, columns = 3 * P.a.width;
-    double sum = 0.0;
-    if (column < columns)
-        for (int b = wave; b < P.blocks; b += 4) sum += P.a.partial[static_cast<int64_t>(b) * columns + column];
-    part[wave][lane] = sum;
-    __syncthreads();
-    if (wave != 0 || column >= columns) return;
+__global__ __launch_bounds__(1024) void block_norm_sums_kernel(BlockParams P) {
+    const int column = blockIdx.x * kSumColumns + threadIdx.x % kSumColumns, columns = 3 * P.a.width;
+    const float all = sum_of_column(P.a.partial, P.blocks, columns, column);
+    if (threadIdx.x >= kSumColumns || column >= columns) return;
     float* to[3] = {P.a.d_scale, P.a.d_post_weight, P.a.d_pre_weight};
     float* at = to[column / P.a.width];
-    if (at) at[column % P.a.width] = static_cast<float>((part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]));
+    if (at) at[column % P.a.width] = all;
 }
 
 int launched(const char* name) {
@@ -272,7 +265,7 @@ int run(BlockParams& P, bool back, hipStream_t stream) {
     }
     const unsigned lds = P.a.partial ? kVecs * 8 * 256 * sizeof(float) : 0;
     hipLaunchKernelGGL((block_norm_backward_kernel<E, R, kLanes, kVecs>), dim3(P.blocks), dim3(256), lds, stream, P);
-    if (P.a.partial) hipLaunchKernelGGL(block_norm_sums_kernel, dim3((3 * P.a.width + 63) / 64), dim3(256), 0, stream, P);
+    if (P.a.partial) hipLaunchKernelGGL(block_norm_sums_kernel, dim3((3 * P.a.width + kSumColumns - 1) / kSumColumns), dim3(1024), 0, stream, P);
     return launched("navi_block_norm_backward");
 }
 

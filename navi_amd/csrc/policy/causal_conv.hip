@@ -316,19 +316,11 @@ __global__ __launch_bounds__(256) void causal_conv_backward_kernel(ConvParams P)
     }
 }
 
-// The partial sums of 64 columns by four waves.
 template <int kTaps>
-__global__ __launch_bounds__(256) void causal_conv_sums_kernel(ConvParams P) {
-    __shared__ double part[4][64];
-    const int32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int32_t column = blockIdx.x * 64 + lane, columns = (kTaps + 1) * P.a.channels;
-    double sum = 0.0;
-    if (column < columns)
-        for (int32_t b = wave; b < P.down_blocks; b += 4) sum += P.a.partial[static_cast<int64_t>(b) * columns + column];
-    part[wave][lane] = sum;
-    __syncthreads();
-    if (wave != 0 || column >= columns) return;
-    const float all = static_cast<float>((part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]));
+__global__ __launch_bounds__(1024) void causal_conv_sums_kernel(ConvParams P) {
+    const int32_t column = blockIdx.x * kSumColumns + threadIdx.x % kSumColumns, columns = (kTaps + 1) * P.a.channels;
+    const float all = sum_of_column(P.a.partial, P.down_blocks, columns, column);
+    if (threadIdx.x >= kSumColumns || column >= columns) return;
     const int32_t k = column / P.a.channels, channel = column % P.a.channels;
     if (k == kTaps) {
         if (P.a.d_bias) P.a.d_bias[channel] = all;
@@ -411,7 +403,8 @@ int run(ConvParams& P, bool back, hipStream_t stream) {
     const unsigned lds = P.a.partial ? (kTaps + 1) * kVec * 256 * sizeof(float) : 0;
     hipLaunchKernelGGL((causal_conv_backward_kernel<E, kVec, kTaps>), dim3(static_cast<unsigned>(blocks)), dim3(256), lds, stream, P);
     if (P.a.partial)
-        hipLaunchKernelGGL((causal_conv_sums_kernel<kTaps>), dim3(((kTaps + 1) * P.a.channels + 63) / 64), dim3(256), 0, stream, P);
+        hipLaunchKernelGGL((causal_conv_sums_kernel<kTaps>), dim3(((kTaps + 1) * P.a.channels + kSumColumns - 1) / kSumColumns), dim3(1024), 0,
+                           stream, P);
     return launched("navi_causal_conv_backward");
 }
 

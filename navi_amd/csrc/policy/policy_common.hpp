@@ -158,6 +158,35 @@ __device__ inline u2 read_transposed(const uint16_t* lds) {
     return __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((pointer)(lds)));
 }
 
+// Sums of a column of partial sums by a workgroup of 1024 that takes 16 columns: 64 threads a column,
+// four rows in flight each, in float64. Thread 16 r + c has column c and rows r, r + 64, ...; the sum is
+// thread c's.
+constexpr int kSumColumns = 16;
+
+__device__ inline float sum_of_column(const float* partial, int rows, int columns, int column) {
+    __shared__ double part[16][kSumColumns];
+    double sum = 0.0;
+    if (column < columns) {
+        int row = threadIdx.x / kSumColumns;
+        for (; row + 192 < rows; row += 256) {
+            float x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = partial[static_cast<int64_t>(row + 64 * i) * columns + column];
+            sum += (static_cast<double>(x[0]) + x[1]) + (static_cast<double>(x[2]) + x[3]);
+        }
+        for (; row < rows; row += 64) sum += partial[static_cast<int64_t>(row) * columns + column];
+    }
+    sum += __shfl_xor(sum, 16);
+    sum += __shfl_xor(sum, 32);
+    if ((threadIdx.x & 63) < kSumColumns) part[threadIdx.x >> 6][threadIdx.x & 15] = sum;
+    __syncthreads();
+    double all = 0.0;
+    if (threadIdx.x < kSumColumns)
+#pragma unroll
+        for (int w = 0; w < 16; ++w) all += part[w][threadIdx.x];
+    return static_cast<float>(all);
+}
+
 // Buffer accesses: a scalar base and size and a lane's 32-bit offset; loads from kOutside or
 // past the size give 0, stores there are dropped, so tails need no branches. The whole offset
 // is the lane's: a scalar part beyond the size would turn the range check around (it compares

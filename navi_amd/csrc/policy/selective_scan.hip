@@ -94,6 +94,32 @@ struct ScanParams {
     Role role[3];
 };
 
+// A lane's neighbours by moves within the vector unit: lane l - n of its row of 16, or (143 and 142) the
+// last lane of the row or the half before it; 0 where there is none.
+template <int kControl, int kRows = 15>
+__device__ inline double lane_before(double x) {
+    const u2 w = __builtin_bit_cast(u2, x);
+    return __builtin_bit_cast(double, u2{static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(w.x), kControl, kRows, 15, false)),
+                                         static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(w.y), kControl, kRows, 15, false))});
+}
+
+// Sums over the lanes up to each.
+__device__ inline double sum_up(double x) {
+    x += lane_before<0x111>(x);
+    x += lane_before<0x112>(x);
+    x += lane_before<0x114>(x);
+    x += lane_before<0x118>(x);
+    x += lane_before<0x142, 10>(x);
+    x += lane_before<0x143, 12>(x);
+    return x;
+}
+
+__device__ inline double of_lane(double x, int lane) {
+    const u2 w = __builtin_bit_cast(u2, x);
+    return __builtin_bit_cast(double, u2{static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(w.x), lane)),
+                                         static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(w.y), lane))});
+}
+
 __device__ inline float softplus(float z) { return fmaxf(z, 0.0f) + log1pf(expf(-fabsf(z))); }
 
 // A chunk's gates in LDS.
@@ -102,6 +128,8 @@ struct ScanGates {
     float e[kChunk], f[kChunk];    // E; F, times beta where that is on the values
     float beta[kChunk], diagonal[kChunk];  // (diagonal: q . k of each token)
     int32_t episode[kChunk];       // episodes begun in the chunk so far
+    // D_ij (beta_j) of tiles below the diagonal as down_i across_j, from and to the first token of i's tile
+    float down[kChunk], across[3][kChunk];
 };
 
 struct ScanGatesFetch {
@@ -130,17 +158,24 @@ struct ScanGatesFetch {
         const bool decays = inside && !(reverse && lane == 0 && low + tokens == P.steps);
         const double g = decays ? static_cast<double>(reverse ? softplus(after + bias) : beta) * a : 0.0;
         const bool starts = start != 0 || g < kStart;
-        double sum = starts ? 0.0 : g;
+        const double sum = sum_up(starts ? 0.0 : g);
         const uint64_t all = __ballot(starts);
         const int episode = __popcll(all << (63 - lane)), last_episode = __popcll(all);
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const double s = __shfl_up(sum, d);
-            sum += lane >= d ? s : 0.0;
-        }
         const float hi = static_cast<float>(sum), lo = static_cast<float>(sum - hi);
-        const double last = __shfl(sum, 63);
+        const double last = of_lane(sum, 63);
         const float f = episode == last_episode ? expf(static_cast<float>(last - sum)) : 0.0f;
+        double own = of_lane(sum, 0);  // of the first token of the lane's tile
+        int own_episode = __builtin_amdgcn_readlane(episode, 0);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+            const double first = of_lane(sum, 16 * i + 16);
+            const int first_episode = __builtin_amdgcn_readlane(episode, 16 * i + 16);
+            const float x = episode == first_episode ? expf(static_cast<float>(first - sum)) : 0.0f;
+            gates.across[i][lane] = reverse ? x : x * beta;
+            own = lane >= 16 * i + 16 ? first : own;
+            own_episode = lane >= 16 * i + 16 ? first_episode : own_episode;
+        }
+        gates.down[lane] = episode == own_episode ? expf(static_cast<float>(sum - own)) : 0.0f;
         gates.hi[lane] = hi;
         gates.lo[lane] = lo;
         gates.e[lane] = episode == 0 ? expf(hi) * (1.0f + lo) : 0.0f;
@@ -152,12 +187,18 @@ struct ScanGatesFetch {
 
 template <class E, int KP>
 struct ScanLds {
-    uint16_t q[kPlanes<E>][kChunk][KP + 8];
+    union {
+        uint16_t q[kPlanes<E>][kChunk][KP + 8];
+        Triangle<3> p;  // once the queries have been used
+    };
     uint16_t k[kPlanes<E>][kChunk][KP + 8];
     uint16_t v[kPlanes<E>][kChunk][kColumns + 8];
-    Triangle<3> p;
     ScanGates gates;
-    float dots[2][4][kChunk];
+};
+
+template <class E, int KP>
+struct ScanGradientsLds : ScanLds<E, KP> {
+    float dots[2][4][2][kChunk];
 };
 
 // Rows of a chunk on their way to LDS: kCols columns from `column` on, 256 threads.
@@ -171,10 +212,22 @@ struct RowsFetch {
         const E* base = static_cast<const E*>(from.p) + env * from.stride[0] + low * from.stride[1] + head / from.share * from.stride[2];
         const Buffer rows = buffer_of(base, (tokens - 1) * row_bytes + width * sizeof(E));
         const int c = column + threadIdx.x % kAcross * 8;
+        if (from.wide) {
+            // Rows past the last are beyond the buffer's end in either order (backwards their offsets wrap
+            // around to 2^31 and more).
+            const int t = threadIdx.x / kAcross;
+            const uint32_t lane = (c < width ? c * static_cast<uint32_t>(sizeof(E)) : kOutside) + (reverse ? tokens - 1 - t : t) * row_bytes;
+            const uint32_t step = (reverse ? -kDown : kDown) * row_bytes;
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i) {
-            const int t = threadIdx.x / kAcross + i * kDown, row = reverse ? tokens - 1 - t : t;
-            part[i].load(rows, row * row_bytes + c * sizeof(E), t < tokens ? width - c : 0, from.wide);
+            for (int i = 0; i < kPieces; ++i)
+#pragma unroll
+                for (int w = 0; w < Part<E, 8>::kWords; ++w) part[i].words[w] = buffer_load16(rows, lane + i * step + 16 * w);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) {
+                const int t = threadIdx.x / kAcross + i * kDown, row = reverse ? tokens - 1 - t : t;
+                part[i].load(rows, row * row_bytes + c * sizeof(E), t < tokens ? width - c : 0, false);
+            }
         }
     }
 
@@ -225,37 +278,51 @@ __device__ inline f4 four_of(const uint16_t (&rows)[N][kChunk][kPitch], int row,
     return x;
 }
 
-// P without its diagonal into LDS, the diagonal of q k^T beside it.
-template <class E, int KP>
-__device__ inline void make_triangle(ScanLds<E, KP>& lds, bool reverse, float sign, int wave) {
-    constexpr int N = kPlanes<E>, kEach = (kTiles + 3) / 4;
-    const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+// The tiles of a triangle that a wave computes: its own on the diagonal, and of those below one or two
+// (i and j, two bits each, for n = 1 and 2; 3 for none).
+__device__ inline int tile_of_wave(int wave, int n) {
+    constexpr uint32_t kBelow = 0x84u | 0xc9u << 8 | 0x3du << 16 | 0x3eu << 24;
+    return n == 0 ? 5 * wave : kBelow >> (8 * wave + 4 * (n - 1)) & 15;
+}
+
+// D of a tile (beta_j D_ij forwards), for the lane's column and four rows; zeros on the diagonal and above.
+__device__ inline f4 decays(const ScanGates& gates, int i, int j, bool reverse) {
+    const int lane = threadIdx.x & 63, g = lane >> 4, column = 16 * j + (lane & 15), row = 16 * i + 4 * g;
+    if (i != j) return *reinterpret_cast<const f4*>(&gates.down[row]) * gates.across[i - 1][column];
+    const float hi = gates.hi[column], lo = gates.lo[column], beta = reverse ? 1.0f : gates.beta[column];
+    const int episode = gates.episode[column];
+    const f4 row_hi = *reinterpret_cast<const f4*>(&gates.hi[row]), row_lo = *reinterpret_cast<const f4*>(&gates.lo[row]);
+    using i4 = int32_t __attribute__((ext_vector_type(4)));
+    const i4 row_episode = *reinterpret_cast<const i4*>(&gates.episode[row]);
+    f4 x;
 #pragma unroll
-    for (int n = 0; n < kEach; ++n) {
-        const int tile = wave + 4 * n < kTiles ? wave + 4 * n : kTiles - 1;
-        const int i = tile_row(tile), j = tile - tile_of(i, 0);
-        f4 qk = {0, 0, 0, 0};
-#pragma unroll
-        for (int m = 0; m < KP / 32; ++m) {
-            u4 qi[N], kj[N];
-            operand_rows(lane, lds.q, 16 * i, m, qi);
-            operand_rows(lane, lds.k, 16 * j, m, kj);
-            qk = mma(qi, kj, qk);
-        }
-        const int column = 16 * j + col;
-        const float hi = lds.gates.hi[column], lo = lds.gates.lo[column], beta = reverse ? 1.0f : lds.gates.beta[column];
-        const int episode = lds.gates.episode[column];
-        f4 p;
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            const int row = 16 * i + 4 * g + s;
-            const float d = (lds.gates.hi[row] - hi) + (lds.gates.lo[row] - lo);
-            const bool inside = row > column && lds.gates.episode[row] == episode;
-            p[s] = inside ? __builtin_amdgcn_exp2f(d * kLog2E) * beta * qk[s] : 0.0f;
-            if (row == column) lds.gates.diagonal[row] = sign * qk[s];
-        }
-        store_slot<3>(lds.p, tile, lane, p);
+    for (int s = 0; s < 4; ++s) {
+        const float d = (row_hi[s] - hi) + (row_lo[s] - lo);
+        x[s] = row + s > column && row_episode[s] == episode ? __builtin_amdgcn_exp2f(d * kLog2E) * beta : 0.0f;
     }
+    return x;
+}
+
+// Rows i of q times rows j of k.
+template <int N, int kPitch>
+__device__ inline f4 tile_product(const uint16_t (&q)[N][kChunk][kPitch], const uint16_t (&k)[N][kChunk][kPitch], int i, int j) {
+    const int lane = threadIdx.x & 63;
+    f4 x = {0, 0, 0, 0};
+#pragma unroll
+    for (int m = 0; m < kPitch / 32; ++m) {
+        u4 qi[N], kj[N];
+        operand_rows(lane, q, 16 * i, m, qi);
+        operand_rows(lane, k, 16 * j, m, kj);
+        x = mma(qi, kj, x);
+    }
+    return x;
+}
+
+// The lane's number of a tile's diagonal, if it has one.
+template <class F>
+__device__ inline void diagonal_of(f4 x, F to) {
+    const int lane = threadIdx.x & 63, s = (lane & 15) - 4 * (lane >> 4);
+    if (s >= 0 && s < 4) to(lane & 15, s == 0 ? x[0] : s == 1 ? x[1] : s == 2 ? x[2] : x[3]);
 }
 
 template <int KP>
@@ -282,26 +349,73 @@ __device__ inline void store_state(const Role& R, float* to, int64_t row, int64_
         }
 }
 
-// A workgroup walks the chunks of a segment with 64 columns of a head's state in registers, 16 a
-// wave. kSummary: what a segment makes of zeros, and what it multiplies a state before it with.
-template <class E, int KP, bool kSummary>
-__global__ __launch_bounds__(256, 2) void selective_scan_kernel(ScanParams P) {
+// Results alone; with what the gradients of the gates need; what a segment makes of zeros, and what it
+// multiplies a state before it with.
+enum { kResults, kGradients, kSegments };
+
+// Four numbers of a row each of the lane's tokens (l % 16 of each tile), its columns of the wave's 16.
+template <class E>
+struct FourFetch {
+    using Words = std::conditional_t<sizeof(E) == 4, u4, u2>;
+    Words words[4];
+
+    __device__ void fetch(const Operand& from, int64_t env, int head, int64_t low, int tokens, bool reverse, int first, int width) {
+        const int lane = threadIdx.x & 63, t = lane & 15, c = first + 4 * (lane >> 4);
+        const uint32_t row_bytes = static_cast<uint32_t>(from.stride[1]) * sizeof(E);
+        const E* base = static_cast<const E*>(from.p) + env * from.stride[0] + low * from.stride[1] + head / from.share * from.stride[2];
+        const Buffer rows = buffer_of(base, (tokens - 1) * row_bytes + width * sizeof(E));
+        const uint32_t at = (c < width ? c * static_cast<uint32_t>(sizeof(E)) : kOutside) + (reverse ? tokens - 1 - t : t) * row_bytes;
+        const uint32_t step = (reverse ? -16 : 16) * row_bytes;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (from.wide) {
+                if constexpr (sizeof(E) == 4)
+                    words[i] = buffer_load16(rows, at + i * step);
+                else
+                    words[i] = __builtin_bit_cast(u2, __builtin_amdgcn_raw_buffer_load_b64(rows, at + i * step, 0, 0));
+            } else {
+                E x[4];
+#pragma unroll
+                for (int s = 0; s < 4; ++s) x[s] = buffer_load<E>(rows, c + s < width ? at + i * step + s * static_cast<uint32_t>(sizeof(E)) : kOutside);
+                words[i] = __builtin_bit_cast(Words, x);
+            }
+        }
+    }
+
+    __device__ f4 floats(int i) const {
+        if constexpr (sizeof(E) == 4) {
+            return __builtin_bit_cast(f4, words[i]);
+        } else {
+            f4 x;
+#pragma unroll
+            for (int s = 0; s < 4; ++s) x[s] = to_float(__builtin_bit_cast(E, static_cast<uint16_t>(words[i][s / 2] >> (16 * (s % 2)))));
+            return x;
+        }
+    }
+};
+
+// A workgroup walks the chunks of a segment with 64 columns of a head's state in registers, 16 a wave.
+template <class E, int KP, int kMode>
+__global__ __launch_bounds__(256, (kPlanes<E> == 1 && KP == 64 ? 3 : 2)) void selective_scan_kernel(ScanParams P) {
+    constexpr bool kSummary = kMode == kSegments, kGates = kMode == kGradients;
     constexpr int N = kPlanes<E>;
     extern __shared__ char lds_bytes[];
-    auto& lds = *reinterpret_cast<ScanLds<E, KP>*>(lds_bytes);
+    auto& lds = *reinterpret_cast<std::conditional_t<kGates, ScanGradientsLds<E, KP>, ScanLds<E, KP>>*>(lds_bytes);
     const Role& R = P.role[blockIdx.y];
-    const int wave = wave_of_workgroup(), lane = threadIdx.x & 63, g = lane >> 4, segment = blockIdx.z;
-    // Workgroups go round the 8 XCDs in turn: those of one env and group, which read the same
-    // rows, are 8 apart.
-    const uint32_t inner = P.group * R.blocks, round = blockIdx.x / 8;
-    const int64_t outer = static_cast<int64_t>(round / inner) * 8 + blockIdx.x % 8;
-    const int64_t groups = P.heads / P.group;
-    if (outer >= P.envs * groups) return;
-    const int64_t env = outer / groups;
+    const int wave = wave_of_workgroup(), lane = threadIdx.x & 63, g = lane >> 4;
+    // Workgroups go round the 8 XCDs in turn: those of one env, group and segment, which read the same
+    // rows, are 8 apart (or one after the other where there are fewer than 8 such).
+    const uint32_t inner = P.group * R.blocks, segments = kSummary ? P.n_segments - 1 : P.n_segments;
+    const int64_t groups = P.heads / P.group, units = P.envs * groups * segments;
+    const uint32_t round = units < 8 ? blockIdx.x : blockIdx.x / 8;
+    const int64_t unit = units < 8 ? round / inner : static_cast<int64_t>(round / inner) * 8 + blockIdx.x % 8;
+    if (unit >= units) return;
+    const int segment = static_cast<int>(unit % segments);
+    const int64_t outer = unit / segments, env = outer / groups;
     const int head = static_cast<int>(outer % groups) * P.group + static_cast<int>(round % inner) / R.blocks;
     const int block = static_cast<int>(round % inner) % R.blocks, first = block * kColumns + 16 * wave;
     const int64_t sequence = env * P.heads + head, kv = static_cast<int64_t>(R.K) * R.V;
-    const bool reverse = R.reverse, working = first < R.V;
+    const bool reverse = kMode != kResults && R.reverse, working = first < R.V;
     const int begin = static_cast<int>(static_cast<int64_t>(segment) * P.n_chunks / P.n_segments);
     const int end = static_cast<int>((segment + 1ll) * P.n_chunks / P.n_segments);
 
@@ -355,136 +469,141 @@ __global__ __launch_bounds__(256, 2) void selective_scan_kernel(ScanParams P) {
         if (chunk + 1 < end) fetch(chunk + 1);
         const float keep = lds.gates.e[kChunk - 1];
         total = keep == 0.0f ? 0.0f : total * keep;
-        if constexpr (!kSummary) {
-            make_triangle<E, KP>(lds, reverse, sign, wave);
-            __syncthreads();
-        }
-        // z . o of a lane's tokens, the wave's columns
-        const auto dots = [&](const f4 (&o)[4], float (&to)[kChunk]) {
-            const int column = first + 4 * g;
-            const E* z = static_cast<const E*>(R.z.p) + env * R.z.stride[0] + low * R.z.stride[1] + head / R.z.share * R.z.stride[2];
+        FourFetch<E> z;
+        if (kGates && R.state_dots) z.fetch(R.z, env, head, low, tokens, reverse, first, working ? R.V : 0);
+        // z . o of the lane's tokens and columns
+        const auto dots = [&](const f4 (&o)[4], float (&to)[2][kChunk]) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int t = 16 * i + (lane & 15), row = reverse ? tokens - 1 - t : t;
-                float dot = 0.0f;
-                if (t < tokens) {
-#pragma unroll
-                    for (int s = 0; s < 4; ++s)
-                        if (column + s < R.V) dot += o[i][s] * to_float(z[row * R.z.stride[1] + column + s]);
-                }
-                dot += __shfl_xor(dot, 16);
-                dot += __shfl_xor(dot, 32);
-                if (g == 0) to[t] = sign * dot;
+                const f4 x = z.floats(i) * o[i];
+                float sum = sign * ((x[0] + x[1]) + (x[2] + x[3]));
+                sum += __shfl_xor(sum, 32);
+                if (g < 2) to[g][16 * i + (lane & 15)] = sum;
             }
         };
-        f4 o[4];
+        f4 o[4], p[3];
         const int64_t slot = ((sequence * P.n_chunks + place) * R.blocks + block) * 4 + wave;
-        if (!kSummary && R.through && !working && lane == 0) R.through[slot] = 0.0f;
-        if (working) {
-            if constexpr (!kSummary) {
-                if (R.keep_states && place >= R.keep_from && place < R.keep_to) {
-                    f4* to = reinterpret_cast<f4*>(R.keep_states) + slot * (KP / 16) * 64 + lane;
+        if (kGates && R.through && !working && lane == 0) R.through[slot] = 0.0f;
+        if constexpr (kGates) {
+            if (working && R.keep_states && place >= R.keep_from && place < R.keep_to) {
+                f4* to = reinterpret_cast<f4*>(R.keep_states) + slot * (KP / 16) * 64 + lane;
 #pragma unroll
-                    for (int i = 0; i < KP / 16; ++i) to[i * 64] = state[i];
-                }
-                if (R.through) {
-                    float dot = 0.0f;
-                    if (place >= R.keep_from && place < R.keep_to) {
-                        const f4* from = reinterpret_cast<const f4*>(R.other_states) + slot * (KP / 16) * 64 + lane;
-#pragma unroll
-                        for (int i = 0; i < KP / 16; ++i) {
-                            const f4 x = state[i] * from[i * 64];
-                            dot += (x[0] + x[1]) + (x[2] + x[3]);
-                        }
-#pragma unroll
-                        for (int d = 1; d < 64; d *= 2) dot += __shfl_xor(dot, d);
-                    }
-                    // (what is held backwards has not passed the decay before the chunk's first place)
-                    if (lane == 0) R.through[slot] = lds.gates.e[0] == 0.0f ? 0.0f : lds.gates.e[0] * dot;
-                }
+                for (int i = 0; i < KP / 16; ++i) to[i * 64] = state[i];
             }
-            u4 value[2][N];
+            if (working && R.through) {
+                float dot = 0.0f;
+                if (place >= R.keep_from && place < R.keep_to) {
+                    const f4* from = reinterpret_cast<const f4*>(R.other_states) + slot * (KP / 16) * 64 + lane;
+#pragma unroll
+                    for (int i = 0; i < KP / 16; ++i) {
+                        const f4 x = state[i] * from[i * 64];
+                        dot += (x[0] + x[1]) + (x[2] + x[3]);
+                    }
+#pragma unroll
+                    for (int d = 1; d < 64; d *= 2) dot += __shfl_xor(dot, d);
+                }
+                // (what is held backwards has not passed the decay before the chunk's first place)
+                if (lane == 0) R.through[slot] = lds.gates.e[0] == 0.0f ? 0.0f : lds.gates.e[0] * dot;
+            }
+        }
+        if constexpr (!kSummary) {
+#pragma unroll
+            for (int n = 0; n < 3; ++n) {
+                const int tile = tile_of_wave(wave, n), i = tile >> 2, j = tile & 3;
+                if (tile == 3) continue;
+                p[n] = tile_product(lds.q, lds.k, i, j);
+                if (n == 0) diagonal_of(p[0], [&](int t, float x) { lds.gates.diagonal[16 * i + t] = sign * x; });
+                p[n] *= decays(lds.gates, i, j, reverse);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = f4{0, 0, 0, 0};
+            // (a state that the chunk's first token forgets may hold anything)
+            if (lds.gates.e[0] == 0.0f)
+#pragma unroll
+                for (int i = 0; i < KP / 16; ++i) state[i] = f4{0, 0, 0, 0};
+            if (working && !empty && lds.gates.e[0] != 0.0f) {
+#pragma unroll
+                for (int m = 0; m < KP / 32; ++m) {
+                    u4 b[3];
+                    split8(state[2 * m], state[2 * m + 1], b);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        u4 a[N];
+                        operand_rows(lane, lds.q, 16 * i, m, a);
+                        o[i] = mma(b, a, o[i]);  // (transposed: the operands hold rows and columns alike)
+                    }
+                    }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[i] = lds.gates.e[16 * i + (lane & 15)] * o[i];
+            }
+            if constexpr (kGates) {
+                if (R.state_dots && working) dots(o, lds.dots[0][wave]);
+            }
+            __syncthreads();
+#pragma unroll
+            for (int n = 0; n < 3; ++n) {
+                const int tile = tile_of_wave(wave, n);
+                if (tile != 3) store_slot<3>(lds.p, tile_of(tile >> 2, tile & 3), lane, p[n]);
+            }
+        }
+        u4 value[2][N];
+        if (working) {
 #pragma unroll
             for (int m = 0; m < 2; ++m) operand_columns(lane, lds.v, wave, m, value[m]);
-            if constexpr (!kSummary) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) o[i] = f4{0, 0, 0, 0};
-                // (a state that the chunk's first token forgets may hold anything)
-                if (lds.gates.e[0] == 0.0f)
+            for (int i = 0; i < KP / 16; ++i)
 #pragma unroll
-                    for (int i = 0; i < KP / 16; ++i) state[i] = f4{0, 0, 0, 0};
-                if (!empty && lds.gates.e[0] != 0.0f) {
-#pragma unroll
-                    for (int m = 0; m < KP / 32; ++m) {
-                        u4 b[3], a[4][N];
-                        split8(state[2 * m], state[2 * m + 1], b);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) operand_rows(lane, lds.q, 16 * i, m, a[i]);
-                        mma_each_transposed<4>(a, b, o);
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) o[i] = lds.gates.e[16 * i + (lane & 15)] * o[i];
-                }
-                if (R.state_dots) dots(o, lds.dots[0][wave]);
-            }
-            // The state first: the next chunk waits for it.
-            u4 r[2][3];
+                for (int s = 0; s < 4; ++s) state[i][s] = keep == 0.0f ? 0.0f : keep * state[i][s];
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
+                u4 r[3];
                 float x[8];
                 join8(value[m], x);
                 const f4 f0 = *reinterpret_cast<const f4*>(&lds.gates.f[32 * m + 4 * g]);
                 const f4 f1 = *reinterpret_cast<const f4*>(&lds.gates.f[32 * m + 16 + 4 * g]);
-                split8(f0 * f4{x[0], x[1], x[2], x[3]}, f1 * f4{x[4], x[5], x[6], x[7]}, r[m]);
-            }
+                split8(f0 * f4{x[0], x[1], x[2], x[3]}, f1 * f4{x[4], x[5], x[6], x[7]}, r);
 #pragma unroll
-            for (int i = 0; i < KP / 16; ++i) {
-#pragma unroll
-                for (int s = 0; s < 4; ++s) state[i][s] = keep == 0.0f ? 0.0f : keep * state[i][s];
-            }
-#pragma unroll
-            for (int i = 0; i < KP / 16; i += 4) {
-                f4 x[4] = {state[i], state[i + 1], state[i + 2], state[i + 3]};
-#pragma unroll
-                for (int m = 0; m < 2; ++m) {
-                    u4 a[4][N];
-#pragma unroll
-                    for (int n = 0; n < 4; ++n) operand_columns(lane, lds.k, i + n, m, a[n]);
-                    mma_each<4>(a, r[m], x);
+                for (int i = 0; i < KP / 16; ++i) {
+                    u4 a[N];
+                    operand_columns(lane, lds.k, i, m, a);
+                    state[i] = mma(a, r, state[i]);
                 }
-#pragma unroll
-                for (int n = 0; n < 4; ++n) state[i + n] = x[n];
             }
             empty = false;
-            if constexpr (!kSummary) {
-                u4 a[4][3];
+        }
+        if constexpr (!kSummary) {
+            __syncthreads();
+            if (working) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) operand_triangle<3>(lane, lds.p, i, 0, a[i]);
-                mma_each_transposed<4>(a, value[0], o);
-                u4 below[2][3];
-                f4 y[2] = {o[2], o[3]};
-#pragma unroll
-                for (int i = 0; i < 2; ++i) operand_triangle<3>(lane, lds.p, 2 + i, 1, below[i]);
-                mma_each_transposed<2>(below, value[1], y);
-                o[2] = y[0];
-                o[3] = y[1];
+                for (int i = 0; i < 4; ++i) {
+                    u4 a[3];
+                    operand_triangle<3>(lane, lds.p, i, 0, a);
+                    o[i] = mma(value[0], a, o[i]);
+                    if (i >= 2) {
+                        operand_triangle<3>(lane, lds.p, i, 1, a);
+                        o[i] = mma(value[1], a, o[i]);
+                    }
+                    }
             }
         }
         if constexpr (kSummary) continue;
-        if (R.state_dots) {
+        if constexpr (kGates) if (R.state_dots) {
             if (working) {
                 if (R.dots) dots(o, lds.dots[1][wave]);
-            } else if (lane < 16) {
+            } else {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) lds.dots[0][wave][16 * i + lane] = lds.dots[1][wave][16 * i + lane] = 0.0f;
+                for (int i = 0; i < 2; ++i) lds.dots[0][wave][i][lane] = lds.dots[1][wave][i][lane] = 0.0f;
             }
             __syncthreads();
-            if (wave < 2 && lane < tokens) {
-                float* to = wave == 0 ? R.state_dots : R.dots;
-                const auto& from = lds.dots[wave];
-                if (to)
-                    to[(sequence * R.blocks + block) * P.steps + low + (reverse ? tokens - 1 - lane : lane)] =
-                        (from[0][lane] + from[1][lane]) + (from[2][lane] + from[3][lane]);
+            float* to = wave == 0 ? R.state_dots : R.dots;
+            if (wave < 2 && lane < tokens && to) {
+                float sum = 0.0f;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const auto& from = lds.dots[wave][w];
+                    sum += from[0][lane] + from[1][lane];
+                }
+                to[(sequence * R.blocks + block) * P.steps + low + (reverse ? tokens - 1 - lane : lane)] = sum;
             }
         }
         if (!working) continue;
@@ -496,22 +615,26 @@ __global__ __launch_bounds__(256, 2) void selective_scan_kernel(ScanParams P) {
             using T = std::remove_reference_t<decltype(*base)>;
             const uint32_t row_bytes = static_cast<uint32_t>(P.heads) * R.V * sizeof(T);
             const Buffer to = buffer_of(base + row0 * R.V + first, (tokens - 1) * row_bytes + width * sizeof(T));
+            // (rows past the last: as in RowsFetch)
+            const uint32_t own = (column < width ? column * static_cast<uint32_t>(sizeof(T)) : kOutside) +
+                                 (reverse ? tokens - 1 - (lane & 15) : lane & 15) * row_bytes;
+            const uint32_t step = (reverse ? -16 : 16) * row_bytes;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int t = 16 * i + (lane & 15), row = reverse ? tokens - 1 - t : t;
+                const int t = 16 * i + (lane & 15);
                 const float beta = lds.gates.beta[t];
                 const f4 x = (reverse ? sign * beta : sign) * o[i] + (beta * lds.gates.diagonal[t] + skip) * four_of(lds.v, t, wave, g);
-                const uint32_t offset = t < tokens ? row * row_bytes + column * sizeof(T) : kOutside;
+                const uint32_t offset = own + i * step;
                 const T y[4] = {from_float<T>(x[0]), from_float<T>(x[1]), from_float<T>(x[2]), from_float<T>(x[3])};
                 if (R.wide_out) {
-                    buffer_store_four(to, column < width ? offset : kOutside, y);
+                    buffer_store_four(to, offset, y);
                 } else {
 #pragma unroll
                     for (int s = 0; s < 4; ++s) buffer_store<T>(to, column + s < width ? offset + s * sizeof(T) : kOutside, y[s]);
                 }
             }
         };
-        if (R.out_heads)
+        if (kGates && R.out_heads)
             store(R.out_heads);
         else
             store(static_cast<E*>(R.out));
@@ -578,25 +701,6 @@ struct GateLds {
     float bc[kChunk], dyx[kChunk], pairs[kChunk];
 };
 
-template <class E, int KP>
-__device__ inline void tiles_of(const GateLds<E, KP>& lds, int wave, f4 (&x)[3]) {
-    constexpr int N = kPlanes<E>;
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int n = 0; n < 3; ++n) {
-        const int tile = wave + 4 * n < kTiles ? wave + 4 * n : kTiles - 1;
-        const int i = tile_row(tile), j = tile - tile_of(i, 0);
-        x[n] = f4{0, 0, 0, 0};
-#pragma unroll
-        for (int m = 0; m < KP / 32; ++m) {
-            u4 qi[N], kj[N];
-            operand_rows(lane, lds.q, 16 * i, m, qi);
-            operand_rows(lane, lds.k, 16 * j, m, kj);
-            x[n] = mma(qi, kj, x[n]);
-        }
-    }
-}
-
 // dg of a chunk's tokens and what follows from it, a workgroup a chunk of a head: both triangles of
 // products, W, its sums (a product with the triangle of ones: sum over j < t, then over rows i >= t),
 // and a token a lane.
@@ -624,29 +728,26 @@ __global__ __launch_bounds__(256, 2) void selective_gates_kernel(GateParams P) {
     c.put(lds.q);
     b.put(lds.k, sign < 0.0f ? 0x80008000u : 0u);
     __syncthreads();
-    f4 bc[3], dyx[3];
-    tiles_of(lds, wave, bc);
+    f4 bc[3];
+#pragma unroll
+    for (int n = 0; n < 3; ++n) {
+        const int tile = tile_of_wave(wave, n);
+        if (tile != 3) bc[n] = tile_product(lds.q, lds.k, tile >> 2, tile & 3);
+    }
     __syncthreads();
     dy.put(lds.q);
     x.put(lds.k, sign < 0.0f ? 0x80008000u : 0u);
     __syncthreads();
-    tiles_of(lds, wave, dyx);
 #pragma unroll
     for (int n = 0; n < 3; ++n) {
-        const int tile = wave + 4 * n < kTiles ? wave + 4 * n : kTiles - 1;
-        const int i = tile_row(tile), j = tile - tile_of(i, 0), column = 16 * j + col;
-        const float hi = lds.gates.hi[column], lo = lds.gates.lo[column], beta = lds.gates.beta[column];
-        const int episode = lds.gates.episode[column];
-        f4 w;
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            const int row = 16 * i + 4 * g + s;
-            const float d = (lds.gates.hi[row] - hi) + (lds.gates.lo[row] - lo);
-            const bool inside = row > column && lds.gates.episode[row] == episode;
-            w[s] = inside ? __builtin_amdgcn_exp2f(d * kLog2E) * beta * bc[n][s] * (sign * dyx[n][s]) : 0.0f;  // (of either sign as well)
-            if (row == column) lds.bc[row] = sign * bc[n][s], lds.dyx[row] = sign * dyx[n][s];
+        const int tile = tile_of_wave(wave, n), i = tile >> 2, j = tile & 3;
+        if (tile == 3) continue;
+        const f4 dyx = sign * tile_product(lds.q, lds.k, i, j);
+        if (n == 0) {
+            diagonal_of(bc[0], [&](int t, float y) { lds.bc[16 * i + t] = sign * y; });
+            diagonal_of(dyx, [&](int t, float y) { lds.dyx[16 * i + t] = y; });
         }
-        store_slot<3>(lds.w, tile, lane, w);
+        store_slot<3>(lds.w, tile_of(i, j), lane, decays(lds.gates, i, j, false) * bc[n] * dyx);  // (of either sign as well)
     }
     __syncthreads();
     {
@@ -904,35 +1005,36 @@ int launched(const char* name) {
     return NAVI_POLICY_OK;
 }
 
-template <class E, int KP, bool kSummary>
+template <class E, int KP, int kMode>
 int launch_scan(const ScanParams& P, int roles, int segments, hipStream_t stream) {
-    constexpr int lds = sizeof(ScanLds<E, KP>);
+    constexpr int lds = kMode == kGradients ? sizeof(ScanGradientsLds<E, KP>) : sizeof(ScanLds<E, KP>);
     static_assert(lds <= 160 * 1024, "a CU's LDS");
-    const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void*>(selective_scan_kernel<E, KP, kSummary>),
+    const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void*>(selective_scan_kernel<E, KP, kMode>),
                                                hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (err != hipSuccess) return set_error(NAVI_POLICY_E_LAUNCH, "navi_selective_scan: %s", hipGetErrorString(err));
     int blocks = 0;
     for (int i = 0; i < roles; ++i) blocks = std::max(blocks, P.role[i].blocks);
-    const int64_t outer = P.envs * (P.heads / P.group), inner = static_cast<int64_t>(P.group) * blocks;
-    hipLaunchKernelGGL((selective_scan_kernel<E, KP, kSummary>), dim3(static_cast<unsigned>((outer + 7) / 8 * 8 * inner), roles, segments),
-                       dim3(256), lds, stream, P);
+    const int64_t units = P.envs * (P.heads / P.group) * segments, inner = static_cast<int64_t>(P.group) * blocks;
+    const int64_t grid = (units < 8 ? units : (units + 7) / 8 * 8) * inner;
+    if (grid > INT32_MAX) return set_error(NAVI_POLICY_E_ARG, "navi_selective_scan: too many envs, heads and segments");
+    hipLaunchKernelGGL((selective_scan_kernel<E, KP, kMode>), dim3(static_cast<unsigned>(grid), roles), dim3(256), lds, stream, P);
     return launched("navi_selective_scan");
 }
 
 // All roles of P (of one KP) over all segments.
 template <class E, int KP>
-int scan(const ScanParams& P, int roles, hipStream_t stream) {
+int scan(const ScanParams& P, int roles, bool back, hipStream_t stream) {
     if (P.n_segments > 1) {
-        const int code = launch_scan<E, KP, true>(P, roles, P.n_segments - 1, stream);
+        const int code = launch_scan<E, KP, kSegments>(P, roles, P.n_segments - 1, stream);
         if (code != NAVI_POLICY_OK) return code;
         const int64_t numbers = P.envs * P.heads * P.role[0].K * P.role[0].V;
         hipLaunchKernelGGL(selective_join_kernel, dim3(static_cast<unsigned>((numbers + 255) / 256), roles), dim3(256), 0, stream, P);
     }
-    return launch_scan<E, KP, false>(P, roles, P.n_segments, stream);
+    return back ? launch_scan<E, KP, kGradients>(P, roles, P.n_segments, stream) : launch_scan<E, KP, kResults>(P, roles, P.n_segments, stream);
 }
 
 template <class E>
-int scans(const ScanParams& P, int roles, hipStream_t stream) {
+int scans(const ScanParams& P, int roles, bool back, hipStream_t stream) {
     // those of one KP together
     ScanParams few = P, many = P;
     int n_few = 0, n_many = 0;
@@ -943,10 +1045,10 @@ int scans(const ScanParams& P, int roles, hipStream_t stream) {
             many.role[n_many++] = P.role[i];
     }
     if (n_few > 0) {
-        const int code = scan<E, 64>(few, n_few, stream);
+        const int code = scan<E, 64>(few, n_few, back, stream);
         if (code != NAVI_POLICY_OK) return code;
     }
-    return n_many > 0 ? scan<E, 128>(many, n_many, stream) : NAVI_POLICY_OK;
+    return n_many > 0 ? scan<E, 128>(many, n_many, back, stream) : NAVI_POLICY_OK;
 }
 
 template <class E, int KP>
@@ -966,10 +1068,10 @@ int gates(const GateParams& P, hipStream_t stream) {
     return std::max(P.state_dim, P.head_dim) <= 64 ? launch_gates<E, 64>(P, stream) : launch_gates<E, 128>(P, stream);
 }
 
-int scans_typed(const ScanParams& P, int32_t dtype, int roles, hipStream_t stream) {
-    if (dtype == NAVI_POLICY_F32) return scans<float>(P, roles, stream);
-    if (dtype == NAVI_POLICY_BF16) return scans<bf16>(P, roles, stream);
-    return scans<f16>(P, roles, stream);
+int scans_typed(const ScanParams& P, int32_t dtype, int roles, bool back, hipStream_t stream) {
+    if (dtype == NAVI_POLICY_F32) return scans<float>(P, roles, back, stream);
+    if (dtype == NAVI_POLICY_BF16) return scans<bf16>(P, roles, back, stream);
+    return scans<f16>(P, roles, back, stream);
 }
 
 float* place_segments(Role& r, const navi_selective_scan_args& a, int32_t segments, float* at) {
@@ -1059,7 +1161,7 @@ extern "C" int navi_selective_scan(const navi_selective_scan_args* args, void* s
     r.from = args->initial_state;
     r.to = args->final_state;
     place_segments(r, *args, s.P.n_segments, static_cast<float*>(args->scratch));
-    return scans_typed(s.P, args->dtype, 1, as_stream(stream));
+    return scans_typed(s.P, args->dtype, 1, false, as_stream(stream));
 }
 
 extern "C" int64_t navi_selective_scan_scratch(const navi_selective_scan_args* args) {
@@ -1120,11 +1222,11 @@ extern "C" int navi_selective_scan_backward(const navi_selective_scan_args* args
     GateParams G{};
     G.scan = P;
     // (the db scan reads what the dc scan leaves)
-    int result = scans_typed(P, a.dtype, needed ? 2 : 3, as_stream(stream));
+    int result = scans_typed(P, a.dtype, needed ? 2 : 3, true, as_stream(stream));
     if (result != NAVI_POLICY_OK) return result;
     if (needed) {
         P.role[0] = db;
-        result = scans_typed(P, a.dtype, 1, as_stream(stream));
+        result = scans_typed(P, a.dtype, 1, true, as_stream(stream));
         if (result != NAVI_POLICY_OK) return result;
     }
     G.x = s.x;
