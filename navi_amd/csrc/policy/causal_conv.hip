@@ -11,36 +11,60 @@
 // zero, an infinity of another episode is not seen.
 #include <algorithm>
 #include <climits>
+#include <cstdlib>
+#include <type_traits>
 
 #include "policy_common.hpp"
 
 namespace navi_policy {
 namespace {
 
-constexpr int kBatch = 8;          // rows asked for at once
+constexpr int kBatch = 8, kBackBatch = 4;  // rows asked for at once
 constexpr int kMaxTaps = NAVI_POLICY_MAX_TAPS;
 constexpr int kPartialBlocks = NAVI_POLICY_CONV_PARTIALS;  // most workgroups' worth of sums a channel has
 
 struct ConvParams {
     navi_causal_conv_args a;
+    int32_t across, rows;    // of a workgroup: pieces of a row, and segments at once
     int32_t groups;          // pieces of a row
-    int32_t across, rows;    // of a workgroup: pieces, and segments at once
     int32_t across_blocks;   // workgroups that a row takes
     int32_t down_blocks;     // workgroups down the segments
     int32_t segment;         // tokens
-    int64_t segments;        // of an env
+    uint32_t items, segments;  // segments, of all envs and of one
+    Divisor by_segments, by_across, by_across_blocks;
 };
 
 // Pieces of rows as they lie in memory.
 template <class E, int kVec>
 struct Piece {
-    u4 words;
-    __device__ void load(const E* from) { words = *reinterpret_cast<const u4*>(from); }
-    __device__ void store(E* to) const { *reinterpret_cast<u4*>(to) = words; }
-    __device__ void clear() { words = u4{0, 0, 0, 0}; }
+    static constexpr int kBytes = kVec * sizeof(E);
+    using Words = std::conditional_t<kBytes == 16, u4, std::conditional_t<kBytes == 8, u2, std::conditional_t<kBytes == 4, uint32_t, uint16_t>>>;
+    Words words;
+
+    __device__ void load(Buffer from, uint32_t offset) {
+        if constexpr (kBytes == 16)
+            words = buffer_load16(from, offset);
+        else if constexpr (kBytes == 8)
+            words = __builtin_bit_cast(u2, __builtin_amdgcn_raw_buffer_load_b64(from, offset, 0, 0));
+        else if constexpr (kBytes == 4)
+            words = __builtin_amdgcn_raw_buffer_load_b32(from, offset, 0, 0);
+        else
+            words = __builtin_amdgcn_raw_buffer_load_b16(from, offset, 0, 0);
+    }
+    __device__ void store(Buffer to, uint32_t offset) const {
+        if constexpr (kBytes == 16)
+            __builtin_amdgcn_raw_buffer_store_b128(words, to, offset, 0, 0);
+        else if constexpr (kBytes == 8)
+            __builtin_amdgcn_raw_buffer_store_b64(words, to, offset, 0, 0);
+        else if constexpr (kBytes == 4)
+            __builtin_amdgcn_raw_buffer_store_b32(words, to, offset, 0, 0);
+        else
+            __builtin_amdgcn_raw_buffer_store_b16(words, to, offset, 0, 0);
+    }
+    __device__ void clear() { words = Words{}; }
     __device__ void floats(float (&x)[kVec]) const {
         union {
-            u4 words;
+            Words words;
             E elements[kVec];
         } got{words};
 #pragma unroll
@@ -48,7 +72,7 @@ struct Piece {
     }
     __device__ void from(const float (&x)[kVec]) {
         union {
-            u4 words;
+            Words words;
             E elements[kVec];
         } put;
 #pragma unroll
@@ -57,61 +81,64 @@ struct Piece {
     }
 };
 
-template <class E>
-struct Piece<E, 1> {
-    E element;
-    __device__ void load(const E* from) { element = *from; }
-    __device__ void store(E* to) const { *to = element; }
-    __device__ void clear() { element = from_float<E>(0.0f); }
-    __device__ void floats(float (&x)[1]) const { x[0] = to_float(element); }
-    __device__ void from(const float (&x)[1]) { element = from_float<E>(x[0]); }
-};
-
 // 1 / (1 + e^-z): e^-z overflows to infinity for z below -88, and its reciprocal to 0.
 __device__ inline float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + __expf(-z)); }
 
-// Where a thread works: a piece of the channels, and segments from `item` on.
-struct Place {
-    int32_t channel;
-    int64_t item, step;
-    bool inside;
+// Rows [env][step][channels] of an array from an env on, and where a lane is in them: accesses by 32-bit
+// offsets, kOutside for what is not there, without branches.
+struct Lines {
+    Buffer buffer;
+    uint32_t lane, step;  // bytes: of the lane's env and channel, and from step to step
+
+    __device__ Lines(const void* base, int64_t stride0, int64_t stride1, uint32_t bytes, uint32_t env0, uint32_t env, int32_t channel) {
+        buffer = buffer_of(static_cast<const char*>(base) + env0 * stride0 * bytes, base ? 0x80000000u : 0u);
+        lane = static_cast<uint32_t>((env - env0) * stride0 + channel) * bytes;
+        step = static_cast<uint32_t>(stride1) * bytes;
+    }
+    __device__ uint32_t at(int32_t t, bool there) const { return there ? lane + static_cast<uint32_t>(t) * step : kOutside; }
 };
 
+// A thread's place: a piece of the channels, and segments from `item` on.
 template <int kVec>
-__device__ inline Place place_of(const ConvParams& P) {
-    const int32_t block = blockIdx.x % P.across_blocks, down = blockIdx.x / P.across_blocks;
-    const int32_t c = threadIdx.x % P.across, r = threadIdx.x / P.across;
-    const int32_t group = block * P.across + c;
-    return Place{group * kVec, static_cast<int64_t>(down) * P.rows + r, static_cast<int64_t>(P.down_blocks) * P.rows,
-                 r < P.rows && group < P.groups};
-}
+struct Place {
+    uint32_t first, row, step;  // the workgroup's first segment, the thread's among them, segments from turn to turn
+    int32_t channel, block, down;
+    bool inside;
+
+    __device__ explicit Place(const ConvParams& P) {
+        down = static_cast<int32_t>(divide(blockIdx.x, P.by_across_blocks));
+        block = static_cast<int32_t>(blockIdx.x) - down * P.across_blocks;
+        row = divide(threadIdx.x, P.by_across);
+        const int32_t group = block * P.across + static_cast<int32_t>(threadIdx.x - row * P.across);
+        channel = group * kVec;
+        first = down * P.rows;
+        step = P.down_blocks * P.rows;
+        inside = row < static_cast<uint32_t>(P.rows) && group < P.groups;
+    }
+};
 
 // The inputs before a segment's first token, in its episode: held[k] is that of k + 1 tokens before.
 template <class E, int kVec, int kTaps>
-__device__ inline void begin_segment(const ConvParams& P, int64_t env, int64_t t0, int32_t channel, Piece<E, kVec> (&held)[kTaps - 1]) {
-    const E* x = static_cast<const E*>(P.a.x) + env * P.a.x_stride[0] + channel;
-    const E* window = P.a.window ? static_cast<const E*>(P.a.window) + env * (kTaps - 1) * P.a.channels + channel : nullptr;
-    bool same = true;  // no token after the one k + 1 before has begun an episode
+__device__ inline void begin_segment(const Lines& x, const Lines& window, const Lines& starts, int32_t t0, bool inside, Piece<E, kVec> (&held)[kTaps - 1]) {
+    bool same = inside;  // no token after the one k + 1 before has begun an episode
 #pragma unroll
     for (int k = 0; k < kTaps - 1; ++k) {
-        held[k].clear();
-        const int64_t t = t0 - 1 - k;
-        if (k > 0 && t + 1 >= 0 && P.a.starts && P.a.starts[env * P.a.starts_stride[0] + (t + 1) * P.a.starts_stride[1]]) same = false;
-        if (!same) continue;
-        if (t >= 0)
-            held[k].load(x + t * P.a.x_stride[1]);
-        else if (window)
-            held[k].load(window + (kTaps - 1 + t) * P.a.channels);
+        const int32_t t = t0 - 1 - k;
+        if (k > 0) same = same && __builtin_amdgcn_raw_buffer_load_b8(starts.buffer, starts.at(t + 1, t + 1 >= 0 && inside), 0, 0) == 0;
+        Piece<E, kVec> before;
+        held[k].load(x.buffer, x.at(t, t >= 0 && same));
+        before.load(window.buffer, window.at(kTaps - 1 + t, t < 0 && same));
+        held[k].words = t < 0 ? before.words : held[k].words;
     }
 }
 
 template <class E, int kVec, int kTaps>
-__device__ inline void load_weights(const ConvParams& P, int32_t channel, float (&weight)[kTaps][kVec], float (&bias)[kVec]) {
+__device__ inline void load_weights(const ConvParams& P, int32_t channel, bool inside, float (&weight)[kTaps][kVec], float (&bias)[kVec]) {
 #pragma unroll
     for (int i = 0; i < kVec; ++i) {
-        bias[i] = P.a.bias ? P.a.bias[channel + i] : 0.0f;
+        bias[i] = P.a.bias && inside ? P.a.bias[channel + i] : 0.0f;
 #pragma unroll
-        for (int k = 0; k < kTaps; ++k) weight[k][i] = P.a.weight[static_cast<int64_t>(channel + i) * kTaps + kTaps - 1 - k];
+        for (int k = 0; k < kTaps; ++k) weight[k][i] = inside ? P.a.weight[static_cast<int64_t>(channel + i) * kTaps + kTaps - 1 - k] : 0.0f;
     }
 }
 
@@ -140,32 +167,34 @@ __device__ inline void push(const Piece<E, kVec>& x, Piece<E, kVec> (&held)[kTap
 
 template <class E, int kVec, int kTaps>
 __global__ __launch_bounds__(256) void causal_conv_kernel(ConvParams P) {
-    const Place at = place_of<kVec>(P);
-    if (!at.inside) return;
+    const Place<kVec> place(P);
     float weight[kTaps][kVec], bias[kVec];
-    load_weights<E, kVec, kTaps>(P, at.channel, weight, bias);
-    for (int64_t item = at.item; item < P.a.envs * P.segments; item += at.step) {
-        const int64_t env = item / P.segments, t0 = (item - env * P.segments) * P.segment;
-        const int64_t t1 = t0 + P.segment < P.a.steps ? t0 + P.segment : P.a.steps;
-        const E* x = static_cast<const E*>(P.a.x) + env * P.a.x_stride[0] + at.channel;
-        const uint8_t* starts = P.a.starts ? P.a.starts + env * P.a.starts_stride[0] : nullptr;
-        E* out = static_cast<E*>(P.a.out) + env * P.a.steps * P.a.channels + at.channel;
+    load_weights<E, kVec, kTaps>(P, place.channel, place.inside, weight, bias);
+    const int64_t dense = static_cast<int64_t>(P.a.steps) * P.a.channels, kept = static_cast<int64_t>(kTaps - 1) * P.a.channels;
+    const int32_t steps = static_cast<int32_t>(P.a.steps);
+    for (uint32_t first = place.first; first < P.items; first += place.step) {
+        const uint32_t item = first + place.row, env0 = divide(first, P.by_segments);
+        const bool inside = place.inside && item < P.items;
+        const uint32_t env = divide(inside ? item : first, P.by_segments);
+        const int32_t t0 = static_cast<int32_t>((inside ? item : first) - env * P.segments) * P.segment;
+        const int32_t t1 = t0 + P.segment < steps ? t0 + P.segment : steps;
+        const Lines x(P.a.x, P.a.x_stride[0], P.a.x_stride[1], sizeof(E), env0, env, place.channel);
+        const Lines starts(P.a.starts, P.a.starts_stride[0], P.a.starts_stride[1], 1, env0, env, 0);
+        const Lines out(P.a.out, dense, P.a.channels, sizeof(E), env0, env, place.channel);
+        const Lines window(P.a.window, kept, P.a.channels, sizeof(E), env0, env, place.channel);
         Piece<E, kVec> held[kTaps - 1];
-        begin_segment<E, kVec, kTaps>(P, env, t0, at.channel, held);
-        for (int64_t t = t0; t < t1; t += kBatch) {
+        begin_segment<E, kVec, kTaps>(x, window, starts, t0, inside, held);
+        for (int32_t t = t0; t < t1; t += kBatch) {
             Piece<E, kVec> row[kBatch];
-            bool start[kBatch];
+            uint8_t start[kBatch];
 #pragma unroll
             for (int i = 0; i < kBatch; ++i) {
-                start[i] = false;
-                if (t + i < t1) {
-                    row[i].load(x + (t + i) * P.a.x_stride[1]);
-                    if (starts) start[i] = starts[(t + i) * P.a.starts_stride[1]] != 0;
-                }
+                const bool there = inside && t + i < t1;
+                row[i].load(x.buffer, x.at(t + i, there));
+                start[i] = __builtin_amdgcn_raw_buffer_load_b8(starts.buffer, starts.at(t + i, there), 0, 0);
             }
 #pragma unroll
             for (int i = 0; i < kBatch; ++i) {
-                if (t + i >= t1) break;
                 if (start[i])
 #pragma unroll
                     for (int k = 0; k < kTaps - 1; ++k) held[k].clear();
@@ -176,127 +205,183 @@ __global__ __launch_bounds__(256) void causal_conv_kernel(ConvParams P) {
                     for (int n = 0; n < kVec; ++n) z[n] *= sigmoid(z[n]);
                 Piece<E, kVec> y;
                 y.from(z);
-                y.store(out + (t + i) * P.a.channels);
-                push<E, kVec, kTaps>(row[i], held);
+                y.store(out.buffer, out.at(t + i, inside && t + i < t1));
+                if (t + i < t1) push<E, kVec, kTaps>(row[i], held);
             }
         }
-        if (P.a.window_out && t1 == P.a.steps) {
-            E* to = static_cast<E*>(P.a.window_out) + env * (kTaps - 1) * P.a.channels + at.channel;
+        if (P.a.window_out) {
+            const Lines after(P.a.window_out, kept, P.a.channels, sizeof(E), env0, env, place.channel);
 #pragma unroll
-            for (int k = 0; k < kTaps - 1; ++k) held[k].store(to + (kTaps - 2 - k) * P.a.channels);
+            for (int k = 0; k < kTaps - 1; ++k) held[k].store(after.buffer, after.at(kTaps - 2 - k, inside && t1 == steps));
         }
     }
 }
 
-// A segment's lane walks its tokens and taps - 1 after them, dz of each once: `pending[k]` is what
-// the input k tokens before has got so far.
+// A lane's walk over a segment: `pending[k]` is what the input k tokens before has got so far.
 template <class E, int kVec, int kTaps>
-__global__ __launch_bounds__(256) void causal_conv_backward_kernel(ConvParams P) {
+struct BackwardWalk {
+    float weight[kTaps][kVec], bias[kVec];
+    float sums[kTaps + 1][kVec];  // of dz x for each tap, and of dz
+    float pending[kTaps][kVec];
+    Piece<E, kVec> held[kTaps - 1];
+    int since;  // tokens since the last start, as far as any tap asks
+
+    template <bool kSums>
+    __device__ void token(const Piece<E, kVec>& x, const Piece<E, kVec>& dy, bool start, bool silu) {
+        since = start ? 0 : since < kTaps ? since + 1 : kTaps;
+        if (start)
+#pragma unroll
+            for (int k = 0; k < kTaps - 1; ++k) held[k].clear();
+        float z[kVec], dz[kVec];
+        convolve<E, kVec, kTaps>(x, held, weight, bias, z);
+        dy.floats(dz);
+        if (silu)
+#pragma unroll
+            for (int n = 0; n < kVec; ++n) {
+                const float s = sigmoid(z[n]);
+                dz[n] *= s + z[n] * s * (1.0f - s);
+            }
+        if (since >= kTaps - 1) {
+#pragma unroll
+            for (int k = 0; k < kTaps; ++k)
+#pragma unroll
+                for (int n = 0; n < kVec; ++n) pending[k][n] += weight[k][n] * dz[n];
+        } else {
+#pragma unroll
+            for (int k = 0; k < kTaps; ++k)
+                if (k <= since)
+#pragma unroll
+                    for (int n = 0; n < kVec; ++n) pending[k][n] += weight[k][n] * dz[n];
+        }
+        if constexpr (kSums) {
+            float in[kVec];
+            x.floats(in);
+#pragma unroll
+            for (int n = 0; n < kVec; ++n) {
+                sums[0][n] += dz[n] * in[n];
+                sums[kTaps][n] += dz[n];
+            }
+#pragma unroll
+            for (int k = 1; k < kTaps; ++k) {
+                held[k - 1].floats(in);
+#pragma unroll
+                for (int n = 0; n < kVec; ++n) sums[k][n] += dz[n] * in[n];
+            }
+        }
+        push<E, kVec, kTaps>(x, held);
+    }
+
+    // The oldest input has all that it gets.
+    __device__ Piece<E, kVec> finish() {
+        Piece<E, kVec> d;
+        d.from(pending[kTaps - 1]);
+#pragma unroll
+        for (int k = kTaps - 1; k > 0; --k)
+#pragma unroll
+            for (int n = 0; n < kVec; ++n) pending[k][n] = pending[k - 1][n];
+#pragma unroll
+        for (int n = 0; n < kVec; ++n) pending[0][n] = 0.0f;
+        return d;
+    }
+};
+
+// Segments' inputs and dy once, with those of the taps - 1 tokens after each segment (whole segments but
+// for an env's last, whose walk ends with its last token). Four numbers a lane, also of 16 bits: sums,
+// weights and what is pending of eight would leave a SIMD one wave.
+template <class E, int kVec, int kTaps>
+__global__ __launch_bounds__(256, sizeof(E) == 4 ? 2 : 4) void causal_conv_backward_kernel(ConvParams P) {
     constexpr int kSums = kTaps + 1;
     extern __shared__ float sums_lds[];
-    const Place at = place_of<kVec>(P);
-    float sums[kSums][kVec] = {};
-    if (at.inside) {
-        float weight[kTaps][kVec], bias[kVec];
-        load_weights<E, kVec, kTaps>(P, at.channel, weight, bias);
-        for (int64_t item = at.item; item < P.a.envs * P.segments; item += at.step) {
-            const int64_t env = item / P.segments, t0 = (item - env * P.segments) * P.segment;
-            const int64_t t1 = t0 + P.segment < P.a.steps ? t0 + P.segment : P.a.steps;
-            const int64_t first = t0 == 0 ? -(kTaps - 1) : t0;  // the first segment has the window's gradients too
-            const int64_t last = t1 + kTaps - 1 < P.a.steps ? t1 + kTaps - 1 : P.a.steps;
-            const E* x = static_cast<const E*>(P.a.x) + env * P.a.x_stride[0] + at.channel;
-            const E* dy = static_cast<const E*>(P.a.grad_out) + env * P.a.grad_out_stride[0] + at.channel;
-            const uint8_t* starts = P.a.starts ? P.a.starts + env * P.a.starts_stride[0] : nullptr;
-            E* dx = static_cast<E*>(P.a.d_x) + env * P.a.steps * P.a.channels + at.channel;
-            E* d_window = P.a.d_window ? static_cast<E*>(P.a.d_window) + env * (kTaps - 1) * P.a.channels + at.channel : nullptr;
-            Piece<E, kVec> held[kTaps - 1];
-            begin_segment<E, kVec, kTaps>(P, env, t0, at.channel, held);
-            float pending[kTaps][kVec] = {};
-            int since = kTaps;  // tokens since the last start, as far as any tap asks
-            const auto finish = [&](int64_t t) {  // the oldest has all that it gets
-                if (t >= first && t < t1) {
-                    Piece<E, kVec> d;
-                    d.from(pending[kTaps - 1]);
-                    if (t >= 0)
-                        d.store(dx + t * P.a.channels);
-                    else if (d_window)
-                        d.store(d_window + (kTaps - 1 + t) * P.a.channels);
-                }
+    const Place<kVec> place(P);
+    BackwardWalk<E, kVec, kTaps> w;
 #pragma unroll
-                for (int k = kTaps - 1; k > 0; --k)
+    for (int s = 0; s < kSums; ++s)
 #pragma unroll
-                    for (int n = 0; n < kVec; ++n) pending[k][n] = pending[k - 1][n];
+        for (int n = 0; n < kVec; ++n) w.sums[s][n] = 0.0f;
+    load_weights<E, kVec, kTaps>(P, place.channel, place.inside, w.weight, w.bias);
+    const bool silu = P.a.activation == NAVI_POLICY_SILU;
+    const int64_t dense = static_cast<int64_t>(P.a.steps) * P.a.channels, kept = static_cast<int64_t>(kTaps - 1) * P.a.channels;
+    const int32_t steps = static_cast<int32_t>(P.a.steps);
+    for (uint32_t first = place.first; first < P.items; first += place.step) {
+        const uint32_t item = first + place.row, env0 = divide(first, P.by_segments);
+        const bool inside = place.inside && item < P.items;
+        const uint32_t env = divide(inside ? item : first, P.by_segments);
+        const int32_t t0 = static_cast<int32_t>((inside ? item : first) - env * P.segments) * P.segment;
+        const int32_t t1 = t0 + P.segment < steps ? t0 + P.segment : steps;
+        const int32_t last = t1 + kTaps - 1 < steps ? t1 + kTaps - 1 : steps;
+        const Lines x(P.a.x, P.a.x_stride[0], P.a.x_stride[1], sizeof(E), env0, env, place.channel);
+        const Lines dy(P.a.grad_out, P.a.grad_out_stride[0], P.a.grad_out_stride[1], sizeof(E), env0, env, place.channel);
+        const Lines starts(P.a.starts, P.a.starts_stride[0], P.a.starts_stride[1], 1, env0, env, 0);
+        const Lines dx(P.a.d_x, dense, P.a.channels, sizeof(E), env0, env, place.channel);
+        const Lines window(P.a.window, kept, P.a.channels, sizeof(E), env0, env, place.channel);
+        const Lines d_window(P.a.d_window, kept, P.a.channels, sizeof(E), env0, env, place.channel);
+        const auto finish = [&](int32_t t) {
+            const Piece<E, kVec> d = w.finish();
+            d.store(dx.buffer, dx.at(t, inside && t >= t0 && t < t1));
+        };
+        begin_segment<E, kVec, kTaps>(x, window, starts, t0, inside, w.held);
 #pragma unroll
-                for (int n = 0; n < kVec; ++n) pending[0][n] = 0.0f;
-            };
-            for (int64_t t = t0; t < last; t += kBatch) {
-                Piece<E, kVec> row[kBatch], grad[kBatch];
-                bool start[kBatch];
+        for (int k = 0; k < kTaps; ++k)
 #pragma unroll
-                for (int i = 0; i < kBatch; ++i) {
-                    start[i] = false;
-                    if (t + i < last) {
-                        row[i].load(x + (t + i) * P.a.x_stride[1]);
-                        grad[i].load(dy + (t + i) * P.a.grad_out_stride[1]);
-                        if (starts) start[i] = starts[(t + i) * P.a.starts_stride[1]] != 0;
-                    }
-                }
+            for (int n = 0; n < kVec; ++n) w.pending[k][n] = 0.0f;
+        w.since = kTaps;
+        Piece<E, kVec> after[kTaps - 1], after_dy[kTaps - 1];  // the tokens after the segment
+        uint8_t after_start[kTaps - 1];
 #pragma unroll
-                for (int i = 0; i < kBatch; ++i) {
-                    if (t + i >= last) break;
-                    since = start[i] ? 0 : since < kTaps ? since + 1 : kTaps;
-                    if (start[i])
+        for (int k = 0; k < kTaps - 1; ++k) {
+            const bool there = inside && t1 + k < last;
+            after[k].load(x.buffer, x.at(t1 + k, there));
+            after_dy[k].load(dy.buffer, dy.at(t1 + k, there));
+            after_start[k] = __builtin_amdgcn_raw_buffer_load_b8(starts.buffer, starts.at(t1 + k, there), 0, 0);
+        }
+        for (int32_t t = t0; t < t1; t += kBackBatch) {
+            Piece<E, kVec> row[kBackBatch], grad[kBackBatch];
+            uint8_t start[kBackBatch];
 #pragma unroll
-                        for (int k = 0; k < kTaps - 1; ++k) held[k].clear();
-                    float z[kVec], dz[kVec];
-                    convolve<E, kVec, kTaps>(row[i], held, weight, bias, z);
-                    grad[i].floats(dz);
-                    if (P.a.activation == NAVI_POLICY_SILU)
+            for (int i = 0; i < kBackBatch; ++i) {
+                const bool there = inside && t + i < t1;
+                row[i].load(x.buffer, x.at(t + i, there));
+                grad[i].load(dy.buffer, dy.at(t + i, there));
+                start[i] = __builtin_amdgcn_raw_buffer_load_b8(starts.buffer, starts.at(t + i, there), 0, 0);
+            }
 #pragma unroll
-                        for (int n = 0; n < kVec; ++n) {
-                            const float s = sigmoid(z[n]);
-                            dz[n] *= s + z[n] * s * (1.0f - s);
-                        }
-#pragma unroll
-                    for (int k = 0; k < kTaps; ++k)
-                        if (k <= since)
-#pragma unroll
-                            for (int n = 0; n < kVec; ++n) pending[k][n] += weight[k][n] * dz[n];
-                    if (t + i < t1) {
-                        float in[kVec];
-                        row[i].floats(in);
-#pragma unroll
-                        for (int n = 0; n < kVec; ++n) {
-                            sums[0][n] += dz[n] * in[n];
-                            sums[kTaps][n] += dz[n];
-                        }
-#pragma unroll
-                        for (int k = 1; k < kTaps; ++k) {
-                            held[k - 1].floats(in);
-#pragma unroll
-                            for (int n = 0; n < kVec; ++n) sums[k][n] += dz[n] * in[n];
-                        }
-                    }
-                    push<E, kVec, kTaps>(row[i], held);
+            for (int i = 0; i < kBackBatch; ++i) {
+                if (t + i >= t1) break;
+                w.template token<true>(row[i], grad[i], start[i] != 0, silu);
+                if (t == 0 && i < kTaps - 1 && P.a.d_window) {  // (what leaves before the first step)
+                    const Piece<E, kVec> d = w.finish();
+                    d.store(d_window.buffer, d_window.at(i, inside));
+                } else {
                     finish(t + i - (kTaps - 1));
                 }
             }
-            // What is left: inputs whose last readers are done, and those that the window after
-            // the last step holds (pending[k + 1] is the input k + 1 tokens before `last`).
-            const E* grad_window = P.a.grad_window && last == P.a.steps
-                                       ? static_cast<const E*>(P.a.grad_window) + env * (kTaps - 1) * P.a.channels + at.channel : nullptr;
+        }
+#pragma unroll
+        for (int k = 0; k < kTaps - 1; ++k) {
+            if (t1 + k >= last) break;
+            w.template token<false>(after[k], after_dy[k], after_start[k] != 0, silu);
+            finish(t1 + k - (kTaps - 1));
+        }
+        // What is left: inputs whose last readers are done, and those that the window after
+        // the last step holds (pending[k + 1] is the input k + 1 tokens before `last`).
+        if (P.a.grad_window) {
+            const Lines grad_window(P.a.grad_window, kept, P.a.channels, sizeof(E), env0, env, place.channel);
 #pragma unroll
             for (int k = 0; k < kTaps - 1; ++k) {
-                if (!grad_window || k > since) continue;
                 Piece<E, kVec> g;
-                g.load(grad_window + (kTaps - 2 - k) * P.a.channels);
-                float x[kVec];
-                g.floats(x);
+                g.load(grad_window.buffer, grad_window.at(kTaps - 2 - k, inside && last == steps && k <= w.since));
+                float d[kVec];
+                g.floats(d);
 #pragma unroll
-                for (int n = 0; n < kVec; ++n) pending[k + 1][n] += x[n];
+                for (int n = 0; n < kVec; ++n) w.pending[k + 1][n] += d[n];
             }
+        }
 #pragma unroll
-            for (int k = 0; k < kTaps - 1; ++k) finish(last - (kTaps - 1) + k);
+        for (int k = 0; k < kTaps - 1; ++k) {
+            const int32_t t = last - (kTaps - 1) + k;
+            const Piece<E, kVec> d = w.finish();
+            d.store(dx.buffer, dx.at(t, inside && t >= t0 && t < t1));
+            d.store(d_window.buffer, d_window.at(kTaps - 1 + t, inside && t < 0 && t0 == 0));
         }
     }
     if (!P.a.partial) return;
@@ -304,15 +389,15 @@ __global__ __launch_bounds__(256) void causal_conv_backward_kernel(ConvParams P)
 #pragma unroll
     for (int s = 0; s < kSums; ++s)
 #pragma unroll
-        for (int n = 0; n < kVec; ++n) sums_lds[(s * kVec + n) * 256 + threadIdx.x] = sums[s][n];
+        for (int n = 0; n < kVec; ++n) sums_lds[(s * kVec + n) * 256 + threadIdx.x] = w.sums[s][n];
     __syncthreads();
-    const int32_t block = blockIdx.x % P.across_blocks, down = blockIdx.x / P.across_blocks;
     for (int32_t i = threadIdx.x; i < P.across * kSums * kVec; i += 256) {
-        const int32_t c = i % P.across, s = i / P.across, channel = (block * P.across + c) * kVec + s % kVec;
-        if (block * P.across + c >= P.groups) continue;
+        const int32_t s = static_cast<int32_t>(divide(i, P.by_across)), c = i - s * P.across;
+        const int32_t channel = (place.block * P.across + c) * kVec + s % kVec;
+        if (place.block * P.across + c >= P.groups) continue;
         float sum = 0.0f;
         for (int32_t r = 0; r < P.rows; ++r) sum += sums_lds[s * 256 + r * P.across + c];
-        P.a.partial[(static_cast<int64_t>(down) * kSums + s / kVec) * P.a.channels + channel] = sum;
+        P.a.partial[(static_cast<int64_t>(place.down) * kSums + s / kVec) * P.a.channels + channel] = sum;
     }
 }
 
@@ -329,20 +414,38 @@ __global__ __launch_bounds__(1024) void causal_conv_sums_kernel(ConvParams P) {
     }
 }
 
+constexpr int64_t kReach = int64_t{1} << 31;  // bytes that a workgroup's 32-bit offsets reach
+
 // How a call is laid out. Segments are as long as leaves 2^16 lanes (of 2^18 that the card holds at
-// once) their own; longer ones read fewer inputs twice, shorter ones fill the card.
-void lay_out(ConvParams& P, int vec, bool back) {
+// once) their own; longer ones read fewer inputs twice, shorter ones fill the card. false: too large.
+bool lay_out(ConvParams& P, int vec, bool back) {
     const navi_causal_conv_args& a = P.a;
     P.groups = a.channels / vec;
     P.across = std::min(P.groups, 256);
-    P.rows = 256 / P.across;
     P.across_blocks = (P.groups + P.across - 1) / P.across;
     P.segment = 64;
     while (P.segment > 8 && a.envs * ((a.steps + P.segment - 1) / P.segment) * P.groups < (1 << 16)) P.segment /= 2;
-    P.segments = std::max<int64_t>(1, (a.steps + P.segment - 1) / P.segment);
-    const int64_t down = (a.envs * P.segments + P.rows - 1) / P.rows;
-    const int64_t most = back ? std::max(1, kPartialBlocks / P.across_blocks) : INT32_MAX / P.across_blocks;
+    const int64_t segments = std::max<int64_t>(1, (a.steps + P.segment - 1) / P.segment), items = a.envs * segments;
+    // What a workgroup reaches from the first of its envs on: as many as it has rows, if that is near enough.
+    const int64_t bytes = a.dtype == NAVI_POLICY_F32 ? 4 : 2;
+    const auto reach = [&](int64_t envs) {
+        const auto rows = [&](int64_t env, int64_t step) { return envs * std::abs(env) + a.steps * std::abs(step) + a.channels; };
+        int64_t most = std::max(rows(a.x_stride[0], a.x_stride[1]), rows(a.steps * a.channels, a.channels));
+        if (back) most = std::max(most, rows(a.grad_out_stride[0], a.grad_out_stride[1]));
+        return std::max(most * bytes, a.starts ? rows(a.starts_stride[0], a.starts_stride[1]) : 0);
+    };
+    P.rows = 256 / P.across;
+    if (reach((P.rows + segments - 1) / segments + 1) >= kReach) P.rows = 1;
+    if (reach(0) >= kReach || items > INT32_MAX / 2) return false;
+    P.items = static_cast<uint32_t>(items);
+    P.segments = static_cast<uint32_t>(segments);
+    const int64_t down = (items + P.rows - 1) / P.rows;
+    const int64_t most = back ? std::max(1, kPartialBlocks / P.across_blocks) : (1 << 30) / P.across_blocks;
     P.down_blocks = static_cast<int32_t>(std::min(down, most));
+    P.by_segments = divisor_of(segments);
+    P.by_across = divisor_of(P.across);
+    P.by_across_blocks = divisor_of(P.across_blocks);
+    return true;
 }
 
 int check(const navi_causal_conv_args* a) {
@@ -355,6 +458,8 @@ int check(const navi_causal_conv_args* a) {
         return set_error(NAVI_POLICY_E_ARG, "activation must be none or silu");
     if (a->envs < 0 || a->steps < 0 || a->envs > INT32_MAX || a->steps > INT32_MAX || a->envs * std::max<int64_t>(a->steps, 1) > (int64_t{1} << 40))
         return set_error(NAVI_POLICY_E_ARG, "envs and steps must not be negative, and below 2^31 (2^40 together)");
+    for (const int64_t (*stride)[2] : {&a->x_stride, &a->starts_stride, &a->grad_out_stride})
+        if ((*stride)[0] < 0 || (*stride)[1] < 0) return set_error(NAVI_POLICY_E_ARG, "strides must not be negative");
     if (a->envs == 0) return 1;
     if (!a->weight || (a->steps > 0 && !a->x)) return set_error(NAVI_POLICY_E_ARG, "x and weight must be non-null");
     const int64_t bytes = a->dtype == NAVI_POLICY_F32 ? 4 : 2;
@@ -393,41 +498,49 @@ int launched(const char* name) {
 
 template <class E, int kVec, int kTaps>
 int run(ConvParams& P, bool back, hipStream_t stream) {
-    lay_out(P, kVec, back);
-    const int64_t blocks = static_cast<int64_t>(P.across_blocks) * P.down_blocks;
-    if (blocks > INT32_MAX) return set_error(NAVI_POLICY_E_ARG, "navi_causal_conv: too many envs, steps and channels");
-    if (!back) {
-        hipLaunchKernelGGL((causal_conv_kernel<E, kVec, kTaps>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, P);
-        return launched("navi_causal_conv");
+    if (!lay_out(P, kVec, back))
+        return set_error(NAVI_POLICY_E_ARG, "navi_causal_conv: an env's steps must lie within 2 GiB, and envs * steps / 8 below 2^30");
+    const dim3 grid(static_cast<unsigned>(P.across_blocks * P.down_blocks));
+    if constexpr (kVec == 1 || kVec * sizeof(E) == 16) {
+        if (!back) {
+            hipLaunchKernelGGL((causal_conv_kernel<E, kVec, kTaps>), grid, dim3(256), 0, stream, P);
+            return launched("navi_causal_conv");
+        }
     }
-    const unsigned lds = P.a.partial ? (kTaps + 1) * kVec * 256 * sizeof(float) : 0;
-    hipLaunchKernelGGL((causal_conv_backward_kernel<E, kVec, kTaps>), dim3(static_cast<unsigned>(blocks)), dim3(256), lds, stream, P);
-    if (P.a.partial)
-        hipLaunchKernelGGL((causal_conv_sums_kernel<kTaps>), dim3(((kTaps + 1) * P.a.channels + kSumColumns - 1) / kSumColumns), dim3(1024), 0,
-                           stream, P);
+    if constexpr (kVec <= 4) {
+        const unsigned lds = P.a.partial ? (kTaps + 1) * kVec * 256 * sizeof(float) : 0;
+        hipLaunchKernelGGL((causal_conv_backward_kernel<E, kVec, kTaps>), grid, dim3(256), lds, stream, P);
+        if (P.a.partial)
+            hipLaunchKernelGGL((causal_conv_sums_kernel<kTaps>), dim3(((kTaps + 1) * P.a.channels + kSumColumns - 1) / kSumColumns), dim3(1024),
+                               0, stream, P);
+    }
     return launched("navi_causal_conv_backward");
 }
 
-bool wide(const navi_causal_conv_args& a, bool back) {
+// Whether rows are whole pieces of `piece` bytes at their addresses.
+bool wide(const navi_causal_conv_args& a, bool back, int64_t piece) {
     const int64_t bytes = a.dtype == NAVI_POLICY_F32 ? 4 : 2;
     const auto rows = [&](const void* p, const int64_t(&s)[2]) {
-        return aligned16(p) && s[0] * bytes % 16 == 0 && s[1] * bytes % 16 == 0;
+        return aligned(piece, p) && s[0] * bytes % piece == 0 && s[1] * bytes % piece == 0;
     };
-    bool fine = a.channels * bytes % 16 == 0 && rows(a.x, a.x_stride) && aligned16(a.window);
-    if (!back) return fine && aligned16(a.out) && aligned16(a.window_out);
-    return fine && rows(a.grad_out, a.grad_out_stride) && aligned16(a.d_x) && aligned16(a.d_window) && aligned16(a.grad_window);
+    const bool fine = a.channels * bytes % piece == 0 && rows(a.x, a.x_stride) && aligned(piece, a.window);
+    if (!back) return fine && aligned(piece, a.out, a.window_out);
+    return fine && rows(a.grad_out, a.grad_out_stride) && aligned(piece, a.d_x, a.d_window, a.grad_window);
+}
+
+template <class E, int kVec>
+int tapped(ConvParams& P, bool back, hipStream_t stream) {
+    if (P.a.taps == 2) return run<E, kVec, 2>(P, back, stream);
+    if (P.a.taps == 3) return run<E, kVec, 3>(P, back, stream);
+    return run<E, kVec, 4>(P, back, stream);
 }
 
 template <class E>
 int typed(ConvParams& P, bool back, hipStream_t stream) {
-    const auto taps = [&](auto vec) {
-        constexpr int kVec = decltype(vec)::value;
-        if (P.a.taps == 2) return run<E, kVec, 2>(P, back, stream);
-        if (P.a.taps == 3) return run<E, kVec, 3>(P, back, stream);
-        return run<E, kVec, 4>(P, back, stream);
-    };
-    if (wide(P.a, back)) return taps(std::integral_constant<int, 16 / sizeof(E)>{});
-    return taps(std::integral_constant<int, 1>{});
+    constexpr int kForward = 16 / sizeof(E);
+    if (!back && wide(P.a, back, 16)) return tapped<E, kForward>(P, back, stream);
+    if (back && wide(P.a, back, 4 * sizeof(E))) return tapped<E, 4>(P, back, stream);
+    return tapped<E, 1>(P, back, stream);
 }
 
 int run_typed(const navi_causal_conv_args* args, bool back, hipStream_t stream) {
@@ -458,7 +571,7 @@ extern "C" int64_t navi_causal_conv_workspace(const navi_causal_conv_args* args)
     using namespace navi_policy;
     const int code = check(args);
     if (code != NAVI_POLICY_OK) return code < 0 ? code : 0;
-    const int64_t groups = args->channels * (args->dtype == NAVI_POLICY_F32 ? 4 : 2) / 16;  // (of 16 bytes: the fewest)
+    const int64_t groups = args->channels / 4;  // (the fewest pieces of a row)
     const int64_t most = std::max<int64_t>(1, kPartialBlocks / std::max<int64_t>(1, (groups + 255) / 256));
     const int64_t down = std::min(most, args->envs * std::max<int64_t>(1, (args->steps + 7) / 8));
     return down * (args->taps + 1) * args->channels * 4;

@@ -394,9 +394,13 @@ struct FourFetch {
     }
 };
 
+// Workgroups that a CU's LDS holds: 42 KB each for bfloat16 and 64, up to 147 KB for float32 and 128.
+template <class E, int KP>
+inline constexpr int kWorkgroups = kPlanes<E> == 1 ? (KP == 64 ? 3 : 2) : kPlanes<E> == 2 && KP == 64 ? 2 : 1;
+
 // A workgroup walks the chunks of a segment with 64 columns of a head's state in registers, 16 a wave.
 template <class E, int KP, int kMode>
-__global__ __launch_bounds__(256, (kPlanes<E> == 1 && KP == 64 ? 3 : 2)) void selective_scan_kernel(ScanParams P) {
+__global__ __launch_bounds__(256, (kWorkgroups<E, KP>)) void selective_scan_kernel(ScanParams P) {
     constexpr bool kSummary = kMode == kSegments, kGates = kMode == kGradients;
     constexpr int N = kPlanes<E>;
     extern __shared__ char lds_bytes[];
