@@ -28,35 +28,103 @@ using h8 = _Float16 __attribute__((ext_vector_type(8)));
 using h4 = _Float16 __attribute__((ext_vector_type(4)));
 using f16x16 = float __attribute__((ext_vector_type(16)));
 
-constexpr int kMatrices = 28;       // of a launch: its arguments stay under 4 KiB
+constexpr int kMatrices = 62;       // of a launch: its arguments stay under 4 KiB
 constexpr int kNormBlocks = 64;     // workgroups that sum a matrix's squares
-constexpr int kDepth = 64;          // of a product's step
+constexpr int kDepth = 32;          // of a product's stage
+constexpr int kStages = 4;          // in LDS at once
 constexpr float kScaleA = 1024.0f;  // of A and P
-constexpr int64_t kGroupBytes = int64_t{1} << 30;  // of workspace that matrices in one launch share
+constexpr int64_t kGroupBytes = int64_t{4} << 30;  // of workspace that matrices in one launch share
 
 struct Matrix {
     const void* from;
     void* to;
-    int64_t from_stride[2], to_stride[2];  // of X's rows and columns
+    int64_t from_line;      // elements between X's rows, or (`turned`) its columns; those along them lie side by side
+    int64_t to_stride[2];   // of X's rows and columns
+    int32_t m, n;           // X
+    int32_t first_tile, first_piece;  // of those of all matrices
+    uint32_t place;         // in the workspace, 256 bytes
+    int8_t from_dtype, to_dtype, turned;
+    int8_t scale;           // X times two to this
+};
+static_assert(sizeof(Matrix) == 64, "a launch's arguments");
+
+struct Params {
+    Matrix matrix[kMatrices];
+    char* workspace;
+    int32_t count, tiles;
+    int32_t tile;      // M and N are m and n rounded up to it
+    int32_t current;   // which of the two X^T is this step's
+    float a, b, c, eps;
+};
+static_assert(sizeof(Params) <= 4096, "a launch's arguments");
+
+// Where a matrix's part of the workspace holds what.
+template <int kPlanes16>
+struct Parts {
+    int32_t M, N;
+    int64_t size, square;
     _Float16* rows;     // [planes][M][N] X
     _Float16* turned;   // [2][2][N][M] X^T, this step's and the next's, each hi and what it leaves
     _Float16* gram;     // [planes][M][M]
     _Float16* poly;     // [planes][M][M] P without its diagonal
     float* diagonal;    // [M] a + P's diagonal
     double* squares;    // [kNormBlocks]
-    int32_t m, n, M, N;  // and rounded up to whole tiles
-    int32_t from_dtype, to_dtype;
-    int32_t first_tile, first_piece;  // of those of all matrices
-    float scale;        // of X
+    float scale;
+
+    __device__ Parts(const Params& P, const Matrix& x, int tile) {
+        M = (x.m + tile - 1) / tile * tile;
+        N = (x.n + tile - 1) / tile * tile;
+        size = static_cast<int64_t>(M) * N;
+        square = static_cast<int64_t>(M) * M;
+        squares = reinterpret_cast<double*>(P.workspace + 256 * static_cast<uint64_t>(x.place));
+        diagonal = reinterpret_cast<float*>(squares + kNormBlocks);
+        rows = reinterpret_cast<_Float16*>(diagonal + M);
+        turned = rows + kPlanes16 * size;
+        gram = turned + 4 * size;
+        poly = gram + kPlanes16 * square;
+        scale = __builtin_ldexpf(1.0f, x.scale);
+    }
 };
 
-struct Params {
-    Matrix matrix[kMatrices];
-    int32_t count, tiles;
-    int32_t current;   // which of the two X^T is this step's
-    float a, b, c, eps;
+// Sixteen bytes at any element's address (vector accesses of global memory need no more).
+template <class E>
+struct __attribute__((packed, aligned(sizeof(E)))) Vector {
+    u4 words;
 };
-static_assert(sizeof(Params) <= 4096, "a launch's arguments");
+
+// The squares of `count` numbers, by 256 threads. In float64: those of any float32 are in range.
+template <class E>
+__device__ inline double sum_of_squares(const E* from, int64_t count) {
+    constexpr int kEach = 16 / sizeof(E);
+    const int64_t whole = count / kEach;
+    double sum = 0.0;
+    const auto add = [&](u4 words) {
+        union {
+            u4 words;
+            E elements[kEach];
+        } got{words};
+#pragma unroll
+        for (int n = 0; n < kEach; ++n) {
+            const double v = to_float(got.elements[n]);
+            sum += v * v;
+        }
+    };
+    int64_t i = threadIdx.x;
+    for (; i + 768 < whole; i += 1024) {
+        u4 words[4];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) words[n] = reinterpret_cast<const Vector<E>*>(from)[i + 256 * n].words;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) add(words[n]);
+    }
+    for (; i < whole; i += 256) add(reinterpret_cast<const Vector<E>*>(from)[i].words);
+    const int64_t left = whole * kEach + threadIdx.x;
+    if (left < count) {
+        const double v = to_float(from[left]);
+        sum += v * v;
+    }
+    return sum;
+}
 
 __device__ inline float load_any(const void* from, int32_t dtype, int64_t at) {
     if (dtype == NAVI_POLICY_F32) return static_cast<const float*>(from)[at];
@@ -64,32 +132,33 @@ __device__ inline float load_any(const void* from, int32_t dtype, int64_t at) {
     return to_float(static_cast<const f16*>(from)[at]);
 }
 
-__device__ inline void store_any(void* to, int32_t dtype, int64_t at, float x) {
-    if (dtype == NAVI_POLICY_F32)
-        static_cast<float*>(to)[at] = x;
-    else if (dtype == NAVI_POLICY_BF16)
-        static_cast<bf16*>(to)[at] = from_float<bf16>(x);
-    else
-        static_cast<f16*>(to)[at] = from_float<f16>(x);
-}
-
-// Squares of a matrix: workgroups take lines along its contiguous axis in turn.
+// Squares of a matrix: workgroups take lines along its contiguous axis in turn, or parts of all of them
+// where those lie one after the other.
 __global__ __launch_bounds__(256) void newton_squares_kernel(Params P) {
     __shared__ double part[4];
     const Matrix& x = P.matrix[blockIdx.y];
-    const bool along = x.from_stride[1] == 1;
-    const int64_t lines = along ? x.m : x.n, length = along ? x.n : x.m, stride = along ? x.from_stride[0] : x.from_stride[1];
+    int64_t lines = x.turned ? x.n : x.m, length = x.turned ? x.m : x.n, stride = x.from_line;
+    if (stride == length) {  // (parts begin at multiples of 16 bytes from the first number)
+        const int64_t all = lines * length;
+        length = ((all + kNormBlocks - 1) / kNormBlocks + 7) / 8 * 8;
+        lines = (all + length - 1) / length;
+        stride = length;
+        if (static_cast<int64_t>(blockIdx.x) + 1 == lines) length = all - blockIdx.x * length;
+    }
     double sum = 0.0;
-    for (int64_t line = blockIdx.x; line < lines; line += kNormBlocks)
-        for (int64_t i = threadIdx.x; i < length; i += 256) {
-            const double v = load_any(x.from, x.from_dtype, line * stride + i);
-            sum += v * v;
-        }
+    for (int64_t line = blockIdx.x; line < lines; line += kNormBlocks) {
+        if (x.from_dtype == NAVI_POLICY_F32)
+            sum += sum_of_squares(static_cast<const float*>(x.from) + line * stride, length);
+        else if (x.from_dtype == NAVI_POLICY_BF16)
+            sum += sum_of_squares(static_cast<const bf16*>(x.from) + line * stride, length);
+        else
+            sum += sum_of_squares(static_cast<const f16*>(x.from) + line * stride, length);
+    }
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = sum;
     __syncthreads();
-    if (threadIdx.x == 0) x.squares[blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]);
+    if (threadIdx.x == 0) Parts<1>(P, x, P.tile).squares[blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]);
 }
 
 // The last matrix whose first tile (or piece) is not after `at`.
@@ -117,31 +186,32 @@ __global__ __launch_bounds__(256) void newton_begin_kernel(Params P) {
     __shared__ float tile[64][65];
     const int at = blockIdx.x, index = matrix_of(P, at, [](const Matrix& x) { return x.first_piece; });
     const Matrix& x = P.matrix[index];
-    const int piece = at - x.first_piece, across = x.N / 64, row0 = piece / across * 64, col0 = piece % across * 64;
+    const Parts<kPlanes16> w(P, x, P.tile);
+    const int piece = at - x.first_piece, across = w.N / 64, row0 = piece / across * 64, col0 = piece % across * 64;
     const int lane = threadIdx.x & 63, wave = wave_of_workgroup();
-    double sum = x.squares[lane];
+    double sum = w.squares[lane];
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
-    const double factor = x.scale / (sqrt(sum) + static_cast<double>(P.eps));
-    const bool along = x.from_stride[1] == 1;
+    const double factor = w.scale / (sqrt(sum) + static_cast<double>(P.eps));
+    const bool along = !x.turned;
     for (int i = wave; i < 64; i += 4) {
         const int row = row0 + (along ? i : lane), col = col0 + (along ? lane : i);
         float v = 0.0f;
         if (row < x.m && col < x.n)
-            v = static_cast<float>(load_any(x.from, x.from_dtype, row * x.from_stride[0] + col * x.from_stride[1]) * factor);
+            v = static_cast<float>(load_any(x.from, x.from_dtype, along ? row * x.from_line + col : col * x.from_line + row) * factor);
         tile[along ? i : lane][along ? lane : i] = v;
     }
     __syncthreads();
-    const int64_t size = static_cast<int64_t>(x.M) * x.N;
-    _Float16* turned = x.turned + P.current * 2 * size;
+    const int64_t size = w.size;
+    _Float16* turned = w.turned + P.current * 2 * size;
     for (int i = wave; i < 64; i += 4) {
         _Float16 hi, lo;
         split(tile[i][lane], hi, lo);
-        const int64_t to = static_cast<int64_t>(row0 + i) * x.N + col0 + lane;
-        x.rows[to] = hi;
-        if (kPlanes16 == 2) x.rows[size + to] = lo;
+        const int64_t to = static_cast<int64_t>(row0 + i) * w.N + col0 + lane;
+        w.rows[to] = hi;
+        if (kPlanes16 == 2) w.rows[size + to] = lo;
         split(tile[lane][i], hi, lo);
-        const int64_t back = static_cast<int64_t>(col0 + i) * x.M + row0 + lane;
+        const int64_t back = static_cast<int64_t>(col0 + i) * w.M + row0 + lane;
         turned[back] = hi;
         turned[size + back] = lo;
     }
@@ -149,33 +219,118 @@ __global__ __launch_bounds__(256) void newton_begin_kernel(Params P) {
 
 enum { kGram, kPoly, kApply, kLast };
 
-// A product's operands from memory to LDS, 16 bytes a lane, without registers between: a row of 64
-// numbers is eight pieces, piece p of row r in place p ^ (r % 8), so that the eight lanes that read
-// one piece of eight rows at once find them in all banks.
-template <int kRows, int kThreads>
+// A product's operands lie in LDS in rows of 32 numbers, four pieces of 16 bytes; piece p of row r in place
+// p ^ place_of_row(r), so that the lanes that read one piece of 8 or 16 rows at once find them in all banks.
+__device__ inline int place_of_row(int row) { return ((row >> 1) ^ (row >> 3)) & 3; }
+
+// From memory to LDS, 16 bytes a lane, without registers between.
+template <int kRows>
 __device__ inline void stage(const _Float16* from, int64_t stride, _Float16* lds) {
-    constexpr int kAtOnce = kThreads / 8;  // rows
-    const int row = threadIdx.x >> 3, piece = (threadIdx.x & 7) ^ (row & 7);
+    const int row = threadIdx.x >> 2, piece = (threadIdx.x & 3) ^ place_of_row(row);
     const _Float16* lane = from + row * stride + piece * 8;
     _Float16* to = lds + wave_of_workgroup() * 512;  // (the wave's; its lanes follow each other)
 #pragma unroll
-    for (int i = 0; i < kRows / kAtOnce; ++i)
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(lane + i * kAtOnce * stride),
-                                         (__attribute__((address_space(3))) void*)(to + i * kAtOnce * kDepth), 16, 0, 0);
+    for (int i = 0; i < kRows / 64; ++i)
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(lane + i * 64 * stride),
+                                         (__attribute__((address_space(3))) void*)(to + i * 64 * kDepth), 16, 0, 0);
 }
 
-// Tiles of one of the three products, kTile x kTile a workgroup, kTile / 2 x 64 a wave.
+// A tile of results on its way to memory: its columns one after the other, apart by rows that begin in
+// other banks.
+template <int kTile>
+using Tile = _Float16[kTile][kTile + 8];
+
+// From an array whose rows are the tile's columns.
+template <int kTile>
+__device__ inline void get_tile(Tile<kTile>& tile, const _Float16* from, int64_t stride) {
+    constexpr int kAcross = kTile / 8, kAtOnce = 256 / kAcross, kBatch = kTile / kAtOnce < 8 ? kTile / kAtOnce : 8;
+    const int row = threadIdx.x / kAcross, column = threadIdx.x % kAcross * 8;
+    for (int i = row; i < kTile; i += kAtOnce * kBatch) {
+        h8 x[kBatch];
+#pragma unroll
+        for (int n = 0; n < kBatch; ++n) x[n] = *reinterpret_cast<const h8*>(from + (i + n * kAtOnce) * stride + column);
+#pragma unroll
+        for (int n = 0; n < kBatch; ++n) *reinterpret_cast<h8*>(&tile[i + n * kAtOnce][column]) = x[n];
+    }
+}
+
+// And back.
+template <int kTile>
+__device__ inline void put_straight(const Tile<kTile>& tile, _Float16* to, int64_t stride) {
+    constexpr int kAcross = kTile / 8, kAtOnce = 256 / kAcross;
+    const int row = threadIdx.x / kAcross, column = threadIdx.x % kAcross * 8;
+#pragma unroll 4
+    for (int k = 0; k < kTile / kAtOnce; ++k)
+        *reinterpret_cast<h8*>(to + (row + k * kAtOnce) * stride + column) = *reinterpret_cast<const h8*>(&tile[row + k * kAtOnce][column]);
+}
+
+// Sixteen rows of the tile (numbers 16 r to 16 r + 15 of its columns), 32 columns from 32 c on: a lane has
+// row 16 r + l % 16, columns 32 c + 8 (l / 16) to + 7.
+template <int kTile>
+__device__ inline h8 turned_eight(const Tile<kTile>& tile, int r, int c) {
+    const int lane = threadIdx.x & 63, i = lane & 15;
+    const _Float16* from = &tile[32 * c + 8 * (lane >> 4) + (i >> 2)][16 * r + 4 * (i & 3)];
+    const u2 a = read_transposed(reinterpret_cast<const uint16_t*>(from)), b = read_transposed(reinterpret_cast<const uint16_t*>(from + 4 * (kTile + 8)));
+    return __builtin_bit_cast(h8, u4{a.x, a.y, b.x, b.y});
+}
+
+// To an array whose rows are the tile's rows.
+template <int kTile>
+__device__ inline void put_turned(const Tile<kTile>& tile, _Float16* to, int64_t stride) {
+    const int wave = wave_of_workgroup(), lane = threadIdx.x & 63;
+#pragma unroll 4
+    for (int k = 0; k < kTile / 16 * (kTile / 32) / 4; ++k) {
+        const int n = 4 * k + wave, r = n / (kTile / 32), c = n % (kTile / 32);
+        *reinterpret_cast<h8*>(to + (16 * r + (lane & 15)) * stride + 32 * c + 8 * (lane >> 4)) = turned_eight<kTile>(tile, r, c);
+    }
+}
+
+// Eight numbers `step` apart, those of `count` that there are.
+__device__ inline void put_eight(_Float16* to, int64_t step, h8 x, int count) {
+    if (step == 1 && count >= 8 && reinterpret_cast<uintptr_t>(to) % 16 == 0) {
+        *reinterpret_cast<h8*>(to) = x;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < count) to[i * step] = x[i];
+    }
+}
+
+// Both for results of 16 bits at any address, the first `rows` of the array's rows, `columns` of its columns.
+template <int kTile>
+__device__ inline void put_straight_to(const Tile<kTile>& tile, _Float16* to, int64_t stride, int rows, int columns) {
+    constexpr int kAcross = kTile / 8, kAtOnce = 256 / kAcross;
+    const int column = threadIdx.x % kAcross * 8;
+    for (int i = threadIdx.x / kAcross; i < rows; i += kAtOnce)
+        put_eight(to + i * stride + column, 1, *reinterpret_cast<const h8*>(&tile[i][column]), columns - column);
+}
+
+template <int kTile>
+__device__ inline void put_turned_to(const Tile<kTile>& tile, _Float16* to, int64_t stride, int64_t step, int rows, int columns) {
+    const int wave = wave_of_workgroup(), lane = threadIdx.x & 63;
+    for (int n = wave; n < kTile / 16 * (kTile / 32); n += 4) {
+        const int row = n / (kTile / 32) * 16 + (lane & 15), column = n % (kTile / 32) * 32 + 8 * (lane >> 4);
+        const h8 x = turned_eight<kTile>(tile, n / (kTile / 32), n % (kTile / 32));  // (by all lanes)
+        if (row < rows) put_eight(to + row * stride + column * step, step, x, columns - column);
+    }
+}
+
+// Tiles of one of the three products, kTile x kTile a workgroup, a quarter a wave. Four stages of 32
+// numbers along the contracted axis are on their way or in LDS; a wave reads the operands of the
+// next 16 while it multiplies those it has.
 template <int kTile, int kPlanes16, int kMode>
-__global__ __launch_bounds__(kTile * 2) void newton_product_kernel(Params P) {
-    constexpr int kThreads = kTile * 2, kAcross = kTile / 64;  // waves side by side (two down)
-    constexpr int kDown = kTile / 64;                          // results of 32 x 32 of a wave: down, and two across
+__global__ __launch_bounds__(256, kTile == 256 ? 1 : kTile == 128 ? 2 : 4) void newton_product_kernel(Params P) {
+    constexpr int kEach = kTile / 64;          // results of 32 x 32 of a wave, down and across
+    constexpr int kLoads = 2 * kTile / 64;     // of a lane for a stage
     constexpr bool kSymmetric = kMode == kGram || kMode == kPoly;
-    __shared__ __attribute__((aligned(16))) _Float16 lds[2][2][kTile * kDepth];
+    extern __shared__ __attribute__((aligned(16))) char lds_bytes[];
+    auto& lds = *reinterpret_cast<_Float16 (*)[kStages][2][kTile * kDepth]>(lds_bytes);
     const int wave = wave_of_workgroup(), lane = threadIdx.x & 63;
     // Workgroups go round the 8 XCDs in turn: each XCD takes a run of tiles.
     const int each = (P.tiles + 7) / 8, at = static_cast<int>(blockIdx.x % 8) * each + static_cast<int>(blockIdx.x / 8);
     if (static_cast<int>(blockIdx.x / 8) >= each || at >= P.tiles) return;
     const Matrix& x = P.matrix[matrix_of(P, at, [](const Matrix& y) { return y.first_tile; })];
+    const Parts<kPlanes16> w(P, x, kTile);
     int tile_row, tile_col;
     {
         const int n = at - x.first_tile;
@@ -186,125 +341,170 @@ __global__ __launch_bounds__(kTile * 2) void newton_product_kernel(Params P) {
             tile_col = j;
             tile_row = n - j * (j + 1) / 2;
         } else {  // all rows of tiles of a column after the other: P is read again, X once
-            const int down = x.M / kTile;
+            const int down = w.M / kTile;
             tile_col = n / down;
             tile_row = n % down;
         }
     }
-    const int64_t size = static_cast<int64_t>(x.M) * x.N, square = static_cast<int64_t>(x.M) * x.M;
-    const _Float16* turned = x.turned + P.current * 2 * size;
-    const int depth = kMode == kGram ? x.N : x.M;
-    const _Float16* left = kMode == kGram ? x.rows : kMode == kPoly ? x.gram : x.poly;
-    const _Float16* right = kMode == kGram ? x.rows : kMode == kPoly ? x.gram : turned;
+    const int64_t size = w.size, square = w.square;
+    const _Float16* turned = w.turned + P.current * 2 * size;
+    const int depth = kMode == kGram ? w.N : w.M;
+    const _Float16* left = kMode == kGram ? w.rows : kMode == kPoly ? w.gram : w.poly;
+    const _Float16* right = kMode == kGram ? w.rows : kMode == kPoly ? w.gram : turned;
     const int64_t left_plane = kMode == kGram ? size : square, right_plane = kMode == kPoly ? square : size;
     left += static_cast<int64_t>(tile_row) * kTile * depth;
     right += static_cast<int64_t>(tile_col) * kTile * depth;
-    const int steps = depth / kDepth, all = (kPlanes16 == 2 ? 3 : 1) * steps;
+    const int steps = depth / kDepth, all = (kPlanes16 == 2 ? 3 : 1) * steps;  // (at least four)
     const auto load = [&](int step, int buffer) {  // the smallest products first
         const int term = kPlanes16 == 2 ? step / steps : 2, k = kPlanes16 == 2 ? step % steps : step;
-        stage<kTile, kThreads>(left + (term == 0 ? left_plane : 0) + k * kDepth, depth, lds[buffer][0]);
-        stage<kTile, kThreads>(right + (term == 1 ? right_plane : 0) + k * kDepth, depth, lds[buffer][1]);
+        stage<kTile>(left + (term == 0 ? left_plane : 0) + k * kDepth, depth, lds[buffer][0]);
+        stage<kTile>(right + (term == 1 ? right_plane : 0) + k * kDepth, depth, lds[buffer][1]);
     };
-    const int row0 = wave / kAcross * (kTile / 2), col0 = wave % kAcross * 64;  // the wave's in the tile
-    f16x16 sum[kDown][2];
+    const int row0 = (wave >> 1) * (kTile / 2), col0 = (wave & 1) * (kTile / 2);  // the wave's in the tile
+    const auto read = [&](int buffer, int k, h8 (&a)[kEach], h8 (&b)[kEach]) {
+        const int piece = ((2 * k + (lane >> 5)) ^ place_of_row(lane & 31)) * 8;
 #pragma unroll
-    for (int i = 0; i < kDown; ++i)
+        for (int i = 0; i < kEach; ++i) {
+            a[i] = *reinterpret_cast<const h8*>(&lds[buffer][0][(row0 + 32 * i + (lane & 31)) * kDepth + piece]);
+            b[i] = *reinterpret_cast<const h8*>(&lds[buffer][1][(col0 + 32 * i + (lane & 31)) * kDepth + piece]);
+        }
+    };
+    f16x16 sum[kEach][kEach];
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+    for (int i = 0; i < kEach; ++i)
+#pragma unroll
+        for (int j = 0; j < kEach; ++j)
 #pragma unroll
             for (int s = 0; s < 16; ++s) sum[i][j][s] = 0.0f;
-    load(0, 0);
+    const auto multiply = [&](const h8 (&a)[kEach], const h8 (&b)[kEach], int from, int to) {
+#pragma unroll
+        for (int i = from; i < to; ++i)
+#pragma unroll
+            for (int j = 0; j < kEach; ++j) sum[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i], b[j], sum[i][j], 0, 0, 0);
+    };
+    h8 a[2][kEach], b[2][kEach];
+#pragma unroll
+    for (int s = 0; s < kStages; ++s) load(s, s);
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((kStages - 1) * kLoads) : "memory");
+    read(0, 0, a[0], b[0]);
     for (int step = 0; step < all; ++step) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        multiply(a[0], b[0], 0, 1);  // (these operands have come: nothing else is waited for)
+        __builtin_amdgcn_sched_barrier(0);
+        read(step % kStages, 1, a[1], b[1]);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(a[0], b[0], 1, kEach);
+        __builtin_amdgcn_sched_barrier(0);
+        // This stage has been read by all waves (each waits for what it read), the next has come for all:
+        // two more may be on their way. (Past the end the last stage comes again, unused.)
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((kStages - 2) * kLoads) : "memory");
+        load(step + kStages < all ? step + kStages : all - 1, step % kStages);
+        read((step + 1) % kStages, 0, a[0], b[0]);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(a[1], b[1], 0, kEach);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    // (nothing comes into LDS any more)
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    auto& tile = *reinterpret_cast<Tile<kTile>*>(lds_bytes);
+    const int64_t first_row = static_cast<int64_t>(tile_row) * kTile, first_col = static_cast<int64_t>(tile_col) * kTile;
+    // A lane has column l % 32 of each 32 x 32, rows 8 q + 4 (l / 32) to + 3: f(their place in the tile, their sums).
+    const auto each_four = [&](auto f) {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+#pragma unroll
+            for (int j = 0; j < kEach; ++j)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    f4 v = {sum[i][j][4 * q], sum[i][j][4 * q + 1], sum[i][j][4 * q + 2], sum[i][j][4 * q + 3]};
+                    f(row0 + 32 * i + 8 * q + 4 * (lane >> 5), col0 + 32 * j + (lane & 31), v);
+#pragma unroll
+                    for (int s = 0; s < 4; ++s) sum[i][j][4 * q + s] = v[s];
+                }
+    };
+    // Adds a factor (of each row) times a tile of an array whose rows are the tile's columns.
+    const auto add_tile = [&](const _Float16* from, int64_t stride, auto factor) {
+        get_tile<kTile>(tile, from + first_col * stride + first_row, stride);
         __syncthreads();
-        if (step + 1 < all) load(step + 1, (step + 1) & 1);
-        const _Float16* l = lds[step & 1][0];
-        const _Float16* r = lds[step & 1][1];
+        each_four([&](int row, int col, f4& v) { v += factor(row) * __builtin_convertvector(*reinterpret_cast<const h4*>(&tile[col][row]), f4); });
+        __syncthreads();
+    };
+    // What the sums round to, into the tile; they keep the rest.
+    const auto put_rounded = [&] {
+        each_four([&](int row, int col, f4& v) {
+            const h4 hi = __builtin_convertvector(v, h4);
+            *reinterpret_cast<h4*>(&tile[col][row]) = hi;
+            v -= __builtin_convertvector(hi, f4);
+        });
+        __syncthreads();
+    };
+    if constexpr (kSymmetric) {
+        _Float16* to = kMode == kGram ? w.gram : w.poly;
+        const float scale = kMode == kGram ? kScaleA / (w.scale * w.scale) : P.c / kScaleA;
+        each_four([&](int, int, f4& v) { v *= scale; });
+        if constexpr (kMode == kPoly) {
 #pragma unroll
-        for (int k = 0; k < kDepth / 16; ++k) {
-            const int piece = ((2 * k + (lane >> 5)) ^ (lane & 7)) * 8;
-            h8 a[kDown], b[2];
+            for (int plane = kPlanes16 - 1; plane >= 0; --plane) add_tile(w.gram + plane * square, w.M, [&](int) { return P.b; });
+            if (tile_row == tile_col)
+                each_four([&](int row, int col, f4& v) {
 #pragma unroll
-            for (int i = 0; i < kDown; ++i) a[i] = *reinterpret_cast<const h8*>(&l[(row0 + 32 * i + (lane & 31)) * kDepth + piece]);
+                    for (int s = 0; s < 4; ++s)
+                        if (row + s == col) {
+                            w.diagonal[first_col + col] = P.a + v[s] * (1.0f / kScaleA);
+                            v[s] = 0.0f;
+                        }
+                });
+        }
 #pragma unroll
-            for (int j = 0; j < 2; ++j) b[j] = *reinterpret_cast<const h8*>(&r[(col0 + 32 * j + (lane & 31)) * kDepth + piece]);
+        for (int plane = 0; plane < kPlanes16; ++plane) {
+            put_rounded();
+            put_straight<kTile>(tile, to + plane * square + first_col * w.M + first_row, w.M);
+            if (tile_row != tile_col) put_turned<kTile>(tile, to + plane * square + first_row * w.M + first_col, w.M);
+            if (plane + 1 < kPlanes16) __syncthreads();
+        }
+    } else {
+        each_four([&](int, int, f4& v) { v *= 1.0f / kScaleA; });
 #pragma unroll
-            for (int i = 0; i < kDown; ++i)
+        for (int plane = 1; plane >= 0; --plane)
+            add_tile(turned + plane * size, w.M, [&](int row) { return *reinterpret_cast<const f4*>(w.diagonal + first_row + row); });
+        if constexpr (kMode == kApply) {
+            _Float16* next = w.turned + (1 - P.current) * 2 * size;
 #pragma unroll
-                for (int j = 0; j < 2; ++j) sum[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i], b[j], sum[i][j], 0, 0, 0);
+            for (int plane = 0; plane < 2; ++plane) {
+                put_rounded();
+                put_straight<kTile>(tile, next + plane * size + first_col * w.M + first_row, w.M);
+                if (plane < kPlanes16) put_turned<kTile>(tile, w.rows + plane * size + first_row * w.N + first_col, w.N);
+                if (plane == 0) __syncthreads();
+            }
+        } else {
+            const float scale = 1.0f / w.scale;
+            const int rows = static_cast<int>(x.m - first_row < kTile ? x.m - first_row : kTile);
+            const int cols = static_cast<int>(x.n - first_col < kTile ? x.n - first_col : kTile);
+            const int64_t down = x.to_stride[0], across = x.to_stride[1], base = first_row * down + first_col * across;
+            if (x.to_dtype == NAVI_POLICY_F32) {
+                float* to = static_cast<float*>(x.to) + base;
+                each_four([&](int row, int col, f4& v) {
+#pragma unroll
+                    for (int s = 0; s < 4; ++s)
+                        if (row + s < rows && col < cols) to[(row + s) * down + col * across] = v[s] * scale;
+                });
+            } else {
+                each_four([&](int row, int col, f4& v) {
+                    h4 y;
+#pragma unroll
+                    for (int s = 0; s < 4; ++s)
+                        y[s] = x.to_dtype == NAVI_POLICY_F16 ? static_cast<_Float16>(v[s] * scale)
+                                                              : __builtin_bit_cast(_Float16, static_cast<__bf16>(v[s] * scale));
+                    *reinterpret_cast<h4*>(&tile[col][row]) = y;
+                });
+                __syncthreads();
+                _Float16* to = static_cast<_Float16*>(x.to) + base;
+                if (down == 1)
+                    put_straight_to<kTile>(tile, to, across, cols, rows);
+                else
+                    put_turned_to<kTile>(tile, to, down, across, rows, cols);
+            }
         }
     }
-    // A lane has column l % 32 of each 32 x 32, rows 8 q + 4 (l / 32) to + 3.
-    _Float16* next = x.turned + (1 - P.current) * 2 * size;
-#pragma unroll
-    for (int i = 0; i < kDown; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int row = tile_row * kTile + row0 + 32 * i + 8 * q + 4 * (lane >> 5), col = tile_col * kTile + col0 + 32 * j + (lane & 31);
-                f4 v = {sum[i][j][4 * q], sum[i][j][4 * q + 1], sum[i][j][4 * q + 2], sum[i][j][4 * q + 3]};
-                if constexpr (kSymmetric) {
-                    _Float16* to = kMode == kGram ? x.gram : x.poly;
-                    if constexpr (kMode == kGram) {
-                        v = v * (kScaleA / (x.scale * x.scale));
-                    } else {
-                        const h4 hi = *reinterpret_cast<const h4*>(x.gram + static_cast<int64_t>(col) * x.M + row);
-                        f4 g = __builtin_convertvector(hi, f4);
-                        if constexpr (kPlanes16 == 2)
-                            g += __builtin_convertvector(*reinterpret_cast<const h4*>(x.gram + square + static_cast<int64_t>(col) * x.M + row), f4);
-                        v = P.b * g + v * (P.c / kScaleA);
-#pragma unroll
-                        for (int s = 0; s < 4; ++s)
-                            if (row + s == col) {
-                                x.diagonal[col] = P.a + v[s] * (1.0f / kScaleA);
-                                v[s] = 0.0f;
-                            }
-                    }
-                    h4 hi, lo;
-#pragma unroll
-                    for (int s = 0; s < 4; ++s) {
-                        _Float16 h, r;
-                        split(v[s], h, r);
-                        hi[s] = h;
-                        lo[s] = r;
-                    }
-                    *reinterpret_cast<h4*>(to + static_cast<int64_t>(col) * x.M + row) = hi;
-                    if constexpr (kPlanes16 == 2) *reinterpret_cast<h4*>(to + square + static_cast<int64_t>(col) * x.M + row) = lo;
-                    if (tile_row != tile_col) {
-#pragma unroll
-                        for (int s = 0; s < 4; ++s) {
-                            to[static_cast<int64_t>(row + s) * x.M + col] = hi[s];
-                            if constexpr (kPlanes16 == 2) to[square + static_cast<int64_t>(row + s) * x.M + col] = lo[s];
-                        }
-                    }
-                } else {
-                    const int64_t back = static_cast<int64_t>(col) * x.M + row;
-                    const f4 own = __builtin_convertvector(*reinterpret_cast<const h4*>(turned + back), f4) +
-                                   __builtin_convertvector(*reinterpret_cast<const h4*>(turned + size + back), f4);
-                    v = *reinterpret_cast<const f4*>(x.diagonal + row) * own + v * (1.0f / kScaleA);
-                    if constexpr (kMode == kApply) {
-                        h4 hi, lo;
-#pragma unroll
-                        for (int s = 0; s < 4; ++s) {
-                            _Float16 h, r;
-                            split(v[s], h, r);
-                            hi[s] = h;
-                            lo[s] = r;
-                            const int64_t to = static_cast<int64_t>(row + s) * x.N + col;
-                            x.rows[to] = h;
-                            if constexpr (kPlanes16 == 2) x.rows[size + to] = r;
-                        }
-                        *reinterpret_cast<h4*>(next + back) = hi;
-                        *reinterpret_cast<h4*>(next + size + back) = lo;
-                    } else {
-#pragma unroll
-                        for (int s = 0; s < 4; ++s)
-                            if (row + s < x.m && col < x.n)
-                                store_any(x.to, x.to_dtype, (row + s) * x.to_stride[0] + col * x.to_stride[1], v[s] / x.scale);
-                    }
-                }
-            }
 }
 
 int launched() {
@@ -316,19 +516,22 @@ int launched() {
 
 int64_t rounded(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
-// Matrices of few tiles take smaller ones: with 256 x 256 a CU holds one workgroup, whose waves have
-// twice the products for what they read.
+// The largest tiles that leave every CU one (256 x 256: a CU holds one workgroup, whose waves have twice the
+// products for what they read of 128's; 64 for matrices of a small policy).
 int tile_of(const navi_orthogonalize_matrix* x, int count) {
-    int64_t tiles = 0;
-    for (int i = 0; i < count; ++i) tiles += ((x[i].rows + 255) / 256) * ((x[i].cols + 255) / 256);
-    return tiles >= 256 ? 256 : 128;
+    for (const int tile : {256, 128}) {
+        int64_t tiles = 0;
+        for (int i = 0; i < count; ++i) tiles += ((x[i].rows + tile - 1) / tile) * ((x[i].cols + tile - 1) / tile);
+        if (tiles >= 256) return tile;
+    }
+    return 64;
 }
 
 int planes_of(const navi_orthogonalize_matrix& x) { return x.to_dtype == NAVI_POLICY_BF16 ? 1 : 2; }
 
 int64_t bytes_of(const navi_orthogonalize_matrix& x, int tile, int planes) {
     const int64_t M = rounded(std::min(x.rows, x.cols), tile), N = rounded(std::max(x.rows, x.cols), tile);
-    return 2 * (planes * M * N + 4 * M * N + 2 * planes * M * M) + rounded(4 * M, 256) + 8 * kNormBlocks;
+    return 8 * kNormBlocks + 4 * M + 2 * (planes * M * N + 4 * M * N + 2 * planes * M * M);  // (a multiple of 256: M is one of 64)
 }
 
 // Matrices from `at` on that go together: of one number of planes, as many as a launch names and the
@@ -401,28 +604,36 @@ int check_apart(const navi_orthogonalize_matrix* x, int count) {
     return NAVI_POLICY_OK;
 }
 
+template <int kTile, int kPlanes16, int kMode>
+int launch(const Params& P, hipStream_t stream) {
+    constexpr int staged = kStages * 2 * kTile * kDepth * sizeof(_Float16), tile = sizeof(Tile<kTile>), lds = staged > tile ? staged : tile;
+    const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void*>(newton_product_kernel<kTile, kPlanes16, kMode>),
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (err != hipSuccess) return set_error(NAVI_POLICY_E_LAUNCH, "navi_orthogonalize: %s", hipGetErrorString(err));
+    hipLaunchKernelGGL((newton_product_kernel<kTile, kPlanes16, kMode>), dim3((P.tiles + 7) / 8 * 8), dim3(256), lds, stream, P);
+    return launched();
+}
+
 template <int kTile, int kPlanes16>
-int run_group(Params& P, int squares_rows, int pieces, int steps, hipStream_t stream) {
-    hipLaunchKernelGGL(newton_squares_kernel, dim3(kNormBlocks, squares_rows), dim3(256), 0, stream, P);
+int run_group(Params& P, int pieces, int steps, hipStream_t stream) {
+    hipLaunchKernelGGL(newton_squares_kernel, dim3(kNormBlocks, P.count), dim3(256), 0, stream, P);
     hipLaunchKernelGGL(newton_begin_kernel<kPlanes16>, dim3(pieces), dim3(256), 0, stream, P);
     Params S = P, X = P;  // tiles of the symmetric products, and of the other
     S.tiles = X.tiles = 0;
     for (int i = 0; i < P.count; ++i) {
-        const int down = P.matrix[i].M / kTile, across = P.matrix[i].N / kTile;
+        const int down = (P.matrix[i].m + kTile - 1) / kTile, across = (P.matrix[i].n + kTile - 1) / kTile;
         S.matrix[i].first_tile = S.tiles;
         X.matrix[i].first_tile = X.tiles;
         S.tiles += down * (down + 1) / 2;
         X.tiles += down * across;
     }
-    const dim3 symmetric((S.tiles + 7) / 8 * 8), whole((X.tiles + 7) / 8 * 8), threads(kTile * 2);
     for (int step = 0; step < steps; ++step) {
         S.current = X.current = step & 1;
-        hipLaunchKernelGGL((newton_product_kernel<kTile, kPlanes16, kGram>), symmetric, threads, 0, stream, S);
-        hipLaunchKernelGGL((newton_product_kernel<kTile, kPlanes16, kPoly>), symmetric, threads, 0, stream, S);
-        if (step + 1 < steps)
-            hipLaunchKernelGGL((newton_product_kernel<kTile, kPlanes16, kApply>), whole, threads, 0, stream, X);
-        else
-            hipLaunchKernelGGL((newton_product_kernel<kTile, kPlanes16, kLast>), whole, threads, 0, stream, X);
+        int code = launch<kTile, kPlanes16, kGram>(S, stream);
+        if (code == NAVI_POLICY_OK) code = launch<kTile, kPlanes16, kPoly>(S, stream);
+        if (code == NAVI_POLICY_OK)
+            code = step + 1 < steps ? launch<kTile, kPlanes16, kApply>(X, stream) : launch<kTile, kPlanes16, kLast>(X, stream);
+        if (code != NAVI_POLICY_OK) return code;
     }
     return launched();
 }
@@ -465,8 +676,10 @@ extern "C" int navi_orthogonalize(int32_t count, const navi_orthogonalize_matrix
         P.b = b;
         P.c = c;
         P.eps = eps;
+        P.workspace = static_cast<char*>(workspace);
+        P.tile = tile;
         int planes = 1, pieces = 0;
-        char* place = static_cast<char*>(workspace);
+        int64_t place = 0;
         for (; at < end; ++at) {
             const navi_orthogonalize_matrix& given = matrices[at];
             if (given.rows == 0 || given.cols == 0) continue;
@@ -475,35 +688,28 @@ extern "C" int navi_orthogonalize(int32_t count, const navi_orthogonalize_matrix
             const int turn = given.rows > given.cols;  // X is the transpose
             x.from = given.from;
             x.to = given.to;
-            for (int k = 0; k < 2; ++k) {
-                x.from_stride[k] = given.from_stride[k ^ turn];
-                x.to_stride[k] = given.to_stride[k ^ turn];
-            }
+            x.turned = given.from_stride[1 ^ turn] != 1;
+            x.from_line = given.from_stride[x.turned ? 1 ^ turn : turn];
+            for (int k = 0; k < 2; ++k) x.to_stride[k] = given.to_stride[k ^ turn];
             x.m = static_cast<int32_t>(turn ? given.cols : given.rows);
             x.n = static_cast<int32_t>(turn ? given.rows : given.cols);
-            x.M = static_cast<int32_t>(rounded(x.m, tile));
-            x.N = static_cast<int32_t>(rounded(x.n, tile));
-            x.from_dtype = given.from_dtype;
-            x.to_dtype = given.to_dtype;
-            x.scale = std::exp2(std::round(std::log2(std::sqrt(static_cast<float>(x.n)))) + 6.0f);
+            x.from_dtype = static_cast<int8_t>(given.from_dtype);
+            x.to_dtype = static_cast<int8_t>(given.to_dtype);
+            x.scale = static_cast<int8_t>(std::lround(0.5 * std::log2(static_cast<double>(x.n)))) + 6;
             x.first_piece = pieces;
-            pieces += x.M / 64 * (x.N / 64);
-            const int64_t size = static_cast<int64_t>(x.M) * x.N, square = static_cast<int64_t>(x.M) * x.M;
-            x.rows = reinterpret_cast<_Float16*>(place);
-            x.turned = x.rows + planes * size;
-            x.gram = x.turned + 4 * size;
-            x.poly = x.gram + planes * square;
-            x.diagonal = reinterpret_cast<float*>(x.poly + planes * square);
-            x.squares = reinterpret_cast<double*>(reinterpret_cast<char*>(x.diagonal) + rounded(4 * static_cast<int64_t>(x.M), 256));
-            place = reinterpret_cast<char*>(x.squares + kNormBlocks);
+            pieces += static_cast<int>(rounded(x.m, tile) / 64 * (rounded(x.n, tile) / 64));
+            x.place = static_cast<uint32_t>(place / 256);
+            place += bytes_of(given, tile, planes);
         }
         if (P.count == 0) continue;
         hipStream_t on = as_stream(stream);
         int result;
         if (tile == 256)
-            result = planes == 1 ? run_group<256, 1>(P, P.count, pieces, steps, on) : run_group<256, 2>(P, P.count, pieces, steps, on);
+            result = planes == 1 ? run_group<256, 1>(P, pieces, steps, on) : run_group<256, 2>(P, pieces, steps, on);
+        else if (tile == 128)
+            result = planes == 1 ? run_group<128, 1>(P, pieces, steps, on) : run_group<128, 2>(P, pieces, steps, on);
         else
-            result = planes == 1 ? run_group<128, 1>(P, P.count, pieces, steps, on) : run_group<128, 2>(P, P.count, pieces, steps, on);
+            result = planes == 1 ? run_group<64, 1>(P, pieces, steps, on) : run_group<64, 2>(P, pieces, steps, on);
         if (result != NAVI_POLICY_OK) return result;
     }
     return NAVI_POLICY_OK;
