@@ -31,7 +31,6 @@ using f16x16 = float __attribute__((ext_vector_type(16)));
 constexpr int kMatrices = 62;       // of a launch: its arguments stay under 4 KiB
 constexpr int kNormBlocks = 64;     // workgroups that sum a matrix's squares
 constexpr int kDepth = 32;          // of a product's stage
-constexpr int kStages = 4;          // in LDS at once
 constexpr float kScaleA = 1024.0f;  // of A and P
 constexpr int64_t kGroupBytes = int64_t{4} << 30;  // of workspace that matrices in one launch share
 
@@ -315,16 +314,21 @@ __device__ inline void put_turned_to(const Tile<kTile>& tile, _Float16* to, int6
     }
 }
 
-// Tiles of one of the three products, kTile x kTile a workgroup, a quarter a wave. Four stages of 32
-// numbers along the contracted axis are on their way or in LDS; a wave reads the operands of the
-// next 16 while it multiplies those it has.
+// Stages in LDS at once: as many as 128 KB hold, four at most.
+template <int kTile, int kPlanes16>
+inline constexpr int kStages = kTile * kPlanes16 <= 256 ? 4 : 2;
+
+// Tiles of one of the three products, kTile x kTile a workgroup, a quarter a wave. Two or four stages of 32
+// numbers along the contracted axis, of all planes, are on their way or in LDS; a wave reads the operands of
+// the next 16 while it multiplies those it has.
 template <int kTile, int kPlanes16, int kMode>
-__global__ __launch_bounds__(256, kTile == 256 ? 1 : kTile == 128 ? 2 : 4) void newton_product_kernel(Params P) {
+__global__ __launch_bounds__(256, kTile == 256 ? 1 : kTile == 128 && kPlanes16 == 2 ? 1 : 2) void newton_product_kernel(Params P) {
     constexpr int kEach = kTile / 64;          // results of 32 x 32 of a wave, down and across
-    constexpr int kLoads = 2 * kTile / 64;     // of a lane for a stage
+    constexpr int kLoads = 2 * kPlanes16 * kTile / 64;  // of a lane for a stage
+    constexpr int kBuffers = kStages<kTile, kPlanes16>;
     constexpr bool kSymmetric = kMode == kGram || kMode == kPoly;
     extern __shared__ __attribute__((aligned(16))) char lds_bytes[];
-    auto& lds = *reinterpret_cast<_Float16 (*)[kStages][2][kTile * kDepth]>(lds_bytes);
+    auto& lds = *reinterpret_cast<_Float16 (*)[kBuffers][2][kPlanes16][kTile * kDepth]>(lds_bytes);
     const int wave = wave_of_workgroup(), lane = threadIdx.x & 63;
     // Workgroups go round the 8 XCDs in turn: each XCD takes a run of tiles.
     const int each = (P.tiles + 7) / 8, at = static_cast<int>(blockIdx.x % 8) * each + static_cast<int>(blockIdx.x / 8);
@@ -354,20 +358,25 @@ __global__ __launch_bounds__(256, kTile == 256 ? 1 : kTile == 128 ? 2 : 4) void 
     const int64_t left_plane = kMode == kGram ? size : square, right_plane = kMode == kPoly ? square : size;
     left += static_cast<int64_t>(tile_row) * kTile * depth;
     right += static_cast<int64_t>(tile_col) * kTile * depth;
-    const int steps = depth / kDepth, all = (kPlanes16 == 2 ? 3 : 1) * steps;  // (at least four)
-    const auto load = [&](int step, int buffer) {  // the smallest products first
-        const int term = kPlanes16 == 2 ? step / steps : 2, k = kPlanes16 == 2 ? step % steps : step;
-        stage<kTile>(left + (term == 0 ? left_plane : 0) + k * kDepth, depth, lds[buffer][0]);
-        stage<kTile>(right + (term == 1 ? right_plane : 0) + k * kDepth, depth, lds[buffer][1]);
+    const int steps = depth / kDepth;  // (at least two)
+    const auto load = [&](int step, int buffer) {
+#pragma unroll
+        for (int n = 0; n < kPlanes16; ++n) {
+            stage<kTile>(left + n * left_plane + step * kDepth, depth, lds[buffer][0][n]);
+            stage<kTile>(right + n * right_plane + step * kDepth, depth, lds[buffer][1][n]);
+        }
     };
     const int row0 = (wave >> 1) * (kTile / 2), col0 = (wave & 1) * (kTile / 2);  // the wave's in the tile
-    const auto read = [&](int buffer, int k, h8 (&a)[kEach], h8 (&b)[kEach]) {
+    using Operand = h8[kPlanes16][kEach];
+    const auto read = [&](int buffer, int k, Operand& a, Operand& b) {
         const int piece = ((2 * k + (lane >> 5)) ^ place_of_row(lane & 31)) * 8;
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            a[i] = *reinterpret_cast<const h8*>(&lds[buffer][0][(row0 + 32 * i + (lane & 31)) * kDepth + piece]);
-            b[i] = *reinterpret_cast<const h8*>(&lds[buffer][1][(col0 + 32 * i + (lane & 31)) * kDepth + piece]);
-        }
+        for (int n = 0; n < kPlanes16; ++n)
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+                a[n][i] = *reinterpret_cast<const h8*>(&lds[buffer][0][n][(row0 + 32 * i + (lane & 31)) * kDepth + piece]);
+                b[n][i] = *reinterpret_cast<const h8*>(&lds[buffer][1][n][(col0 + 32 * i + (lane & 31)) * kDepth + piece]);
+            }
     };
     f16x16 sum[kEach][kEach];
 #pragma unroll
@@ -376,29 +385,33 @@ __global__ __launch_bounds__(256, kTile == 256 ? 1 : kTile == 128 ? 2 : 4) void 
         for (int j = 0; j < kEach; ++j)
 #pragma unroll
             for (int s = 0; s < 16; ++s) sum[i][j][s] = 0.0f;
-    const auto multiply = [&](const h8 (&a)[kEach], const h8 (&b)[kEach], int from, int to) {
+    // Rows of results from `from` to `to`, the smallest products first.
+    const auto multiply = [&](const Operand& a, const Operand& b, int from, int to) {
 #pragma unroll
-        for (int i = from; i < to; ++i)
+        for (int term = 2 * (kPlanes16 - 1); term >= 0; --term)
 #pragma unroll
-            for (int j = 0; j < kEach; ++j) sum[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i], b[j], sum[i][j], 0, 0, 0);
+            for (int i = from; i < to; ++i)
+#pragma unroll
+                for (int j = 0; j < kEach; ++j)
+                    sum[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[term == 2][i], b[term == 1][j], sum[i][j], 0, 0, 0);
     };
-    h8 a[2][kEach], b[2][kEach];
+    Operand a[2], b[2];
 #pragma unroll
-    for (int s = 0; s < kStages; ++s) load(s, s);
-    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((kStages - 1) * kLoads) : "memory");
+    for (int s = 0; s < kBuffers; ++s) load(s < steps ? s : steps - 1, s);
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((kBuffers - 1) * kLoads) : "memory");
     read(0, 0, a[0], b[0]);
-    for (int step = 0; step < all; ++step) {
+    for (int step = 0; step < steps; ++step) {
         multiply(a[0], b[0], 0, 1);  // (these operands have come: nothing else is waited for)
         __builtin_amdgcn_sched_barrier(0);
-        read(step % kStages, 1, a[1], b[1]);
+        read(step % kBuffers, 1, a[1], b[1]);
         __builtin_amdgcn_sched_barrier(0);
         multiply(a[0], b[0], 1, kEach);
         __builtin_amdgcn_sched_barrier(0);
-        // This stage has been read by all waves (each waits for what it read), the next has come for all:
-        // two more may be on their way. (Past the end the last stage comes again, unused.)
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((kStages - 2) * kLoads) : "memory");
-        load(step + kStages < all ? step + kStages : all - 1, step % kStages);
-        read((step + 1) % kStages, 0, a[0], b[0]);
+        // This stage has been read by all waves (each waits for what it read), the next has come for all;
+        // those after it may be on their way. (Past the end the last stage comes again, unused.)
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((kBuffers - 2) * kLoads) : "memory");
+        load(step + kBuffers < steps ? step + kBuffers : steps - 1, step % kBuffers);
+        read((step + 1) % kBuffers, 0, a[0], b[0]);
         __builtin_amdgcn_sched_barrier(0);
         multiply(a[1], b[1], 0, kEach);
         __builtin_amdgcn_sched_barrier(0);
@@ -606,7 +619,7 @@ int check_apart(const navi_orthogonalize_matrix* x, int count) {
 
 template <int kTile, int kPlanes16, int kMode>
 int launch(const Params& P, hipStream_t stream) {
-    constexpr int staged = kStages * 2 * kTile * kDepth * sizeof(_Float16), tile = sizeof(Tile<kTile>), lds = staged > tile ? staged : tile;
+    constexpr int staged = kStages<kTile, kPlanes16> * 2 * kPlanes16 * kTile * kDepth * sizeof(_Float16), tile = sizeof(Tile<kTile>), lds = staged > tile ? staged : tile;
     const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void*>(newton_product_kernel<kTile, kPlanes16, kMode>),
                                                hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (err != hipSuccess) return set_error(NAVI_POLICY_E_LAUNCH, "navi_orthogonalize: %s", hipGetErrorString(err));
