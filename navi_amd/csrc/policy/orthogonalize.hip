@@ -40,15 +40,13 @@ struct Matrix {
     int64_t from_line;      // elements between X's rows, or (`turned`) its columns; those along them lie side by side
     int64_t to_stride[2];   // of X's rows and columns
     int32_t m, n;           // X
-    int32_t first_tile, first_piece;  // of those of all matrices
     uint32_t place;         // in the workspace, 256 bytes
     int8_t from_dtype, to_dtype, turned;
     int8_t scale;           // X times two to this
 };
-static_assert(sizeof(Matrix) == 64, "a launch's arguments");
-
 struct Params {
     Matrix matrix[kMatrices];
+    int32_t first[kMatrices];  // of a launch's tiles (or pieces) of all matrices
     char* workspace;
     int32_t count, tiles;
     int32_t tile;      // M and N are m and n rounded up to it
@@ -160,18 +158,11 @@ __global__ __launch_bounds__(256) void newton_squares_kernel(Params P) {
     if (threadIdx.x == 0) Parts<1>(P, x, P.tile).squares[blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]);
 }
 
-// The last matrix whose first tile (or piece) is not after `at`.
-template <class F>
-__device__ inline int matrix_of(const Params& P, int at, F first) {
-    int lo = 0, hi = P.count - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) / 2;
-        if (first(P.matrix[mid]) <= at)
-            lo = mid;
-        else
-            hi = mid - 1;
-    }
-    return lo;
+// The matrix that tile (or piece) `at` of a launch is of: the last whose first is not after it, each lane
+// looking at one (arguments come from the host's memory: a search would wait for them several times).
+__device__ inline int matrix_of(const Params& P, int at) {
+    const int lane = threadIdx.x & 63;
+    return __builtin_amdgcn_readfirstlane(__popcll(__ballot(lane < P.count && P.first[lane < kMatrices ? lane : 0] <= at)) - 1);
 }
 
 __device__ inline void split(float x, _Float16& hi, _Float16& lo) {
@@ -183,10 +174,10 @@ __device__ inline void split(float x, _Float16& hi, _Float16& lo) {
 template <int kPlanes16>
 __global__ __launch_bounds__(256) void newton_begin_kernel(Params P) {
     __shared__ float tile[64][65];
-    const int at = blockIdx.x, index = matrix_of(P, at, [](const Matrix& x) { return x.first_piece; });
+    const int at = blockIdx.x, index = matrix_of(P, at);
     const Matrix& x = P.matrix[index];
     const Parts<kPlanes16> w(P, x, P.tile);
-    const int piece = at - x.first_piece, across = w.N / 64, row0 = piece / across * 64, col0 = piece % across * 64;
+    const int piece = at - P.first[index], across = w.N / 64, row0 = piece / across * 64, col0 = piece % across * 64;
     const int lane = threadIdx.x & 63, wave = wave_of_workgroup();
     double sum = w.squares[lane];
 #pragma unroll
@@ -333,11 +324,12 @@ __global__ __launch_bounds__(256, kTile == 256 ? 1 : kTile == 128 && kPlanes16 =
     // Workgroups go round the 8 XCDs in turn: each XCD takes a run of tiles.
     const int each = (P.tiles + 7) / 8, at = static_cast<int>(blockIdx.x % 8) * each + static_cast<int>(blockIdx.x / 8);
     if (static_cast<int>(blockIdx.x / 8) >= each || at >= P.tiles) return;
-    const Matrix& x = P.matrix[matrix_of(P, at, [](const Matrix& y) { return y.first_tile; })];
+    const int index = matrix_of(P, at);
+    const Matrix& x = P.matrix[index];
     const Parts<kPlanes16> w(P, x, kTile);
     int tile_row, tile_col;
     {
-        const int n = at - x.first_tile;
+        const int n = at - P.first[index];
         if (kSymmetric) {  // tiles (i, j) with i <= j, a column of tiles after the other
             int j = static_cast<int>((sqrtf(8.0f * n + 1.0f) - 1.0f) * 0.5f);
             while ((j + 1) * (j + 2) / 2 <= n) ++j;
@@ -635,8 +627,8 @@ int run_group(Params& P, int pieces, int steps, hipStream_t stream) {
     S.tiles = X.tiles = 0;
     for (int i = 0; i < P.count; ++i) {
         const int down = (P.matrix[i].m + kTile - 1) / kTile, across = (P.matrix[i].n + kTile - 1) / kTile;
-        S.matrix[i].first_tile = S.tiles;
-        X.matrix[i].first_tile = X.tiles;
+        S.first[i] = S.tiles;
+        X.first[i] = X.tiles;
         S.tiles += down * (down + 1) / 2;
         X.tiles += down * across;
     }
@@ -709,7 +701,7 @@ extern "C" int navi_orthogonalize(int32_t count, const navi_orthogonalize_matrix
             x.from_dtype = static_cast<int8_t>(given.from_dtype);
             x.to_dtype = static_cast<int8_t>(given.to_dtype);
             x.scale = static_cast<int8_t>(std::lround(0.5 * std::log2(static_cast<double>(x.n)))) + 6;
-            x.first_piece = pieces;
+            P.first[P.count - 1] = pieces;
             pieces += static_cast<int>(rounded(x.m, tile) / 64 * (rounded(x.n, tile) / 64));
             x.place = static_cast<uint32_t>(place / 256);
             place += bytes_of(given, tile, planes);
