@@ -1,4 +1,5 @@
-"""ctypes binding of ``libnavi_policy.so`` (the C ABI declared in ``include/policy/navi_policy.h``).
+"""ctypes binding of ``libnavi_policy.so`` (the C ABI declared in ``include/policy/navi_policy.h``),
+and ``calls``, the extension that makes calls of one frame of it (``csrc/policy/calls.cpp``).
 
 Importing this module loads the HIP library and raises ``ImportError`` when it has not been
 built; there is no fallback.
@@ -7,12 +8,17 @@ built; there is no fallback.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 import struct
 from pathlib import Path
 
+import torch  # noqa: F401  (the extension's libraries)
+
 LIB_DIR = Path(__file__).resolve().parent / "_lib"
 LIB_PATH = Path(os.environ.get("NAVI_POLICY_LIB", LIB_DIR / "libnavi_policy.so"))
+CALLS_PATH = LIB_DIR / "_policy_calls.so"
 
 NAVI_POLICY_OK = 0
 NAVI_POLICY_E_ARG = -1
@@ -24,11 +30,12 @@ NORM_PARTIALS = 2048
 MAX_TAPS, MAX_BLOCK_WIDTH, MAX_STATE_DIM = 4, 8192, 128
 ACT_NONE, ACT_SILU = 0, 1
 
-if not LIB_PATH.exists():
-    raise ImportError(
-        f"libnavi_policy.so not found at {LIB_PATH}; build it with "
-        "`python -c 'import __graft_entry__ as g; g.build()'` (or `make -C navi_amd/csrc/policy`)."
-    )
+for _path in (LIB_PATH, CALLS_PATH):
+    if not _path.exists():
+        raise ImportError(
+            f"{_path.name} not found at {_path}; build it with "
+            "`python -c 'import __graft_entry__ as g; g.build()'` (or `make -C navi_amd/csrc/policy`)."
+        )
 _lib = ctypes.CDLL(str(LIB_PATH))
 
 _vp, _i32, _i64, _f32 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float
@@ -138,6 +145,17 @@ _lib.navi_orthogonalize_workspace.restype = _i64
 _lib.navi_orthogonalize_workspace.argtypes = [_i32, _vp]
 _lib.navi_clip_grad_norm.restype = ctypes.c_int
 _lib.navi_clip_grad_norm.argtypes = [_i32, _vp, _vp, _vp, _vp, _f32, _f32, _vp, _vp, _vp]
+
+
+def _load_calls():
+    loader = importlib.machinery.ExtensionFileLoader("_policy_calls", str(CALLS_PATH))
+    module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_policy_calls", loader))
+    module.bind(*[ctypes.cast(getattr(_lib, name), _vp).value
+                  for name in ("navi_selective_step", "navi_causal_conv", "navi_block_norm")])
+    return module
+
+
+calls = _load_calls()
 
 
 def lib() -> ctypes.CDLL:

@@ -36,7 +36,10 @@ _DTYPES = {torch.float32: _native.F32, torch.bfloat16: _native.BF16, torch.float
 _MASKS = (torch.bool, torch.uint8)
 
 # Arguments are looked over twice: `_fine` in one expression on every call (a call of one frame
-# is bound by the host), and by name, for the message, where that found something.
+# is bound by the host), and by name, for the message, where that found something. Where a call of
+# one frame or of a few rows takes the device less time than its arguments take Python, the
+# extension `_native.calls` makes it whole, if it is in order and asks for no gradients; a call that
+# it leaves (None) goes the way below.
 
 
 def _check(cond: bool, msg: str) -> None:
@@ -72,6 +75,13 @@ def _call(function, device: torch.device, *args) -> None:
             code = function(*args, torch._C._cuda_getCurrentRawStream(index))
     if code:
         _native.check(code)
+
+
+def _done(result):
+    """What the extension returned: outputs, or the code of an entry point that refused."""
+    if type(result) is int:
+        _native.check(result)
+    return result
 
 
 def _ptr(t) -> int:
@@ -643,6 +653,10 @@ def selective_scan_step(x: torch.Tensor, dt: torch.Tensor, a: torch.Tensor, b: t
     may be ``x`` itself. Autograd is told of both writes: what has saved either raises backward.
     No gradients: this is the form for acting.
     """
+    if forward_ad._current_level < 0:
+        done = _native.calls.selective_step(x, dt, a, b, c, state, d, dt_bias, starts, out)
+        if done is not None:
+            return _done(done)
     _check_scan(x, dt, a, b, c, d, dt_bias, starts, ("Envs",))
     _check_scan_state("state", state, x, b)
     written = [state]
@@ -813,6 +827,11 @@ def causal_conv_step(x: torch.Tensor, weight: torch.Tensor, window: torch.Tensor
     ``out`` (like ``x``, contiguous) if given, which shares no memory with the inputs but may be
     ``x`` itself. Autograd is told of both writes. No gradients: this is the form for acting.
     """
+    if forward_ad._current_level < 0:
+        number = 0 if activation is None else 1 if type(activation) is str and activation == "silu" else None
+        done = _native.calls.conv_step(x, weight, window, bias, starts, number, out)
+        if done is not None:
+            return _done(done)
     _check_conv(x, weight, bias, starts, activation, ("Envs",))
     _check_window("window", window, x, weight)
     written = [window]
@@ -935,8 +954,12 @@ def block_norm(y: torch.Tensor, residual: torch.Tensor, *, gate: torch.Tensor | 
     ``scale``, ``post_weight``, ``pre_weight``: ``[Width]`` float32. Returns ``stream`` like
     ``residual`` and ``normed`` like ``y``; ``normed`` is that of the sum before it is rounded.
     """
-    _check_block(y, residual, gate, scale, post_weight, pre_weight)
     eps = float(eps)
+    if 0.0 <= eps < math.inf and forward_ad._current_level < 0:
+        done = _native.calls.block_norm(y, residual, gate, scale, post_weight, pre_weight, eps)
+        if done is not None:
+            return _done(done)
+    _check_block(y, residual, gate, scale, post_weight, pre_weight)
     _check(math.isfinite(eps) and eps >= 0.0, "eps must be finite and not negative")
     inputs = (y, residual, gate, scale, post_weight, pre_weight)
     _check_tangents(*inputs)
