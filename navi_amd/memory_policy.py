@@ -12,6 +12,11 @@ command is one rollout of every actor, traced by ``bench_sdfdag``'s harness: whi
 ``gated_delta_step`` carries a state per actor, an actor that collides begins a new episode;
 then ``gated_delta_rule`` reads the whole rollout with gradients, from the state at its
 beginning, and ``clip_grad_norm`` bounds the update.
+
+``SelectivePolicy`` (``--core selective``) is the same with a selective state space scan behind a
+short convolution as its core (the reference's Mamba-2 cores are of this kind), and ``block_norm``
+between the blocks of its residual stream. ``MatrixUpdates`` (``--optimizer orthogonal``) steps the
+weight matrices by orthogonalised momenta.
 """
 
 from __future__ import annotations
@@ -83,6 +88,138 @@ class MemoryPolicy(torch.nn.Module):
         return self._output(policy.gated_delta_step(q, k, v, g, beta, state, starts=starts), h)
 
 
+class SelectiveBlock(torch.nn.Module):
+    """A short convolution, a selective scan and what stands after them in a residual stream; both
+    a window of inputs and a state are carried from frame to frame."""
+
+    def __init__(self, width: int, heads: int, head_dim: int, groups: int, state_dim: int, taps: int, dtype, device) -> None:
+        super().__init__()
+        self.dims, self.dtype = (heads, head_dim, groups, state_dim), dtype
+        self.inner, self.shared = heads * head_dim, groups * state_dim
+        self.taps, self.channels = taps, self.inner + 2 * self.shared
+        self.project = torch.nn.Linear(width, self.channels + width, bias=False, device=device)
+        self.steps = torch.nn.Linear(width, heads, bias=False, device=device)
+        self.merge = torch.nn.Linear(self.inner, width, bias=False, device=device)
+        vector = lambda *values: torch.nn.Parameter(torch.tensor(values, device=device))  # noqa: E731
+        self.taps_weight = torch.nn.Parameter(torch.randn(self.channels, taps, device=device) * taps ** -0.5)
+        self.taps_bias = vector(*[0.0] * self.channels)
+        self.rate = vector(*[-0.5 * 2.0 ** (h % 6) for h in range(heads)])
+        self.skip = vector(*[1.0] * heads)
+        self.step_bias = vector(*[-2.0] * heads)  # softplus of it: 0.13 of a step
+        self.scale, self.post, self.pre = (vector(*[v] * width) for v in (0.5, 1.0, 1.0))
+
+    def initial_state(self, actors: int) -> tuple[torch.Tensor, torch.Tensor]:
+        heads, head_dim, _, state_dim = self.dims
+        return (torch.zeros(actors, self.taps - 1, self.channels, dtype=self.dtype, device=self.scale.device),
+                torch.zeros(actors, heads, state_dim, head_dim, device=self.scale.device))
+
+    def _parts(self, y: torch.Tensor):
+        """x, b and c: views of the convolution's output."""
+        heads, head_dim, groups, state_dim = self.dims
+        x, b, c = y.split((self.inner, self.shared, self.shared), dim=-1)
+        return (x.unflatten(-1, (heads, head_dim)), *(t.unflatten(-1, (groups, state_dim)) for t in (b, c)))
+
+    def _after(self, o: torch.Tensor, gate: torch.Tensor, stream: torch.Tensor):
+        y = self.merge(o.flatten(-2).float()).to(self.dtype)
+        return policy.block_norm(y, stream, gate=gate, scale=self.scale, post_weight=self.post, pre_weight=self.pre)
+
+    def forward(self, normed, stream, starts, state):
+        """Rollouts ``[Actors, Steps, Width]``: the stream after the block and its norm."""
+        window, memory = (None, None) if state is None else state
+        taken, gate = self.project(normed.float()).to(self.dtype).split((self.channels, stream.shape[-1]), dim=-1)
+        taken = policy.causal_conv(taken, self.taps_weight, bias=self.taps_bias, starts=starts, initial_window=window)
+        x, b, c = self._parts(taken)
+        o = policy.selective_scan(x, self.steps(normed.float()), -self.rate.abs(), b, c, d=self.skip, dt_bias=self.step_bias,
+                                  starts=starts, initial_state=memory)
+        return self._after(o, gate, stream)
+
+    def act(self, normed, stream, starts, state):
+        """One frame ``[Actors, Width]``; the state is updated in place."""
+        window, memory = state
+        taken, gate = self.project(normed.float()).to(self.dtype).split((self.channels, stream.shape[-1]), dim=-1)
+        taken = policy.causal_conv_step(taken, self.taps_weight, window, bias=self.taps_bias, starts=starts)
+        x, b, c = self._parts(taken)
+        o = policy.selective_scan_step(x, self.steps(normed.float()), -self.rate.abs(), b, c, memory, d=self.skip,
+                                       dt_bias=self.step_bias, starts=starts)
+        return tuple(t.squeeze(1) for t in self._after(o[:, None], gate[:, None], stream[:, None]))
+
+
+class SelectivePolicy(torch.nn.Module):
+    """As ``MemoryPolicy``, with blocks of a selective scan; the state of each block is two tensors."""
+
+    def __init__(self, inputs: int = POOL[0] * POOL[1], width: int = 256, heads: int = 4, head_dim: int = 64, groups: int = 1,
+                 state_dim: int = 64, taps: int = 4, blocks: int = 2, dtype: torch.dtype = torch.bfloat16, device="cuda") -> None:
+        super().__init__()
+        self.dtype = dtype
+        self.encode = torch.nn.Linear(inputs, width, device=device)
+        self.blocks = torch.nn.ModuleList(
+            SelectiveBlock(width, heads, head_dim, groups, state_dim, taps, dtype, device) for _ in range(blocks))
+        self.predict = torch.nn.Linear(width, inputs, device=device)
+
+    def initial_state(self, actors: int) -> tuple[torch.Tensor, ...]:
+        return tuple(t for block in self.blocks for t in block.initial_state(actors))
+
+    def forward(self, x, starts, positions=None, state=None):
+        """Rollouts, as ``MemoryPolicy.forward`` (places in the episode are not read)."""
+        stream = F.gelu(self.encode(x))
+        normed = stream.to(self.dtype)
+        for i, block in enumerate(self.blocks):
+            stream, normed = block(normed, stream, starts, None if state is None else state[2 * i:2 * i + 2])
+        return self.predict(normed.float())
+
+    @torch.no_grad()
+    def act(self, x, starts, positions, state):
+        """One frame, as ``MemoryPolicy.act``."""
+        stream = F.gelu(self.encode(x))
+        normed = stream.to(self.dtype)
+        for i, block in enumerate(self.blocks):
+            stream, normed = block.act(normed, stream, starts, state[2 * i:2 * i + 2])
+        return self.predict(normed.float())
+
+
+class MatrixUpdates:
+    """An optimizer: weight matrices are stepped by their orthogonalised momenta, all of them in one
+    call, the other parameters by Adam. A matrix's step has the root-mean-square of ``lr * 0.2`` whatever its
+    shape (an orthogonalised ``m x n`` matrix has ``1 / sqrt(max(m, n))``)."""
+
+    def __init__(self, parameters, lr: float = 1e-3, momentum: float = 0.95) -> None:
+        parameters = list(parameters)
+        self.matrices = [p for p in parameters if p.dim() == 2]
+        others = [p for p in parameters if p.dim() != 2]
+        self.adam = torch.optim.Adam(others, lr=lr) if others else None
+        self.lr, self.momentum = lr, momentum
+        self.held = [torch.zeros_like(p) for p in self.matrices]
+        self.updates = [torch.empty_like(p, dtype=torch.bfloat16) for p in self.matrices]
+
+    def zero_grad(self, set_to_none: bool = True) -> None:
+        for p in self.matrices:
+            p.grad = None if set_to_none or p.grad is None else p.grad.zero_()
+        if self.adam is not None:
+            self.adam.zero_grad(set_to_none=set_to_none)
+
+    @torch.no_grad()
+    def step(self) -> None:
+        at = [i for i, p in enumerate(self.matrices) if p.grad is not None]
+        if at:
+            held, updates = [self.held[i] for i in at], [self.updates[i] for i in at]
+            torch._foreach_lerp_(held, [self.matrices[i].grad for i in at], 1.0 - self.momentum)
+            policy.orthogonalize(held, out=updates)
+            for i, update in zip(at, updates):
+                p = self.matrices[i]
+                p.add_(update, alpha=-0.2 * self.lr * max(p.shape) ** 0.5)
+        if self.adam is not None:
+            self.adam.step()
+
+
+CORES = {"delta": MemoryPolicy, "selective": SelectivePolicy}
+OPTIMIZERS = {"adam": torch.optim.Adam, "orthogonal": MatrixUpdates}
+
+
+def copied(state):
+    """A copy of a policy's state, a tensor or several."""
+    return tuple(t.clone() for t in state) if isinstance(state, tuple) else state.clone()
+
+
 class Rollout:
     """One rollout's frames, episode starts and places, and the state before it (None before the first)."""
 
@@ -91,10 +228,10 @@ class Rollout:
         self.starts = torch.zeros(actors, steps + 1, dtype=torch.bool, device=device)
         self.positions = torch.zeros(actors, steps + 1, dtype=torch.int32, device=device)
         self.acted = torch.empty(actors, steps, inputs, device=device)
-        self.state: torch.Tensor | None = None
+        self.state: torch.Tensor | tuple[torch.Tensor, ...] | None = None
 
 
-def collect(harness, model: MemoryPolicy, rollout: Rollout, state: torch.Tensor, starts: torch.Tensor,
+def collect(harness, model: torch.nn.Module, rollout: Rollout, state, starts: torch.Tensor,
             positions: torch.Tensor) -> None:
     """Steps every actor through a rollout; ``state`` (before the rollout's last frame), ``starts`` and
     ``positions`` (of that frame) are carried on in place. The last frame is only predicted: the next
@@ -105,7 +242,7 @@ def collect(harness, model: MemoryPolicy, rollout: Rollout, state: torch.Tensor,
         rollout.frames[:, 0] = features(harness.obs[:, 0])
     else:
         rollout.frames[:, 0] = rollout.frames[:, steps]
-    rollout.state = state.clone()
+    rollout.state = copied(state)
     rollout.starts[:, 0], rollout.positions[:, 0] = starts, positions
     for t in range(steps):
         rollout.acted[:, t] = model.act(rollout.frames[:, t], starts, positions, state)
@@ -116,7 +253,7 @@ def collect(harness, model: MemoryPolicy, rollout: Rollout, state: torch.Tensor,
         rollout.starts[:, t + 1], rollout.positions[:, t + 1] = starts, positions
 
 
-def learn(model: MemoryPolicy, optimizer, rollout: Rollout, max_norm: float) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+def learn(model: torch.nn.Module, optimizer, rollout: Rollout, max_norm: float) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """One update over a rollout: (loss, gradient norm, predictions)."""
     said = model(rollout.frames[:, :-1], rollout.starts[:, :-1], rollout.positions[:, :-1], rollout.state)
     same = ~rollout.starts[:, 1:, None]  # the next frame belongs to the episode
@@ -129,13 +266,15 @@ def learn(model: MemoryPolicy, optimizer, rollout: Rollout, max_norm: float) -> 
 
 
 def run(scenes, *, actors: int, steps: int, updates: int, azimuth_bins: int, elevation_bins: int, max_distance: float,
-        sdf_max_steps: int, seed: int, max_norm: float = 1.0, dtype: torch.dtype = torch.bfloat16) -> dict[str, Any]:
+        sdf_max_steps: int, seed: int, max_norm: float = 1.0, dtype: torch.dtype = torch.bfloat16, core: str = "delta",
+        optimizer: str = "adam") -> dict[str, Any]:
     from .bench_sdfdag import ObservationHarness
 
     torch.manual_seed(seed)
     harness = ObservationHarness(scenes, actors, azimuth_bins, elevation_bins, max_distance, sdf_max_steps, seed=seed)
-    model = MemoryPolicy(dtype=dtype, device=harness.dev, positions=updates * steps + 1)
-    optimizer = torch.optim.Adam(model.parameters(), lr=1e-3)
+    more = {"positions": updates * steps + 1} if core == "delta" else {}
+    model = CORES[core](dtype=dtype, device=harness.dev, **more)
+    stepper = OPTIMIZERS[optimizer](model.parameters(), lr=1e-3)
     state = model.initial_state(actors)
     starts = torch.ones(actors, dtype=torch.bool, device=harness.dev)
     positions = torch.zeros(actors, dtype=torch.int32, device=harness.dev)
@@ -147,7 +286,7 @@ def run(scenes, *, actors: int, steps: int, updates: int, azimuth_bins: int, ele
         collect(harness, model, rollout, state, starts, positions)
         torch.cuda.synchronize()
         collected = time.perf_counter()
-        loss, norm, said = learn(model, optimizer, rollout, max_norm)
+        loss, norm, said = learn(model, stepper, rollout, max_norm)
         torch.cuda.synchronize()
         act_ms.append((collected - began) * 1e3 / steps)
         learn_ms.append((time.perf_counter() - collected) * 1e3)
@@ -171,6 +310,8 @@ def main(argv: list[str] | None = None) -> int:
     ap.add_argument("--max-distance", type=float, default=30.0)
     ap.add_argument("--sdf-max-steps", type=int, default=256)
     ap.add_argument("--seed", type=int, default=0)
+    ap.add_argument("--core", choices=sorted(CORES), default="delta")
+    ap.add_argument("--optimizer", choices=sorted(OPTIMIZERS), default="adam")
     ap.add_argument("--json", action="store_true")
     args = ap.parse_args(argv)
     if min(args.actors, args.steps, args.updates) < 1:
@@ -186,10 +327,10 @@ def main(argv: list[str] | None = None) -> int:
         room = S.box_room()
         scenes = [(room.compile(), room.bbox_min, room.bbox_max)]
     summary = {"gmdag_file": [str(Path(f).expanduser()) for f in args.gmdag_file or []], "actors": args.actors,
-               "steps": args.steps, "updates": args.updates,
+               "steps": args.steps, "updates": args.updates, "core": args.core, "optimizer": args.optimizer,
                **run(scenes, actors=args.actors, steps=args.steps, updates=args.updates, azimuth_bins=args.azimuth_bins,
                      elevation_bins=args.elevation_bins, max_distance=args.max_distance,
-                     sdf_max_steps=args.sdf_max_steps, seed=args.seed)}
+                     sdf_max_steps=args.sdf_max_steps, seed=args.seed, core=args.core, optimizer=args.optimizer)}
     if args.json:
         print(json.dumps(summary, indent=2))
     else:
