@@ -1,5 +1,5 @@
 """ctypes binding of ``libnavi_policy.so`` (the C ABI declared in ``include/policy/navi_policy.h``),
-and ``calls``, the extension that makes calls of one frame of it (``csrc/policy/calls.cpp``).
+and ``calls``, the extension that makes calls of some of it in one step (``csrc/policy/calls.cpp``).
 
 Importing this module loads the HIP library and raises ``ImportError`` when it has not been
 built; there is no fallback.
@@ -151,7 +151,10 @@ def _load_calls():
     loader = importlib.machinery.ExtensionFileLoader("_policy_calls", str(CALLS_PATH))
     module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_policy_calls", loader))
     module.bind(*[ctypes.cast(getattr(_lib, name), _vp).value
-                  for name in ("navi_selective_step", "navi_causal_conv", "navi_block_norm")])
+                  for name in ("navi_selective_step", "navi_selective_scan", "navi_selective_scan_backward",
+                               "navi_selective_scan_scratch", "navi_selective_scan_workspace", "navi_causal_conv",
+                               "navi_causal_conv_backward", "navi_causal_conv_workspace", "navi_block_norm",
+                               "navi_block_norm_backward", "navi_block_norm_workspace", "navi_policy_last_error")])
     return module
 
 

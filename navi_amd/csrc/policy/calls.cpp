@@ -1,19 +1,28 @@
-// Calls of the policy's operators for a frame of every environment, from Python in one step: arguments looked
-// over, output allocated, launched, autograd told of the writes. On the device such a call takes a few
-// microseconds, a Python program's own reads of the tensors' shapes and strides three times that (a frame of one
-// environment: 14.8 us a call through ctypes; each function below states what it takes).
+// Calls of a block's operators (selective scan, convolution, norms) from Python, in one step: outputs and
+// workspaces allocated, structures filled, launched, autograd told of writes. On the device a frame of every
+// environment takes a few microseconds; a Python program's own reads of the tensors' shapes and strides, and its
+// filling of structures, take more (a frame of one environment: 14.8 us a call through ctypes, 5.2 here; a training
+// pass of a small scan, forward and backward: 201 us through ctypes and a function of Python's, 82 here).
 //
-// A function takes a call that is in order in every respect, and returns None for any other, with nothing done:
-// navi_amd/policy.py then says by name what is wrong, or goes the way that keeps gradients. So nothing is
-// refused here, and what is in order is what policy.py's `_fine_...` functions say.
+// selective_step, conv_step and block_norm look their arguments over too. They take a call that is in order in
+// every respect, and return None for any other, with nothing done: navi_amd/policy.py then says by name what is
+// wrong, or goes the way that keeps gradients. What is in order is what policy.py's `_fine_...` functions say. The
+// others are policy.py's calls of whole rollouts, of arguments that it has looked over, with their gradients.
 #define __HIP_PLATFORM_AMD__ 1  // (the host compiler reads HIP's headers)
 #include <Python.h>
 
+#include <cstring>
+#include <initializer_list>
+#include <optional>
+
 #include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "navi_policy.h"
@@ -21,14 +30,27 @@
 namespace {
 
 using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
 
-using Step = int (*)(const navi_selective_scan_args*, void*);
-using Conv = int (*)(const navi_causal_conv_args*, void*);
-using Block = int (*)(const navi_block_norm_args*, void*);
+// The library's entry points, in the order in which policy.py's binding gives their addresses.
+struct Entries {
+    int (*selective_step)(const navi_selective_scan_args*, void*);
+    int (*selective_scan)(const navi_selective_scan_args*, void*);
+    int (*selective_scan_backward)(const navi_selective_scan_args*, void*);
+    int64_t (*selective_scan_scratch)(const navi_selective_scan_args*);
+    int64_t (*selective_scan_workspace)(const navi_selective_scan_args*);
+    int (*causal_conv)(const navi_causal_conv_args*, void*);
+    int (*causal_conv_backward)(const navi_causal_conv_args*, void*);
+    int64_t (*causal_conv_workspace)(const navi_causal_conv_args*);
+    int (*block_norm)(const navi_block_norm_args*, void*);
+    int (*block_norm_backward)(const navi_block_norm_args*, void*);
+    int64_t (*block_norm_workspace)(const navi_block_norm_args*);
+    const char* (*last_error)(void);
+};
+constexpr Py_ssize_t kEntries = sizeof(Entries) / sizeof(void*);
 
-Step step_entry = nullptr;
-Conv conv_entry = nullptr;
-Block block_entry = nullptr;
+Entries entries{};
 
 // A tensor of a call. `fine` falls to false at the first that is neither a plain tensor nor, where that is
 // allowed, None.
@@ -93,19 +115,32 @@ bool stream_of(c10::Device device, void** stream) {
     return true;
 }
 
-template <typename Entry, typename Args> int launch(Entry entry, const Args& args, void* stream) {
-    int code;
-    Py_BEGIN_ALLOW_THREADS code = entry(&args, stream);
-    Py_END_ALLOW_THREADS return code;
+int64_t checked(int64_t code) {
+    TORCH_CHECK(code >= 0, entries.last_error());
+    return code;
 }
 
-// (an entry point's refusal is told by policy.py, which asks for its words)
-PyObject* refused(int code) { return PyLong_FromLong(code); }
+// (a backward pass runs in a thread of autograd's, which does not hold Python's lock)
+struct Unlocked {
+    PyThreadState* kept = PyGILState_Check() ? PyEval_SaveThread() : nullptr;
+    ~Unlocked() {
+        if (kept) PyEval_RestoreThread(kept);
+    }
+};
 
-// selective_step(x, dt, a, b, c, state, d, dt_bias, starts, out): the output, None or an entry point's code.
+template <typename Entry, typename Args> void launch(Entry entry, const Args& args, void* stream) {
+    int code;
+    {
+        const Unlocked unlocked;
+        code = entry(&args, stream);
+    }
+    checked(code);
+}
+
+// selective_step(x, dt, a, b, c, state, d, dt_bias, starts, out): the output, or None.
 PyObject* selective_step(PyObject*, PyObject* const* v, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    if (n != 10 || !step_entry) Py_RETURN_NONE;
+    if (n != 10 || !entries.selective_step) Py_RETURN_NONE;
     Call call;
     const Tensor *x = call.tensor(v[0]), *dt = call.tensor(v[1]), *a = call.tensor(v[2]), *b = call.tensor(v[3]),
                  *c = call.tensor(v[4]), *state = call.tensor(v[5]), *d = call.maybe(v[6]), *dt_bias = call.maybe(v[7]),
@@ -142,7 +177,7 @@ PyObject* selective_step(PyObject*, PyObject* const* v, Py_ssize_t n) {
     s.starts = read_of<uint8_t>(starts), s.starts_stride[0] = starts ? starts->stride(0) : 0;
     s.final_state = static_cast<float*>(at_of(state)), s.initial_state = s.final_state;
     s.out = at_of(&out);
-    if (const int code = launch(step_entry, s, stream)) return refused(code);
+    launch(entries.selective_step, s, stream);
     wrote(*state);
     if (!to) return THPVariable_Wrap(std::move(out));
     wrote(out);
@@ -151,10 +186,10 @@ PyObject* selective_step(PyObject*, PyObject* const* v, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// conv_step(x, weight, window, bias, starts, activation's number, out): the output, None or an entry point's code.
+// conv_step(x, weight, window, bias, starts, activation's number, out): the output, or None.
 PyObject* conv_step(PyObject*, PyObject* const* v, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    if (n != 7 || !conv_entry || !PyLong_CheckExact(v[5])) Py_RETURN_NONE;
+    if (n != 7 || !entries.causal_conv || !PyLong_CheckExact(v[5])) Py_RETURN_NONE;
     Call call;
     const Tensor *x = call.tensor(v[0]), *weight = call.tensor(v[1]), *window = call.tensor(v[2]), *bias = call.maybe(v[3]),
                  *starts = call.maybe(v[4]), *to = call.maybe(v[6]);
@@ -181,7 +216,7 @@ PyObject* conv_step(PyObject*, PyObject* const* v, Py_ssize_t n) {
     s.starts = read_of<uint8_t>(starts), s.starts_stride[0] = starts ? starts->stride(0) : 0;
     s.window_out = at_of(window), s.window = s.window_out;
     s.out = at_of(&out);
-    if (const int code = launch(conv_entry, s, stream)) return refused(code);
+    launch(entries.causal_conv, s, stream);
     wrote(*window);
     if (!to) return THPVariable_Wrap(std::move(out));
     wrote(out);
@@ -190,10 +225,10 @@ PyObject* conv_step(PyObject*, PyObject* const* v, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// block_norm(y, residual, gate, scale, post_weight, pre_weight, eps): both outputs, None or an entry point's code.
+// block_norm(y, residual, gate, scale, post_weight, pre_weight, eps): both outputs, or None.
 PyObject* block_norm(PyObject*, PyObject* const* v, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    if (n != 7 || !block_entry || !PyFloat_CheckExact(v[6])) Py_RETURN_NONE;
+    if (n != 7 || !entries.block_norm || !PyFloat_CheckExact(v[6])) Py_RETURN_NONE;
     Call call;
     const Tensor *y = call.tensor(v[0]), *residual = call.tensor(v[1]), *gate = call.maybe(v[2]), *scale = call.maybe(v[3]),
                  *post = call.maybe(v[4]), *pre = call.maybe(v[5]);
@@ -221,7 +256,7 @@ PyObject* block_norm(PyObject*, PyObject* const* v, Py_ssize_t n) {
     }
     s.scale = read_of<float>(scale), s.post_weight = read_of<float>(post), s.pre_weight = read_of<float>(pre);
     s.stream = at_of(&sum), s.normed = at_of(&normed);
-    if (const int code = launch(block_entry, s, stream)) return refused(code);
+    launch(entries.block_norm, s, stream);
     PyObject* pair = PyTuple_New(2);
     if (!pair) return nullptr;
     PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(std::move(sum)));
@@ -230,23 +265,368 @@ PyObject* block_norm(PyObject*, PyObject* const* v, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// bind(selective_step's, causal_conv's, block_norm's address): the library's entry points.
+// ---- whole rollouts and their gradients, of arguments that policy.py has looked over ----
+
+// Arguments: None is an undefined tensor.
+variable_list given(PyObject* const* v, size_t n) {
+    variable_list to(n);
+    for (size_t i = 0; i < n; i++)
+        if (v[i] != Py_None) {
+            TORCH_CHECK(THPVariable_Check(v[i]), "a tensor is expected");
+            to[i] = THPVariable_Unpack(v[i]);
+        }
+    return to;
+}
+
+template <typename T> const T* read_of(const Tensor& t) { return read_of<T>(t.defined() ? &t : nullptr); }
+
+template <typename T> T* write_of(const Tensor& t) { return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr; }
+
+template <size_t n> void strides_of(int64_t (&to)[n], const Tensor& t) {
+    for (size_t i = 0; i < n; i++) to[i] = t.defined() ? t.stride(int64_t(i)) : 0;
+}
+
+Tensor like(const Tensor& t) { return t.defined() ? empty_like(t, t.scalar_type()) : Tensor(); }
+
+// An input that may be left out, as autograd takes it.
+using Maybe = std::optional<Tensor>;
+
+Maybe maybe(const Tensor& t) { return t.defined() ? Maybe(t) : Maybe(); }
+
+Tensor or_none(const Maybe& t) { return t ? *t : Tensor(); }
+
+// The gradient of saved input i, if one is asked for (autograd counts the inputs that are there).
+Tensor like(const AutogradContext* ctx, const variable_list& saved, size_t i) {
+    size_t edge = 0;
+    for (size_t j = 0; j < i; j++) edge += saved[j].defined();
+    return saved[i].defined() && ctx->needs_input_grad(edge) ? like(saved[i]) : Tensor();
+}
+
+Tensor floats(const Tensor& of, int64_t bytes) {
+    return at::empty({bytes / 4}, of.options().dtype(at::kFloat).requires_grad(false));
+}
+
+// A gradient with its last axis dense; undefined stays so.
+Tensor dense(const Tensor& t) { return !t.defined() || dense_last(t) ? t : t.contiguous(); }
+
+// Steps that do not overlap and lie within the reach of the chunked kernels (policy.py's `_rows_apart`).
+Tensor rows_apart(const Tensor& t) {
+    constexpr int64_t farthest = INT32_MAX / NAVI_POLICY_CHUNK - (1 << 18);
+    if (t.size(1) <= 1 || (t.size(3) <= t.stride(1) && t.stride(1) <= farthest / int64_t(t.element_size()))) return t;
+    return t.contiguous();
+}
+
+// The device of a call is the current one during it: its stream.
+struct On {
+    c10::DeviceGuard guard;
+    void* stream;
+    explicit On(const Tensor& t) : guard(t.device()), stream(c10::hip::getCurrentHIPStream(t.device().index()).stream()) {}
+};
+
+// The gradients of a backward pass that itself is differentiated (create_graph): there are none of them, which is
+// an error where one is asked for, and no silence.
+variable_list once(AutogradContext* ctx, const variable_list& given,
+                   variable_list (*gradients)(AutogradContext*, const variable_list&)) {
+    variable_list grads;
+    {
+        c10::AutoGradMode off(false);
+        grads = gradients(ctx, given);
+    }
+    if (!c10::GradMode::is_enabled()) return grads;
+    for (Tensor& t : grads)
+        if (t.defined()) t.requires_grad_();
+    const auto fail = std::make_shared<torch::autograd::DelayedError>(
+        "the gradients of the policy's operators have no gradients of their own", int64_t(grads.size()));
+    return (*fail)(std::move(grads));
+}
+
+bool records(std::initializer_list<const Tensor*> inputs) {
+    if (c10::GradMode::is_enabled())
+        for (const Tensor* t : inputs)
+            if (t->defined() && t->requires_grad()) return true;
+    return false;
+}
+
+// One output, or the outputs as a tuple.
+PyObject* results(const variable_list& tensors) {
+    if (tensors.size() == 1) return THPVariable_Wrap(tensors[0]);
+    PyObject* tuple = PyTuple_New(Py_ssize_t(tensors.size()));
+    if (!tuple) throw python_error();
+    for (size_t i = 0; i < tensors.size(); i++) PyTuple_SET_ITEM(tuple, Py_ssize_t(i), THPVariable_Wrap(tensors[i]));
+    return tuple;
+}
+
+void count(Py_ssize_t n, Py_ssize_t want) { TORCH_CHECK(n == want && entries.last_error, "wrong number of arguments"); }
+
+struct Scan {
+    Tensor x, dt, a, b, c, d, dt_bias, state, starts;
+    explicit Scan(const variable_list& v)
+        : x(v[0]), dt(v[1]), a(v[2]), b(v[3]), c(v[4]), d(v[5]), dt_bias(v[6]), state(v[7]), starts(v[8]) {}
+    navi_selective_scan_args args() const {
+        navi_selective_scan_args s{};
+        s.dtype = type_of(x), s.heads = int32_t(x.size(2)), s.groups = int32_t(b.size(2)), s.state_dim = int32_t(b.size(3));
+        s.head_dim = int32_t(x.size(3)), s.envs = x.size(0), s.steps = x.size(1);
+        s.x = read_of<void>(x), s.b = read_of<void>(b), s.c = read_of<void>(c);
+        strides_of(s.x_stride, x), strides_of(s.b_stride, b), strides_of(s.c_stride, c);
+        s.dt = read_of<float>(dt), s.a = read_of<float>(a), s.d = read_of<float>(d), s.dt_bias = read_of<float>(dt_bias);
+        strides_of(s.dt_stride, dt);
+        s.starts = read_of<uint8_t>(starts), strides_of(s.starts_stride, starts);
+        s.initial_state = read_of<float>(state);
+        return s;
+    }
+    variable_list forward(bool return_state, bool stepwise) const {
+        const On on(x);
+        variable_list to{like(x)};
+        if (return_state)
+            to.push_back(at::empty({x.size(0), x.size(2), b.size(3), x.size(3)}, dt.options().requires_grad(false)));
+        auto s = args();
+        s.out = write_of<void>(to[0]), s.final_state = return_state ? write_of<float>(to[1]) : nullptr;
+        if (stepwise) {
+            launch(entries.selective_step, s, on.stream);
+            return to;
+        }
+        Tensor scratch;
+        if (const int64_t bytes = checked(entries.selective_scan_scratch(&s))) {
+            scratch = floats(x, bytes);
+            s.scratch = scratch.data_ptr();
+        }
+        launch(entries.selective_scan, s, on.stream);
+        return to;
+    }
+};
+
+struct ScanFunction : torch::autograd::Function<ScanFunction> {
+    static variable_list forward(AutogradContext* ctx, Tensor x, Tensor dt, Tensor a, Tensor b, Tensor c, Maybe d,
+                                 Maybe dt_bias, Maybe state, Maybe starts, bool return_state) {
+        const variable_list inputs{x, dt, a, b, c, or_none(d), or_none(dt_bias), or_none(state), or_none(starts)};
+        ctx->save_for_backward(inputs);
+        ctx->set_materialize_grads(false);
+        return Scan(inputs).forward(return_state, false);
+    }
+
+    static variable_list backward(AutogradContext* ctx, variable_list given) { return once(ctx, given, gradients); }
+
+    static variable_list gradients(AutogradContext* ctx, const variable_list& given) {
+        variable_list to(10);
+        Tensor grad = given[0], grad_state = given.size() > 1 ? given[1] : Tensor();
+        if (!grad.defined() && !grad_state.defined()) return to;
+        const variable_list saved = ctx->get_saved_variables();
+        const Scan g(saved);
+        const On on(g.x);
+        grad = grad.defined() ? rows_apart(dense(grad)) : like(g.x).zero_();
+        if (grad_state.defined()) grad_state = grad_state.contiguous();
+        Tensor d_x = like(g.x), d_dt = like(g.dt), d_b = like(g.b), d_c = like(g.c), d_a = like(ctx, saved, 2),
+               d_d = like(ctx, saved, 5), d_bias = like(ctx, saved, 6), d_state = like(ctx, saved, 7);
+        if (g.x.numel() == 0) {
+            for (Tensor t : {d_a, d_d, d_bias})
+                if (t.defined()) t.zero_();
+            if (d_state.defined()) grad_state.defined() ? d_state.copy_(grad_state) : d_state.zero_();
+        } else {
+            auto s = g.args();
+            s.grad_out = read_of<void>(grad), s.grad_final_state = read_of<float>(grad_state);
+            strides_of(s.grad_out_stride, grad);
+            s.d_x = write_of<void>(d_x), s.d_b = write_of<void>(d_b), s.d_c = write_of<void>(d_c), s.d_dt = write_of<float>(d_dt);
+            s.d_a = write_of<float>(d_a), s.d_d = write_of<float>(d_d), s.d_dt_bias = write_of<float>(d_bias);
+            s.d_initial_state = write_of<float>(d_state);
+            const Tensor workspace = floats(g.x, checked(entries.selective_scan_workspace(&s)));
+            s.workspace = workspace.data_ptr();
+            launch(entries.selective_scan_backward, s, on.stream);
+        }
+        return {d_x, d_dt, d_a, d_b, d_c, d_d, d_bias, d_state, Tensor(), Tensor()};
+    }
+};
+
+// scan(x, dt, a, b, c, d, dt_bias, initial_state, starts, return_state, stepwise): out, or (out, state).
+PyObject* scan(PyObject*, PyObject* const* v, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    count(n, 11);
+    const variable_list in = given(v, 9);
+    const bool return_state = v[9] == Py_True;
+    if (records({&in[0], &in[1], &in[2], &in[3], &in[4], &in[5], &in[6], &in[7]}))
+        return results(ScanFunction::apply(in[0], in[1], in[2], in[3], in[4], maybe(in[5]), maybe(in[6]), maybe(in[7]),
+                                           maybe(in[8]), return_state));
+    return results(Scan(in).forward(return_state, v[10] == Py_True));
+    END_HANDLE_TH_ERRORS
+}
+
+struct Convolution {
+    Tensor x, weight, bias, window, starts;
+    int64_t activation;
+    Convolution(const variable_list& v, int64_t activation)
+        : x(v[0]), weight(v[1]), bias(v[2]), window(v[3]), starts(v[4]), activation(activation) {}
+    navi_causal_conv_args args() const {
+        navi_causal_conv_args s{};
+        s.dtype = type_of(x), s.channels = int32_t(x.size(2)), s.taps = int32_t(weight.size(1));
+        s.activation = int32_t(activation), s.envs = x.size(0), s.steps = x.size(1);
+        s.x = read_of<void>(x), s.weight = read_of<float>(weight), s.bias = read_of<float>(bias);
+        strides_of(s.x_stride, x);
+        s.starts = read_of<uint8_t>(starts), strides_of(s.starts_stride, starts);
+        s.window = read_of<void>(window);
+        return s;
+    }
+    variable_list forward(bool return_window) const {
+        const On on(x);
+        variable_list to{like(x)};
+        if (return_window) to.push_back(at::empty({x.size(0), weight.size(1) - 1, x.size(2)}, x.options().requires_grad(false)));
+        auto s = args();
+        s.out = write_of<void>(to[0]), s.window_out = return_window ? write_of<void>(to[1]) : nullptr;
+        launch(entries.causal_conv, s, on.stream);
+        return to;
+    }
+};
+
+struct ConvolutionFunction : torch::autograd::Function<ConvolutionFunction> {
+    static variable_list forward(AutogradContext* ctx, Tensor x, Tensor weight, Maybe bias, Maybe window, Maybe starts,
+                                 int64_t activation, bool return_window) {
+        const variable_list inputs{x, weight, or_none(bias), or_none(window), or_none(starts)};
+        ctx->save_for_backward(inputs);
+        ctx->saved_data["activation"] = activation;
+        ctx->set_materialize_grads(false);
+        return Convolution(inputs, activation).forward(return_window);
+    }
+
+    static variable_list backward(AutogradContext* ctx, variable_list given) { return once(ctx, given, gradients); }
+
+    static variable_list gradients(AutogradContext* ctx, const variable_list& given) {
+        variable_list to(7);
+        Tensor grad = given[0], grad_window = given.size() > 1 ? given[1] : Tensor();
+        if (!grad.defined() && !grad_window.defined()) return to;
+        const variable_list saved = ctx->get_saved_variables();
+        const Convolution g(saved, ctx->saved_data["activation"].toInt());
+        const On on(g.x);
+        grad = grad.defined() ? dense(grad) : like(g.x).zero_();
+        if (grad_window.defined()) grad_window = grad_window.contiguous();
+        Tensor d_x = like(g.x), d_weight = like(ctx, saved, 1), d_bias = like(ctx, saved, 2),
+               d_window = like(ctx, saved, 3);
+        if (g.x.numel() == 0) {
+            for (Tensor t : {d_weight, d_bias})
+                if (t.defined()) t.zero_();
+            if (d_window.defined()) grad_window.defined() ? d_window.copy_(grad_window) : d_window.zero_();
+        } else {
+            auto s = g.args();
+            s.grad_out = read_of<void>(grad), s.grad_window = read_of<void>(grad_window);
+            strides_of(s.grad_out_stride, grad);
+            s.d_x = write_of<void>(d_x), s.d_weight = write_of<float>(d_weight), s.d_bias = write_of<float>(d_bias);
+            s.d_window = write_of<void>(d_window);
+            Tensor partial;
+            if (d_weight.defined() || d_bias.defined()) {
+                partial = floats(g.x, checked(entries.causal_conv_workspace(&s)));
+                s.partial = write_of<float>(partial);
+            }
+            launch(entries.causal_conv_backward, s, on.stream);
+        }
+        return {d_x, d_weight, d_bias, d_window, Tensor(), Tensor(), Tensor()};
+    }
+};
+
+// conv(x, weight, bias, window, starts, activation's number, return_window): out, or (out, window after).
+PyObject* conv(PyObject*, PyObject* const* v, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    count(n, 7);
+    const variable_list in = given(v, 5);
+    const int64_t activation = PyLong_AsLong(v[5]);
+    const bool return_window = v[6] == Py_True;
+    if (records({&in[0], &in[1], &in[2], &in[3]}))
+        return results(ConvolutionFunction::apply(in[0], in[1], maybe(in[2]), maybe(in[3]), maybe(in[4]), activation,
+                                                  return_window));
+    return results(Convolution(in, activation).forward(return_window));
+    END_HANDLE_TH_ERRORS
+}
+
+struct Between {
+    Tensor y, residual, gate, scale, post, pre;
+    double eps;
+    Between(const variable_list& v, double eps)
+        : y(v[0]), residual(v[1]), gate(v[2]), scale(v[3]), post(v[4]), pre(v[5]), eps(eps) {}
+    navi_block_norm_args args() const {
+        navi_block_norm_args s{};
+        s.dtype = type_of(y), s.stream_dtype = type_of(residual), s.width = int32_t(y.size(2)), s.eps = float(eps);
+        s.envs = y.size(0), s.steps = y.size(1);
+        s.y = read_of<void>(y), s.residual = read_of<void>(residual), s.gate = read_of<void>(gate);
+        strides_of(s.y_stride, y), strides_of(s.residual_stride, residual), strides_of(s.gate_stride, gate);
+        s.scale = read_of<float>(scale), s.post_weight = read_of<float>(post), s.pre_weight = read_of<float>(pre);
+        return s;
+    }
+    variable_list forward() const {
+        const On on(y);
+        variable_list to{empty_like(y, residual.scalar_type()), like(y)};
+        auto s = args();
+        s.stream = write_of<void>(to[0]), s.normed = write_of<void>(to[1]);
+        launch(entries.block_norm, s, on.stream);
+        return to;
+    }
+};
+
+struct BetweenFunction : torch::autograd::Function<BetweenFunction> {
+    static variable_list forward(AutogradContext* ctx, Tensor y, Tensor residual, Maybe gate, Maybe scale, Maybe post,
+                                 Maybe pre, double eps) {
+        const variable_list inputs{y, residual, or_none(gate), or_none(scale), or_none(post), or_none(pre)};
+        ctx->save_for_backward(inputs);
+        ctx->saved_data["eps"] = eps;
+        ctx->set_materialize_grads(false);
+        return Between(inputs, eps).forward();
+    }
+
+    static variable_list backward(AutogradContext* ctx, variable_list given) { return once(ctx, given, gradients); }
+
+    static variable_list gradients(AutogradContext* ctx, const variable_list& given) {
+        if (!given[0].defined() && !given[1].defined()) return variable_list(7);
+        const variable_list saved = ctx->get_saved_variables();
+        const Between g(saved, ctx->saved_data["eps"].toDouble());
+        const On on(g.y);
+        const Tensor grad_sum = dense(given[0]), grad_normed = dense(given[1]);
+        Tensor d_y = like(g.y), d_residual = like(g.residual), d_gate = like(ctx, saved, 2), d_scale = like(ctx, saved, 3),
+               d_post = like(ctx, saved, 4), d_pre = like(ctx, saved, 5);
+        if (g.y.numel() == 0) {
+            for (Tensor t : {d_scale, d_post, d_pre})
+                if (t.defined()) t.zero_();
+        } else {
+            auto s = g.args();
+            s.grad_stream = read_of<void>(grad_sum), s.grad_normed = read_of<void>(grad_normed);
+            strides_of(s.grad_stream_stride, grad_sum), strides_of(s.grad_normed_stride, grad_normed);
+            s.d_y = write_of<void>(d_y), s.d_residual = write_of<void>(d_residual), s.d_gate = write_of<void>(d_gate);
+            s.d_scale = write_of<float>(d_scale), s.d_post_weight = write_of<float>(d_post);
+            s.d_pre_weight = write_of<float>(d_pre);
+            Tensor partial;
+            if (d_scale.defined() || d_post.defined() || d_pre.defined()) {
+                partial = floats(g.y, checked(entries.block_norm_workspace(&s)));
+                s.partial = write_of<float>(partial);
+            }
+            launch(entries.block_norm_backward, s, on.stream);
+        }
+        return {d_y, d_residual, d_gate, d_scale, d_post, d_pre, Tensor()};
+    }
+};
+
+// block(y, residual, gate, scale, post_weight, pre_weight, eps): (stream, normed).
+PyObject* block(PyObject*, PyObject* const* v, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    count(n, 7);
+    const variable_list in = given(v, 6);
+    const double eps = PyFloat_AsDouble(v[6]);
+    if (records({&in[0], &in[1], &in[2], &in[3], &in[4], &in[5]}))
+        return results(BetweenFunction::apply(in[0], in[1], maybe(in[2]), maybe(in[3]), maybe(in[4]), maybe(in[5]), eps));
+    return results(Between(in, eps).forward());
+    END_HANDLE_TH_ERRORS
+}
+
+// bind(the library's entry points): their addresses in the order above.
 PyObject* bind(PyObject*, PyObject* const* v, Py_ssize_t n) {
-    if (n != 3) {
-        PyErr_SetString(PyExc_TypeError, "bind takes three addresses");
+    if (n != kEntries) {
+        PyErr_Format(PyExc_TypeError, "bind takes %zd addresses", kEntries);
         return nullptr;
     }
-    void* at[3];
-    for (int i = 0; i < 3; i++)
+    void* at[kEntries];
+    for (Py_ssize_t i = 0; i < n; i++)
         if (!(at[i] = PyLong_AsVoidPtr(v[i])) && PyErr_Occurred()) return nullptr;
-    step_entry = reinterpret_cast<Step>(at[0]);
-    conv_entry = reinterpret_cast<Conv>(at[1]);
-    block_entry = reinterpret_cast<Block>(at[2]);
+    static_assert(sizeof(at) == sizeof(entries), "addresses alone");
+    memcpy(&entries, at, sizeof(at));
     Py_RETURN_NONE;
 }
 
 #define METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {METHOD(bind), METHOD(selective_step), METHOD(conv_step), METHOD(block_norm), {nullptr, nullptr, 0, nullptr}};
+PyMethodDef methods[] = {METHOD(bind), METHOD(selective_step), METHOD(conv_step), METHOD(block_norm),
+                         METHOD(scan), METHOD(conv), METHOD(block), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_policy_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -39,7 +39,7 @@ _MASKS = (torch.bool, torch.uint8)
 # is bound by the host), and by name, for the message, where that found something. Where a call of
 # one frame or of a few rows takes the device less time than its arguments take Python, the
 # extension `_native.calls` makes it whole, if it is in order and asks for no gradients; a call that
-# it leaves (None) goes the way below.
+# it leaves (None) goes the way below. Allocation and launch of a block's operators are its work too.
 
 
 def _check(cond: bool, msg: str) -> None:
@@ -75,13 +75,6 @@ def _call(function, device: torch.device, *args) -> None:
             code = function(*args, torch._C._cuda_getCurrentRawStream(index))
     if code:
         _native.check(code)
-
-
-def _done(result):
-    """What the extension returned: outputs, or the code of an entry point that refused."""
-    if type(result) is int:
-        _native.check(result)
-    return result
 
 
 def _ptr(t) -> int:
@@ -534,74 +527,6 @@ def _check_scan_state(name: str, state, x, b) -> None:
     raise RuntimeError(f"{name} must be contiguous")
 
 
-def _pack_scan(x, dt, a, b, c, d, dt_bias, starts, initial_state, out, final_state, scratch=None, backward=(0,) * 14) -> bytes:
-    envs, steps, heads, head_dim = x.shape
-    groups, state_dim = b.shape[2:]
-    return _native.PACK_SCAN(
-        _DTYPES[x.dtype], heads, groups, state_dim, head_dim, envs, steps, x.data_ptr(), b.data_ptr(), c.data_ptr(),
-        *x.stride()[:3], *b.stride()[:3], *c.stride()[:3], dt.data_ptr(), *dt.stride(), a.data_ptr(), _ptr(d), _ptr(dt_bias),
-        *((0, 0, 0) if starts is None else (starts.data_ptr(), *starts.stride())), _ptr(initial_state), _ptr(out),
-        _ptr(final_state), _ptr(scratch), *backward)
-
-
-def _scan_forward(x, dt, a, b, c, d, dt_bias, starts, initial_state, return_state):
-    device = x.device
-    out = torch.empty(x.shape, dtype=x.dtype, device=device)
-    state = scratch = None
-    if return_state:
-        state = torch.empty((x.size(0), x.size(2), b.size(3), x.size(3)), dtype=torch.float32, device=device)
-    args = (x, dt, a, b, c, d, dt_bias, starts, initial_state, out, state)
-    packed, lib = _pack_scan(*args), _native.lib()
-    size = _native.check(lib.navi_selective_scan_scratch(packed))
-    if size:
-        scratch = torch.empty(size // 4, dtype=torch.float32, device=device)
-        packed = _pack_scan(*args, scratch)
-    _call(lib.navi_selective_scan, device, packed)
-    return out, state
-
-
-class _SelectiveScan(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, dt, a, b, c, d, dt_bias, initial_state, starts, return_state):
-        out, state = _scan_forward(x, dt, a, b, c, d, dt_bias, starts, initial_state, return_state)
-        ctx.save_for_backward(x, dt, a, b, c, d, dt_bias, initial_state, starts)
-        ctx.set_materialize_grads(False)
-        return (out, state) if return_state else out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_out, grad_state=None):
-        x, dt, a, b, c, d, dt_bias, initial_state, starts = ctx.saved_tensors
-        if grad_out is None and grad_state is None:
-            return (None,) * 10
-        if grad_out is None:
-            grad_out = torch.zeros(x.shape, dtype=x.dtype, device=x.device)
-        if not _dense_last(grad_out):  # (of a broadcast, for one)
-            grad_out = grad_out.contiguous()
-        grad_out = _rows_apart(grad_out)
-        if grad_state is not None:
-            grad_state = grad_state.contiguous()
-        need = ctx.needs_input_grad
-        d_state = torch.empty_like(initial_state) if initial_state is not None and need[7] else None
-        d_vectors = [torch.empty_like(t) if t is not None and need[i] else None for i, t in ((2, a), (5, d), (6, dt_bias))]
-        d_x, d_dt, d_b, d_c = (torch.empty(t.shape, dtype=t.dtype, device=x.device) for t in (x, dt, b, c))
-        if x.numel() == 0:
-            if d_state is not None:
-                d_state = torch.zeros_like(d_state) if grad_state is None else grad_state.clone()
-            for t in d_vectors:
-                if t is not None:
-                    t.zero_()
-        else:
-            lib = _native.lib()
-            args = (x, dt, a, b, c, d, dt_bias, starts, initial_state, None, None, None)
-            back = (grad_out.data_ptr(), *grad_out.stride()[:3], _ptr(grad_state), d_x.data_ptr(), d_b.data_ptr(), d_c.data_ptr(),
-                    d_dt.data_ptr(), *[_ptr(t) for t in d_vectors], _ptr(d_state))
-            size = _native.check(lib.navi_selective_scan_workspace(_pack_scan(*args, (*back, 0))))
-            workspace = torch.empty(size // 4, dtype=torch.float32, device=x.device)
-            _call(lib.navi_selective_scan_backward, x.device, _pack_scan(*args, (*back, workspace.data_ptr())))
-        return d_x, d_dt, d_vectors[0], d_b, d_c, d_vectors[1], d_vectors[2], d_state, None, None
-
-
 def selective_scan(x: torch.Tensor, dt: torch.Tensor, a: torch.Tensor, b: torch.Tensor, c: torch.Tensor, *,
                    d: torch.Tensor | None = None, dt_bias: torch.Tensor | None = None, starts: torch.Tensor | None = None,
                    initial_state: torch.Tensor | None = None, return_state: bool = False):
@@ -628,19 +553,10 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, a: torch.Tensor, b: torch.
     inputs = (x, dt, a, b, c, d, dt_bias, initial_state)
     _check_tangents(*inputs)
     grad = torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in inputs])
-    if not grad and x.size(1) <= _STEPWISE:  # (as for the gated delta rule)
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        state = None
-        if return_state:
-            state = torch.empty((x.size(0), x.size(2), b.size(3), x.size(3)), dtype=torch.float32, device=x.device)
-        _call(_native.lib().navi_selective_step, x.device,
-              _pack_scan(x, dt, a, b, c, d, dt_bias, starts, initial_state, out, state))
-        return (out, state) if return_state else out
-    x, b, c = _rows_apart(x), _rows_apart(b), _rows_apart(c)
-    if grad:
-        return _SelectiveScan.apply(x, dt, a, b, c, d, dt_bias, initial_state, starts, bool(return_state))
-    out, state = _scan_forward(x, dt, a, b, c, d, dt_bias, starts, initial_state, return_state)
-    return (out, state) if return_state else out
+    stepwise = not grad and x.size(1) <= _STEPWISE  # (as for the gated delta rule)
+    if not stepwise:
+        x, b, c = _rows_apart(x), _rows_apart(b), _rows_apart(c)
+    return _native.calls.scan(x, dt, a, b, c, d, dt_bias, initial_state, starts, bool(return_state), stepwise)
 
 
 def selective_scan_step(x: torch.Tensor, dt: torch.Tensor, a: torch.Tensor, b: torch.Tensor, c: torch.Tensor,
@@ -656,7 +572,7 @@ def selective_scan_step(x: torch.Tensor, dt: torch.Tensor, a: torch.Tensor, b: t
     if forward_ad._current_level < 0:
         done = _native.calls.selective_step(x, dt, a, b, c, state, d, dt_bias, starts, out)
         if done is not None:
-            return _done(done)
+            return done
     _check_scan(x, dt, a, b, c, d, dt_bias, starts, ("Envs",))
     _check_scan_state("state", state, x, b)
     written = [state]
@@ -731,65 +647,6 @@ def _check_window(name: str, window, x, weight) -> None:
     raise RuntimeError(f"{name} must be contiguous")
 
 
-def _pack_conv(x, weight, bias, starts, activation, window, out, window_out, backward=(0,) * 9) -> bytes:
-    envs, steps, channels = x.shape
-    return _native.PACK_CONV(
-        _DTYPES[x.dtype], channels, weight.size(1), _ACTIVATIONS[activation], envs, steps, x.data_ptr(), *x.stride()[:2],
-        weight.data_ptr(), _ptr(bias), *((0, 0, 0) if starts is None else (starts.data_ptr(), *starts.stride())),
-        _ptr(window), _ptr(out), _ptr(window_out), *backward)
-
-
-def _conv_forward(x, weight, bias, starts, activation, window, return_window):
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    after = torch.empty((x.size(0), weight.size(1) - 1, x.size(2)), dtype=x.dtype, device=x.device) if return_window else None
-    _call(_native.lib().navi_causal_conv, x.device, _pack_conv(x, weight, bias, starts, activation, window, out, after))
-    return out, after
-
-
-class _CausalConv(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, window, starts, activation, return_window):
-        ctx.save_for_backward(x, weight, bias, window, starts)
-        ctx.activation = activation
-        ctx.set_materialize_grads(False)
-        out, after = _conv_forward(x, weight, bias, starts, activation, window, return_window)
-        return (out, after) if return_window else out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_out, grad_window=None):
-        x, weight, bias, window, starts = ctx.saved_tensors
-        if grad_out is None and grad_window is None:
-            return (None,) * 7
-        if grad_out is None:
-            grad_out = torch.zeros((), dtype=x.dtype, device=x.device).expand(x.shape)
-        if not _dense_last(grad_out):
-            grad_out = grad_out.contiguous()
-        if grad_window is not None:
-            grad_window = grad_window.contiguous()
-        need = ctx.needs_input_grad
-        d_x = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        d_weight = torch.empty_like(weight) if need[1] else None
-        d_bias = torch.empty_like(bias) if bias is not None and need[2] else None
-        d_window = torch.empty_like(window) if window is not None and need[3] else None
-        if x.numel() == 0:
-            for t in (d_weight, d_bias):
-                if t is not None:
-                    t.zero_()
-            if d_window is not None:
-                d_window = torch.zeros_like(d_window) if grad_window is None else grad_window.clone()
-            return d_x, d_weight, d_bias, d_window, None, None, None
-        lib, partial = _native.lib(), None
-        args = (x, weight, bias, starts, ctx.activation, window, None, None)
-        if d_weight is not None or d_bias is not None:
-            size = _native.check(lib.navi_causal_conv_workspace(_pack_conv(*args)))
-            partial = torch.empty(size // 4, dtype=torch.float32, device=x.device)
-        _call(lib.navi_causal_conv_backward, x.device, _pack_conv(*args, (
-            grad_out.data_ptr(), *grad_out.stride()[:2], _ptr(grad_window), d_x.data_ptr(), _ptr(d_weight), _ptr(d_bias),
-            _ptr(d_window), _ptr(partial))))
-        return d_x, d_weight, d_bias, d_window, None, None, None
-
-
 def causal_conv(x: torch.Tensor, weight: torch.Tensor, *, bias: torch.Tensor | None = None,
                 starts: torch.Tensor | None = None, initial_window: torch.Tensor | None = None,
                 return_window: bool = False, activation: str | None = "silu"):
@@ -812,10 +669,7 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, *, bias: torch.Tensor | N
         _check_window("initial_window", initial_window, x, weight)
     inputs = (x, weight, bias, initial_window)
     _check_tangents(*inputs)
-    if torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in inputs]):
-        return _CausalConv.apply(*inputs, starts, activation, bool(return_window))
-    out, after = _conv_forward(x, weight, bias, starts, activation, initial_window, return_window)
-    return (out, after) if return_window else out
+    return _native.calls.conv(*inputs, starts, _ACTIVATIONS[activation], bool(return_window))
 
 
 def causal_conv_step(x: torch.Tensor, weight: torch.Tensor, window: torch.Tensor, *, bias: torch.Tensor | None = None,
@@ -831,7 +685,7 @@ def causal_conv_step(x: torch.Tensor, weight: torch.Tensor, window: torch.Tensor
         number = 0 if activation is None else 1 if type(activation) is str and activation == "silu" else None
         done = _native.calls.conv_step(x, weight, window, bias, starts, number, out)
         if done is not None:
-            return _done(done)
+            return done
     _check_conv(x, weight, bias, starts, activation, ("Envs",))
     _check_window("window", window, x, weight)
     written = [window]
@@ -890,56 +744,6 @@ def _check_block(y, residual, gate, scale, post_weight, pre_weight) -> None:
     raise RuntimeError("y, residual, gate, scale and the weights do not go together")
 
 
-def _pack_block(y, residual, gate, scale, post_weight, pre_weight, eps, outputs, backward=(0,) * 13) -> bytes:
-    envs, steps, width = y.shape
-    return _native.PACK_BLOCK(
-        _DTYPES[y.dtype], _DTYPES[residual.dtype], width, eps, envs, steps, y.data_ptr(), residual.data_ptr(), _ptr(gate),
-        *y.stride()[:2], *residual.stride()[:2], *((0, 0) if gate is None else gate.stride()[:2]), _ptr(scale),
-        _ptr(post_weight), _ptr(pre_weight), *outputs, *backward)
-
-
-def _block_forward(y, residual, *rest):
-    stream = torch.empty(y.shape, dtype=residual.dtype, device=y.device)
-    normed = torch.empty(y.shape, dtype=y.dtype, device=y.device)
-    _call(_native.lib().navi_block_norm, y.device, _pack_block(y, residual, *rest, (stream.data_ptr(), normed.data_ptr())))
-    return stream, normed
-
-
-class _BlockNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, y, residual, gate, scale, post_weight, pre_weight, eps):
-        ctx.save_for_backward(y, residual, gate, scale, post_weight, pre_weight)
-        ctx.eps = eps
-        ctx.set_materialize_grads(False)
-        return _block_forward(y, residual, gate, scale, post_weight, pre_weight, eps)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_stream, grad_normed):
-        y, residual, gate, *vectors = ctx.saved_tensors
-        if grad_stream is None and grad_normed is None:
-            return (None,) * 7
-        grads = [t if t is None or _dense_last(t) else t.contiguous() for t in (grad_stream, grad_normed)]
-        need = ctx.needs_input_grad
-        d_y, d_residual = (torch.empty(t.shape, dtype=t.dtype, device=y.device) for t in (y, residual))
-        d_gate = torch.empty(y.shape, dtype=y.dtype, device=y.device) if gate is not None and need[2] else None
-        d_vectors = [torch.empty_like(t) if t is not None and need[3 + i] else None for i, t in enumerate(vectors)]
-        if y.numel() == 0:
-            for t in d_vectors:
-                if t is not None:
-                    t.zero_()
-            return d_y, d_residual, d_gate, *d_vectors, None
-        args, lib, partial = (y, residual, gate, *vectors, ctx.eps, (0, 0)), _native.lib(), None
-        if any([t is not None for t in d_vectors]):
-            size = _native.check(lib.navi_block_norm_workspace(_pack_block(*args)))
-            partial = torch.empty(size // 4, dtype=torch.float32, device=y.device)
-        strides = [s for t in grads for s in ((0, 0) if t is None else t.stride()[:2])]
-        _call(lib.navi_block_norm_backward, y.device, _pack_block(*args, (
-            *[_ptr(t) for t in grads], *strides, d_y.data_ptr(), d_residual.data_ptr(), _ptr(d_gate),
-            *[_ptr(t) for t in d_vectors], _ptr(partial))))
-        return d_y, d_residual, d_gate, *d_vectors, None
-
-
 def block_norm(y: torch.Tensor, residual: torch.Tensor, *, gate: torch.Tensor | None = None,
                scale: torch.Tensor | None = None, post_weight: torch.Tensor | None = None,
                pre_weight: torch.Tensor | None = None, eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor]:
@@ -958,14 +762,12 @@ def block_norm(y: torch.Tensor, residual: torch.Tensor, *, gate: torch.Tensor | 
     if 0.0 <= eps < math.inf and forward_ad._current_level < 0:
         done = _native.calls.block_norm(y, residual, gate, scale, post_weight, pre_weight, eps)
         if done is not None:
-            return _done(done)
+            return done
     _check_block(y, residual, gate, scale, post_weight, pre_weight)
     _check(math.isfinite(eps) and eps >= 0.0, "eps must be finite and not negative")
     inputs = (y, residual, gate, scale, post_weight, pre_weight)
     _check_tangents(*inputs)
-    if torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in inputs]):
-        return _BlockNorm.apply(*inputs, eps)
-    return _block_forward(*inputs, eps)
+    return _native.calls.block(*inputs, eps)
 
 
 # ---- the norm of all gradients ----

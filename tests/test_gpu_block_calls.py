@@ -254,6 +254,42 @@ def test_forward_mode_is_refused(policy, name):
             policy.orthogonalize([forward_ad.make_dual(g, torch.ones_like(g))])
 
 
+@pytest.mark.parametrize("name", ["selective_scan", "causal_conv", "block_norm"])
+def test_gradients_have_no_gradients(policy, name):
+    """A second derivative is an error where it is asked for; a first one with its graph kept is the same numbers."""
+    given = {n: t.requires_grad_(t.is_floating_point()) for n, t in inputs()[name].items()}
+    leaves = [t for t in given.values() if t.requires_grad]
+
+    def loss():
+        out = getattr(policy, name)(**given)
+        return (out[0] if name == "block_norm" else out).square().sum()
+
+    first = torch.autograd.grad(loss(), leaves, create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(first, torch.autograd.grad(loss(), leaves)))
+    with pytest.raises(RuntimeError, match="no gradients of their own"):
+        sum(g.sum() for g in first).backward()
+
+
+def test_a_second_pass_through_a_graph_is_an_error(policy):
+    x = inputs()["causal_conv"]["x"].requires_grad_()
+    y = policy.causal_conv(x, inputs()["causal_conv"]["weight"])
+    y.sum().backward(retain_graph=True)
+    y.sum().backward()
+    with pytest.raises(RuntimeError, match="second time"):
+        y.sum().backward()
+    assert x.grad is not None
+
+
+def test_an_input_that_changes_before_the_backward_pass(policy):
+    for name, args in inputs().items():
+        leaves = {n: t.requires_grad_() if t.is_floating_point() else t for n, t in args.items()}
+        out = getattr(policy, name)(**leaves)
+        with torch.no_grad():
+            next(iter(leaves.values())).mul_(2.0)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            (out[0] if name == "block_norm" else out).sum().backward()
+
+
 def test_inference_tensors(policy):
     want = together(policy, inputs(), matrices())
     with torch.inference_mode():
@@ -293,6 +329,7 @@ def test_calls_in_one_step_and_by_parts_are_the_same(policy, dtype, monkeypatch)
 
     class Leaves:
         selective_step = conv_step = block_norm = staticmethod(lambda *_: None)
+        block = staticmethod(policy._native.calls.block)
 
     monkeypatch.setattr(policy._native, "calls", Leaves)
     for a, b, c in zip(want, run(), leaves):
