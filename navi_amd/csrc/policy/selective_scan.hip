@@ -724,6 +724,26 @@ __global__ __launch_bounds__(256, 2) void selective_gates_kernel(GateParams P) {
     b.fetch(P.b, env, head, t0, tokens, false, 0, P.state_dim);
     dy.fetch(P.dy, env, head, t0, tokens, false, 0, P.head_dim);
     x.fetch(P.x, env, head, t0, tokens, false, 0, P.head_dim);
+    const bool inside = lane < tokens;
+    const int64_t t = t0 + lane;
+    // What the last wave needs at the end it reads now (1024 x 128 steps of 4 heads: 66 us, 77 with loads there and
+    // sums by shuffles). Both dimensions have two blocks of columns at most.
+    static_assert(NAVI_POLICY_MAX_STATE_DIM <= 2 * kColumns, "partial sums of rho, kappa and delta");
+    float rho = 0.0f, kappa = 0.0f, delta = 0.0f, through = 0.0f, z = 0.0f, more[3] = {};
+    if (wave == 3) {
+        if (inside) {
+            rho = P.rho[sequence * P.rho_blocks * S.steps + t];
+            kappa = P.kappa[sequence * P.delta_blocks * S.steps + t];
+            delta = P.delta[sequence * P.delta_blocks * S.steps + t];
+            if (P.rho_blocks > 1) more[0] = P.rho[(sequence * P.rho_blocks + 1) * S.steps + t];
+            if (P.delta_blocks > 1) {
+                more[1] = P.kappa[(sequence * P.delta_blocks + 1) * S.steps + t];
+                more[2] = P.delta[(sequence * P.delta_blocks + 1) * S.steps + t];
+            }
+            z = S.dt[env * S.dt_stride[0] + t * S.dt_stride[1] + head * S.dt_stride[2]];
+        }
+        if (P.through && lane < P.through_waves) through = P.through[(sequence * S.n_chunks + chunk) * P.through_waves + lane];
+    }
     if (wave == 0) {
         ScanGatesFetch gates;
         gates.fetch(S, false, env, head, t0, tokens);
@@ -784,48 +804,28 @@ __global__ __launch_bounds__(256, 2) void selective_gates_kernel(GateParams P) {
         if (g == 0) lds.pairs[t] = sign * sum;
     }
     __syncthreads();
-    if (wave != 0) return;
-    const bool inside = lane < tokens;
-    const int64_t t = t0 + lane;
-    float rho = 0.0f, kappa = 0.0f, delta = 0.0f, through = 0.0f, z = 0.0f;
-    const float beta = lds.gates.beta[lane], a = S.a[head];
-    if (inside) {
-        for (int n = 0; n < P.rho_blocks; ++n) rho += P.rho[(sequence * P.rho_blocks + n) * S.steps + t];
-        for (int n = 0; n < P.delta_blocks; ++n) {
-            kappa += P.kappa[(sequence * P.delta_blocks + n) * S.steps + t];
-            delta += P.delta[(sequence * P.delta_blocks + n) * S.steps + t];
-        }
-        z = S.dt[env * S.dt_stride[0] + t * S.dt_stride[1] + head * S.dt_stride[2]] + (S.dt_bias ? S.dt_bias[head] : 0.0f);
-    }
-    kappa *= beta;
-    if (P.through)
-        for (int n = 0; n < P.through_waves; ++n) through += P.through[(sequence * S.n_chunks + chunk) * P.through_waves + n];
-    const float keep = lds.gates.e[kChunk - 1];
-    through = keep == 0.0f ? 0.0f : keep * through;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const float r = __shfl_down(rho, d), k = __shfl_up(kappa, d);
-        rho += lane + d < 64 ? r : 0.0f;
-        kappa += lane >= d ? k : 0.0f;
-    }
-    kappa = __shfl_up(kappa, 1);
-    if (lane == 0) kappa = 0.0f;
-    const float dg = lds.pairs[lane] + (rho + kappa) + through;
+    if (wave != 3) return;
+    const float beta = lds.gates.beta[lane], a = S.a[head], keep = lds.gates.e[kChunk - 1];
+    z += S.dt_bias ? S.dt_bias[head] : 0.0f;
+    const double carried = of_lane(sum_up(through), 63);
+    // sums from each token on, and up to the token before each
+    const double from = rho + more[0], to = static_cast<double>(beta) * (kappa + more[1]);
+    const double from_up = sum_up(from), to_up = sum_up(to);
+    const double dg = lds.pairs[lane] + (of_lane(from_up, 63) - (from_up - from)) + (to_up - to) + (keep == 0.0f ? 0.0 : keep * carried);
     double sums[3] = {};
     if (inside) {
-        const float dbeta = delta + lds.bc[lane] * lds.dyx[lane] + a * dg;
-        const float d_dt = dbeta / (1.0f + expf(-z));
+        const double dbeta = (delta + more[2]) + static_cast<double>(lds.bc[lane]) * lds.dyx[lane] + a * dg;
+        const float d_dt = static_cast<float>(dbeta) / (1.0f + expf(-z));
         P.d_dt[(env * S.steps + t) * S.heads + head] = d_dt;
-        sums[0] = static_cast<double>(beta) * dg;
+        sums[0] = beta * dg;
         sums[1] = lds.dyx[lane];
         sums[2] = d_dt;
     }
     if (!P.partial) return;
 #pragma unroll
     for (int n = 0; n < 3; ++n) {
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) sums[n] += __shfl_xor(sums[n], d);
-        if (lane == 0) P.partial[3 * static_cast<int64_t>(blockIdx.x) + n] = sums[n];
+        const double sum = of_lane(sum_up(sums[n]), 63);
+        if (lane == 0) P.partial[3 * static_cast<int64_t>(blockIdx.x) + n] = sum;
     }
 }
 
@@ -865,7 +865,17 @@ __global__ __launch_bounds__(256) void selective_groups_kernel(const float* from
         float sum[8] = {};
         const float* at = from + row * group * dim + c;
         if (dim % 8 == 0) {
-            for (int32_t h = 0; h < group; ++h) {
+            int32_t h = 0;
+            for (; h + 4 <= group; h += 4) {  // (on their way at once: 1024 x 128 rows of 4 heads of 64 take 60 us, 5 TB/s)
+                float x[4][8];
+#pragma unroll
+                for (int m = 0; m < 4; ++m) load_eight(at + static_cast<int64_t>(h + m) * dim, x[m]);
+#pragma unroll
+                for (int m = 0; m < 4; ++m)
+#pragma unroll
+                    for (int n = 0; n < 8; ++n) sum[n] += x[m][n];
+            }
+            for (; h < group; ++h) {
                 float x[8];
                 load_eight(at + static_cast<int64_t>(h) * dim, x);
 #pragma unroll
