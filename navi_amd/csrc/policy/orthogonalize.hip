@@ -123,12 +123,6 @@ __device__ inline double sum_of_squares(const E* from, int64_t count) {
     return sum;
 }
 
-__device__ inline float load_any(const void* from, int32_t dtype, int64_t at) {
-    if (dtype == NAVI_POLICY_F32) return static_cast<const float*>(from)[at];
-    if (dtype == NAVI_POLICY_BF16) return to_float(static_cast<const bf16*>(from)[at]);
-    return to_float(static_cast<const f16*>(from)[at]);
-}
-
 // Squares of a matrix: workgroups take lines along its contiguous axis in turn, or parts of all of them
 // where those lie one after the other.
 __global__ __launch_bounds__(256) void newton_squares_kernel(Params P) {
@@ -184,26 +178,51 @@ __global__ __launch_bounds__(256) void newton_begin_kernel(Params P) {
     for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
     const double factor = w.scale / (sqrt(sum) + static_cast<double>(P.eps));
     const bool along = !x.turned;
-    for (int i = wave; i < 64; i += 4) {
-        const int row = row0 + (along ? i : lane), col = col0 + (along ? lane : i);
-        float v = 0.0f;
-        if (row < x.m && col < x.n)
-            v = static_cast<float>(load_any(x.from, x.from_dtype, along ? row * x.from_line + col : col * x.from_line + row) * factor);
-        tile[along ? i : lane][along ? lane : i] = v;
+    // Sixteen numbers a lane, all on their way at once; eight at a time leave.
+    float v[16];
+    const auto fetch = [&](const auto* from) {
+#pragma unroll
+        for (int n = 0; n < 16; ++n) {
+            const int i = wave + 4 * n, row = row0 + (along ? i : lane), col = col0 + (along ? lane : i);
+            v[n] = 0.0f;
+            if (row < x.m && col < x.n) v[n] = to_float(from[along ? row * x.from_line + col : col * x.from_line + row]);
+        }
+    };
+    if (x.from_dtype == NAVI_POLICY_F32)
+        fetch(static_cast<const float*>(x.from));
+    else if (x.from_dtype == NAVI_POLICY_BF16)
+        fetch(static_cast<const bf16*>(x.from));
+    else
+        fetch(static_cast<const f16*>(x.from));
+#pragma unroll
+    for (int n = 0; n < 16; ++n) {
+        const int i = wave + 4 * n;
+        tile[along ? i : lane][along ? lane : i] = static_cast<float>(v[n] * factor);
     }
     __syncthreads();
     const int64_t size = w.size;
     _Float16* turned = w.turned + P.current * 2 * size;
-    for (int i = wave; i < 64; i += 4) {
-        _Float16 hi, lo;
-        split(tile[i][lane], hi, lo);
-        const int64_t to = static_cast<int64_t>(row0 + i) * w.N + col0 + lane;
-        w.rows[to] = hi;
-        if (kPlanes16 == 2) w.rows[size + to] = lo;
-        split(tile[lane][i], hi, lo);
-        const int64_t back = static_cast<int64_t>(col0 + i) * w.M + row0 + lane;
-        turned[back] = hi;
-        turned[size + back] = lo;
+    const int c = threadIdx.x % 8 * 8;
+#pragma unroll
+    for (int r = threadIdx.x / 8; r < 64; r += 32) {
+        h8 hi, lo;
+        const auto part = [&](auto number) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                _Float16 high, low;
+                split(number(k), high, low);
+                hi[k] = high;
+                lo[k] = low;
+            }
+        };
+        part([&](int k) { return tile[r][c + k]; });
+        const int64_t to = static_cast<int64_t>(row0 + r) * w.N + col0 + c;
+        *reinterpret_cast<h8*>(w.rows + to) = hi;
+        if (kPlanes16 == 2) *reinterpret_cast<h8*>(w.rows + size + to) = lo;
+        part([&](int k) { return tile[c + k][r]; });
+        const int64_t back = static_cast<int64_t>(col0 + r) * w.M + row0 + c;
+        *reinterpret_cast<h8*>(turned + back) = hi;
+        *reinterpret_cast<h8*>(turned + size + back) = lo;
     }
 }
 
