@@ -324,9 +324,11 @@ __device__ inline void put_turned_to(const Tile<kTile>& tile, _Float16* to, int6
     }
 }
 
-// Stages in LDS at once: as many as 128 KB hold, four at most.
-template <int kTile, int kPlanes16>
-inline constexpr int kStages = kTile * kPlanes16 <= 256 ? 4 : 2;
+// Stages in LDS at once: as many as 128 KB hold, four at most. X's products of tiles of 64 take 32 KB, so that four
+// workgroups share a CU and one reads and writes X while others multiply (26 matrices of width 256, two planes: 15.7
+// us, with 64 KB 18.0; the symmetric ones, whose tiles the card holds at once, 9.6 with 64 KB, 10.7 with 32).
+template <int kTile, int kPlanes16, int kMode>
+inline constexpr int kStages = kTile == 64 && (kMode == kApply || kMode == kLast) ? 4 / kPlanes16 : kTile * kPlanes16 <= 256 ? 4 : 2;
 
 // Tiles of one of the three products, kTile x kTile a workgroup, a quarter a wave. Two or four stages of 32
 // numbers along the contracted axis, of all planes, are on their way or in LDS; a wave reads the operands of
@@ -335,7 +337,7 @@ template <int kTile, int kPlanes16, int kMode>
 __global__ __launch_bounds__(256, kTile == 256 ? 1 : kTile == 128 && kPlanes16 == 2 ? 1 : 2) void newton_product_kernel(Params P) {
     constexpr int kEach = kTile / 64;          // results of 32 x 32 of a wave, down and across
     constexpr int kLoads = 2 * kPlanes16 * kTile / 64;  // of a lane for a stage
-    constexpr int kBuffers = kStages<kTile, kPlanes16>;
+    constexpr int kBuffers = kStages<kTile, kPlanes16, kMode>;
     constexpr bool kSymmetric = kMode == kGram || kMode == kPoly;
     extern __shared__ __attribute__((aligned(16))) char lds_bytes[];
     auto& lds = *reinterpret_cast<_Float16 (*)[kBuffers][2][kPlanes16][kTile * kDepth]>(lds_bytes);
@@ -630,7 +632,7 @@ int check_apart(const navi_orthogonalize_matrix* x, int count) {
 
 template <int kTile, int kPlanes16, int kMode>
 int launch(const Params& P, hipStream_t stream) {
-    constexpr int staged = kStages<kTile, kPlanes16> * 2 * kPlanes16 * kTile * kDepth * sizeof(_Float16), tile = sizeof(Tile<kTile>), lds = staged > tile ? staged : tile;
+    constexpr int staged = kStages<kTile, kPlanes16, kMode> * 2 * kPlanes16 * kTile * kDepth * sizeof(_Float16), tile = sizeof(Tile<kTile>), lds = staged > tile ? staged : tile;
     const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void*>(newton_product_kernel<kTile, kPlanes16, kMode>),
                                                hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (err != hipSuccess) return set_error(NAVI_POLICY_E_LAUNCH, "navi_orthogonalize: %s", hipGetErrorString(err));
