@@ -211,7 +211,7 @@ typedef struct navi_causal_conv_args {
     const void* window; /* [envs][taps - 1][channels] or NULL */
     void* out;
     void* window_out;   /* like window, or NULL */
-    /* the backward pass (out and window_out are not read): */
+    /* the backward pass (out and window_out are not read); what it writes shares no memory with anything else: */
     const void* grad_out;
     int64_t grad_out_stride[2];
     const void* grad_window; /* of window_out, contiguous, or NULL */
@@ -254,7 +254,7 @@ typedef struct navi_block_norm_args {
     const float* pre_weight;  /* likewise */
     void* stream;
     void* normed;
-    /* the backward pass (stream and normed are not read): */
+    /* the backward pass (stream and normed are not read); what it writes shares no memory with anything else: */
     const void* grad_stream; /* or NULL for zeros */
     const void* grad_normed; /* or NULL for zeros */
     int64_t grad_stream_stride[2], grad_normed_stride[2];
@@ -310,7 +310,8 @@ typedef struct navi_selective_scan_args {
                              out, which there may be x itself (contiguous) */
     void* scratch;        /* navi_selective_scan_scratch bytes for navi_selective_scan, 16-byte aligned (NULL
                              where that is 0) */
-    /* the backward pass (out, final_state and scratch are not read): */
+    /* the backward pass (out, final_state and scratch are not read); what it writes shares no memory with anything
+       else: */
     const void* grad_out;
     int64_t grad_out_stride[3];
     const float* grad_final_state; /* contiguous, or NULL for zeros */

@@ -267,13 +267,16 @@ PyObject* block_norm(PyObject*, PyObject* const* v, Py_ssize_t n) {
 
 // ---- whole rollouts and their gradients, of arguments that policy.py has looked over ----
 
+// Memory that holds what a tensor shows: that of a lazily negated view holds its negative.
+Tensor plain(const Tensor& t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
+
 // Arguments: None is an undefined tensor.
 variable_list given(PyObject* const* v, size_t n) {
     variable_list to(n);
     for (size_t i = 0; i < n; i++)
         if (v[i] != Py_None) {
             TORCH_CHECK(THPVariable_Check(v[i]), "a tensor is expected");
-            to[i] = THPVariable_Unpack(v[i]);
+            to[i] = plain(THPVariable_Unpack(v[i]));
         }
     return to;
 }
@@ -307,7 +310,10 @@ Tensor floats(const Tensor& of, int64_t bytes) {
 }
 
 // A gradient with its last axis dense; undefined stays so.
-Tensor dense(const Tensor& t) { return !t.defined() || dense_last(t) ? t : t.contiguous(); }
+Tensor dense(const Tensor& given) {
+    const Tensor t = plain(given);
+    return !t.defined() || dense_last(t) ? t : t.contiguous();
+}
 
 // Steps that do not overlap and lie within the reach of the chunked kernels (policy.py's `_rows_apart`).
 Tensor rows_apart(const Tensor& t) {
@@ -414,7 +420,7 @@ struct ScanFunction : torch::autograd::Function<ScanFunction> {
         const Scan g(saved);
         const On on(g.x);
         grad = grad.defined() ? rows_apart(dense(grad)) : like(g.x).zero_();
-        if (grad_state.defined()) grad_state = grad_state.contiguous();
+        if (grad_state.defined()) grad_state = plain(grad_state).contiguous();
         Tensor d_x = like(g.x), d_dt = like(g.dt), d_b = like(g.b), d_c = like(g.c), d_a = like(ctx, saved, 2),
                d_d = like(ctx, saved, 5), d_bias = like(ctx, saved, 6), d_state = like(ctx, saved, 7);
         if (g.x.numel() == 0) {
@@ -495,7 +501,7 @@ struct ConvolutionFunction : torch::autograd::Function<ConvolutionFunction> {
         const Convolution g(saved, ctx->saved_data["activation"].toInt());
         const On on(g.x);
         grad = grad.defined() ? dense(grad) : like(g.x).zero_();
-        if (grad_window.defined()) grad_window = grad_window.contiguous();
+        if (grad_window.defined()) grad_window = plain(grad_window).contiguous();
         Tensor d_x = like(g.x), d_weight = like(ctx, saved, 1), d_bias = like(ctx, saved, 2),
                d_window = like(ctx, saved, 3);
         if (g.x.numel() == 0) {

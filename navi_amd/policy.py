@@ -41,6 +41,7 @@ __all__ = ["gated_delta_rule", "gated_delta_step", "qk_norm", "clip_grad_norm", 
 
 _DTYPES = {torch.float32: _native.F32, torch.bfloat16: _native.BF16, torch.float16: _native.F16}
 _MASKS = (torch.bool, torch.uint8)
+_MOST = torch.finfo(torch.float32).max
 
 # Arguments are looked over twice: `_fine` in one expression on every call (a call of one frame
 # is bound by the host), and by name, for the message, where that found something. Where a call of
@@ -63,6 +64,11 @@ def _check_tensor(name: str, t, dtypes, dims: int, device=None) -> None:
 
 def _dense_last(t: torch.Tensor) -> bool:
     return t.stride(-1) == 1 or t.size(-1) <= 1
+
+
+def _check_plain(*tensors) -> None:
+    """Memory holds what a tensor shows (that of a lazily negated view holds its negative)."""
+    _check(not any([t is not None and t.is_neg() for t in tensors]), "lazily negated views are not taken: resolve_neg() them")
 
 
 def _check_tangents(*tensors) -> None:
@@ -592,6 +598,7 @@ def selective_scan_step(x: torch.Tensor, dt: torch.Tensor, a: torch.Tensor, b: t
     if torch.is_grad_enabled():
         _check(not any([t is not None and t.requires_grad for t in inputs]),
                "selective_scan_step has no gradients; use selective_scan, or torch.no_grad()")
+    _check_plain(*inputs)
     if out is None:
         out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     envs, heads, head_dim = x.shape
@@ -705,6 +712,7 @@ def causal_conv_step(x: torch.Tensor, weight: torch.Tensor, window: torch.Tensor
     if torch.is_grad_enabled():
         _check(not any([t is not None and t.requires_grad for t in inputs]),
                "causal_conv_step has no gradients; use causal_conv, or torch.no_grad()")
+    _check_plain(*inputs)
     if out is None:
         out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     at = window.data_ptr()
@@ -766,12 +774,12 @@ def block_norm(y: torch.Tensor, residual: torch.Tensor, *, gate: torch.Tensor | 
     ``residual`` and ``normed`` like ``y``; ``normed`` is that of the sum before it is rounded.
     """
     eps = float(eps)
-    if 0.0 <= eps < math.inf and forward_ad._current_level < 0:
+    if 0.0 <= eps <= _MOST and forward_ad._current_level < 0:
         done = _native.calls.block_norm(y, residual, gate, scale, post_weight, pre_weight, eps)
         if done is not None:
             return done
     _check_block(y, residual, gate, scale, post_weight, pre_weight)
-    _check(math.isfinite(eps) and eps >= 0.0, "eps must be finite and not negative")
+    _check(0.0 <= eps <= _MOST, "eps must be finite (in float32) and not negative")
     inputs = (y, residual, gate, scale, post_weight, pre_weight)
     _check_tangents(*inputs)
     return _native.calls.block(*inputs, eps)
@@ -864,8 +872,8 @@ def orthogonalize(updates: Iterable[torch.Tensor | None], *, steps: int = 5,
     steps, eps = int(steps), float(eps)
     a, b, c = (float(x) for x in factors)
     _check(1 <= steps <= 100, "steps must be in [1, 100]")
-    _check(math.isfinite(eps) and eps >= 0.0, "eps must be finite and not negative")
-    _check(math.isfinite(a) and math.isfinite(b) and math.isfinite(c), "factors must be finite")
+    _check(0.0 <= eps <= _MOST, "eps must be finite (in float32) and not negative")
+    _check(max(abs(a), abs(b), abs(c)) <= _MOST, "factors must be finite (in float32)")
     updates = list(updates)
     to = updates if out is None else list(out)
     _check(len(to) == len(updates), "out must be as long as updates")
@@ -875,6 +883,10 @@ def orthogonalize(updates: Iterable[torch.Tensor | None], *, steps: int = 5,
     _check(len(updates) > 0, "updates must hold at least one matrix")
     _check_matrices(updates, to)
     _check_tangents(*updates, *to)
+    if torch.is_grad_enabled():
+        _check(not any([x.requires_grad for x in updates]) and (to is updates or not any([y.requires_grad for y in to])),
+               "orthogonalize has no gradients; use torch.no_grad()")
+    _check_plain(*updates, *(() if to is updates else to))
     n, device = len(updates), updates[0].device
     packed = b"".join([_native.PACK_MATRIX(x.data_ptr(), y.data_ptr(), *x.shape, *_strides_of(x), *_strides_of(y),
                                            _DTYPES[x.dtype], _DTYPES[y.dtype]) for x, y in zip(updates, to)])

@@ -150,7 +150,7 @@ def test_refusals_of_groups_activations_and_eps(policy):
         policy.selective_scan(**{**scan, "b": three, "c": three})
     with pytest.raises(RuntimeError, match="activation must be"):
         policy.causal_conv(**given["causal_conv"], activation="gelu")
-    for eps in (-1e-6, float("nan"), float("inf")):
+    for eps in (-1e-6, float("nan"), float("inf"), 1e39):
         with pytest.raises(RuntimeError, match="eps must be"):
             policy.block_norm(**given["block_norm"], eps=eps)
 
@@ -189,7 +189,8 @@ def test_refusals_of_matrices(policy):
     other = torch.randn(8, 12, device="cuda")
     with pytest.raises(RuntimeError, match="share memory"):
         policy.orthogonalize([g, other], out=[other, torch.empty_like(g)])
-    for more in (dict(steps=0), dict(steps=101), dict(eps=-1.0), dict(eps=float("nan")), dict(factors=(1.0, float("inf"), 0.0))):
+    for more in (dict(steps=0), dict(steps=101), dict(eps=-1.0), dict(eps=float("nan")), dict(eps=1e39), dict(factors=(1.0, float("inf"), 0.0)),
+                 dict(factors=(1.0, 0.0, -1e39))):
         with pytest.raises(RuntimeError):
             policy.orthogonalize([g], **more)
 
@@ -350,6 +351,53 @@ def test_frames_are_read_where_they_lie(policy):
                      for i, t in enumerate(again)]
             got = step_of(policy, name)(*moved, **more)
             assert torch.equal(got, want) and torch.equal(moved[-1], carried)
+
+
+def negated(t):
+    """The same numbers as a lazily negated view (the imaginary part of a conjugate)."""
+    z = torch.view_as_complex(torch.stack([torch.zeros_like(t), -t], -1)).conj().imag
+    assert z.is_neg() and torch.equal(z, t)
+    return z
+
+
+def test_lazily_negated_views(policy):
+    """Their memory holds the negative: they are resolved, or refused where something is written."""
+    given = inputs()
+    for name, args in given.items():
+        for n in ("x", "y", "gate", "dt", "b"):
+            if n in args:
+                got, want = (getattr(policy, name)(**{**args, n: t}) for t in (negated(args[n]).contiguous() if n in "xyb" else args[n], args[n]))
+                assert all(torch.equal(p, q) for p, q in zip(*([r] if torch.is_tensor(r) else r for r in (got, want))))
+    args = given["selective_scan"]
+    assert torch.equal(policy.selective_scan(**{**args, "a": negated(args["a"]).clone(), "dt": negated(args["dt"])}), policy.selective_scan(**args))
+    block = given["block_norm"]
+    x = block["y"].clone().requires_grad_()
+    s, n = policy.block_norm(x, block["residual"])
+    got, want = (torch.autograd.grad([s, n], x, [g, g], retain_graph=True)[0] for g in (negated(torch.ones_like(s)), torch.ones_like(s)))
+    assert torch.equal(got, want)
+    for name in STEPS:
+        args, more, carried = frame(name, given[name])
+        if name == "selective_scan":
+            with pytest.raises(RuntimeError, match="negated"):
+                step_of(policy, name)(args[0], negated(args[1]), *args[2:], **more)
+    g = matrices()[0]
+    z = torch.view_as_complex(torch.stack([g, g], -1)).conj().imag
+    with pytest.raises(RuntimeError, match="negated|contiguous"):
+        policy.orthogonalize([z])
+
+
+def test_matrices_that_require_grad(policy):
+    g = matrices()[0]
+    want = torch.empty_like(g)
+    policy.orthogonalize([g], out=[want])
+    leaf, kept = g.clone().requires_grad_(), g.clone()
+    for updates, out in (([leaf], None), ([g], [leaf]), ([leaf * 1.0], None)):
+        with pytest.raises(RuntimeError, match="no gradients"):
+            policy.orthogonalize(updates, out=out)
+    assert torch.equal(leaf, kept)
+    with torch.no_grad():
+        policy.orthogonalize([leaf])
+    assert torch.equal(leaf, want)
 
 
 # ---- streams, threads, graphs ----
