@@ -193,6 +193,12 @@ struct ScanGatesFetch {
     }
 };
 
+// Values of a chunk: planes, or float32 as it is, which takes less of the LDS than three of them: two workgroups of
+// 64 rows fit a CU (float32, 1024 x 128 steps of 4 heads of 64 x 64: forward 169 us, 261 with planes; with gradients
+// 924 and 1371).
+template <class E>
+using Values = std::conditional_t<sizeof(E) == 4, float[kChunk][kColumns + 4], uint16_t[kPlanes<E>][kChunk][kColumns + 8]>;
+
 template <class E, int KP>
 struct ScanLds {
     union {
@@ -200,7 +206,7 @@ struct ScanLds {
         Triangle<3> p;  // once the queries have been used
     };
     uint16_t k[kPlanes<E>][kChunk][KP + 8];
-    uint16_t v[kPlanes<E>][kChunk][kColumns + 8];
+    __attribute__((aligned(16))) Values<E> v;
     ScanGates gates;
 };
 
@@ -260,6 +266,18 @@ struct RowsFetch {
     }
 };
 
+// As they are, where they are float32.
+template <int kPieces, int kPitch>
+__device__ inline void put_floats(const Part<float, 8> (&part)[kPieces], float (&rows)[kChunk][kPitch]) {
+    const int c = threadIdx.x % (kColumns / 8) * 8;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+        const int t = threadIdx.x / (kColumns / 8) + i * (256 / (kColumns / 8));
+#pragma unroll
+        for (int w = 0; w < 2; ++w) *reinterpret_cast<u4*>(&rows[t][c + 4 * w]) = part[i].words[w];
+    }
+}
+
 // Eight numbers of operands as floats: their planes' sum.
 template <int N>
 __device__ inline void join8(const u4 (&plane)[N], float (&x)[8]) {
@@ -288,6 +306,18 @@ __device__ inline f4 four_of(const uint16_t (&rows)[N][kChunk][kPitch], int row,
 
 // The tiles of a triangle that a wave computes: its own on the diagonal, and of those below one or two
 // (i and j, two bits each, for n = 1 and 2; 3 for none).
+template <int kPitch>
+__device__ inline f4 four_of(const float (&rows)[kChunk][kPitch], int row, int c, int g) {
+    return *reinterpret_cast<const f4*>(&rows[row][16 * c + 4 * g]);
+}
+
+// The wave's 16 columns of 32 tokens of values that are float32, as operand_columns orders them.
+template <int kPitch>
+__device__ inline void column_values(int lane, const float (&v)[kChunk][kPitch], int wave, int m, float (&x)[8]) {
+#pragma unroll
+    for (int s = 0; s < 8; ++s) x[s] = v[32 * m + 16 * (s >> 2) + 4 * (lane >> 4) + (s & 3)][16 * wave + (lane & 15)];
+}
+
 __device__ inline int tile_of_wave(int wave, int n) {
     constexpr uint32_t kBelow = 0x84u | 0xc9u << 8 | 0x3du << 16 | 0x3eu << 24;
     return n == 0 ? 5 * wave : kBelow >> (8 * wave + 4 * (n - 1)) & 15;
@@ -402,9 +432,9 @@ struct FourFetch {
     }
 };
 
-// Workgroups that a CU's LDS holds: 42 KB each for bfloat16 and 64, up to 147 KB for float32 and 128.
+// Workgroups that a CU's LDS holds: 42 KB each for bfloat16 and 64, up to 137 KB for float32 and 128.
 template <class E, int KP>
-inline constexpr int kWorkgroups = kPlanes<E> == 1 ? (KP == 64 ? 3 : 2) : kPlanes<E> == 2 && KP == 64 ? 2 : 1;
+inline constexpr int kWorkgroups = kPlanes<E> == 1 ? (KP == 64 ? 3 : 2) : KP == 64 ? 2 : 1;
 
 // A workgroup walks the chunks of a segment with 64 columns of a head's state in registers, 16 a wave.
 template <class E, int KP, int kMode>
@@ -475,7 +505,10 @@ __global__ __launch_bounds__(256, (kWorkgroups<E, KP>)) void selective_scan_kern
         }
         if (!kSummary) q_next.put(lds.q);
         k_next.put(lds.k, sign < 0.0f ? 0x80008000u : 0u);
-        v_next.put(lds.v);
+        if constexpr (sizeof(E) == 4)
+            put_floats(v_next.part, lds.v);
+        else
+            v_next.put(lds.v);
         if (wave == 0) gates_next.put(P, lds.gates, reverse, head, low, tokens);
         __syncthreads();
         if (chunk + 1 < end) fetch(chunk + 1);
@@ -559,9 +592,17 @@ __global__ __launch_bounds__(256, (kWorkgroups<E, KP>)) void selective_scan_kern
             }
         }
         u4 value[2][N];
+        float values[sizeof(E) == 4 ? 2 : 1][8];
         if (working) {
 #pragma unroll
-            for (int m = 0; m < 2; ++m) operand_columns(lane, lds.v, wave, m, value[m]);
+            for (int m = 0; m < 2; ++m) {
+                if constexpr (sizeof(E) == 4) {
+                    column_values(lane, lds.v, wave, m, values[m]);
+                    split8(values[m], value[m]);
+                } else {
+                    operand_columns(lane, lds.v, wave, m, value[m]);
+                }
+            }
 #pragma unroll
             for (int i = 0; i < KP / 16; ++i)
 #pragma unroll
@@ -569,8 +610,8 @@ __global__ __launch_bounds__(256, (kWorkgroups<E, KP>)) void selective_scan_kern
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
                 u4 r[3];
-                float x[8];
-                join8(value[m], x);
+                float(&x)[8] = values[sizeof(E) == 4 ? m : 0];
+                if constexpr (sizeof(E) != 4) join8(value[m], x);
                 const f4 f0 = *reinterpret_cast<const f4*>(&lds.gates.f[32 * m + 4 * g]);
                 const f4 f1 = *reinterpret_cast<const f4*>(&lds.gates.f[32 * m + 16 + 4 * g]);
                 split8(f0 * f4{x[0], x[1], x[2], x[3]}, f1 * f4{x[4], x[5], x[6], x[7]}, r);
@@ -1030,7 +1071,7 @@ int launched(const char* name) {
 template <class E, int KP, int kMode>
 int launch_scan(const ScanParams& P, int roles, int segments, hipStream_t stream) {
     constexpr int lds = kMode == kGradients ? sizeof(ScanGradientsLds<E, KP>) : sizeof(ScanLds<E, KP>);
-    static_assert(lds <= 160 * 1024, "a CU's LDS");
+    static_assert(lds * kWorkgroups<E, KP> <= 160 * 1024, "a CU's LDS");
     const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void*>(selective_scan_kernel<E, KP, kMode>),
                                                hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (err != hipSuccess) return set_error(NAVI_POLICY_E_LAUNCH, "navi_selective_scan: %s", hipGetErrorString(err));
