@@ -4,10 +4,11 @@
 // filling of structures, take more (a frame of one environment: 14.8 us a call through ctypes, 5.2 here; a training
 // pass of a small scan, forward and backward: 201 us through ctypes and a function of Python's, 82 here).
 //
-// selective_step, conv_step and block_norm look their arguments over too. They take a call that is in order in
-// every respect, and return None for any other, with nothing done: navi_amd/policy.py then says by name what is
-// wrong, or goes the way that keeps gradients. What is in order is what policy.py's `_fine_...` functions say. The
-// others are policy.py's calls of whole rollouts, of arguments that it has looked over, with their gradients.
+// selective_step, conv_step, selective_scan, causal_conv and block_norm look their arguments over too. They take a
+// call that is in order in every respect (and a frame's that asks for no gradients), and return None for any other,
+// with nothing done: navi_amd/policy.py then says by name what is wrong, or takes tensors of a user's own class or
+// of another device than the current one. What is in order is what policy.py's `_fine_...` functions say. scan, conv
+// and block are the rollouts' calls of arguments that policy.py has looked over.
 #define __HIP_PLATFORM_AMD__ 1  // (the host compiler reads HIP's headers)
 #include <Python.h>
 
@@ -56,8 +57,9 @@ Entries entries{};
 // allowed, None.
 struct Call {
     bool fine = true;
-    bool grad = c10::GradMode::is_enabled();
-    c10::Device device{c10::DeviceType::CPU};
+    const bool grad;  // gradients would be asked for and are not to be had
+
+    explicit Call(bool differentiable) : grad(!differentiable && c10::GradMode::is_enabled()) {}
 
     const Tensor* tensor(PyObject* o) {
         if (!THPVariable_CheckExact(o)) {  // (a tensor or a parameter, no class of a user's)
@@ -73,6 +75,12 @@ struct Call {
     }
     const Tensor* maybe(PyObject* o) { return o == Py_None ? nullptr : tensor(o); }
 };
+
+// Several of a call's arguments.
+bool all_fine(Call& call, PyObject* const* v, int needed, int all) {
+    for (int i = 0; i < all; i++) i < needed ? call.tensor(v[i]) : call.maybe(v[i]);
+    return call.fine;
+}
 
 int type_of(const Tensor& t) {
     switch (t.scalar_type()) {
@@ -93,6 +101,14 @@ bool vector(const Tensor* t, c10::Device device, int64_t length) {
 bool mask(const Tensor* t, c10::Device device, int64_t length) {
     return !t || ((t->scalar_type() == at::kBool || t->scalar_type() == at::kByte) && t->device() == device &&
                   t->dim() == 1 && t->size(0) == length);
+}
+
+// (tensors that may be undefined)
+bool vector(const Tensor& t, c10::Device device, int64_t length) { return vector(t.defined() ? &t : nullptr, device, length); }
+
+bool mask(const Tensor& t, const Tensor& x) {
+    return !t.defined() || ((t.scalar_type() == at::kBool || t.scalar_type() == at::kByte) && t.device() == x.device() &&
+                            t.dim() == 2 && t.size(0) == x.size(0) && t.size(1) == x.size(1));
 }
 
 void* at_of(const Tensor* t) { return t ? t->data_ptr() : nullptr; }
@@ -141,7 +157,7 @@ template <typename Entry, typename Args> void launch(Entry entry, const Args& ar
 PyObject* selective_step(PyObject*, PyObject* const* v, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     if (n != 10 || !entries.selective_step) Py_RETURN_NONE;
-    Call call;
+    Call call(false);
     const Tensor *x = call.tensor(v[0]), *dt = call.tensor(v[1]), *a = call.tensor(v[2]), *b = call.tensor(v[3]),
                  *c = call.tensor(v[4]), *state = call.tensor(v[5]), *d = call.maybe(v[6]), *dt_bias = call.maybe(v[7]),
                  *starts = call.maybe(v[8]), *to = call.maybe(v[9]);
@@ -190,7 +206,7 @@ PyObject* selective_step(PyObject*, PyObject* const* v, Py_ssize_t n) {
 PyObject* conv_step(PyObject*, PyObject* const* v, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     if (n != 7 || !entries.causal_conv || !PyLong_CheckExact(v[5])) Py_RETURN_NONE;
-    Call call;
+    Call call(false);
     const Tensor *x = call.tensor(v[0]), *weight = call.tensor(v[1]), *window = call.tensor(v[2]), *bias = call.maybe(v[3]),
                  *starts = call.maybe(v[4]), *to = call.maybe(v[6]);
     if (!call.fine) Py_RETURN_NONE;
@@ -222,46 +238,6 @@ PyObject* conv_step(PyObject*, PyObject* const* v, Py_ssize_t n) {
     wrote(out);
     Py_INCREF(v[6]);
     return v[6];
-    END_HANDLE_TH_ERRORS
-}
-
-// block_norm(y, residual, gate, scale, post_weight, pre_weight, eps): both outputs, or None.
-PyObject* block_norm(PyObject*, PyObject* const* v, Py_ssize_t n) {
-    HANDLE_TH_ERRORS
-    if (n != 7 || !entries.block_norm || !PyFloat_CheckExact(v[6])) Py_RETURN_NONE;
-    Call call;
-    const Tensor *y = call.tensor(v[0]), *residual = call.tensor(v[1]), *gate = call.maybe(v[2]), *scale = call.maybe(v[3]),
-                 *post = call.maybe(v[4]), *pre = call.maybe(v[5]);
-    if (!call.fine) Py_RETURN_NONE;
-    const auto device = y->device();
-    const int type = type_of(*y), stream_type = type_of(*residual);
-    void* stream;
-    if (type < 0 || y->dim() != 3 || !stream_of(device, &stream)) Py_RETURN_NONE;
-    const int64_t width = y->size(2);
-    if (residual->device() != device || (stream_type != type && stream_type != NAVI_POLICY_F32) ||
-        residual->sizes() != y->sizes() || width <= 0 || width > NAVI_POLICY_MAX_BLOCK_WIDTH || !dense_last(*y) ||
-        !dense_last(*residual) ||
-        (gate && (gate->scalar_type() != y->scalar_type() || gate->device() != device || gate->sizes() != y->sizes() ||
-                  !dense_last(*gate))) ||
-        !vector(scale, device, width) || !vector(post, device, width) || !vector(pre, device, width))
-        Py_RETURN_NONE;
-    Tensor sum = empty_like(*y, residual->scalar_type()), normed = empty_like(*y, y->scalar_type());
-    navi_block_norm_args s{};
-    s.dtype = type, s.stream_dtype = stream_type, s.width = int32_t(width), s.eps = float(PyFloat_AS_DOUBLE(v[6]));
-    s.envs = y->size(0), s.steps = y->size(1);
-    s.y = read_of<void>(y), s.residual = read_of<void>(residual), s.gate = read_of<void>(gate);
-    for (int i = 0; i < 2; i++) {
-        s.y_stride[i] = y->stride(i), s.residual_stride[i] = residual->stride(i);
-        s.gate_stride[i] = gate ? gate->stride(i) : 0;
-    }
-    s.scale = read_of<float>(scale), s.post_weight = read_of<float>(post), s.pre_weight = read_of<float>(pre);
-    s.stream = at_of(&sum), s.normed = at_of(&normed);
-    launch(entries.block_norm, s, stream);
-    PyObject* pair = PyTuple_New(2);
-    if (!pair) return nullptr;
-    PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(std::move(sum)));
-    PyTuple_SET_ITEM(pair, 1, THPVariable_Wrap(std::move(normed)));
-    return pair;
     END_HANDLE_TH_ERRORS
 }
 
@@ -442,16 +418,47 @@ struct ScanFunction : torch::autograd::Function<ScanFunction> {
     }
 };
 
-// scan(x, dt, a, b, c, d, dt_bias, initial_state, starts, return_state, stepwise): out, or (out, state).
+PyObject* scan_of(const variable_list& in, bool return_state, int64_t stepwise) {
+    if (records({&in[0], &in[1], &in[2], &in[3], &in[4], &in[5], &in[6], &in[7]}))
+        return results(ScanFunction::apply(rows_apart(in[0]), in[1], in[2], rows_apart(in[3]), rows_apart(in[4]), maybe(in[5]),
+                                           maybe(in[6]), maybe(in[7]), maybe(in[8]), return_state));
+    if (in[0].size(1) <= stepwise) return results(Scan(in).forward(return_state, true));
+    return results(Scan({rows_apart(in[0]), in[1], in[2], rows_apart(in[3]), rows_apart(in[4]), in[5], in[6], in[7], in[8]})
+                       .forward(return_state, false));
+}
+
+// scan(x, dt, a, b, c, d, dt_bias, initial_state, starts, return_state, the most steps that go token by token): out, or
+// (out, state).
 PyObject* scan(PyObject*, PyObject* const* v, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     count(n, 11);
+    return scan_of(given(v, 9), v[9] == Py_True, PyLong_AsLong(v[10]));
+    END_HANDLE_TH_ERRORS
+}
+
+// selective_scan(the same): the same of a call that is in order, or None.
+PyObject* selective_scan(PyObject*, PyObject* const* v, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    Call call(true);
+    if (n != 11 || !entries.selective_scan || !all_fine(call, v, 5, 9)) Py_RETURN_NONE;
     const variable_list in = given(v, 9);
-    const bool return_state = v[9] == Py_True;
-    if (records({&in[0], &in[1], &in[2], &in[3], &in[4], &in[5], &in[6], &in[7]}))
-        return results(ScanFunction::apply(in[0], in[1], in[2], in[3], in[4], maybe(in[5]), maybe(in[6]), maybe(in[7]),
-                                           maybe(in[8]), return_state));
-    return results(Scan(in).forward(return_state, v[10] == Py_True));
+    const Tensor &x = in[0], &dt = in[1], &b = in[3], &c = in[4], &state = in[7];
+    void* stream;
+    if (type_of(x) < 0 || x.dim() != 4 || b.dim() != 4 || c.dim() != 4 || dt.dim() != 3 || !stream_of(x.device(), &stream))
+        Py_RETURN_NONE;
+    const auto device = x.device();
+    const int64_t envs = x.size(0), steps = x.size(1), heads = x.size(2), width = x.size(3), groups = b.size(2), dim = b.size(3);
+    if (b.scalar_type() != x.scalar_type() || c.scalar_type() != x.scalar_type() || dt.scalar_type() != at::kFloat ||
+        b.device() != device || c.device() != device || dt.device() != device || b.size(0) != envs || b.size(1) != steps ||
+        c.sizes() != b.sizes() || dt.size(0) != envs || dt.size(1) != steps || dt.size(2) != heads || groups <= 0 ||
+        groups > heads || heads % groups || heads > INT32_MAX || width <= 0 || width > NAVI_POLICY_MAX_STATE_DIM || dim <= 0 ||
+        dim > NAVI_POLICY_MAX_STATE_DIM || !dense_last(x) || !dense_last(b) || !dense_last(c) || !vector(in[2], device, heads) ||
+        !vector(in[5], device, heads) || !vector(in[6], device, heads) || !mask(in[8], x) ||
+        (state.defined() && (state.scalar_type() != at::kFloat || state.device() != device || state.dim() != 4 ||
+                             state.size(0) != envs || state.size(1) != heads || state.size(2) != dim || state.size(3) != width ||
+                             !state.is_contiguous())))
+        Py_RETURN_NONE;
+    return scan_of(in, v[9] == Py_True, PyLong_AsLong(v[10]));
     END_HANDLE_TH_ERRORS
 }
 
@@ -525,17 +532,40 @@ struct ConvolutionFunction : torch::autograd::Function<ConvolutionFunction> {
     }
 };
 
-// conv(x, weight, bias, window, starts, activation's number, return_window): out, or (out, window after).
-PyObject* conv(PyObject*, PyObject* const* v, Py_ssize_t n) {
-    HANDLE_TH_ERRORS
-    count(n, 7);
-    const variable_list in = given(v, 5);
-    const int64_t activation = PyLong_AsLong(v[5]);
-    const bool return_window = v[6] == Py_True;
+PyObject* conv_of(const variable_list& in, int64_t activation, bool return_window) {
     if (records({&in[0], &in[1], &in[2], &in[3]}))
         return results(ConvolutionFunction::apply(in[0], in[1], maybe(in[2]), maybe(in[3]), maybe(in[4]), activation,
                                                   return_window));
     return results(Convolution(in, activation).forward(return_window));
+}
+
+// conv(x, weight, bias, window, starts, activation's number, return_window): out, or (out, window after).
+PyObject* conv(PyObject*, PyObject* const* v, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    count(n, 7);
+    return conv_of(given(v, 5), PyLong_AsLong(v[5]), v[6] == Py_True);
+    END_HANDLE_TH_ERRORS
+}
+
+// causal_conv(the same): the same of a call that is in order, or None.
+PyObject* causal_conv(PyObject*, PyObject* const* v, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    Call call(true);
+    if (n != 7 || !entries.causal_conv || !PyLong_CheckExact(v[5]) || !all_fine(call, v, 2, 5)) Py_RETURN_NONE;
+    const variable_list in = given(v, 5);
+    const Tensor &x = in[0], &weight = in[1], &window = in[3];
+    void* stream;
+    if (type_of(x) < 0 || x.dim() != 3 || weight.dim() != 2 || !stream_of(x.device(), &stream)) Py_RETURN_NONE;
+    const auto device = x.device();
+    const int64_t channels = x.size(2), taps = weight.size(1);
+    if (channels <= 0 || channels > 65536 || taps < 2 || taps > NAVI_POLICY_MAX_TAPS || !dense_last(x) ||
+        weight.scalar_type() != at::kFloat || weight.device() != device || weight.size(0) != channels || !weight.is_contiguous() ||
+        !vector(in[2], device, channels) || !mask(in[4], x) ||
+        (window.defined() && (window.scalar_type() != x.scalar_type() || window.device() != device || window.dim() != 3 ||
+                              window.size(0) != x.size(0) || window.size(1) != taps - 1 || window.size(2) != channels ||
+                              !window.is_contiguous())))
+        Py_RETURN_NONE;
+    return conv_of(in, PyLong_AsLong(v[5]), v[6] == Py_True);
     END_HANDLE_TH_ERRORS
 }
 
@@ -604,15 +634,39 @@ struct BetweenFunction : torch::autograd::Function<BetweenFunction> {
     }
 };
 
+PyObject* block_of(const variable_list& in, double eps) {
+    if (records({&in[0], &in[1], &in[2], &in[3], &in[4], &in[5]}))
+        return results(BetweenFunction::apply(in[0], in[1], maybe(in[2]), maybe(in[3]), maybe(in[4]), maybe(in[5]), eps));
+    return results(Between(in, eps).forward());
+}
+
 // block(y, residual, gate, scale, post_weight, pre_weight, eps): (stream, normed).
 PyObject* block(PyObject*, PyObject* const* v, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     count(n, 7);
+    return block_of(given(v, 6), PyFloat_AsDouble(v[6]));
+    END_HANDLE_TH_ERRORS
+}
+
+// block_norm(the same): the same of a call that is in order, or None.
+PyObject* block_norm(PyObject*, PyObject* const* v, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    Call call(true);
+    if (n != 7 || !entries.block_norm || !PyFloat_CheckExact(v[6]) || !all_fine(call, v, 2, 6)) Py_RETURN_NONE;
     const variable_list in = given(v, 6);
-    const double eps = PyFloat_AsDouble(v[6]);
-    if (records({&in[0], &in[1], &in[2], &in[3], &in[4], &in[5]}))
-        return results(BetweenFunction::apply(in[0], in[1], maybe(in[2]), maybe(in[3]), maybe(in[4]), maybe(in[5]), eps));
-    return results(Between(in, eps).forward());
+    const Tensor &y = in[0], &residual = in[1], &gate = in[2];
+    const auto device = y.device();
+    const int type = type_of(y), stream_type = type_of(residual);
+    void* stream;
+    if (type < 0 || y.dim() != 3 || !stream_of(device, &stream)) Py_RETURN_NONE;
+    const int64_t width = y.size(2);
+    if (residual.device() != device || (stream_type != type && stream_type != NAVI_POLICY_F32) || residual.sizes() != y.sizes() ||
+        width <= 0 || width > NAVI_POLICY_MAX_BLOCK_WIDTH || !dense_last(y) || !dense_last(residual) ||
+        (gate.defined() && (gate.scalar_type() != y.scalar_type() || gate.device() != device || gate.sizes() != y.sizes() ||
+                            !dense_last(gate))) ||
+        !vector(in[3], device, width) || !vector(in[4], device, width) || !vector(in[5], device, width))
+        Py_RETURN_NONE;
+    return block_of(in, PyFloat_AS_DOUBLE(v[6]));
     END_HANDLE_TH_ERRORS
 }
 
@@ -632,7 +686,8 @@ PyObject* bind(PyObject*, PyObject* const* v, Py_ssize_t n) {
 
 #define METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {METHOD(bind), METHOD(selective_step), METHOD(conv_step), METHOD(block_norm),
-                         METHOD(scan), METHOD(conv), METHOD(block), {nullptr, nullptr, 0, nullptr}};
+                         METHOD(scan), METHOD(selective_scan), METHOD(conv), METHOD(causal_conv), METHOD(block),
+                         {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_policy_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -46,8 +46,9 @@ _MOST = torch.finfo(torch.float32).max
 # Arguments are looked over twice: `_fine` in one expression on every call (a call of one frame
 # is bound by the host), and by name, for the message, where that found something. Where a call of
 # one frame or of a few rows takes the device less time than its arguments take Python, the
-# extension `_native.calls` makes it whole, if it is in order and asks for no gradients; a call that
-# it leaves (None) goes the way below. Allocation and launch of a block's operators are its work too.
+# extension `_native.calls` makes it whole, if it is in order (and a frame's asks for no gradients); a
+# call that it leaves (None) goes the way below. Allocation, launch and gradients of a block's operators
+# are its work too.
 
 
 def _check(cond: bool, msg: str) -> None:
@@ -560,16 +561,17 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, a: torch.Tensor, b: torch.
     infinity in the inputs may reach every token of its chunk of 64 tokens and what follows
     them, beyond the start of an episode too.
     """
+    return_state = bool(return_state)
+    if forward_ad._current_level < 0:
+        done = _native.calls.selective_scan(x, dt, a, b, c, d, dt_bias, initial_state, starts, return_state, _STEPWISE)
+        if done is not None:
+            return done
     _check_scan(x, dt, a, b, c, d, dt_bias, starts, ("Envs", "Steps"))
     if initial_state is not None:
         _check_scan_state("initial_state", initial_state, x, b)
-    inputs = (x, dt, a, b, c, d, dt_bias, initial_state)
-    _check_tangents(*inputs)
-    grad = torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in inputs])
-    stepwise = not grad and x.size(1) <= _STEPWISE  # (as for the gated delta rule)
-    if not stepwise:
-        x, b, c = _rows_apart(x), _rows_apart(b), _rows_apart(c)
-    return _native.calls.scan(x, dt, a, b, c, d, dt_bias, initial_state, starts, bool(return_state), stepwise)
+    _check_tangents(x, dt, a, b, c, d, dt_bias, initial_state)
+    # (rollouts of few steps without gradients go token by token, as for the gated delta rule)
+    return _native.calls.scan(x, dt, a, b, c, d, dt_bias, initial_state, starts, return_state, _STEPWISE)
 
 
 def selective_scan_step(x: torch.Tensor, dt: torch.Tensor, a: torch.Tensor, b: torch.Tensor, c: torch.Tensor,
@@ -619,13 +621,17 @@ def selective_scan_step(x: torch.Tensor, dt: torch.Tensor, a: torch.Tensor, b: t
 _ACTIVATIONS = {"silu": _native.ACT_SILU, None: _native.ACT_NONE}
 
 
+def _number_of(activation) -> int | None:
+    return _ACTIVATIONS.get(activation) if activation is None or isinstance(activation, str) else None
+
+
 def _fine_conv(x, weight, bias, starts, activation) -> bool:
     try:
         channels, device = x.size(-1), x.device
         return (x.dtype in _DTYPES and device.type == "cuda" and (x.stride(-1) == 1 or channels == 1) and 0 < channels <= 65536
                 and weight.dtype is torch.float32 and weight.device == device and weight.dim() == 2
                 and weight.size(0) == channels and 2 <= weight.size(1) <= _native.MAX_TAPS and weight.is_contiguous()
-                and _fine_vectors(device, (bias, channels)) and activation in _ACTIVATIONS
+                and _fine_vectors(device, (bias, channels)) and _number_of(activation) is not None
                 and (starts is None or (starts.dtype in _MASKS and starts.device == device and starts.shape == x.shape[:-1])))
     except (AttributeError, TypeError, ValueError, IndexError, RuntimeError):
         return False
@@ -647,7 +653,7 @@ def _check_conv(x, weight, bias, starts, activation, lead: tuple[str, ...]) -> N
     if starts is not None:
         _check_like("x", "starts", starts, _MASKS, n, x.device)
         _check(starts.shape == x.shape[:-1], f"starts must be [{shape}]")
-    _check(activation in _ACTIVATIONS, "activation must be 'silu' or None")
+    _check(_number_of(activation) is not None, "activation must be 'silu' or None")
     raise RuntimeError("x, weight, bias and starts do not go together")
 
 
@@ -678,12 +684,17 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, *, bias: torch.Tensor | N
     ``Taps - 1`` inputs, zeros in place of those of an earlier episode. Sums are float32's, rounded
     once at the end.
     """
+    return_window, number = bool(return_window), _number_of(activation)
+    if forward_ad._current_level < 0:
+        done = _native.calls.causal_conv(x, weight, bias, initial_window, starts, number, return_window)
+        if done is not None:
+            return done
     _check_conv(x, weight, bias, starts, activation, ("Envs", "Steps"))
     if initial_window is not None:
         _check_window("initial_window", initial_window, x, weight)
     inputs = (x, weight, bias, initial_window)
     _check_tangents(*inputs)
-    return _native.calls.conv(*inputs, starts, _ACTIVATIONS[activation], bool(return_window))
+    return _native.calls.conv(*inputs, starts, number, return_window)
 
 
 def causal_conv_step(x: torch.Tensor, weight: torch.Tensor, window: torch.Tensor, *, bias: torch.Tensor | None = None,
@@ -696,8 +707,7 @@ def causal_conv_step(x: torch.Tensor, weight: torch.Tensor, window: torch.Tensor
     ``x`` itself. Autograd is told of both writes. No gradients: this is the form for acting.
     """
     if forward_ad._current_level < 0:
-        number = 0 if activation is None else 1 if type(activation) is str and activation == "silu" else None
-        done = _native.calls.conv_step(x, weight, window, bias, starts, number, out)
+        done = _native.calls.conv_step(x, weight, window, bias, starts, _number_of(activation), out)
         if done is not None:
             return done
     _check_conv(x, weight, bias, starts, activation, ("Envs",))

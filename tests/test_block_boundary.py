@@ -324,6 +324,10 @@ def test_the_extension_leaves_what_it_does_not_take():
     assert calls.conv_step(x, x, x, None, None, None, None) is None
     assert calls.block_norm(x, x, None, None, None, None, 1e-6) is None
     assert calls.block_norm(x, x, None, None, None, None, "1") is None
+    assert calls.selective_scan(x, x, x, x, x, None, None, None, None, False, 4) is None
+    assert calls.selective_scan(x) is None
+    assert calls.causal_conv(x, x, None, None, None, 1, False) is None
+    assert calls.causal_conv(x, x, None, None, None, None, False) is None
     sparse = torch.eye(4).to_sparse()
     assert calls.block_norm(sparse, sparse, None, None, None, None, 1e-6) is None
     with pytest.raises(TypeError):

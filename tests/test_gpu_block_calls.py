@@ -148,8 +148,9 @@ def test_refusals_of_groups_activations_and_eps(policy):
     three = torch.cat([scan["b"], scan["b"][:, :, :1]], 2)
     with pytest.raises(RuntimeError, match="multiple of the groups"):
         policy.selective_scan(**{**scan, "b": three, "c": three})
-    with pytest.raises(RuntimeError, match="activation must be"):
-        policy.causal_conv(**given["causal_conv"], activation="gelu")
+    for activation in ("gelu", 1, ["silu"], torch.ones(2)):
+        with pytest.raises(RuntimeError, match="activation must be"):
+            policy.causal_conv(**given["causal_conv"], activation=activation)
     for eps in (-1e-6, float("nan"), float("inf"), 1e39):
         with pytest.raises(RuntimeError, match="eps must be"):
             policy.block_norm(**given["block_norm"], eps=eps)
@@ -324,13 +325,23 @@ def test_calls_in_one_step_and_by_parts_are_the_same(policy, dtype, monkeypatch)
                     made += [got, args[-1]]
         made += policy.block_norm(**{n: change(t) for n, t in given["block_norm"].items()}, eps=1e-5)
         made += policy.block_norm(change(given["block_norm"]["y"]), given["block_norm"]["residual"])
+        for name in STEPS:
+            args = {n: change(t) for n, t in given[name].items()}
+            short = {n: t[:, :3] if n in ("x", "dt", "b", "c", "starts") else t for n, t in args.items()}
+            more = {"return_state" if name == "selective_scan" else "return_window": True}
+            for a in (args, short):
+                made += getattr(policy, name)(**a, **more)
+            leaves = {n: t.detach().requires_grad_(t.is_floating_point()) for n, t in given[name].items()}
+            out, after = getattr(policy, name)(**{n: change(t) for n, t in leaves.items()}, **more)
+            wanted = [t for t in leaves.values() if t.requires_grad]
+            made += torch.autograd.grad([out, after], wanted, [torch.ones_like(out), torch.ones_like(after)])
         return made
 
     want, leaves = run(), run(lambda t: t.as_subclass(Named))
 
     class Leaves:
-        selective_step = conv_step = block_norm = staticmethod(lambda *_: None)
-        block = staticmethod(policy._native.calls.block)
+        selective_step = conv_step = selective_scan = causal_conv = block_norm = staticmethod(lambda *_: None)
+        scan, conv, block = (staticmethod(getattr(policy._native.calls, n)) for n in ("scan", "conv", "block"))
 
     monkeypatch.setattr(policy._native, "calls", Leaves)
     for a, b, c in zip(want, run(), leaves):
