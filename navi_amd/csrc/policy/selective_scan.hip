@@ -1097,12 +1097,12 @@ int scan(const ScanParams& P, int roles, bool back, hipStream_t stream) {
 }
 
 template <class E>
-int scans(const ScanParams& P, int roles, bool back, hipStream_t stream) {
+int scans(const ScanParams& P, int roles, bool back, bool wide, hipStream_t stream) {
     // those of one KP together
     ScanParams few = P, many = P;
     int n_few = 0, n_many = 0;
     for (int i = 0; i < roles; ++i) {
-        if (P.role[i].K <= 64)
+        if (P.role[i].K <= 64 && !wide)
             few.role[n_few++] = P.role[i];
         else
             many.role[n_many++] = P.role[i];
@@ -1131,10 +1131,10 @@ int gates(const GateParams& P, hipStream_t stream) {
     return std::max(P.state_dim, P.head_dim) <= 64 ? launch_gates<E, 64>(P, stream) : launch_gates<E, 128>(P, stream);
 }
 
-int scans_typed(const ScanParams& P, int32_t dtype, int roles, bool back, hipStream_t stream) {
-    if (dtype == NAVI_POLICY_F32) return scans<float>(P, roles, back, stream);
-    if (dtype == NAVI_POLICY_BF16) return scans<bf16>(P, roles, back, stream);
-    return scans<f16>(P, roles, back, stream);
+int scans_typed(const ScanParams& P, int32_t dtype, int roles, bool back, bool wide, hipStream_t stream) {
+    if (dtype == NAVI_POLICY_F32) return scans<float>(P, roles, back, wide, stream);
+    if (dtype == NAVI_POLICY_BF16) return scans<bf16>(P, roles, back, wide, stream);
+    return scans<f16>(P, roles, back, wide, stream);
 }
 
 float* place_segments(Role& r, const navi_selective_scan_args& a, int32_t segments, float* at) {
@@ -1148,6 +1148,16 @@ float* place_segments(Role& r, const navi_selective_scan_args& a, int32_t segmen
 int32_t keep_from(const navi_selective_scan_args& a) { return a.initial_state ? 0 : 1; }
 int32_t keep_to(const navi_selective_scan_args& a) { return static_cast<int32_t>(chunks_of(a.steps)) - (a.grad_final_state ? 0 : 1); }
 bool states_needed(const navi_selective_scan_args& a) { return keep_from(a) < keep_to(a); }
+
+// The gradients' scans have keys of state_dim and head_dim numbers, and kernels of 64 and 128 rows run one after the
+// other. Where both are needed and the card holds all workgroups of 128 at once, all scans take those: dc and dx then
+// run together (bfloat16 with gradients: 9 x 77 steps of 6 heads of 48 x 80, 51 us on the device and 65 apart; 20 x 40
+// of 4 heads of 128 x 64, 37 and 46).
+bool widened(const navi_selective_scan_args& a, int32_t segments) {
+    const int64_t resident = 256 * (a.dtype == NAVI_POLICY_F32 ? kWorkgroups<float, 128> : a.dtype == NAVI_POLICY_BF16 ? kWorkgroups<bf16, 128> : kWorkgroups<f16, 128>);
+    const int32_t blocks = blocks_of(a.head_dim) + (states_needed(a) ? 1 : 2) * blocks_of(a.state_dim);
+    return (a.state_dim <= 64) != (a.head_dim <= 64) && a.envs * a.heads * segments * blocks <= resident;
+}
 
 // What the backward pass keeps for itself.
 struct Workspace {
@@ -1169,7 +1179,7 @@ Workspace workspace_of(const navi_selective_scan_args& a) {
     w.delta = take(tokens * blocks_of(a.head_dim));
     const bool needed = states_needed(a);
     w.through = take(needed ? sequences * chunks * blocks_of(a.state_dim) * 4 : 0);
-    w.states = take(needed ? sequences * chunks * blocks_of(a.state_dim) * kColumns * (a.head_dim <= 64 ? 64 : 128) : 0);
+    w.states = take(needed ? sequences * chunks * blocks_of(a.state_dim) * kColumns * (a.head_dim <= 64 && !widened(a, segments_of(a, true)) ? 64 : 128) : 0);
     const int64_t heads = a.heads > a.groups ? tokens * a.state_dim : 0;
     w.db = take(heads);
     w.dc = take(heads);
@@ -1224,7 +1234,7 @@ extern "C" int navi_selective_scan(const navi_selective_scan_args* args, void* s
     r.from = args->initial_state;
     r.to = args->final_state;
     place_segments(r, *args, s.P.n_segments, static_cast<float*>(args->scratch));
-    return scans_typed(s.P, args->dtype, 1, false, as_stream(stream));
+    return scans_typed(s.P, args->dtype, 1, false, false, as_stream(stream));
 }
 
 extern "C" int64_t navi_selective_scan_scratch(const navi_selective_scan_args* args) {
@@ -1285,11 +1295,12 @@ extern "C" int navi_selective_scan_backward(const navi_selective_scan_args* args
     GateParams G{};
     G.scan = P;
     // (the db scan reads what the dc scan leaves)
-    int result = scans_typed(P, a.dtype, needed ? 2 : 3, true, as_stream(stream));
+    const bool wide = widened(a, P.n_segments);
+    int result = scans_typed(P, a.dtype, needed ? 2 : 3, true, wide, as_stream(stream));
     if (result != NAVI_POLICY_OK) return result;
     if (needed) {
         P.role[0] = db;
-        result = scans_typed(P, a.dtype, 1, true, as_stream(stream));
+        result = scans_typed(P, a.dtype, 1, true, wide, as_stream(stream));
         if (result != NAVI_POLICY_OK) return result;
     }
     G.x = s.x;
