@@ -344,6 +344,8 @@ int navi_selective_step(const navi_selective_scan_args* args, void* stream);
  * any strides. Results in bfloat16 take products of float16, float32 and float16 ones products of
  * two float16 each (22 bits). A matrix may be written in its place; otherwise what is written shares
  * no memory with what else is written or read. `matrices` is a host array, read during the call.
+ * Factors that can take singular values s past 7.9 before the last step, or |b s^2 + c s^4| past 62 in
+ * one (from s = 1 on), are refused.
  */
 typedef struct navi_orthogonalize_matrix {
     const void* from;

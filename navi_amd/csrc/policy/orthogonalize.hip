@@ -9,8 +9,11 @@
 // both orders. Products run on the matrix cores in float16: of one plane for results of 16 bits of
 // 8-bit precision, of two (hi and what it leaves, 22 bits; the product of the two small ones, 2^-24, is
 // left out) for float32 and float16 results. Numbers are scaled by powers of two so that neither plane
-// leaves float16's range: X (|X| about 1) by 64 sqrt(n), its entries then are about 1 to 64, A and P by
-// 2^10. Sums are float32's; what X keeps of itself (a X, and P's diagonal times X) never goes through
+// leaves float16's range: A and P by 2^10, X (|X| about 1) by 64 sqrt(n), which brings the entries of an X
+// whose size is spread out to about 1 to 64, but by no more than leaves an entry of X's largest singular value
+// (all of it in one place) below 65504: 2^15 with the default factors, whose steps take singular values
+// to 1.2025. An X of a million columns spread out then has entries of 32. Factors that take singular values
+// past 7.9 between steps, or P past 62, are refused: their planes would not hold A or P. Sums are float32's; what X keeps of itself (a X, and P's diagonal times X) never goes through
 // one plane: X is held in two, the diagonal apart in float32. With one plane, what is left of the
 // rounding of A and P to 11 bits is 2 to 5 parts in 10^4 of the result (bfloat16's own: 16); X in one plane too
 // would leave 10^-2 where singular values lie far apart.
@@ -549,6 +552,34 @@ int launched() {
 
 int64_t rounded(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
+// The largest that X's singular values s come to before a step, and b A + c A A in one, whatever X is: at the
+// ends of [0, s] and where the polynomials' slopes are zero. No entry is larger. (X's last values are no plane's.)
+struct Largest {
+    double x, gram, poly;
+};
+
+Largest largest_of(double a, double b, double c, int steps) {
+    Largest most{1.0, 1.0, 0.0};
+    double s = 1.0;  // (|X| <= 1)
+    for (int step = 0; step < steps; ++step) {
+        const double t = s * s;  // of A
+        double poly = std::fabs(b * t + c * t * t), next = std::fabs(s * (a + b * t + c * t * t));
+        const double top = -b / (2.0 * c);
+        if (top > 0.0 && top < t) poly = std::max(poly, std::fabs(top * (b + c * top)));
+        const double root = 9.0 * b * b - 20.0 * a * c;  // of a + 3 b t + 5 c t^2
+        for (const double sign : {-1.0, 1.0}) {
+            const double at = c == 0.0 ? -a / (3.0 * b) : root >= 0.0 ? (-3.0 * b + sign * std::sqrt(root)) / (10.0 * c) : 0.0;
+            if (at > 0.0 && at < t) next = std::max(next, std::fabs(std::sqrt(at) * (a + b * at + c * at * at)));
+        }
+        most = {std::max(most.x, s), std::max(most.gram, t), std::max(most.poly, poly)};
+        if (!(most.gram < 1e30 && most.poly < 1e30)) break;  // (out of any range, and before it is out of double's)
+        s = next;
+    }
+    return most;
+}
+
+constexpr double kLargest = 65504.0 / 1.02;  // of float16; the planes' roundings change singular values by less
+
 // The largest tiles that leave every CU one (256 x 256: a CU holds one workgroup, whose waves have twice the
 // products for what they read of 128's; 64 for matrices of a small policy).
 int tile_of(const navi_orthogonalize_matrix* x, int count) {
@@ -696,6 +727,10 @@ extern "C" int navi_orthogonalize(int32_t count, const navi_orthogonalize_matrix
     if (steps < 1 || steps > 100) return set_error(NAVI_POLICY_E_ARG, "steps must be in [1, 100]");
     if (!(eps >= 0.0f)) return set_error(NAVI_POLICY_E_ARG, "eps must not be negative");
     if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c)) return set_error(NAVI_POLICY_E_ARG, "the factors must be finite");
+    const Largest most = largest_of(a, b, c, steps);
+    if (!(kScaleA * most.gram <= kLargest && kScaleA * most.poly <= kLargest))
+        return set_error(NAVI_POLICY_E_ARG, "the factors take singular values s past 7.9 between steps, or b s^2 + c s^4 past 62");
+    const int most_scale = static_cast<int>(std::floor(std::log2(kLargest / most.x)));
     const int shared = check_apart(matrices, count);
     if (shared != NAVI_POLICY_OK) return shared;
     const int tile = tile_of(matrices, count);
@@ -728,7 +763,7 @@ extern "C" int navi_orthogonalize(int32_t count, const navi_orthogonalize_matrix
             x.n = static_cast<int32_t>(turn ? given.rows : given.cols);
             x.from_dtype = static_cast<int8_t>(given.from_dtype);
             x.to_dtype = static_cast<int8_t>(given.to_dtype);
-            x.scale = static_cast<int8_t>(std::lround(0.5 * std::log2(static_cast<double>(x.n)))) + 6;
+            x.scale = static_cast<int8_t>(std::min(static_cast<int>(std::lround(0.5 * std::log2(static_cast<double>(x.n)))) + 6, most_scale));
             P.first[P.count - 1] = pieces;
             pieces += static_cast<int>(rounded(x.m, tile) / 64 * (rounded(x.n, tile) / 64));
             x.place = static_cast<uint32_t>(place / 256);

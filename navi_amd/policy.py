@@ -877,7 +877,9 @@ def orthogonalize(updates: Iterable[torch.Tensor | None], *, steps: int = 5,
     results go to ``out``, tensors of the same shapes (of any of these types and any strides that do
     not overlap). Tensors that are written share no memory with others. Results in bfloat16 take
     products of float16 (2 to 5 parts in 10^4 before their rounding), others products of two float16
-    each, of float32's precision. A matrix that holds an infinity or NaN comes out without meaning.
+    each, of float32's precision. Factors that can take singular values ``s`` past 7.9 before the last step, or
+    ``b s^2 + c s^4`` past 62 in one, are refused (from ``s = 1`` on; the products' operands hold no more). A
+    matrix that holds an infinity or NaN comes out without meaning.
     """
     steps, eps = int(steps), float(eps)
     a, b, c = (float(x) for x in factors)
