@@ -341,8 +341,8 @@ int navi_selective_step(const navi_selective_scan_args* args, void* stream);
  * `steps` times X <- a X + (b A + c A A) X with A = X X^T (X is G or its transpose, the one with no
  * more rows than columns), into `to` in G's orientation.
  * from: rows x cols numbers with the strides (in elements) of rows and columns, one of them 1; to:
- * any strides. Results in bfloat16 take products of float16, float32 and float16 ones products of
- * two float16 each (22 bits). A matrix may be written in its place; otherwise what is written shares
+ * any strides. Products are of two float16 each (22 bits), but for bfloat16 results of matrices with more
+ * than 256 rows and columns of one (11 bits). A matrix may be written in its place; otherwise what is written shares
  * no memory with what else is written or read. `matrices` is a host array, read during the call.
  * Factors that can take singular values s past 7.9 before the last step, or |b s^2 + c s^4| past 62 in
  * one (from s = 1 on), are refused.

@@ -6,17 +6,18 @@
 //
 // Three products a step, of the form L R^T with both operands' rows along the contracted axis: A and P
 // are symmetric (tiles on and above the diagonal are computed, and stored twice), and X is kept in
-// both orders. Products run on the matrix cores in float16: of one plane for results of 16 bits of
-// 8-bit precision, of two (hi and what it leaves, 22 bits; the product of the two small ones, 2^-24, is
-// left out) for float32 and float16 results. Numbers are scaled by powers of two so that neither plane
+// both orders. Products run on the matrix cores in float16: of one plane for bfloat16 results of matrices with more
+// than 256 rows and columns, of two (hi and what it leaves, 22 bits; the product of the two small ones, 2^-24, is
+// left out) for all others. Numbers are scaled by powers of two so that neither plane
 // leaves float16's range: A and P by 2^10, X (|X| about 1) by 64 sqrt(n), which brings the entries of an X
 // whose size is spread out to about 1 to 64, but by no more than leaves an entry of X's largest singular value
 // (all of it in one place) below 65504: 2^15 with the default factors, whose steps take singular values
 // to 1.2025. An X of a million columns spread out then has entries of 32. Factors that take singular values
 // past 7.9 between steps, or P past 62, are refused: their planes would not hold A or P. Sums are float32's; what X keeps of itself (a X, and P's diagonal times X) never goes through
 // one plane: X is held in two, the diagonal apart in float32. With one plane, what is left of the
-// rounding of A and P to 11 bits is 2 to 5 parts in 10^4 of the result (bfloat16's own: 16); X in one plane too
-// would leave 10^-2 where singular values lie far apart.
+// rounding of A, P and the X in products to 11 bits is 3 to 7 parts in 10^4 of the result before its own rounding
+// (bfloat16's: 16; 6 at widths of 300, 3.3 at 2000); X in one plane too would leave 10^-2 where singular values lie
+// far apart. With two, 1 to 3 parts in 10^6.
 //
 // 8 blocks of width 2000 (32 squares, 16 of twice the length; 9.6e12 operations, of which symmetry spares a third)
 // take 15 ms: A 0.72 ms and P 0.58 at 840 and 800 TFLOP/s of what is computed, X 1.7 ms at 640: a workgroup's 256 x 256
@@ -580,33 +581,42 @@ Largest largest_of(double a, double b, double c, int steps) {
 
 constexpr double kLargest = 65504.0 / 1.02;  // of float16; the planes' roundings change singular values by less
 
+// One plane for bfloat16 results, but for matrices with a short side of up to 256: few products, whose errors do
+// not average out (6 to 16 parts in 10^4 of the result with one plane, as much as its own rounding), and times that
+// the launches are most of (26 matrices of 4 blocks of width 64: 170 us either way; width 256: 204 and 255 with two;
+// 98 of 16 blocks: 621 and 880). From 8 blocks of width 512 on two take 1.8 to 2.4 times as long: 976 us and 1734, of 2000
+// 15.8 ms and 37.1.
+constexpr int64_t kShort = 256;
+
+int planes_of(const navi_orthogonalize_matrix& x) {
+    return x.to_dtype == NAVI_POLICY_BF16 && std::min(x.rows, x.cols) > kShort ? 1 : 2;
+}
+
+bool takes_part(const navi_orthogonalize_matrix& x, int planes) { return x.rows > 0 && x.cols > 0 && planes_of(x) == planes; }
+
 // The largest tiles that leave every CU one (256 x 256: a CU holds one workgroup, whose waves have twice the
-// products for what they read of 128's; 64 for matrices of a small policy).
-int tile_of(const navi_orthogonalize_matrix* x, int count) {
+// products for what they read of 128's; 64 for matrices of a small policy), by the matrices of `planes` planes.
+int tile_of(const navi_orthogonalize_matrix* x, int count, int planes) {
     for (const int tile : {256, 128}) {
         int64_t tiles = 0;
-        for (int i = 0; i < count; ++i) tiles += ((x[i].rows + tile - 1) / tile) * ((x[i].cols + tile - 1) / tile);
+        for (int i = 0; i < count; ++i)
+            if (takes_part(x[i], planes)) tiles += ((x[i].rows + tile - 1) / tile) * ((x[i].cols + tile - 1) / tile);
         if (tiles >= 256) return tile;
     }
     return 64;
 }
-
-int planes_of(const navi_orthogonalize_matrix& x) { return x.to_dtype == NAVI_POLICY_BF16 ? 1 : 2; }
 
 int64_t bytes_of(const navi_orthogonalize_matrix& x, int tile, int planes) {
     const int64_t M = rounded(std::min(x.rows, x.cols), tile), N = rounded(std::max(x.rows, x.cols), tile);
     return 8 * kNormBlocks + 4 * M + 2 * (planes * M * N + 4 * M * N + 2 * planes * M * M);  // (a multiple of 256: M is one of 64)
 }
 
-// Matrices from `at` on that go together: of one number of planes, as many as a launch names and the
-// workspace holds.
-int group_end(const navi_orthogonalize_matrix* x, int count, int at, int tile, int64_t* bytes) {
-    const int planes = planes_of(x[at]);
+// Matrices of `planes` planes from `at` on that go together: as many as a launch names and the workspace holds.
+int group_end(const navi_orthogonalize_matrix* x, int count, int at, int planes, int tile, int64_t* bytes) {
     int64_t total = 0;
     int end = at, named = 0;
     for (; end < count && named < kMatrices; ++end) {
-        if (x[end].rows == 0 || x[end].cols == 0) continue;
-        if (planes_of(x[end]) != planes) break;
+        if (!takes_part(x[end], planes)) continue;
         const int64_t own = bytes_of(x[end], tile, planes);
         if (named > 0 && total + own > kGroupBytes) break;
         total += own;
@@ -702,6 +712,71 @@ int run_group(Params& P, int pieces, int steps, hipStream_t stream) {
     return launched();
 }
 
+// A call whose arguments have been looked over.
+struct Matrices {
+    const navi_orthogonalize_matrix* given;
+    int count, steps;
+    float a, b, c, eps;
+    int most_scale;
+    char* workspace;
+    hipStream_t stream;
+
+    // The matrices of `planes` planes, group after group.
+    int run(int planes) const {
+        const int tile = tile_of(given, count, planes);
+        for (int at = 0; at < count;) {
+            int64_t bytes;
+            const int end = group_end(given, count, at, planes, tile, &bytes);
+            if (bytes > 0 && (!workspace || !aligned(256, workspace)))
+                return set_error(NAVI_POLICY_E_ARG, "workspace must be non-null and 256-byte aligned");
+            Params P{};
+            P.a = a;
+            P.b = b;
+            P.c = c;
+            P.eps = eps;
+            P.workspace = workspace;
+            P.tile = tile;
+            int pieces = 0;
+            int64_t place = 0;
+            for (; at < end; ++at) {
+                if (!takes_part(given[at], planes)) continue;
+                P.first[P.count] = pieces;
+                P.matrix[P.count] = matrix_at(given[at], place);
+                const Matrix& x = P.matrix[P.count++];
+                pieces += static_cast<int>(rounded(x.m, tile) / 64 * (rounded(x.n, tile) / 64));
+                place += bytes_of(given[at], tile, planes);
+            }
+            if (P.count == 0) continue;
+            int code;
+            if (tile == 256)
+                code = planes == 1 ? run_group<256, 1>(P, pieces, steps, stream) : run_group<256, 2>(P, pieces, steps, stream);
+            else if (tile == 128)
+                code = planes == 1 ? run_group<128, 1>(P, pieces, steps, stream) : run_group<128, 2>(P, pieces, steps, stream);
+            else
+                code = planes == 1 ? run_group<64, 1>(P, pieces, steps, stream) : run_group<64, 2>(P, pieces, steps, stream);
+            if (code != NAVI_POLICY_OK) return code;
+        }
+        return NAVI_POLICY_OK;
+    }
+
+    Matrix matrix_at(const navi_orthogonalize_matrix& from, int64_t place) const {
+        Matrix x{};
+        const int turn = from.rows > from.cols;  // X is the transpose
+        x.from = from.from;
+        x.to = from.to;
+        x.turned = from.from_stride[1 ^ turn] != 1;
+        x.from_line = from.from_stride[x.turned ? 1 ^ turn : turn];
+        for (int k = 0; k < 2; ++k) x.to_stride[k] = from.to_stride[k ^ turn];
+        x.m = static_cast<int32_t>(turn ? from.cols : from.rows);
+        x.n = static_cast<int32_t>(turn ? from.rows : from.cols);
+        x.place = static_cast<uint32_t>(place / 256);
+        x.from_dtype = static_cast<int8_t>(from.from_dtype);
+        x.to_dtype = static_cast<int8_t>(from.to_dtype);
+        x.scale = static_cast<int8_t>(std::min(static_cast<int>(std::lround(0.5 * std::log2(static_cast<double>(x.n)))) + 6, most_scale));
+        return x;
+    }
+};
+
 }  // namespace
 }  // namespace navi_policy
 
@@ -709,12 +784,14 @@ extern "C" int64_t navi_orthogonalize_workspace(int32_t count, const navi_orthog
     using namespace navi_policy;
     const int code = check(matrices, count);
     if (code != NAVI_POLICY_OK) return code;
-    const int tile = tile_of(matrices, count);
     int64_t most = 0;
-    for (int at = 0; at < count;) {
-        int64_t bytes;
-        at = group_end(matrices, count, at, tile, &bytes);
-        most = std::max(most, bytes);
+    for (const int planes : {1, 2}) {
+        const int tile = tile_of(matrices, count, planes);
+        for (int at = 0; at < count;) {
+            int64_t bytes;
+            at = group_end(matrices, count, at, planes, tile, &bytes);
+            most = std::max(most, bytes);
+        }
     }
     return most;
 }
@@ -733,52 +810,10 @@ extern "C" int navi_orthogonalize(int32_t count, const navi_orthogonalize_matrix
     const int most_scale = static_cast<int>(std::floor(std::log2(kLargest / most.x)));
     const int shared = check_apart(matrices, count);
     if (shared != NAVI_POLICY_OK) return shared;
-    const int tile = tile_of(matrices, count);
-    for (int at = 0; at < count;) {
-        int64_t bytes;
-        const int end = group_end(matrices, count, at, tile, &bytes);
-        if (bytes > 0 && (!workspace || !aligned(256, workspace)))
-            return set_error(NAVI_POLICY_E_ARG, "workspace must be non-null and 256-byte aligned");
-        Params P{};
-        P.a = a;
-        P.b = b;
-        P.c = c;
-        P.eps = eps;
-        P.workspace = static_cast<char*>(workspace);
-        P.tile = tile;
-        int planes = 1, pieces = 0;
-        int64_t place = 0;
-        for (; at < end; ++at) {
-            const navi_orthogonalize_matrix& given = matrices[at];
-            if (given.rows == 0 || given.cols == 0) continue;
-            planes = planes_of(given);
-            Matrix& x = P.matrix[P.count++];
-            const int turn = given.rows > given.cols;  // X is the transpose
-            x.from = given.from;
-            x.to = given.to;
-            x.turned = given.from_stride[1 ^ turn] != 1;
-            x.from_line = given.from_stride[x.turned ? 1 ^ turn : turn];
-            for (int k = 0; k < 2; ++k) x.to_stride[k] = given.to_stride[k ^ turn];
-            x.m = static_cast<int32_t>(turn ? given.cols : given.rows);
-            x.n = static_cast<int32_t>(turn ? given.rows : given.cols);
-            x.from_dtype = static_cast<int8_t>(given.from_dtype);
-            x.to_dtype = static_cast<int8_t>(given.to_dtype);
-            x.scale = static_cast<int8_t>(std::min(static_cast<int>(std::lround(0.5 * std::log2(static_cast<double>(x.n)))) + 6, most_scale));
-            P.first[P.count - 1] = pieces;
-            pieces += static_cast<int>(rounded(x.m, tile) / 64 * (rounded(x.n, tile) / 64));
-            x.place = static_cast<uint32_t>(place / 256);
-            place += bytes_of(given, tile, planes);
-        }
-        if (P.count == 0) continue;
-        hipStream_t on = as_stream(stream);
-        int result;
-        if (tile == 256)
-            result = planes == 1 ? run_group<256, 1>(P, pieces, steps, on) : run_group<256, 2>(P, pieces, steps, on);
-        else if (tile == 128)
-            result = planes == 1 ? run_group<128, 1>(P, pieces, steps, on) : run_group<128, 2>(P, pieces, steps, on);
-        else
-            result = planes == 1 ? run_group<64, 1>(P, pieces, steps, on) : run_group<64, 2>(P, pieces, steps, on);
-        if (result != NAVI_POLICY_OK) return result;
+    Matrices call{matrices, count, steps, a, b, c, eps, most_scale, static_cast<char*>(workspace), as_stream(stream)};
+    for (const int planes : {1, 2}) {
+        const int code = call.run(planes);
+        if (code != NAVI_POLICY_OK) return code;
     }
     return NAVI_POLICY_OK;
 }

@@ -875,9 +875,10 @@ def orthogonalize(updates: Iterable[torch.Tensor | None], *, steps: int = 5,
     ``updates``: float32, bfloat16 and float16 matrices of one device in any mix of sizes and types
     (None is skipped), each contiguous along its rows or its columns; they are replaced, or the
     results go to ``out``, tensors of the same shapes (of any of these types and any strides that do
-    not overlap). Tensors that are written share no memory with others. Results in bfloat16 take
-    products of float16 (2 to 5 parts in 10^4 before their rounding), others products of two float16
-    each, of float32's precision. Factors that can take singular values ``s`` past 7.9 before the last step, or
+    not overlap). Tensors that are written share no memory with others. Products are of two float16
+    each, of float32's precision, but for bfloat16 results of matrices with more than 256 rows and columns: those
+    take products of one float16 (3 to 7 parts in 10^4 of the result before its rounding, which leaves 16; who
+    wants less gives a float32 ``out``). Factors that can take singular values ``s`` past 7.9 before the last step, or
     ``b s^2 + c s^4`` past 62 in one, are refused (from ``s = 1`` on; the products' operands hold no more). A
     matrix that holds an infinity or NaN comes out without meaning.
     """
