@@ -415,6 +415,7 @@ __global__ __launch_bounds__(1024) void causal_conv_sums_kernel(ConvParams P) {
     }
 }
 
+constexpr int64_t kMostBlocks = (1 << 24) - 1;  // of 256 threads: a launch has fewer than 2^32
 constexpr int64_t kReach = int64_t{1} << 31;  // bytes that a workgroup's 32-bit offsets reach
 
 // How a call is laid out. Segments are as long as leaves 2^16 lanes (of 2^18 that the card holds at
@@ -441,7 +442,7 @@ bool lay_out(ConvParams& P, int vec, bool back) {
     P.items = static_cast<uint32_t>(items);
     P.segments = static_cast<uint32_t>(segments);
     const int64_t down = (items + P.rows - 1) / P.rows;
-    const int64_t most = back ? std::max(1, kPartialBlocks / P.across_blocks) : (1 << 30) / P.across_blocks;
+    const int64_t most = back ? std::max(1, kPartialBlocks / P.across_blocks) : kMostBlocks / P.across_blocks;
     P.down_blocks = static_cast<int32_t>(std::min(down, most));
     P.by_segments = divisor_of(segments);
     P.by_across = divisor_of(P.across);

@@ -312,6 +312,9 @@ inline Divisor divisor_of(int64_t d) {
 
 __device__ inline uint32_t divide(uint32_t n, Divisor by) { return by.m == 0 ? n : __umulhi(n, by.m) >> by.shift; }
 
+// HIP launches fewer than 2^32 threads along an axis of a grid.
+inline bool launchable(int64_t blocks, int64_t threads) { return blocks * threads <= UINT32_MAX; }
+
 inline hipStream_t as_stream(void* stream) { return static_cast<hipStream_t>(stream); }
 
 template <class... P>

@@ -1002,6 +1002,12 @@ Operand operand_of(const void* p, const int64_t (&stride)[3], int64_t bytes, int
 // An output's rows of `heads` heads: stores reach them by 32-bit offsets.
 bool wide_out(const void* p, int32_t dim) { return aligned16(p) && dim % 4 == 0; }
 
+// Workgroups of a launch of scans whose states have up to `blocks` blocks of columns.
+int64_t scan_grid(const ScanParams& P, int64_t segments, int blocks) {
+    const int64_t units = P.envs * (P.heads / P.group) * segments;
+    return (units < 8 ? units : (units + 7) / 8 * 8) * P.group * blocks;
+}
+
 struct Setup {
     ScanParams P{};
     Operand x, b, c, dy;
@@ -1034,6 +1040,9 @@ int setup(const navi_selective_scan_args* args, bool back, Setup& s) {
     P.group = group;
     P.n_chunks = static_cast<int32_t>(chunks_of(a.steps));
     P.n_segments = segments_of(a, back);
+    if (!launchable(scan_grid(P, P.n_segments, blocks_of(back ? std::max(a.head_dim, a.state_dim) : a.head_dim)), 256) ||
+        (back && !launchable(a.envs * a.heads * P.n_chunks, 256)))
+        return set_error(NAVI_POLICY_E_ARG, "too many envs and heads (in the backward pass: and chunks): a launch has fewer than 2^32 threads");
     P.dt = a.dt;
     std::copy(a.dt_stride, a.dt_stride + 3, P.dt_stride);
     P.a = a.a;
@@ -1077,10 +1086,8 @@ int launch_scan(const ScanParams& P, int roles, int segments, hipStream_t stream
     if (err != hipSuccess) return set_error(NAVI_POLICY_E_LAUNCH, "navi_selective_scan: %s", hipGetErrorString(err));
     int blocks = 0;
     for (int i = 0; i < roles; ++i) blocks = std::max(blocks, P.role[i].blocks);
-    const int64_t units = P.envs * (P.heads / P.group) * segments, inner = static_cast<int64_t>(P.group) * blocks;
-    const int64_t grid = (units < 8 ? units : (units + 7) / 8 * 8) * inner;
-    if (grid > INT32_MAX) return set_error(NAVI_POLICY_E_ARG, "navi_selective_scan: too many envs, heads and segments");
-    hipLaunchKernelGGL((selective_scan_kernel<E, KP, kMode>), dim3(static_cast<unsigned>(grid), roles), dim3(256), lds, stream, P);
+    const dim3 grid(static_cast<unsigned>(scan_grid(P, segments, blocks)), roles);  // (setup has looked at it)
+    hipLaunchKernelGGL((selective_scan_kernel<E, KP, kMode>), grid, dim3(256), lds, stream, P);
     return launched("navi_selective_scan");
 }
 

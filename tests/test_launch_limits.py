@@ -1,0 +1,66 @@
+"""A launch has fewer than 2^32 threads: calls of the selective scan that would need more are refused before anything
+runs. Without a GPU: addresses are never read, and calls within the limit end at an argument that is left out."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+
+from navi_amd import _policy_native as native
+
+from .test_block_boundary import PAGE, refused, scan, three
+
+FAR = 1 << 44  # (inputs of that many environments end before the next)
+
+
+def large(**over):
+    places = {name: FAR * (i + 1) for i, name in enumerate(("x", "b", "c", "dt", "a"))}
+    return scan(**{**places, "out": None, "scratch": 9 * PAGE, **over})
+
+
+LIMITS = [  # the last that fits, the first that does not: workgroups of 64 columns of a head, rounded up to 8 envs
+    (dict(envs=(1 << 22) - 8, heads=4, groups=4), dict(envs=1 << 22, heads=4, groups=4)),
+    (dict(envs=(1 << 22) - 8, heads=4, groups=1, b_stride=three(160, 16, 16), c_stride=three(160, 16, 16)),
+     dict(envs=(1 << 22) - 2, heads=4, groups=1, b_stride=three(160, 16, 16), c_stride=three(160, 16, 16))),
+    (dict(envs=(1 << 20) - 8, heads=8, groups=8, head_dim=72, x_stride=three(5760, 576, 72)), dict(envs=1 << 20, heads=8, groups=8, head_dim=128)),
+]
+
+
+@pytest.mark.parametrize("fits, does_not", LIMITS[:2])
+def test_scans(fits, does_not):
+    lib = native.lib()
+    refused(lib.navi_selective_scan(ctypes.byref(large(**fits)), None), "out must be")
+    refused(lib.navi_selective_scan(ctypes.byref(large(**does_not)), None), "fewer than 2^32 threads")
+    refused(lib.navi_selective_scan_backward(ctypes.byref(large(**does_not, grad_out=20 * FAR, grad_out_stride=three(320, 32, 8))), None),
+            "fewer than 2^32 threads")
+
+
+def test_scans_of_two_blocks_of_columns():
+    fits, does_not = LIMITS[2]
+    lib = native.lib()
+    refused(lib.navi_selective_scan(ctypes.byref(large(**fits)), None), "out must be")
+    refused(lib.navi_selective_scan(ctypes.byref(large(**does_not, x_stride=three(10240, 1024, 128))), None), "fewer than 2^32 threads")
+    # backward also those of the state's columns
+    wide = dict(envs=1 << 20, heads=8, groups=8, state_dim=65, b_stride=three(5200, 520, 65), c_stride=three(5200, 520, 65),
+                x_stride=three(640, 64, 8), grad_out=20 * FAR, grad_out_stride=three(640, 64, 8))
+    refused(lib.navi_selective_scan(ctypes.byref(large(**wide)), None), "out must be")
+    refused(lib.navi_selective_scan_backward(ctypes.byref(large(**wide)), None), "fewer than 2^32 threads")
+
+
+def test_gradients_of_many_chunks():
+    """A workgroup a chunk of 64 tokens of a head."""
+    lib = native.lib()
+    size = dict(envs=1024, heads=16, groups=16, x_stride=three(1 << 23, 128, 8), b_stride=three(1 << 24, 256, 16),
+                c_stride=three(1 << 24, 256, 16), grad_out=20 * FAR, grad_out_stride=three(1 << 23, 128, 8))
+    refused(lib.navi_selective_scan(ctypes.byref(large(**size, steps=65536)), None), "out must be")
+    refused(lib.navi_selective_scan_backward(ctypes.byref(large(**size, steps=65536)), None), "fewer than 2^32 threads")
+    refused(lib.navi_selective_scan_backward(ctypes.byref(large(**size, steps=65472)), None), "must be non-null")
+
+
+def test_single_tokens():
+    """Four waves a workgroup, a wave 32 columns of a head (8 where rows are not multiples of four)."""
+    lib = native.lib()
+    one = dict(steps=1, heads=16, groups=16, x_stride=three(128, 128, 8), b_stride=three(256, 256, 16), c_stride=three(256, 256, 16),
+               dt_stride=three(16, 16, 1), initial_state=30 * FAR, final_state=30 * FAR, out=40 * FAR)
+    refused(lib.navi_selective_step(ctypes.byref(large(**{**one, "envs": 1 << 22})), None), "fewer than 2^32 threads")
