@@ -48,7 +48,9 @@ extern "C" {
  * last axis is contiguous, and so are out and the states. g is meant to be <= 0; one of
  * -infinity (below -1e5) starts an episode as `starts` does. An initial state that a start at
  * the first step clears may hold anything. Other inputs are finite: in the chunked form a NaN
- * or infinity may reach every token of its chunk of 64 and what follows them.
+ * or infinity may reach every token of its chunk of 64 and what follows them. A launch has fewer than
+ * 2^32 threads: envs x value_heads x chunks and envs x value_heads x ceil(value_dim / 64) stay below 2^24 (2^23
+ * chunks backward, and 128 columns for 64, where a workgroup has 512 threads).
  */
 typedef struct navi_delta_rule {
     int32_t dtype;              /* NAVI_POLICY_* of q, k, v, out and their gradients */

@@ -1169,7 +1169,6 @@ template <class E, int KP, bool kBack, bool kSummary>
 int walk(const RuleParams& P, unsigned segments, hipStream_t stream) {
     constexpr size_t lds = sizeof(ScanLds<E, KP>);
     const int64_t blocks = (P.r.envs * P.r.value_heads + 7) / 8 * 8 * (kSummary ? P.summary_blocks : P.blocks);
-    if (blocks > INT32_MAX) return set_error(NAVI_POLICY_E_ARG, "envs * value_heads * value_dim is too large");
     const dim3 grid(static_cast<unsigned>(blocks), 1, segments), threads(kWalkThreads<E, KP>);
     if constexpr (kBack)
         hipLaunchKernelGGL((delta_reverse_kernel<E, KP, kSummary>), grid, threads, lds, stream, P);
@@ -1302,7 +1301,7 @@ int check_apart(const navi_delta_rule* r, bool in_place) {
 
 namespace {
 
-int setup(const navi_delta_rule* r, RuleParams& P) {
+int setup(const navi_delta_rule* r, bool back, RuleParams& P) {
     const int code = check_rule(r);
     if (code != NAVI_POLICY_OK) return code;
     P.r = *r;
@@ -1314,6 +1313,11 @@ int setup(const navi_delta_rule* r, RuleParams& P) {
     const int64_t bytes = r->dtype == NAVI_POLICY_F32 ? 4 : 2;
     if (r->envs * r->value_heads * chunks_of(r->steps) > INT32_MAX)
         return set_error(NAVI_POLICY_E_ARG, "envs * value_heads * chunks must be below 2^31");
+    const int64_t sequences = r->envs * r->value_heads, walks = (sequences + 7) / 8 * 8 * std::max(P.blocks, P.n_segments > 1 ? P.summary_blocks : 0);
+    const int walk_threads = r->dtype == NAVI_POLICY_F32 && r->key_dim > 64 ? kWalkThreads<float, 128> : kWalkThreads<bf16, 64>;
+    const int chunk_threads = !back ? 256 : 64 * (r->dtype == NAVI_POLICY_F16 && r->key_dim <= 64 ? kGradientWaves<f16, 64> : kGradientWaves<bf16, 64>);
+    if (!launchable(walks, walk_threads) || !launchable(sequences * P.n_chunks, chunk_threads))
+        return set_error(NAVI_POLICY_E_ARG, "envs * value_heads * chunks or * value_dim is too large (a launch has fewer than 2^32 threads)");
     if (P.n_chunks > 0 && (!r->matrices || !aligned16(r->matrices)))
         return set_error(NAVI_POLICY_E_ARG, "matrices must be non-null and 16-byte aligned");
     if (r->value_heads > kFarthest / 4 / std::max(r->value_dim, r->key_dim))
@@ -1345,7 +1349,7 @@ using namespace navi_policy;
 
 extern "C" int navi_delta_forward(const navi_delta_rule* rule, void* stream) {
     RuleParams P{};
-    const int code = setup(rule, P);
+    const int code = setup(rule, false, P);
     if (code != NAVI_POLICY_OK) return code < 0 ? code : NAVI_POLICY_OK;
     if (!rule->states != !rule->updates && P.n_chunks > 1)
         return set_error(NAVI_POLICY_E_ARG, "states and updates are saved together or not at all");
@@ -1378,7 +1382,7 @@ extern "C" int64_t navi_delta_workspace(const navi_delta_rule* rule) {
 
 extern "C" int navi_delta_backward(const navi_delta_rule* rule, const navi_delta_gradients* gradients, void* stream) {
     RuleParams P{};
-    const int code = setup(rule, P);
+    const int code = setup(rule, true, P);
     if (code != NAVI_POLICY_OK) return code < 0 ? code : NAVI_POLICY_OK;
     if (!gradients) return set_error(NAVI_POLICY_E_ARG, "gradients must be non-null");
     P.d = *gradients;

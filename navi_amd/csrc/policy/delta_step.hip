@@ -150,7 +150,8 @@ int step(StepParams& P, hipStream_t stream) {
     P.units = P.r.envs * P.r.value_heads * P.blocks;
     const unsigned threads = P.units >= 4096 ? 256 : 64;  // few waves: each on a CU of its own
     const int64_t blocks = (P.units + threads / 64 - 1) / (threads / 64);
-    if (blocks > INT32_MAX) return set_error(NAVI_POLICY_E_ARG, "navi_delta_step: too many envs, heads and columns");
+    if (!launchable(blocks, threads))
+        return set_error(NAVI_POLICY_E_ARG, "navi_delta_step: too many envs, heads and columns (a launch has fewer than 2^32 threads)");
     hipLaunchKernelGGL((delta_step_kernel<E, kRows, kColumns>), dim3(static_cast<unsigned>(blocks)), dim3(threads), 0, stream, P);
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess)

@@ -1,5 +1,5 @@
-"""A launch has fewer than 2^32 threads: calls of the selective scan that would need more are refused before anything
-runs. Without a GPU: addresses are never read, and calls within the limit end at an argument that is left out."""
+"""A launch has fewer than 2^32 threads: calls of the selective scan and the gated delta rule that would need more are
+refused before anything runs (a larger grid is cut off without an error). Without a GPU: addresses are never read, and calls within the limit end at an argument that is left out."""
 
 from __future__ import annotations
 
@@ -10,6 +10,7 @@ import pytest
 from navi_amd import _policy_native as native
 
 from .test_block_boundary import PAGE, refused, scan, three
+from .test_policy_boundary import rule
 
 FAR = 1 << 44  # (inputs of that many environments end before the next)
 
@@ -64,3 +65,37 @@ def test_single_tokens():
     one = dict(steps=1, heads=16, groups=16, x_stride=three(128, 128, 8), b_stride=three(256, 256, 16), c_stride=three(256, 256, 16),
                dt_stride=three(16, 16, 1), initial_state=30 * FAR, final_state=30 * FAR, out=40 * FAR)
     refused(lib.navi_selective_step(ctypes.byref(large(**{**one, "envs": 1 << 22})), None), "fewer than 2^32 threads")
+
+
+@pytest.mark.parametrize("fits, does_not", [
+    (dict(envs=(1 << 22) - 8, steps=1), dict(envs=1 << 22, steps=1)),
+    (dict(envs=(1 << 20) - 8, steps=1, value_dim=256), dict(envs=1 << 20, steps=1, value_dim=256)),
+    (dict(envs=1024, steps=64 * 4095), dict(envs=1024, steps=64 * 4096)),
+    (dict(envs=(1 << 21) - 8, steps=1, key_dim=100, value_dim=129), dict(envs=1 << 21, steps=1, key_dim=100, value_dim=129)),  # (512 threads)
+])
+def test_delta_rules(fits, does_not):
+    lib = native.lib()
+    strides = dict(q_stride=three(1 << 40, 1 << 10, 128), k_stride=three(1 << 40, 1 << 10, 128), v_stride=three(1 << 40, 1 << 10, 256))
+    if "value_dim" not in fits:
+        assert lib.navi_delta_forward(ctypes.byref(rule(**strides, **fits, states=4096)), None) == native.NAVI_POLICY_E_ARG
+        assert "2^32" not in native.last_error()
+    refused(lib.navi_delta_forward(ctypes.byref(rule(**strides, **does_not)), None), "fewer than 2^32 threads")
+    gradients = native.DeltaGradients()
+    refused(lib.navi_delta_backward(ctypes.byref(rule(**strides, **does_not)), ctypes.byref(gradients), None), "fewer than 2^32 threads")
+
+
+def test_gradients_of_delta_rules():
+    """512 threads a chunk, 256 for float16 and keys of up to 64."""
+    lib = native.lib()
+    strides = dict(q_stride=three(1 << 40, 1 << 10, 128), k_stride=three(1 << 40, 1 << 10, 128), v_stride=three(1 << 40, 1 << 10, 256))
+    gradients = native.DeltaGradients()
+    for dtype, key_dim, chunks in ((native.F32, 64, 2047), (native.BF16, 64, 2047), (native.F16, 64, 4095), (native.F16, 65, 2047)):
+        size = dict(envs=1024, dtype=dtype, key_dim=key_dim)
+        refused(lib.navi_delta_backward(ctypes.byref(rule(**strides, **size, steps=64 * chunks)), ctypes.byref(gradients), None), "must be non-null")
+        refused(lib.navi_delta_backward(ctypes.byref(rule(**strides, **size, steps=64 * chunks + 1)), ctypes.byref(gradients), None),
+                "fewer than 2^32 threads")
+
+
+def test_single_tokens_of_delta_rules():
+    assert native.lib().navi_delta_step(ctypes.byref(rule(envs=1 << 24, steps=1, final_state=1 << 50, out=1 << 55)), None) == native.NAVI_POLICY_E_ARG
+    assert "fewer than 2^32 threads" in native.last_error()
