@@ -159,6 +159,10 @@ class SelectivePolicy(torch.nn.Module):
     def initial_state(self, actors: int) -> tuple[torch.Tensor, ...]:
         return tuple(t for block in self.blocks for t in block.initial_state(actors))
 
+    def filters(self) -> list[torch.nn.Parameter]:
+        """The convolutions' taps: a filter a channel, no linear map."""
+        return [block.taps_weight for block in self.blocks]
+
     def forward(self, x, starts, positions=None, state=None):
         """Rollouts, as ``MemoryPolicy.forward`` (places in the episode are not read)."""
         stream = F.gelu(self.encode(x))
@@ -180,12 +184,21 @@ class SelectivePolicy(torch.nn.Module):
 class MatrixUpdates:
     """An optimizer: weight matrices are stepped by their orthogonalised momenta, all of them in one
     call, the other parameters by Adam. A matrix's step has the root-mean-square of ``lr * 0.2`` whatever its
-    shape (an orthogonalised ``m x n`` matrix has ``1 / sqrt(max(m, n))``)."""
+    shape (an orthogonalised ``m x n`` matrix has ``1 / sqrt(max(m, n))``). ``filters``: those of the parameters that
+    are two-dimensional but no linear map (a convolution's taps, a filter a row): they are Adam's too."""
 
-    def __init__(self, parameters, lr: float = 1e-3, momentum: float = 0.95) -> None:
+    @classmethod
+    def of(cls, model: torch.nn.Module, lr: float = 1e-3) -> "MatrixUpdates":
+        """For a policy's parameters, with the filters that it names, if any."""
+        return cls(model.parameters(), lr=lr, filters=model.filters() if hasattr(model, "filters") else ())
+
+    def __init__(self, parameters, lr: float = 1e-3, momentum: float = 0.95, filters=()) -> None:
         parameters = list(parameters)
-        self.matrices = [p for p in parameters if p.dim() == 2]
-        others = [p for p in parameters if p.dim() != 2]
+        apart = {id(p) for p in filters}
+        if not apart <= {id(p) for p in parameters}:
+            raise ValueError("filters must be among the parameters")
+        self.matrices = [p for p in parameters if p.dim() == 2 and id(p) not in apart]
+        others = [p for p in parameters if p.dim() != 2 or id(p) in apart]
         self.adam = torch.optim.Adam(others, lr=lr) if others else None
         self.lr, self.momentum = lr, momentum
         self.held = [torch.zeros_like(p) for p in self.matrices]
@@ -212,7 +225,7 @@ class MatrixUpdates:
 
 
 CORES = {"delta": MemoryPolicy, "selective": SelectivePolicy}
-OPTIMIZERS = {"adam": torch.optim.Adam, "orthogonal": MatrixUpdates}
+OPTIMIZERS = {"adam": lambda model, lr: torch.optim.Adam(model.parameters(), lr=lr), "orthogonal": MatrixUpdates.of}
 
 
 def copied(state):
@@ -274,7 +287,7 @@ def run(scenes, *, actors: int, steps: int, updates: int, azimuth_bins: int, ele
     harness = ObservationHarness(scenes, actors, azimuth_bins, elevation_bins, max_distance, sdf_max_steps, seed=seed)
     more = {"positions": updates * steps + 1} if core == "delta" else {}
     model = CORES[core](dtype=dtype, device=harness.dev, **more)
-    stepper = OPTIMIZERS[optimizer](model.parameters(), lr=1e-3)
+    stepper = OPTIMIZERS[optimizer](model, lr=1e-3)
     state = model.initial_state(actors)
     starts = torch.ones(actors, dtype=torch.bool, device=harness.dev)
     positions = torch.zeros(actors, dtype=torch.int32, device=harness.dev)
