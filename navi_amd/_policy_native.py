@@ -2,7 +2,8 @@
 and ``calls``, the extension that makes calls of some of it in one step (``csrc/policy/calls.cpp``).
 
 Importing this module loads the HIP library and raises ``ImportError`` when it has not been
-built; there is no fallback.
+built; there is no fallback. Where the extension is missing, or made for another PyTorch, its operators
+(selective scan, convolution, block norms) raise, and all others work.
 """
 
 from __future__ import annotations
@@ -30,12 +31,10 @@ NORM_PARTIALS = 2048
 MAX_TAPS, MAX_BLOCK_WIDTH, MAX_STATE_DIM = 4, 8192, 128
 ACT_NONE, ACT_SILU = 0, 1
 
-for _path in (LIB_PATH, CALLS_PATH):
-    if not _path.exists():
-        raise ImportError(
-            f"{_path.name} not found at {_path}; build it with "
-            "`python -c 'import __graft_entry__ as g; g.build()'` (or `make -C navi_amd/csrc/policy`)."
-        )
+_BUILD = "build it with `python -c 'import __graft_entry__ as g; g.build()'` (or `make -C navi_amd/csrc/policy`)."
+
+if not LIB_PATH.exists():
+    raise ImportError(f"{LIB_PATH.name} not found at {LIB_PATH}; {_BUILD}")
 _lib = ctypes.CDLL(str(LIB_PATH))
 
 _vp, _i32, _i64, _f32 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float
@@ -147,9 +146,24 @@ _lib.navi_clip_grad_norm.restype = ctypes.c_int
 _lib.navi_clip_grad_norm.argtypes = [_i32, _vp, _vp, _vp, _vp, _f32, _f32, _vp, _vp, _vp]
 
 
+class _NoCalls:
+    """In the extension's place where there is none: whoever asks for one of its calls is told why."""
+
+    def __init__(self, why: str) -> None:
+        self._why = why
+
+    def __getattr__(self, name: str):
+        raise RuntimeError(self._why)
+
+
 def _load_calls():
+    if not CALLS_PATH.exists():
+        return _NoCalls(f"{CALLS_PATH.name} not found at {CALLS_PATH}; {_BUILD}")
     loader = importlib.machinery.ExtensionFileLoader("_policy_calls", str(CALLS_PATH))
-    module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_policy_calls", loader))
+    try:
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_policy_calls", loader))
+    except ImportError as e:  # (made for another PyTorch or Python)
+        return _NoCalls(f"{CALLS_PATH.name} does not load ({e}); {_BUILD}")
     module.bind(*[ctypes.cast(getattr(_lib, name), _vp).value
                   for name in ("navi_selective_step", "navi_selective_scan", "navi_selective_scan_backward",
                                "navi_selective_scan_scratch", "navi_selective_scan_workspace", "navi_causal_conv",
