@@ -121,7 +121,7 @@ def _packer(structure) -> struct.Struct:
 
 
 PACK_RULE, PACK_GRADIENTS, PACK_NORM = (_packer(s).pack for s in (DeltaRule, DeltaGradients, QkNorm))
-PACK_CONV, PACK_BLOCK, PACK_SCAN = (_packer(s).pack for s in (CausalConv, BlockNorm, SelectiveScan))
+PACK_CONV, PACK_SCAN = (_packer(s).pack for s in (CausalConv, SelectiveScan))
 PACK_MATRIX = _packer(OrthogonalizeMatrix).pack
 
 _lib.navi_policy_last_error.restype = ctypes.c_char_p
