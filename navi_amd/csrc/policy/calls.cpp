@@ -298,6 +298,13 @@ Tensor rows_apart(const Tensor& t) {
     return t.contiguous();
 }
 
+// An env's steps within 2 GiB, which the convolution's offsets reach (rows of one element for masks).
+Tensor steps_near(const Tensor& t) {
+    if (!t.defined() || t.size(1) <= 1) return t;
+    const int64_t row = t.dim() > 2 ? t.size(2) : 1;
+    return t.stride(1) < ((int64_t{1} << 31) / int64_t(t.element_size()) - row) / t.size(1) ? t : t.contiguous();
+}
+
 // The device of a call is the current one during it: its stream.
 struct On {
     c10::DeviceGuard guard;
@@ -507,7 +514,7 @@ struct ConvolutionFunction : torch::autograd::Function<ConvolutionFunction> {
         const variable_list saved = ctx->get_saved_variables();
         const Convolution g(saved, ctx->saved_data["activation"].toInt());
         const On on(g.x);
-        grad = grad.defined() ? dense(grad) : like(g.x).zero_();
+        grad = grad.defined() ? steps_near(dense(grad)) : like(g.x).zero_();
         if (grad_window.defined()) grad_window = plain(grad_window).contiguous();
         Tensor d_x = like(g.x), d_weight = like(ctx, saved, 1), d_bias = like(ctx, saved, 2),
                d_window = like(ctx, saved, 3);
@@ -533,10 +540,10 @@ struct ConvolutionFunction : torch::autograd::Function<ConvolutionFunction> {
 };
 
 PyObject* conv_of(const variable_list& in, int64_t activation, bool return_window) {
+    const Tensor x = steps_near(in[0]), starts = steps_near(in[4]);
     if (records({&in[0], &in[1], &in[2], &in[3]}))
-        return results(ConvolutionFunction::apply(in[0], in[1], maybe(in[2]), maybe(in[3]), maybe(in[4]), activation,
-                                                  return_window));
-    return results(Convolution(in, activation).forward(return_window));
+        return results(ConvolutionFunction::apply(x, in[1], maybe(in[2]), maybe(in[3]), maybe(starts), activation, return_window));
+    return results(Convolution({x, in[1], in[2], in[3], starts}, activation).forward(return_window));
 }
 
 // conv(x, weight, bias, window, starts, activation's number, return_window): out, or (out, window after).
