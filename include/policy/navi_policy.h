@@ -287,16 +287,17 @@ int64_t navi_block_norm_workspace(const navi_block_norm_args* args);
  * inputs are finite: in the chunked form a NaN or infinity may reach every token of its chunk of
  * NAVI_POLICY_CHUNK and what follows them.
  *
- * heads: at most 16384. A launch has fewer than 2^32 threads, 256 a workgroup: scans take envs (rounded up to 8 /
+ * A launch has fewer than 2^32 threads, 256 a workgroup: scans take envs (rounded up to 8 /
  * groups where there are more) x heads x ceil(head_dim / 64) workgroups below 2^24, backward also with state_dim for
  * head_dim, and envs x heads x chunks; single tokens a wave of 64 for each 32 columns of a head (8 where head_dim is not
  * a multiple of four or states are not aligned to 16 bytes), below 2^26.
  */
 #define NAVI_POLICY_MAX_STATE_DIM 128 /* and head_dim */
+#define NAVI_POLICY_MAX_HEADS 16384
 
 typedef struct navi_selective_scan_args {
     int32_t dtype;
-    int32_t heads, groups;
+    int32_t heads, groups; /* heads: 1 to NAVI_POLICY_MAX_HEADS, a multiple of groups */
     int32_t state_dim, head_dim;
     int64_t envs, steps;
     const void* x;

@@ -28,7 +28,7 @@ F32, BF16, F16 = 0, 1, 2
 MAX_KEY_DIM, MAX_NORM_DIM, CHUNK, CHUNK_MATRICES = 128, 1024, 64, 5248
 NORM_RMS, NORM_L2 = 0, 1
 NORM_PARTIALS = 2048
-MAX_TAPS, MAX_BLOCK_WIDTH, MAX_STATE_DIM = 4, 8192, 128
+MAX_TAPS, MAX_BLOCK_WIDTH, MAX_STATE_DIM, MAX_HEADS = 4, 8192, 128, 16384
 ACT_NONE, ACT_SILU = 0, 1
 
 _BUILD = "build it with `python -c 'import __graft_entry__ as g; g.build()'` (or `make -C navi_amd/csrc/policy`)."

@@ -174,7 +174,7 @@ PyObject* selective_step(PyObject*, PyObject* const* v, Py_ssize_t n) {
         state->scalar_type() != at::kFloat || b->device() != device || c->device() != device || dt->device() != device ||
         state->device() != device || b->size(0) != envs || c->sizes() != b->sizes() || dt->size(0) != envs ||
         dt->size(1) != heads || groups <= 0 || groups > heads || heads % groups || width <= 0 ||
-        width > NAVI_POLICY_MAX_STATE_DIM || dim <= 0 || dim > NAVI_POLICY_MAX_STATE_DIM || heads > INT32_MAX ||
+        width > NAVI_POLICY_MAX_STATE_DIM || dim <= 0 || dim > NAVI_POLICY_MAX_STATE_DIM || heads > NAVI_POLICY_MAX_HEADS ||
         !dense_last(*x) || !dense_last(*b) || !dense_last(*c) || state->size(0) != envs || state->size(1) != heads ||
         state->size(2) != dim || state->size(3) != width || !state->is_contiguous() || !vector(a, device, heads) ||
         !vector(d, device, heads) || !vector(dt_bias, device, heads) || !mask(starts, device, envs) ||
@@ -458,7 +458,7 @@ PyObject* selective_scan(PyObject*, PyObject* const* v, Py_ssize_t n) {
     if (b.scalar_type() != x.scalar_type() || c.scalar_type() != x.scalar_type() || dt.scalar_type() != at::kFloat ||
         b.device() != device || c.device() != device || dt.device() != device || b.size(0) != envs || b.size(1) != steps ||
         c.sizes() != b.sizes() || dt.size(0) != envs || dt.size(1) != steps || dt.size(2) != heads || groups <= 0 ||
-        groups > heads || heads % groups || heads > INT32_MAX || width <= 0 || width > NAVI_POLICY_MAX_STATE_DIM || dim <= 0 ||
+        groups > heads || heads % groups || heads > NAVI_POLICY_MAX_HEADS || width <= 0 || width > NAVI_POLICY_MAX_STATE_DIM || dim <= 0 ||
         dim > NAVI_POLICY_MAX_STATE_DIM || !dense_last(x) || !dense_last(b) || !dense_last(c) || !vector(in[2], device, heads) ||
         !vector(in[5], device, heads) || !vector(in[6], device, heads) || !mask(in[8], x) ||
         (state.defined() && (state.scalar_type() != at::kFloat || state.device() != device || state.dim() != 4 ||

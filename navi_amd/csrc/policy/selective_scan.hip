@@ -972,7 +972,7 @@ int check(const navi_selective_scan_args* a) {
         return set_error(NAVI_POLICY_E_ARG, "heads must be a positive multiple of groups");
     if (a->state_dim <= 0 || a->state_dim > NAVI_POLICY_MAX_STATE_DIM || a->head_dim <= 0 || a->head_dim > NAVI_POLICY_MAX_STATE_DIM)
         return set_error(NAVI_POLICY_E_ARG, "state_dim and head_dim must be in [1, %d]", NAVI_POLICY_MAX_STATE_DIM);
-    if (a->heads > 16384) return set_error(NAVI_POLICY_E_ARG, "heads must be at most 16384");
+    if (a->heads > NAVI_POLICY_MAX_HEADS) return set_error(NAVI_POLICY_E_ARG, "heads must be at most %d", NAVI_POLICY_MAX_HEADS);
     if (a->envs < 0 || a->steps < 0) return set_error(NAVI_POLICY_E_ARG, "envs and steps must not be negative");
     if (a->steps > INT32_MAX || a->envs > INT32_MAX / 4 / a->heads)
         return set_error(NAVI_POLICY_E_ARG, "steps and 4 * envs * heads must be below 2^31");

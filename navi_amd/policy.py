@@ -488,7 +488,7 @@ def _fine_scan(x, dt, a, b, c, d, dt_bias, starts) -> bool:
         (heads, head_dim), (groups, state_dim) = x.shape[-2:], b.shape[-2:]
         return (dtype in _DTYPES and b.dtype is dtype and c.dtype is dtype and device.type == "cuda" and b.device == device
                 and c.device == device and dt.device == device and dt.dtype is torch.float32 and dt.shape == x.shape[:-1]
-                and b.shape[:-2] == lead and c.shape == b.shape and 0 < groups <= heads and heads % groups == 0
+                and b.shape[:-2] == lead and c.shape == b.shape and 0 < groups <= heads <= _native.MAX_HEADS and heads % groups == 0
                 and 0 < head_dim <= _native.MAX_STATE_DIM and 0 < state_dim <= _native.MAX_STATE_DIM
                 and (x.stride(-1) == 1 or head_dim == 1) and (b.stride(-1) == 1 or state_dim == 1)
                 and (c.stride(-1) == 1 or state_dim == 1) and a is not None
@@ -513,6 +513,7 @@ def _check_scan(x, dt, a, b, c, d, dt_bias, starts, lead: tuple[str, ...]) -> No
     _check(b.shape == c.shape and b.shape[:n] == x.shape[:n], f"b and c must both be [{shape}, Groups, StateDim]")
     heads, groups = x.size(n), b.size(n)
     _check(heads > 0 and groups > 0 and heads % groups == 0, "the heads must be a multiple of the groups")
+    _check(heads <= _native.MAX_HEADS, f"the heads must be at most {_native.MAX_HEADS}")
     _check(0 < x.size(-1) <= _native.MAX_STATE_DIM and 0 < b.size(-1) <= _native.MAX_STATE_DIM,
            f"the head and state dimensions must be in [1, {_native.MAX_STATE_DIM}]")
     _check(dt.shape == x.shape[:-1], f"dt must be [{shape}, Heads]")
@@ -550,7 +551,7 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, a: torch.Tensor, b: torch.
     numbers: ``S <- exp(beta a) S + beta b x^T``, ``y = S^T c + d x``.
     ``x``: ``[Envs, Steps, Heads, HeadDim]`` in float32, bfloat16 or float16, ``b``, ``c``:
     ``[Envs, Steps, Groups, StateDim]`` of the same type, with ``Heads`` a multiple of ``Groups``
-    (head h reads group ``h // (Heads // Groups)``); both dimensions up to 128. ``dt``:
+    (head h reads group ``h // (Heads // Groups)``) and at most 16384; both dimensions up to 128. ``dt``:
     ``[Envs, Steps, Heads]`` float32; ``a`` (rates, at most 0), ``d`` and ``dt_bias`` (zeros by
     default): ``[Heads]`` float32. ``starts``: ``[Envs, Steps]`` bool or uint8, tokens that begin an
     episode: the state before one is forgotten (at the first step, whatever it holds).
