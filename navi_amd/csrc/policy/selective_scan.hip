@@ -304,8 +304,7 @@ __device__ inline f4 four_of(const uint16_t (&rows)[N][kChunk][kPitch], int row,
     return x;
 }
 
-// The tiles of a triangle that a wave computes: its own on the diagonal, and of those below one or two
-// (i and j, two bits each, for n = 1 and 2; 3 for none).
+// The same of values that are float32.
 template <int kPitch>
 __device__ inline f4 four_of(const float (&rows)[kChunk][kPitch], int row, int c, int g) {
     return *reinterpret_cast<const f4*>(&rows[row][16 * c + 4 * g]);
@@ -318,6 +317,8 @@ __device__ inline void column_values(int lane, const float (&v)[kChunk][kPitch],
     for (int s = 0; s < 8; ++s) x[s] = v[32 * m + 16 * (s >> 2) + 4 * (lane >> 4) + (s & 3)][16 * wave + (lane & 15)];
 }
 
+// The tiles of a triangle that a wave computes: its own on the diagonal, and of those below one or two
+// (i and j, two bits each, for n = 1 and 2; 3 for none).
 __device__ inline int tile_of_wave(int wave, int n) {
     constexpr uint32_t kBelow = 0x84u | 0xc9u << 8 | 0x3du << 16 | 0x3eu << 24;
     return n == 0 ? 5 * wave : kBelow >> (8 * wave + 4 * (n - 1)) & 15;
@@ -432,7 +433,8 @@ struct FourFetch {
     }
 };
 
-// Workgroups that a CU's LDS holds: 42 KB each for bfloat16 and 64, up to 137 KB for float32 and 128.
+// Workgroups that a CU's LDS holds and its registers allow: 36 KiB each for bfloat16 and 64 (40 with gradients), up to
+// 122 (126) for float32 and 128.
 template <class E, int KP>
 inline constexpr int kWorkgroups = kPlanes<E> == 1 ? (KP == 64 ? 3 : 2) : KP == 64 ? 2 : 1;
 
@@ -577,7 +579,7 @@ __global__ __launch_bounds__(256, (kWorkgroups<E, KP>)) void selective_scan_kern
                         operand_rows(lane, lds.q, 16 * i, m, a);
                         o[i] = mma(b, a, o[i]);  // (transposed: the operands hold rows and columns alike)
                     }
-                    }
+                }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) o[i] = lds.gates.e[16 * i + (lane & 15)] * o[i];
             }
@@ -636,7 +638,7 @@ __global__ __launch_bounds__(256, (kWorkgroups<E, KP>)) void selective_scan_kern
                         operand_triangle<3>(lane, lds.p, i, 1, a);
                         o[i] = mma(value[1], a, o[i]);
                     }
-                    }
+                }
             }
         }
         if constexpr (kSummary) continue;
