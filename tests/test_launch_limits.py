@@ -4,6 +4,7 @@ refused before anything runs (a larger grid is cut off without an error). Withou
 from __future__ import annotations
 
 import ctypes
+from pathlib import Path
 
 import pytest
 
@@ -99,3 +100,8 @@ def test_gradients_of_delta_rules():
 def test_single_tokens_of_delta_rules():
     assert native.lib().navi_delta_step(ctypes.byref(rule(envs=1 << 24, steps=1, final_state=1 << 50, out=1 << 55)), None) == native.NAVI_POLICY_E_ARG
     assert "fewer than 2^32 threads" in native.last_error()
+
+
+def test_heads_are_those_of_the_header():
+    header = (Path(__file__).resolve().parents[1] / "include" / "policy" / "navi_policy.h").read_text()
+    assert f"#define NAVI_POLICY_MAX_HEADS {native.MAX_HEADS}\n" in header
