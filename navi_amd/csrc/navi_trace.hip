@@ -187,7 +187,8 @@ int launch_raw(const uint64_t* pool, uint64_t n_words, Box dom, const navi_scene
                int64_t n_rays, int32_t max_steps, float max_distance, float hit_eps, void* stream) {
     const int threads = 256;
     const int64_t blocks = (n_rays + threads - 1) / threads;
-    if (blocks > 0x7fffffff) return set_error(NAVI_E_ARG, "too many rays for one launch");
+    // (a grid of 2^32 threads or more is cut off without an error)
+    if (blocks * threads > UINT32_MAX) return set_error(NAVI_E_ARG, "too many rays for one launch (fewer than 2^32 - 255)");
     g_last_launch = navi_launch_info{};
     g_last_launch.kernels = NAVI_KERNEL_RAW;
     g_last_launch.pair = -1;

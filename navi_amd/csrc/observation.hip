@@ -558,6 +558,8 @@ int launch_as(const PostParams& P, hipStream_t stream, size_t lds) {
     const int64_t point_blocks = P.points_per_env > 0 ? 0 : (static_cast<int64_t>(P.n_points) + kThreads - 1) / kThreads;
     const int64_t blocks = static_cast<int64_t>(P.n_envs) + point_blocks;
     if (blocks == 0) return NAVI_OK;
+    // (a grid of 2^32 threads or more is cut off without an error)
+    if (blocks * kThreads > UINT32_MAX) return set_error(NAVI_E_ARG, "too many envs and points for one launch (below 2^23 envs)");
     PostParams Q = P;
     Q.point_blocks = static_cast<int32_t>(point_blocks);
     hipLaunchKernelGGL((observation_kernel<kObs, kDelta, kF16, kWide, kThreads>), dim3(static_cast<unsigned>(blocks)),

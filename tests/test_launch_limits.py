@@ -1,4 +1,4 @@
-"""A launch has fewer than 2^32 threads: calls of the selective scan and the gated delta rule that would need more are
+"""A launch has fewer than 2^32 threads: calls of the selective scan, the gated delta rule, the raw tracer and the observation pass that would need more are
 refused before anything runs (a larger grid is cut off without an error). Without a GPU: addresses are never read, and calls within the limit end at an argument that is left out."""
 
 from __future__ import annotations
@@ -8,6 +8,7 @@ from pathlib import Path
 
 import pytest
 
+from navi_amd import _native as tracer
 from navi_amd import _policy_native as native
 
 from .test_block_boundary import PAGE, refused, scan, three
@@ -105,3 +106,14 @@ def test_single_tokens_of_delta_rules():
 def test_heads_are_those_of_the_header():
     header = (Path(__file__).resolve().parents[1] / "include" / "policy" / "navi_policy.h").read_text()
     assert f"#define NAVI_POLICY_MAX_HEADS {native.MAX_HEADS}\n" in header
+
+
+def test_rays_and_observations():
+    """The raw tracer takes a ray a thread, the observation pass a workgroup of 512 an environment."""
+    lib, f3 = tracer.lib(), tracer.float3
+    for rays in ((1 << 32) - 255, 1 << 32, 1 << 36):
+        code = lib.navi_cast_rays(4096, 1, 4096, 4096, 4096, 4096, rays, 4, 1.0, f3([0, 0, 0]), f3([1, 1, 1]), 1, 0.01, None, None, None)
+        assert code == tracer.NAVI_E_ARG and "too many rays" in tracer.last_error()
+    for envs in (1 << 23, (1 << 31) - 1):
+        seen = tracer.Observation(distances=4096, semantics=4096, n_envs=envs, azimuth_bins=4, elevation_bins=2, max_distance=1.0, obs=1 << 50)
+        assert lib.navi_observe(ctypes.byref(seen), None, None) == tracer.NAVI_E_ARG and "too many envs" in tracer.last_error()
