@@ -13,8 +13,9 @@
 // whose size is spread out to about 1 to 64, but by no more than leaves an entry of X's largest singular value
 // (all of it in one place) below 65504: 2^15 with the default factors, whose steps take singular values
 // to 1.2025. An X of a million columns spread out then has entries of 32. Factors that take singular values
-// past 7.9 between steps, or P past 62, are refused: their planes would not hold A or P. Sums are float32's; what X keeps of itself (a X, and P's diagonal times X) never goes through
-// one plane: X is held in two, the diagonal apart in float32. With one plane, what is left of the
+// past 7.9 between steps, or P past 62, are refused: their planes would not hold A or P. Sums are float32's;
+// what X keeps of itself (a X, and P's diagonal times X) never goes through one plane: X is held in two, the
+// diagonal apart in float32. With one plane, what is left of the
 // rounding of A, P and the X in products to 11 bits is 3 to 7 parts in 10^4 of the result before its own rounding
 // (bfloat16's: 16; 6 at widths of 300, 3.3 at 2000); X in one plane too would leave 10^-2 where singular values lie
 // far apart. With two, 1 to 3 parts in 10^6.
@@ -567,11 +568,10 @@ Largest largest_of(double a, double b, double c, int steps) {
         double poly = std::fabs(b * t + c * t * t), next = std::fabs(s * (a + b * t + c * t * t));
         const double top = -b / (2.0 * c);
         if (top > 0.0 && top < t) poly = std::max(poly, std::fabs(top * (b + c * top)));
-        const double root = 9.0 * b * b - 20.0 * a * c;  // of a + 3 b t + 5 c t^2
-        for (const double sign : {-1.0, 1.0}) {
-            const double at = c == 0.0 ? -a / (3.0 * b) : root >= 0.0 ? (-3.0 * b + sign * std::sqrt(root)) / (10.0 * c) : 0.0;
-            if (at > 0.0 && at < t) next = std::max(next, std::fabs(std::sqrt(at) * (a + b * at + c * at * at)));
-        }
+        // a + 3 b t + 5 c t^2 = 0 (no difference of numbers that are nearly the same, and c may be 0)
+        const double root = 9.0 * b * b - 20.0 * a * c, q = -0.5 * (3.0 * b + std::copysign(std::sqrt(std::max(root, 0.0)), b));
+        for (const double at : {q / (5.0 * c), a / q})
+            if (root >= 0.0 && at > 0.0 && at < t) next = std::max(next, std::fabs(std::sqrt(at) * (a + b * at + c * at * at)));
         most = {std::max(most.x, s), std::max(most.gram, t), std::max(most.poly, poly)};
         if (!(most.gram < 1e30 && most.poly < 1e30)) break;  // (out of any range, and before it is out of double's)
         s = next;

@@ -4,6 +4,8 @@ are never read (calls that are in order name no matrix)."""
 from __future__ import annotations
 
 import math
+import random
+import struct
 
 import pytest
 
@@ -35,6 +37,7 @@ FACTORS = [
     (1, (0.0, 300.0, -300.0)), (2, (20.0, -20.0, 0.0)), (2, (40.0, -40.0, 0.0)), (2, (30.0, -60.0, 30.0)), (2, (0.0, 0.0, 0.0)),
     (3, (2.0, 0.0, 0.0)), (4, (2.0, 0.0, 0.0)), (100, (1.01, 0.0, 0.0)), (100, (1.05, 0.0, 0.0)), (50, (3.0, 3.0, 3.0)),
     (2, (3e38, 3e38, 3e38)), (100, (-1.0, 2.0, -0.5)),
+    (2, (22.0, -22.0, 1e-30)), (2, (22.0, -22.0, -1e-30)), (2, (10.0, -10.0, 1e-30)), (2, (22.0, -1e-30, -22.0)), (2, (-30.0, 1e-20, 30.0)),
 ]
 
 
@@ -50,6 +53,22 @@ def test_factors_within_and_past_the_range(steps, factors):
         assert code == native.NAVI_POLICY_E_ARG and "the factors take" in native.last_error()
     else:
         assert code == native.NAVI_POLICY_OK, native.last_error()
+
+
+def test_factors_of_all_sizes():
+    """Drawn ones against the grid, but for those within a part in 50 of the border."""
+    rng, room, kinds = random.Random(7), 65504 / 1024 / 1.02, set()
+    for _ in range(300):
+        steps = rng.randint(1, 4)
+        factors = tuple(rng.choice((-1, 1)) * 10 ** rng.uniform(-9, 1.9) if rng.random() < 0.9 else 0.0 for _ in range(3))
+        factors = tuple(struct.unpack("f", struct.pack("f", x))[0] for x in factors)
+        s, poly = largest(steps, factors, 2001)
+        if min(abs(s * s / room - 1.0), abs(poly / room - 1.0)) < 0.02:
+            continue
+        past = max(s * s, poly) > room
+        kinds.add(past)
+        assert call(steps, factors) == (native.NAVI_POLICY_E_ARG if past else native.NAVI_POLICY_OK), (steps, factors)
+    assert kinds == {False, True}
 
 
 def test_what_is_no_number_is_refused():
